@@ -78,7 +78,7 @@ def draw(rng):
             heads = rng.randint(1, 32)
         elif op == "qk_packed":
             heads = kv = rng.randint(2, 32)
-        tokens = _log(rng, 17, min(65536, (40 << 20) // ((heads + kv) * dim)))
+        tokens = _log(rng, 17, min(65536, ((20 if c["dtype"] == "fp32" else 40) << 20) // ((heads + kv) * dim)))
         batch = rng.choice([1, 1, 2, 3, 5])
         c.update(batch=batch, seq=max(1, tokens // batch), heads=heads, dim=dim, rotary=rotary,
                  interleaved=rng.random() < 0.4, shared_positions=rng.random() < 0.5,
