@@ -90,6 +90,42 @@ PF_DECL int pf_rope(const void* x, void* out, const void* cos_t, const void* sin
 PF_DECL int pf_rope_qkv(const void* x, void* out, const void* cos_t, const void* sin_t,
                         long long rows, int S, int H, int D, int inverse, int dtype, void* stream);
 
+// ---- qk_rope.cu : rotary positions of every layout, alone or behind an RMS norm of each head
+PF_DECL int pf_heads_fwd(const void* q, const void* k, const void* v, void* yq, void* yk, void* yv,
+                         const void* wq, const void* wk, const void* cos_t, const void* sin_t,
+                         const void* pos, long long B, int S, int Hq, int Hk, int D, int R,
+                         const long long* sq, const long long* sk, const long long* syq,
+                         const long long* syk, const long long* spos, long long rows,
+                         int interleaved, int inverse, float eps, int dtype, int sm_count,
+                         void* stream);
+PF_DECL int pf_heads_bwd_rows(int Hq, int Hk, int sm_count);
+PF_DECL int pf_heads_bwd(const void* gq, const void* gk, const void* gv, const void* q,
+                         const void* k, void* dq, void* dk, void* dv, const void* wq,
+                         const void* wk, void* dwq, void* dwk, void* scratch, const void* cos_t,
+                         const void* sin_t, const void* pos, long long B, int S, int Hq, int Hk,
+                         int D, int R, const long long* sgq, const long long* sgk,
+                         const long long* sq, const long long* sk, const long long* sdq,
+                         const long long* sdk, const long long* spos, long long rows,
+                         int interleaved, float eps, int accumulate, int dtype, int sm_count,
+                         void* stream);
+
+// ---- tune_loss.cu : preference and policy losses
+PF_DECL int pf_preference_fwd(const void* logits, const void* labels, const void* ref, void* loss,
+                              void* rewards, void* stats, void* coef, void* scratch, long long N,
+                              int T, int V, long long n, long long t, long long ignore_index,
+                              float beta, float smoothing, int dtype, int sm_count, void* stream);
+PF_DECL int pf_policy_fwd(const void* logits, const void* actions, const void* old, const void* ref,
+                          const void* adv, void* loss, void* kl, void* clipped, void* inv,
+                          void* logp, void* coef, void* stats, void* scratch, long long N, int T,
+                          int V, long long n, long long t, long long adv_n, long long adv_t,
+                          long long ignore_index, float low, float high, float kl_coef,
+                          float inv_temperature, int dtype, int sm_count, void* stream);
+PF_DECL int pf_token_loss_bwd(const void* logits, const void* labels, const void* stats,
+                              const void* coef, const void* gout, const void* inv, void* dlogits,
+                              long long N, int T, int V, long long n, long long t,
+                              long long ignore_index, int per, float inv_temperature, int dtype,
+                              int sm_count, void* stream);
+
 // ---- attn_sm100.cu : flash attention on tcgen05 (strides in elements: batch, seq, head)
 PF_DECL int pf_attn_fwd(const void* q, const void* k, const void* v, void* o, void* lse, int B,
                         int H, int Sq, int Sk, int D, const long long* sq, const long long* sk,

@@ -56,9 +56,10 @@ NVCC_FLAGS = [
     "--expt-relaxed-constexpr",
 ]
 # Approximate division / square root / transcendentals are fine for activations and softmax,
-# not for the optimizer update: those two files are bandwidth-bound and keep IEEE arithmetic.
+# not for the optimizer update: those two files are bandwidth-bound and keep IEEE arithmetic, as do
+# the head norms and the token losses, which name the approximations that they use.
 FAST_MATH = ["--use_fast_math"]
-PRECISE_SOURCES = {"optim.cu", "dp_fused.cu"}
+PRECISE_SOURCES = {"optim.cu", "dp_fused.cu", "qk_rope.cu", "tune_loss.cu"}
 CXX_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-pthread"]
 
 

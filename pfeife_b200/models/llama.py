@@ -1,7 +1,8 @@
 """Llama-2-shaped decoder on the native ops (the reference trains HF ``LlamaForCausalLM`` with
 eager attention, bench_models/models/train_llama.py:486-520).
 
-Per layer: RMSNorm -> fused QKV GEMM -> RoPE on Q and K -> causal flash attention -> output
+Per layer: RMSNorm -> fused QKV GEMM -> (RMS norm of each head of Q and K, in the pass of the
+rotation) RoPE on Q and K -> causal flash attention -> output
 GEMM with the residual in its epilogue -> RMSNorm -> fused gate|up GEMM -> SwiGLU -> down GEMM
 with the residual in its epilogue.  The score matrix is never materialised, which is what lets
 the sequence-2048 configuration fit comfortably.  ``tie_embeddings`` shares the token embedding
@@ -10,6 +11,7 @@ with the LM head (a parameter used by the first and the last pipeline stage).
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Optional
 
 import torch
 import torch.nn as nn
@@ -28,6 +30,10 @@ class LlamaConfig:
     rms_eps: float = 1e-5
     rope_theta: float = 10000.0
     tie_embeddings: bool = False
+    qk_norm: bool = False                          # RMS norm of each head of the queries and keys
+    rope_dim: Optional[int] = None                 # values of a head that rotate (default: all)
+    rope_interleaved: bool = False                 # pairs (2i, 2i + 1)
+    rope_scaling: Optional[ops.RopeScaling] = None
 
 
 LLAMA_CONFIGS = {
@@ -49,6 +55,11 @@ class LlamaBlock(nn.Module):
         self.eps = cfg.rms_eps
         self.input_norm = nn.Parameter(torch.ones(d))
         self.qkv = nn.Linear(d, 3 * d, bias=False)
+        self.interleaved = cfg.rope_interleaved
+        self.q_norm = self.k_norm = None
+        if cfg.qk_norm:
+            self.q_norm = nn.Parameter(torch.ones(d // cfg.num_heads))
+            self.k_norm = nn.Parameter(torch.ones(d // cfg.num_heads))
         self.o_proj = nn.Linear(d, d, bias=False)
         self.post_norm = nn.Parameter(torch.ones(d))
         self.gate_up = nn.Linear(d, 2 * cfg.intermediate_size, bias=False)
@@ -65,8 +76,12 @@ class LlamaBlock(nn.Module):
         else:
             y, x = ops.rms_norm(delta, self.input_norm, self.eps, residual=x)
         qkv = ops.linear(y, self.qkv.weight).view(B, S, 3, H, d // H)
-        if ops.rope_qkv_in_one(qkv):
-            a = ops.attention_qkv(ops.rope_qkv(qkv, cos, sin), causal=True)
+        if self.q_norm is not None:
+            qkv = ops.qk_norm_rope_qkv(qkv, self.q_norm, self.k_norm, cos, sin, self.eps,
+                                       interleaved=self.interleaved)
+            a = ops.attention_qkv(qkv, causal=True)
+        elif self.interleaved or 2 * cos.shape[1] < d // H or ops.rope_qkv_in_one(qkv):
+            a = ops.attention_qkv(ops.rope_qkv(qkv, cos, sin, interleaved=self.interleaved), causal=True)
         else:
             q, k = ops.rope(qkv[:, :, 0], cos, sin), ops.rope(qkv[:, :, 1], cos, sin)
             a = ops.attention(q, k, qkv[:, :, 2], causal=True)
@@ -87,8 +102,8 @@ class Llama(nn.Module):
         self.lm_head = nn.Linear(cfg.hidden_size, cfg.vocab_size, bias=False)
         if cfg.tie_embeddings:
             self.lm_head.weight = self.embed.weight
-        cos, sin = ops.rope_tables(cfg.max_seq_len, cfg.hidden_size // cfg.num_heads,
-                                   cfg.rope_theta)
+        cos, sin = ops.rope_tables(cfg.max_seq_len, cfg.rope_dim or cfg.hidden_size // cfg.num_heads,
+                                   cfg.rope_theta, scaling=cfg.rope_scaling)
         self.register_buffer("rope_cos", cos, persistent=False)
         self.register_buffer("rope_sin", sin, persistent=False)
         for m in self.modules():

@@ -20,7 +20,7 @@ import contextlib
 import math
 import threading
 from dataclasses import dataclass
-from typing import Dict, Optional, Tuple
+from typing import Dict, NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -962,6 +962,222 @@ def mse_loss(a: Tensor, b: Tensor) -> Tensor:
     return _call(mse_fwd, a, b)
 
 
+# --------------------------------------------------------------------------- preference and policy losses
+def _tokens_counted(labels: Tensor, V: int, ignore_index: int) -> Tensor:
+    return (labels >= 0) & (labels < V) & (labels != ignore_index)
+
+
+def _token_logps_ref(logits: Tensor, labels: Tensor, temperature: float, ignore_index: int):
+    """(log softmax(logits / temperature) at the labels in 64 bits, 0 where none counts; which count; the stats)"""
+    counted = _tokens_counted(labels, logits.shape[-1], ignore_index)
+    z = _wide(logits) / temperature
+    top = z.amax(-1, keepdim=True)
+    top = top.masked_fill(top == -math.inf, 0.0)          # of a row without a finite logit, which has no softmax
+    total = (z - top).exp().sum(-1)
+    picked = (z - top).gather(-1, labels.masked_fill(~counted, 0).unsqueeze(-1)).squeeze(-1)
+    logp = (picked.double() - total.double().log()).masked_fill(~counted, 0.0)
+    return logp, counted, torch.stack([top.squeeze(-1).float() / math.log(2.0), total.float()], -1)
+
+
+@_custom_op("pfeife::preference_fwd")
+def preference_fwd(logits: Tensor, labels: Tensor, ref_logps: Tensor, beta: float, smoothing: float,
+                   ignore_index: int) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """-> (loss, rewards [N], two statistics per row, what each sequence's log-probability gets of the loss)"""
+    if _native(logits) or (logits.is_cuda and logits.dtype == torch.float32):
+        return kx.preference_fwd(logits, labels, ref_logps, beta, smoothing, ignore_index)
+    logp, _, stats = _token_logps_ref(logits, labels, 1.0, ignore_index)
+    rewards = beta * (logp.sum(1) - ref_logps.double())
+    margin = rewards[: len(rewards) // 2] - rewards[len(rewards) // 2:]
+    loss = torch.zeros_like(margin)
+    if smoothing < 1.0:
+        loss = loss - (1 - smoothing) * F.logsigmoid(margin)
+    if smoothing > 0.0:
+        loss = loss - smoothing * F.logsigmoid(-margin)
+    coef = -beta / len(margin) * ((1 - smoothing) * torch.sigmoid(-margin) - smoothing * torch.sigmoid(margin))
+    return loss.mean().float(), rewards.float(), stats, torch.cat([coef, -coef]).float()
+
+
+@preference_fwd.register_fake
+def _(logits, labels, ref_logps, beta, smoothing, ignore_index):
+    N, T, _ = logits.shape
+    new = lambda *shape: logits.new_empty(shape, dtype=torch.float32)
+    return new(), new(N), new(N, T, 2), new(N)
+
+
+@_custom_op("pfeife::token_loss_bwd")
+def token_loss_bwd(dloss: Tensor, logits: Tensor, labels: Tensor, stats: Tensor, coef: Tensor, inv: Optional[Tensor],
+                   ignore_index: int, temperature: float) -> Tensor:
+    """dlogits = dloss * coef * inv * (onehot - p), zero in rows that do not count; `coef` has one value for each
+    sequence [N] or each row [N, T]."""
+    if _native(logits) or (logits.is_cuda and logits.dtype == torch.float32):
+        return kx.token_loss_bwd(dloss, logits, labels, stats, coef, inv, ignore_index, temperature)
+    counted = _tokens_counted(labels, logits.shape[-1], ignore_index)
+    g = (coef if coef.dim() == 2 else coef.unsqueeze(1)) * dloss
+    if inv is not None:
+        g = g * inv
+    p = torch.softmax(_wide(logits) / temperature, -1)
+    onehot = torch.zeros_like(p).scatter_(-1, labels.masked_fill(~counted, 0).unsqueeze(-1), 1.0)
+    d = g.unsqueeze(-1) * (onehot - p)
+    return d.masked_fill(~(counted & (g != 0)).unsqueeze(-1), 0.0).to(logits.dtype)
+
+
+@token_loss_bwd.register_fake
+def _(dloss, logits, labels, stats, coef, inv, ignore_index, temperature):
+    return logits.new_empty(logits.shape)
+
+
+def _preference_setup(ctx, inputs, output):
+    logits, labels, _, _, _, ignore_index = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(logits, labels, output[2], output[3])
+    ctx.ignore_index = ignore_index
+
+
+def _preference_backward(ctx, dloss, *unused):
+    if dloss is None:
+        return (None,) * 6
+    logits, labels, stats, coef = ctx.saved_tensors
+    d = _bwd(ctx, token_loss_bwd)(dloss, logits, labels, stats, coef, None, ctx.ignore_index, 1.0)
+    return (d,) + (None,) * 5
+
+
+_autograd(preference_fwd, 2, _preference_backward, setup=_preference_setup)
+
+
+class PreferenceLoss(NamedTuple):
+    loss: Tensor          # mean over the pairs
+    rewards: Tensor       # [2P] beta * (log-probability - the reference's), without a gradient
+
+
+class PolicyLoss(NamedTuple):
+    loss: Tensor          # mean over the tokens that count
+    logps: Tensor         # log-probabilities of the actions, 0 where none counts; the last three without a gradient
+    kl: Tensor            # mean estimate of KL(policy || reference), 0 without a reference
+    clipped: Tensor       # share of the tokens whose ratio the clipping holds
+
+
+def _check_tokens(what: str, logits: Tensor, labels: Tensor, **values: Optional[Tensor]) -> None:
+    if labels.shape != logits.shape[:-1] or labels.device != logits.device or labels.is_floating_point():
+        raise ValueError(f"{what}: integer labels {tuple(logits.shape[:-1])} on {logits.device} are needed, not "
+                         f"{labels.dtype} {tuple(labels.shape)} on {labels.device}")
+    for name, t in values.items():
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"{what}: {name} on {t.device}, logits on {logits.device}")
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what}: {name} gets no gradient; detach it")
+
+
+def preference_loss(logits: Tensor, labels: Tensor, ref_logps: Tensor, beta: float = 0.1,
+                    label_smoothing: float = 0.0, ignore_index: int = -100) -> PreferenceLoss:
+    """Loss on paired log ratios.  logits [2P, T, V]: the P chosen sequences, then the P rejected ones in the same
+    order; labels [2P, T]: the token that each row predicts, ``ignore_index`` or any number outside the vocabulary
+    where none counts (prompts, padding); ref_logps [2P]: the sequences' log-probabilities under the reference.
+    With l the sum of a sequence's log-probabilities and m = beta ((l - ref of the chosen) - (l - ref of the
+    rejected)) the loss is the mean of -(1 - label_smoothing) log sig(m) - label_smoothing log sig(-m).
+    Rows that do not count are not read and get a gradient of zero, whatever their logits."""
+    if isinstance(logits, Tensor):
+        N = logits.shape[0] if logits.dim() == 3 else 0
+        if N < 2 or N % 2 or logits.shape[2] < 1:
+            raise ValueError(f"preference_loss: logits [2P, T, V] are needed, not {tuple(logits.shape)}")
+        _check_tokens("preference_loss", logits, labels, ref_logps=ref_logps)
+        if ref_logps.shape != (N,):
+            raise ValueError(f"preference_loss: ref_logps [{N}] are needed, not {tuple(ref_logps.shape)}")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"preference_loss: label_smoothing {label_smoothing} is not between 0 and 1")
+    loss, rewards = _call(preference_fwd, logits, labels, ref_logps, float(beta), float(label_smoothing), ignore_index)
+    return PreferenceLoss(loss, rewards.detach())
+
+
+@_custom_op("pfeife::policy_fwd")
+def policy_fwd(logits: Tensor, actions: Tensor, old_logps: Tensor, advantages: Tensor, ref_logps: Optional[Tensor],
+               low: float, high: float, kl_coef: float, temperature: float, ignore_index: int
+               ) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """-> (loss, log-probabilities [N, T], KL, clipped share, two statistics per row, what each log-probability gets
+    of its term, one over the tokens that count)"""
+    if _native(logits) or (logits.is_cuda and logits.dtype == torch.float32):
+        return kx.policy_fwd(logits, actions, old_logps, advantages, ref_logps, low, high, kl_coef, temperature,
+                             ignore_index)
+    logp, counted, stats = _token_logps_ref(logits, actions, temperature, ignore_index)
+    adv = advantages.double()
+    ratio = torch.exp(logp - old_logps.double())
+    free, held = ratio * adv, ratio.clamp(1 - low, 1 + high) * adv
+    cut = free > held
+    term, coef = -torch.where(cut, held, free), torch.where(cut, 0.0, -free)
+    inv = 1.0 / counted.sum().clamp(min=1).double()
+    mean = lambda t: (t.masked_fill(~counted, 0.0).sum() * inv).float()
+    kl = torch.zeros((), device=logits.device)
+    if ref_logps is not None:
+        d = ref_logps.double() - logp
+        each = torch.expm1(d) - d
+        term, coef, kl = term + kl_coef * each, coef - kl_coef * torch.expm1(d), mean(each)
+    coef = (coef / temperature).masked_fill(~counted, 0.0).float()
+    return mean(term), logp.float(), kl, mean(cut.double()), stats, coef, inv.float()
+
+
+@policy_fwd.register_fake
+def _(logits, actions, old_logps, advantages, ref_logps, low, high, kl_coef, temperature, ignore_index):
+    N, T, _ = logits.shape
+    new = lambda *shape: logits.new_empty(shape, dtype=torch.float32)
+    return new(), new(N, T), new(), new(), new(N, T, 2), new(N, T), new()
+
+
+def _policy_setup(ctx, inputs, output):
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(inputs[0], inputs[1], *output[4:])
+    ctx.temperature, ctx.ignore_index = inputs[8], inputs[9]
+
+
+def _policy_backward(ctx, dloss, *unused):
+    if dloss is None:
+        return (None,) * 10
+    logits, actions, stats, coef, inv = ctx.saved_tensors
+    d = _bwd(ctx, token_loss_bwd)(dloss, logits, actions, stats, coef, inv, ctx.ignore_index, ctx.temperature)
+    return (d,) + (None,) * 9
+
+
+_autograd(policy_fwd, 4, _policy_backward, setup=_policy_setup)
+
+
+def policy_loss(logits: Tensor, actions: Tensor, old_logps: Tensor, advantages: Tensor,
+                ref_logps: Optional[Tensor] = None, clip_low: float = 0.2, clip_high: float = 0.2,
+                kl_coef: float = 0.0, temperature: float = 1.0, ignore_index: int = -100) -> PolicyLoss:
+    """Clipped policy loss over sampled tokens.  logits [..., V]; actions [...]: the token taken at each row,
+    ``ignore_index`` or any number outside the vocabulary where none counts; old_logps [...]: its log-probability
+    when it was sampled; advantages: of the shape of the actions or one that expands to it ([N, 1]: one for each
+    sequence).  With l = log softmax(logits / temperature)[action] and r = exp(l - old) a token's term is
+    -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(ref - l) - (ref - l) - 1), the last with
+    ``ref_logps`` [...] only; the loss is the mean over the tokens that count, 0 if there are none.
+    Rows that do not count are not read and get a gradient of zero, whatever their logits."""
+    shape = actions.shape
+    if isinstance(logits, Tensor):
+        if logits.dim() < 2 or logits.shape[-1] < 1:
+            raise ValueError(f"policy_loss: logits [..., V] are needed, not {tuple(logits.shape)}")
+        _check_tokens("policy_loss", logits, actions, old_logps=old_logps, advantages=advantages,
+                      ref_logps=ref_logps)
+        for name, t in (("old_logps", old_logps), ("ref_logps", ref_logps)):
+            if t is not None and t.shape != shape:
+                raise ValueError(f"policy_loss: {name} {tuple(shape)} are needed, not {tuple(t.shape)}")
+    if temperature <= 0.0 or not 0.0 <= clip_low <= 1.0 or clip_high < 0.0:
+        raise ValueError(f"policy_loss: a temperature {temperature} above 0, clip_low {clip_low} between 0 and 1 and "
+                         f"clip_high {clip_high} of at least 0 are needed")
+    if advantages.shape != shape:
+        try:
+            advantages = advantages.expand(shape)
+        except RuntimeError:
+            raise ValueError(f"policy_loss: advantages {tuple(advantages.shape)} do not expand to {tuple(shape)}") \
+                from None
+    if len(shape) != 2:                    # rows of one sequence, or of as many as all leading dims have
+        fold = (1, -1) if len(shape) == 1 else (-1, shape[-1])
+        if 0 in shape:
+            fold = (1, 0)
+        logits = logits.reshape(*fold, logits.shape[-1])
+        actions, old_logps, advantages = (t.reshape(fold) for t in (actions, old_logps, advantages))
+        ref_logps = None if ref_logps is None else ref_logps.reshape(fold)
+    loss, logps, kl, clipped = _call(policy_fwd, logits, actions, old_logps, advantages, ref_logps, float(clip_low),
+                                     float(clip_high), float(kl_coef), float(temperature), ignore_index)
+    return PolicyLoss(loss, logps.detach().view(shape), kl.detach(), clipped.detach())
+
+
 # =========================================================================== embedding / rope
 @_custom_op("pfeife::embed_fwd")
 def embed_fwd(ids: Tensor, table: Tensor, out_dtype: torch.dtype) -> Tensor:
@@ -1020,14 +1236,17 @@ def embedding(ids: Tensor, table: Tensor, out_dtype: Optional[torch.dtype] = Non
 
 @_custom_op("pfeife::rope_apply")
 def rope_apply(x: Tensor, cos: Tensor, sin: Tensor, inverse: bool) -> Tensor:
-    """x [B, S, H, D]; cos/sin fp32 [S, D/2]; half-split pairing (i, i + D/2)."""
+    """x [B, S, H, D]; cos/sin fp32 [S, D/2]; half-split pairing (i, i + D/2).  Narrower tables rotate a part."""
+    if cos.dim() == 2 and 2 * cos.shape[1] < x.shape[-1]:
+        _check_angles(x, cos, sin, None)
+        return rope_at.plain(x, cos, sin, None, False, inverse)
     if _native(x) or (x.is_cuda and x.dtype == torch.float32):
         return kx.rope(x if x.stride(-1) == 1 else x.contiguous(), cos.float(), sin.float(), inverse)
     D = x.shape[-1]
     xf = x.float()
     x1, x2 = xf[..., : D // 2], xf[..., D // 2:]
-    c = cos.float()[None, :, None, :]
-    s = sin.float()[None, :, None, :]
+    c = cos.float()[None, :x.shape[1], None, :]      # the first rows, as on CUDA
+    s = sin.float()[None, :x.shape[1], None, :]
     if inverse:
         s = -s
     return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], -1).to(x.dtype)
@@ -1051,13 +1270,25 @@ def _rope_backward(ctx, dy):
 _autograd(rope_apply, 1, _rope_backward, setup=_rope_setup)
 
 
-def rope(x: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
-    return _call(rope_apply, x, cos, sin, False)
+def rope(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None,
+         interleaved: bool = False) -> Tensor:
+    """Rotates the heads of x [B, S, H, D] by their positions: pairs (i, i + R/2), or (2i, 2i + 1) when
+    ``interleaved``, of the first R values, R twice the width of the tables cos / sin (``rope_tables``); values
+    beyond R stay.  ``positions``, integers [S] or [B, S], are the rows of the tables to turn by (default: row s
+    for token s).  A row that the tables do not have makes the token's rotated values NaN on CUDA, where looking
+    for it would wait for the device, and an IndexError on the CPU."""
+    if positions is None and not interleaved:
+        return _call(rope_apply, x, cos, sin, False)
+    _check_angles(x, cos, sin, positions)
+    return _call(rope_at, x, cos, sin, positions, interleaved, False)
 
 
 @_custom_op("pfeife::rope_qkv_apply")
 def rope_qkv_apply(qkv: Tensor, cos: Tensor, sin: Tensor, inverse: bool) -> Tensor:
     """qkv [B, S, 3, H, D] -> a contiguous tensor with the queries and keys rotated."""
+    if cos.dim() == 2 and 2 * cos.shape[1] < qkv.shape[-1]:
+        _check_angles(qkv, cos, sin, None)
+        return rope_qkv_at.plain(qkv, cos, sin, None, False, inverse)
     if _native(qkv):
         qkv = qkv.contiguous()
         if kx.rope_qkv_supported(qkv, cos, sin):
@@ -1079,10 +1310,14 @@ def _rope_qkv_backward(ctx, dy):
 _autograd(rope_qkv_apply, 1, _rope_qkv_backward, setup=_rope_setup)
 
 
-def rope_qkv(qkv: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
+def rope_qkv(qkv: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None,
+             interleaved: bool = False) -> Tensor:
     """``rope`` of the queries and keys of a fused projection [B, S, 3, H, D], for ``attention_qkv``."""
-    y = _native_call("rope_qkv", qkv, cos, sin)
-    return y if y is not None else _call(rope_qkv_apply, qkv, cos, sin, False)
+    if positions is None and not interleaved:
+        y = _native_call("rope_qkv", qkv, cos, sin)
+        return y if y is not None else _call(rope_qkv_apply, qkv, cos, sin, False)
+    _check_angles(qkv, cos, sin, positions)
+    return _call(rope_qkv_at, qkv, cos, sin, positions, interleaved, False)
 
 
 def rope_qkv_in_one(qkv: Tensor) -> bool:
@@ -1091,12 +1326,327 @@ def rope_qkv_in_one(qkv: Tensor) -> bool:
     return _native(qkv) and qkv.shape[-1] % 16 == 0
 
 
-def rope_tables(seq_len: int, head_dim: int, theta: float = 10000.0, device=None
-                ) -> Tuple[Tensor, Tensor]:
+@dataclass(frozen=True)
+class RopeScaling:
+    """Rotary frequencies for contexts of ``factor`` times the ``original_len`` positions a model was trained on:
+      * ``linear``: positions divided by the factor;
+      * ``ntk``: a base grown so that the slowest frequency is divided by the factor;
+      * ``yarn``: frequencies that turn more than ``fast`` times in the original context are kept, those that turn
+        less than ``slow`` times divided by the factor, with a ramp over the frequency's number between them, and
+        cosines and sines grown by 0.1 ln(factor) + 1 (``grown`` replaces that);
+      * ``bands``: the same by wavelength: kept above ``fast`` turns, divided below ``slow``, interpolated between."""
+    kind: str
+    factor: float
+    original_len: int = 2048
+    fast: Optional[float] = None          # yarn: 32, bands: 4
+    slow: float = 1.0
+    grown: Optional[float] = None
+
+
+def _scaled_frequencies(rotary_dim: int, theta: float, s: RopeScaling, device) -> Tuple[Tensor, float]:
+    """-> (radians per position of each pair, in 64 bits; what cosines and sines are multiplied by)"""
+    if s.kind not in ("linear", "ntk", "yarn", "bands"):
+        raise ValueError(f"RopeScaling: unknown kind {s.kind!r}")
+    if s.factor < 1.0 or s.original_len < 1 or s.slow <= 0.0 or (s.fast is not None and s.fast <= s.slow):
+        raise ValueError(f"RopeScaling: factor at least 1, a positive length and 0 < slow < fast are needed: {s}")
+    i = torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float64)
+    if s.kind == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("RopeScaling: a single pair has no slowest frequency beside its first")
+        theta = theta * s.factor ** (rotary_dim / (rotary_dim - 2))
+    inv = 1.0 / theta ** (i / rotary_dim)
+    if s.kind == "linear":
+        inv = inv / s.factor
+    elif s.kind == "yarn":
+        def pair(turns):                  # number of the frequency that turns so often
+            return rotary_dim * math.log(s.original_len / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        low = max(math.floor(pair(s.fast or 32.0)), 0)
+        high = min(math.ceil(pair(s.slow)), rotary_dim - 1)
+        ramp = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0, 1)
+        inv = inv * (1 - ramp) + inv / s.factor * ramp
+    elif s.kind == "bands":
+        kept = ((s.original_len * inv / (2 * math.pi) - s.slow) / ((s.fast or 4.0) - s.slow)).clamp(0, 1)
+        inv = inv * kept + inv / s.factor * (1 - kept)
+    grown = s.grown if s.grown is not None else 0.1 * math.log(s.factor) + 1.0 if s.kind == "yarn" else 1.0
+    return inv, grown
+
+
+def rope_tables(seq_len: int, head_dim: int, theta: float = 10000.0, device=None,
+                scaling: Optional[RopeScaling] = None) -> Tuple[Tensor, Tensor]:
+    """fp32 cosines and sines [seq_len, head_dim / 2]; for a rotation of a part of each head, ``head_dim`` is that
+    part.  Scaled tables, which are for far positions, are computed in 64 bits."""
+    if scaling is not None:
+        inv, grown = _scaled_frequencies(head_dim, theta, scaling, device)
+        ang = torch.outer(torch.arange(seq_len, device=device, dtype=torch.float64), inv)
+        return (ang.cos() * grown).float(), (ang.sin() * grown).float()
     inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, device=device, dtype=torch.float32)
                            / head_dim))
     ang = torch.outer(torch.arange(seq_len, device=device, dtype=torch.float32), inv)
     return ang.cos(), ang.sin()
+
+
+# --------------------------------------------------------------------------- rotations of any layout, head norms
+def _check_angles(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor]) -> None:
+    """Refuses angles that do not fit x [B, S, .., D]; what a symbolic trace passes is checked when it runs."""
+    if not isinstance(x, Tensor):
+        return
+    S = x.shape[1]
+    if cos.dim() != 2 or cos.shape != sin.shape or not 0 < 2 * cos.shape[1] <= x.shape[-1]:
+        raise ValueError(f"tables [rows, R/2] with 0 < R <= {x.shape[-1]} are needed, not {tuple(cos.shape)} "
+                         f"and {tuple(sin.shape)}")
+    if cos.device != x.device or sin.device != x.device:
+        raise ValueError(f"tables on {cos.device} and {sin.device} for heads on {x.device}")
+    if positions is None:
+        if cos.shape[0] < S:
+            raise ValueError(f"tables of {cos.shape[0]} rows for {S} tokens")
+    elif positions.device != x.device or positions.dtype not in (torch.int64, torch.int32) \
+            or tuple(positions.shape) not in ((S,), (x.shape[0], S)):
+        raise ValueError(f"positions are integers [{S}] or [{x.shape[0]}, {S}] on {x.device}, not "
+                         f"{positions.dtype} {tuple(positions.shape)} on {positions.device}")
+
+
+def _wide(x: Tensor) -> Tensor:
+    return x if x.dtype == torch.float64 else x.float()
+
+
+def _turn_ref(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor], interleaved: bool,
+              inverse: bool) -> Tensor:
+    """The rotation of x [B, S, H, D] in its own type."""
+    if positions is None:
+        c, s = cos[:x.shape[1]], sin[:x.shape[1]]
+    else:
+        at = positions.long()
+        bad = (at < 0) | (at >= cos.shape[0])
+        if not x.is_cuda and bad.any():
+            raise IndexError(f"a position lies outside the {cos.shape[0]} rows of the tables")
+        at = at.clamp(0, cos.shape[0] - 1)
+        c, s = (t[at].masked_fill(bad.unsqueeze(-1), math.nan) for t in (cos, sin))
+    c, s = c.to(x.dtype).unsqueeze(-2), s.to(x.dtype).unsqueeze(-2)
+    half = cos.shape[1]
+    if inverse:
+        s = -s
+    if interleaved:
+        a, b = x[..., 0:2 * half:2], x[..., 1:2 * half:2]
+        turned = torch.stack([a * c - b * s, b * c + a * s], -1).flatten(-2)
+    else:
+        a, b = x[..., :half], x[..., half:2 * half]
+        turned = torch.cat([a * c - b * s, b * c + a * s], -1)
+    return torch.cat([turned, x[..., 2 * half:]], -1)
+
+
+@_custom_op("pfeife::rope_at")
+def rope_at(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor], interleaved: bool,
+            inverse: bool) -> Tensor:
+    """x [B, S, H, D] of any strides -> packed; cos / sin [rows, R/2]; positions [S] or [B, S]."""
+    if kx.heads_supported(x):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        kx.heads_fwd(x, None, None, y, None, None, cos, sin, positions, interleaved=interleaved, inverse=inverse)
+        return y
+    return _turn_ref(_wide(x), cos, sin, positions, interleaved, inverse).to(x.dtype).contiguous()
+
+
+@rope_at.register_fake
+def _(x, cos, sin, positions, interleaved, inverse):
+    return x.new_empty(x.shape)
+
+
+def _rope_at_setup(ctx, inputs, output):
+    _, cos, sin, positions, interleaved, inverse = inputs
+    ctx.save_for_backward(cos, sin, positions)
+    ctx.interleaved, ctx.inverse = interleaved, inverse
+
+
+def _rope_at_backward(op):
+    def backward(ctx, dy):
+        cos, sin, positions = ctx.saved_tensors
+        return (_bwd(ctx, op)(dy, cos, sin, positions, ctx.interleaved, not ctx.inverse),) + (None,) * 5
+    return backward
+
+
+_autograd(rope_at, 1, _rope_at_backward(rope_at), setup=_rope_at_setup)
+
+
+@_custom_op("pfeife::rope_qkv_at")
+def rope_qkv_at(qkv: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor], interleaved: bool,
+                inverse: bool) -> Tensor:
+    """qkv [B, S, 3, H, D] -> packed, with the queries and keys rotated and the values copied."""
+    q, k, v = qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2]
+    if kx.heads_supported(qkv):
+        y = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        kx.heads_fwd(q, k, v, y[:, :, 0], y[:, :, 1], y[:, :, 2], cos, sin, positions, interleaved=interleaved,
+                     inverse=inverse)
+        return y
+    q, k = (_turn_ref(_wide(t), cos, sin, positions, interleaved, inverse).to(qkv.dtype) for t in (q, k))
+    return torch.stack([q, k, v], dim=2)
+
+
+@rope_qkv_at.register_fake
+def _(qkv, cos, sin, positions, interleaved, inverse):
+    return qkv.new_empty(qkv.shape)
+
+
+_autograd(rope_qkv_at, 1, _rope_at_backward(rope_qkv_at), setup=_rope_at_setup)
+
+
+def _head_norm_ref(x: Tensor, w: Tensor, eps: float) -> Tensor:
+    return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * w.to(x.dtype)
+
+
+def _head_norm_grad_ref(g: Tensor, x: Tensor, w: Tensor, eps: float) -> Tuple[Tensor, Tensor]:
+    """(dx, dw) from the gradient g of the normed heads"""
+    r = torch.rsqrt(x.square().mean(-1, keepdim=True) + eps)
+    xh, gw = x * r, g * w.to(x.dtype)
+    return r * (gw - xh * (gw * xh).mean(-1, keepdim=True)), (g * xh).sum((0, 1, 2))
+
+
+def _head_norm_buckets(wq: Tensor, wk: Tensor, x: Tensor):
+    """(where the gradients of both gains go, whether they are registered buckets, which are added to)"""
+    bq, bk = _grad_bucket(wq), _grad_bucket(wk)
+    if bq is not None and bk is not None:
+        return bq, bk, True
+    return *(torch.empty(x.shape[-1], dtype=torch.float32, device=x.device) for _ in range(2)), False
+
+
+def _gains_out(dwq: Tensor, dwk: Tensor, added: bool) -> Tuple[Tensor, Tensor]:
+    return (dwq.new_empty(0), dwk.new_empty(0)) if added else (dwq, dwk)
+
+
+@_custom_op("pfeife::qk_norm_rope_fwd")
+def qk_norm_rope_fwd(q: Tensor, k: Tensor, wq: Tensor, wk: Tensor, cos: Tensor, sin: Tensor,
+                     positions: Optional[Tensor], eps: float, interleaved: bool) -> Tuple[Tensor, Tensor]:
+    if kx.heads_supported(q, k):
+        yq, yk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+        kx.heads_fwd(q, k, None, yq, yk, None, cos, sin, positions, wq=wq, wk=wk, eps=eps, interleaved=interleaved)
+        return yq, yk
+    return tuple(_turn_ref(_head_norm_ref(_wide(t), w, eps), cos, sin, positions, interleaved, False)
+                 .to(t.dtype).contiguous() for t, w in ((q, wq), (k, wk)))
+
+
+@qk_norm_rope_fwd.register_fake
+def _(q, k, wq, wk, cos, sin, positions, eps, interleaved):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@_custom_op("pfeife::qk_norm_rope_bwd")
+def qk_norm_rope_bwd(gq: Tensor, gk: Tensor, q: Tensor, k: Tensor, wq: Tensor, wk: Tensor, cos: Tensor, sin: Tensor,
+                     positions: Optional[Tensor], eps: float, interleaved: bool
+                     ) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """-> (dq, dk, dwq, dwk); gains' gradients that went into registered buckets come back empty."""
+    if kx.heads_supported(q, k):
+        dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+        dwq, dwk, added = _head_norm_buckets(wq, wk, q)
+        kx.heads_bwd(gq, gk, None, q, k, dq, dk, None, wq, wk, cos, sin, positions, dwq, dwk, eps=eps,
+                     interleaved=interleaved, accumulate=added)
+        return dq, dk, *_gains_out(dwq, dwk, added)
+    out = []
+    for g, x, w in ((gq, q, wq), (gk, k, wk)):
+        g = _turn_ref(g.to(_wide(x).dtype), cos, sin, positions, interleaved, True)
+        out.append(_head_norm_grad_ref(g, _wide(x), w, eps))
+    (dq, dwq), (dk, dwk) = out
+    return dq.to(q.dtype), dk.to(k.dtype), dwq, dwk
+
+
+@qk_norm_rope_bwd.register_fake
+def _(gq, gk, q, k, wq, wk, cos, sin, positions, eps, interleaved):
+    w = q.new_empty(q.shape[-1], dtype=torch.float32)
+    return q.new_empty(q.shape), k.new_empty(k.shape), w, torch.empty_like(w)
+
+
+def _gain_grad(dw: Tensor, w: Tensor) -> Optional[Tensor]:
+    return dw.to(w.dtype) if dw.numel() else None
+
+
+def _qk_norm_rope_setup(ctx, inputs, output):
+    *saved, ctx.eps, ctx.interleaved = inputs
+    ctx.save_for_backward(*saved)
+
+
+def _qk_norm_rope_backward(ctx, gq, gk):
+    q, k, wq, wk, *angles = ctx.saved_tensors
+    dq, dk, dwq, dwk = _bwd(ctx, qk_norm_rope_bwd)(gq, gk, q, k, wq, wk, *angles, ctx.eps, ctx.interleaved)
+    return (dq, dk, _gain_grad(dwq, wq), _gain_grad(dwk, wk)) + (None,) * 5
+
+
+_autograd(qk_norm_rope_fwd, 2, _qk_norm_rope_backward, setup=_qk_norm_rope_setup)
+
+
+def _check_gains(x: Tensor, *weights: Tensor) -> None:
+    for w in weights:
+        if isinstance(x, Tensor) and isinstance(w, Tensor) and (w.shape != x.shape[-1:] or w.device != x.device):
+            raise ValueError(f"a gain [{x.shape[-1]}] on {x.device} is needed, not {tuple(w.shape)} on {w.device}")
+
+
+def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor,
+                 eps: float = 1e-6, positions: Optional[Tensor] = None, interleaved: bool = False
+                 ) -> Tuple[Tensor, Tensor]:
+    """RMS norm of each head of q [B, S, Hq, D] and k [B, S, Hk, D] with the gains q_weight and k_weight [D], then
+    ``rope`` of both, in one pass.  q and k may be slices of a projection."""
+    if isinstance(q, Tensor) and isinstance(k, Tensor) and (
+            q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] \
+            or q.dtype != k.dtype or q.device != k.device):
+        raise ValueError(f"queries [B, S, Hq, D] and keys [B, S, Hk, D] of one type and device are needed, not "
+                         f"{q.dtype} {tuple(q.shape)} and {k.dtype} {tuple(k.shape)}")
+    _check_angles(q, cos, sin, positions)
+    _check_gains(q, q_weight, k_weight)
+    return _call(qk_norm_rope_fwd, q, k, q_weight, k_weight, cos, sin, positions, float(eps), interleaved)
+
+
+@_custom_op("pfeife::qk_norm_rope_qkv_fwd")
+def qk_norm_rope_qkv_fwd(qkv: Tensor, wq: Tensor, wk: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor],
+                         eps: float, interleaved: bool) -> Tensor:
+    q, k, v = qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2]
+    if kx.heads_supported(qkv):
+        y = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        kx.heads_fwd(q, k, v, y[:, :, 0], y[:, :, 1], y[:, :, 2], cos, sin, positions, wq=wq, wk=wk, eps=eps,
+                     interleaved=interleaved)
+        return y
+    return torch.stack([*qk_norm_rope_fwd.plain(q, k, wq, wk, cos, sin, positions, eps, interleaved), v], dim=2)
+
+
+@qk_norm_rope_qkv_fwd.register_fake
+def _(qkv, wq, wk, cos, sin, positions, eps, interleaved):
+    return qkv.new_empty(qkv.shape)
+
+
+@_custom_op("pfeife::qk_norm_rope_qkv_bwd")
+def qk_norm_rope_qkv_bwd(dy: Tensor, qkv: Tensor, wq: Tensor, wk: Tensor, cos: Tensor, sin: Tensor,
+                         positions: Optional[Tensor], eps: float, interleaved: bool
+                         ) -> Tuple[Tensor, Tensor, Tensor]:
+    """-> (d(qkv) packed, dwq, dwk); gains' gradients that went into registered buckets come back empty."""
+    (gq, gk, gv), (q, k, _) = dy.unbind(2), qkv.unbind(2)
+    if kx.heads_supported(qkv):
+        d = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        dwq, dwk, added = _head_norm_buckets(wq, wk, q)
+        kx.heads_bwd(gq, gk, gv, q, k, *d.unbind(2), wq, wk, cos, sin, positions, dwq, dwk, eps=eps,
+                     interleaved=interleaved, accumulate=added)
+        return d, *_gains_out(dwq, dwk, added)
+    dq, dk, dwq, dwk = qk_norm_rope_bwd.plain(gq, gk, q, k, wq, wk, cos, sin, positions, eps, interleaved)
+    return torch.stack([dq, dk, gv.to(dq.dtype)], dim=2), dwq, dwk
+
+
+@qk_norm_rope_qkv_bwd.register_fake
+def _(dy, qkv, wq, wk, cos, sin, positions, eps, interleaved):
+    w = qkv.new_empty(qkv.shape[-1], dtype=torch.float32)
+    return qkv.new_empty(qkv.shape), w, torch.empty_like(w)
+
+
+def _qk_norm_rope_qkv_backward(ctx, dy):
+    qkv, wq, wk, *angles = ctx.saved_tensors
+    d, dwq, dwk = _bwd(ctx, qk_norm_rope_qkv_bwd)(dy, qkv, wq, wk, *angles, ctx.eps, ctx.interleaved)
+    return (d, _gain_grad(dwq, wq), _gain_grad(dwk, wk)) + (None,) * 5
+
+
+_autograd(qk_norm_rope_qkv_fwd, 1, _qk_norm_rope_qkv_backward, setup=_qk_norm_rope_setup)
+
+
+def qk_norm_rope_qkv(qkv: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor, eps: float = 1e-6,
+                     positions: Optional[Tensor] = None, interleaved: bool = False) -> Tensor:
+    """``qk_norm_rope`` of the queries and keys of a fused projection [B, S, 3, H, D], for ``attention_qkv``."""
+    if isinstance(qkv, Tensor) and (qkv.dim() != 5 or qkv.shape[2] != 3):
+        raise ValueError(f"a projection [B, S, 3, H, D] is needed, not {tuple(qkv.shape)}")
+    _check_angles(qkv, cos, sin, positions)
+    _check_gains(qkv, q_weight, k_weight)
+    return _call(qk_norm_rope_qkv_fwd, qkv, q_weight, k_weight, cos, sin, positions, float(eps), interleaved)
 
 
 # =========================================================================== attention

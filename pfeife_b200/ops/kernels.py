@@ -465,6 +465,161 @@ def rope_qkv(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, inverse: boo
     return out
 
 
+# --------------------------------------------------------------------------- norms and rotations of heads
+MAX_HEAD_DIM = 256                         # qk_rope.cu: a head lies across one warp
+_HEAD_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def heads_supported(*heads: torch.Tensor) -> bool:
+    """True when the kernels over heads cover these [.., D] tensors."""
+    x = heads[0]
+    return all(t.is_cuda and t.dtype == x.dtype and t.shape[-1] == x.shape[-1] for t in heads) \
+        and x.dtype in _HEAD_TYPES and 2 <= x.shape[-1] <= MAX_HEAD_DIM
+
+
+def _heads(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """[B, S, H, D] as the kernels over heads read it: any strides, D innermost."""
+    return t if t is None or t.stride(3) == 1 else t.contiguous()
+
+
+def _steps(t: Optional[torch.Tensor]) -> Optional[Tuple[int, ...]]:
+    """Strides (batch, seq, head); one of a single place is never used, and must not spoil the alignment."""
+    return None if t is None else tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3]))
+
+
+def _positions(positions: Optional[torch.Tensor], B: int, S: int):
+    """(int64 positions [S] or [B, S], their strides)"""
+    if positions is None:
+        return None, None
+    positions = positions.long()
+    assert positions.shape in ((S,), (B, S))
+    return positions, (0 if positions.dim() == 1 else positions.stride(0), positions.stride(-1))
+
+
+def _turns(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor]):
+    """What every call on heads has of angles: packed tables, positions and their strides."""
+    assert cos.dim() == 2 and cos.shape == sin.shape and 0 < 2 * cos.shape[1] <= x.shape[3]
+    assert positions is not None or cos.shape[0] >= x.shape[1]
+    for t in (cos, sin) if positions is None else (cos, sin, positions):
+        assert t.device == x.device
+    return (_floats(cos), _floats(sin), *_positions(positions, x.shape[0], x.shape[1]))
+
+
+def heads_fwd(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Tensor], yq: torch.Tensor,
+              yk: Optional[torch.Tensor], yv: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
+              positions: Optional[torch.Tensor], *, wq: Optional[torch.Tensor] = None,
+              wk: Optional[torch.Tensor] = None, eps: float = 0.0, interleaved: bool = False,
+              inverse: bool = False) -> None:
+    """q [B, S, Hq, D] -> yq, and k [B, S, Hk, D] -> yk, v -> yv where given: queries and keys normed (with gains wq
+    and wk [D]) and rotated, values copied.  cos / sin [rows, R/2]: the first R values of a head rotate."""
+    L = _lib.calls()
+    cos, sin, positions, steps = _turns(q, cos, sin, positions)
+    q, k, v = _heads(q), _heads(k), _heads(v)
+    if v is not None:
+        assert _steps(v) == _steps(k) and _steps(yv) == _steps(yk)
+    B, S, H, D = q.shape
+    for x, y in ((q, yq), (k, yk), (v, yv)):
+        assert (x is None) == (y is None)
+        assert x is None or (x.shape == y.shape and x.shape[:2] == (B, S) and x.shape[3] == D
+                             and x.dtype == y.dtype == q.dtype and y.stride(3) == 1)
+    for w in (wq, wk):
+        assert w is None or w.shape == (D,)
+    wq, wk = (None if w is None else _floats(w) for w in (wq, wk))
+    check(L.pf_heads_fwd(q, k, v, yq, yk, yv, wq, wk, cos, sin, positions, B, S, H,
+                         0 if k is None else k.shape[2], D, 2 * cos.shape[1], _steps(q), _steps(k), _steps(yq),
+                         _steps(yk), steps, cos.shape[0], int(interleaved), int(inverse), eps, dt(q.dtype),
+                         sm_count(q.device), stream_of(q)), "pf_heads_fwd")
+
+
+def heads_bwd(gq: torch.Tensor, gk: torch.Tensor, gv: Optional[torch.Tensor], q: torch.Tensor, k: torch.Tensor,
+              dq: torch.Tensor, dk: torch.Tensor, dv: Optional[torch.Tensor], wq: torch.Tensor, wk: torch.Tensor,
+              cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor], dwq: Optional[torch.Tensor],
+              dwk: Optional[torch.Tensor], *, eps: float, interleaved: bool = False, accumulate: bool = False
+              ) -> None:
+    """Gradients of the outputs of ``heads_fwd`` with norms -> dq, dk, dv and (None: not needed) dwq, dwk fp32 [D]."""
+    L = _lib.calls()
+    cos, sin, positions, steps = _turns(q, cos, sin, positions)
+    q, k = _heads(q), _heads(k)
+    gq, gk, gv = _heads(_like(gq, q)), _heads(_like(gk, q)), _heads(_like(gv, q))
+    if gv is not None:
+        assert _steps(gv) == _steps(gk) and _steps(dv) == _steps(dk) and gv.shape == gk.shape
+    B, S, H, D = q.shape
+    for x, g, d in ((q, gq, dq), (k, gk, dk)):
+        assert x.shape == g.shape == d.shape and x.shape[:2] == (B, S) and x.shape[3] == D
+        assert x.dtype == d.dtype == q.dtype and d.stride(3) == 1
+    for w in (wq, wk):
+        assert w.shape == (D,)
+    for w in (dwq, dwk):
+        assert w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() == D)
+    sms, Hk = sm_count(q.device), k.shape[2]
+    scratch = None
+    if dwq is not None or dwk is not None:
+        scratch = torch.empty(L.pf_heads_bwd_rows(H, Hk, sms) * D, dtype=torch.float32, device=q.device)
+    check(L.pf_heads_bwd(gq, gk, gv, q, k, dq, dk, dv, _floats(wq), _floats(wk), dwq, dwk, scratch, cos, sin,
+                         positions, B, S, H, Hk, D, 2 * cos.shape[1], _steps(gq), _steps(gk), _steps(q), _steps(k),
+                         _steps(dq), _steps(dk), steps, cos.shape[0], int(interleaved), eps, int(accumulate),
+                         dt(q.dtype), sms, stream_of(q)), "pf_heads_bwd")
+
+
+# --------------------------------------------------------------------------- preference and policy losses
+def _token_rows(logits: torch.Tensor, labels: torch.Tensor):
+    """(logits [N, T, V] with V innermost, packed int64 labels)"""
+    assert logits.dim() == 3 and labels.shape == logits.shape[:2] and labels.device == logits.device
+    return logits if logits.stride(2) == 1 or logits.shape[2] == 1 else logits.contiguous(), labels.long().contiguous()
+
+
+def preference_fwd(logits: torch.Tensor, labels: torch.Tensor, ref: torch.Tensor, beta: float, smoothing: float,
+                   ignore_index: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """-> (loss, rewards [N], stats [N, T, 2], coef [N]), all fp32; stats and coef are for ``token_loss_bwd``."""
+    L = _lib.calls()
+    z, labels = _token_rows(logits, labels)
+    N, T, V = z.shape
+    assert N >= 2 and N % 2 == 0 and ref.shape == (N,) and ref.device == z.device
+    new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=z.device)
+    loss, rewards, stats, coef = new(), new(N), new(N, T, 2), new(N)
+    scratch = torch.empty(N * T + N, dtype=torch.float64, device=z.device)
+    check(L.pf_preference_fwd(z, labels, _floats(ref), loss, rewards, stats, coef, scratch, N, T, V, z.stride(0),
+                              z.stride(1), ignore_index, beta, smoothing, dt(z.dtype), sm_count(z.device),
+                              stream_of(z)), "pf_preference_fwd")
+    return loss, rewards, stats, coef
+
+
+def policy_fwd(logits: torch.Tensor, actions: torch.Tensor, old: torch.Tensor, adv: torch.Tensor,
+               ref: Optional[torch.Tensor], low: float, high: float, kl_coef: float, temperature: float,
+               ignore_index: int) -> Tuple[torch.Tensor, ...]:
+    """-> (loss, logps [N, T], kl, clipped, stats [N, T, 2], coef [N, T], one over the tokens that count), all fp32."""
+    L = _lib.calls()
+    z, actions = _token_rows(logits, actions)
+    N, T, V = z.shape
+    for t in (old, adv, ref):
+        assert t is None or (t.shape == (N, T) and t.device == z.device)
+    adv = adv if adv.dtype == torch.float32 else adv.float()
+    new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=z.device)
+    loss, kl, clipped, inv = new(), new(), new(), new()
+    logps, coef, stats, scratch = new(N, T), new(N, T), new(N, T, 2), new(N, T, 4)
+    check(L.pf_policy_fwd(z, actions, _floats(old), None if ref is None else _floats(ref), adv, loss, kl, clipped,
+                          inv, logps, coef, stats, scratch, N, T, V, z.stride(0), z.stride(1), adv.stride(0),
+                          adv.stride(1), ignore_index, low, high, kl_coef, 1.0 / temperature, dt(z.dtype),
+                          sm_count(z.device), stream_of(z)), "pf_policy_fwd")
+    return loss, logps, kl, clipped, stats, coef, inv
+
+
+def token_loss_bwd(gout: torch.Tensor, logits: torch.Tensor, labels: torch.Tensor, stats: torch.Tensor,
+                   coef: torch.Tensor, inv: Optional[torch.Tensor], ignore_index: int, temperature: float
+                   ) -> torch.Tensor:
+    """dlogits [N, T, V] = gout * coef * inv * (onehot - p); coef has a value for each sequence or for each row."""
+    L = _lib.calls()
+    z, labels = _token_rows(logits, labels)
+    N, T, V = z.shape
+    assert gout.numel() == 1 and stats.numel() == 2 * N * T and coef.numel() in (N, N * T)
+    d = torch.empty((N, T, V), dtype=z.dtype, device=z.device)
+    check(L.pf_token_loss_bwd(z, labels, _vectors(_floats(stats)), _floats(coef), _floats(gout),
+                              None if inv is None else _floats(inv), d, N, T, V, z.stride(0), z.stride(1),
+                              ignore_index, 1 if coef.numel() == N * T else T, 1.0 / temperature, dt(z.dtype),
+                              sm_count(z.device), stream_of(z)), "pf_token_loss_bwd")
+    return d
+
+
 # --------------------------------------------------------------------------- attention
 def attention_supported(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bool:
     """True when the native flash-attention kernels cover this problem."""

@@ -1,0 +1,465 @@
+"""Preference and policy losses, forward and backward, against their formulas in 64 bits.
+
+Bounds.  u is half a step of a type, E = 2^-24 that of fp32.  A row's sum of exponentials: each exponent k z - M is
+rounded twice (k and the difference) at the size of the largest |k z|, each exponential is off by 2^-22 of its value,
+and a thread adds up at most V / 32 + 64 of them one after the other, so the sum is off by
+R = (V / 32 + 68 + 4 max |k z|) E + 2^-22, and a log-probability l by R + E (|z| + |l|).  A gradient
+g (onehot - p) has p off by 2 R and g by what its loss makes of the error of l."""
+import math
+
+import pytest
+import torch
+
+from pfeife_b200 import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+TINY = {torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -126}
+E = 2.0 ** -24
+
+
+def near(got, want, off):
+    """|got - want| <= u |want| + off"""
+    got64 = got.double()
+    assert torch.isfinite(got).all()
+    bound = U[got.dtype] * want.abs() + 1.01 * off + TINY[got.dtype]
+    worst = ((got64 - want).abs() / bound).max() if got.numel() else 0.0
+    assert worst <= 1.0, float(worst)
+
+
+def batch(N, T, V, device, dtype, seed, layout="packed", masked=0.4):
+    g = torch.Generator().manual_seed(seed)
+    new = lambda *s: (torch.randn(*s, generator=g) * 2).to(device=device, dtype=dtype)
+    if layout == "shifted":                      # all but the last position of longer sequences
+        z = new(N, T + 1, V)[:, :-1]
+    elif layout == "seq first":
+        z = new(T, N, V).transpose(0, 1)
+    elif layout == "columns":                    # V is not innermost
+        z = new(N, V, T).transpose(1, 2)
+    elif layout == "wide":                       # some words of a padded vocabulary, off the vectors
+        z = new(N, T, V + 5)[..., 3:3 + V]
+    else:
+        z = new(N, T, V)
+    labels = torch.randint(0, V, (N, T), generator=g)
+    labels[torch.rand(N, T, generator=g) < masked] = -100
+    return z, labels.to(device)
+
+
+def rows64(z, labels, temperature):
+    """(l, its error bound, softmax, its relative error bound, which rows count) in 64 bits"""
+    V = z.shape[-1]
+    counted = (labels >= 0) & (labels < V)
+    x = z.double() / temperature
+    lse = x.logsumexp(-1)
+    zl = x.gather(-1, labels.clamp(0, V - 1).unsqueeze(-1))[..., 0]
+    l = (zl - lse).masked_fill(~counted, 0.0)
+    big = x.masked_fill(x.isinf(), 0.0).abs().amax(-1) * 1.4427
+    rel = (V / 32 + 68 + 4 * big) * E + 2.0 ** -22
+    return l, (rel + E * (zl.abs() + l.abs())).masked_fill(~counted, 0.0), torch.softmax(x, -1), 2 * rel, counted
+
+
+def gradient(g, dg, p, rel, labels, counted):
+    """(g (onehot - p), its error bound), zero where nothing counts"""
+    hot = torch.zeros_like(p).scatter_(-1, labels.masked_fill(~counted, 0).unsqueeze(-1), 1.0)
+    g, dg = (t.masked_fill(~counted, 0.0).unsqueeze(-1) for t in (g, dg))
+    off = dg * (hot + p) + g.abs() * p * rel.unsqueeze(-1) + 4 * E * g.abs() * (hot + p)
+    at = counted.unsqueeze(-1)
+    return (g * (hot - p)).masked_fill(~at, 0.0), off.masked_fill(~at, 0.0)
+
+
+# rows of a warp, of a CTA and of a wide CTA; odd lengths, fewer words than a vector
+SIZES = [(2, 1, 1), (2, 3, 7), (4, 5, 256), (2, 9, 1000), (6, 30, 1025), (2, 33, 2049), (2, 2, 9001), (4, 60, 8192),
+         (2, 40, 32003)]
+LAYOUTS = ["packed", "shifted", "seq first", "columns", "wide"]
+
+
+def _cases():
+    out = []
+    for i, size in enumerate(SIZES):
+        for j, dtype in enumerate(DTYPES):
+            out.append((*size, dtype, LAYOUTS[(3 * i + j) % 5]))
+    return out
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("N,T,V,dtype,layout", _cases(), ids=str)
+def test_preference_loss(N, T, V, dtype, layout, device):
+    for seed, (beta, smoothing) in enumerate(((0.1, 0.0), (0.5, 0.2))):
+        z, labels = batch(N, T, V, device, dtype, seed, layout)
+        z.requires_grad_()
+        l, dl, p, rel, counted = rows64(z.detach(), labels, 1.0)
+        ref = (l.sum(1) + torch.randn(N, generator=torch.Generator().manual_seed(9)).to(device) * 3).float()
+        out = ops.preference_loss(z, labels, ref, beta=beta, label_smoothing=smoothing)
+        gout = torch.tensor(2.5, device=device)
+        (dz,) = torch.autograd.grad(out.loss, z, gout)
+        assert dz.shape == z.shape and dz.dtype == dtype and not out.rewards.requires_grad
+        P = N // 2
+        r, dr = beta * (l.sum(1) - ref.double()), beta * dl.sum(1) + 2 * E * beta * (l.sum(1).abs() + ref.abs())
+        near(out.rewards, r, dr)
+        m, dm = r[:P] - r[P:], dr[:P] + dr[P:]
+        sig = lambda t: 1 / (1 + (-t).exp())
+        want = -(1 - smoothing) * sig(m).log() - smoothing * sig(-m).log()
+        near(out.loss.detach(), want.mean(), dm.mean() + 4 * E * want.mean())
+        c = -beta / P * ((1 - smoothing) * sig(-m) - smoothing * sig(m))
+        c = torch.cat([c, -c])[:, None].expand(N, T) * 2.5
+        dc = (2.5 * beta / P * torch.cat([dm, dm]) / 4)[:, None].expand(N, T)     # sig' <= 1/4
+        near(dz, *gradient(c, dc + 4 * E * 2.5 * beta / P, p, rel, labels, counted))
+        assert not dz[~counted].any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("N,T,V,dtype,layout", _cases(), ids=str)
+def test_policy_loss(N, T, V, dtype, layout, device):
+    for seed, (kl, temperature, lo, hi, per_token) in enumerate(((0.0, 1.0, 0.2, 0.2, True), (0.3, 0.7, 0.1, 0.3, False))):
+        z, actions = batch(N, T, V, device, dtype, seed, layout)
+        z.requires_grad_()
+        l, dl, p, rel, counted = rows64(z.detach(), actions, temperature)
+        g = torch.Generator().manual_seed(3)
+        noise = lambda *s: torch.randn(*s, generator=g).to(device)
+        old = (l + 0.2 * noise(N, T)).float()
+        r = (l - old.double()).exp()
+        # no ratio so near a border that the error of l could carry it over
+        for border in (1 - lo, 1 + hi):
+            old = torch.where((r - border).abs() < 4e-3 + 4 * dl, l.float(), old)
+        r = (l - old.double()).exp()
+        adv = noise(N, T) if per_token else noise(N, 1)
+        ref = (l + 0.3 * noise(N, T)).float() if kl else None
+        out = ops.policy_loss(z, actions, old, adv, ref, lo, hi, kl, temperature)
+        (dz,) = torch.autograd.grad(out.loss, z)
+        assert dz.shape == z.shape and dz.dtype == dtype and not any(t.requires_grad for t in out[1:])
+        near(out.logps, l, dl)
+        n, A = max(1, int(counted.sum())), adv.double().expand(N, T)
+        held = ((A > 0) & (r > 1 + hi)) | ((A < 0) & (r < 1 - lo))
+        term = -torch.where(held, torch.where(A > 0, 1 + hi, 1 - lo).double(), r) * A
+        c, off = torch.where(held, 0.0, -A * r), (A * r).abs() * (dl * 1.1 + 8 * E)
+        dc = off.clone()
+        if kl:
+            d = ref.double() - l
+            term, c = term + kl * (torch.expm1(d) - d), c - kl * torch.expm1(d)
+            off = off + kl * (torch.expm1(d).abs() * 1.1 * dl + 4 * E * (torch.expm1(d).abs() + d.abs()))
+            dc = dc + kl * d.exp() * 1.1 * dl + 4 * E * kl * torch.expm1(d).abs()
+            each = (torch.expm1(d) - d)
+            near(out.kl, each[counted].sum() / n, (torch.expm1(d).abs() * 1.1 * dl + 2 * E * each)[counted].sum() / n)
+        else:
+            assert float(out.kl) == 0.0
+        off = off + 4 * E * term.abs()
+        near(out.loss.detach(), term[counted].sum() / n, off[counted].sum() / n)
+        near(out.clipped, (held & counted).sum().double() / n, torch.zeros((), device=device))
+        near(dz, *gradient(c / (n * temperature), (dc + 4 * E * c.abs()) / (n * temperature), p, rel, actions, counted))
+        assert not dz[~counted].any()
+
+
+def test_gradients_are_those_of_differences():
+    torch.manual_seed(1)
+    z = torch.randn(4, 3, 6, dtype=torch.float64, requires_grad=True)
+    labels = torch.tensor([[0, 5, -100], [1, 1, 2], [3, -1, 6], [0, 2, 4]])
+    ref = torch.tensor([-3.0, -5.0, -4.0, -6.0])
+    # losses are rounded to 32 bits: differences of 1e-2 and a tolerance of their curvature and that rounding
+    check = lambda f: torch.autograd.gradcheck(f, [z], eps=1e-2, atol=2e-4, rtol=1e-3)
+    assert check(lambda x: ops.preference_loss(x, labels, ref, 0.5, 0.1).loss.double())
+    lp = torch.log_softmax(z.detach(), -1).gather(-1, labels.clamp(0, 5).unsqueeze(-1))[..., 0]
+    old = (lp + torch.tensor([0.4, -0.05, 0.05])).float()          # held or not by a wide margin
+    adv = torch.tensor([[1.0], [-1.0], [2.0], [0.5]])
+    assert check(lambda x: ops.policy_loss(x, labels, old, adv, old, kl_coef=0.5).loss.double())
+    assert check(lambda x: ops.policy_loss(x, labels, old.flip(1), adv, temperature=2.0).loss.double())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [40, 3001])
+def test_masked_words_and_what_stands_in_rows_that_do_not_count(V, dtype, device):
+    """Logits of -inf and of the type's lowest value have no probability and no gradient; NaN and infinities in rows
+    that do not count reach nothing; labels beyond the vocabulary count as little as the ignored one."""
+    z, labels = batch(4, 6, V, device, dtype, 5, masked=0.0)
+    z[..., V // 2:] = -math.inf
+    z[..., V // 4:V // 2] = torch.finfo(dtype).min
+    labels = labels % (V // 4)
+    labels[0, 1], labels[1, :], labels[2, 3], labels[3, 0] = -100, V, -1, 1 << 40
+    counted = (labels >= 0) & (labels < V)
+    clean = z.clone()
+    z[~counted] = torch.tensor([math.nan, math.inf, -math.inf, 1.0], dtype=dtype).repeat(V // 4 + 1)[:V].to(device)
+    got, want = [], []
+    for values, to in ((z, got), (clean, want)):
+        values = values.detach().requires_grad_()
+        a = ops.preference_loss(values, labels, torch.zeros(4, device=device))
+        old = torch.full((4, 6), -3.0, device=device)
+        b = ops.policy_loss(values, labels, old, torch.ones(4, 1, device=device), old - 1, kl_coef=0.1)
+        to += [a.loss, a.rewards, *b, *torch.autograd.grad(a.loss + b.loss, values)]
+    for a, b in zip(got, want):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    assert not got[-1][..., V // 4:].any() and not got[-1][~counted].any() and got[-1][counted].any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_row_that_counts_keeps_its_nan(device):
+    """A NaN logit, and a row of -inf alone, which has no softmax, are not smoothed over."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    for V in (9, 2500):
+        for fill in (math.nan, -math.inf):
+            z, labels = batch(2, 3, V, device, dtype, 1, masked=0.0)
+            z[0, 1] = fill
+            if fill != fill:
+                z[0, 1, : V - 1] = 0.0
+            labels[0, 1] = 0
+            out = ops.policy_loss(z, labels, torch.zeros(2, 3, device=device), torch.ones(2, 3, device=device))
+            assert torch.isnan(out.loss) and torch.isnan(out.logps[0, 1]) and torch.isfinite(out.logps[1]).all()
+            assert torch.isnan(ops.preference_loss(z, labels, torch.zeros(2, device=device)).loss)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_nothing_counts(device):
+    dtype = torch.float32 if device == "cpu" else torch.float16
+    z, labels = batch(2, 4, 33, device, dtype, 1)
+    labels.fill_(-100)
+    z.requires_grad_()
+    zeros = torch.zeros(2, 4, device=device)
+    out = ops.policy_loss(z, labels, zeros, zeros + 1, zeros, kl_coef=1.0)
+    assert float(out.loss.detach()) == float(out.kl) == float(out.clipped) == 0.0 and not out.logps.any()
+    assert not torch.autograd.grad(out.loss, z)[0].any()
+    pref = ops.preference_loss(z, labels, torch.tensor([1.0, 3.0], device=device), beta=0.5)
+    assert torch.allclose(pref.rewards, torch.tensor([-0.5, -1.5], device=device))
+    assert abs(float(pref.loss.detach()) - math.log1p(math.exp(-1.0))) < 1e-6
+    assert not torch.autograd.grad(pref.loss, z)[0].any()
+    # no tokens at all
+    empty = torch.zeros(2, 0, 33, device=device, dtype=dtype).requires_grad_()
+    none = torch.zeros(2, 0, dtype=torch.int64, device=device)
+    out = ops.policy_loss(empty, none, none.float(), none.float())
+    assert float(out.loss.detach()) == 0.0 and torch.autograd.grad(out.loss, empty)[0].shape == (2, 0, 33)
+    pref = ops.preference_loss(empty, none, torch.zeros(2, device=device))
+    assert abs(float(pref.loss.detach()) - math.log(2)) < 1e-6
+    assert torch.autograd.grad(pref.loss, empty)[0].shape == (2, 0, 33)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_far_margins_do_not_overflow(device):
+    """Margins of hundreds of nats, and an impossible token: -log sig(m) is 0 or -m."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    z, labels = batch(2, 4, 50, device, dtype, 1, masked=0.0)
+    z.requires_grad_()
+    for ref, want in (((0.0, 5000.0), 0.0), ((5000.0, 0.0), None)):
+        ref = torch.tensor(ref, device=device)
+        out = ops.preference_loss(z, labels, ref, beta=1.0)
+        m = float(out.rewards[0] - out.rewards[1])
+        assert abs(float(out.loss.detach()) - max(-m, 0.0)) <= 1e-5 * abs(m)
+        (dz,) = torch.autograd.grad(out.loss, z)
+        assert torch.isfinite(dz).all() and (dz.any() if want is None else True)
+    with torch.no_grad():
+        z[1, 2, labels[1, 2]] = -math.inf
+    assert float(ops.preference_loss(z, labels, torch.zeros(2, device=device)).loss.detach()) == 0.0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_shapes_types_and_an_ignored_word(device):
+    """One dimension of tokens or three, labels of 32 bits, a word of the vocabulary that does not count, advantages
+    and log-probabilities of other types."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    z, labels = batch(6, 4, 33, device, dtype, 1, masked=0.0)
+    labels[2, 1] = 0
+    old, adv = torch.full((6, 4), -3.0, device=device), torch.linspace(-1, 1, 24, device=device).view(6, 4)
+    z.requires_grad_()
+    def both(z, labels, old, adv, ref=None):
+        out = ops.policy_loss(z, labels, old, adv, ref, ignore_index=0, kl_coef=0.1)
+        return out.loss, out.logps.reshape(6, 4), torch.autograd.grad(out.loss, z)[0].reshape(6, 4, 33)
+    want = both(z, labels, old, adv)
+    flat = z.detach().view(24, 33).requires_grad_()
+    deep = z.detach().view(2, 3, 4, 33).requires_grad_()
+    for got in (both(flat, labels.view(24), old.view(24), adv.view(24)),
+                both(deep, labels.view(2, 3, 4), old.view(2, 3, 4), adv.view(2, 3, 4)),
+                both(z, labels.int(), old.double(), adv.double())):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert not want[1][labels == 0].any() and not want[2][labels == 0].any()
+    some = torch.linspace(-1, 1, 6, device=device)[:, None]
+    a, b = (both(z, labels, old, t, old) for t in (some, some.expand(6, 4).contiguous()))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    pa, pb = (ops.preference_loss(z, t, torch.zeros(6, device=device).to(r), ignore_index=0) for t, r in
+              ((labels, torch.float32), (labels.int(), torch.float64)))
+    assert torch.equal(pa.loss, pb.loss) and torch.equal(pa.rewards, pb.rewards)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    z, labels = batch(2, 3, 9, device, torch.float32, 1)
+    v, ref = torch.zeros(2, 3, device=device), torch.zeros(2, device=device)
+    other = "meta" if device == "cpu" else "cpu"
+    for bad in (dict(logits=z[:1], labels=labels[:1], ref_logps=ref[:1]), dict(logits=z[0], labels=labels[0]),
+                dict(labels=labels[:, :2]), dict(labels=v), dict(labels=labels.to(other)), dict(ref_logps=v),
+                dict(ref_logps=ref.to(other)), dict(ref_logps=ref.clone().requires_grad_()), dict(label_smoothing=-0.1),
+                dict(label_smoothing=1.5), dict(logits=z[..., :0])):
+        with pytest.raises(ValueError):
+            ops.preference_loss(**{**dict(logits=z, labels=labels, ref_logps=ref), **bad})
+    for bad in (dict(logits=z[0, 0], actions=labels[0, 0]), dict(actions=labels[:, :2]), dict(old_logps=v[:1]),
+                dict(ref_logps=v[:, :1]), dict(advantages=v[:, :2]), dict(advantages=ref), dict(temperature=0.0),
+                dict(temperature=-1.0), dict(clip_low=1.5), dict(clip_high=-0.1), dict(old_logps=v.to(other)),
+                dict(advantages=v.clone().requires_grad_()), dict(actions=v)):
+        with pytest.raises(ValueError):
+            ops.policy_loss(**{**dict(logits=z, actions=labels, old_logps=v, advantages=v), **bad})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,V", [(70001, 33), (9000, 1500)])
+def test_many_rows(rows, V):
+    z, labels = batch(1, rows, V, "cuda", torch.bfloat16, 1)
+    z.requires_grad_()
+    l, dl, p, rel, counted = rows64(z.detach(), labels, 1.0)
+    old = l.float()
+    adv = torch.rand(1, rows, device="cuda") + 0.5
+    out = ops.policy_loss(z, labels, old, adv)
+    n = int(counted.sum())
+    near(out.logps, l, dl)
+    near(out.loss.detach(), -(adv.double() * counted).sum() / n, (adv * (1.1 * dl + 8 * E) * counted).sum() / n)
+    two = torch.cat([z, z.flip(1)]).detach().requires_grad_()
+    ref = torch.stack([l.sum(), l.sum() - 1]).float()[0].reshape(1, -1)[0]
+    pref = ops.preference_loss(two, torch.cat([labels, labels.flip(1)]), torch.cat([ref, ref - 1]))
+    near(pref.rewards, 0.1 * torch.tensor([0.0, 1.0], device="cuda", dtype=torch.float64),
+         (0.1 * dl.sum() + 4 * E * l.sum().abs()).expand(2))
+    (dz,) = torch.autograd.grad(pref.loss, two)
+    assert torch.isfinite(dz).all() and not dz[0][~counted[0]].any()
+
+
+@pytest.mark.gpu
+def test_other_streams_graphs_and_bits_that_repeat():
+    from pfeife_b200.ops import functional as f
+    z, labels = batch(4, 37, 5001, "cuda", torch.bfloat16, 1)
+    old = torch.full((4, 37), -9.0, device="cuda")
+    adv, ref, one = torch.randn(4, 1, device="cuda"), torch.zeros(4, device="cuda"), torch.ones((), device="cuda")
+
+    def both(z):
+        a = f.policy_fwd(z, labels, old, adv.expand(4, 37), old, 0.2, 0.2, 0.1, 1.0, -100)
+        b = f.preference_fwd(z, labels, ref, 0.1, 0.1, -100)
+        da = f.token_loss_bwd(one, z, labels, a[4], a[5], a[6], -100, 1.0)
+        db = f.token_loss_bwd(one, z, labels, b[2], b[3], None, -100, 1.0)
+        return [*a[:4], b[0], b[1], da, db]
+
+    with torch.no_grad():
+        want = both(z)
+        assert all(torch.equal(a, b) for a, b in zip(both(z), want))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = both(z)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        static = torch.zeros_like(z)
+        graphs = []
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                out = both(static)
+            graphs.append((g, out))
+        static.copy_(z)
+        for g, _ in graphs + graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Rows whose logits lie further than 2^31 elements in, and whose gradient does."""
+    N, T, V = 2, 35000, 32000                    # 2.2e9 elements
+    z = torch.zeros(N, T, V, device="cuda", dtype=torch.bfloat16)
+    z[1, T - 3:].normal_()
+    labels = torch.full((N, T), -100, device="cuda")
+    labels[0, 5], labels[1, T - 3:] = 3, 7
+    z.requires_grad_()
+    out = ops.preference_loss(z, labels, torch.zeros(2, device="cuda"))
+    (dz,) = torch.autograd.grad(out.loss, z)
+    l, dl, p, rel, counted = rows64(z.detach()[1:, T - 3:], labels[1:, T - 3:], 1.0)
+    near(out.rewards[1], 0.1 * l.sum(), 0.1 * dl.sum() + 4 * E * l.sum().abs())
+    m = (out.rewards[0] - out.rewards[1]).double()
+    c = (0.1 * torch.sigmoid(-m)).expand(1, 3)
+    near(dz[1:, T - 3:], *gradient(c, c * 1e-5, p, rel, labels[1:, T - 3:], counted))
+    assert int(dz.count_nonzero(-1).ne(0).sum()) == 4
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_ops_are_seen_by_tracers_and_modes(device):
+    from pfeife_b200.ops import functional as f
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    z, labels = batch(4, 5, 12, device, dtype, 1)
+    z.requires_grad_()
+    v, ref = torch.zeros(4, 5, device=device), torch.zeros(4, device=device)
+    checks = ("test_schema", "test_faketensor", "test_autograd_registration")
+    torch.library.opcheck(f.preference_fwd, (z, labels, ref, 0.1, 0.0, -100), test_utils=checks)
+    torch.library.opcheck(f.policy_fwd, (z, labels, v, v, None, 0.2, 0.2, 0.0, 1.0, -100), test_utils=checks)
+    fn = lambda t: ops.preference_loss(t, labels, ref).loss + ops.policy_loss(t, labels, v, v + 1, v, kl_coef=0.1).loss
+    want = fn(z)
+    got = torch.compile(fn, backend="eager", fullgraph=True)(z)
+    assert torch.equal(got, want)
+    assert torch.equal(torch.autograd.grad(got, z)[0], torch.autograd.grad(want, z)[0])
+
+
+# ------------------------------------------------------------------------------ together
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("loss", ["preference", "policy"])
+def test_a_decoder_with_normed_heads_tuned_on_a_loss(loss, device):
+    """One step of a decoder with normed queries and keys and a scaled, partial, interleaved rotation: the loss and
+    every gradient against the same model in plain 64-bit PyTorch."""
+    from pfeife_b200.models.llama import Llama, llama_config
+    torch.manual_seed(0)
+    cfg = llama_config("llama_tiny", qk_norm=True, rope_dim=8, rope_interleaved=True, num_layers=2,
+                       rope_scaling=ops.RopeScaling("yarn", 2.0, 16))
+    model = Llama(cfg)
+    with torch.no_grad():
+        for name, p in model.named_parameters():
+            if name.endswith("norm"):
+                p.add_(0.3 * torch.randn_like(p))
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    model = model.to(device)
+    for p in model.parameters():
+        if p.dim() > 1:
+            p.data = p.data.to(dtype)
+    g = torch.Generator().manual_seed(1)
+    ids = torch.randint(0, 256, (4, 24), generator=g).to(device)
+    labels = torch.cat([ids[:, 1:], ids.new_full((4, 1), -100)], 1)
+    labels[:, :5] = -100
+    labels[1, 15:] = -100
+    ref, old = torch.randn(4, generator=g).to(device) - 80, torch.full((4, 24), -5.4, device=device)
+    adv = torch.tensor([[1.0], [-0.5], [0.7], [-1.2]], device=device)
+
+    def tuned(logits):
+        if loss == "preference":
+            return ops.preference_loss(logits, labels, ref).loss
+        return ops.policy_loss(logits, labels, old, adv, old, 0.6, 0.8, kl_coef=0.1).loss
+
+    got = tuned(model(ids))
+    names = [n for n, _ in model.named_parameters()]
+    grads = torch.autograd.grad(got, list(model.parameters()))
+
+    w = {n: p.detach().double().requires_grad_() for n, p in model.named_parameters()}
+    def norm(x, gain, eps=cfg.rms_eps):
+        return x * (x.square().mean(-1, keepdim=True) + eps).rsqrt() * gain
+    x = w["embed.weight"][ids]
+    for i in range(cfg.num_layers):
+        at = lambda n: w[f"layers.{i}.{n}"]
+        qkv = (norm(x, at("input_norm")) @ at("qkv.weight").t()).view(4, 24, 3, 4, 16)
+        where = (model.rope_cos.double()[:24, None], model.rope_sin.double()[:24, None])
+        def turn(t):
+            a, b = t[..., 0:8:2], t[..., 1:8:2]
+            c, s = where
+            return torch.cat([torch.stack([a * c - b * s, b * c + a * s], -1).flatten(-2), t[..., 8:]], -1)
+        q, k = turn(norm(qkv[:, :, 0], at("q_norm"))), turn(norm(qkv[:, :, 1], at("k_norm")))
+        scores = torch.einsum("bqhd,bkhd->bhqk", q, k) / 4
+        scores = scores.masked_fill(torch.ones(24, 24, dtype=torch.bool, device=device).triu(1), -math.inf)
+        a = torch.einsum("bhqk,bkhd->bqhd", scores.softmax(-1), qkv[:, :, 2]).reshape(4, 24, 64)
+        x = x + a @ at("o_proj.weight").t()
+        gate, up = (norm(x, at("post_norm")) @ at("gate_up.weight").t()).chunk(2, -1)
+        x = x + (torch.nn.functional.silu(gate) * up) @ at("down.weight").t()
+    z = norm(x, w["norm"]) @ w["lm_head.weight"].t()
+    l = torch.log_softmax(z, -1).gather(-1, labels.clamp(min=0).unsqueeze(-1))[..., 0] * (labels >= 0)
+    if loss == "preference":
+        r = 0.1 * (l.sum(1) - ref)
+        want = -torch.nn.functional.logsigmoid(r[:2] - r[2:]).mean()
+    else:
+        ratio, d = (l - old).exp(), old - l
+        term = -torch.minimum(ratio * adv, ratio.clamp(0.4, 1.8) * adv) + 0.1 * (d.exp() - d - 1)
+        want = (term * (labels >= 0)).sum() / (labels >= 0).sum()
+    exact = torch.autograd.grad(want, list(w.values()))
+    # some 40 roundings of 2^-8 lie between a weight and the loss in 16 bits, 2^-24 in 32; they add up at random
+    rel = 40 * (2.0 ** -24 * 8 if device == "cpu" else 2.0 ** -8 / 2)
+    got, want = float(got.detach()), float(want.detach())
+    assert abs(got - want) < rel * abs(want) + rel * 0.1
+    for name, a, b in zip(names, grads, exact):
+        assert (a.double() - b).norm() <= rel * b.norm() + 1e-12, name
