@@ -580,6 +580,171 @@ struct DirectRopeQkv : torch::autograd::Function<DirectRopeQkv> {
   }
 };
 
+// ------------------------------------------------------------------------------ rotations of any layout, head norms
+// Heads [B, S, H, D], or one of the slices of a projection [B, S, 3, H, D], as qk_rope.cu takes them.
+struct HeadView {
+  char* at;
+  long long steps[3];
+  explicit HeadView(const Tensor& t, int slice = -1) : at(static_cast<char*>(t.data_ptr())) {
+    const bool packed = slice >= 0;
+    const int d[3] = {0, 1, packed ? 3 : 2};
+    for (int i = 0; i < 3; ++i) steps[i] = t.size(d[i]) > 1 ? t.stride(d[i]) : 0;
+    if (packed) at += slice * t.stride(2) * (long long)t.element_size();
+  }
+};
+bool number(const Tensor& t) { return half(t) || t.scalar_type() == at::kFloat; }
+bool head_view_fits(const Tensor& t, int dim) {
+  return t.dim() == dim && number(t) && t.numel() > 0 && t.stride(dim - 1) == 1 && t.size(dim - 1) >= 2 &&
+         t.size(dim - 1) <= 256 && (dim == 4 || t.size(2) == 3);
+}
+// tables and positions for x [B, S, .., D]
+bool angles_fit(const Tensor& x, const Tensor& cos, const Tensor& sin, const Tensor& pos) {
+  const int64_t B = x.size(0), S = x.size(1);
+  for (const Tensor* t : {&cos, &sin})
+    if (t->scalar_type() != at::kFloat || t->dim() != 2 || !t->is_contiguous()) return false;
+  if (cos.sizes() != sin.sizes() || cos.size(1) < 1 || 2 * cos.size(1) > x.size(-1)) return false;
+  if (!pos.defined()) return cos.size(0) >= S;
+  return pos.scalar_type() == at::kLong &&
+         ((pos.dim() == 1 && pos.size(0) == S) || (pos.dim() == 2 && pos.size(0) == B && pos.size(1) == S));
+}
+struct Angles {
+  const Tensor &cos, &sin, &pos;
+  long long steps[2];
+  Angles(const Tensor& c, const Tensor& s, const Tensor& p) : cos(c), sin(s), pos(p), steps{0, 0} {
+    if (!p.defined()) return;
+    steps[0] = p.dim() == 2 ? p.stride(0) : 0;
+    steps[1] = p.stride(-1);
+  }
+};
+Tensor inner_packed(const Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+
+// q -> yq, and where given k -> yk and (slices of a projection) v -> yv
+void heads_run(const Env& e, const Tensor& like, const HeadView& q, const HeadView* k, const HeadView* v, const HeadView& yq,
+               const HeadView* yk, const HeadView* yv, const Tensor& wq, const Tensor& wk, const Angles& a,
+               int64_t hq, int64_t hk, bool interleaved, bool inverse, double eps) {
+  ok(pf_heads_fwd(q.at, k ? k->at : nullptr, v ? v->at : nullptr, yq.at, yk ? yk->at : nullptr, yv ? yv->at : nullptr,
+                  at_or_null(wq), at_or_null(wk), a.cos.data_ptr(), a.sin.data_ptr(), at_or_null(a.pos), like.size(0),
+                  (int)like.size(1), (int)hq, (int)hk, (int)like.size(-1), (int)(2 * a.cos.size(1)), q.steps,
+                  k ? k->steps : nullptr, yq.steps, yk ? yk->steps : nullptr, a.steps, a.cos.size(0), interleaved,
+                  inverse, (float)eps, code_of(like), e.sms, e.stream),
+     "pf_heads_fwd");
+}
+Tensor rotate(const Tensor& x, const Tensor& cos, const Tensor& sin, const Tensor& pos, bool interleaved, bool inverse) {
+  const Env e(x);
+  const Tensor y = empty(x.sizes(), x);
+  const Angles a(cos, sin, pos);
+  if (x.dim() == 4) {
+    heads_run(e, x, HeadView(x), nullptr, nullptr, HeadView(y), nullptr, nullptr, {}, {}, a, x.size(2), 0, interleaved,
+              inverse, 0.0);
+  } else {
+    const HeadView k(x, 1), v(x, 2), yk(y, 1), yv(y, 2);
+    heads_run(e, x, HeadView(x, 0), &k, &v, HeadView(y, 0), &yk, &yv, {}, {}, a, x.size(3), x.size(3), interleaved,
+              inverse, 0.0);
+  }
+  return y;
+}
+struct DirectRotate : torch::autograd::Function<DirectRotate> {
+  static Tensor forward(AutogradContext* ctx, Tensor x, Tensor cos, Tensor sin, Maybe positions, bool interleaved) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    ctx->save_for_backward({cos, sin, value(positions)});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["dim"] = x.dim();
+    return rotate(x, cos, sin, value(positions), interleaved, false);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &cos = s[0], &sin = s[1], &pos = s[2];
+    const Tensor dy = inner_packed(grads[0]);
+    const bool interleaved = ctx->saved_data["interleaved"].toBool();
+    const int dim = (int)ctx->saved_data["dim"].toInt();
+    Tensor dx;
+    if (direct(dy, cos, sin, pos) && head_view_fits(dy, dim) && angles_fit(dy, cos, sin, pos))
+      below([&] { dx = rotate(dy, cos, sin, pos, interleaved, true); return 0; });
+    else
+      dx = dispatched(dim == 4 ? "pfeife::rope_at" : "pfeife::rope_qkv_at",
+                      {dy, cos, sin, opt(pos), interleaved, true})[0].toTensor();
+    return {dx, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+bool gain_fits(const Tensor& w, const Tensor& x) { return packed_floats(w, x.size(-1)) && w.dim() == 1; }
+bool same_heads(const Tensor& q, const Tensor& k) {
+  return head_view_fits(q, 4) && head_view_fits(k, 4) && q.scalar_type() == k.scalar_type() && q.size(0) == k.size(0) &&
+         q.size(1) == k.size(1) && q.size(3) == k.size(3);
+}
+// q and k, or the projection qkv in the place of q (k not defined)
+variable_list norm_rotate(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& cos,
+                          const Tensor& sin, const Tensor& pos, double eps, bool interleaved) {
+  const Env e(q);
+  const Angles a(cos, sin, pos);
+  const Tensor y = empty(q.sizes(), q);
+  if (k.defined()) {
+    const Tensor z = empty(k.sizes(), k);
+    const HeadView kv(k), zv(z);
+    heads_run(e, q, HeadView(q), &kv, nullptr, HeadView(y), &zv, nullptr, wq, wk, a, q.size(2), k.size(2), interleaved,
+              false, eps);
+    return {y, z};
+  }
+  const HeadView kv(q, 1), vv(q, 2), zk(y, 1), zv(y, 2);
+  heads_run(e, q, HeadView(q, 0), &kv, &vv, HeadView(y, 0), &zk, &zv, wq, wk, a, q.size(3), q.size(3), interleaved,
+            false, eps);
+  return {y};
+}
+struct DirectNormRotate : torch::autograd::Function<DirectNormRotate> {
+  static variable_list forward(AutogradContext* ctx, Tensor q, Maybe keys, Tensor wq, Tensor wk, Tensor cos,
+                               Tensor sin, Maybe positions, double eps, bool interleaved) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    ctx->save_for_backward({q, value(keys), wq, wk, cos, sin, value(positions)});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    return norm_rotate(q, value(keys), wq, wk, cos, sin, value(positions), eps, interleaved);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &q = s[0], &k = s[1], &wq = s[2], &wk = s[3], &cos = s[4], &sin = s[5], &pos = s[6];
+    const double eps = ctx->saved_data["eps"].toDouble();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool(), two = k.defined();
+    const Tensor gq = inner_packed(grads[0]), gk = two ? inner_packed(grads[1]) : Tensor();
+    Tensor dq, dk, dwq, dwk;
+    const bool fits = two ? same_heads(q, k) && matches(gq, q) && matches(gk, k)
+                          : head_view_fits(q, 5) && matches(gq, q);
+    if (direct(gq, gk, q, k, wq, wk, cos, sin, pos) && fits && gain_fits(wq, q) && gain_fits(wk, q) &&
+        angles_fit(q, cos, sin, pos)) {
+      below([&] {
+        const Env e(gq);
+        const Angles a(cos, sin, pos);
+        const int D = (int)q.size(-1), hq = (int)q.size(two ? 2 : 3), hk = (int)(two ? k.size(2) : hq);
+        dq = empty(q.sizes(), q);
+        if (two) dk = empty(k.sizes(), k);
+        dwq = floats(D, q);
+        dwk = floats(D, q);
+        const Tensor scratch = floats((int64_t)pf_heads_bwd_rows(hq, hk, e.sms) * D, q);
+        const int at = two ? -1 : 0;
+        const HeadView vgq(gq, at), vq(q, at), vdq(dq, at);
+        const HeadView vgk = two ? HeadView(gk) : HeadView(gq, 1), vk = two ? HeadView(k) : HeadView(q, 1),
+                       vdk = two ? HeadView(dk) : HeadView(dq, 1);
+        char* gv = two ? nullptr : HeadView(gq, 2).at;
+        char* dv = two ? nullptr : HeadView(dq, 2).at;
+        ok(pf_heads_bwd(vgq.at, vgk.at, gv, vq.at, vk.at, vdq.at, vdk.at, dv, wq.data_ptr(), wk.data_ptr(),
+                        dwq.data_ptr(), dwk.data_ptr(), scratch.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+                        at_or_null(pos), q.size(0), (int)q.size(1), hq, hk, D, (int)(2 * cos.size(1)), vgq.steps,
+                        vgk.steps, vq.steps, vk.steps, vdq.steps, vdk.steps, a.steps, cos.size(0), interleaved,
+                        (float)eps, 0, code_of(q), e.sms, e.stream),
+           "pf_heads_bwd");
+        return 0;
+      });
+    } else if (two) {
+      auto out = dispatched("pfeife::qk_norm_rope_bwd",
+                            {gq, gk, q, k, wq, wk, cos, sin, opt(pos), eps, interleaved});
+      dq = out[0].toTensor(); dk = out[1].toTensor(); dwq = given(out[2]); dwk = given(out[3]);
+    } else {
+      auto out = dispatched("pfeife::qk_norm_rope_qkv_bwd", {gq, q, wq, wk, cos, sin, opt(pos), eps, interleaved});
+      dq = out[0].toTensor(); dwq = given(out[1]); dwk = given(out[2]);
+    }
+    return {dq, dk, dwq, dwk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
 Tensor glu_forward(const Tensor& gu, bool gelu) {
   const Env e(gu);
   const int64_t H = gu.size(-1) / 2;
@@ -671,6 +836,133 @@ struct DirectCrossEntropy : torch::autograd::Function<DirectCrossEntropy> {
               .toTensor();
     }
     return {d, Tensor(), Tensor()};
+  }
+};
+
+// ------------------------------------------------------------------------------ preference and policy losses
+// Logits [N, T, V] and a label for each row.
+bool tokens_fit(const Tensor& z, const Tensor& labels) {
+  return z.dim() == 3 && number(z) && z.numel() > 0 && z.stride(2) == 1 && z.size(2) < (1ll << 31) &&
+         z.size(1) < (1ll << 31) && labels.scalar_type() == at::kLong && labels.dim() == 2 && labels.is_contiguous() &&
+         labels.size(0) == z.size(0) && labels.size(1) == z.size(1);
+}
+float* float_at(const Tensor& t, int64_t i) { return static_cast<float*>(t.data_ptr()) + i; }
+
+// What the backward of both needs lies in one buffer: two statistics a row, then `n` factors (one for each sequence or
+// each row) and, for a policy, one over the number of tokens that count.
+struct Kept {
+  Tensor all;
+  int64_t rows, n;
+  bool inv;
+  int64_t size() const { return 2 * rows + n + inv; }
+  float* stats() const { return float_at(all, 0); }
+  float* coef() const { return float_at(all, 2 * rows); }
+  float* one_over() const { return inv ? float_at(all, 2 * rows + n) : nullptr; }
+};
+variable_list token_loss_backward(AutogradContext* ctx, const Tensor& g, int inputs) {
+  variable_list out(inputs);
+  if (!g.defined()) return out;
+  const auto s = ctx->get_saved_variables();
+  const Tensor &z = s[0], &labels = s[1];
+  const int64_t ignore = ctx->saved_data["ignore"].toInt();
+  const double temperature = ctx->saved_data["temperature"].toDouble();
+  const bool inv = ctx->saved_data["inv"].toBool();
+  const int64_t N = z.size(0), T = z.dim() > 1 ? z.size(1) : 0;
+  const Kept kept{s[2], N * T, inv ? N * T : N, inv};
+  if (direct(g, z, labels, kept.all) && tokens_fit(z, labels) && packed_floats(kept.all, kept.size()) &&
+      aligned(kept.all) && packed_floats(g, 1)) {
+    below([&] {
+      const Env e(z);
+      out[0] = empty(z.sizes(), z);
+      ok(pf_token_loss_bwd(z.data_ptr(), labels.data_ptr(), kept.stats(), kept.coef(), g.data_ptr(), kept.one_over(),
+                           out[0].data_ptr(), N, (int)T, (int)z.size(2), z.stride(0), z.stride(1), ignore,
+                           inv ? 1 : (int)T, (float)(1.0 / temperature), code_of(z), e.sms, e.stream),
+         "pf_token_loss_bwd");
+      return 0;
+    });
+    return out;
+  }
+  const Tensor a = kept.all;
+  Tensor coef = a.narrow(0, 2 * kept.rows, kept.n), one;
+  if (inv) {
+    coef = coef.view({N, T});
+    one = a.narrow(0, 2 * kept.rows + kept.n, 1).view({});
+  }
+  out[0] = dispatched("pfeife::token_loss_bwd", {g, z, labels, a.narrow(0, 0, 2 * kept.rows).view({N, T, 2}), coef,
+                                                 opt(one), ignore, temperature})[0].toTensor();
+  return out;
+}
+
+variable_list preference_forward(const Tensor& z, const Tensor& labels, const Tensor& ref, double beta, double smoothing,
+                                 int64_t ignore, Tensor& all) {
+  const Env e(z);
+  const int64_t N = z.size(0), T = z.size(1);
+  const Kept kept{floats(2 * N * T + N, z), N * T, N, false};
+  all = kept.all;
+  const Tensor loss = empty({}, at::kFloat, z), rewards = floats(N, z), scratch = empty({N * T + N}, at::kDouble, z);
+  ok(pf_preference_fwd(z.data_ptr(), labels.data_ptr(), ref.data_ptr(), loss.data_ptr(), rewards.data_ptr(),
+                       kept.stats(), kept.coef(), scratch.data_ptr(), N, (int)T, (int)z.size(2), z.stride(0),
+                       z.stride(1), ignore, (float)beta, (float)smoothing, code_of(z), e.sms, e.stream),
+     "pf_preference_fwd");
+  return {loss, rewards};
+}
+struct DirectPreference : torch::autograd::Function<DirectPreference> {
+  static variable_list forward(AutogradContext* ctx, Tensor z, Tensor labels, Tensor ref, double beta, double smoothing,
+                               int64_t ignore) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    Tensor all;
+    const variable_list out = preference_forward(z, labels, ref, beta, smoothing, ignore, all);
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({out[1]});
+    ctx->save_for_backward({z, labels, all});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["temperature"] = 1.0;
+    ctx->saved_data["inv"] = false;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return token_loss_backward(ctx, grads[0], 6);
+  }
+};
+
+// the advantages' strides for [N, T]; one of a single place is expanded
+bool advantages_fit(const Tensor& a, int64_t N, int64_t T) {
+  return a.scalar_type() == at::kFloat && a.dim() == 2 && (a.size(0) == N || a.size(0) == 1) &&
+         (a.size(1) == T || a.size(1) == 1);
+}
+struct Clipping { double low, high, kl, temperature; };
+variable_list policy_forward(const Tensor& z, const Tensor& actions, const Tensor& old, const Tensor& adv,
+                             const Tensor& ref, const Clipping& c, int64_t ignore, Tensor& all) {
+  const Env e(z);
+  const int64_t N = z.size(0), T = z.size(1), rows = N * T;
+  const Kept kept{floats(3 * rows + 1, z), rows, rows, true};
+  all = kept.all;
+  const Tensor loss = empty({}, at::kFloat, z), logps = empty({N, T}, at::kFloat, z), kl = empty({}, at::kFloat, z),
+               clipped = empty({}, at::kFloat, z), scratch = floats(4 * rows, z);
+  ok(pf_policy_fwd(z.data_ptr(), actions.data_ptr(), old.data_ptr(), at_or_null(ref), adv.data_ptr(), loss.data_ptr(),
+                   kl.data_ptr(), clipped.data_ptr(), kept.one_over(), logps.data_ptr(), kept.coef(), kept.stats(),
+                   scratch.data_ptr(), N, (int)T, (int)z.size(2), z.stride(0), z.stride(1),
+                   adv.size(0) > 1 ? adv.stride(0) : 0, adv.size(1) > 1 ? adv.stride(1) : 0, ignore, (float)c.low,
+                   (float)c.high, (float)c.kl, (float)(1.0 / c.temperature), code_of(z), e.sms, e.stream),
+     "pf_policy_fwd");
+  return {loss, logps, kl, clipped};
+}
+struct DirectPolicy : torch::autograd::Function<DirectPolicy> {
+  static variable_list forward(AutogradContext* ctx, Tensor z, Tensor actions, Tensor old, Tensor adv, Maybe ref,
+                               double low, double high, double kl, double temperature, int64_t ignore) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    Tensor all;
+    const variable_list out = policy_forward(z, actions, old, adv, value(ref), {low, high, kl, temperature}, ignore, all);
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({out[1], out[2], out[3]});
+    ctx->save_for_backward({z, actions, all});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["inv"] = true;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return token_loss_backward(ctx, grads[0], 10);
   }
 };
 
@@ -1045,6 +1337,89 @@ PF_OP(cross_entropy) {
   END_HANDLE_TH_ERRORS
 }
 
+PF_OP(rotate_heads) {
+  HANDLE_TH_ERRORS
+  Args a(args, n, 5);
+  if (PyErr_Occurred()) return nullptr;
+  const Tensor x = a.tensor(0), cos = a.tensor(1), sin = a.tensor(2), pos = a.tensor(3, true);
+  const bool interleaved = a.boolean(4);
+  if (!a.fits || !all_plain(x, cos, sin, pos) || !head_view_fits(x, x.dim() == 5 ? 5 : 4) ||
+      !angles_fit(x, cos, sin, pos))
+    Py_RETURN_NONE;
+  if (!recorded(x, cos, sin))
+    return run(x, [&] { return unrecorded([&] { return rotate(x, cos, sin, pos, interleaved, false); }); });
+  return run(x, [&] { return DirectRotate::apply(x, cos, sin, maybe(pos), interleaved); });
+  END_HANDLE_TH_ERRORS
+}
+
+// queries and keys, or a projection and None
+PF_OP(norm_rotate_heads) {
+  HANDLE_TH_ERRORS
+  Args a(args, n, 9);
+  if (PyErr_Occurred()) return nullptr;
+  const Tensor q = a.tensor(0), k = a.tensor(1, true), wq = a.tensor(2), wk = a.tensor(3), cos = a.tensor(4),
+               sin = a.tensor(5), pos = a.tensor(6, true);
+  const double eps = a.real(7);
+  const bool interleaved = a.boolean(8);
+  if (!a.fits || !all_plain(q, k, wq, wk, cos, sin, pos) || !(k.defined() ? same_heads(q, k) : head_view_fits(q, 5)) ||
+      !gain_fits(wq, q) || !gain_fits(wk, q) || !angles_fit(q, cos, sin, pos))
+    Py_RETURN_NONE;
+  if (!recorded(q, k, wq, wk, cos, sin))
+    return run(q, [&] {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      return norm_rotate(q, k, wq, wk, cos, sin, pos, eps, interleaved);
+    });
+  return run(q, [&] { return DirectNormRotate::apply(q, maybe(k), wq, wk, cos, sin, maybe(pos), eps, interleaved); });
+  END_HANDLE_TH_ERRORS
+}
+
+PF_OP(preference_loss) {
+  HANDLE_TH_ERRORS
+  Args a(args, n, 6);
+  if (PyErr_Occurred()) return nullptr;
+  const Tensor z = a.tensor(0), labels = a.tensor(1), ref = a.tensor(2);
+  const double beta = a.real(3), smoothing = a.real(4);
+  const int64_t ignore = a.integer(5);
+  if (!a.fits || !all_plain(z, labels, ref) || !tokens_fit(z, labels) || z.size(0) % 2 || ref.dim() != 1 ||
+      !packed_floats(ref, z.size(0)) || ref.requires_grad() || !(smoothing >= 0.0 && smoothing <= 1.0))
+    Py_RETURN_NONE;
+  if (!recorded(z))
+    return run(z, [&] {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      Tensor all;
+      return preference_forward(z, labels, ref, beta, smoothing, ignore, all);
+    });
+  return run(z, [&] { return DirectPreference::apply(z, labels, ref, beta, smoothing, ignore); });
+  END_HANDLE_TH_ERRORS
+}
+
+PF_OP(policy_loss) {
+  HANDLE_TH_ERRORS
+  Args a(args, n, 10);
+  if (PyErr_Occurred()) return nullptr;
+  const Tensor z = a.tensor(0), actions = a.tensor(1), old = a.tensor(2), adv = a.tensor(3), ref = a.tensor(4, true);
+  const Clipping c{a.real(5), a.real(6), a.real(7), a.real(8)};
+  const int64_t ignore = a.integer(9);
+  if (!a.fits || !all_plain(z, actions, old, adv, ref) || !tokens_fit(z, actions)) Py_RETURN_NONE;
+  const int64_t N = z.size(0), T = z.size(1);
+  for (const Tensor* t : {&old, &ref})
+    if (t->defined() && (!packed_floats(*t, N * T) || t->dim() != 2 || t->size(0) != N || t->requires_grad()))
+      Py_RETURN_NONE;
+  if (!advantages_fit(adv, N, T) || adv.requires_grad() || !(c.temperature > 0.0) || !(c.low >= 0.0 && c.low <= 1.0) ||
+      !(c.high >= 0.0))
+    Py_RETURN_NONE;
+  if (!recorded(z))
+    return run(z, [&] {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      Tensor all;
+      return policy_forward(z, actions, old, adv, ref, c, ignore, all);
+    });
+  return run(z, [&] {
+    return DirectPolicy::apply(z, actions, old, adv, maybe(ref), c.low, c.high, c.kl, c.temperature, ignore);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
 PF_OP(group_norm) {
   HANDLE_TH_ERRORS
   Args a(args, n, 6);
@@ -1097,6 +1472,7 @@ PyObject* launches(PyObject*, PyObject*) { return PyLong_FromLongLong(g_launches
 PyMethodDef methods[] = {
     PF_ENTRY(linear), PF_ENTRY(mlp), PF_ENTRY(norm), PF_ENTRY(attention), PF_ENTRY(attention_qkv),
     PF_ENTRY(rope_qkv), PF_ENTRY(glu), PF_ENTRY(cross_entropy), PF_ENTRY(group_norm), PF_ENTRY(conv2d),
+    PF_ENTRY(rotate_heads), PF_ENTRY(norm_rotate_heads), PF_ENTRY(preference_loss), PF_ENTRY(policy_loss),
     PF_ENTRY(setup), {"launches", launches, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "pfeife_b200_eager", "eager calls of the ops", -1, methods,
                           nullptr, nullptr, nullptr, nullptr};

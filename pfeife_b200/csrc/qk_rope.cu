@@ -10,13 +10,12 @@
 // A head lies across a group of lanes, a power of two of them.  A lane owns slots of 2 VW values: in the pairs the
 // VW values from i and those they turn with, behind them 2 VW in a row, so that a rotation needs no other lane
 // and the norm one sum over the group.  Slot v turns by the frequencies VW v .. VW v + VW in both layouts: cosines
-// and sines are loaded once per item, which is up to HEADS heads of one token, and stay in registers.
+// and sines are loaded once per item, which is some heads of one token, and stay in registers.
 #include "common.cuh"
 #include "api.h"
 
 namespace pf {
 
-constexpr int HEADS = 4;           // heads of a token that a group has in flight
 constexpr int MAX_HEAD_DIM = 256;
 
 struct HeadsView {                 // [B, S, heads, D] in any order of memory with D innermost
@@ -38,7 +37,7 @@ struct HeadsArgs {
   long long pos_b, pos_s, rows;
   int S, D, R, lg, chunks, per_item, interleaved, inverse;
   unsigned tokens, items;
-  float eps;
+  float eps, inv_D;
 };
 
 template <int BYTES> struct Raw;
@@ -87,18 +86,31 @@ struct Slots {
     T* e1 = reinterpret_cast<T*>(&r[1]);
 #pragma unroll
     for (int j = 0; j < VW; ++j) { e0[j] = from_f32<T>(v[j]); e1[j] = from_f32<T>(v[VW + j]); }
+    put(y, n, r);
+  }
+  __device__ __forceinline__ void put(T* y, int n, const raw (&r)[2]) const {
     if (a[n] >= 0) *reinterpret_cast<raw*>(y + a[n]) = r[0];
     if (b[n] >= 0) *reinterpret_cast<raw*>(y + b[n]) = r[1];
   }
   // gain of the norm at the slots' values
   __device__ __forceinline__ void gains(const float* w, float (&v)[NS][N]) const {
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
+    for (int n = 0; n < NS; ++n) {
+      take(w, a[n], v[n], 0.f);
+      take(w, b[n], v[n] + VW, 0.f);
+    }
+  }
+  // VW floats, or `none` where at is negative
+  static __device__ __forceinline__ void take(const float* t, long long at, float* v, float none) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int at = j < VW ? a[n] : b[n];
-        v[n][j] = w && at >= 0 ? w[at + (j < VW ? j : j - VW)] : 1.f;
+    for (int j = 0; j < VW; j += (VW < 4 ? 1 : 4)) {
+      if constexpr (VW >= 4) {
+        const float4 q = at >= 0 ? __ldg(reinterpret_cast<const float4*>(t + at + j)) : make_float4(none, none, none, none);
+        v[j] = q.x; v[j + 1] = q.y; v[j + 2] = q.z; v[j + 3] = q.w;
+      } else {
+        v[j] = at >= 0 ? __ldg(t + at + j) : none;
       }
+    }
   }
   // Cosines and sines at a token's row of the tables; NaN for a row that they do not have, which no kernel can
   // refuse without the host waiting for it.
@@ -107,23 +119,10 @@ struct Slots {
     const bool there = row >= 0 && row < p.rows;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-      const long long at = row * (p.R / 2) + VW * (lane + (n << p.lg));
-#pragma unroll
-      for (int j = 0; j < VW; j += (VW < 4 ? 1 : 4)) {
-        if (!turns[n]) continue;
-        if constexpr (VW >= 4) {
-          float4 cv = make_float4(NAN, NAN, NAN, NAN), sv = cv;
-          if (there) {
-            cv = __ldg(reinterpret_cast<const float4*>(p.cos_t + at + j));
-            sv = __ldg(reinterpret_cast<const float4*>(p.sin_t + at + j));
-          }
-          c[n][j] = cv.x; c[n][j + 1] = cv.y; c[n][j + 2] = cv.z; c[n][j + 3] = cv.w;
-          s[n][j] = sv.x; s[n][j + 1] = sv.y; s[n][j + 2] = sv.z; s[n][j + 3] = sv.w;
-        } else {
-          c[n][j] = there ? __ldg(p.cos_t + at + j) : NAN;
-          s[n][j] = there ? __ldg(p.sin_t + at + j) : NAN;
-        }
-      }
+      if (!turns[n]) continue;
+      const long long at = there ? row * (p.R / 2) + VW * (lane + (n << p.lg)) : -1;
+      take(p.cos_t, at, c[n], NAN);
+      take(p.sin_t, at, s[n], NAN);
     }
   }
   // v turned by (c, s)
@@ -165,12 +164,18 @@ __device__ __forceinline__ T* head_at(const HeadsView& v, unsigned b, unsigned s
 }
 
 // x -> y.  The backward of a rotation without a norm is the same kernel with `inverse`.
+constexpr int FWD = 128;
+#ifndef XL
+#define XL 1536
+#endif
+constexpr long long FWD_LANES = XL;
 template <typename T, int VW, int NS, bool NORM>
-__global__ void __launch_bounds__(256) heads_fwd_kernel(const HeadsArgs p) {
+__global__ void __launch_bounds__(FWD, NORM ? 5 : 6) heads_fwd_kernel(const __grid_constant__ HeadsArgs p) {
+  constexpr int HEADS = NORM ? 4 : 2;                // heads that a group has in flight
   after_previous();
   using S = Slots<T, VW, NS>;
   const int lane = threadIdx.x & ((1 << p.lg) - 1);
-  const unsigned item = blockIdx.x * (256u >> p.lg) + (threadIdx.x >> p.lg);
+  const unsigned item = blockIdx.x * ((unsigned)FWD >> p.lg) + (threadIdx.x >> p.lg);
   const bool live = item < p.items;
   const unsigned token = live ? item / p.chunks : 0;
   int chunk = live ? item - token * p.chunks : 0, k = 0;
@@ -179,63 +184,78 @@ __global__ void __launch_bounds__(256) heads_fwd_kernel(const HeadsArgs p) {
   const unsigned b = token / p.S, s = token - b * p.S;
   const int h0 = chunk * p.per_item, heads = live ? min(p.per_item, part.heads - h0) : 0;
   const S slot(p, lane);
+  const T* x = head_at<const T>(part.x, b, s, h0);
+  T* y = head_at<T>(part.y, b, s, h0);
 
+  // the row's number, the heads and then what hangs on the number: two latencies in a row, not three
+  const long long row = part.turn ? table_row(p, b, s) : 0;
   typename S::raw raw[HEADS][NS][2];
 #pragma unroll
   for (int u = 0; u < HEADS; ++u)
-    if (u < heads) slot.load(head_at<const T>(part.x, b, s, h0 + u), raw[u]);
-  float c[NS][VW], sn[NS][VW];
+    if (u < heads) slot.load(x + u * part.x.h, raw[u]);
+  float c[NS][VW], sn[NS][VW], w[NS][S::N];
   if (part.turn) {
-    slot.angles(p, table_row(p, b, s), lane, c, sn);
+    slot.angles(p, row, lane, c, sn);
     if (p.inverse)
 #pragma unroll
       for (int n = 0; n < NS; ++n)
 #pragma unroll
         for (int j = 0; j < VW; ++j) sn[n][j] = -sn[n][j];
+    if constexpr (NORM) slot.gains(part.w, w);
   }
-  float w[NS][S::N], r[HEADS];
-  if constexpr (NORM) {
-    slot.gains(part.w, w);
+  for (int u0 = 0;;) {
+    float r[HEADS];
+    if constexpr (NORM) {
 #pragma unroll
-    for (int u = 0; u < HEADS; ++u) {
-      r[u] = 0.f;
-      if (u < heads)
+      for (int u = 0; u < HEADS; ++u) {
+        r[u] = 0.f;
+        if (u0 + u < heads)
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+            float v[S::N];
+            S::widen(raw[u][n], v);
+#pragma unroll
+            for (int j = 0; j < S::N; ++j) r[u] += v[j] * v[j];
+          }
+      }
+      group_sum(r, p.lg);
+#pragma unroll
+      for (int u = 0; u < HEADS; ++u) r[u] = rsqrtf(r[u] * p.inv_D + p.eps);
+    }
+#pragma unroll
+    for (int u = 0; u < HEADS; ++u)
+      if (u0 + u < heads)
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
+          if (!part.turn) {                          // the values of a projection
+            slot.put(y + u * part.y.h, n, raw[u][n]);
+            continue;
+          }
           float v[S::N];
           S::widen(raw[u][n], v);
+          if constexpr (NORM)
 #pragma unroll
-          for (int j = 0; j < S::N; ++j) r[u] += v[j] * v[j];
+            for (int j = 0; j < S::N; ++j) v[j] *= r[u] * w[n][j];
+          if (slot.turns[n]) S::turn(p.interleaved, c[n], sn[n], v);
+          slot.store(y + u * part.y.h, n, v);
         }
-    }
-    group_sum(r, p.lg);
+    u0 += HEADS;
+    if (u0 >= p.per_item) return;                    // the same for all items
+    x += HEADS * part.x.h;
+    y += HEADS * part.y.h;
 #pragma unroll
-    for (int u = 0; u < HEADS; ++u) r[u] = part.w ? rsqrtf(r[u] / p.D + p.eps) : 1.f;
+    for (int u = 0; u < HEADS; ++u)
+      if (u0 + u < heads) slot.load(x + u * part.x.h, raw[u]);
   }
-#pragma unroll
-  for (int u = 0; u < HEADS; ++u)
-    if (u < heads) {
-      T* y = head_at<T>(part.y, b, s, h0 + u);
-#pragma unroll
-      for (int n = 0; n < NS; ++n) {
-        float v[S::N];
-        S::widen(raw[u][n], v);
-        if constexpr (NORM)
-#pragma unroll
-          for (int j = 0; j < S::N; ++j) v[j] *= r[u] * w[n][j];
-        if (part.turn && slot.turns[n]) S::turn(p.interleaved, c[n], sn[n], v);
-        slot.store(y, n, v);
-      }
-    }
 }
 
 // Gradients behind a norm.  A CTA stays with one part, its groups walk over that part's items, and a lane adds up
 // dw of its values in registers; the CTA leaves one row of sums, which heads_fold_kernel adds in order.
 template <typename T, int VW, int NS>
-__global__ void __launch_bounds__(256) heads_bwd_kernel(const HeadsArgs p) {
+__global__ void __launch_bounds__(256, 2) heads_bwd_kernel(const __grid_constant__ HeadsArgs p) {
   after_previous();
   using S = Slots<T, VW, NS>;
-  constexpr int N = S::N, U = HEADS / 2;            // two tensors in flight: half as many heads
+  constexpr int N = S::N, U = 2;                     // heads that a group has in flight
   __shared__ float sums[8][MAX_HEAD_DIM];
   const int lane = threadIdx.x & ((1 << p.lg) - 1), groups = 256 >> p.lg;
   int k = 0;
@@ -244,7 +264,7 @@ __global__ void __launch_bounds__(256) heads_bwd_kernel(const HeadsArgs p) {
   const unsigned cta = blockIdx.x - part.cta0, items = p.tokens * part.chunks, step = part.ctas * groups;
   const S slot(p, lane);
   float w[NS][N], dw[NS][N] = {};
-  slot.gains(part.w, w);
+  if (part.w) slot.gains(part.w, w);
   // whole warps stay in the loop together: the sums over a group are made by all lanes
   for (unsigned first = cta * groups; first < items; first += step) {
     const unsigned item = first + (threadIdx.x >> p.lg);
@@ -268,11 +288,7 @@ __global__ void __launch_bounds__(256) heads_bwd_kernel(const HeadsArgs p) {
           if (u0 + u < heads) {
             T* y = head_at<T>(part.y, b, s, h0 + u0 + u);
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-              float g[N];
-              S::widen(gr[u][n], g);
-              slot.store(y, n, g);
-            }
+            for (int n = 0; n < NS; ++n) slot.put(y, n, gr[u][n]);
           }
         continue;
       }
@@ -304,7 +320,7 @@ __global__ void __launch_bounds__(256) heads_bwd_kernel(const HeadsArgs p) {
       for (int u = 0; u < U; ++u)
         if (u0 + u < heads) {
           T* y = head_at<T>(part.y, b, s, h0 + u0 + u);
-          const float r = rsqrtf(sum[u] / p.D + p.eps), m = r * sum[U + u] / p.D;
+          const float r = rsqrtf(sum[u] * p.inv_D + p.eps), m = r * sum[U + u] * p.inv_D;
 #pragma unroll
           for (int n = 0; n < NS; ++n) {
             float x[N], g[N];
@@ -410,7 +426,7 @@ int prepare(HeadsArgs& p, int parts, const void* cos_t, const void* sin_t, const
   if (reinterpret_cast<uintptr_t>(cos_t) % 4 || reinterpret_cast<uintptr_t>(sin_t) % 4 ||
       reinterpret_cast<uintptr_t>(pos) % 8)
     return -2;
-  if (vw >= 4 && !on_vectors((const char*)cos_t, (const char*)sin_t)) vw = 2;
+  if (vw >= 4 && !on_vectors(p.part[0].w, p.part[parts > 1].w, (const float*)cos_t, (const float*)sin_t)) vw = 2;
   p.cos_t = (const float*)cos_t;
   p.sin_t = (const float*)sin_t;
   p.pos = (const long long*)pos;
@@ -420,24 +436,23 @@ int prepare(HeadsArgs& p, int parts, const void* cos_t, const void* sin_t, const
   p.S = S; p.D = D; p.R = R;
   p.interleaved = interleaved;
   p.eps = eps;
+  p.inv_D = 1.f / D;
   p.tokens = (unsigned)(B * S);
   const int slots = R / (2 * vw) + (D - R + 2 * vw - 1) / (2 * vw), each = vw >= 4 ? 1 : vw == 2 ? 2 : 4;
   p.lg = pow2_log((slots + each - 1) / each);
   return vw;
 }
 
-// Heads of an item: HEADS where the items still fill the SMs twice over, else one.
-void deal(HeadsArgs& p, int parts, int sms) {
-  for (p.per_item = HEADS;; p.per_item = 1) {
-    long long items = 0;
+// Heads of an item: as many as leave every SM `lanes` lanes with an item of their own.
+void deal(HeadsArgs& p, int parts, long long lanes) {
+  for (p.per_item = 16;; p.per_item /= 2) {
     p.chunks = 0;
     for (int k = 0; k < parts; ++k) {
       p.part[k].chunks = (p.part[k].heads + p.per_item - 1) / p.per_item;
       p.chunks += p.part[k].chunks;
     }
-    items = (long long)p.tokens * p.chunks;
-    p.items = (unsigned)items;
-    if (p.per_item == 1 || (items << p.lg) >= 2ll * 2048 * sms) return;
+    p.items = p.tokens * (unsigned)p.chunks;
+    if (p.per_item == 1 || ((long long)p.items << p.lg) >= lanes) return;
   }
 }
 
@@ -464,9 +479,9 @@ struct Forward {
   bool norm;
   cudaStream_t st;
   template <typename T, int VW, int NS> void operator()() {
-    const unsigned per = 256u >> p.lg, grid = (p.items + per - 1) / per;
-    if (norm) after(heads_fwd_kernel<T, VW, NS, true>, grid, 256, 0, st)(p);
-    else after(heads_fwd_kernel<T, VW, NS, false>, grid, 256, 0, st)(p);
+    const unsigned per = (unsigned)FWD >> p.lg, grid = (p.items + per - 1) / per;
+    if (norm) after(heads_fwd_kernel<T, VW, NS, true>, grid, FWD, 0, st)(p);
+    else after(heads_fwd_kernel<T, VW, NS, false>, grid, FWD, 0, st)(p);
   }
 };
 struct Backward {
@@ -503,7 +518,7 @@ PF_API int pf_heads_fwd(const void* q, const void* k, const void* v, void* yq, v
   if (vw < 0) return vw;
   p.inverse = inverse;
   if ((long long)B * S * (Hq + 2ll * Hk) > 0x7fffffffll) return -3;
-  deal(p, parts, sm_count);
+  deal(p, parts, FWD_LANES * sm_count);
   if (p.items == 0) return 0;
   const int code = by_width(dtype, vw, Forward{p, wq != nullptr, reinterpret_cast<cudaStream_t>(stream)});
   if (code) return code;
@@ -533,7 +548,7 @@ PF_API int pf_heads_bwd(const void* gq, const void* gk, const void* gv, const vo
   const int vw = prepare(p, parts, cos_t, sin_t, pos, spos, B, S, D, R, rows, interleaved, eps, dtype);
   if (vw < 0) return vw;
   if ((long long)B * S * (Hq + 2ll * Hk) > 0x7fffffffll) return -3;
-  deal(p, parts, sm_count);
+  deal(p, parts, 1024ll * sm_count);
   const int groups = 256 >> p.lg;
   int ctas = 0;
   float* left = (float*)scratch;

@@ -3,10 +3,14 @@
 //
 // Both take logits z [N, T, V] (any strides, V innermost) and a label for each row; a row whose label is the ignored
 // one or outside the vocabulary does not count: its logits are not read, and its gradient is zero.
-// The forward passes over a row once and keeps M and s = sum 2^(k z - M), k = log2(e) / temperature, M near the
-// largest k z: log p = ln 2 (k z_label - M - log2 s).  What follows is a few operations per row and is done in 64
-// bits, by one thread: a preference subtracts sums over thousands of tokens from one another, and a KL estimate
-// exp(d) - d - 1 loses d^2 / 2 next to 1.
+// The forward passes over a row once and keeps M and s = sum 2^(k z - M), k = log2(e) / temperature, M the largest
+// k z rounded up to an integer: log p = ln 2 (k z_label - M - log2 s).
+// A preference subtracts sums over thousands of tokens from one another, which show what is off by the same little
+// part in every row (rewards of sequences of 1024 tokens were 3e-5 off).  So parts of a row are joined between
+// integers, by powers of two, which are exact; and each lane has a fraction of its own between its reference and
+// the integer, since 16-bit logits lie on a grid on which the exponential's errors would be the same in every row.
+// What follows is a few operations per row, done in 64 bits by one thread: those differences, and a KL estimate
+// exp(d) - d - 1, which loses d^2 / 2 next to 1.
 // The backward passes over it again: dz = g (onehot - p) with p = 2^(k z - M) / s and g what the loss has for the
 // row's log-probability, so that only M, s and g are kept.
 #include "common.cuh"
@@ -15,6 +19,10 @@
 namespace pf {
 
 constexpr double LN2 = 0.693147180559945309417;
+// ex2.approx cuts its last bits off: it is low by this part of its value on average (over 2^20 arguments of one
+// binade), and so is s.  A single probability hides that in its rounding, a sum over a sequence does not.  The
+// backward divides such values by such sums, where it cancels.
+constexpr double EXP2_LOW = 5.06e-8;
 
 struct Logits {                    // z [N, T, V]
   const void* at;
@@ -38,7 +46,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// (M, s) of two parts of a row; a part without a finite element is (-inf, 0), or (-inf, NaN) when it holds a NaN,
+// (M, s) of two parts of a row, with integers M; a part without a finite element is (-inf, 0), or (-inf, NaN) when it holds a NaN,
 // which no maximum shows: the sums are always added, and -inf counts as 0 where it is subtracted.
 __device__ __forceinline__ void part_merge(float& m, float& s, float m2, float s2) {
   const float mm = fmaxf(m, m2), sub = mm == -INFINITY ? 0.f : mm;
@@ -104,7 +112,7 @@ row_fwd_kernel(const Logits z, float2* __restrict__ stats, const Row finish) {
   const T* x = static_cast<const T*>(z.at) + z.row(row);
   const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int head = min(z.V, mis ? VN - mis : 0), nvec = (z.V - head) / VN;
-  const float k = z.k;
+  const float k = z.k, fraction = (threadIdx.x & 31) * (1.f / 32);
   float m = -INFINITY, s = 0.f;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   for (int i0 = tid; i0 < nvec; i0 += U * THREADS) {
@@ -122,7 +130,7 @@ row_fwd_kernel(const Logits z, float2* __restrict__ stats, const Row finish) {
       }
     // a NaN does not move the maximum but reaches the sum below; parts that are -inf so far subtract 0, which
     // leaves their exponentials at zero
-    const float mm = fmaxf(m, lm * k), sub = mm == -INFINITY ? 0.f : mm;
+    const float mm = fmaxf(m, ceilf(lm * k) + fraction), sub = mm == -INFINITY ? 0.f : mm;
     if (mm > m) s *= exp2_fast(m - sub);
     float a = 0.f;
 #pragma unroll
@@ -138,9 +146,14 @@ row_fwd_kernel(const Logits z, float2* __restrict__ stats, const Row finish) {
   // the elements before the first and after the last vector (at most 2 (VN - 1))
   for (int i = tid; i < z.V - nvec * VN; i += THREADS) {
     const float v = to_f32<T>(x[i < head ? i : nvec * VN + i]);
-    const float mm = fmaxf(m, v * k), sub = mm == -INFINITY ? 0.f : mm;
+    const float mm = fmaxf(m, ceilf(v * k) + fraction), sub = mm == -INFINITY ? 0.f : mm;
     s = s * exp2_fast(m - sub) + exp2_fast(fmaf(v, k, -sub));
     m = mm;
+  }
+  if (m > -INFINITY) {
+    const float whole = ceilf(m);
+    s *= exp2f(m - whole);
+    m = whole;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
@@ -158,7 +171,7 @@ row_fwd_kernel(const Logits z, float2* __restrict__ stats, const Row finish) {
   }
   if (tid == 0) {
     stats[row] = make_float2(m, s);
-    const double lp = LN2 * ((double)to_f32<T>(x[label]) * (double)k - (double)m) - log((double)s);
+    const double lp = LN2 * ((double)to_f32<T>(x[label]) * (double)k - (double)m) - log((double)s) - EXP2_LOW;
     finish(z, row, true, lp);
   }
 }

@@ -1075,6 +1075,9 @@ def preference_loss(logits: Tensor, labels: Tensor, ref_logps: Tensor, beta: flo
     With l the sum of a sequence's log-probabilities and m = beta ((l - ref of the chosen) - (l - ref of the
     rejected)) the loss is the mean of -(1 - label_smoothing) log sig(m) - label_smoothing log sig(-m).
     Rows that do not count are not read and get a gradient of zero, whatever their logits."""
+    out = _native_call("preference_loss", logits, labels, ref_logps, float(beta), float(label_smoothing), ignore_index)
+    if out is not None:
+        return PreferenceLoss(*out)
     if isinstance(logits, Tensor):
         N = logits.shape[0] if logits.dim() == 3 else 0
         if N < 2 or N % 2 or logits.shape[2] < 1:
@@ -1148,6 +1151,10 @@ def policy_loss(logits: Tensor, actions: Tensor, old_logps: Tensor, advantages: 
     -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(ref - l) - (ref - l) - 1), the last with
     ``ref_logps`` [...] only; the loss is the mean over the tokens that count, 0 if there are none.
     Rows that do not count are not read and get a gradient of zero, whatever their logits."""
+    out = _native_call("policy_loss", logits, actions, old_logps, advantages, ref_logps, float(clip_low),
+                       float(clip_high), float(kl_coef), float(temperature), ignore_index)
+    if out is not None:
+        return PolicyLoss(*out)
     shape = actions.shape
     if isinstance(logits, Tensor):
         if logits.dim() < 2 or logits.shape[-1] < 1:
@@ -1279,6 +1286,9 @@ def rope(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None
     for it would wait for the device, and an IndexError on the CPU."""
     if positions is None and not interleaved:
         return _call(rope_apply, x, cos, sin, False)
+    y = _native_call("rotate_heads", x, cos, sin, positions, interleaved)
+    if y is not None:
+        return y
     _check_angles(x, cos, sin, positions)
     return _call(rope_at, x, cos, sin, positions, interleaved, False)
 
@@ -1316,6 +1326,9 @@ def rope_qkv(qkv: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] 
     if positions is None and not interleaved:
         y = _native_call("rope_qkv", qkv, cos, sin)
         return y if y is not None else _call(rope_qkv_apply, qkv, cos, sin, False)
+    y = _native_call("rotate_heads", qkv, cos, sin, positions, interleaved)
+    if y is not None:
+        return y
     _check_angles(qkv, cos, sin, positions)
     return _call(rope_qkv_at, qkv, cos, sin, positions, interleaved, False)
 
@@ -1581,6 +1594,9 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos: 
                  ) -> Tuple[Tensor, Tensor]:
     """RMS norm of each head of q [B, S, Hq, D] and k [B, S, Hk, D] with the gains q_weight and k_weight [D], then
     ``rope`` of both, in one pass.  q and k may be slices of a projection."""
+    out = _native_layer("norm_rotate_heads", q, k, q_weight, k_weight, cos, sin, positions, float(eps), interleaved)
+    if out is not None:
+        return out
     if isinstance(q, Tensor) and isinstance(k, Tensor) and (
             q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] \
             or q.dtype != k.dtype or q.device != k.device):
@@ -1642,6 +1658,9 @@ _autograd(qk_norm_rope_qkv_fwd, 1, _qk_norm_rope_qkv_backward, setup=_qk_norm_ro
 def qk_norm_rope_qkv(qkv: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tensor, sin: Tensor, eps: float = 1e-6,
                      positions: Optional[Tensor] = None, interleaved: bool = False) -> Tensor:
     """``qk_norm_rope`` of the queries and keys of a fused projection [B, S, 3, H, D], for ``attention_qkv``."""
+    y = _native_layer("norm_rotate_heads", qkv, None, q_weight, k_weight, cos, sin, positions, float(eps), interleaved)
+    if y is not None:
+        return y
     if isinstance(qkv, Tensor) and (qkv.dim() != 5 or qkv.shape[2] != 3):
         raise ValueError(f"a projection [B, S, 3, H, D] is needed, not {tuple(qkv.shape)}")
     _check_angles(qkv, cos, sin, positions)
