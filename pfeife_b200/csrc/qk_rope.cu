@@ -7,16 +7,17 @@
 // rotation), xh = x r:  dx = r (g w - xh mean(g w xh)),  dw = sum over tokens and heads of g xh.
 // r is computed again in the backward, which reads x anyway.
 //
-// A head lies across a group of lanes, a power of two of them.  A lane owns slots of 2 VW values: in the pairs the
-// VW values from i and those they turn with, behind them 2 VW in a row, so that a rotation needs no other lane
-// and the norm one sum over the group.  Slot v turns by the frequencies VW v .. VW v + VW in both layouts: cosines
-// and sines are loaded once per item, which is some heads of one token, and stay in registers.
+// A head lies across a group of lanes, a power of two of them.  A lane owns slots of two halves of VW values, VW i
+// and VW i + R/2 on in the pairs, so that a rotation needs no other lane and the norm one sum over the group.
+// Cosines and sines are loaded once per token and stay in registers, as does the gain.
 #include "common.cuh"
 #include "api.h"
 
 namespace pf {
 
 constexpr int MAX_HEAD_DIM = 256;
+constexpr int BACK_CTAS = 2;         // of the backward behind a norm, that an SM holds
+constexpr int RING_BYTES = 196608;   // of an SM's shared memory, through which heads come
 
 struct HeadsView {                 // [B, S, heads, D] in any order of memory with D innermost
   char* at;
@@ -25,18 +26,17 @@ struct HeadsView {                 // [B, S, heads, D] in any order of memory wi
 struct HeadsPart {
   HeadsView x, y, g;               // forward: x -> y; backward: x and the gradient g -> y
   const float* w;                  // gain of the norm, or null
-  float* dw;                       // backward: [ctas][D] partial sums
-  int heads, chunks;               // chunks: items of a token
-  int turn;                        // 0: the values of a projection, which are copied
-  int cta0, ctas;                  // backward: the CTAs of this part
+  float* dw;                       // backward: partial sums, one row [D] for each CTA of the call
+  int heads, turn;                 // turn 0: the values of a projection, which are copied
+  int cta0, ctas, per;             // the CTAs of this part, and the heads that a group of lanes takes
 };
 struct HeadsArgs {
   HeadsPart part[3];
   const float *cos_t, *sin_t;      // [rows, R/2]
   const long long* pos;            // row of the tables for each token, or null: the token's place
   long long pos_b, pos_s, rows;
-  int S, D, R, lg, chunks, per_item, interleaved, inverse;
-  unsigned tokens, items;
+  int S, D, R, lg;
+  unsigned tokens;
   float eps, inv_D;
 };
 
@@ -46,24 +46,43 @@ template <> struct Raw<8> { using type = uint2; };
 template <> struct Raw<4> { using type = uint32_t; };
 template <> struct Raw<2> { using type = unsigned short; };
 
-// Where a lane's slots lie in a head, and by how much they turn.
-template <typename T, int VW, int NS>
+// two values of a pair of registers, rounded to 16 bits in one operation
+template <typename T> __device__ __forceinline__ void narrow2(T* to, float a, float b) { to[0] = a; to[1] = b; }
+template <> __device__ __forceinline__ void narrow2(__half* to, float a, float b) {
+  *reinterpret_cast<__half2*>(to) = __floats2half2_rn(a, b);
+}
+template <> __device__ __forceinline__ void narrow2(__nv_bfloat16* to, float a, float b) {
+  *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(a, b);
+}
+
+// Where a lane's slots lie in a head, and by how much they turn.  In registers the values of a slot are VW pairs
+// (x, y) that turn together, x and y each packed two by two, whatever their order in memory.
+template <typename T, int VW, int NS, bool INTER>
 struct Slots {
-  static constexpr int N = 2 * VW;
+  static constexpr int P = (VW + 1) / 2;             // packed registers of the x and of the y of a slot
+  struct Values { uint64_t x[P], y[P]; };
   using raw = typename Raw<VW * sizeof(T)>::type;
   int a[NS], b[NS];                // first values of both halves, -1 where there is none
+  int f[NS], g[NS];                // first frequencies of both halves of the cosines
   bool turns[NS];
 
+  // Both halves lie apart even where pairs lie side by side or do not turn, so that the lanes of a group read and
+  // write whole sectors together (32 bytes a lane, 16 at a time: 41 us for 26, [1, 32768, 8, 128] interleaved).
   __device__ __forceinline__ Slots(const HeadsArgs& p, int lane) {
-    const int pairs = p.R / N;
+    const int pairs = p.R / (2 * VW), apart = ((p.D - p.R) / VW + 1) / 2;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-      const int v = lane + (n << p.lg);
+      const int v = lane + (n << p.lg), w = v - pairs;
       turns[n] = v < pairs;
-      a[n] = turns[n] ? (p.interleaved ? N * v : VW * v) : p.R + N * (v - pairs);
-      b[n] = turns[n] && !p.interleaved ? a[n] + p.R / 2 : a[n] + VW;
-      if (a[n] >= p.D) a[n] = -1;
-      if (b[n] >= p.D || a[n] < 0) b[n] = -1;
+      constexpr bool single = VW == 1 && INTER;       // a half is no pair
+      a[n] = !turns[n] ? p.R + VW * w : single ? 2 * v : VW * v;
+      b[n] = !turns[n] ? a[n] + VW * apart : single ? 2 * v + 1 : VW * v + p.R / 2;
+      f[n] = INTER && !single ? VW / 2 * v : VW * v;
+      g[n] = INTER ? p.R / 4 + VW / 2 * v : VW * v + VW / 2;
+      if (!turns[n]) {
+        if (w >= apart) a[n] = b[n] = -1;
+        if (b[n] >= p.D) b[n] = -1;
+      }
     }
   }
   __device__ __forceinline__ void load(const T* x, raw (&r)[NS][2]) const {
@@ -74,78 +93,119 @@ struct Slots {
       if (b[n] >= 0) r[n][1] = *reinterpret_cast<const raw*>(x + b[n]);
     }
   }
-  static __device__ __forceinline__ void widen(const raw (&r)[2], float (&v)[N]) {
-    const T* e0 = reinterpret_cast<const T*>(&r[0]);
-    const T* e1 = reinterpret_cast<const T*>(&r[1]);
+  // the pairs of two halves: (a, b) of equal places, or neighbours
+  template <typename E>
+  static __device__ __forceinline__ Values pairs_of(const E* a, const E* b) {
+    float x[2 * P] = {}, y[2 * P] = {};
 #pragma unroll
-    for (int j = 0; j < VW; ++j) { v[j] = to_f32<T>(e0[j]); v[VW + j] = to_f32<T>(e1[j]); }
+    for (int j = 0; j < VW; ++j) {
+      const E* h = j < VW / 2 ? a : b;
+      const int at = j < VW / 2 ? 2 * j : 2 * j - VW;
+      x[j] = to_f32<E>(INTER && VW > 1 ? h[at] : a[j]);
+      y[j] = to_f32<E>(INTER && VW > 1 ? h[at + 1] : b[j]);
+    }
+    Values v;
+#pragma unroll
+    for (int j = 0; j < P; ++j) { v.x[j] = f2_pack(x[2 * j], x[2 * j + 1]); v.y[j] = f2_pack(y[2 * j], y[2 * j + 1]); }
+    return v;
   }
-  __device__ __forceinline__ void store(T* y, int n, const float (&v)[N]) const {
-    raw r[2];
-    T* e0 = reinterpret_cast<T*>(&r[0]);
-    T* e1 = reinterpret_cast<T*>(&r[1]);
+  static __device__ __forceinline__ Values widen(const raw (&r)[2]) {
+    return pairs_of(reinterpret_cast<const T*>(&r[0]), reinterpret_cast<const T*>(&r[1]));
+  }
+  __device__ __forceinline__ void store(T* to, int n, const Values& v) const {
+    float x[2 * P], y[2 * P];
 #pragma unroll
-    for (int j = 0; j < VW; ++j) { e0[j] = from_f32<T>(v[j]); e1[j] = from_f32<T>(v[VW + j]); }
-    put(y, n, r);
+    for (int j = 0; j < P; ++j) { f2_unpack(v.x[j], x[2 * j], x[2 * j + 1]); f2_unpack(v.y[j], y[2 * j], y[2 * j + 1]); }
+    raw r[2];
+    T* a = reinterpret_cast<T*>(&r[0]);
+    T* b = reinterpret_cast<T*>(&r[1]);
+    if constexpr (VW == 1) {
+      *a = from_f32<T>(x[0]);
+      *b = from_f32<T>(y[0]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VW; j += 2) {
+        if constexpr (INTER) {
+          narrow2(a + j, x[j / 2], y[j / 2]);
+          narrow2(b + j, x[VW / 2 + j / 2], y[VW / 2 + j / 2]);
+        } else {
+          narrow2(a + j, x[j], x[j + 1]);
+          narrow2(b + j, y[j], y[j + 1]);
+        }
+      }
+    }
+    put(to, n, r);
   }
   __device__ __forceinline__ void put(T* y, int n, const raw (&r)[2]) const {
     if (a[n] >= 0) *reinterpret_cast<raw*>(y + a[n]) = r[0];
     if (b[n] >= 0) *reinterpret_cast<raw*>(y + b[n]) = r[1];
   }
   // gain of the norm at the slots' values
-  __device__ __forceinline__ void gains(const float* w, float (&v)[NS][N]) const {
+  __device__ __forceinline__ void gains(const float* w, Values (&v)[NS]) const {
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-      take(w, a[n], v[n], 0.f);
-      take(w, b[n], v[n] + VW, 0.f);
+      float first[VW], second[VW];
+      take<VW>(w, a[n], first, 0.f);
+      take<VW>(w, b[n], second, 0.f);
+      v[n] = pairs_of(first, second);
     }
   }
-  // VW floats, or `none` where at is negative
+  // K floats, or `none` where at is negative
+  template <int K>
   static __device__ __forceinline__ void take(const float* t, long long at, float* v, float none) {
+    if constexpr (K % 4 == 0) {
 #pragma unroll
-    for (int j = 0; j < VW; j += (VW < 4 ? 1 : 4)) {
-      if constexpr (VW >= 4) {
+      for (int j = 0; j < K; j += 4) {
         const float4 q = at >= 0 ? __ldg(reinterpret_cast<const float4*>(t + at + j)) : make_float4(none, none, none, none);
         v[j] = q.x; v[j + 1] = q.y; v[j + 2] = q.z; v[j + 3] = q.w;
-      } else {
-        v[j] = at >= 0 ? __ldg(t + at + j) : none;
       }
+    } else if constexpr (VW >= 4) {
+      const float2 q = at >= 0 ? __ldg(reinterpret_cast<const float2*>(t + at)) : make_float2(none, none);
+      v[0] = q.x; v[1] = q.y;
+    } else {
+#pragma unroll
+      for (int j = 0; j < K; ++j) v[j] = at >= 0 ? __ldg(t + at + j) : none;
     }
   }
   // Cosines and sines at a token's row of the tables; NaN for a row that they do not have, which no kernel can
   // refuse without the host waiting for it.
-  __device__ __forceinline__ void angles(const HeadsArgs& p, long long row, int lane, float (&c)[NS][VW],
-                                         float (&s)[NS][VW]) const {
+  struct Angles { float c[2 * P], s[2 * P]; };
+  __device__ __forceinline__ void angles(const HeadsArgs& p, long long row, Angles (&to)[NS]) const {
     const bool there = row >= 0 && row < p.rows;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
       if (!turns[n]) continue;
-      const long long at = there ? row * (p.R / 2) + VW * (lane + (n << p.lg)) : -1;
-      take(p.cos_t, at, c[n], NAN);
-      take(p.sin_t, at, s[n], NAN);
+      const long long at = row * (p.R / 2), first = there ? at + f[n] : -1, second = there ? at + g[n] : -1;
+      constexpr int K = VW > 1 ? VW / 2 : 1;
+      take<K>(p.cos_t, first, to[n].c, NAN);
+      take<K>(p.sin_t, first, to[n].s, NAN);
+      if constexpr (VW > 1) {
+        take<K>(p.cos_t, second, to[n].c + K, NAN);
+        take<K>(p.sin_t, second, to[n].s + K, NAN);
+      }
     }
   }
-  // v turned by (c, s)
-  static __device__ __forceinline__ void turn(bool interleaved, const float (&c)[VW], const float (&s)[VW],
-                                              float (&v)[N]) {
-    float t[N];
-    if (interleaved) {
+  // (x, y) -> (x c - y s, y c + x s), or with -s; the subtraction is not packed: packed operations do not negate
+  template <bool INVERSE>
+  static __device__ __forceinline__ void turn(const Angles& by, Values& v) {
 #pragma unroll
-      for (int j = 0; j < VW; ++j) {
-        t[2 * j] = v[2 * j] * c[j] - v[2 * j + 1] * s[j];
-        t[2 * j + 1] = v[2 * j + 1] * c[j] + v[2 * j] * s[j];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < VW; ++j) {
-        t[j] = v[j] * c[j] - v[VW + j] * s[j];
-        t[VW + j] = v[VW + j] * c[j] + v[j] * s[j];
-      }
+    for (int j = 0; j < P; ++j) {
+      const uint64_t c = f2_pack(by.c[2 * j], by.c[2 * j + 1]), s = f2_pack(by.s[2 * j], by.s[2 * j + 1]);
+      const uint64_t x = v.x[j], y = v.y[j], plus = fma2(INVERSE ? y : x, s, mul2(INVERSE ? x : y, c));
+      float a0, a1, o0, o1;
+      f2_unpack(mul2(INVERSE ? y : x, c), a0, a1);
+      f2_unpack(INVERSE ? x : y, o0, o1);
+      const uint64_t minus = f2_pack(fmaf(-o0, by.s[2 * j], a0), fmaf(-o1, by.s[2 * j + 1], a1));
+      v.x[j] = INVERSE ? plus : minus;
+      v.y[j] = INVERSE ? minus : plus;
     }
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = t[j];
   }
 };
+__device__ __forceinline__ float halves(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
 
 // sums of U values over the group of a lane; every lane of the warp calls it
 template <int U>
@@ -155,214 +215,266 @@ __device__ __forceinline__ void group_sum(float (&v)[U], int lg) {
     for (int u = 0; u < U; ++u) v[u] += __shfl_xor_sync(0xffffffffu, v[u], o);
 }
 
+// Where a group is in its walk over the heads of a part, token by token, and their place in one tensor.
+struct Walk {
+  unsigned b, s;
+  int h;
+  long long at;
+  __device__ __forceinline__ Walk(const HeadsArgs& p, const HeadsPart& part, const HeadsView& v, unsigned first) {
+    const unsigned token = first / part.heads;
+    h = first - token * part.heads;
+    b = token / p.S;
+    s = token - b * p.S;
+    at = place(v) + h * v.h;
+  }
+  __device__ __forceinline__ long long place(const HeadsView& v) const {
+    return (long long)b * v.b + (long long)s * v.s;
+  }
+  __device__ __forceinline__ bool next(const HeadsArgs& p, const HeadsPart& part, const HeadsView& v) {
+    at += v.h;
+    if (++h < part.heads) return false;
+    h = 0;
+    if (++s == (unsigned)p.S) { s = 0; ++b; }
+    at = place(v);
+    return true;                                     // the next token
+  }
+};
+// row of the tables for a token; that of one behind the last is never used
 __device__ __forceinline__ long long table_row(const HeadsArgs& p, unsigned b, unsigned s) {
+  if (b * p.S + s >= p.tokens) return -1;
   return p.pos ? __ldg(p.pos + b * p.pos_b + s * p.pos_s) : (long long)s;
 }
-template <typename T>
-__device__ __forceinline__ T* head_at(const HeadsView& v, unsigned b, unsigned s, int h) {
-  return reinterpret_cast<T*>(v.at) + (long long)b * v.b + (long long)s * v.s + (long long)h * v.h;
+
+template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const void* from) {
+  if constexpr (BYTES == 16) cp_async16(to, from);
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(from), "n"(BYTES) : "memory");
 }
 
-// x -> y.  The backward of a rotation without a norm is the same kernel with `inverse`.
-constexpr int FWD = 128;
-#ifndef XL
-#define XL 1536
-#endif
-constexpr long long FWD_LANES = XL;
-template <typename T, int VW, int NS, bool NORM>
-__global__ void __launch_bounds__(FWD, NORM ? 5 : 6) heads_fwd_kernel(const __grid_constant__ HeadsArgs p) {
-  constexpr int HEADS = NORM ? 4 : 2;                // heads that a group has in flight
-  after_previous();
-  using S = Slots<T, VW, NS>;
+enum { ROTATE, UNROTATE, NORM, NORM_BACK };                    // what a call does
+
+// What a thread has on its way through shared memory: its own vectors of the next STAGES heads, in which no other
+// thread has a part, so that it waits for its own copies only.
+template <typename T, int VW, int NS, int MODE>
+struct HeadsRing {
+  static constexpr bool BACK = MODE == NORM_BACK;
+  // CTAs that an SM holds, by registers
+  static constexpr int CTAS = BACK ? BACK_CTAS : (MODE == NORM ? 3 : 4) - (VW == 1);
+  static constexpr int TENSORS = BACK ? 2 : 1, VEC = VW * (int)sizeof(T);
+  static constexpr bool ASYNC = VEC >= 4;            // no copy moves 2 bytes
+  static constexpr int STAGE = 256 * TENSORS * NS * 2 * VEC;
+  static constexpr int FIT = RING_BYTES / CTAS / STAGE, STAGES = ASYNC ? (FIT > 12 ? 12 : FIT) : 1;
+  static constexpr int BYTES = STAGES * STAGE > 8 * MAX_HEAD_DIM * 4 ? STAGES * STAGE : 8 * MAX_HEAD_DIM * 4;
+};
+
+// ROTATE and NORM: x -> y; UNROTATE is the backward of a rotation alone.  NORM_BACK: x and the gradient g of the
+// result -> y and the sums for dw, one row a CTA, which heads_fold_kernel adds in order.
+// A CTA stays with one part.  Its groups take `per` heads each, one after the other, token by token: the parts of a
+// call and the heads of a part need not divide anything, and no group has more than one head above another.
+template <typename T, int VW, int NS, int MODE, bool INTER>
+__global__ void __launch_bounds__(256, HeadsRing<T, VW, NS, MODE>::CTAS)
+heads_kernel(const __grid_constant__ HeadsArgs p) {
+  using S = Slots<T, VW, NS, INTER>;
+  using R = HeadsRing<T, VW, NS, MODE>;
+  using raw = typename S::raw;
+  constexpr int P = S::P, STEP = 256 * R::TENSORS * NS * 2;  // raws of a stage
+  constexpr bool BACK = MODE == NORM_BACK;
+  extern __shared__ __align__(16) char heads_smem[];
+  raw* ring = reinterpret_cast<raw*>(heads_smem) + threadIdx.x;
+  auto place = [&](int stage, int tensor, int n, int side) -> raw* {
+    return ring + stage * STEP + ((tensor * NS + n) * 2 + side) * 256;
+  };
   const int lane = threadIdx.x & ((1 << p.lg) - 1);
-  const unsigned item = blockIdx.x * ((unsigned)FWD >> p.lg) + (threadIdx.x >> p.lg);
-  const bool live = item < p.items;
-  const unsigned token = live ? item / p.chunks : 0;
-  int chunk = live ? item - token * p.chunks : 0, k = 0;
-  while (chunk >= p.part[k].chunks) chunk -= p.part[k++].chunks;
-  const HeadsPart& part = p.part[k];
-  const unsigned b = token / p.S, s = token - b * p.S;
-  const int h0 = chunk * p.per_item, heads = live ? min(p.per_item, part.heads - h0) : 0;
-  const S slot(p, lane);
-  const T* x = head_at<const T>(part.x, b, s, h0);
-  T* y = head_at<T>(part.y, b, s, h0);
-
-  // the row's number, the heads and then what hangs on the number: two latencies in a row, not three
-  const long long row = part.turn ? table_row(p, b, s) : 0;
-  typename S::raw raw[HEADS][NS][2];
-#pragma unroll
-  for (int u = 0; u < HEADS; ++u)
-    if (u < heads) slot.load(x + u * part.x.h, raw[u]);
-  float c[NS][VW], sn[NS][VW], w[NS][S::N];
-  if (part.turn) {
-    slot.angles(p, row, lane, c, sn);
-    if (p.inverse)
-#pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int j = 0; j < VW; ++j) sn[n][j] = -sn[n][j];
-    if constexpr (NORM) slot.gains(part.w, w);
-  }
-  for (int u0 = 0;;) {
-    float r[HEADS];
-    if constexpr (NORM) {
-#pragma unroll
-      for (int u = 0; u < HEADS; ++u) {
-        r[u] = 0.f;
-        if (u0 + u < heads)
-#pragma unroll
-          for (int n = 0; n < NS; ++n) {
-            float v[S::N];
-            S::widen(raw[u][n], v);
-#pragma unroll
-            for (int j = 0; j < S::N; ++j) r[u] += v[j] * v[j];
-          }
-      }
-      group_sum(r, p.lg);
-#pragma unroll
-      for (int u = 0; u < HEADS; ++u) r[u] = rsqrtf(r[u] * p.inv_D + p.eps);
-    }
-#pragma unroll
-    for (int u = 0; u < HEADS; ++u)
-      if (u0 + u < heads)
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          if (!part.turn) {                          // the values of a projection
-            slot.put(y + u * part.y.h, n, raw[u][n]);
-            continue;
-          }
-          float v[S::N];
-          S::widen(raw[u][n], v);
-          if constexpr (NORM)
-#pragma unroll
-            for (int j = 0; j < S::N; ++j) v[j] *= r[u] * w[n][j];
-          if (slot.turns[n]) S::turn(p.interleaved, c[n], sn[n], v);
-          slot.store(y + u * part.y.h, n, v);
-        }
-    u0 += HEADS;
-    if (u0 >= p.per_item) return;                    // the same for all items
-    x += HEADS * part.x.h;
-    y += HEADS * part.y.h;
-#pragma unroll
-    for (int u = 0; u < HEADS; ++u)
-      if (u0 + u < heads) slot.load(x + u * part.x.h, raw[u]);
-  }
-}
-
-// Gradients behind a norm.  A CTA stays with one part, its groups walk over that part's items, and a lane adds up
-// dw of its values in registers; the CTA leaves one row of sums, which heads_fold_kernel adds in order.
-template <typename T, int VW, int NS>
-__global__ void __launch_bounds__(256, 2) heads_bwd_kernel(const __grid_constant__ HeadsArgs p) {
-  after_previous();
-  using S = Slots<T, VW, NS>;
-  constexpr int N = S::N, U = 2;                     // heads that a group has in flight
-  __shared__ float sums[8][MAX_HEAD_DIM];
-  const int lane = threadIdx.x & ((1 << p.lg) - 1), groups = 256 >> p.lg;
   int k = 0;
   while (blockIdx.x >= (unsigned)(p.part[k].cta0 + p.part[k].ctas)) ++k;
   const HeadsPart& part = p.part[k];
-  const unsigned cta = blockIdx.x - part.cta0, items = p.tokens * part.chunks, step = part.ctas * groups;
+  const unsigned group = (blockIdx.x - part.cta0) * (256u >> p.lg) + (threadIdx.x >> p.lg);
+  const unsigned all = p.tokens * (unsigned)part.heads;
+  const unsigned first = (unsigned)min((unsigned long long)group * part.per, (unsigned long long)all);
+  const int mine = min(all - first, (unsigned)part.per);       // part.per steps are made by all, for the sums' sake
   const S slot(p, lane);
-  float w[NS][N], dw[NS][N] = {};
-  if (part.w) slot.gains(part.w, w);
-  // whole warps stay in the loop together: the sums over a group are made by all lanes
-  for (unsigned first = cta * groups; first < items; first += step) {
-    const unsigned item = first + (threadIdx.x >> p.lg);
-    const bool live = item < items;
-    const unsigned token = live ? item / part.chunks : 0, chunk = live ? item - token * part.chunks : 0;
-    const unsigned b = token / p.S, s = token - b * p.S;
-    const int h0 = chunk * p.per_item, heads = live ? min(p.per_item, part.heads - h0) : 0;
-    float c[NS][VW], sn[NS][VW];
-    if (part.turn) slot.angles(p, table_row(p, b, s), lane, c, sn);
-    for (int u0 = 0; u0 < p.per_item; u0 += U) {
-      typename S::raw xr[U][NS][2], gr[U][NS][2];
+  after_previous();
+
+  Walk in(p, part, BACK ? part.g : part.x, first), x_in(p, part, part.x, first), out(p, part, part.y, first);
+  int filled = 0;                                    // the stage that the next fetch fills
+  raw now[R::TENSORS][NS][2] = {}, then[R::TENSORS][NS][2] = {};
+  auto fetch = [&](int step) {                       // one head of the walk, if the group still has it
+    if (step < mine) {
+      const T* from[2] = {reinterpret_cast<const T*>((BACK ? part.g : part.x).at) + in.at,
+                          BACK ? reinterpret_cast<const T*>(part.x.at) + x_in.at : nullptr};
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u0 + u < heads) {
-          slot.load(head_at<const T>(part.g, b, s, h0 + u0 + u), gr[u]);
-          if (part.w) slot.load(head_at<const T>(part.x, b, s, h0 + u0 + u), xr[u]);
-        }
-      if (!part.w) {                                 // the values of a projection
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (u0 + u < heads) {
-            T* y = head_at<T>(part.y, b, s, h0 + u0 + u);
-#pragma unroll
-            for (int n = 0; n < NS; ++n) slot.put(y, n, gr[u][n]);
-          }
-        continue;
-      }
-      float sum[2 * U];                              // of x^2, then of g w x
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        sum[u] = sum[U + u] = 0.f;
-        if (u0 + u < heads)
+      for (int q = 0; q < R::TENSORS; ++q) {
+        if (BACK && q == 1 && !part.turn) continue;  // the values of a projection: only their gradient is read
+        if constexpr (R::ASYNC) {
 #pragma unroll
           for (int n = 0; n < NS; ++n) {
-            float x[N], g[N];
-            S::widen(xr[u][n], x);
-            S::widen(gr[u][n], g);
-            if (slot.turns[n]) {
-              float back[VW];
-#pragma unroll
-              for (int j = 0; j < VW; ++j) back[j] = -sn[n][j];
-              S::turn(p.interleaved, c[n], back, g);
-            }
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-              sum[u] += x[j] * x[j];
-              sum[U + u] += g[j] * w[n][j] * x[j];
-            }
+            if (slot.a[n] >= 0) copy_async<R::VEC>(place(filled, q, n, 0), from[q] + slot.a[n]);
+            if (slot.b[n] >= 0) copy_async<R::VEC>(place(filled, q, n, 1), from[q] + slot.b[n]);
           }
+        } else {
+          slot.load(from[q], then[q]);
+        }
       }
+      in.next(p, part, BACK ? part.g : part.x);
+      if (BACK) x_in.next(p, part, part.x);
+    }
+    if constexpr (R::ASYNC) {
+      cp_async_commit();
+      filled = filled + 1 < R::STAGES ? filled + 1 : 0;
+    }
+  };
+  if constexpr (R::ASYNC) {
+    for (int i = 0; i < R::STAGES - 1; ++i) fetch(i);
+  } else {
+    fetch(0);
+  }
+
+  typename S::Angles by[NS] = {};
+  typename S::Values w[NS] = {}, dw[NS] = {};
+  unsigned nb = out.b, ns = out.s;                   // the token whose row of the tables is on its way
+  long long row = -1;
+  auto next_angles = [&] {
+    slot.angles(p, row, by);
+    if (++ns == (unsigned)p.S) { ns = 0; ++nb; }
+    row = table_row(p, nb, ns);
+  };
+  if (part.turn && mine > 0) {
+    row = table_row(p, nb, ns);
+    next_angles();
+    if constexpr (MODE == NORM || BACK) slot.gains(part.w, w);
+  }
+
+  int stage = 0;
+  for (int step = 0; step < part.per; ++step) {
+    if constexpr (R::ASYNC) {
+      cp_async_wait<R::STAGES - 2>();
+#pragma unroll
+      for (int q = 0; q < R::TENSORS; ++q)
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          now[q][n][0] = now[q][n][1] = raw{};
+          if (step < mine && slot.a[n] >= 0) now[q][n][0] = *place(stage, q, n, 0);
+          if (step < mine && slot.b[n] >= 0) now[q][n][1] = *place(stage, q, n, 1);
+        }
+      stage = stage + 1 < R::STAGES ? stage + 1 : 0;
+      fetch(step + R::STAGES - 1);                   // into the place that the step before this one has read
+    } else {
+#pragma unroll
+      for (int q = 0; q < R::TENSORS; ++q)
+#pragma unroll
+        for (int n = 0; n < NS; ++n) { now[q][n][0] = then[q][n][0]; now[q][n][1] = then[q][n][1]; }
+      fetch(step + 1);
+    }
+    T* y = reinterpret_cast<T*>(part.y.at) + out.at;
+    if (!part.turn) {                                // the values of a projection
+      if (step < mine) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) slot.put(y, n, now[0][n]);
+        out.next(p, part, part.y);
+      }
+      continue;
+    }
+    typename S::Values v[NS];                        // BACK: the gradient, turned back
+    if constexpr (!BACK) {
+      uint64_t squares = 0;                          // two zeros
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        v[n] = S::widen(now[0][n]);
+        if constexpr (MODE == NORM)
+#pragma unroll
+          for (int j = 0; j < P; ++j) {
+            squares = fma2(v[n].x[j], v[n].x[j], squares);
+            squares = fma2(v[n].y[j], v[n].y[j], squares);
+            v[n].x[j] = mul2(v[n].x[j], w[n].x[j]);
+            v[n].y[j] = mul2(v[n].y[j], w[n].y[j]);
+          }
+        if (slot.turns[n]) S::template turn<MODE == UNROTATE>(by[n], v[n]);
+      }
+      if constexpr (MODE == NORM) {                  // what hangs on the sum comes last
+        float sum[1] = {halves(squares)};
+        group_sum(sum, p.lg);
+        const float r = rsqrtf(sum[0] * p.inv_D + p.eps);
+        const uint64_t r2 = f2_pack(r, r);
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+          for (int j = 0; j < P; ++j) { v[n].x[j] = mul2(v[n].x[j], r2); v[n].y[j] = mul2(v[n].y[j], r2); }
+      }
+    } else {
+      uint64_t squares = 0, dots = 0;
+      typename S::Values x[NS];
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        v[n] = S::widen(now[0][n]);
+        if (slot.turns[n]) S::template turn<true>(by[n], v[n]);
+        x[n] = S::widen(now[1][n]);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          squares = fma2(x[n].x[j], x[n].x[j], squares);
+          squares = fma2(x[n].y[j], x[n].y[j], squares);
+          dots = fma2(mul2(v[n].x[j], w[n].x[j]), x[n].x[j], dots);
+          dots = fma2(mul2(v[n].y[j], w[n].y[j]), x[n].y[j], dots);
+        }
+      }
+      float sum[2] = {halves(squares), halves(dots)};
       group_sum(sum, p.lg);
+      // r (g w - xh m) with xh = x r and m = mean(g w xh) is (g w) r + x (-r^3 mean(g w x))
+      const float r = rsqrtf(sum[0] * p.inv_D + p.eps), m = -(r * (r * (r * (sum[1] * p.inv_D))));
+      const uint64_t r2 = f2_pack(r, r), m2 = f2_pack(m, m);
+      if (step < mine)
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u0 + u < heads) {
-          T* y = head_at<T>(part.y, b, s, h0 + u0 + u);
-          const float r = rsqrtf(sum[u] * p.inv_D + p.eps), m = r * sum[U + u] * p.inv_D;
+        for (int n = 0; n < NS; ++n)
 #pragma unroll
-          for (int n = 0; n < NS; ++n) {
-            float x[N], g[N];
-            S::widen(xr[u][n], x);
-            S::widen(gr[u][n], g);
-            if (slot.turns[n]) {
-              float back[VW];
-#pragma unroll
-              for (int j = 0; j < VW; ++j) back[j] = -sn[n][j];
-              S::turn(p.interleaved, c[n], back, g);
-            }
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-              const float xh = x[j] * r;
-              dw[n][j] += g[j] * xh;
-              x[j] = r * (g[j] * w[n][j] - xh * m);
-            }
-            slot.store(y, n, x);
+          for (int j = 0; j < P; ++j) {
+            const uint64_t gx = mul2(v[n].x[j], r2), gy = mul2(v[n].y[j], r2);
+            dw[n].x[j] = fma2(gx, x[n].x[j], dw[n].x[j]);
+            dw[n].y[j] = fma2(gy, x[n].y[j], dw[n].y[j]);
+            v[n].x[j] = fma2(x[n].x[j], m2, mul2(gx, w[n].x[j]));
+            v[n].y[j] = fma2(x[n].y[j], m2, mul2(gy, w[n].y[j]));
           }
-        }
+    }
+    if (step < mine) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n) slot.store(y, n, v[n]);
+      if (out.next(p, part, part.y)) next_angles();
     }
   }
-  if (!part.dw) return;                              // the same for the whole CTA
+
+  if constexpr (BACK) {
+    if (!part.dw) return;                            // the same for the whole CTA
+    float(*sums)[MAX_HEAD_DIM] = reinterpret_cast<float(*)[MAX_HEAD_DIM]>(heads_smem);
+    if constexpr (R::ASYNC) cp_async_wait<0>();
+    __syncthreads();                                 // nobody's copies are still on their way into the ring
 #pragma unroll
-  for (int n = 0; n < NS; ++n)
+    for (int n = 0; n < NS; ++n) {
+      float x[2 * P], y[2 * P];
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      for (int o = 1 << p.lg; o < 32; o <<= 1) dw[n][j] += __shfl_xor_sync(0xffffffffu, dw[n][j], o);
-  if ((threadIdx.x & 31) < (1 << p.lg))
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int at = j < VW ? slot.a[n] : slot.b[n];
-        if (at >= 0) sums[threadIdx.x >> 5][at + (j < VW ? j : j - VW)] = dw[n][j];
+      for (int j = 0; j < P; ++j) {
+        f2_unpack(dw[n].x[j], x[2 * j], x[2 * j + 1]);
+        f2_unpack(dw[n].y[j], y[2 * j], y[2 * j + 1]);
       }
-  __syncthreads();
-  if (threadIdx.x < p.D) {
-    float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t += sums[i][threadIdx.x];
-    part.dw[(long long)cta * p.D + threadIdx.x] = t;
+      for (int j = 0; j < VW; ++j) {
+        for (int o = 1 << p.lg; o < 32; o <<= 1) {
+          x[j] += __shfl_xor_sync(0xffffffffu, x[j], o);
+          y[j] += __shfl_xor_sync(0xffffffffu, y[j], o);
+        }
+        constexpr bool beside = INTER && VW > 1;     // as in pairs_of
+        const int half = j < VW / 2 ? slot.a[n] : slot.b[n], at = j < VW / 2 ? 2 * j : 2 * j - VW;
+        const int x_at = beside ? half + at : slot.a[n] + j, y_at = beside ? half + at + 1 : slot.b[n] + j;
+        if ((threadIdx.x & 31) < (1 << p.lg)) {
+          if ((beside ? half : slot.a[n]) >= 0) sums[threadIdx.x >> 5][x_at] = x[j];
+          if ((beside ? half : slot.b[n]) >= 0) sums[threadIdx.x >> 5][y_at] = y[j];
+        }
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < p.D) {
+      float t = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t += sums[i][threadIdx.x];
+      part.dw[(long long)blockIdx.x * p.D + threadIdx.x] = t;
+    }
   }
 }
 
@@ -407,8 +519,8 @@ int pow2_log(int n) { int l = 0; while ((1 << l) < n) ++l; return l; }
 
 // Fills in what a call's parts have in common and returns the values VW of a slot's halves, or a refusal.
 int prepare(HeadsArgs& p, int parts, const void* cos_t, const void* sin_t, const void* pos,
-            const long long* pos_strides, long long B, int S, int D, int R, long long rows, int interleaved,
-            float eps, int dtype) {
+            const long long* pos_strides, long long B, int S, int D, int R, long long rows, float eps,
+            int dtype) {
   if (dtype != PF_F32 && dtype != PF_F16 && dtype != PF_BF16) return -1;
   if (D < 1 || D > MAX_HEAD_DIM || R < 2 || R > D || R % 2) return -3;
   if (B * S > 0x7fffffffll) return -3;
@@ -434,7 +546,6 @@ int prepare(HeadsArgs& p, int parts, const void* cos_t, const void* sin_t, const
   p.pos_s = pos ? pos_strides[1] : 0;
   p.rows = rows;
   p.S = S; p.D = D; p.R = R;
-  p.interleaved = interleaved;
   p.eps = eps;
   p.inv_D = 1.f / D;
   p.tokens = (unsigned)(B * S);
@@ -443,17 +554,24 @@ int prepare(HeadsArgs& p, int parts, const void* cos_t, const void* sin_t, const
   return vw;
 }
 
-// Heads of an item: as many as leave every SM `lanes` lanes with an item of their own.
-void deal(HeadsArgs& p, int parts, long long lanes) {
-  for (p.per_item = 16;; p.per_item /= 2) {
-    p.chunks = 0;
-    for (int k = 0; k < parts; ++k) {
-      p.part[k].chunks = (p.part[k].heads + p.per_item - 1) / p.per_item;
-      p.chunks += p.part[k].chunks;
-    }
-    p.items = p.tokens * (unsigned)p.chunks;
-    if (p.per_item == 1 || ((long long)p.items << p.lg) >= lanes) return;
+// CTAs and heads of their groups for each part: `most` CTAs altogether, shared by the bytes that the parts move,
+// and no more than a part has heads for.  Returns the number of CTAs.
+int deal(HeadsArgs& p, int parts, int most, const int* weight) {
+  const int groups = 256 >> p.lg;
+  long long total = 0;
+  for (int k = 0; k < parts; ++k) total += (long long)weight[k] * p.part[k].heads;
+  int ctas = 0;
+  for (int k = 0; k < parts; ++k) {
+    HeadsPart& part = p.part[k];
+    const long long all = (long long)p.tokens * part.heads;
+    long long share = total ? (long long)most * weight[k] * part.heads / total : 0;
+    if (share < 1) share = 1;
+    part.per = (int)((all + share * groups - 1) / (share * groups));
+    part.ctas = part.per ? (int)((all + (long long)part.per * groups - 1) / ((long long)part.per * groups)) : 0;
+    part.cta0 = ctas;
+    ctas += part.ctas;
   }
+  return ctas;
 }
 
 HeadsView view(const void* at, const long long* strides) {
@@ -462,7 +580,7 @@ HeadsView view(const void* at, const long long* strides) {
 
 // calls f<T, VW, NS>()
 template <typename F>
-int by_width(int dtype, int vw, F&& f) {
+int by_width(int dtype, int vw, F& f) {
 #define PF_W(T, W, NSLOTS) \
   if (vw == W) { f.template operator()<T, W, NSLOTS>(); return 0; }
   if (dtype == PF_F32) { PF_W(float, 4, 1) PF_W(float, 2, 2) PF_W(float, 1, 4) }
@@ -474,32 +592,39 @@ int by_width(int dtype, int vw, F&& f) {
   return -1;
 }
 
-struct Forward {
-  const HeadsArgs& p;
-  bool norm;
+template <int MODE>
+struct Launch {
+  HeadsArgs& p;
+  int parts, interleaved, sms;
+  const int* weight;
   cudaStream_t st;
+  int code = 0;
   template <typename T, int VW, int NS> void operator()() {
-    const unsigned per = (unsigned)FWD >> p.lg, grid = (p.items + per - 1) / per;
-    if (norm) after(heads_fwd_kernel<T, VW, NS, true>, grid, FWD, 0, st)(p);
-    else after(heads_fwd_kernel<T, VW, NS, false>, grid, FWD, 0, st)(p);
+    if (interleaved) go<T, VW, NS, true>();
+    else go<T, VW, NS, false>();
+  }
+  template <typename T, int VW, int NS, bool INTER> void go() {
+    using R = HeadsRing<T, VW, NS, MODE>;
+    const int ctas = deal(p, parts, R::CTAS * sms, weight);
+    if (ctas == 0) return;
+    static bool done[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (R::BYTES > 48 * 1024 && (dev < 0 || dev >= 64 || !done[dev])) {
+      const cudaError_t e = cudaFuncSetAttribute(heads_kernel<T, VW, NS, MODE, INTER>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, R::BYTES);
+      if (e != cudaSuccess) { code = (int)e; return; }
+      if (dev >= 0 && dev < 64) done[dev] = true;
+    }
+    after(heads_kernel<T, VW, NS, MODE, INTER>, ctas, 256, R::BYTES, st)(p);
   }
 };
-struct Backward {
-  const HeadsArgs& p;
-  int ctas;
-  cudaStream_t st;
-  template <typename T, int VW, int NS> void operator()() {
-    after(heads_bwd_kernel<T, VW, NS>, ctas, 256, 0, st)(p);
-  }
-};
-
-// CTAs of the backward's parts, by their heads: together two per SM of the caller's count, no more than a part
-// has items for.
-int bwd_ctas(int heads, int all_heads, int sms) {
-  const long long n = all_heads > 0 ? 2ll * sms * heads / all_heads : 0;
-  return n < 1 ? 1 : (int)n;
+template <int MODE>
+int launch(HeadsArgs& p, int parts, const int* weight, int interleaved, int dtype, int vw, int sms, void* stream) {
+  Launch<MODE> f{p, parts, interleaved, sms, weight, reinterpret_cast<cudaStream_t>(stream)};
+  const int code = by_width(dtype, vw, f);
+  return code ? code : f.code;
 }
-
 }  // namespace
 
 // x: q [B, S, Hq, D], k [B, S, Hk, D] (null: none), v (null: none; strides of k, copied) -> yq, yk, yv.  wq / wk fp32
@@ -511,25 +636,23 @@ PF_API int pf_heads_fwd(const void* q, const void* k, const void* v, void* yq, v
                         int interleaved, int inverse, float eps, int dtype, int sm_count, void* stream) {
   HeadsArgs p = {};
   int parts = 0;
-  p.part[parts++] = {view(q, sq), view(yq, syq), {}, (const float*)wq, nullptr, Hq, 0, 1, 0, 0};
-  if (k) p.part[parts++] = {view(k, sk), view(yk, syk), {}, (const float*)wk, nullptr, Hk, 0, 1, 0, 0};
+  p.part[parts++] = {view(q, sq), view(yq, syq), {}, (const float*)wq, nullptr, Hq, 1, 0, 0, 0};
+  if (k) p.part[parts++] = {view(k, sk), view(yk, syk), {}, (const float*)wk, nullptr, Hk, 1, 0, 0, 0};
   if (v) p.part[parts++] = {view(v, sk), view(yv, syk), {}, nullptr, nullptr, Hk, 0, 0, 0, 0};
-  const int vw = prepare(p, parts, cos_t, sin_t, pos, spos, B, S, D, R, rows, interleaved, eps, dtype);
+  const int vw = prepare(p, parts, cos_t, sin_t, pos, spos, B, S, D, R, rows, eps, dtype);
   if (vw < 0) return vw;
-  p.inverse = inverse;
   if ((long long)B * S * (Hq + 2ll * Hk) > 0x7fffffffll) return -3;
-  deal(p, parts, FWD_LANES * sm_count);
-  if (p.items == 0) return 0;
-  const int code = by_width(dtype, vw, Forward{p, wq != nullptr, reinterpret_cast<cudaStream_t>(stream)});
+  const int even[3] = {1, 1, 1};
+  const int code = wq ? launch<NORM>(p, parts, even, interleaved, dtype, vw, sm_count, stream)
+                   : inverse ? launch<UNROTATE>(p, parts, even, interleaved, dtype, vw, sm_count, stream)
+                             : launch<ROTATE>(p, parts, even, interleaved, dtype, vw, sm_count, stream);
   if (code) return code;
   PF_CHECK_LAUNCH();
   return 0;
 }
 
-// Rows of partial sums that pf_heads_bwd needs: floats [that many][D].
-PF_API int pf_heads_bwd_rows(int Hq, int Hk, int sm_count) {
-  return bwd_ctas(Hq, Hq + Hk, sm_count) + bwd_ctas(Hk, Hq + Hk, sm_count);
-}
+// Rows of partial sums that pf_heads_bwd needs: floats [that many][D].  No part gets less than one CTA.
+PF_API int pf_heads_bwd_rows(int Hq, int Hk, int sm_count) { return BACK_CTAS * sm_count + 2; }
 
 // Gradients of pf_heads_fwd with a norm: gq, gk, gv (the outputs') -> dq, dk, dv and dwq, dwk fp32 [D] (null: not
 // needed; accumulate: added to what is there).  gv null: there are no values.
@@ -542,35 +665,23 @@ PF_API int pf_heads_bwd(const void* gq, const void* gk, const void* gv, const vo
                         void* stream) {
   HeadsArgs p = {};
   int parts = 0;
-  p.part[parts++] = {view(q, sq), view(dq, sdq), view(gq, sgq), (const float*)wq, nullptr, Hq, 0, 1, 0, 0};
-  p.part[parts++] = {view(k, sk), view(dk, sdk), view(gk, sgk), (const float*)wk, nullptr, Hk, 0, 1, 0, 0};
+  p.part[parts++] = {view(q, sq), view(dq, sdq), view(gq, sgq), (const float*)wq, nullptr, Hq, 1, 0, 0, 0};
+  p.part[parts++] = {view(k, sk), view(dk, sdk), view(gk, sgk), (const float*)wk, nullptr, Hk, 1, 0, 0, 0};
   if (gv) p.part[parts++] = {{}, view(dv, sdk), view(gv, sgk), nullptr, nullptr, Hk, 0, 0, 0, 0};
-  const int vw = prepare(p, parts, cos_t, sin_t, pos, spos, B, S, D, R, rows, interleaved, eps, dtype);
+  const int vw = prepare(p, parts, cos_t, sin_t, pos, spos, B, S, D, R, rows, eps, dtype);
   if (vw < 0) return vw;
   if ((long long)B * S * (Hq + 2ll * Hk) > 0x7fffffffll) return -3;
-  deal(p, parts, 1024ll * sm_count);
-  const int groups = 256 >> p.lg;
-  int ctas = 0;
-  float* left = (float*)scratch;
-  for (int i = 0; i < parts; ++i) {
-    HeadsPart& part = p.part[i];
-    const long long items = (long long)p.tokens * part.chunks, most = (items + groups - 1) / groups;
-    part.ctas = i < 2 ? bwd_ctas(part.heads, Hq + Hk, sm_count) : sm_count;
-    if (part.ctas > most) part.ctas = (int)most;
-    part.cta0 = ctas;
-    ctas += part.ctas;
-    if (i < 2 && (i ? dwk : dwq)) part.dw = left;
-    if (i < 2) left += (long long)part.ctas * D;
-  }
+  // the sums' rows lie where the parts' CTAs do, at most BACK_CTAS an SM and one more for each of two parts
+  const int weight[3] = {3, 3, 2};
+  if (dwq) p.part[0].dw = (float*)scratch;
+  if (dwk) p.part[1].dw = (float*)scratch;
+  const int code = launch<NORM_BACK>(p, parts, weight, interleaved, dtype, vw, sm_count, stream);
+  if (code) return code;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (ctas) {
-    const int code = by_width(dtype, vw, Backward{p, ctas, st});
-    if (code) return code;
-  }
   if (dwq || dwk)
     after(heads_fold_kernel, dim3((D + 31) / 32, 2), 256, 0, st)(
-        (const float*)p.part[0].dw, (const float*)p.part[1].dw, (float*)dwq, (float*)dwk, p.part[0].ctas,
-        p.part[1].ctas, D, accumulate);
+        (const float*)scratch, (const float*)scratch + (long long)p.part[1].cta0 * D, (float*)dwq, (float*)dwk,
+        p.part[0].ctas, p.part[1].ctas, D, accumulate);
   PF_CHECK_LAUNCH();
   return 0;
 }
