@@ -846,6 +846,11 @@ bool tokens_fit(const Tensor& z, const Tensor& labels) {
          z.size(1) < (1ll << 31) && labels.scalar_type() == at::kLong && labels.dim() == 2 && labels.is_contiguous() &&
          labels.size(0) == z.size(0) && labels.size(1) == z.size(1);
 }
+Tensor loss_scratch(const Tensor& like, int64_t N, int64_t T) {
+  const int n = pf_token_loss_scratch(N, (int)T);
+  if (n < 0) throw Failed{n, "pf_token_loss_scratch"};
+  return empty({n}, at::kDouble, like);
+}
 float* float_at(const Tensor& t, int64_t i) { return static_cast<float*>(t.data_ptr()) + i; }
 
 // What the backward of both needs lies in one buffer: two statistics a row, then `n` factors (one for each sequence or
@@ -899,7 +904,7 @@ variable_list preference_forward(const Tensor& z, const Tensor& labels, const Te
   const int64_t N = z.size(0), T = z.size(1);
   const Kept kept{floats(2 * N * T + N, z), N * T, N, false};
   all = kept.all;
-  const Tensor loss = empty({}, at::kFloat, z), rewards = floats(N, z), scratch = empty({N * T + N}, at::kDouble, z);
+  const Tensor loss = empty({}, at::kFloat, z), rewards = floats(N, z), scratch = loss_scratch(z, N, T);
   ok(pf_preference_fwd(z.data_ptr(), labels.data_ptr(), ref.data_ptr(), loss.data_ptr(), rewards.data_ptr(),
                        kept.stats(), kept.coef(), scratch.data_ptr(), N, (int)T, (int)z.size(2), z.stride(0),
                        z.stride(1), ignore, (float)beta, (float)smoothing, code_of(z), e.sms, e.stream),
@@ -938,7 +943,7 @@ variable_list policy_forward(const Tensor& z, const Tensor& actions, const Tenso
   const Kept kept{floats(3 * rows + 1, z), rows, rows, true};
   all = kept.all;
   const Tensor loss = empty({}, at::kFloat, z), logps = empty({N, T}, at::kFloat, z), kl = empty({}, at::kFloat, z),
-               clipped = empty({}, at::kFloat, z), scratch = floats(4 * rows, z);
+               clipped = empty({}, at::kFloat, z), scratch = loss_scratch(z, N, T);
   ok(pf_policy_fwd(z.data_ptr(), actions.data_ptr(), old.data_ptr(), at_or_null(ref), adv.data_ptr(), loss.data_ptr(),
                    kl.data_ptr(), clipped.data_ptr(), kept.one_over(), logps.data_ptr(), kept.coef(), kept.stats(),
                    scratch.data_ptr(), N, (int)T, (int)z.size(2), z.stride(0), z.stride(1),

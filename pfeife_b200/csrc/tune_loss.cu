@@ -19,10 +19,10 @@
 namespace pf {
 
 constexpr double LN2 = 0.693147180559945309417;
-// ex2.approx cuts its last bits off: it is low by this part of its value on average (over 2^20 arguments of one
-// binade), and so is s.  A single probability hides that in its rounding, a sum over a sequence does not.  The
-// backward divides such values by such sums, where it cancels.
-constexpr double EXP2_LOW = 5.06e-8;
+// ex2.approx cuts its last bits off, and s is low by this part of its value on average (over 2048 rows of 32000
+// normal logits, bf16 and fp32 alike; a row's own s is off by 4e-8 around that).  A single probability hides it in
+// its rounding, a sum over a sequence does not.  The backward divides such values by such sums, where it cancels.
+constexpr double EXP2_LOW = 3.7e-8;
 
 struct Logits {                    // z [N, T, V]
   const void* at;
@@ -46,6 +46,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// 2^(i/32 - 1), which a lane's sum is multiplied by to get from its reference to the integer (exp2f would be as
+// low as ex2.approx is); lane 0 has an integer
+__constant__ float FRACTION_SCALE[32] = {
+    1.000000000f, 0.510948574f, 0.522136891f, 0.533570200f, 0.545253866f, 0.557193371f, 0.569394317f, 0.581862429f,
+    0.594603558f, 0.607623680f, 0.620928906f, 0.634525479f, 0.648419777f, 0.662618322f, 0.677127773f, 0.691954941f,
+    0.707106781f, 0.722590403f, 0.738413073f, 0.754582214f, 0.771105413f, 0.787990423f, 0.805245166f, 0.822877739f,
+    0.840896415f, 0.859309649f, 0.878126080f, 0.897354538f, 0.917004043f, 0.937083817f, 0.957603281f, 0.978572062f};
+
 // (M, s) of two parts of a row, with integers M; a part without a finite element is (-inf, 0), or (-inf, NaN) when it holds a NaN,
 // which no maximum shows: the sums are always added, and -inf counts as 0 where it is subtracted.
 __device__ __forceinline__ void part_merge(float& m, float& s, float m2, float s2) {
@@ -54,94 +62,120 @@ __device__ __forceinline__ void part_merge(float& m, float& s, float m2, float s
   m = mm;
 }
 
-// What a loss makes of a row, in 64 bits.
-struct PolicyRow {
-  const float *old, *ref, *adv;    // ref null: no reference
-  long long adv_n, adv_t;          // strides of the advantages
-  float low, high, kl;
-  double inv_temperature;
-  float *logp, *coef;              // coef: of the row's own term, before the mean
-  float4* terms;                   // (term, KL, clipped, counted)
-  __device__ __forceinline__ void operator()(const Logits& z, long long r, bool counted, double lp) const {
-    if (!counted) {
-      logp[r] = coef[r] = 0.f;
-      terms[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-      return;
-    }
-    const long long n = r / z.T;
-    const double a = adv[n * adv_n + (r - n * z.T) * adv_t], ratio = exp(lp - (double)old[r]);
-    const double lo = 1.0 - (double)low, hi = 1.0 + (double)high;
-    const double free = ratio * a, held = fmin(fmax(ratio, lo), hi) * a;
-    const bool clipped = free > held;
-    double term = clipped ? -held : -free, c = clipped ? 0.0 : -free, each = 0.0;
-    if (ref) {
-      const double d = (double)ref[r] - lp, e = expm1(d);
-      each = e - d;
-      term += kl * each;
-      c -= kl * e;
-    }
-    logp[r] = (float)lp;
-    coef[r] = (float)(c * inv_temperature);
-    terms[r] = make_float4((float)term, (float)each, clipped ? 1.f : 0.f, 1.f);
+// 16 bytes of a row: its largest value, and its values two by two in fp32.  16-bit maxima are taken two at a time
+// before anything is widened, as fp32 sums and products are: ten instructions a value became six.  What is left are
+// the loads: without its exponentials, 16 a cycle and SM, the pass takes 38 us for 41 (2797 of 4096 rows of 32000
+// bf16; 27 at the copy rate).  More in flight does not help: batches of 8 vectors, the next one in registers or
+// several in shared memory take 42, 42 and 54.
+template <typename T> struct Words;
+template <> struct Words<float> {
+  static constexpr int PAIRS = 2;
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  template <int U> static __device__ __forceinline__ float most(const uint4 (&q)[U]) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(q[u].x), __uint_as_float(q[u].y))),
+                fmaxf(__uint_as_float(q[u].z), __uint_as_float(q[u].w)));
+    return m;
+  }
+  static __device__ __forceinline__ uint64_t pair(const uint4& q, int j) {
+    return j ? f2_pack(__uint_as_float(q.z), __uint_as_float(q.w)) : f2_pack(__uint_as_float(q.x), __uint_as_float(q.y));
   }
 };
-struct PreferenceRow {
-  double* logp;
-  __device__ __forceinline__ void operator()(const Logits&, long long r, bool counted, double lp) const {
-    logp[r] = counted ? lp : 0.0;
+template <typename T2> __device__ __forceinline__ T2 word_of(const uint4& q, int j) {
+  const uint32_t w = j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w;
+  return *reinterpret_cast<const T2*>(&w);
+}
+template <typename T2, int U> __device__ __forceinline__ T2 most_words(const uint4 (&q)[U]) {
+  T2 m = word_of<T2>(q[0], 0);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = __hmax2(m, word_of<T2>(q[u], j));      // the other one of a NaN
+  return m;
+}
+template <> struct Words<__half> {
+  static constexpr int PAIRS = 4;
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+  template <int U> static __device__ __forceinline__ float most(const uint4 (&q)[U]) {
+    const float2 m = __half22float2(most_words<__half2>(q));
+    return fmaxf(m.x, m.y);
+  }
+  static __device__ __forceinline__ uint64_t pair(const uint4& q, int j) {
+    const float2 v = __half22float2(word_of<__half2>(q, j));
+    return f2_pack(v.x, v.y);
+  }
+};
+template <> struct Words<__nv_bfloat16> {
+  static constexpr int PAIRS = 4;
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+  template <int U> static __device__ __forceinline__ float most(const uint4 (&q)[U]) {
+    const float2 m = __bfloat1622float2(most_words<__nv_bfloat162>(q));
+    return fmaxf(m.x, m.y);
+  }
+  static __device__ __forceinline__ uint64_t pair(const uint4& q, int j) {
+    const uint32_t w = word_of<uint32_t>(q, j);
+    return f2_pack(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
 };
 
-// One pass over each row that counts.  THREADS threads a row: whole CTAs, or warps that share a CTA of 256.
-template <typename T, int THREADS, typename Row>
-__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
-row_fwd_kernel(const Logits z, float2* __restrict__ stats, const Row finish) {
+constexpr int ROW_BATCH = 4;       // vectors that a thread takes at a time
+constexpr int ROW_THREADS = 128;   // of most rows, and twelve such rows an SM
+
+// One pass over each row that counts: M and s to stats, the label's logit to `at_label`.  THREADS threads a row:
+// CTAs of their own, or warps that share one of 256.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS < 64 ? 256 : THREADS, THREADS == ROW_THREADS ? 12 : 1)
+row_fwd_kernel(const Logits z, float2* __restrict__ stats, float* __restrict__ at_label) {
   after_previous();
-  constexpr int W = THREADS / 32, VN = 16 / sizeof(T), U = 4;
-  constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
-  static_assert(ROWS == 1 || W == 1, "rows that share a CTA are a warp each");
+  constexpr int W = THREADS / 32, VN = 16 / sizeof(T), U = ROW_BATCH;
+  constexpr int ROWS = W > 1 ? 1 : 8;
   __shared__ float smax[W], ssum[W];
-  const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / THREADS;
+  const long long row = (long long)blockIdx.x * ROWS + (W > 1 ? 0 : threadIdx.x / 32);
   if (row >= z.rows) return;
   const int tid = threadIdx.x % THREADS;
   const long long label = z.labels[row];
-  if (!z.counts(label)) {
-    if (tid == 0) finish(z, row, false, 0.0);
-    return;
-  }
+  if (!z.counts(label)) return;
   const T* x = static_cast<const T*>(z.at) + z.row(row);
+  const float mine = tid == 0 ? to_f32<T>(x[label]) : 0.f;
   const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int head = min(z.V, mis ? VN - mis : 0), nvec = (z.V - head) / VN;
   const float k = z.k, fraction = (threadIdx.x & 31) * (1.f / 32);
   float m = -INFINITY, s = 0.f;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
-  for (int i0 = tid; i0 < nvec; i0 += U * THREADS) {
-    uint4 q[U];
+  const uint64_t k2 = f2_pack(k, k);
+  auto take = [&](uint4 (&q)[U], int i0) {           // -inf behind the row's end, which adds nothing
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      q[u] = Words<T>::none();
       if (i0 + u * THREADS < nvec) q[u] = __ldg(xv + i0 + u * THREADS);
-    float lm = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i0 + u * THREADS < nvec) {
-        const T* e = reinterpret_cast<const T*>(&q[u]);
-#pragma unroll
-        for (int j = 0; j < VN; ++j) lm = fmaxf(lm, to_f32<T>(e[j]));
-      }
+    }
+  };
+  auto add = [&](const uint4 (&q)[U]) {
     // a NaN does not move the maximum but reaches the sum below; parts that are -inf so far subtract 0, which
     // leaves their exponentials at zero
-    const float mm = fmaxf(m, ceilf(lm * k) + fraction), sub = mm == -INFINITY ? 0.f : mm;
+    const float mm = fmaxf(m, ceilf(Words<T>::most(q) * k) + fraction), sub = mm == -INFINITY ? 0.f : mm;
     if (mm > m) s *= exp2_fast(m - sub);
-    float a = 0.f;
+    const uint64_t minus2 = f2_pack(-sub, -sub);
+    uint64_t sums[2] = {0, 0};                       // two zeros each
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (i0 + u * THREADS < nvec) {
-        const T* e = reinterpret_cast<const T*>(&q[u]);
 #pragma unroll
-        for (int j = 0; j < VN; ++j) a += exp2_fast(fmaf(to_f32<T>(e[j]), k, -sub));
+      for (int j = 0; j < Words<T>::PAIRS; ++j) {
+        float a, b;
+        f2_unpack(fma2(Words<T>::pair(q[u], j), k2, minus2), a, b);
+        sums[j & 1] = add2(sums[j & 1], f2_pack(exp2_fast(a), exp2_fast(b)));
       }
-    s += a;
+    float a, b;
+    f2_unpack(add2(sums[0], sums[1]), a, b);
+    s += a + b;
     m = mm;
+  };
+  uint4 q[U];
+  for (int i0 = tid; i0 < nvec; i0 += U * THREADS) {
+    take(q, i0);
+    add(q);
   }
   // the elements before the first and after the last vector (at most 2 (VN - 1))
   for (int i = tid; i < z.V - nvec * VN; i += THREADS) {
@@ -150,9 +184,9 @@ row_fwd_kernel(const Logits z, float2* __restrict__ stats, const Row finish) {
     s = s * exp2_fast(m - sub) + exp2_fast(fmaf(v, k, -sub));
     m = mm;
   }
-  if (m > -INFINITY) {
-    const float whole = ceilf(m);
-    s *= exp2f(m - whole);
+  if (m > -INFINITY) {                               // to the integer above, by the lane's own power where it is that
+    const float whole = ceilf(m), down = m - whole;
+    s *= down == fraction - 1.f ? FRACTION_SCALE[threadIdx.x & 31] : exp2f(down);
     m = whole;
   }
 #pragma unroll
@@ -171,74 +205,128 @@ row_fwd_kernel(const Logits z, float2* __restrict__ stats, const Row finish) {
   }
   if (tid == 0) {
     stats[row] = make_float2(m, s);
-    const double lp = LN2 * ((double)to_f32<T>(x[label]) * (double)k - (double)m) - log((double)s) - EXP2_LOW;
-    finish(z, row, true, lp);
+    at_label[row] = mine;
   }
 }
 
-// sums over a CTA of 1024 threads, for its first warp
-__device__ __forceinline__ double cta_sum(double v, double* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = scratch[threadIdx.x & 31];
+// What follows is one launch: a cluster of CTAs shares the rows, leaves sums in `scratch`, and the first CTA joins
+// them in their order.  (A thread of each row's CTA doing its row's part kept that CTA: 48 us for 42 with the pass.)
+constexpr int TAIL_THREADS = 512, TAIL_CTAS = 8, TAIL_ONE = 512;
+__device__ __forceinline__ double log_prob(const Logits& z, float2 stat, float at_label) {
+  return LN2 * ((double)at_label * (double)z.k - (double)stat.x) - log((double)stat.y) - EXP2_LOW;
+}
+__device__ __forceinline__ double warp_sum64(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// Means over the rows that count: out = (loss, KL, clipped, one over their number).
-__global__ void __launch_bounds__(1024)
-policy_mean_kernel(const float4* __restrict__ terms, float* __restrict__ loss, float* __restrict__ kl,
-                   float* __restrict__ clipped, float* __restrict__ inv, long long rows) {
+struct PolicyArgs {
+  const float *old, *ref, *adv;    // ref null: no reference
+  long long adv_n, adv_t;          // strides of the advantages
+  float low, high, kl;
+  double inv_temperature;
+  float *logp, *coef;              // coef: of the row's own term, before the mean
+  float *loss, *mean_kl, *clipped, *inv;
+};
+__global__ void __launch_bounds__(TAIL_THREADS)
+policy_tail_kernel(const Logits z, const float2* __restrict__ stats, const float* __restrict__ at_label,
+                   const PolicyArgs p, double* __restrict__ scratch) {
   after_previous();
-  __shared__ double scratch[32];
-  double t = 0.0, e = 0.0, c = 0.0, n = 0.0;
-#pragma unroll 4
-  for (long long r = threadIdx.x; r < rows; r += 1024) {
-    const float4 v = terms[r];
-    t += v.x; e += v.y; c += v.z; n += v.w;
+  __shared__ double part[4][TAIL_THREADS / 32];
+  double sums[4] = {};                               // terms, KL, clipped, counted
+  for (long long r = (long long)blockIdx.x * TAIL_THREADS + threadIdx.x; r < z.rows;
+       r += (long long)gridDim.x * TAIL_THREADS) {
+    // all at once, whether the row counts (its statistics are written only then) or not
+    const long long n = r / z.T, label = z.labels[r];
+    const float2 stat = stats[r];
+    const float logit = at_label[r], old = p.old[r], ref = p.ref ? p.ref[r] : 0.f;
+    const float adv = p.adv[n * p.adv_n + (r - n * z.T) * p.adv_t];
+    if (!z.counts(label)) {
+      p.logp[r] = p.coef[r] = 0.f;
+      continue;
+    }
+    const double lp = log_prob(z, stat, logit), a = adv, ratio = exp(lp - (double)old);
+    const double lo = 1.0 - (double)p.low, hi = 1.0 + (double)p.high;
+    const double free = ratio * a, held = fmin(fmax(ratio, lo), hi) * a;
+    const bool clipped = free > held;
+    double term = clipped ? -held : -free, c = clipped ? 0.0 : -free, each = 0.0;
+    if (p.ref) {
+      const double d = (double)ref - lp, e = expm1(d);
+      each = e - d;
+      term += p.kl * each;
+      c -= p.kl * e;
+    }
+    p.logp[r] = (float)lp;
+    p.coef[r] = (float)(c * p.inv_temperature);
+    sums[0] += term; sums[1] += each; sums[2] += clipped ? 1.0 : 0.0; sums[3] += 1.0;
   }
-  t = cta_sum(t, scratch);
-  e = cta_sum(e, scratch);
-  c = cta_sum(c, scratch);
-  n = cta_sum(n, scratch);
-  if (threadIdx.x == 0) {
-    const double one = 1.0 / (n > 0.0 ? n : 1.0);
-    *loss = (float)(t * one);
-    *kl = (float)(e * one);
-    *clipped = (float)(c * one);
-    *inv = (float)one;
+  const int warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sums[i] = warp_sum64(sums[i]);
+    if ((threadIdx.x & 31) == 0) part[i][warp] = sums[i];
+  }
+  __syncthreads();
+  if (threadIdx.x < 4) {
+    double t = 0.0;
+    for (int w = 0; w < TAIL_THREADS / 32; ++w) t += part[threadIdx.x][w];
+    scratch[blockIdx.x * 4 + threadIdx.x] = t;
+  }
+  __syncwarp();
+  if (gridDim.x > 1) cluster_sync();
+  else __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    double t[4] = {};
+    for (unsigned c = 0; c < gridDim.x; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] += __ldcg(scratch + c * 4 + i);
+    const double one = 1.0 / (t[3] > 0.0 ? t[3] : 1.0);
+    *p.loss = (float)(t[0] * one);
+    *p.mean_kl = (float)(t[1] * one);
+    *p.clipped = (float)(t[2] * one);
+    *p.inv = (float)one;
   }
 }
 
-// Rewards of the sequences, the mean loss over the pairs and what a sequence's log-probability gets of it.
-__global__ void __launch_bounds__(1024)
-preference_kernel(const double* __restrict__ logp, const float* __restrict__ ref, float* __restrict__ rewards,
-                  double* __restrict__ sums, float* __restrict__ loss, float* __restrict__ coef, int N, int T,
-                  float beta, float smoothing) {
+// Rewards of the sequences, the mean loss over the pairs and what a sequence's log-probability gets of it.  Warps
+// share the sequences; where there are more warps than sequences, several sum parts of one.
+__global__ void __launch_bounds__(TAIL_THREADS)
+preference_tail_kernel(const Logits z, const float2* __restrict__ stats, const float* __restrict__ at_label,
+                       const float* __restrict__ ref, float* __restrict__ rewards, float* __restrict__ loss,
+                       float* __restrict__ coef, double* __restrict__ scratch, int N, float beta, float smoothing) {
   after_previous();
-  __shared__ double scratch[32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int n = warp; n < N; n += 32) {
+  const int warps = gridDim.x * (TAIL_THREADS / 32), warp = blockIdx.x * (TAIL_THREADS / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, parts = max(1, min(warps / N, (z.T + 31) / 32)), items = N * parts;
+  for (int i = warp; i < items; i += warps) {
+    const int n = i / parts, part = i - n * parts;
     double t = 0.0;
-#pragma unroll 4
-    for (int i = lane; i < T; i += 32) t += logp[(long long)n * T + i];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if (lane == 0) {
-      const double reward = (double)beta * (t - (double)ref[n]);
-      sums[n] = reward;
-      rewards[n] = (float)reward;
+    for (long long j = part * 32 + lane; j < z.T; j += parts * 32) {
+      const long long r = (long long)n * z.T + j, label = z.labels[r];
+      const float2 stat = stats[r];                  // written where the row counts
+      const float logit = at_label[r];
+      if (z.counts(label)) t += log_prob(z, stat, logit);
     }
+    t = warp_sum64(t);
+    if (lane == 0) scratch[i] = t;
   }
-  __syncthreads();
+  __syncwarp();
+  if (gridDim.x > 1) cluster_sync();
+  else __syncthreads();
+  if (blockIdx.x > 0) return;
+  __shared__ double shared[TAIL_THREADS / 32];
+  auto reward = [&](int n) {
+    double t = 0.0;
+    for (int i = 0; i < parts; ++i) t += __ldcg(scratch + n * parts + i);
+    return (double)beta * (t - (double)ref[n]);
+  };
   const int P = N / 2;
   double total = 0.0;
-  for (int p = threadIdx.x; p < P; p += 1024) {
-    const double m = sums[p] - sums[P + p], e = exp(-fabs(m)), near = log1p(e);
+  for (int p = threadIdx.x; p < P; p += TAIL_THREADS) {
+    const double chosen = reward(p), rejected = reward(P + p);
+    rewards[p] = (float)chosen;
+    rewards[P + p] = (float)rejected;
+    const double m = chosen - rejected, e = exp(-fabs(m)), near = log1p(e);
     // -log sig(m) and -log sig(-m), sig(-m) and sig(m), none of which overflows
     const double lp = near + fmax(-m, 0.0), lm = near + fmax(m, 0.0);
     const double big = 1.0 / (1.0 + e), small = e / (1.0 + e);
@@ -249,8 +337,14 @@ preference_kernel(const double* __restrict__ logp, const float* __restrict__ ref
     coef[p] = (float)c;
     coef[P + p] = (float)-c;
   }
-  total = cta_sum(total, scratch);
-  if (threadIdx.x == 0) *loss = (float)(total / P);
+  total = warp_sum64(total);
+  if (lane == 0) shared[threadIdx.x >> 5] = total;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    total = 0.0;
+    for (int w = 0; w < TAIL_THREADS / 32; ++w) total += shared[w];
+    *loss = (float)(total / P);
+  }
 }
 
 // dz = g (onehot - p), g = coef[row / per] * gout * inv (inv null: 1).  THREADS threads a row; with 256 the grid is
@@ -261,8 +355,9 @@ row_bwd_kernel(const Logits z, const float2* __restrict__ stats, const float* __
                const float* __restrict__ gout, const float* __restrict__ inv, T* __restrict__ dz, int per) {
   after_previous();
   constexpr int VN = 16 / sizeof(T), UNROLL = THREADS < 128 ? 1 : THREADS < 256 ? 2 : 4;
-  const long long row = (long long)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
-  if (row >= z.rows) return;
+  // the last rows first: the forward has read them last, and what L2 still holds of them is read from there
+  const long long row = z.rows - 1 - ((long long)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS);
+  if (row < 0) return;
   const T* x = static_cast<const T*>(z.at) + z.row(row);
   T* d = dz + row * z.V;
   const long long label = z.labels[row];
@@ -272,7 +367,7 @@ row_bwd_kernel(const Logits z, const float2* __restrict__ stats, const float* __
   const int mis = (int)((reinterpret_cast<uintptr_t>(d) & 15) / sizeof(T));
   const int head = min(z.V, mis ? VN - mis : 0), nvec = (z.V - head) / VN, rest = z.V - nvec * VN;
   if (g == 0.f) {                    // a row that does not count, or whose ratio is held by the clipping
-    for (int i = first; i < nvec; i += step) reinterpret_cast<uint4*>(d + head)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = first; i < nvec; i += step) __stcs(reinterpret_cast<uint4*>(d + head) + i, make_uint4(0, 0, 0, 0));
     for (int i = first; i < rest; i += step) d[i < head ? i : nvec * VN + i] = from_f32<T>(0.f);
     return;
   }
@@ -285,13 +380,13 @@ row_bwd_kernel(const Logits z, const float2* __restrict__ stats, const float* __
   }
 #pragma unroll UNROLL
   for (int i = first; i < nvec; i += step) {
-    const uint4 in = __ldg(reinterpret_cast<const uint4*>(x + head) + i);
+    const uint4 in = __ldcs(reinterpret_cast<const uint4*>(x + head) + i);
     const T* e = reinterpret_cast<const T*>(&in);
     uint4 o;
     T* oe = reinterpret_cast<T*>(&o);
 #pragma unroll
     for (int j = 0; j < VN; ++j) oe[j] = from_f32<T>(grad(to_f32<T>(e[j]), head + i * VN + j));
-    reinterpret_cast<uint4*>(d + head)[i] = o;
+    __stcs(reinterpret_cast<uint4*>(d + head) + i, o);
   }
   for (int k2 = first; k2 < rest; k2 += step) {
     const int i = k2 < head ? k2 : nvec * VN + k2;
@@ -322,64 +417,86 @@ int logits_of(Logits& z, const void* at, const void* labels, long long N, int T,
   return 0;
 }
 
-template <typename Row>
-int rows_fwd(const Logits& z, void* stats, const Row& finish, int dtype, int sm_count, cudaStream_t st) {
-#define PF_ROWS(THREADS)                                                                                   \
-  after(row_fwd_kernel<T, THREADS, Row>, (unsigned)(THREADS < 256 ? (z.rows + 7) / 8 : z.rows),             \
-        THREADS < 256 ? 256 : THREADS, 0, st)(z, (float2*)stats, finish)
+int rows_fwd(const Logits& z, void* stats, void* at_label, int dtype, int sm_count, cudaStream_t st) {
+#define PF_ROWS(THREADS)                                                                                      \
+  after(row_fwd_kernel<T, THREADS>, (unsigned)(THREADS < 64 ? (z.rows + 7) / 8 : z.rows),                      \
+        THREADS < 64 ? 256 : THREADS, 0, st)(z, (float2*)stats, (float*)at_label)
   PF_DISPATCH3(dtype, {
     if (z.V <= 1024) PF_ROWS(32);
     else if (z.rows <= sm_count && z.V > 8192) PF_ROWS(1024);
-    else PF_ROWS(256);
+    else PF_ROWS(ROW_THREADS);
   });
 #undef PF_ROWS
   return 0;
 }
 
+// A launch of the kernels behind the rows: one CTA, or a cluster.
+template <typename... P>
+LaunchAfter<P...> tail(void (*kernel)(P...), long long rows, cudaStream_t st, cudaLaunchAttribute* cluster) {
+  auto l = after(kernel, rows <= TAIL_ONE ? 1 : TAIL_CTAS, TAIL_THREADS, 0, st);
+  if (rows > TAIL_ONE) {
+    cluster->id = cudaLaunchAttributeClusterDimension;
+    cluster->val.clusterDim.x = TAIL_CTAS;
+    cluster->val.clusterDim.y = cluster->val.clusterDim.z = 1;
+    l.cfg.attrs = cluster;
+    l.cfg.numAttrs = 1;
+  }
+  return l;
+}
+
 }  // namespace
 
+// Doubles of scratch that the forwards need: the cluster's sums (a preference: of up to as many parts of sequences as
+// it has warps), and the logits at the labels.
+PF_API int pf_token_loss_scratch(long long N, int T) {
+  const long long warps = TAIL_CTAS * (TAIL_THREADS / 32), rows = N * T;
+  const long long n = (N > warps ? N : warps) + (rows + 1) / 2;
+  return n > 0x7fffffffll ? -3 : (int)n;
+}
+
 // logits [N, T, V] with strides (n, t); labels int64 [N, T]; ref fp32 [N] -> loss, rewards fp32 [N], and for the
-// backward stats (two floats a row) and coef fp32 [N].  scratch: doubles [N * T + N].  N is even: the chosen
-// sequences, then the rejected ones.
+// backward stats (two floats a row) and coef fp32 [N].  N is even: the chosen sequences, then the rejected ones.
 PF_API int pf_preference_fwd(const void* logits, const void* labels, const void* ref, void* loss, void* rewards,
                              void* stats, void* coef, void* scratch, long long N, int T, int V, long long n,
                              long long t, long long ignore_index, float beta, float smoothing, int dtype,
                              int sm_count, void* stream) {
   Logits z;
-  const int code = logits_of(z, logits, labels, N, T, V, n, t, ignore_index, 1.f, dtype);
+  int code = logits_of(z, logits, labels, N, T, V, n, t, ignore_index, 1.f, dtype);
   if (code) return code;
   if (N < 2 || N % 2) return -3;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  double* logp = (double*)scratch;
-  if (z.rows) {
-    const int c = rows_fwd(z, stats, PreferenceRow{logp}, dtype, sm_count, st);
-    if (c) return c;
-  }
-  after(preference_kernel, 1, 1024, 0, st)(logp, (const float*)ref, (float*)rewards, logp + z.rows, (float*)loss,
-                                           (float*)coef, (int)N, T, beta, smoothing);
+  const long long warps = TAIL_CTAS * (TAIL_THREADS / 32);
+  double* sums = (double*)scratch;
+  float* at_label = (float*)(sums + (N > warps ? N : warps));
+  if (z.rows && (code = rows_fwd(z, stats, at_label, dtype, sm_count, st))) return code;
+  cudaLaunchAttribute cluster;
+  tail(preference_tail_kernel, z.rows, st, &cluster)(z, (const float2*)stats, at_label, (const float*)ref,
+                                                     (float*)rewards, (float*)loss, (float*)coef, sums, (int)N, beta,
+                                                     smoothing);
   PF_CHECK_LAUNCH();
   return 0;
 }
 
 // actions int64, old and ref (null: none) fp32 [N, T], adv fp32 with strides -> loss, kl, clipped, inv (one over the
-// number of rows that count), logp and coef fp32 [N, T], stats two floats a row.  scratch: four floats a row.
+// number of rows that count), logp and coef fp32 [N, T], stats two floats a row.
 PF_API int pf_policy_fwd(const void* logits, const void* actions, const void* old, const void* ref, const void* adv,
                          void* loss, void* kl, void* clipped, void* inv, void* logp, void* coef, void* stats,
                          void* scratch, long long N, int T, int V, long long n, long long t, long long adv_n,
                          long long adv_t, long long ignore_index, float low, float high, float kl_coef,
                          float inv_temperature, int dtype, int sm_count, void* stream) {
   Logits z;
-  const int code = logits_of(z, logits, actions, N, T, V, n, t, ignore_index, inv_temperature, dtype);
+  int code = logits_of(z, logits, actions, N, T, V, n, t, ignore_index, inv_temperature, dtype);
   if (code) return code;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const PolicyRow finish{(const float*)old, (const float*)ref, (const float*)adv, adv_n, adv_t, low, high, kl_coef,
-                         (double)inv_temperature, (float*)logp, (float*)coef, (float4*)scratch};
-  if (z.rows) {
-    const int c = rows_fwd(z, stats, finish, dtype, sm_count, st);
-    if (c) return c;
-  }
-  after(policy_mean_kernel, 1, 1024, 0, st)((const float4*)scratch, (float*)loss, (float*)kl, (float*)clipped,
-                                            (float*)inv, z.rows);
+  const PolicyArgs p{(const float*)old, (const float*)ref, (const float*)adv, adv_n, adv_t, low, high, kl_coef,
+                     (double)inv_temperature, (float*)logp, (float*)coef, (float*)loss, (float*)kl, (float*)clipped,
+                     (float*)inv};
+  const long long warps = TAIL_CTAS * (TAIL_THREADS / 32);
+  double* sums = (double*)scratch;
+  float* at_label = (float*)(sums + (N > warps ? N : warps));
+  if (z.rows && (code = rows_fwd(z, stats, at_label, dtype, sm_count, st))) return code;
+  cudaLaunchAttribute cluster;
+  tail(policy_tail_kernel, z.rows, st, &cluster)(z, (const float2*)stats, at_label, p, sums);
   PF_CHECK_LAUNCH();
   return 0;
 }

@@ -577,7 +577,7 @@ def preference_fwd(logits: torch.Tensor, labels: torch.Tensor, ref: torch.Tensor
     assert N >= 2 and N % 2 == 0 and ref.shape == (N,) and ref.device == z.device
     new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=z.device)
     loss, rewards, stats, coef = new(), new(N), new(N, T, 2), new(N)
-    scratch = torch.empty(N * T + N, dtype=torch.float64, device=z.device)
+    scratch = torch.empty(L.pf_token_loss_scratch(N, T), dtype=torch.float64, device=z.device)
     check(L.pf_preference_fwd(z, labels, _floats(ref), loss, rewards, stats, coef, scratch, N, T, V, z.stride(0),
                               z.stride(1), ignore_index, beta, smoothing, dt(z.dtype), sm_count(z.device),
                               stream_of(z)), "pf_preference_fwd")
@@ -596,7 +596,8 @@ def policy_fwd(logits: torch.Tensor, actions: torch.Tensor, old: torch.Tensor, a
     adv = adv if adv.dtype == torch.float32 else adv.float()
     new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=z.device)
     loss, kl, clipped, inv = new(), new(), new(), new()
-    logps, coef, stats, scratch = new(N, T), new(N, T), new(N, T, 2), new(N, T, 4)
+    logps, coef, stats = new(N, T), new(N, T), new(N, T, 2)
+    scratch = torch.empty(L.pf_token_loss_scratch(N, T), dtype=torch.float64, device=z.device)
     check(L.pf_policy_fwd(z, actions, _floats(old), None if ref is None else _floats(ref), adv, loss, kl, clipped,
                           inv, logps, coef, stats, scratch, N, T, V, z.stride(0), z.stride(1), adv.stride(0),
                           adv.stride(1), ignore_index, low, high, kl_coef, 1.0 / temperature, dt(z.dtype),
