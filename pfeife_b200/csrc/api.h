@@ -110,7 +110,7 @@ PF_DECL int pf_heads_bwd(const void* gq, const void* gk, const void* gv, const v
                          void* stream);
 
 // ---- tune_loss.cu : preference and policy losses
-PF_DECL int pf_token_loss_scratch(long long N, int T);
+PF_DECL int pf_token_loss_scratch(long long N, int T, int V, int dtype, int sm_count);
 PF_DECL int pf_preference_fwd(const void* logits, const void* labels, const void* ref, void* loss,
                               void* rewards, void* stats, void* coef, void* scratch, long long N,
                               int T, int V, long long n, long long t, long long ignore_index,

@@ -29,6 +29,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <atomic>
+#include <cmath>
 
 #include "api.h"
 
@@ -846,8 +847,8 @@ bool tokens_fit(const Tensor& z, const Tensor& labels) {
          z.size(1) < (1ll << 31) && labels.scalar_type() == at::kLong && labels.dim() == 2 && labels.is_contiguous() &&
          labels.size(0) == z.size(0) && labels.size(1) == z.size(1);
 }
-Tensor loss_scratch(const Tensor& like, int64_t N, int64_t T) {
-  const int n = pf_token_loss_scratch(N, (int)T);
+Tensor loss_scratch(const Env& e, const Tensor& like, int64_t N, int64_t T) {
+  const int n = pf_token_loss_scratch(N, (int)T, (int)like.size(2), code_of(like), e.sms);
   if (n < 0) throw Failed{n, "pf_token_loss_scratch"};
   return empty({n}, at::kDouble, like);
 }
@@ -891,7 +892,7 @@ variable_list token_loss_backward(AutogradContext* ctx, const Tensor& g, int inp
   Tensor coef = a.narrow(0, 2 * kept.rows, kept.n), one;
   if (inv) {
     coef = coef.view({N, T});
-    one = a.narrow(0, 2 * kept.rows + kept.n, 1).view({});
+    one = a.select(0, 2 * kept.rows + kept.n);
   }
   out[0] = dispatched("pfeife::token_loss_bwd", {g, z, labels, a.narrow(0, 0, 2 * kept.rows).view({N, T, 2}), coef,
                                                  opt(one), ignore, temperature})[0].toTensor();
@@ -904,7 +905,7 @@ variable_list preference_forward(const Tensor& z, const Tensor& labels, const Te
   const int64_t N = z.size(0), T = z.size(1);
   const Kept kept{floats(2 * N * T + N, z), N * T, N, false};
   all = kept.all;
-  const Tensor loss = empty({}, at::kFloat, z), rewards = floats(N, z), scratch = loss_scratch(z, N, T);
+  const Tensor loss = empty({}, at::kFloat, z), rewards = floats(N, z), scratch = loss_scratch(e, z, N, T);
   ok(pf_preference_fwd(z.data_ptr(), labels.data_ptr(), ref.data_ptr(), loss.data_ptr(), rewards.data_ptr(),
                        kept.stats(), kept.coef(), scratch.data_ptr(), N, (int)T, (int)z.size(2), z.stride(0),
                        z.stride(1), ignore, (float)beta, (float)smoothing, code_of(z), e.sms, e.stream),
@@ -943,7 +944,7 @@ variable_list policy_forward(const Tensor& z, const Tensor& actions, const Tenso
   const Kept kept{floats(3 * rows + 1, z), rows, rows, true};
   all = kept.all;
   const Tensor loss = empty({}, at::kFloat, z), logps = empty({N, T}, at::kFloat, z), kl = empty({}, at::kFloat, z),
-               clipped = empty({}, at::kFloat, z), scratch = loss_scratch(z, N, T);
+               clipped = empty({}, at::kFloat, z), scratch = loss_scratch(e, z, N, T);
   ok(pf_policy_fwd(z.data_ptr(), actions.data_ptr(), old.data_ptr(), at_or_null(ref), adv.data_ptr(), loss.data_ptr(),
                    kl.data_ptr(), clipped.data_ptr(), kept.one_over(), logps.data_ptr(), kept.coef(), kept.stats(),
                    scratch.data_ptr(), N, (int)T, (int)z.size(2), z.stride(0), z.stride(1),
@@ -1410,7 +1411,7 @@ PF_OP(policy_loss) {
   for (const Tensor* t : {&old, &ref})
     if (t->defined() && (!packed_floats(*t, N * T) || t->dim() != 2 || t->size(0) != N || t->requires_grad()))
       Py_RETURN_NONE;
-  if (!advantages_fit(adv, N, T) || adv.requires_grad() || !(c.temperature > 0.0) || !(c.low >= 0.0 && c.low <= 1.0) ||
+  if (!advantages_fit(adv, N, T) || adv.requires_grad() || !(c.temperature > 0.0 && c.temperature < INFINITY) || !(c.low >= 0.0 && c.low <= 1.0) ||
       !(c.high >= 0.0))
     Py_RETURN_NONE;
   if (!recorded(z))

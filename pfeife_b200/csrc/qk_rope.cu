@@ -642,6 +642,7 @@ PF_API int pf_heads_fwd(const void* q, const void* k, const void* v, void* yq, v
   const int vw = prepare(p, parts, cos_t, sin_t, pos, spos, B, S, D, R, rows, eps, dtype);
   if (vw < 0) return vw;
   if ((long long)B * S * (Hq + 2ll * Hk) > 0x7fffffffll) return -3;
+  if (p.tokens == 0 || (Hq == 0 && Hk == 0)) return 0;
   const int even[3] = {1, 1, 1};
   const int code = wq ? launch<NORM>(p, parts, even, interleaved, dtype, vw, sm_count, stream)
                    : inverse ? launch<UNROTATE>(p, parts, even, interleaved, dtype, vw, sm_count, stream)

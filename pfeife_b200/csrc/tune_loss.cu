@@ -121,13 +121,14 @@ template <> struct Words<__nv_bfloat16> {
 };
 
 constexpr int ROW_BATCH = 4;       // vectors that a thread takes at a time
-constexpr int ROW_THREADS = 128;   // of most rows, and twelve such rows an SM
+constexpr int ROW_THREADS = 128;   // of a part of a row, and twelve such parts an SM
+constexpr int ROW_WARP = 1024;     // a row up to here is a warp's
 
-// One pass over each row that counts: M and s to stats, the label's logit to `at_label`.  THREADS threads a row:
-// CTAs of their own, or warps that share one of 256.
+// One pass over each row that counts: M and s of its gridDim.y parts, and the label's logit to `at_label`.  THREADS
+// threads a part: CTAs of their own, or warps (of whole rows) that share one of 256.
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS < 64 ? 256 : THREADS, THREADS == ROW_THREADS ? 12 : 1)
-row_fwd_kernel(const Logits z, float2* __restrict__ stats, float* __restrict__ at_label) {
+row_fwd_kernel(const Logits z, float2* __restrict__ parts, float* __restrict__ at_label) {
   after_previous();
   constexpr int W = THREADS / 32, VN = 16 / sizeof(T), U = ROW_BATCH;
   constexpr int ROWS = W > 1 ? 1 : 8;
@@ -138,18 +139,19 @@ row_fwd_kernel(const Logits z, float2* __restrict__ stats, float* __restrict__ a
   const long long label = z.labels[row];
   if (!z.counts(label)) return;
   const T* x = static_cast<const T*>(z.at) + z.row(row);
-  const float mine = tid == 0 ? to_f32<T>(x[label]) : 0.f;
+  const int part = W > 1 ? blockIdx.y : 0, n_parts = W > 1 ? gridDim.y : 1;
+  const float mine = tid == 0 && part == 0 ? to_f32<T>(x[label]) : 0.f;
   const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int head = min(z.V, mis ? VN - mis : 0), nvec = (z.V - head) / VN;
   const float k = z.k, fraction = (threadIdx.x & 31) * (1.f / 32);
   float m = -INFINITY, s = 0.f;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   const uint64_t k2 = f2_pack(k, k);
-  auto take = [&](uint4 (&q)[U], int i0) {           // -inf behind the row's end, which adds nothing
+  auto take = [&](uint4 (&q)[U], int i0, int end) {  // -inf behind the part's end, which adds nothing
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       q[u] = Words<T>::none();
-      if (i0 + u * THREADS < nvec) q[u] = __ldg(xv + i0 + u * THREADS);
+      if (i0 + u * THREADS < end) q[u] = __ldg(xv + i0 + u * THREADS);
     }
   };
   auto add = [&](const uint4 (&q)[U]) {
@@ -173,12 +175,13 @@ row_fwd_kernel(const Logits z, float2* __restrict__ stats, float* __restrict__ a
     m = mm;
   };
   uint4 q[U];
-  for (int i0 = tid; i0 < nvec; i0 += U * THREADS) {
-    take(q, i0);
+  const int begin = (int)((long long)nvec * part / n_parts), end = (int)((long long)nvec * (part + 1) / n_parts);
+  for (int i0 = begin + tid; i0 < end; i0 += U * THREADS) {
+    take(q, i0, end);
     add(q);
   }
   // the elements before the first and after the last vector (at most 2 (VN - 1))
-  for (int i = tid; i < z.V - nvec * VN; i += THREADS) {
+  for (int i = tid; part == 0 && i < z.V - nvec * VN; i += THREADS) {
     const float v = to_f32<T>(x[i < head ? i : nvec * VN + i]);
     const float mm = fmaxf(m, ceilf(v * k) + fraction), sub = mm == -INFINITY ? 0.f : mm;
     s = s * exp2_fast(m - sub) + exp2_fast(fmaf(v, k, -sub));
@@ -204,14 +207,29 @@ row_fwd_kernel(const Logits z, float2* __restrict__ stats, float* __restrict__ a
       part_merge(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
   }
   if (tid == 0) {
-    stats[row] = make_float2(m, s);
-    at_label[row] = mine;
+    parts[row * n_parts + part] = make_float2(m, s);
+    if (part == 0) at_label[row] = mine;
   }
 }
 
 // What follows is one launch: a cluster of CTAs shares the rows, leaves sums in `scratch`, and the first CTA joins
 // them in their order.  (A thread of each row's CTA doing its row's part kept that CTA: 48 us for 42 with the pass.)
 constexpr int TAIL_THREADS = 512, TAIL_CTAS = 8, TAIL_ONE = 512;
+// What the forward's pass over the rows has left: joined for the backward, and a row's log-probability.
+struct Rows {
+  const float2* parts;             // [rows][n_parts]
+  const float* at_label;
+  float2* stats;                   // [rows]
+  int n_parts;
+  __device__ __forceinline__ float2 join(long long r) const {
+    float2 v = parts[r * n_parts];
+    for (int i = 1; i < n_parts; ++i) {
+      const float2 w = parts[r * n_parts + i];
+      part_merge(v.x, v.y, w.x, w.y);
+    }
+    return v;
+  }
+};
 __device__ __forceinline__ double log_prob(const Logits& z, float2 stat, float at_label) {
   return LN2 * ((double)at_label * (double)z.k - (double)stat.x) - log((double)stat.y) - EXP2_LOW;
 }
@@ -230,8 +248,7 @@ struct PolicyArgs {
   float *loss, *mean_kl, *clipped, *inv;
 };
 __global__ void __launch_bounds__(TAIL_THREADS)
-policy_tail_kernel(const Logits z, const float2* __restrict__ stats, const float* __restrict__ at_label,
-                   const PolicyArgs p, double* __restrict__ scratch) {
+policy_tail_kernel(const Logits z, const Rows rows, const PolicyArgs p, double* __restrict__ scratch) {
   after_previous();
   __shared__ double part[4][TAIL_THREADS / 32];
   double sums[4] = {};                               // terms, KL, clipped, counted
@@ -239,13 +256,14 @@ policy_tail_kernel(const Logits z, const float2* __restrict__ stats, const float
        r += (long long)gridDim.x * TAIL_THREADS) {
     // all at once, whether the row counts (its statistics are written only then) or not
     const long long n = r / z.T, label = z.labels[r];
-    const float2 stat = stats[r];
-    const float logit = at_label[r], old = p.old[r], ref = p.ref ? p.ref[r] : 0.f;
+    const float2 stat = rows.join(r);
+    const float logit = rows.at_label[r], old = p.old[r], ref = p.ref ? p.ref[r] : 0.f;
     const float adv = p.adv[n * p.adv_n + (r - n * z.T) * p.adv_t];
     if (!z.counts(label)) {
       p.logp[r] = p.coef[r] = 0.f;
       continue;
     }
+    rows.stats[r] = stat;
     const double lp = log_prob(z, stat, logit), a = adv, ratio = exp(lp - (double)old);
     const double lo = 1.0 - (double)p.low, hi = 1.0 + (double)p.high;
     const double free = ratio * a, held = fmin(fmax(ratio, lo), hi) * a;
@@ -292,8 +310,7 @@ policy_tail_kernel(const Logits z, const float2* __restrict__ stats, const float
 // Rewards of the sequences, the mean loss over the pairs and what a sequence's log-probability gets of it.  Warps
 // share the sequences; where there are more warps than sequences, several sum parts of one.
 __global__ void __launch_bounds__(TAIL_THREADS)
-preference_tail_kernel(const Logits z, const float2* __restrict__ stats, const float* __restrict__ at_label,
-                       const float* __restrict__ ref, float* __restrict__ rewards, float* __restrict__ loss,
+preference_tail_kernel(const Logits z, const Rows rows, const float* __restrict__ ref, float* __restrict__ rewards, float* __restrict__ loss,
                        float* __restrict__ coef, double* __restrict__ scratch, int N, float beta, float smoothing) {
   after_previous();
   const int warps = gridDim.x * (TAIL_THREADS / 32), warp = blockIdx.x * (TAIL_THREADS / 32) + (threadIdx.x >> 5);
@@ -303,9 +320,12 @@ preference_tail_kernel(const Logits z, const float2* __restrict__ stats, const f
     double t = 0.0;
     for (long long j = part * 32 + lane; j < z.T; j += parts * 32) {
       const long long r = (long long)n * z.T + j, label = z.labels[r];
-      const float2 stat = stats[r];                  // written where the row counts
-      const float logit = at_label[r];
-      if (z.counts(label)) t += log_prob(z, stat, logit);
+      const float2 stat = rows.join(r);              // written where the row counts
+      const float logit = rows.at_label[r];
+      if (z.counts(label)) {
+        rows.stats[r] = stat;
+        t += log_prob(z, stat, logit);
+      }
     }
     t = warp_sum64(t);
     if (lane == 0) scratch[i] = t;
@@ -417,16 +437,42 @@ int logits_of(Logits& z, const void* at, const void* labels, long long N, int T,
   return 0;
 }
 
-int rows_fwd(const Logits& z, void* stats, void* at_label, int dtype, int sm_count, cudaStream_t st) {
-#define PF_ROWS(THREADS)                                                                                      \
-  after(row_fwd_kernel<T, THREADS>, (unsigned)(THREADS < 64 ? (z.rows + 7) / 8 : z.rows),                      \
-        THREADS < 64 ? 256 : THREADS, 0, st)(z, (float2*)stats, (float*)at_label)
+// Parts of a row: enough for the CTAs that the SMs hold, and none of less than a batch (16 rows of 32000 fp32: 6.7 ->
+// 6.2 us; four times as many are slower by 1 to 3 us where rows fill the SMs as they are).
+int row_parts(long long rows, int V, int dtype, int sm_count) {
+  const int batch = ROW_THREADS * ROW_BATCH * (dtype == PF_F32 ? 4 : 8);
+  if (V <= ROW_WARP || rows == 0) return 1;
+  long long n = (12ll * sm_count + rows - 1) / rows;
+  const int most = (V + batch - 1) / batch;
+  if (n > most) n = most;
+  return n < 1 ? 1 : (int)n;
+}
+
+// Scratch of a forward: the cluster's sums (a preference: of up to as many parts of sequences as it has warps), the
+// parts of the rows and the logits at the labels.
+struct Scratch {
+  double* sums;
+  float2* parts;
+  float* at_label;
+  long long doubles;
+  Scratch(void* at, long long N, long long rows, int n_parts) {
+    const long long warps = TAIL_CTAS * (TAIL_THREADS / 32), n = N > warps ? N : warps;
+    sums = (double*)at;
+    parts = (float2*)(sums + n);
+    at_label = (float*)(parts + rows * n_parts);
+    doubles = n + rows * n_parts + (rows + 1) / 2;
+  }
+};
+
+int rows_fwd(const Logits& z, const Scratch& s, int n_parts, int dtype, cudaStream_t st) {
+  if (z.rows == 0) return 0;
   PF_DISPATCH3(dtype, {
-    if (z.V <= 1024) PF_ROWS(32);
-    else if (z.rows <= sm_count && z.V > 8192) PF_ROWS(1024);
-    else PF_ROWS(ROW_THREADS);
+    if (z.V <= ROW_WARP)
+      after(row_fwd_kernel<T, 32>, (unsigned)((z.rows + 7) / 8), 256, 0, st)(z, s.parts, s.at_label);
+    else
+      after(row_fwd_kernel<T, ROW_THREADS>, dim3((unsigned)z.rows, n_parts), ROW_THREADS, 0, st)(z, s.parts,
+                                                                                                 s.at_label);
   });
-#undef PF_ROWS
   return 0;
 }
 
@@ -446,11 +492,9 @@ LaunchAfter<P...> tail(void (*kernel)(P...), long long rows, cudaStream_t st, cu
 
 }  // namespace
 
-// Doubles of scratch that the forwards need: the cluster's sums (a preference: of up to as many parts of sequences as
-// it has warps), and the logits at the labels.
-PF_API int pf_token_loss_scratch(long long N, int T) {
-  const long long warps = TAIL_CTAS * (TAIL_THREADS / 32), rows = N * T;
-  const long long n = (N > warps ? N : warps) + (rows + 1) / 2;
+// Doubles of scratch that a forward needs.
+PF_API int pf_token_loss_scratch(long long N, int T, int V, int dtype, int sm_count) {
+  const long long rows = N * T, n = Scratch(nullptr, N, rows, row_parts(rows, V, dtype, sm_count)).doubles;
   return n > 0x7fffffffll ? -3 : (int)n;
 }
 
@@ -465,14 +509,13 @@ PF_API int pf_preference_fwd(const void* logits, const void* labels, const void*
   if (code) return code;
   if (N < 2 || N % 2) return -3;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const long long warps = TAIL_CTAS * (TAIL_THREADS / 32);
-  double* sums = (double*)scratch;
-  float* at_label = (float*)(sums + (N > warps ? N : warps));
-  if (z.rows && (code = rows_fwd(z, stats, at_label, dtype, sm_count, st))) return code;
+  const int n_parts = row_parts(z.rows, V, dtype, sm_count);
+  const Scratch s(scratch, N, z.rows, n_parts);
+  if ((code = rows_fwd(z, s, n_parts, dtype, st))) return code;
+  const Rows rows{s.parts, s.at_label, (float2*)stats, n_parts};
   cudaLaunchAttribute cluster;
-  tail(preference_tail_kernel, z.rows, st, &cluster)(z, (const float2*)stats, at_label, (const float*)ref,
-                                                     (float*)rewards, (float*)loss, (float*)coef, sums, (int)N, beta,
-                                                     smoothing);
+  tail(preference_tail_kernel, z.rows, st, &cluster)(z, rows, (const float*)ref, (float*)rewards, (float*)loss,
+                                                     (float*)coef, s.sums, (int)N, beta, smoothing);
   PF_CHECK_LAUNCH();
   return 0;
 }
@@ -491,12 +534,12 @@ PF_API int pf_policy_fwd(const void* logits, const void* actions, const void* ol
   const PolicyArgs p{(const float*)old, (const float*)ref, (const float*)adv, adv_n, adv_t, low, high, kl_coef,
                      (double)inv_temperature, (float*)logp, (float*)coef, (float*)loss, (float*)kl, (float*)clipped,
                      (float*)inv};
-  const long long warps = TAIL_CTAS * (TAIL_THREADS / 32);
-  double* sums = (double*)scratch;
-  float* at_label = (float*)(sums + (N > warps ? N : warps));
-  if (z.rows && (code = rows_fwd(z, stats, at_label, dtype, sm_count, st))) return code;
+  const int n_parts = row_parts(z.rows, V, dtype, sm_count);
+  const Scratch s(scratch, N, z.rows, n_parts);
+  if ((code = rows_fwd(z, s, n_parts, dtype, st))) return code;
+  const Rows rows{s.parts, s.at_label, (float2*)stats, n_parts};
   cudaLaunchAttribute cluster;
-  tail(policy_tail_kernel, z.rows, st, &cluster)(z, (const float2*)stats, at_label, p, sums);
+  tail(policy_tail_kernel, z.rows, st, &cluster)(z, rows, p, s.sums);
   PF_CHECK_LAUNCH();
   return 0;
 }

@@ -986,7 +986,7 @@ def preference_fwd(logits: Tensor, labels: Tensor, ref_logps: Tensor, beta: floa
     if _native(logits) or (logits.is_cuda and logits.dtype == torch.float32):
         return kx.preference_fwd(logits, labels, ref_logps, beta, smoothing, ignore_index)
     logp, _, stats = _token_logps_ref(logits, labels, 1.0, ignore_index)
-    rewards = beta * (logp.sum(1) - ref_logps.double())
+    rewards = beta * (logp.sum(1) - ref_logps.float().double())
     margin = rewards[: len(rewards) // 2] - rewards[len(rewards) // 2:]
     loss = torch.zeros_like(margin)
     if smoothing < 1.0:
@@ -1012,9 +1012,10 @@ def token_loss_bwd(dloss: Tensor, logits: Tensor, labels: Tensor, stats: Tensor,
     if _native(logits) or (logits.is_cuda and logits.dtype == torch.float32):
         return kx.token_loss_bwd(dloss, logits, labels, stats, coef, inv, ignore_index, temperature)
     counted = _tokens_counted(labels, logits.shape[-1], ignore_index)
+    coef = coef.float()                  # the declared type, as the kernel reads it
     g = (coef if coef.dim() == 2 else coef.unsqueeze(1)) * dloss
     if inv is not None:
-        g = g * inv
+        g = g * inv.float()
     p = torch.softmax(_wide(logits) / temperature, -1)
     onehot = torch.zeros_like(p).scatter_(-1, labels.masked_fill(~counted, 0).unsqueeze(-1), 1.0)
     d = g.unsqueeze(-1) * (onehot - p)
@@ -1071,7 +1072,8 @@ def preference_loss(logits: Tensor, labels: Tensor, ref_logps: Tensor, beta: flo
                     label_smoothing: float = 0.0, ignore_index: int = -100) -> PreferenceLoss:
     """Loss on paired log ratios.  logits [2P, T, V]: the P chosen sequences, then the P rejected ones in the same
     order; labels [2P, T]: the token that each row predicts, ``ignore_index`` or any number outside the vocabulary
-    where none counts (prompts, padding); ref_logps [2P]: the sequences' log-probabilities under the reference.
+    where none counts (prompts, padding); ref_logps [2P]: the sequences' log-probabilities under the reference,
+    read in 32 bits.
     With l the sum of a sequence's log-probabilities and m = beta ((l - ref of the chosen) - (l - ref of the
     rejected)) the loss is the mean of -(1 - label_smoothing) log sig(m) - label_smoothing log sig(-m).
     Rows that do not count are not read and get a gradient of zero, whatever their logits."""
@@ -1101,8 +1103,8 @@ def policy_fwd(logits: Tensor, actions: Tensor, old_logps: Tensor, advantages: T
         return kx.policy_fwd(logits, actions, old_logps, advantages, ref_logps, low, high, kl_coef, temperature,
                              ignore_index)
     logp, counted, stats = _token_logps_ref(logits, actions, temperature, ignore_index)
-    adv = advantages.double()
-    ratio = torch.exp(logp - old_logps.double())
+    adv = advantages.float().double()
+    ratio = torch.exp(logp - old_logps.float().double())
     free, held = ratio * adv, ratio.clamp(1 - low, 1 + high) * adv
     cut = free > held
     term, coef = -torch.where(cut, held, free), torch.where(cut, 0.0, -free)
@@ -1110,7 +1112,7 @@ def policy_fwd(logits: Tensor, actions: Tensor, old_logps: Tensor, advantages: T
     mean = lambda t: (t.masked_fill(~counted, 0.0).sum() * inv).float()
     kl = torch.zeros((), device=logits.device)
     if ref_logps is not None:
-        d = ref_logps.double() - logp
+        d = ref_logps.float().double() - logp
         each = torch.expm1(d) - d
         term, coef, kl = term + kl_coef * each, coef - kl_coef * torch.expm1(d), mean(each)
     coef = (coef / temperature).masked_fill(~counted, 0.0).float()
@@ -1147,7 +1149,7 @@ def policy_loss(logits: Tensor, actions: Tensor, old_logps: Tensor, advantages: 
     """Clipped policy loss over sampled tokens.  logits [..., V]; actions [...]: the token taken at each row,
     ``ignore_index`` or any number outside the vocabulary where none counts; old_logps [...]: its log-probability
     when it was sampled; advantages: of the shape of the actions or one that expands to it ([N, 1]: one for each
-    sequence).  With l = log softmax(logits / temperature)[action] and r = exp(l - old) a token's term is
+    sequence), all read in 32 bits.  With l = log softmax(logits / temperature)[action] and r = exp(l - old) a token's term is
     -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(ref - l) - (ref - l) - 1), the last with
     ``ref_logps`` [...] only; the loss is the mean over the tokens that count, 0 if there are none.
     Rows that do not count are not read and get a gradient of zero, whatever their logits."""
@@ -1164,7 +1166,7 @@ def policy_loss(logits: Tensor, actions: Tensor, old_logps: Tensor, advantages: 
         for name, t in (("old_logps", old_logps), ("ref_logps", ref_logps)):
             if t is not None and t.shape != shape:
                 raise ValueError(f"policy_loss: {name} {tuple(shape)} are needed, not {tuple(t.shape)}")
-    if temperature <= 0.0 or not 0.0 <= clip_low <= 1.0 or clip_high < 0.0:
+    if not 0.0 < temperature < math.inf or not 0.0 <= clip_low <= 1.0 or not clip_high >= 0.0:
         raise ValueError(f"policy_loss: a temperature {temperature} above 0, clip_low {clip_low} between 0 and 1 and "
                          f"clip_high {clip_high} of at least 0 are needed")
     if advantages.shape != shape:
@@ -1241,10 +1243,15 @@ def embedding(ids: Tensor, table: Tensor, out_dtype: Optional[torch.dtype] = Non
     return _call(embed_fwd, ids, table, out_dtype)
 
 
+def _narrow(cos: Tensor, x: Tensor) -> bool:
+    """Tables of a part of each head."""
+    return isinstance(x, Tensor) and cos.dim() == 2 and 2 * cos.shape[1] < x.shape[-1]
+
+
 @_custom_op("pfeife::rope_apply")
 def rope_apply(x: Tensor, cos: Tensor, sin: Tensor, inverse: bool) -> Tensor:
     """x [B, S, H, D]; cos/sin fp32 [S, D/2]; half-split pairing (i, i + D/2).  Narrower tables rotate a part."""
-    if cos.dim() == 2 and 2 * cos.shape[1] < x.shape[-1]:
+    if _narrow(cos, x):                  # of a symbolic trace, which could not tell
         _check_angles(x, cos, sin, None)
         return rope_at.plain(x, cos, sin, None, False, inverse)
     if _native(x) or (x.is_cuda and x.dtype == torch.float32):
@@ -1284,7 +1291,7 @@ def rope(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None
     beyond R stay.  ``positions``, integers [S] or [B, S], are the rows of the tables to turn by (default: row s
     for token s).  A row that the tables do not have makes the token's rotated values NaN on CUDA, where looking
     for it would wait for the device, and an IndexError on the CPU."""
-    if positions is None and not interleaved:
+    if positions is None and not interleaved and not _narrow(cos, x):
         return _call(rope_apply, x, cos, sin, False)
     y = _native_call("rotate_heads", x, cos, sin, positions, interleaved)
     if y is not None:
@@ -1296,7 +1303,7 @@ def rope(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None
 @_custom_op("pfeife::rope_qkv_apply")
 def rope_qkv_apply(qkv: Tensor, cos: Tensor, sin: Tensor, inverse: bool) -> Tensor:
     """qkv [B, S, 3, H, D] -> a contiguous tensor with the queries and keys rotated."""
-    if cos.dim() == 2 and 2 * cos.shape[1] < qkv.shape[-1]:
+    if _narrow(cos, qkv):
         _check_angles(qkv, cos, sin, None)
         return rope_qkv_at.plain(qkv, cos, sin, None, False, inverse)
     if _native(qkv):
@@ -1323,7 +1330,7 @@ _autograd(rope_qkv_apply, 1, _rope_qkv_backward, setup=_rope_setup)
 def rope_qkv(qkv: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None,
              interleaved: bool = False) -> Tensor:
     """``rope`` of the queries and keys of a fused projection [B, S, 3, H, D], for ``attention_qkv``."""
-    if positions is None and not interleaved:
+    if positions is None and not interleaved and not _narrow(cos, qkv):
         y = _native_call("rope_qkv", qkv, cos, sin)
         return y if y is not None else _call(rope_qkv_apply, qkv, cos, sin, False)
     y = _native_call("rotate_heads", qkv, cos, sin, positions, interleaved)
@@ -1515,7 +1522,7 @@ def _head_norm_grad_ref(g: Tensor, x: Tensor, w: Tensor, eps: float) -> Tuple[Te
 def _head_norm_buckets(wq: Tensor, wk: Tensor, x: Tensor):
     """(where the gradients of both gains go, whether they are registered buckets, which are added to)"""
     bq, bk = _grad_bucket(wq), _grad_bucket(wk)
-    if bq is not None and bk is not None:
+    if bq is not None and bk is not None and bq.data_ptr() != bk.data_ptr():     # one gain for both: autograd adds
         return bq, bk, True
     return *(torch.empty(x.shape[-1], dtype=torch.float32, device=x.device) for _ in range(2)), False
 

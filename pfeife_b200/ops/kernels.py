@@ -551,6 +551,7 @@ def heads_bwd(gq: torch.Tensor, gk: torch.Tensor, gv: Optional[torch.Tensor], q:
         assert w.shape == (D,)
     for w in (dwq, dwk):
         assert w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() == D)
+    assert dwq is None or dwk is None or dwq.data_ptr() != dwk.data_ptr()
     sms, Hk = sm_count(q.device), k.shape[2]
     scratch = None
     if dwq is not None or dwk is not None:
@@ -568,6 +569,14 @@ def _token_rows(logits: torch.Tensor, labels: torch.Tensor):
     return logits if logits.stride(2) == 1 or logits.shape[2] == 1 else logits.contiguous(), labels.long().contiguous()
 
 
+def _loss_scratch(L, z: torch.Tensor) -> torch.Tensor:
+    N, T, V = z.shape
+    n = L.pf_token_loss_scratch(N, T, V, dt(z.dtype), sm_count(z.device))
+    if n < 0:
+        check(n, "pf_token_loss_scratch")
+    return torch.empty(n, dtype=torch.float64, device=z.device)
+
+
 def preference_fwd(logits: torch.Tensor, labels: torch.Tensor, ref: torch.Tensor, beta: float, smoothing: float,
                    ignore_index: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """-> (loss, rewards [N], stats [N, T, 2], coef [N]), all fp32; stats and coef are for ``token_loss_bwd``."""
@@ -577,7 +586,7 @@ def preference_fwd(logits: torch.Tensor, labels: torch.Tensor, ref: torch.Tensor
     assert N >= 2 and N % 2 == 0 and ref.shape == (N,) and ref.device == z.device
     new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=z.device)
     loss, rewards, stats, coef = new(), new(N), new(N, T, 2), new(N)
-    scratch = torch.empty(L.pf_token_loss_scratch(N, T), dtype=torch.float64, device=z.device)
+    scratch = _loss_scratch(L, z)
     check(L.pf_preference_fwd(z, labels, _floats(ref), loss, rewards, stats, coef, scratch, N, T, V, z.stride(0),
                               z.stride(1), ignore_index, beta, smoothing, dt(z.dtype), sm_count(z.device),
                               stream_of(z)), "pf_preference_fwd")
@@ -597,7 +606,7 @@ def policy_fwd(logits: torch.Tensor, actions: torch.Tensor, old: torch.Tensor, a
     new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=z.device)
     loss, kl, clipped, inv = new(), new(), new(), new()
     logps, coef, stats = new(N, T), new(N, T), new(N, T, 2)
-    scratch = torch.empty(L.pf_token_loss_scratch(N, T), dtype=torch.float64, device=z.device)
+    scratch = _loss_scratch(L, z)
     check(L.pf_policy_fwd(z, actions, _floats(old), None if ref is None else _floats(ref), adv, loss, kl, clipped,
                           inv, logps, coef, stats, scratch, N, T, V, z.stride(0), z.stride(1), adv.stride(0),
                           adv.stride(1), ignore_index, low, high, kl_coef, 1.0 / temperature, dt(z.dtype),

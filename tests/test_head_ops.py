@@ -433,6 +433,25 @@ def test_registered_gains_and_bits_that_repeat():
 
 
 @pytest.mark.gpu
+def test_one_registered_gain_for_queries_and_keys():
+    """Both sums reach the one gradient, neither overtaken by the other."""
+    cos, sin = angles(300, 32, "cuda")
+    q, k = (heads(2, 300, h, 64, "cuda", torch.bfloat16, h) for h in (8, 4))
+    w = torch.rand(64, device="cuda").requires_grad_()
+    def grad():
+        out = ops.qk_norm_rope(q, k, w, w, cos, sin)
+        return torch.autograd.grad(out, w, [q, k])[0]
+    want = grad()
+    bucket = torch.zeros(64, device="cuda")
+    try:
+        ops.register_param(w, None, bucket)
+        got = [grad() for _ in range(3)]
+    finally:
+        ops.unregister_params()
+    assert not bucket.any() and all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens,heads_q", [(1, 1), (3, 2), (131072, 1), (4097, 33)])
 def test_many_tokens_and_many_heads(tokens, heads_q):
     """Every item of the grid and of the backward's walks, one CTA to many."""
@@ -490,3 +509,109 @@ def test_ops_are_seen_by_tracers_and_modes(device):
     assert torch.equal(torch.autograd.grad(got, qkv, g)[0], torch.autograd.grad(want, qkv, g)[0])
     gm = torch.fx.symbolic_trace(lambda t: ops.rope(t, cos, sin, pos, True))
     assert torch.equal(gm(x), ops.rope(x, cos, sin, pos, True))
+
+
+# ------------------------------------------------------------------------------ calls that do not go the usual way
+class Watch(torch.utils._python_dispatch.TorchDispatchMode):
+    """Lets every op be seen, which keeps all calls on the dispatcher."""
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+def _functions(device):
+    """name -> (function of the leaves, leaves)"""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    cos, sin = angles(16, 8, device)
+    pos = torch.randint(0, 16, (2, 16), generator=torch.Generator().manual_seed(1)).to(device)
+    new = lambda h, seed: heads(2, 16, h, 16, device, dtype, seed)
+    gain = lambda seed: (torch.rand(16, generator=torch.Generator().manual_seed(seed)) + 0.5).to(device)
+    return {
+        "rope": (lambda x: ops.rope(x, cos, sin, pos), [new(3, 1)]),
+        "interleaved": (lambda x: ops.rope(x, cos, sin, interleaved=True), [new(3, 1)]),
+        "partial": (lambda x: ops.rope(x, cos[:, :3].contiguous(), sin[:, :3].contiguous()), [new(3, 1)]),
+        "rope_qkv": (lambda x: ops.rope_qkv(x, cos, sin, pos, True), [new(6, 1).view(2, 16, 3, 2, 16)]),
+        "qk_norm_rope": (lambda q, k, a, b: torch.cat(ops.qk_norm_rope(q, k, a, b, cos, sin, 1e-5, pos), 2),
+                         [new(4, 1), new(2, 2), gain(1), gain(2)]),
+        "qk_norm_rope_qkv": (lambda x, a, b: ops.qk_norm_rope_qkv(x, a, b, cos, sin, 1e-5, pos, True),
+                             [new(6, 1).view(2, 16, 3, 2, 16), gain(1), gain(2)]),
+    }
+
+
+NAMES = ["rope", "interleaved", "partial", "rope_qkv", "qk_norm_rope", "qk_norm_rope_qkv"]
+
+
+@pytest.fixture(params=DEVICES)
+def direct_device(request, monkeypatch):
+    """On the CPU the direct way is switched on too."""
+    from pfeife_b200.ops import functional
+    monkeypatch.setattr(functional, "_FIRST_DEVICE", -1 if request.param == "cpu" else 0)
+    return request.param
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_direct_calls_and_the_dispatcher_agree(name, direct_device):
+    fn, leaves = _functions(direct_device)[name]
+    leaves = [t.requires_grad_() for t in leaves]
+    y = fn(*leaves)
+    g = torch.randn(y.shape, generator=torch.Generator().manual_seed(3)).to(y)
+    want = torch.autograd.grad(y, leaves, g, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, g), want))     # a second time
+    with Watch():
+        seen = fn(*leaves)
+        got = torch.autograd.grad(seen, leaves, g)
+    assert torch.equal(y, seen) and all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.no_grad():
+        assert torch.equal(fn(*leaves), y) and not fn(*leaves).requires_grad
+    y = fn(*leaves)
+    y.mul_(2.0)                                    # no view to autograd: may be changed in place
+    for a, b in zip(torch.autograd.grad(y, leaves, g / 2), want):
+        assert torch.allclose(a, b, rtol=2e-2, atol=2e-2)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_saved_tensors_of_other_types_and_orders(name, direct_device):
+    """Hooks on saved tensors may return any tensor of the same values."""
+    fn, leaves = _functions(direct_device)[name]
+    leaves = [t.requires_grad_() for t in leaves]
+    y = fn(*leaves)
+    g = torch.ones_like(y)
+    want = torch.autograd.grad(y, leaves, g)
+
+    def unpack(t):
+        if t.is_floating_point():                  # every second element of a wider tensor, or 64 bits
+            return torch.stack([t, t], -1)[..., 0] if t.dim() > 1 else t.double()
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = fn(*leaves)
+    for a, b in zip(torch.autograd.grad(y, leaves, g), want):
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-6)
+    from torch.utils.checkpoint import checkpoint
+    y = checkpoint(fn, *leaves, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, g), want))
+
+
+def test_entry_points_refuse_what_they_cannot_read():
+    """Before anything touches a device."""
+    import ctypes
+    from pfeife_b200.csrc import build
+    from pfeife_b200.ops import _lib
+    if not build.KERNEL_LIB.exists():
+        pytest.skip("the kernel library is not built")
+    calls = _lib.load_calls(ctypes.CDLL(str(build.KERNEL_LIB), mode=ctypes.RTLD_GLOBAL))
+    t = torch.zeros(64).data_ptr()
+    z = (64, 64, 16)
+
+    def fwd(q=t, B=1, S=1, Hq=1, Hk=0, D=16, R=16, cos=t, pos=None, dtype=2):
+        return calls.pf_heads_fwd(q, None, None, t, None, None, None, None, cos, t, pos, B, S, Hq, Hk, D, R, z, None,
+                                  z, None, (0, 1), 1, 0, 0, 1e-6, dtype, 148, None)
+    assert fwd(dtype=5) == -1
+    for bad in (dict(D=257), dict(D=300, R=300), dict(R=17), dict(R=18), dict(R=0), dict(D=0), dict(S=1 << 30, B=4),
+                dict(S=1 << 24, Hq=256)):
+        assert fwd(**bad) == -3, bad
+    for bad in (dict(q=t + 1), dict(cos=t + 2), dict(pos=t + 4), dict(q=t + 2, dtype=0)):
+        assert fwd(**bad) == -2, bad
+    for empty in (dict(B=0), dict(S=0), dict(Hq=0)):
+        assert fwd(**empty) == 0, empty
+    assert calls.pf_heads_bwd_rows(32, 8, 148) >= 2 * 148

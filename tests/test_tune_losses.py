@@ -290,7 +290,8 @@ def test_refusals(device):
             ops.preference_loss(**{**dict(logits=z, labels=labels, ref_logps=ref), **bad})
     for bad in (dict(logits=z[0, 0], actions=labels[0, 0]), dict(actions=labels[:, :2]), dict(old_logps=v[:1]),
                 dict(ref_logps=v[:, :1]), dict(advantages=v[:, :2]), dict(advantages=ref), dict(temperature=0.0),
-                dict(temperature=-1.0), dict(clip_low=1.5), dict(clip_high=-0.1), dict(old_logps=v.to(other)),
+                dict(temperature=-1.0), dict(temperature=math.inf), dict(temperature=math.nan), dict(clip_high=math.nan),
+                dict(clip_low=1.5), dict(clip_high=-0.1), dict(old_logps=v.to(other)),
                 dict(advantages=v.clone().requires_grad_()), dict(actions=v)):
         with pytest.raises(ValueError):
             ops.policy_loss(**{**dict(logits=z, actions=labels, old_logps=v, advantages=v), **bad})
@@ -389,6 +390,79 @@ def test_ops_are_seen_by_tracers_and_modes(device):
     got = torch.compile(fn, backend="eager", fullgraph=True)(z)
     assert torch.equal(got, want)
     assert torch.equal(torch.autograd.grad(got, z)[0], torch.autograd.grad(want, z)[0])
+
+
+# ------------------------------------------------------------------------------ calls that do not go the usual way
+class Watch(torch.utils._python_dispatch.TorchDispatchMode):
+    """Lets every op be seen, which keeps all calls on the dispatcher."""
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("loss", ["preference", "policy"])
+def test_direct_calls_and_the_dispatcher_agree(loss, device, monkeypatch):
+    from pfeife_b200.ops import functional
+    monkeypatch.setattr(functional, "_FIRST_DEVICE", -1 if device == "cpu" else 0)
+    z, labels = batch(4, 7, 300, device, torch.float32 if device == "cpu" else torch.bfloat16, 3)
+    z.requires_grad_()
+    v = torch.full((4, 7), -5.0, device=device)
+
+    def fn(t):
+        if loss == "preference":
+            return ops.preference_loss(t, labels, v[:, 0], 0.3, 0.1)
+        return ops.policy_loss(t, labels, v, v[:, :1] + 6, v + 1, kl_coef=0.2, temperature=1.3)
+
+    out = fn(z)
+    g = torch.tensor(3.0, device=device)
+    (want,) = torch.autograd.grad(out.loss, z, g, retain_graph=True)
+    assert torch.equal(torch.autograd.grad(out.loss, z, g)[0], want)
+    with Watch():
+        seen = fn(z)
+        (got,) = torch.autograd.grad(seen.loss, z, g)
+    assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(out, seen))
+    with torch.no_grad():
+        assert all(torch.equal(a, b) and not b.requires_grad for a, b in zip(out, fn(z)))
+
+    def unpack(t):                                 # every second element of a wider tensor, or another type
+        return torch.stack([t, t], -1)[..., 0] if t.dim() != 1 else t.double() if t.is_floating_point() else t
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        hooked = fn(z).loss
+    assert torch.equal(torch.autograd.grad(hooked, z, g)[0], want)
+    from torch.utils.checkpoint import checkpoint
+    again = checkpoint(lambda t: fn(t).loss, z, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(again, z, g)[0], want)
+    # the other outputs are constants
+    assert not any(t.requires_grad for t in fn(z)[1:])
+
+
+def test_entry_points_refuse_what_they_cannot_read():
+    """Before anything touches a device."""
+    import ctypes
+    from pfeife_b200.csrc import build
+    from pfeife_b200.ops import _lib
+    if not build.KERNEL_LIB.exists():
+        pytest.skip("the kernel library is not built")
+    calls = _lib.load_calls(ctypes.CDLL(str(build.KERNEL_LIB), mode=ctypes.RTLD_GLOBAL))
+    t = torch.zeros(64).data_ptr()
+
+    def preference(z=t, N=2, T=1, V=4, dtype=2):
+        return calls.pf_preference_fwd(z, t, t, t, t, t, t, t, N, T, V, 4, 4, -100, 0.1, 0.0, dtype, 148, None)
+
+    def policy(z=t, N=2, T=1, V=4, dtype=2):
+        return calls.pf_policy_fwd(z, t, t, None, t, t, t, t, t, t, t, t, t, N, T, V, 4, 4, 1, 0, -100, 0.2, 0.2, 0.0,
+                                   1.0, dtype, 148, None)
+
+    def backward(z=t, N=2, T=1, V=4, dtype=2):
+        return calls.pf_token_loss_bwd(z, t, t, t, t, None, t, N, T, V, 4, 4, -100, 1, 1.0, dtype, 148, None)
+    for call in (preference, policy, backward):
+        assert call(dtype=3) == -1 and call(z=t + 1) == -2 and call(z=t + 2, dtype=0) == -2
+        assert call(V=0) == -3 and call(N=1 << 20, T=1 << 20) == -3 and call(N=-2) == -3
+    assert preference(N=3) == -3 and preference(N=0) == -3 and backward(T=0) == 0
+    # more parts of a row only where rows are few, and room for each
+    few, many = (calls.pf_token_loss_scratch(1, n, 32000, 2, 148) for n in (16, 16384))
+    assert few >= 16 * 8 + 8 and many < 4 * 16384
 
 
 # ------------------------------------------------------------------------------ together
