@@ -123,9 +123,9 @@ PF_DECL int pf_policy_fwd(const void* logits, const void* actions, const void* o
                           float inv_temperature, int dtype, int sm_count, void* stream);
 PF_DECL int pf_token_loss_bwd(const void* logits, const void* labels, const void* stats,
                               const void* coef, const void* gout, const void* inv, void* dlogits,
-                              long long N, int T, int V, long long n, long long t,
-                              long long ignore_index, int per, float inv_temperature, int dtype,
-                              int sm_count, void* stream);
+                              long long dlogits_row, long long N, int T, int V, long long n,
+                              long long t, long long ignore_index, int per, float inv_temperature,
+                              int dtype, int sm_count, void* stream);
 
 // ---- attn_sm100.cu : flash attention on tcgen05 (strides in elements: batch, seq, head)
 PF_DECL int pf_attn_fwd(const void* q, const void* k, const void* v, void* o, void* lse, int B,

@@ -865,6 +865,17 @@ struct Kept {
   float* coef() const { return float_at(all, 2 * rows); }
   float* one_over() const { return inv ? float_at(all, 2 * rows + n) : nullptr; }
 };
+// An empty [N, T, V] whose rows lie to 16 bytes as those of the logits do, so that the backward goes through both by
+// vectors: packed, or (some words of a padded vocabulary) with as much space between rows.
+Tensor rows_like(const Tensor& z) {
+  const int64_t N = z.size(0), T = z.size(1), V = z.size(2), size = z.element_size(), per = 16 / size;
+  const int64_t row = T > 1 ? z.stride(1) : V;
+  const int64_t off = (int64_t)(reinterpret_cast<uintptr_t>(z.data_ptr()) % 16) / size;
+  if ((off == 0 && row % per == V % per) || row < V || row > V + 1024 ||
+      (N > 1 && (z.stride(0) - T * row) % per))
+    return empty(z.sizes(), z);
+  return empty({off + N * T * row}, z).as_strided({N, T, V}, {T * row, row, 1}, off);
+}
 variable_list token_loss_backward(AutogradContext* ctx, const Tensor& g, int inputs) {
   variable_list out(inputs);
   if (!g.defined()) return out;
@@ -879,9 +890,9 @@ variable_list token_loss_backward(AutogradContext* ctx, const Tensor& g, int inp
       aligned(kept.all) && packed_floats(g, 1)) {
     below([&] {
       const Env e(z);
-      out[0] = empty(z.sizes(), z);
+      out[0] = rows_like(z);
       ok(pf_token_loss_bwd(z.data_ptr(), labels.data_ptr(), kept.stats(), kept.coef(), g.data_ptr(), kept.one_over(),
-                           out[0].data_ptr(), N, (int)T, (int)z.size(2), z.stride(0), z.stride(1), ignore,
+                           out[0].data_ptr(), out[0].size(1) > 1 ? out[0].stride(1) : out[0].size(2), N, (int)T, (int)z.size(2), z.stride(0), z.stride(1), ignore,
                            inv ? 1 : (int)T, (float)(1.0 / temperature), code_of(z), e.sms, e.stream),
          "pf_token_loss_bwd");
       return 0;

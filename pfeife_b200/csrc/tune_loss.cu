@@ -372,14 +372,15 @@ preference_tail_kernel(const Logits z, const Rows rows, const float* __restrict_
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(256)
 row_bwd_kernel(const Logits z, const float2* __restrict__ stats, const float* __restrict__ coef,
-               const float* __restrict__ gout, const float* __restrict__ inv, T* __restrict__ dz, int per) {
+               const float* __restrict__ gout, const float* __restrict__ inv, T* __restrict__ dz, int per,
+               long long dz_row) {
   after_previous();
   constexpr int VN = 16 / sizeof(T), UNROLL = THREADS < 128 ? 1 : THREADS < 256 ? 2 : 4;
   // the last rows first: the forward has read them last, and what L2 still holds of them is read from there
   const long long row = z.rows - 1 - ((long long)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS);
   if (row < 0) return;
   const T* x = static_cast<const T*>(z.at) + z.row(row);
-  T* d = dz + row * z.V;
+  T* d = dz + row * dz_row;
   const long long label = z.labels[row];
   const bool counted = z.counts(label);
   const float g = counted ? coef[row / per] * gout[0] * (inv ? inv[0] : 1.f) : 0.f;
@@ -544,15 +545,18 @@ PF_API int pf_policy_fwd(const void* logits, const void* actions, const void* ol
   return 0;
 }
 
-// dlogits [N, T, V] packed.  coef: one value for `per` rows; gout: the loss's gradient; inv may be null.
+// dlogits: rows of V values, dlogits_row apart.  coef: one value for `per` rows; gout: the loss's gradient; inv may
+// be null.  Rows that lie to 16 bytes as the logits' do are written by vectors, others element by element.
 PF_API int pf_token_loss_bwd(const void* logits, const void* labels, const void* stats, const void* coef,
-                             const void* gout, const void* inv, void* dlogits, long long N, int T, int V,
-                             long long n, long long t, long long ignore_index, int per, float inv_temperature,
+                             const void* gout, const void* inv, void* dlogits, long long dlogits_row,
+                             long long N, int T, int V, long long n, long long t, long long ignore_index, int per, float inv_temperature,
                              int dtype, int sm_count, void* stream) {
   Logits z;
   const int code = logits_of(z, logits, labels, N, T, V, n, t, ignore_index, inv_temperature, dtype);
   if (code) return code;
   if (z.rows == 0) return 0;
+  if (dlogits_row < V) return -3;
+  if (reinterpret_cast<uintptr_t>(dlogits) % (dtype == PF_F32 ? 4 : 2)) return -2;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   long long slabs = 8ll * sm_count / z.rows;
   const long long most = (V + 2047) / 2048;
@@ -560,7 +564,8 @@ PF_API int pf_token_loss_bwd(const void* logits, const void* labels, const void*
   if (slabs < 1) slabs = 1;
 #define PF_BWD(THREADS, GRID)                                                                             \
   after(row_bwd_kernel<T, THREADS>, GRID, 256, 0, st)(z, (const float2*)stats, (const float*)coef,         \
-                                                      (const float*)gout, (const float*)inv, (T*)dlogits, per)
+                                                      (const float*)gout, (const float*)inv, (T*)dlogits, per,  \
+                                                      dlogits_row)
   PF_DISPATCH3(dtype, {
     if (V / (16 / (int)sizeof(T)) <= 64) PF_BWD(32, (unsigned)((z.rows + 7) / 8));
     else PF_BWD(256, dim3((unsigned)z.rows, (unsigned)slabs));

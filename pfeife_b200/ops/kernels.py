@@ -624,7 +624,7 @@ def token_loss_bwd(gout: torch.Tensor, logits: torch.Tensor, labels: torch.Tenso
     assert gout.numel() == 1 and stats.numel() == 2 * N * T and coef.numel() in (N, N * T)
     d = torch.empty((N, T, V), dtype=z.dtype, device=z.device)
     check(L.pf_token_loss_bwd(z, labels, _vectors(_floats(stats)), _floats(coef), _floats(gout),
-                              None if inv is None else _floats(inv), d, N, T, V, z.stride(0), z.stride(1),
+                              None if inv is None else _floats(inv), d, V, N, T, V, z.stride(0), z.stride(1),
                               ignore_index, 1 if coef.numel() == N * T else T, 1.0 / temperature, dt(z.dtype),
                               sm_count(z.device), stream_of(z)), "pf_token_loss_bwd")
     return d

@@ -298,6 +298,27 @@ def test_refusals(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("pad,off", [(0, 0), (5, 0), (61, 3), (2000, 1), (3, 3)])
+@pytest.mark.parametrize("V", [259, 4099])
+def test_some_words_of_a_padded_vocabulary(pad, off, V):
+    """The gradient of rows with space between them has the same values wherever it lies."""
+    g = torch.Generator().manual_seed(V)
+    wide = torch.randn(2, 5, V + pad + off, generator=g).cuda().half()
+    labels = torch.randint(0, V, (2, 5), generator=g).cuda()
+    labels[0, 2] = -100
+    z = wide[..., off:off + V].detach().requires_grad_()
+    packed = z.detach().clone().requires_grad_()
+    def grad(t):
+        return torch.autograd.grad(ops.preference_loss(t, labels, torch.zeros(2, device="cuda")).loss, t)[0]
+    a, b = grad(z), grad(packed)
+    assert a.shape == b.shape and torch.equal(a, b) and not a[0, 2].any()
+    whole = wide.requires_grad_()                  # and reaches the whole of it
+    (c,) = torch.autograd.grad(ops.preference_loss(whole[..., off:off + V], labels, torch.zeros(2, device="cuda")).loss,
+                               whole)
+    assert torch.equal(c[..., off:off + V], b) and not c[..., :off].any() and not c[..., off + V:].any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,V", [(70001, 33), (9000, 1500)])
 def test_many_rows(rows, V):
     z, labels = batch(1, rows, V, "cuda", torch.bfloat16, 1)
@@ -454,12 +475,12 @@ def test_entry_points_refuse_what_they_cannot_read():
         return calls.pf_policy_fwd(z, t, t, None, t, t, t, t, t, t, t, t, t, N, T, V, 4, 4, 1, 0, -100, 0.2, 0.2, 0.0,
                                    1.0, dtype, 148, None)
 
-    def backward(z=t, N=2, T=1, V=4, dtype=2):
-        return calls.pf_token_loss_bwd(z, t, t, t, t, None, t, N, T, V, 4, 4, -100, 1, 1.0, dtype, 148, None)
+    def backward(z=t, N=2, T=1, V=4, dtype=2, row=4):
+        return calls.pf_token_loss_bwd(z, t, t, t, t, None, t, row, N, T, V, 4, 4, -100, 1, 1.0, dtype, 148, None)
     for call in (preference, policy, backward):
         assert call(dtype=3) == -1 and call(z=t + 1) == -2 and call(z=t + 2, dtype=0) == -2
         assert call(V=0) == -3 and call(N=1 << 20, T=1 << 20) == -3 and call(N=-2) == -3
-    assert preference(N=3) == -3 and preference(N=0) == -3 and backward(T=0) == 0
+    assert preference(N=3) == -3 and preference(N=0) == -3 and backward(T=0) == 0 and backward(row=3) == -3
     # more parts of a row only where rows are few, and room for each
     few, many = (calls.pf_token_loss_scratch(1, n, 32000, 2, 148) for n in (16, 16384))
     assert few >= 16 * 8 + 8 and many < 4 * 16384
