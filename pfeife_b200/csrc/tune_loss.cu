@@ -65,8 +65,8 @@ __device__ __forceinline__ void part_merge(float& m, float& s, float m2, float s
 // 16 bytes of a row: its largest value, and its values two by two in fp32.  16-bit maxima are taken two at a time
 // before anything is widened, as fp32 sums and products are: ten instructions a value became six.  What is left are
 // the loads: without its exponentials, 16 a cycle and SM, the pass takes 38 us for 41 (2797 of 4096 rows of 32000
-// bf16; 27 at the copy rate).  More in flight does not help: batches of 8 vectors, the next one in registers or
-// several in shared memory take 42, 42 and 54.
+// bf16; 27 at the copy rate).  Batches of 4 vectors and twelve CTAs an SM take 41 too, the next batch in registers
+// 42 and several in shared memory 54.
 template <typename T> struct Words;
 template <> struct Words<float> {
   static constexpr int PAIRS = 2;
@@ -120,20 +120,22 @@ template <> struct Words<__nv_bfloat16> {
   }
 };
 
-constexpr int ROW_BATCH = 4;       // vectors that a thread takes at a time
-constexpr int ROW_THREADS = 128;   // of a part of a row, and twelve such parts an SM
-constexpr int ROW_WARP = 1024;     // a row up to here is a warp's
+constexpr int ROW_BATCH = 8;       // vectors that a thread of a CTA takes at a time
+constexpr int ROW_THREADS = 128;   // of a part of a row
+constexpr int ROW_CTAS = 8;        // such CTAs an SM
+
+template <bool B> struct Flag { static constexpr bool value = B; };
 
 // One pass over each row that counts: M and s of its gridDim.y parts, and the label's logit to `at_label`.  THREADS
-// threads a part: CTAs of their own, or warps (of whole rows) that share one of 256.
+// threads a part: CTAs of their own, or 8 or 32 lanes (of whole rows) that share one of 256.
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS < 64 ? 256 : THREADS, THREADS == ROW_THREADS ? 12 : 1)
+__global__ void __launch_bounds__(THREADS < 64 ? 256 : THREADS, THREADS == ROW_THREADS ? ROW_CTAS : 1)
 row_fwd_kernel(const Logits z, float2* __restrict__ parts, float* __restrict__ at_label) {
   after_previous();
-  constexpr int W = THREADS / 32, VN = 16 / sizeof(T), U = ROW_BATCH;
-  constexpr int ROWS = W > 1 ? 1 : 8;
-  __shared__ float smax[W], ssum[W];
-  const long long row = (long long)blockIdx.x * ROWS + (W > 1 ? 0 : threadIdx.x / 32);
+  constexpr int W = THREADS / 32, VN = 16 / sizeof(T), U = W > 1 ? ROW_BATCH : 4;
+  constexpr int ROWS = W > 1 ? 1 : 256 / THREADS;
+  __shared__ float smax[W > 1 ? W : 1], ssum[W > 1 ? W : 1];
+  const long long row = (long long)blockIdx.x * ROWS + (W > 1 ? 0 : threadIdx.x / THREADS);
   if (row >= z.rows) return;
   const int tid = threadIdx.x % THREADS;
   const long long label = z.labels[row];
@@ -147,14 +149,15 @@ row_fwd_kernel(const Logits z, float2* __restrict__ parts, float* __restrict__ a
   float m = -INFINITY, s = 0.f;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   const uint64_t k2 = f2_pack(k, k);
-  auto take = [&](uint4 (&q)[U], int i0, int end) {  // -inf behind the part's end, which adds nothing
+  // A batch of vectors from i0 on, all before `end` or some.
+  auto add = [&](auto whole, int i0, int end) {
+    constexpr bool ALL = decltype(whole)::value;
+    uint4 q[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      q[u] = Words<T>::none();
-      if (i0 + u * THREADS < end) q[u] = __ldg(xv + i0 + u * THREADS);
+    for (int u = 0; u < U; ++u) {                    // -inf behind the end, which adds nothing
+      if (!ALL) q[u] = Words<T>::none();
+      if (ALL || i0 + u * THREADS < end) q[u] = __ldg(xv + i0 + u * THREADS);
     }
-  };
-  auto add = [&](const uint4 (&q)[U]) {
     // a NaN does not move the maximum but reaches the sum below; parts that are -inf so far subtract 0, which
     // leaves their exponentials at zero
     const float mm = fmaxf(m, ceilf(Words<T>::most(q) * k) + fraction), sub = mm == -INFINITY ? 0.f : mm;
@@ -163,23 +166,22 @@ row_fwd_kernel(const Logits z, float2* __restrict__ parts, float* __restrict__ a
     uint64_t sums[2] = {0, 0};                       // two zeros each
 #pragma unroll
     for (int u = 0; u < U; ++u)
+      if (ALL || i0 + u * THREADS < end)
 #pragma unroll
-      for (int j = 0; j < Words<T>::PAIRS; ++j) {
-        float a, b;
-        f2_unpack(fma2(Words<T>::pair(q[u], j), k2, minus2), a, b);
-        sums[j & 1] = add2(sums[j & 1], f2_pack(exp2_fast(a), exp2_fast(b)));
-      }
+        for (int j = 0; j < Words<T>::PAIRS; ++j) {
+          float a, b;
+          f2_unpack(fma2(Words<T>::pair(q[u], j), k2, minus2), a, b);
+          sums[j & 1] = add2(sums[j & 1], f2_pack(exp2_fast(a), exp2_fast(b)));
+        }
     float a, b;
     f2_unpack(add2(sums[0], sums[1]), a, b);
     s += a + b;
     m = mm;
   };
-  uint4 q[U];
   const int begin = (int)((long long)nvec * part / n_parts), end = (int)((long long)nvec * (part + 1) / n_parts);
-  for (int i0 = begin + tid; i0 < end; i0 += U * THREADS) {
-    take(q, i0, end);
-    add(q);
-  }
+  int i0 = begin + tid;
+  for (; i0 + (U - 1) * THREADS < end; i0 += U * THREADS) add(Flag<true>{}, i0, end);
+  if (i0 < end) add(Flag<false>{}, i0, end);
   // the elements before the first and after the last vector (at most 2 (VN - 1))
   for (int i = tid; part == 0 && i < z.V - nvec * VN; i += THREADS) {
     const float v = to_f32<T>(x[i < head ? i : nvec * VN + i]);
@@ -192,9 +194,11 @@ row_fwd_kernel(const Logits z, float2* __restrict__ parts, float* __restrict__ a
     s *= down == fraction - 1.f ? FRACTION_SCALE[threadIdx.x & 31] : exp2f(down);
     m = whole;
   }
+  // the lanes of a row; others of the warp may have left, or have more to add
+  const unsigned lanes = THREADS >= 32 ? 0xffffffffu : ((1u << (THREADS & 31)) - 1) << (threadIdx.x & 31 & ~(THREADS - 1));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    part_merge(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+  for (int o = (THREADS < 32 ? THREADS : 32) / 2; o > 0; o >>= 1)
+    part_merge(m, s, __shfl_xor_sync(lanes, m, o), __shfl_xor_sync(lanes, s, o));
   if (W > 1) {
     const int w = tid >> 5, l = tid & 31;
     if (l == 0) { smax[w] = m; ssum[w] = s; }
@@ -214,7 +218,10 @@ row_fwd_kernel(const Logits z, float2* __restrict__ parts, float* __restrict__ a
 
 // What follows is one launch: a cluster of CTAs shares the rows, leaves sums in `scratch`, and the first CTA joins
 // them in their order.  (A thread of each row's CTA doing its row's part kept that CTA: 48 us for 42 with the pass.)
-constexpr int TAIL_THREADS = 512, TAIL_CTAS = 8, TAIL_ONE = 512;
+// Beyond some thousand rows the 64-bit arithmetic of a row each takes longer than another launch: CTAs that are no
+// cluster, and one that joins (65536 rows of 256: 38 -> 18 us with the pass).
+constexpr int TAIL_THREADS = 512, TAIL_CTAS = 8, TAIL_ONE = 512, TAIL_MANY = 8192, TAIL_MOST = 296;
+enum { WHOLE, SHARE, JOIN };       // one launch, or the first and the second of two
 // What the forward's pass over the rows has left: joined for the backward, and a row's log-probability.
 struct Rows {
   const float2* parts;             // [rows][n_parts]
@@ -247,13 +254,14 @@ struct PolicyArgs {
   float *logp, *coef;              // coef: of the row's own term, before the mean
   float *loss, *mean_kl, *clipped, *inv;
 };
+template <int STEP>
 __global__ void __launch_bounds__(TAIL_THREADS)
-policy_tail_kernel(const Logits z, const Rows rows, const PolicyArgs p, double* __restrict__ scratch) {
+policy_tail_kernel(const Logits z, const Rows rows, const PolicyArgs p, double* __restrict__ scratch, int ctas) {
   after_previous();
   __shared__ double part[4][TAIL_THREADS / 32];
   double sums[4] = {};                               // terms, KL, clipped, counted
-  for (long long r = (long long)blockIdx.x * TAIL_THREADS + threadIdx.x; r < z.rows;
-       r += (long long)gridDim.x * TAIL_THREADS) {
+  for (long long r = (long long)blockIdx.x * TAIL_THREADS + threadIdx.x; STEP != JOIN && r < z.rows;
+       r += (long long)ctas * TAIL_THREADS) {
     // all at once, whether the row counts (its statistics are written only then) or not
     const long long n = r / z.T, label = z.labels[r];
     const float2 stat = rows.join(r);
@@ -279,43 +287,49 @@ policy_tail_kernel(const Logits z, const Rows rows, const PolicyArgs p, double* 
     p.coef[r] = (float)(c * p.inv_temperature);
     sums[0] += term; sums[1] += each; sums[2] += clipped ? 1.0 : 0.0; sums[3] += 1.0;
   }
-  const int warp = threadIdx.x >> 5;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  double total = 0.0;                                // threads 0 to 3: of the CTA, then of all
+  if (STEP != JOIN) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    sums[i] = warp_sum64(sums[i]);
-    if ((threadIdx.x & 31) == 0) part[i][warp] = sums[i];
-  }
-  __syncthreads();
-  if (threadIdx.x < 4) {
-    double t = 0.0;
-    for (int w = 0; w < TAIL_THREADS / 32; ++w) t += part[threadIdx.x][w];
-    scratch[blockIdx.x * 4 + threadIdx.x] = t;
-  }
-  __syncwarp();
-  if (gridDim.x > 1) cluster_sync();
-  else __syncthreads();
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    double t[4] = {};
-    for (unsigned c = 0; c < gridDim.x; ++c)
+    for (int i = 0; i < 4; ++i) {
+      sums[i] = warp_sum64(sums[i]);
+      if (lane == 0) part[i][warp] = sums[i];
+    }
+    __syncthreads();
+    if (threadIdx.x < 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) t[i] += __ldcg(scratch + c * 4 + i);
-    const double one = 1.0 / (t[3] > 0.0 ? t[3] : 1.0);
-    *p.loss = (float)(t[0] * one);
-    *p.mean_kl = (float)(t[1] * one);
-    *p.clipped = (float)(t[2] * one);
-    *p.inv = (float)one;
+      for (int w = 0; w < TAIL_THREADS / 32; ++w) total += part[threadIdx.x][w];
+      if (ctas > 1) scratch[blockIdx.x * 4 + threadIdx.x] = total;
+    }
+    __syncwarp();
+    if (STEP == SHARE) return;
+    if (ctas > 1) cluster_sync();
   }
+  if (blockIdx.x > 0 || warp > 0) return;
+  if (ctas > 1) {                                    // eight lanes for each sum
+    total = 0.0;
+    for (int c = lane >> 2; c < ctas; c += 8) total += __ldcg(scratch + c * 4 + (lane & 3));
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  }
+  const double count = __shfl_sync(0xffffffffu, total, 3), one = 1.0 / (count > 0.0 ? count : 1.0);
+  float* const to[4] = {p.loss, p.mean_kl, p.clipped, p.inv};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane == i) *to[i] = (float)(i == 3 ? one : total * one);
 }
 
 // Rewards of the sequences, the mean loss over the pairs and what a sequence's log-probability gets of it.  Warps
 // share the sequences; where there are more warps than sequences, several sum parts of one.
+template <int STEP>
 __global__ void __launch_bounds__(TAIL_THREADS)
-preference_tail_kernel(const Logits z, const Rows rows, const float* __restrict__ ref, float* __restrict__ rewards, float* __restrict__ loss,
-                       float* __restrict__ coef, double* __restrict__ scratch, int N, float beta, float smoothing) {
+preference_tail_kernel(const Logits z, const Rows rows, const float* __restrict__ ref, float* __restrict__ rewards,
+                       float* __restrict__ loss, float* __restrict__ coef, double* __restrict__ scratch, int N,
+                       float beta, float smoothing, int ctas) {
   after_previous();
-  const int warps = gridDim.x * (TAIL_THREADS / 32), warp = blockIdx.x * (TAIL_THREADS / 32) + (threadIdx.x >> 5);
+  const int warps = ctas * (TAIL_THREADS / 32), warp = blockIdx.x * (TAIL_THREADS / 32) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, parts = max(1, min(warps / N, (z.T + 31) / 32)), items = N * parts;
-  for (int i = warp; i < items; i += warps) {
+  for (int i = warp; STEP != JOIN && i < items; i += warps) {
     const int n = i / parts, part = i - n * parts;
     double t = 0.0;
     for (long long j = part * 32 + lane; j < z.T; j += parts * 32) {
@@ -330,9 +344,12 @@ preference_tail_kernel(const Logits z, const Rows rows, const float* __restrict_
     t = warp_sum64(t);
     if (lane == 0) scratch[i] = t;
   }
+  if (STEP == SHARE) return;
   __syncwarp();
-  if (gridDim.x > 1) cluster_sync();
-  else __syncthreads();
+  if (STEP == WHOLE) {
+    if (ctas > 1) cluster_sync();
+    else __syncthreads();
+  }
   if (blockIdx.x > 0) return;
   __shared__ double shared[TAIL_THREADS / 32];
   auto reward = [&](int n) {
@@ -367,15 +384,15 @@ preference_tail_kernel(const Logits z, const Rows rows, const float* __restrict_
   }
 }
 
-// dz = g (onehot - p), g = coef[row / per] * gout * inv (inv null: 1).  THREADS threads a row; with 256 the grid is
-// (row, slab of the row).
+// dz = g (onehot - p), g = coef[row / per] * gout * inv (inv null: 1).  THREADS threads a row; where they are whole
+// CTAs the grid is (row, slab of the row).
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(256)
 row_bwd_kernel(const Logits z, const float2* __restrict__ stats, const float* __restrict__ coef,
                const float* __restrict__ gout, const float* __restrict__ inv, T* __restrict__ dz, int per,
                long long dz_row) {
   after_previous();
-  constexpr int VN = 16 / sizeof(T), UNROLL = THREADS < 128 ? 1 : THREADS < 256 ? 2 : 4;
+  constexpr int VN = 16 / sizeof(T), UNROLL = THREADS < 32 ? 2 : 4;
   // the last rows first: the forward has read them last, and what L2 still holds of them is read from there
   const long long row = z.rows - 1 - ((long long)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS);
   if (row < 0) return;
@@ -438,17 +455,39 @@ int logits_of(Logits& z, const void* at, const void* labels, long long N, int T,
   return 0;
 }
 
+// Lanes of a row in the forward, 0: CTAs.  What a short row costs beside its values is the same for all lanes that
+// it keeps, so many short rows get few (microseconds with 8, 32 lanes and CTAs of 128, with what follows, bf16:
+// 65536 rows of 256 18, 24 and 53; 16384 of 1000 16, 18 and 23; 16384 of 1500 to 2049 with 32 lanes 23 to 25 and
+// with CTAs 57 to 59; 16384 of 8192 54 and 69; 4096 of 16384 36 and 35).  Few rows take a warp each, or CTAs.
+int row_lanes(long long rows, int V, int sm_count) {
+  if (V <= 1024) return rows >= 32ll * sm_count ? 8 : 32;
+  return V <= 8192 && rows >= 16ll * sm_count ? 32 : 0;
+}
+// The same for the backward, by the vectors of a row (65536 rows of 256 bf16: 17 us with 8 lanes, 29 with 32; 16384
+// of 1500 24 with 32 lanes, 43 with CTAs of 256; 8192 of 4096 31 either way; 64 of 256 2.7 with 8 lanes, 2.1 with 32).
+int back_lanes(long long rows, int nvec, int sm_count) {
+  if (nvec <= 64) return rows >= 32ll * sm_count ? 8 : 32;
+  return nvec <= 256 && rows >= 4ll * sm_count ? 32 : 0;
+}
+
 // Parts of a row: enough for the CTAs that the SMs hold, and none of less than a batch (16 rows of 32000 fp32: 6.7 ->
-// 6.2 us; four times as many are slower by 1 to 3 us where rows fill the SMs as they are).
+// 5.7 us; four times as many are slower by 1 to 3 us where rows fill the SMs as they are).
 int row_parts(long long rows, int V, int dtype, int sm_count) {
   const int batch = ROW_THREADS * ROW_BATCH * (dtype == PF_F32 ? 4 : 8);
-  if (V <= ROW_WARP || rows == 0) return 1;
-  long long n = (12ll * sm_count + rows - 1) / rows;
+  if (rows == 0 || row_lanes(rows, V, sm_count)) return 1;
+  long long n = ROW_CTAS * (long long)sm_count / rows;
   const int most = (V + batch - 1) / batch;
   if (n > most) n = most;
   return n < 1 ? 1 : (int)n;
 }
 
+// CTAs that share the rows behind the pass.
+int tail_ctas(long long rows) {
+  if (rows <= TAIL_ONE) return 1;
+  if (rows <= TAIL_MANY) return TAIL_CTAS;
+  const long long n = (rows + TAIL_THREADS - 1) / TAIL_THREADS;
+  return n < TAIL_MOST ? (int)n : TAIL_MOST;
+}
 // Scratch of a forward: the cluster's sums (a preference: of up to as many parts of sequences as it has warps), the
 // parts of the rows and the logits at the labels.
 struct Scratch {
@@ -457,7 +496,7 @@ struct Scratch {
   float* at_label;
   long long doubles;
   Scratch(void* at, long long N, long long rows, int n_parts) {
-    const long long warps = TAIL_CTAS * (TAIL_THREADS / 32), n = N > warps ? N : warps;
+    const long long warps = (long long)tail_ctas(rows) * (TAIL_THREADS / 32), n = N > warps ? N : warps;
     sums = (double*)at;
     parts = (float2*)(sums + n);
     at_label = (float*)(parts + rows * n_parts);
@@ -465,30 +504,38 @@ struct Scratch {
   }
 };
 
-int rows_fwd(const Logits& z, const Scratch& s, int n_parts, int dtype, cudaStream_t st) {
+int rows_fwd(const Logits& z, const Scratch& s, int n_parts, int dtype, int sm_count, cudaStream_t st) {
   if (z.rows == 0) return 0;
+  const int lanes = row_lanes(z.rows, z.V, sm_count);
+  const dim3 grid(lanes == 0 ? (unsigned)z.rows : (unsigned)((z.rows * lanes + 255) / 256), n_parts);
   PF_DISPATCH3(dtype, {
-    if (z.V <= ROW_WARP)
-      after(row_fwd_kernel<T, 32>, (unsigned)((z.rows + 7) / 8), 256, 0, st)(z, s.parts, s.at_label);
-    else
-      after(row_fwd_kernel<T, ROW_THREADS>, dim3((unsigned)z.rows, n_parts), ROW_THREADS, 0, st)(z, s.parts,
-                                                                                                 s.at_label);
+    if (lanes == 8) after(row_fwd_kernel<T, 8>, grid, 256, 0, st)(z, s.parts, s.at_label);
+    else if (lanes == 32) after(row_fwd_kernel<T, 32>, grid, 256, 0, st)(z, s.parts, s.at_label);
+    else after(row_fwd_kernel<T, ROW_THREADS>, grid, ROW_THREADS, 0, st)(z, s.parts, s.at_label);
   });
   return 0;
 }
 
-// A launch of the kernels behind the rows: one CTA, or a cluster.
-template <typename... P>
-LaunchAfter<P...> tail(void (*kernel)(P...), long long rows, cudaStream_t st, cudaLaunchAttribute* cluster) {
-  auto l = after(kernel, rows <= TAIL_ONE ? 1 : TAIL_CTAS, TAIL_THREADS, 0, st);
-  if (rows > TAIL_ONE) {
-    cluster->id = cudaLaunchAttributeClusterDimension;
-    cluster->val.clusterDim.x = TAIL_CTAS;
-    cluster->val.clusterDim.y = cluster->val.clusterDim.z = 1;
-    l.cfg.attrs = cluster;
+// The launches behind the rows: `whole`, one CTA or a cluster, or `share` and `join`.
+template <typename... P, typename... A>
+void tail(void (*whole)(P...), void (*share)(P...), void (*join)(P...), long long rows, cudaStream_t st,
+          const A&... args) {
+  const int ctas = tail_ctas(rows);
+  if (rows > TAIL_MANY) {
+    after(share, ctas, TAIL_THREADS, 0, st)(args..., ctas);
+    after(join, 1, TAIL_THREADS, 0, st)(args..., ctas);
+    return;
+  }
+  auto l = after(whole, ctas, TAIL_THREADS, 0, st);
+  cudaLaunchAttribute cluster;
+  if (ctas > 1) {
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = ctas;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    l.cfg.attrs = &cluster;
     l.cfg.numAttrs = 1;
   }
-  return l;
+  l(args..., ctas);
 }
 
 }  // namespace
@@ -512,11 +559,10 @@ PF_API int pf_preference_fwd(const void* logits, const void* labels, const void*
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int n_parts = row_parts(z.rows, V, dtype, sm_count);
   const Scratch s(scratch, N, z.rows, n_parts);
-  if ((code = rows_fwd(z, s, n_parts, dtype, st))) return code;
+  if ((code = rows_fwd(z, s, n_parts, dtype, sm_count, st))) return code;
   const Rows rows{s.parts, s.at_label, (float2*)stats, n_parts};
-  cudaLaunchAttribute cluster;
-  tail(preference_tail_kernel, z.rows, st, &cluster)(z, rows, (const float*)ref, (float*)rewards, (float*)loss,
-                                                     (float*)coef, s.sums, (int)N, beta, smoothing);
+  tail(preference_tail_kernel<WHOLE>, preference_tail_kernel<SHARE>, preference_tail_kernel<JOIN>, z.rows, st, z, rows,
+       (const float*)ref, (float*)rewards, (float*)loss, (float*)coef, s.sums, (int)N, beta, smoothing);
   PF_CHECK_LAUNCH();
   return 0;
 }
@@ -537,10 +583,9 @@ PF_API int pf_policy_fwd(const void* logits, const void* actions, const void* ol
                      (float*)inv};
   const int n_parts = row_parts(z.rows, V, dtype, sm_count);
   const Scratch s(scratch, N, z.rows, n_parts);
-  if ((code = rows_fwd(z, s, n_parts, dtype, st))) return code;
+  if ((code = rows_fwd(z, s, n_parts, dtype, sm_count, st))) return code;
   const Rows rows{s.parts, s.at_label, (float2*)stats, n_parts};
-  cudaLaunchAttribute cluster;
-  tail(policy_tail_kernel, z.rows, st, &cluster)(z, rows, p, s.sums);
+  tail(policy_tail_kernel<WHOLE>, policy_tail_kernel<SHARE>, policy_tail_kernel<JOIN>, z.rows, st, z, rows, p, s.sums);
   PF_CHECK_LAUNCH();
   return 0;
 }
@@ -567,7 +612,9 @@ PF_API int pf_token_loss_bwd(const void* logits, const void* labels, const void*
                                                       (const float*)gout, (const float*)inv, (T*)dlogits, per,  \
                                                       dlogits_row)
   PF_DISPATCH3(dtype, {
-    if (V / (16 / (int)sizeof(T)) <= 64) PF_BWD(32, (unsigned)((z.rows + 7) / 8));
+    const int lanes = back_lanes(z.rows, V / (16 / (int)sizeof(T)), sm_count);
+    if (lanes == 8) PF_BWD(8, (unsigned)((z.rows + 31) / 32));
+    else if (lanes == 32) PF_BWD(32, (unsigned)((z.rows + 7) / 8));
     else PF_BWD(256, dim3((unsigned)z.rows, (unsigned)slabs));
   });
 #undef PF_BWD
