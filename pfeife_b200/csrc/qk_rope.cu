@@ -57,14 +57,18 @@ template <> __device__ __forceinline__ void narrow2(__nv_bfloat16* to, float a, 
 
 // Where a lane's slots lie in a head, and by how much they turn.  In registers the values of a slot are VW pairs
 // (x, y) that turn together, x and y each packed two by two, whatever their order in memory.
-template <typename T, int VW, int NS, bool INTER>
+// FIT: a head fills the lanes and turns as a whole, so that nothing has to be asked for.
+template <typename T, int VW, int NS, bool INTER, bool FIT>
 struct Slots {
   static constexpr int P = (VW + 1) / 2;             // packed registers of the x and of the y of a slot
   struct Values { uint64_t x[P], y[P]; };
   using raw = typename Raw<VW * sizeof(T)>::type;
   int a[NS], b[NS];                // first values of both halves, -1 where there is none
   int f[NS], g[NS];                // first frequencies of both halves of the cosines
-  bool turns[NS];
+  bool turns_[NS];
+  __device__ __forceinline__ bool has_a(int n) const { return FIT || a[n] >= 0; }
+  __device__ __forceinline__ bool has_b(int n) const { return FIT || b[n] >= 0; }
+  __device__ __forceinline__ bool turns(int n) const { return FIT || turns_[n]; }
 
   // Both halves lie apart even where pairs lie side by side or do not turn, so that the lanes of a group read and
   // write whole sectors together (32 bytes a lane, 16 at a time: 41 us for 26, [1, 32768, 8, 128] interleaved).
@@ -73,13 +77,13 @@ struct Slots {
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
       const int v = lane + (n << p.lg), w = v - pairs;
-      turns[n] = v < pairs;
+      turns_[n] = FIT || v < pairs;
       constexpr bool single = VW == 1 && INTER;       // a half is no pair
-      a[n] = !turns[n] ? p.R + VW * w : single ? 2 * v : VW * v;
-      b[n] = !turns[n] ? a[n] + VW * apart : single ? 2 * v + 1 : VW * v + p.R / 2;
+      a[n] = !turns_[n] ? p.R + VW * w : single ? 2 * v : VW * v;
+      b[n] = !turns_[n] ? a[n] + VW * apart : single ? 2 * v + 1 : VW * v + p.R / 2;
       f[n] = INTER && !single ? VW / 2 * v : VW * v;
       g[n] = INTER ? p.R / 4 + VW / 2 * v : VW * v + VW / 2;
-      if (!turns[n]) {
+      if (!turns_[n]) {
         if (w >= apart) a[n] = b[n] = -1;
         if (b[n] >= p.D) b[n] = -1;
       }
@@ -89,8 +93,8 @@ struct Slots {
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
       r[n][0] = r[n][1] = raw{};
-      if (a[n] >= 0) r[n][0] = *reinterpret_cast<const raw*>(x + a[n]);
-      if (b[n] >= 0) r[n][1] = *reinterpret_cast<const raw*>(x + b[n]);
+      if (has_a(n)) r[n][0] = *reinterpret_cast<const raw*>(x + a[n]);
+      if (has_b(n)) r[n][1] = *reinterpret_cast<const raw*>(x + b[n]);
     }
   }
   // the pairs of two halves: (a, b) of equal places, or neighbours
@@ -137,8 +141,8 @@ struct Slots {
     put(to, n, r);
   }
   __device__ __forceinline__ void put(T* y, int n, const raw (&r)[2]) const {
-    if (a[n] >= 0) *reinterpret_cast<raw*>(y + a[n]) = r[0];
-    if (b[n] >= 0) *reinterpret_cast<raw*>(y + b[n]) = r[1];
+    if (has_a(n)) *reinterpret_cast<raw*>(y + a[n]) = r[0];
+    if (has_b(n)) *reinterpret_cast<raw*>(y + b[n]) = r[1];
   }
   // gain of the norm at the slots' values
   __device__ __forceinline__ void gains(const float* w, Values (&v)[NS]) const {
@@ -174,7 +178,7 @@ struct Slots {
     const bool there = row >= 0 && row < p.rows;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-      if (!turns[n]) continue;
+      if (!turns(n)) continue;
       const long long at = row * (p.R / 2), first = there ? at + f[n] : -1, second = there ? at + g[n] : -1;
       constexpr int K = VW > 1 ? VW / 2 : 1;
       take<K>(p.cos_t, first, to[n].c, NAN);
@@ -207,36 +211,43 @@ __device__ __forceinline__ float halves(uint64_t v) {
   return a + b;
 }
 
-// sums of U values over the group of a lane; every lane of the warp calls it
+// sums of U values over the lanes of a group, whose other groups of the warp may be done
 template <int U>
-__device__ __forceinline__ void group_sum(float (&v)[U], int lg) {
+__device__ __forceinline__ void group_sum(float (&v)[U], int lg, unsigned lanes) {
   for (int o = (1 << lg) >> 1; o > 0; o >>= 1)
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] += __shfl_xor_sync(0xffffffffu, v[u], o);
+    for (int u = 0; u < U; ++u) v[u] += __shfl_xor_sync(lanes, v[u], o);
 }
 
-// Where a group is in its walk over the heads of a part, token by token, and their place in one tensor.
+// Where a group is in its walk over the heads of a part, token by token, and their places in one tensor or two.
 struct Walk {
   unsigned b, s;
   int h;
-  long long at;
-  __device__ __forceinline__ Walk(const HeadsArgs& p, const HeadsPart& part, const HeadsView& v, unsigned first) {
+  long long at, other;
+  __device__ __forceinline__ Walk(const HeadsArgs& p, const HeadsPart& part, const HeadsView& v, const HeadsView& w,
+                                  unsigned first) {
     const unsigned token = first / part.heads;
     h = first - token * part.heads;
     b = token / p.S;
     s = token - b * p.S;
-    at = place(v) + h * v.h;
+    start(v, w);
+    at += h * v.h;
+    other += h * w.h;
   }
-  __device__ __forceinline__ long long place(const HeadsView& v) const {
-    return (long long)b * v.b + (long long)s * v.s;
+  __device__ __forceinline__ void start(const HeadsView& v, const HeadsView& w) {
+    at = (long long)b * v.b + (long long)s * v.s;
+    other = (long long)b * w.b + (long long)s * w.s;
   }
-  __device__ __forceinline__ bool next(const HeadsArgs& p, const HeadsPart& part, const HeadsView& v) {
+  // whether the next head is another token's
+  __device__ __forceinline__ bool next(const HeadsArgs& p, const HeadsPart& part, const HeadsView& v,
+                                       const HeadsView& w) {
     at += v.h;
+    other += w.h;
     if (++h < part.heads) return false;
     h = 0;
     if (++s == (unsigned)p.S) { s = 0; ++b; }
-    at = place(v);
-    return true;                                     // the next token
+    start(v, w);
+    return true;
   }
 };
 // row of the tables for a token; that of one behind the last is never used
@@ -263,7 +274,7 @@ struct HeadsRing {
   static constexpr int TENSORS = BACK ? 2 : 1, VEC = VW * (int)sizeof(T);
   static constexpr bool ASYNC = VEC >= 4;            // no copy moves 2 bytes
   static constexpr int STAGE = 256 * TENSORS * NS * 2 * VEC;
-  static constexpr int FIT = RING_BYTES / CTAS / STAGE, STAGES = ASYNC ? (FIT > 12 ? 12 : FIT) : 1;
+  static constexpr int ROOM = RING_BYTES / CTAS / STAGE, STAGES = ASYNC ? (ROOM > 12 ? 12 : ROOM) : 1;
   static constexpr int BYTES = STAGES * STAGE > 8 * MAX_HEAD_DIM * 4 ? STAGES * STAGE : 8 * MAX_HEAD_DIM * 4;
 };
 
@@ -271,10 +282,15 @@ struct HeadsRing {
 // result -> y and the sums for dw, one row a CTA, which heads_fold_kernel adds in order.
 // A CTA stays with one part.  Its groups take `per` heads each, one after the other, token by token: the parts of a
 // call and the heads of a part need not divide anything, and no group has more than one head above another.
-template <typename T, int VW, int NS, int MODE, bool INTER>
+// What bounds it is HBM behind some 220 instructions a head and lane, half of them conversions and packed arithmetic:
+// [1, 2048, 3, 32, 128] bf16 21 us forward (4.8 TB/s) and 30 backward with the fold (4.5), a rotation of
+// [1, 32768, 8, 128] 25 (5.3), where an element-wise pass over as many bytes takes 17, 28 and 22.  Heads loaded into
+// registers by the four took 24 and 40 us; all groups going through memory together, 4 or 8 heads each at a time, 30
+// and 43 (angles are loaded more often); the next token's angles in registers 23 (fewer CTAs an SM).
+template <typename T, int VW, int NS, int MODE, bool INTER, bool FIT>
 __global__ void __launch_bounds__(256, HeadsRing<T, VW, NS, MODE>::CTAS)
 heads_kernel(const __grid_constant__ HeadsArgs p) {
-  using S = Slots<T, VW, NS, INTER>;
+  using S = Slots<T, VW, NS, INTER, FIT>;
   using R = HeadsRing<T, VW, NS, MODE>;
   using raw = typename S::raw;
   constexpr int P = S::P, STEP = 256 * R::TENSORS * NS * 2;  // raws of a stage
@@ -291,32 +307,36 @@ heads_kernel(const __grid_constant__ HeadsArgs p) {
   const unsigned group = (blockIdx.x - part.cta0) * (256u >> p.lg) + (threadIdx.x >> p.lg);
   const unsigned all = p.tokens * (unsigned)part.heads;
   const unsigned first = (unsigned)min((unsigned long long)group * part.per, (unsigned long long)all);
-  const int mine = min(all - first, (unsigned)part.per);       // part.per steps are made by all, for the sums' sake
+  const int mine = min(all - first, (unsigned)part.per);
+  // Groups make as many steps as they have heads, and add up among their own lanes; where lanes are left over, all
+  // make as many as any, which keeps the warp together ([2, 4096] tokens of 32 and 8 heads: 34 us for 41).
+  const int steps = FIT ? mine : part.per;
+  const unsigned lanes = !FIT || p.lg == 5 ? 0xffffffffu : ((1u << (1 << p.lg)) - 1) << (threadIdx.x & 31 & ~((1 << p.lg) - 1));
   const S slot(p, lane);
   after_previous();
 
-  Walk in(p, part, BACK ? part.g : part.x, first), x_in(p, part, part.x, first), out(p, part, part.y, first);
+  const HeadsView &first_in = BACK ? part.g : part.x;
+  Walk in(p, part, first_in, part.x, first), out(p, part, part.y, part.y, first);
   int filled = 0;                                    // the stage that the next fetch fills
   raw now[R::TENSORS][NS][2] = {}, then[R::TENSORS][NS][2] = {};
   auto fetch = [&](int step) {                       // one head of the walk, if the group still has it
     if (step < mine) {
-      const T* from[2] = {reinterpret_cast<const T*>((BACK ? part.g : part.x).at) + in.at,
-                          BACK ? reinterpret_cast<const T*>(part.x.at) + x_in.at : nullptr};
+      const T* from[2] = {reinterpret_cast<const T*>(first_in.at) + in.at,
+                          BACK ? reinterpret_cast<const T*>(part.x.at) + in.other : nullptr};
 #pragma unroll
       for (int q = 0; q < R::TENSORS; ++q) {
         if (BACK && q == 1 && !part.turn) continue;  // the values of a projection: only their gradient is read
         if constexpr (R::ASYNC) {
 #pragma unroll
           for (int n = 0; n < NS; ++n) {
-            if (slot.a[n] >= 0) copy_async<R::VEC>(place(filled, q, n, 0), from[q] + slot.a[n]);
-            if (slot.b[n] >= 0) copy_async<R::VEC>(place(filled, q, n, 1), from[q] + slot.b[n]);
+            if (slot.has_a(n)) copy_async<R::VEC>(place(filled, q, n, 0), from[q] + slot.a[n]);
+            if (slot.has_b(n)) copy_async<R::VEC>(place(filled, q, n, 1), from[q] + slot.b[n]);
           }
         } else {
           slot.load(from[q], then[q]);
         }
       }
-      in.next(p, part, BACK ? part.g : part.x);
-      if (BACK) x_in.next(p, part, part.x);
+      in.next(p, part, first_in, part.x);
     }
     if constexpr (R::ASYNC) {
       cp_async_commit();
@@ -345,16 +365,17 @@ heads_kernel(const __grid_constant__ HeadsArgs p) {
   }
 
   int stage = 0;
-  for (int step = 0; step < part.per; ++step) {
+  for (int step = 0; step < steps; ++step) {
+    const bool live = FIT || step < mine;
     if constexpr (R::ASYNC) {
       cp_async_wait<R::STAGES - 2>();
 #pragma unroll
       for (int q = 0; q < R::TENSORS; ++q)
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-          now[q][n][0] = now[q][n][1] = raw{};
-          if (step < mine && slot.a[n] >= 0) now[q][n][0] = *place(stage, q, n, 0);
-          if (step < mine && slot.b[n] >= 0) now[q][n][1] = *place(stage, q, n, 1);
+          if (!FIT) now[q][n][0] = now[q][n][1] = raw{};
+          if (live && slot.has_a(n)) now[q][n][0] = *place(stage, q, n, 0);
+          if (live && slot.has_b(n)) now[q][n][1] = *place(stage, q, n, 1);
         }
       stage = stage + 1 < R::STAGES ? stage + 1 : 0;
       fetch(step + R::STAGES - 1);                   // into the place that the step before this one has read
@@ -367,10 +388,10 @@ heads_kernel(const __grid_constant__ HeadsArgs p) {
     }
     T* y = reinterpret_cast<T*>(part.y.at) + out.at;
     if (!part.turn) {                                // the values of a projection
-      if (step < mine) {
+      if (live) {
 #pragma unroll
         for (int n = 0; n < NS; ++n) slot.put(y, n, now[0][n]);
-        out.next(p, part, part.y);
+        out.next(p, part, part.y, part.y);
       }
       continue;
     }
@@ -388,11 +409,11 @@ heads_kernel(const __grid_constant__ HeadsArgs p) {
             v[n].x[j] = mul2(v[n].x[j], w[n].x[j]);
             v[n].y[j] = mul2(v[n].y[j], w[n].y[j]);
           }
-        if (slot.turns[n]) S::template turn<MODE == UNROTATE>(by[n], v[n]);
+        if (slot.turns(n)) S::template turn<MODE == UNROTATE>(by[n], v[n]);
       }
       if constexpr (MODE == NORM) {                  // what hangs on the sum comes last
         float sum[1] = {halves(squares)};
-        group_sum(sum, p.lg);
+        group_sum(sum, p.lg, lanes);
         const float r = rsqrtf(sum[0] * p.inv_D + p.eps);
         const uint64_t r2 = f2_pack(r, r);
 #pragma unroll
@@ -406,7 +427,7 @@ heads_kernel(const __grid_constant__ HeadsArgs p) {
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
         v[n] = S::widen(now[0][n]);
-        if (slot.turns[n]) S::template turn<true>(by[n], v[n]);
+        if (slot.turns(n)) S::template turn<true>(by[n], v[n]);
         x[n] = S::widen(now[1][n]);
 #pragma unroll
         for (int j = 0; j < P; ++j) {
@@ -417,11 +438,11 @@ heads_kernel(const __grid_constant__ HeadsArgs p) {
         }
       }
       float sum[2] = {halves(squares), halves(dots)};
-      group_sum(sum, p.lg);
+      group_sum(sum, p.lg, lanes);
       // r (g w - xh m) with xh = x r and m = mean(g w xh) is (g w) r + x (-r^3 mean(g w x))
       const float r = rsqrtf(sum[0] * p.inv_D + p.eps), m = -(r * (r * (r * (sum[1] * p.inv_D))));
       const uint64_t r2 = f2_pack(r, r), m2 = f2_pack(m, m);
-      if (step < mine)
+      if (live)
 #pragma unroll
         for (int n = 0; n < NS; ++n)
 #pragma unroll
@@ -433,16 +454,17 @@ heads_kernel(const __grid_constant__ HeadsArgs p) {
             v[n].y[j] = fma2(x[n].y[j], m2, mul2(gy, w[n].y[j]));
           }
     }
-    if (step < mine) {
+    if (live) {
 #pragma unroll
       for (int n = 0; n < NS; ++n) slot.store(y, n, v[n]);
-      if (out.next(p, part, part.y)) next_angles();
+      if (out.next(p, part, part.y, part.y)) next_angles();
     }
   }
 
   if constexpr (BACK) {
     if (!part.dw) return;                            // the same for the whole CTA
     float(*sums)[MAX_HEAD_DIM] = reinterpret_cast<float(*)[MAX_HEAD_DIM]>(heads_smem);
+    __syncwarp();
     if constexpr (R::ASYNC) cp_async_wait<0>();
     __syncthreads();                                 // nobody's copies are still on their way into the ring
 #pragma unroll
@@ -463,8 +485,8 @@ heads_kernel(const __grid_constant__ HeadsArgs p) {
         const int half = j < VW / 2 ? slot.a[n] : slot.b[n], at = j < VW / 2 ? 2 * j : 2 * j - VW;
         const int x_at = beside ? half + at : slot.a[n] + j, y_at = beside ? half + at + 1 : slot.b[n] + j;
         if ((threadIdx.x & 31) < (1 << p.lg)) {
-          if ((beside ? half : slot.a[n]) >= 0) sums[threadIdx.x >> 5][x_at] = x[j];
-          if ((beside ? half : slot.b[n]) >= 0) sums[threadIdx.x >> 5][y_at] = y[j];
+          if (FIT || (beside ? half : slot.a[n]) >= 0) sums[threadIdx.x >> 5][x_at] = x[j];
+          if (FIT || (beside ? half : slot.b[n]) >= 0) sums[threadIdx.x >> 5][y_at] = y[j];
         }
       }
     }
@@ -478,27 +500,25 @@ heads_kernel(const __grid_constant__ HeadsArgs p) {
   }
 }
 
-// dw[part] (+)= the CTAs' sums, in their order.  blockIdx.y: the part; 32 columns and 8 shares of the rows a CTA.
-__global__ void __launch_bounds__(256)
+// dw[part] (+)= the CTAs' sums, in their order.  blockIdx.y: the part; 32 columns and 32 shares of the rows a CTA.
+__global__ void __launch_bounds__(1024)
 heads_fold_kernel(const float* __restrict__ part0, const float* __restrict__ part1, float* __restrict__ dw0,
                   float* __restrict__ dw1, int ctas0, int ctas1, int D, int accumulate) {
   after_previous();
-  __shared__ float sums[8][33];
+  __shared__ float sums[32][33];
   const float* in = blockIdx.y ? part1 : part0;
   float* out = blockIdx.y ? dw1 : dw0;
-  const int n = blockIdx.y ? ctas1 : ctas0, col = blockIdx.x * 32 + (threadIdx.x & 31), share = threadIdx.x >> 5;
+  const int n = blockIdx.y ? ctas1 : ctas0, lane = threadIdx.x & 31, share = threadIdx.x >> 5;
+  int col = blockIdx.x * 32 + lane;
   float t = 0.f;
   if (out && col < D)
 #pragma unroll 4
-    for (int i = share; i < n; i += 8) t += in[(long long)i * D + col];
-  sums[share][threadIdx.x & 31] = t;
+    for (int i = share; i < n; i += 32) t += in[(long long)i * D + col];
+  sums[share][lane] = t;
   __syncthreads();
-  if (out && share == 0 && col < D) {
-    t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t += sums[i][threadIdx.x & 31];
-    out[col] = accumulate ? out[col] + t : t;
-  }
+  t = warp_sum(sums[lane][share]);                   // a warp a column
+  col = blockIdx.x * 32 + share;
+  if (out && lane == 0 && col < D) out[col] = accumulate ? out[col] + t : t;
 }
 
 }  // namespace pf
@@ -600,10 +620,16 @@ struct Launch {
   cudaStream_t st;
   int code = 0;
   template <typename T, int VW, int NS> void operator()() {
-    if (interleaved) go<T, VW, NS, true>();
-    else go<T, VW, NS, false>();
+    if (interleaved) fit<T, VW, NS, true>();
+    else fit<T, VW, NS, false>();
   }
-  template <typename T, int VW, int NS, bool INTER> void go() {
+  // of the widest vectors alone: other heads seldom fill the lanes (a rotation of [1, 32768, 8, 128] 27 -> 25 us)
+  template <typename T, int VW, int NS, bool INTER> void fit() {
+    if constexpr (VW * sizeof(T) == 16)
+      if (p.R == p.D && p.D == 2 * VW * NS << p.lg) return go<T, VW, NS, INTER, true>();
+    go<T, VW, NS, INTER, false>();
+  }
+  template <typename T, int VW, int NS, bool INTER, bool FIT> void go() {
     using R = HeadsRing<T, VW, NS, MODE>;
     const int ctas = deal(p, parts, R::CTAS * sms, weight);
     if (ctas == 0) return;
@@ -611,12 +637,12 @@ struct Launch {
     int dev = 0;
     cudaGetDevice(&dev);
     if (R::BYTES > 48 * 1024 && (dev < 0 || dev >= 64 || !done[dev])) {
-      const cudaError_t e = cudaFuncSetAttribute(heads_kernel<T, VW, NS, MODE, INTER>,
+      const cudaError_t e = cudaFuncSetAttribute(heads_kernel<T, VW, NS, MODE, INTER, FIT>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, R::BYTES);
       if (e != cudaSuccess) { code = (int)e; return; }
       if (dev >= 0 && dev < 64) done[dev] = true;
     }
-    after(heads_kernel<T, VW, NS, MODE, INTER>, ctas, 256, R::BYTES, st)(p);
+    after(heads_kernel<T, VW, NS, MODE, INTER, FIT>, ctas, 256, R::BYTES, st)(p);
   }
 };
 template <int MODE>
@@ -641,7 +667,7 @@ PF_API int pf_heads_fwd(const void* q, const void* k, const void* v, void* yq, v
   if (v) p.part[parts++] = {view(v, sk), view(yv, syk), {}, nullptr, nullptr, Hk, 0, 0, 0, 0};
   const int vw = prepare(p, parts, cos_t, sin_t, pos, spos, B, S, D, R, rows, eps, dtype);
   if (vw < 0) return vw;
-  if ((long long)B * S * (Hq + 2ll * Hk) > 0x7fffffffll) return -3;
+  if ((long long)B * S * (Hq + 2ll * Hk) > 0x7fffffffll || (k && !wq != !wk)) return -3;
   if (p.tokens == 0 || (Hq == 0 && Hk == 0)) return 0;
   const int even[3] = {1, 1, 1};
   const int code = wq ? launch<NORM>(p, parts, even, interleaved, dtype, vw, sm_count, stream)
@@ -671,7 +697,7 @@ PF_API int pf_heads_bwd(const void* gq, const void* gk, const void* gv, const vo
   if (gv) p.part[parts++] = {{}, view(dv, sdk), view(gv, sgk), nullptr, nullptr, Hk, 0, 0, 0, 0};
   const int vw = prepare(p, parts, cos_t, sin_t, pos, spos, B, S, D, R, rows, eps, dtype);
   if (vw < 0) return vw;
-  if ((long long)B * S * (Hq + 2ll * Hk) > 0x7fffffffll) return -3;
+  if ((long long)B * S * (Hq + 2ll * Hk) > 0x7fffffffll || !wq || !wk) return -3;
   // the sums' rows lie where the parts' CTAs do, at most BACK_CTAS an SM and one more for each of two parts
   const int weight[3] = {3, 3, 2};
   if (dwq) p.part[0].dw = (float*)scratch;
@@ -680,7 +706,7 @@ PF_API int pf_heads_bwd(const void* gq, const void* gk, const void* gv, const vo
   if (code) return code;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (dwq || dwk)
-    after(heads_fold_kernel, dim3((D + 31) / 32, 2), 256, 0, st)(
+    after(heads_fold_kernel, dim3((D + 31) / 32, 2), 1024, 0, st)(
         (const float*)scratch, (const float*)scratch + (long long)p.part[1].cta0 * D, (float*)dwq, (float*)dwk,
         p.part[0].ctas, p.part[1].ctas, D, accumulate);
   PF_CHECK_LAUNCH();
