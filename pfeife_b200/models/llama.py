@@ -102,7 +102,10 @@ class Llama(nn.Module):
         self.lm_head = nn.Linear(cfg.hidden_size, cfg.vocab_size, bias=False)
         if cfg.tie_embeddings:
             self.lm_head.weight = self.embed.weight
-        cos, sin = ops.rope_tables(cfg.max_seq_len, cfg.rope_dim or cfg.hidden_size // cfg.num_heads,
+        head_dim = cfg.hidden_size // cfg.num_heads
+        if cfg.rope_dim is not None and (cfg.rope_dim % 2 or not 0 < cfg.rope_dim <= head_dim):
+            raise ValueError(f"rope_dim {cfg.rope_dim} is no even part of a head of {head_dim}")
+        cos, sin = ops.rope_tables(cfg.max_seq_len, cfg.rope_dim or head_dim,
                                    cfg.rope_theta, scaling=cfg.rope_scaling)
         self.register_buffer("rope_cos", cos, persistent=False)
         self.register_buffer("rope_sin", sin, persistent=False)

@@ -1149,8 +1149,8 @@ def policy_loss(logits: Tensor, actions: Tensor, old_logps: Tensor, advantages: 
     """Clipped policy loss over sampled tokens.  logits [..., V]; actions [...]: the token taken at each row,
     ``ignore_index`` or any number outside the vocabulary where none counts; old_logps [...]: its log-probability
     when it was sampled; advantages: of the shape of the actions or one that expands to it ([N, 1]: one for each
-    sequence), all read in 32 bits.  With l = log softmax(logits / temperature)[action] and r = exp(l - old) a token's term is
-    -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(ref - l) - (ref - l) - 1), the last with
+    sequence), all read in 32 bits.  With l = log softmax(logits / temperature)[action] and r = exp(l - old) a token's
+    term is -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(ref - l) - (ref - l) - 1), the last with
     ``ref_logps`` [...] only; the loss is the mean over the tokens that count, 0 if there are none.
     Rows that do not count are not read and get a gradient of zero, whatever their logits."""
     out = _native_call("policy_loss", logits, actions, old_logps, advantages, ref_logps, float(clip_low),
@@ -1293,6 +1293,8 @@ def rope(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None
     for it would wait for the device, and an IndexError on the CPU."""
     if positions is None and not interleaved and not _narrow(cos, x):
         return _call(rope_apply, x, cos, sin, False)
+    if isinstance(x, Tensor) and x.dim() != 4:
+        raise ValueError(f"heads [B, S, H, D] are needed, not {tuple(x.shape)}")
     y = _native_call("rotate_heads", x, cos, sin, positions, interleaved)
     if y is not None:
         return y
@@ -1333,6 +1335,7 @@ def rope_qkv(qkv: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] 
     if positions is None and not interleaved and not _narrow(cos, qkv):
         y = _native_call("rope_qkv", qkv, cos, sin)
         return y if y is not None else _call(rope_qkv_apply, qkv, cos, sin, False)
+    _check_projection(qkv)
     y = _native_call("rotate_heads", qkv, cos, sin, positions, interleaved)
     if y is not None:
         return y
@@ -1406,6 +1409,11 @@ def rope_tables(seq_len: int, head_dim: int, theta: float = 10000.0, device=None
 
 
 # --------------------------------------------------------------------------- rotations of any layout, head norms
+def _check_projection(qkv: Tensor) -> None:
+    if isinstance(qkv, Tensor) and (qkv.dim() != 5 or qkv.shape[2] != 3):
+        raise ValueError(f"a projection [B, S, 3, H, D] is needed, not {tuple(qkv.shape)}")
+
+
 def _check_angles(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor]) -> None:
     """Refuses angles that do not fit x [B, S, .., D]; what a symbolic trace passes is checked when it runs."""
     if not isinstance(x, Tensor):
@@ -1416,10 +1424,11 @@ def _check_angles(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tenso
                          f"and {tuple(sin.shape)}")
     if cos.device != x.device or sin.device != x.device:
         raise ValueError(f"tables on {cos.device} and {sin.device} for heads on {x.device}")
+    if cos.shape[0] < (S if positions is None else min(S, 1)):
+        raise ValueError(f"tables of {cos.shape[0]} rows for {S} tokens")
     if positions is None:
-        if cos.shape[0] < S:
-            raise ValueError(f"tables of {cos.shape[0]} rows for {S} tokens")
-    elif positions.device != x.device or positions.dtype not in (torch.int64, torch.int32) \
+        return
+    if positions.device != x.device or positions.dtype not in (torch.int64, torch.int32) \
             or tuple(positions.shape) not in ((S,), (x.shape[0], S)):
         raise ValueError(f"positions are integers [{S}] or [{x.shape[0]}, {S}] on {x.device}, not "
                          f"{positions.dtype} {tuple(positions.shape)} on {positions.device}")
@@ -1668,8 +1677,7 @@ def qk_norm_rope_qkv(qkv: Tensor, q_weight: Tensor, k_weight: Tensor, cos: Tenso
     y = _native_layer("norm_rotate_heads", qkv, None, q_weight, k_weight, cos, sin, positions, float(eps), interleaved)
     if y is not None:
         return y
-    if isinstance(qkv, Tensor) and (qkv.dim() != 5 or qkv.shape[2] != 3):
-        raise ValueError(f"a projection [B, S, 3, H, D] is needed, not {tuple(qkv.shape)}")
+    _check_projection(qkv)
     _check_angles(qkv, cos, sin, positions)
     _check_gains(qkv, q_weight, k_weight)
     return _call(qk_norm_rope_qkv_fwd, qkv, q_weight, k_weight, cos, sin, positions, float(eps), interleaved)

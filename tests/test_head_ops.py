@@ -320,6 +320,16 @@ def test_refusals(device):
         ops.qk_norm_rope_qkv(torch.stack([x, x], 2), w, w, cos, sin)
     with pytest.raises(ValueError):
         ops.rope(x, cos[:, :4], sin[:3, :4])                     # a partial rotation of too few rows
+    with pytest.raises(ValueError):
+        ops.rope(x, cos[:0], sin[:0], torch.zeros(4, dtype=torch.int64, device=device))
+    packed = torch.stack([x, x, x], 2)
+    for wrong, call in ((packed, ops.rope), (x, ops.rope_qkv), (packed[:, :, :2], ops.rope_qkv), (x[0], ops.rope)):
+        with pytest.raises(ValueError):
+            call(wrong, cos, sin, interleaved=True)
+    from pfeife_b200.models.llama import Llama, llama_config
+    for dim in (7, 0, 18):
+        with pytest.raises(ValueError):
+            Llama(llama_config("llama_tiny", rope_dim=dim))
 
 
 # ------------------------------------------------------------------------------ scaled tables
