@@ -114,6 +114,7 @@ def test_mixed_precision_on_one_gpu(cuda_graphs):
     runner.gather_params()
     graphs = len(runner.worker.graphs)
     runner.close()
+    ops.unregister_params()              # later calls of this process are of plain tensors again
     assert (graphs > 0) == cuda_graphs
     for (name, p), q, s in zip(model.named_parameters(), ref.parameters(), start):
         # the way that a weight went: some 40 roundings of 2^-9 lie between it and its gradient, four steps
