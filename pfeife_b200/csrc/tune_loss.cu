@@ -54,8 +54,8 @@ __constant__ float FRACTION_SCALE[32] = {
     0.707106781f, 0.722590403f, 0.738413073f, 0.754582214f, 0.771105413f, 0.787990423f, 0.805245166f, 0.822877739f,
     0.840896415f, 0.859309649f, 0.878126080f, 0.897354538f, 0.917004043f, 0.937083817f, 0.957603281f, 0.978572062f};
 
-// (M, s) of two parts of a row, with integers M; a part without a finite element is (-inf, 0), or (-inf, NaN) when it holds a NaN,
-// which no maximum shows: the sums are always added, and -inf counts as 0 where it is subtracted.
+// (M, s) of two parts of a row, with integers M; a part without a finite element is (-inf, 0), or (-inf, NaN) when it
+// holds a NaN, which no maximum shows: the sums are always added, and -inf counts as 0 where it is subtracted.
 __device__ __forceinline__ void part_merge(float& m, float& s, float m2, float s2) {
   const float mm = fmaxf(m, m2), sub = mm == -INFINITY ? 0.f : mm;
   s = s * exp2_fast(m - sub) + s2 * exp2_fast(m2 - sub);
@@ -238,7 +238,8 @@ struct Rows {
   }
 };
 __device__ __forceinline__ double log_prob(const Logits& z, float2 stat, float at_label) {
-  return LN2 * ((double)at_label * (double)z.k - (double)stat.x) - log((double)stat.y) - EXP2_LOW;
+  const double l = LN2 * ((double)at_label * (double)z.k - (double)stat.x) - log((double)stat.y) - EXP2_LOW;
+  return l > 0.0 ? 0.0 : l;          // a row of one word by 1e-7; a NaN stays
 }
 __device__ __forceinline__ double warp_sum64(double v) {
 #pragma unroll

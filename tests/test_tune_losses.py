@@ -208,6 +208,21 @@ def test_a_row_that_counts_keeps_its_nan(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_certain_words(device):
+    """A word that has all the probability, alone in its vocabulary or not: no log-probability above 0."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    for V in (1, 2, 70, 3000):
+        z = torch.full((4, 50, V), -300.0, device=device)
+        z[..., 0] = torch.linspace(-90, 90, 200, device=device).view(4, 50)
+        z, labels = z.to(dtype).requires_grad_(), torch.zeros(4, 50, dtype=torch.int64, device=device)
+        v = torch.zeros(4, 50, device=device)
+        out = ops.policy_loss(z, labels, v, v + 1)
+        assert (out.logps <= 0).all() and (out.logps > -1e-6).all() and abs(float(out.loss.detach()) + 1) < 1e-6
+        (dz,) = torch.autograd.grad(out.loss, z)
+        assert (dz.abs() <= 1e-6 / 200).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_nothing_counts(device):
     dtype = torch.float32 if device == "cpu" else torch.float16
     z, labels = batch(2, 4, 33, device, dtype, 1)
