@@ -11,6 +11,9 @@
 // the integer, since 16-bit logits lie on a grid on which the exponential's errors would be the same in every row.
 // What follows is a few operations per row, done in 64 bits by one thread: those differences, and a KL estimate
 // exp(d) - d - 1, which loses d^2 / 2 next to 1.
+// Where |M| is 2^22 or more (a row that a mask of the type's lowest value has left nothing, say), k z - M has lost what
+// the softmax is made of, and there may be no M: such a part of a row is passed over once more, with its largest z in
+// the place of M, sum 2^(k (z - M)), which has a minus to tell it.
 // The backward passes over it again: dz = g (onehot - p) with p = 2^(k z - M) / s and g what the loss has for the
 // row's log-probability, so that only M, s and g are kept.
 #include "common.cuh"
@@ -23,6 +26,8 @@ constexpr double LN2 = 0.693147180559945309417;
 // normal logits, bf16 and fp32 alike; a row's own s is off by 4e-8 around that).  A single probability hides it in
 // its rounding, a sum over a sequence does not.  The backward divides such values by such sums, where it cancels.
 constexpr double EXP2_LOW = 3.7e-8;
+
+constexpr float FAR = 4194304.f;
 
 struct Logits {                    // z [N, T, V]
   const void* at;
@@ -39,6 +44,11 @@ struct Logits {                    // z [N, T, V]
     return label >= 0 && label < V && label != ignore;
   }
 };
+
+// M in powers of two, in its far form too
+__device__ __forceinline__ double reference(const Logits& z, float2 stat) {
+  return stat.y < 0.f ? (double)z.k * (double)stat.x : (double)stat.x;
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -70,7 +80,9 @@ __device__ __forceinline__ void part_merge(float& m, float& s, float m2, float s
 template <typename T> struct Words;
 template <> struct Words<float> {
   static constexpr int PAIRS = 2;
-  static __device__ __forceinline__ uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  static __device__ __forceinline__ uint4 none() {
+    return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+  }
   template <int U> static __device__ __forceinline__ float most(const uint4 (&q)[U]) {
     float m = -INFINITY;
 #pragma unroll
@@ -80,7 +92,7 @@ template <> struct Words<float> {
     return m;
   }
   static __device__ __forceinline__ uint64_t pair(const uint4& q, int j) {
-    return j ? f2_pack(__uint_as_float(q.z), __uint_as_float(q.w)) : f2_pack(__uint_as_float(q.x), __uint_as_float(q.y));
+    return f2_pack(__uint_as_float(j ? q.z : q.x), __uint_as_float(j ? q.w : q.y));
   }
 };
 template <typename T2> __device__ __forceinline__ T2 word_of(const uint4& q, int j) {
@@ -97,7 +109,9 @@ template <typename T2, int U> __device__ __forceinline__ T2 most_words(const uin
 }
 template <> struct Words<__half> {
   static constexpr int PAIRS = 4;
-  static __device__ __forceinline__ uint4 none() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+  static __device__ __forceinline__ uint4 none() {
+    return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
+  }
   template <int U> static __device__ __forceinline__ float most(const uint4 (&q)[U]) {
     const float2 m = __half22float2(most_words<__half2>(q));
     return fmaxf(m.x, m.y);
@@ -109,7 +123,9 @@ template <> struct Words<__half> {
 };
 template <> struct Words<__nv_bfloat16> {
   static constexpr int PAIRS = 4;
-  static __device__ __forceinline__ uint4 none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+  static __device__ __forceinline__ uint4 none() {
+    return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+  }
   template <int U> static __device__ __forceinline__ float most(const uint4 (&q)[U]) {
     const float2 m = __bfloat1622float2(most_words<__nv_bfloat162>(q));
     return fmaxf(m.x, m.y);
@@ -146,7 +162,7 @@ row_fwd_kernel(const Logits z, float2* __restrict__ parts, float* __restrict__ a
   const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int head = min(z.V, mis ? VN - mis : 0), nvec = (z.V - head) / VN;
   const float k = z.k, fraction = (threadIdx.x & 31) * (1.f / 32);
-  float m = -INFINITY, s = 0.f;
+  float m = -FAR, s = 0.f;                           // a reference below would have sums that are infinite
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   const uint64_t k2 = f2_pack(k, k);
   // A batch of vectors from i0 on, all before `end` or some.
@@ -158,11 +174,10 @@ row_fwd_kernel(const Logits z, float2* __restrict__ parts, float* __restrict__ a
       if (!ALL) q[u] = Words<T>::none();
       if (ALL || i0 + u * THREADS < end) q[u] = __ldg(xv + i0 + u * THREADS);
     }
-    // a NaN does not move the maximum but reaches the sum below; parts that are -inf so far subtract 0, which
-    // leaves their exponentials at zero
-    const float mm = fmaxf(m, ceilf(Words<T>::most(q) * k) + fraction), sub = mm == -INFINITY ? 0.f : mm;
-    if (mm > m) s *= exp2_fast(m - sub);
-    const uint64_t minus2 = f2_pack(-sub, -sub);
+    // a NaN does not move the maximum but reaches the sum below
+    const float mm = fmaxf(m, ceilf(Words<T>::most(q) * k) + fraction);
+    if (mm > m) s *= exp2_fast(m - mm);
+    const uint64_t minus2 = f2_pack(-mm, -mm);
     uint64_t sums[2] = {0, 0};                       // two zeros each
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -185,30 +200,63 @@ row_fwd_kernel(const Logits z, float2* __restrict__ parts, float* __restrict__ a
   // the elements before the first and after the last vector (at most 2 (VN - 1))
   for (int i = tid; part == 0 && i < z.V - nvec * VN; i += THREADS) {
     const float v = to_f32<T>(x[i < head ? i : nvec * VN + i]);
-    const float mm = fmaxf(m, ceilf(v * k) + fraction), sub = mm == -INFINITY ? 0.f : mm;
-    s = s * exp2_fast(m - sub) + exp2_fast(fmaf(v, k, -sub));
+    const float mm = fmaxf(m, ceilf(v * k) + fraction);
+    s = s * exp2_fast(m - mm) + exp2_fast(fmaf(v, k, -mm));
     m = mm;
   }
-  if (m > -INFINITY) {                               // to the integer above, by the lane's own power where it is that
+  {                                                  // to the integer above, by the lane's own power where it is that
     const float whole = ceilf(m), down = m - whole;
     s *= down == fraction - 1.f ? FRACTION_SCALE[threadIdx.x & 31] : exp2f(down);
     m = whole;
   }
   // the lanes of a row; others of the warp may have left, or have more to add
-  const unsigned lanes = THREADS >= 32 ? 0xffffffffu : ((1u << (THREADS & 31)) - 1) << (threadIdx.x & 31 & ~(THREADS - 1));
+  const unsigned lanes =
+      THREADS >= 32 ? 0xffffffffu : ((1u << (THREADS & 31)) - 1) << (threadIdx.x & 31 & ~(THREADS - 1));
 #pragma unroll
   for (int o = (THREADS < 32 ? THREADS : 32) / 2; o > 0; o >>= 1)
     part_merge(m, s, __shfl_xor_sync(lanes, m, o), __shfl_xor_sync(lanes, s, o));
-  if (W > 1) {
+  if constexpr (W > 1) {
     const int w = tid >> 5, l = tid & 31;
     if (l == 0) { smax[w] = m; ssum[w] = s; }
     __syncthreads();
-    if (w > 0) return;
-    m = l < W ? smax[l] : -INFINITY;
-    s = l < W ? ssum[l] : 0.f;
+    m = smax[l % W];
+    s = ssum[l % W];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+    for (int o = W / 2; o > 0; o >>= 1)
       part_merge(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+  }
+  if (!(fabsf(m) < FAR)) {                           // all threads of the part
+    const int from = head + begin * VN, to = head + end * VN, most = part == 0 ? z.V - nvec * VN : 0;
+    auto each = [&](auto f) {
+      for (int i = from + tid; i < to; i += THREADS) f(to_f32<T>(x[i]));
+      for (int i = tid; i < most; i += THREADS) f(to_f32<T>(x[i < head ? i : nvec * VN + i]));
+    };
+    float top = -INFINITY, sum = 0.f;
+    each([&](float v) { top = fmaxf(top, v); });
+#pragma unroll
+    for (int o = (THREADS < 32 ? THREADS : 32) / 2; o > 0; o >>= 1)
+      top = fmaxf(top, __shfl_xor_sync(lanes, top, o));
+    if (W > 1) {
+      __syncthreads();                               // both have been read
+      if ((tid & 31) == 0) smax[tid >> 5] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < W; ++w) top = fmaxf(top, smax[w]);
+    }
+    m = top;                                         // -inf: a part without a finite element, its sum 0 or NaN
+    if (top > -INFINITY) {
+      each([&](float v) { sum += exp2_fast((v - top) * k); });
+#pragma unroll
+      for (int o = (THREADS < 32 ? THREADS : 32) / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(lanes, sum, o);
+      if (W > 1) {
+        if ((tid & 31) == 0) ssum[tid >> 5] = sum;
+        __syncthreads();
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) sum += ssum[w];
+      }
+      s = -sum;
+    }
   }
   if (tid == 0) {
     parts[row * n_parts + part] = make_float2(m, s);
@@ -222,23 +270,31 @@ row_fwd_kernel(const Logits z, float2* __restrict__ parts, float* __restrict__ a
 // cluster, and one that joins (65536 rows of 256: 38 -> 18 us with the pass).
 constexpr int TAIL_THREADS = 512, TAIL_CTAS = 8, TAIL_ONE = 512, TAIL_MANY = 8192, TAIL_MOST = 296;
 enum { WHOLE, SHARE, JOIN };       // one launch, or the first and the second of two
+
 // What the forward's pass over the rows has left: joined for the backward, and a row's log-probability.
 struct Rows {
   const float2* parts;             // [rows][n_parts]
   const float* at_label;
   float2* stats;                   // [rows]
   int n_parts;
-  __device__ __forceinline__ float2 join(long long r) const {
+  __device__ __forceinline__ float2 join(const Logits& z, long long r) const {
     float2 v = parts[r * n_parts];
     for (int i = 1; i < n_parts; ++i) {
       const float2 w = parts[r * n_parts + i];
-      part_merge(v.x, v.y, w.x, w.y);
+      if (!(v.y < 0.f) && !(w.y < 0.f)) {
+        part_merge(v.x, v.y, w.x, w.y);
+      } else {                                       // the sum with the greater reference takes the other one
+        const double d = reference(z, w) - reference(z, v);
+        const float2 less = d > 0.0 ? v : w;
+        if (d > 0.0) v = w;
+        v.y += copysignf(exp2f(-fabsf((float)d)), v.y) * fabsf(less.y);
+      }
     }
     return v;
   }
 };
 __device__ __forceinline__ double log_prob(const Logits& z, float2 stat, float at_label) {
-  const double l = LN2 * ((double)at_label * (double)z.k - (double)stat.x) - log((double)stat.y) - EXP2_LOW;
+  const double l = LN2 * ((double)at_label * (double)z.k - reference(z, stat)) - log(fabs((double)stat.y)) - EXP2_LOW;
   return l > 0.0 ? 0.0 : l;          // a row of one word by 1e-7; a NaN stays
 }
 __device__ __forceinline__ double warp_sum64(double v) {
@@ -265,7 +321,7 @@ policy_tail_kernel(const Logits z, const Rows rows, const PolicyArgs p, double* 
        r += (long long)ctas * TAIL_THREADS) {
     // all at once, whether the row counts (its statistics are written only then) or not
     const long long n = r / z.T, label = z.labels[r];
-    const float2 stat = rows.join(r);
+    const float2 stat = rows.join(z, r);
     const float logit = rows.at_label[r], old = p.old[r], ref = p.ref ? p.ref[r] : 0.f;
     const float adv = p.adv[n * p.adv_n + (r - n * z.T) * p.adv_t];
     if (!z.counts(label)) {
@@ -335,7 +391,7 @@ preference_tail_kernel(const Logits z, const Rows rows, const float* __restrict_
     double t = 0.0;
     for (long long j = part * 32 + lane; j < z.T; j += parts * 32) {
       const long long r = (long long)n * z.T + j, label = z.labels[r];
-      const float2 stat = rows.join(r);              // written where the row counts
+      const float2 stat = rows.join(z, r);              // written where the row counts
       const float logit = rows.at_label[r];
       if (z.counts(label)) {
         rows.stats[r] = stat;
@@ -411,7 +467,12 @@ row_bwd_kernel(const Logits z, const float2* __restrict__ stats, const float* __
     return;
   }
   const float2 st = stats[row];
-  const float M = st.x == -INFINITY ? 0.f : st.x, q = -g / st.y, k = z.k;
+  const float M = st.x == -INFINITY ? 0.f : st.x, q = -g / fabsf(st.y), k = z.k;
+  if (st.y < 0.f) {
+    for (int i = first; i < z.V; i += step)
+      d[i] = from_f32<T>(fmaf(exp2_fast((to_f32<T>(x[i]) - M) * k), q, i == label ? g : 0.f));
+    return;
+  }
   auto grad = [&](float v, int i) { return fmaf(exp2_fast(fmaf(v, k, -M)), q, i == label ? g : 0.f); };
   if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) != 0) {
     for (int i = first; i < z.V; i += step) d[i] = from_f32<T>(grad(to_f32<T>(x[i]), i));
@@ -595,8 +656,8 @@ PF_API int pf_policy_fwd(const void* logits, const void* actions, const void* ol
 // be null.  Rows that lie to 16 bytes as the logits' do are written by vectors, others element by element.
 PF_API int pf_token_loss_bwd(const void* logits, const void* labels, const void* stats, const void* coef,
                              const void* gout, const void* inv, void* dlogits, long long dlogits_row,
-                             long long N, int T, int V, long long n, long long t, long long ignore_index, int per, float inv_temperature,
-                             int dtype, int sm_count, void* stream) {
+                             long long N, int T, int V, long long n, long long t, long long ignore_index, int per,
+                             float inv_temperature, int dtype, int sm_count, void* stream) {
   Logits z;
   const int code = logits_of(z, logits, labels, N, T, V, n, t, ignore_index, inv_temperature, dtype);
   if (code) return code;

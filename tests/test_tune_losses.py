@@ -208,6 +208,52 @@ def test_a_row_that_counts_keeps_its_nan(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V,T", [(9, 4), (260, 6), (260, 3000), (2500, 3), (40001, 3)])
+def test_rows_far_from_zero(V, T, dtype, device):
+    """Rows that count though a mask of the type's lowest value, or of another large one, has left them nothing: the
+    softmax of their differences.  Per row: everything masked; all but the label, the label alone; in the first half
+    only; a large positive mask; next to words of ordinary size; -inf beside it.
+
+    Differences of such values are 0 or so large that the exponential is 0, where nothing is rounded but the sum:
+    l is off by R of the module's bound without its |k z|, and by E |l|."""
+    low = torch.finfo(dtype).min
+    z, _ = batch(2, T, V, device, dtype, 3)
+    labels = torch.full((2, T), 1, device=device)
+    rows = z.view(-1, V)
+    for i in range(0, 2 * T):
+        fill, kind = (low, -1e9, -1e30, 1e12, -5e6, 3e38)[i % 6], i % 7
+        if kind < 5:
+            rows[i] = fill
+        if kind == 1:
+            rows[i, 1] = fill * 1.5 if abs(fill) < 1e38 else fill / 2
+        elif kind == 2:
+            rows[i, V // 2:] = -math.inf
+        elif kind == 3:
+            rows[i, V // 2:] = low
+        elif kind == 4:
+            rows[i, V // 2:] = -7.0
+        elif kind == 5:
+            rows[i, V // 2:] = min(fill, -fill)
+    z.requires_grad_()
+    x = z.detach().double()
+    l = torch.log_softmax(x, -1)[..., 1]
+    p = torch.softmax(x, -1)
+    ok = l > -50
+    # words of ordinary size are the only ones whose differences have a rounding, of |k z| < 24
+    R = (V / 32 + 68 + 4 * 24) * E + 2.0 ** -22
+    out = ops.policy_loss(z, labels, torch.where(ok, l.float(), -3.0), torch.ones(2, 1, device=device))
+    near(out.logps, l, R + 2 * E * l.abs())
+    # old = l: the ratio is 1 but for l's rounding, and the gradient -(onehot - p) / (2 T); 0 for the impossible
+    (dz,) = torch.autograd.grad(out.loss, z)
+    g = torch.where(ok, -1.0, 0.0).double() / (2 * T)
+    dg = (R + 3 * E * l.abs() + 2.0 ** -20) / (2 * T)
+    bound = gradient(g, dg, p, torch.full_like(l, 2 * R), labels, torch.ones_like(ok))
+    near(dz[ok], bound[0][ok], bound[1][ok])
+    assert torch.isfinite(dz).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_certain_words(device):
     """A word that has all the probability, alone in its vocabulary or not: no log-probability above 0."""
     dtype = torch.float32 if device == "cpu" else torch.bfloat16
