@@ -336,9 +336,11 @@ policy_tail_kernel(const Logits z, const Rows rows, const PolicyArgs p, double* 
     double term = clipped ? -held : -free, c = clipped ? 0.0 : -free, each = 0.0;
     if (p.ref) {
       const double d = (double)ref - lp, e = expm1(d);
-      each = e - d;
-      term += p.kl * each;
-      c -= p.kl * e;
+      each = e == INFINITY ? e : e - d;
+      if (p.kl != 0.f) {                             // 0 x inf is not 0
+        term += p.kl * each;
+        c -= p.kl * e;
+      }
     }
     p.logp[r] = (float)lp;
     p.coef[r] = (float)(c * p.inv_temperature);
@@ -391,7 +393,7 @@ preference_tail_kernel(const Logits z, const Rows rows, const float* __restrict_
     double t = 0.0;
     for (long long j = part * 32 + lane; j < z.T; j += parts * 32) {
       const long long r = (long long)n * z.T + j, label = z.labels[r];
-      const float2 stat = rows.join(z, r);              // written where the row counts
+      const float2 stat = rows.join(z, r);           // written where the row counts
       const float logit = rows.at_label[r];
       if (z.counts(label)) {
         rows.stats[r] = stat;

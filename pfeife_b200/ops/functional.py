@@ -1113,8 +1113,11 @@ def policy_fwd(logits: Tensor, actions: Tensor, old_logps: Tensor, advantages: T
     kl = torch.zeros((), device=logits.device)
     if ref_logps is not None:
         d = ref_logps.float().double() - logp
-        each = torch.expm1(d) - d
-        term, coef, kl = term + kl_coef * each, coef - kl_coef * torch.expm1(d), mean(each)
+        e = torch.expm1(d)
+        each = torch.where(e == math.inf, e, e - d)
+        kl = mean(each)
+        if kl_coef != 0.0:
+            term, coef = term + kl_coef * each, coef - kl_coef * e
     coef = (coef / temperature).masked_fill(~counted, 0.0).float()
     return mean(term), logp.float(), kl, mean(cut.double()), stats, coef, inv.float()
 

@@ -269,6 +269,26 @@ def test_certain_words(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_an_impossible_token_beside_a_reference(device):
+    """A sampled word that a mask has taken since: its estimate of the KL is infinite, and reaches neither the loss
+    nor a gradient where the coefficient is 0."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    z, labels = batch(2, 3, 40, device, dtype, 2, masked=0.0)
+    labels[0, 1] = 7
+    z[0, 1, 7] = -math.inf
+    z.requires_grad_()
+    old, adv = torch.full((2, 3), -3.0, device=device), torch.ones(2, 3, device=device)
+    alone = ops.policy_loss(z, labels, old, adv)
+    for ref in (old, old - 800):
+        out = ops.policy_loss(z, labels, old, adv, ref)
+        assert out.kl == math.inf and out.logps[0, 1] == -math.inf
+        assert torch.equal(out.loss, alone.loss) and torch.isfinite(out.loss)
+        for a, b in zip(torch.autograd.grad(out.loss, z), torch.autograd.grad(alone.loss, z, retain_graph=True)):
+            assert torch.equal(a, b) and torch.isfinite(a).all()
+        assert ops.policy_loss(z, labels, old, adv, ref, kl_coef=0.1).loss == math.inf
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_nothing_counts(device):
     dtype = torch.float32 if device == "cpu" else torch.float16
     z, labels = batch(2, 4, 33, device, dtype, 1)
