@@ -892,8 +892,9 @@ variable_list token_loss_backward(AutogradContext* ctx, const Tensor& g, int inp
       const Env e(z);
       out[0] = rows_like(z);
       ok(pf_token_loss_bwd(z.data_ptr(), labels.data_ptr(), kept.stats(), kept.coef(), g.data_ptr(), kept.one_over(),
-                           out[0].data_ptr(), out[0].size(1) > 1 ? out[0].stride(1) : out[0].size(2), N, (int)T, (int)z.size(2), z.stride(0), z.stride(1), ignore,
-                           inv ? 1 : (int)T, (float)(1.0 / temperature), code_of(z), e.sms, e.stream),
+                           out[0].data_ptr(), T > 1 ? out[0].stride(1) : z.size(2), N, (int)T, (int)z.size(2),
+                           z.stride(0), z.stride(1), ignore, inv ? 1 : (int)T, (float)(1.0 / temperature), code_of(z),
+                           e.sms, e.stream),
          "pf_token_loss_bwd");
       return 0;
     });
@@ -1422,8 +1423,8 @@ PF_OP(policy_loss) {
   for (const Tensor* t : {&old, &ref})
     if (t->defined() && (!packed_floats(*t, N * T) || t->dim() != 2 || t->size(0) != N || t->requires_grad()))
       Py_RETURN_NONE;
-  if (!advantages_fit(adv, N, T) || adv.requires_grad() || !(c.temperature > 0.0 && c.temperature < INFINITY) || !(c.low >= 0.0 && c.low <= 1.0) ||
-      !(c.high >= 0.0))
+  if (!advantages_fit(adv, N, T) || adv.requires_grad() || !(c.temperature >= 1e-30 && c.temperature <= 1e30) ||
+      !(c.low >= 0.0 && c.low <= 1.0) || !(c.high >= 0.0))
     Py_RETURN_NONE;
   if (!recorded(z))
     return run(z, [&] {

@@ -1169,9 +1169,9 @@ def policy_loss(logits: Tensor, actions: Tensor, old_logps: Tensor, advantages: 
         for name, t in (("old_logps", old_logps), ("ref_logps", ref_logps)):
             if t is not None and t.shape != shape:
                 raise ValueError(f"policy_loss: {name} {tuple(shape)} are needed, not {tuple(t.shape)}")
-    if not 0.0 < temperature < math.inf or not 0.0 <= clip_low <= 1.0 or not clip_high >= 0.0:
-        raise ValueError(f"policy_loss: a temperature {temperature} above 0, clip_low {clip_low} between 0 and 1 and "
-                         f"clip_high {clip_high} of at least 0 are needed")
+    if not 1e-30 <= temperature <= 1e30 or not 0.0 <= clip_low <= 1.0 or not clip_high >= 0.0:
+        raise ValueError(f"policy_loss: a temperature {temperature} of 1e-30 to 1e30, clip_low {clip_low} between 0 "
+                         f"and 1 and clip_high {clip_high} of at least 0 are needed")
     if advantages.shape != shape:
         try:
             advantages = advantages.expand(shape)

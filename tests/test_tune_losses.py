@@ -254,6 +254,26 @@ def test_rows_far_from_zero(V, T, dtype, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("V", [65, 3001])
+def test_temperatures_of_all_sizes(V, device):
+    """From the largest word alone to all words alike.  z / temperature is rounded twice, and its difference to the
+    largest once: l is off by 4 E of it besides R.  What fp32 cannot invert is refused."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    z, labels = batch(2, 4, V, device, dtype, 8, masked=0.0)
+    v = torch.full((2, 4), -3.0, device=device)
+    for temperature in (1e-30, 1e-12, 1e-6, 1e-3, 1e6, 1e30):
+        x = z.double() / temperature
+        far = (x - x.amax(-1, keepdim=True)).gather(-1, labels.unsqueeze(-1))[..., 0].abs()
+        l = torch.log_softmax(x, -1).gather(-1, labels.unsqueeze(-1))[..., 0]
+        big = x.abs().amax(-1).clamp(max=2.0 ** 22) * 1.4427      # beyond it there is no rounded reference
+        R = (V / 32 + 68 + 4 * big) * E + 2.0 ** -22
+        near(ops.policy_loss(z, labels, v, v + 1, temperature=temperature).logps, l, R + 4 * E * far + E * l.abs())
+    for temperature in (1e-31, 1e-320, 1e31):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.policy_loss(z, labels, v, v, temperature=temperature)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_certain_words(device):
     """A word that has all the probability, alone in its vocabulary or not: no log-probability above 0."""
     dtype = torch.float32 if device == "cpu" else torch.bfloat16
