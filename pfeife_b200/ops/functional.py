@@ -1373,8 +1373,14 @@ def _scaled_frequencies(rotary_dim: int, theta: float, s: RopeScaling, device) -
     """-> (radians per position of each pair, in 64 bits; what cosines and sines are multiplied by)"""
     if s.kind not in ("linear", "ntk", "yarn", "bands"):
         raise ValueError(f"RopeScaling: unknown kind {s.kind!r}")
-    if s.factor < 1.0 or s.original_len < 1 or s.slow <= 0.0 or (s.fast is not None and s.fast <= s.slow):
-        raise ValueError(f"RopeScaling: factor at least 1, a positive length and 0 < slow < fast are needed: {s}")
+    fast = s.fast if s.fast is not None else 32.0 if s.kind == "yarn" else 4.0
+    numbers = (s.factor, s.original_len, s.slow, fast, 1.0 if s.grown is None else s.grown)
+    if not (all(map(math.isfinite, numbers)) and s.factor >= 1.0 and s.original_len >= 1):
+        raise ValueError(f"RopeScaling: a factor of at least 1, a positive length and finite numbers are needed: {s}")
+    if s.kind in ("yarn", "bands") and not 0.0 < s.slow < fast:
+        raise ValueError(f"RopeScaling: 0 < slow < fast are needed, not {s.slow} and {fast}: {s}")
+    if not (math.isfinite(theta) and (theta > 1.0 if s.kind == "yarn" else theta > 0.0)):
+        raise ValueError(f"RopeScaling: {s.kind} has no frequencies of the base {theta}")
     i = torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float64)
     if s.kind == "ntk":
         if rotary_dim < 4:
@@ -1386,12 +1392,12 @@ def _scaled_frequencies(rotary_dim: int, theta: float, s: RopeScaling, device) -
     elif s.kind == "yarn":
         def pair(turns):                  # number of the frequency that turns so often
             return rotary_dim * math.log(s.original_len / (turns * 2 * math.pi)) / (2 * math.log(theta))
-        low = max(math.floor(pair(s.fast or 32.0)), 0)
+        low = max(math.floor(pair(fast)), 0)
         high = min(math.ceil(pair(s.slow)), rotary_dim - 1)
         ramp = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0, 1)
         inv = inv * (1 - ramp) + inv / s.factor * ramp
     elif s.kind == "bands":
-        kept = ((s.original_len * inv / (2 * math.pi) - s.slow) / ((s.fast or 4.0) - s.slow)).clamp(0, 1)
+        kept = ((s.original_len * inv / (2 * math.pi) - s.slow) / (fast - s.slow)).clamp(0, 1)
         inv = inv * kept + inv / s.factor * (1 - kept)
     grown = s.grown if s.grown is not None else 0.1 * math.log(s.factor) + 1.0 if s.kind == "yarn" else 1.0
     return inv, grown

@@ -625,3 +625,22 @@ def test_entry_points_refuse_what_they_cannot_read():
     for empty in (dict(B=0), dict(S=0), dict(Hq=0)):
         assert fwd(**empty) == 0, empty
     assert calls.pf_heads_bwd_rows(32, 8, 148) >= 2 * 148
+
+
+def test_scalings_whose_ramp_would_run_backwards():
+    """The defaults of ``fast`` are held to the same order as a value that is given, and nothing that is no number
+    becomes a table."""
+    S = ops.RopeScaling
+    for bad in (S("bands", 2.0, slow=8.0), S("bands", 2.0, slow=4.0), S("yarn", 2.0, slow=64.0), S("yarn", 2.0, slow=32.0),
+                S("bands", 2.0, fast=0.0), S("linear", math.nan), S("ntk", math.inf), S("yarn", 2.0, fast=math.nan),
+                S("yarn", 2.0, grown=math.inf), S("bands", 2.0, slow=math.nan), S("linear", 2.0, math.nan)):
+        with pytest.raises(ValueError, match="RopeScaling"):
+            ops.rope_tables(8, 16, scaling=bad)
+    for kind, theta in (("yarn", 1.0), ("yarn", 0.5), ("linear", 0.0), ("bands", -2.0), ("ntk", math.nan)):
+        with pytest.raises(ValueError, match="base"):
+            ops.rope_tables(8, 16, theta, scaling=S(kind, 2.0))
+    # an order that is right, with a value given or not: the fastest pair is kept, the slowest divided
+    for good in (S("bands", 2.0, 64), S("bands", 2.0, 64, slow=3.5), S("bands", 2.0, 64, fast=8.0, slow=6.0)):
+        cos, _ = ops.rope_tables(8, 16, scaling=good)
+        assert abs(float(cos[1, 0]) - math.cos(1.0)) < 1e-7
+        assert abs(float(cos[1, 7]) - math.cos(_frequency("linear", 7, 16, 1e4, 2.0, 64))) < 1e-7
