@@ -1362,9 +1362,9 @@ PF_OP(rotate_heads) {
   const Tensor x = a.tensor(0), cos = a.tensor(1), sin = a.tensor(2), pos = a.tensor(3, true);
   const bool interleaved = a.boolean(4);
   if (!a.fits || !all_plain(x, cos, sin, pos) || !head_view_fits(x, x.dim() == 5 ? 5 : 4) ||
-      !angles_fit(x, cos, sin, pos))
+      !angles_fit(x, cos, sin, pos) || recorded(cos, sin))            // tables get no gradient: refused in Python
     Py_RETURN_NONE;
-  if (!recorded(x, cos, sin))
+  if (!recorded(x))
     return run(x, [&] { return unrecorded([&] { return rotate(x, cos, sin, pos, interleaved, false); }); });
   return run(x, [&] { return DirectRotate::apply(x, cos, sin, maybe(pos), interleaved); });
   END_HANDLE_TH_ERRORS
@@ -1380,9 +1380,9 @@ PF_OP(norm_rotate_heads) {
   const double eps = a.real(7);
   const bool interleaved = a.boolean(8);
   if (!a.fits || !all_plain(q, k, wq, wk, cos, sin, pos) || !(k.defined() ? same_heads(q, k) : head_view_fits(q, 5)) ||
-      !gain_fits(wq, q) || !gain_fits(wk, q) || !angles_fit(q, cos, sin, pos))
+      !gain_fits(wq, q) || !gain_fits(wk, q) || !angles_fit(q, cos, sin, pos) || recorded(cos, sin))
     Py_RETURN_NONE;
-  if (!recorded(q, k, wq, wk, cos, sin))
+  if (!recorded(q, k, wq, wk))
     return run(q, [&] {
       at::AutoDispatchBelowADInplaceOrView guard;
       return norm_rotate(q, k, wq, wk, cos, sin, pos, eps, interleaved);

@@ -1433,6 +1433,8 @@ def _check_angles(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tenso
                          f"and {tuple(sin.shape)}")
     if cos.device != x.device or sin.device != x.device:
         raise ValueError(f"tables on {cos.device} and {sin.device} for heads on {x.device}")
+    if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+        raise ValueError("tables get no gradient; detach them")
     if cos.shape[0] < (S if positions is None else min(S, 1)):
         raise ValueError(f"tables of {cos.shape[0]} rows for {S} tokens")
     if positions is None:

@@ -644,3 +644,27 @@ def test_scalings_whose_ramp_would_run_backwards():
         cos, _ = ops.rope_tables(8, 16, scaling=good)
         assert abs(float(cos[1, 0]) - math.cos(1.0)) < 1e-7
         assert abs(float(cos[1, 7]) - math.cos(_frequency("linear", 7, 16, 1e4, 2.0, 64))) < 1e-7
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_tables_that_want_a_gradient(device):
+    """They get none, and are told so; where nothing is recorded they are tables as any other."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    tables = angles(6, 8, device)
+    x = heads(2, 6, 3, 16, device, dtype, 1)
+    qkv = heads(2, 6, 6, 16, device, dtype, 2).view(2, 6, 3, 2, 16)
+    w, pos = torch.ones(16, device=device), torch.arange(6, device=device)
+    calls = [lambda c, s: ops.rope(x, c, s, pos), lambda c, s: ops.rope(x, c, s, interleaved=True),
+             lambda c, s: ops.rope(x, c[:, :4], s[:, :4]), lambda c, s: ops.rope_qkv(qkv, c, s, pos),
+             lambda c, s: ops.qk_norm_rope(x, x, w, w, c, s), lambda c, s: ops.qk_norm_rope_qkv(qkv, w, w, c, s)]
+    for i in range(2):
+        wanted = [t.clone().requires_grad_(i == j) for j, t in enumerate(tables)]
+        for call in calls:
+            for leaf in (x, qkv):
+                leaf.requires_grad_(i == 1)
+            with pytest.raises(ValueError, match="no gradient"):
+                call(*wanted)
+            with torch.no_grad():
+                got, want = call(*wanted), call(*tables)
+            for a, b in zip(got, want):
+                assert torch.equal(a, b) and not a.requires_grad
