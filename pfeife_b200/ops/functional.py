@@ -969,6 +969,7 @@ def _tokens_counted(labels: Tensor, V: int, ignore_index: int) -> Tensor:
 
 def _token_logps_ref(logits: Tensor, labels: Tensor, temperature: float, ignore_index: int):
     """(log softmax(logits / temperature) at the labels in 64 bits, 0 where none counts; which count; the stats)"""
+    labels = labels.long()               # as the kernel reads them: neither V nor ignore_index need fit their type
     counted = _tokens_counted(labels, logits.shape[-1], ignore_index)
     z = _wide(logits) / temperature
     top = z.amax(-1, keepdim=True)
@@ -1011,6 +1012,7 @@ def token_loss_bwd(dloss: Tensor, logits: Tensor, labels: Tensor, stats: Tensor,
     sequence [N] or each row [N, T]."""
     if _native(logits) or (logits.is_cuda and logits.dtype == torch.float32):
         return kx.token_loss_bwd(dloss, logits, labels, stats, coef, inv, ignore_index, temperature)
+    labels = labels.long()
     counted = _tokens_counted(labels, logits.shape[-1], ignore_index)
     coef = coef.float()                  # the declared type, as the kernel reads it
     g = (coef if coef.dim() == 2 else coef.unsqueeze(1)) * dloss
@@ -1058,7 +1060,8 @@ class PolicyLoss(NamedTuple):
 
 
 def _check_tokens(what: str, logits: Tensor, labels: Tensor, **values: Optional[Tensor]) -> None:
-    if labels.shape != logits.shape[:-1] or labels.device != logits.device or labels.is_floating_point():
+    if labels.shape != logits.shape[:-1] or labels.device != logits.device or labels.is_floating_point() \
+            or labels.is_complex():
         raise ValueError(f"{what}: integer labels {tuple(logits.shape[:-1])} on {logits.device} are needed, not "
                          f"{labels.dtype} {tuple(labels.shape)} on {labels.device}")
     for name, t in values.items():

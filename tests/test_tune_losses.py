@@ -659,3 +659,28 @@ def test_a_decoder_with_normed_heads_tuned_on_a_loss(loss, device):
     assert abs(got - want) < rel * abs(want) + rel * 0.1
     for name, a, b in zip(names, grads, exact):
         assert (a.double() - b).norm() <= rel * b.norm() + 1e-12, name
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int16, torch.int8, torch.uint8])
+def test_labels_of_small_types(dtype, device):
+    """Numbers are read as 64 bits before they are compared: a vocabulary or an ignored number beyond the labels' type
+    is neither an error nor wrapped around."""
+    kind = torch.float32 if device == "cpu" else torch.bfloat16
+    z, _ = batch(4, 5, 400, device, kind, 4)
+    z.requires_grad_()
+    labels = torch.arange(20, device=device).view(4, 5) * 6            # up to 114
+    v, ref = torch.full((4, 5), -5.0, device=device), torch.zeros(4, device=device)
+    for ignore in (-100, 6, 300):
+        got, want = [], []
+        for t, to in ((labels.to(dtype), got), (labels, want)):
+            a = ops.preference_loss(z, t, ref, ignore_index=ignore)
+            b = ops.policy_loss(z, t, v, v + 6, v, kl_coef=0.1, ignore_index=ignore)
+            to += [a.loss, a.rewards, *b, *torch.autograd.grad(a.loss + b.loss, z)]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert bool(want[-1][0, 1].any()) == (ignore != 6)
+    for wrong in (labels.float(), labels.to(torch.complex64)):
+        with pytest.raises(ValueError, match="labels"):
+            ops.preference_loss(z, wrong, ref)
+        with pytest.raises(ValueError, match="labels"):
+            ops.policy_loss(z, wrong, v, v)
