@@ -294,7 +294,9 @@ struct Rows {
   }
 };
 __device__ __forceinline__ double log_prob(const Logits& z, float2 stat, float at_label) {
-  const double l = LN2 * ((double)at_label * (double)z.k - reference(z, stat)) - log(fabs((double)stat.y)) - EXP2_LOW;
+  // the far form's largest exponentials are 2^0, which is exact
+  const double low = stat.y < 0.f ? 0.0 : EXP2_LOW;
+  const double l = LN2 * ((double)at_label * (double)z.k - reference(z, stat)) - log(fabs((double)stat.y)) - low;
   return l > 0.0 ? 0.0 : l;          // a row of one word by 1e-7; a NaN stays
 }
 __device__ __forceinline__ double warp_sum64(double v) {

@@ -684,3 +684,22 @@ def test_labels_of_small_types(dtype, device):
             ops.preference_loss(z, wrong, ref)
         with pytest.raises(ValueError, match="labels"):
             ops.policy_loss(z, wrong, v, v)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("V", [2, 300, 5000, 40001])
+def test_rows_far_from_zero_hide_nothing(V, device):
+    """The exponential of the largest word is 1 there without a rounding, and so are those of all that are alike: a
+    word that has all the probability has a log-probability of 0, V words alike -ln V to its rounding in 32 bits."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    for value in (1e8, -1e30):
+        z = torch.full((2, 3, V), value, device=device)
+        z[:, 1:, V // 2] = value * (1.5 if value > 0 else 0.5)
+        z, labels = z.to(dtype), torch.full((2, 3), V // 2, dtype=torch.int64, device=device)
+        v = torch.zeros(2, 3, device=device)
+        logps = ops.policy_loss(z, labels, v, v).logps
+        assert not logps[:, 1:].any()
+        # half a step of a value between 2^k and 2^(k+1), beside 64-bit logarithms
+        assert ((logps[:, 0].double() + math.log(V)).abs() <= 2.0 ** (math.floor(math.log2(math.log(V))) - 24) + 1e-12).all()
+        rewards = ops.preference_loss(z[:, 1:], labels[:, 1:], torch.zeros(2, device=device)).rewards
+        assert not rewards.any()
