@@ -114,17 +114,17 @@ PF_DECL int pf_token_loss_scratch(long long N, int T, int V, int dtype, int sm_c
 PF_DECL int pf_preference_fwd(const void* logits, const void* labels, const void* ref, void* loss,
                               void* rewards, void* stats, void* coef, void* scratch, long long N,
                               int T, int V, long long n, long long t, long long ignore_index,
-                              float beta, float smoothing, int dtype, int sm_count, void* stream);
+                              double beta, double smoothing, int dtype, int sm_count, void* stream);
 PF_DECL int pf_policy_fwd(const void* logits, const void* actions, const void* old, const void* ref,
                           const void* adv, void* loss, void* kl, void* clipped, void* inv,
                           void* logp, void* coef, void* stats, void* scratch, long long N, int T,
                           int V, long long n, long long t, long long adv_n, long long adv_t,
-                          long long ignore_index, float low, float high, float kl_coef,
-                          float inv_temperature, int dtype, int sm_count, void* stream);
+                          long long ignore_index, double low, double high, double kl_coef,
+                          double inv_temperature, int dtype, int sm_count, void* stream);
 PF_DECL int pf_token_loss_bwd(const void* logits, const void* labels, const void* stats,
                               const void* coef, const void* gout, const void* inv, void* dlogits,
                               long long dlogits_row, long long N, int T, int V, long long n,
-                              long long t, long long ignore_index, int per, float inv_temperature,
+                              long long t, long long ignore_index, int per, double inv_temperature,
                               int dtype, int sm_count, void* stream);
 
 // ---- attn_sm100.cu : flash attention on tcgen05 (strides in elements: batch, seq, head)

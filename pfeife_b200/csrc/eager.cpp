@@ -893,7 +893,7 @@ variable_list token_loss_backward(AutogradContext* ctx, const Tensor& g, int inp
       out[0] = rows_like(z);
       ok(pf_token_loss_bwd(z.data_ptr(), labels.data_ptr(), kept.stats(), kept.coef(), g.data_ptr(), kept.one_over(),
                            out[0].data_ptr(), T > 1 ? out[0].stride(1) : z.size(2), N, (int)T, (int)z.size(2),
-                           z.stride(0), z.stride(1), ignore, inv ? 1 : (int)T, (float)(1.0 / temperature), code_of(z),
+                           z.stride(0), z.stride(1), ignore, inv ? 1 : (int)T, 1.0 / temperature, code_of(z),
                            e.sms, e.stream),
          "pf_token_loss_bwd");
       return 0;
@@ -920,7 +920,7 @@ variable_list preference_forward(const Tensor& z, const Tensor& labels, const Te
   const Tensor loss = empty({}, at::kFloat, z), rewards = floats(N, z), scratch = loss_scratch(e, z, N, T);
   ok(pf_preference_fwd(z.data_ptr(), labels.data_ptr(), ref.data_ptr(), loss.data_ptr(), rewards.data_ptr(),
                        kept.stats(), kept.coef(), scratch.data_ptr(), N, (int)T, (int)z.size(2), z.stride(0),
-                       z.stride(1), ignore, (float)beta, (float)smoothing, code_of(z), e.sms, e.stream),
+                       z.stride(1), ignore, beta, smoothing, code_of(z), e.sms, e.stream),
      "pf_preference_fwd");
   return {loss, rewards};
 }
@@ -960,8 +960,8 @@ variable_list policy_forward(const Tensor& z, const Tensor& actions, const Tenso
   ok(pf_policy_fwd(z.data_ptr(), actions.data_ptr(), old.data_ptr(), at_or_null(ref), adv.data_ptr(), loss.data_ptr(),
                    kl.data_ptr(), clipped.data_ptr(), kept.one_over(), logps.data_ptr(), kept.coef(), kept.stats(),
                    scratch.data_ptr(), N, (int)T, (int)z.size(2), z.stride(0), z.stride(1),
-                   adv.size(0) > 1 ? adv.stride(0) : 0, adv.size(1) > 1 ? adv.stride(1) : 0, ignore, (float)c.low,
-                   (float)c.high, (float)c.kl, (float)(1.0 / c.temperature), code_of(z), e.sms, e.stream),
+                   adv.size(0) > 1 ? adv.stride(0) : 0, adv.size(1) > 1 ? adv.stride(1) : 0, ignore, c.low, c.high,
+                   c.kl, 1.0 / c.temperature, code_of(z), e.sms, e.stream),
      "pf_policy_fwd");
   return {loss, logps, kl, clipped};
 }

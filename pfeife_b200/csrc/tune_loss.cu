@@ -308,8 +308,7 @@ __device__ __forceinline__ double warp_sum64(double v) {
 struct PolicyArgs {
   const float *old, *ref, *adv;    // ref null: no reference
   long long adv_n, adv_t;          // strides of the advantages
-  float low, high, kl;
-  double inv_temperature;
+  double low, high, kl, inv_temperature;
   float *logp, *coef;              // coef: of the row's own term, before the mean
   float *loss, *mean_kl, *clipped, *inv;
 };
@@ -332,14 +331,14 @@ policy_tail_kernel(const Logits z, const Rows rows, const PolicyArgs p, double* 
     }
     rows.stats[r] = stat;
     const double lp = log_prob(z, stat, logit), a = adv, ratio = exp(lp - (double)old);
-    const double lo = 1.0 - (double)p.low, hi = 1.0 + (double)p.high;
+    const double lo = 1.0 - p.low, hi = 1.0 + p.high;
     const double free = ratio * a, held = fmin(fmax(ratio, lo), hi) * a;
     const bool clipped = free > held;
     double term = clipped ? -held : -free, c = clipped ? 0.0 : -free, each = 0.0;
     if (p.ref) {
       const double d = (double)ref - lp, e = expm1(d);
       each = e == INFINITY ? e : e - d;
-      if (p.kl != 0.f) {                             // 0 x inf is not 0
+      if (p.kl != 0.0) {                             // 0 x inf is not 0
         term += p.kl * each;
         c -= p.kl * e;
       }
@@ -386,7 +385,7 @@ template <int STEP>
 __global__ void __launch_bounds__(TAIL_THREADS)
 preference_tail_kernel(const Logits z, const Rows rows, const float* __restrict__ ref, float* __restrict__ rewards,
                        float* __restrict__ loss, float* __restrict__ coef, double* __restrict__ scratch, int N,
-                       float beta, float smoothing, int ctas) {
+                       double beta, double smoothing, int ctas) {
   after_previous();
   const int warps = ctas * (TAIL_THREADS / 32), warp = blockIdx.x * (TAIL_THREADS / 32) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, parts = max(1, min(warps / N, (z.T + 31) / 32)), items = N * parts;
@@ -416,7 +415,7 @@ preference_tail_kernel(const Logits z, const Rows rows, const float* __restrict_
   auto reward = [&](int n) {
     double t = 0.0;
     for (int i = 0; i < parts; ++i) t += __ldcg(scratch + n * parts + i);
-    return (double)beta * (t - (double)ref[n]);
+    return beta * (t - (double)ref[n]);
   };
   const int P = N / 2;
   double total = 0.0;
@@ -428,10 +427,9 @@ preference_tail_kernel(const Logits z, const Rows rows, const float* __restrict_
     // -log sig(m) and -log sig(-m), sig(-m) and sig(m), none of which overflows
     const double lp = near + fmax(-m, 0.0), lm = near + fmax(m, 0.0);
     const double big = 1.0 / (1.0 + e), small = e / (1.0 + e);
-    total += smoothing < 1.f ? (1.0 - (double)smoothing) * lp : 0.0;      // 0 x inf is not 0
-    total += smoothing > 0.f ? (double)smoothing * lm : 0.0;
-    const double c = -(double)beta / P * ((1.0 - (double)smoothing) * (m > 0.0 ? small : big) -
-                                          (double)smoothing * (m > 0.0 ? big : small));
+    total += smoothing < 1.0 ? (1.0 - smoothing) * lp : 0.0;      // 0 x inf is not 0
+    total += smoothing > 0.0 ? smoothing * lm : 0.0;
+    const double c = -beta / P * ((1.0 - smoothing) * (m > 0.0 ? small : big) - smoothing * (m > 0.0 ? big : small));
     coef[p] = (float)c;
     coef[P + p] = (float)-c;
   }
@@ -513,11 +511,11 @@ using namespace pf;
 namespace {
 
 int logits_of(Logits& z, const void* at, const void* labels, long long N, int T, int V, long long n, long long t,
-              long long ignore, float inv_temperature, int dtype) {
+              long long ignore, double inv_temperature, int dtype) {
   if (dtype != PF_F32 && dtype != PF_F16 && dtype != PF_BF16) return -1;
   if (reinterpret_cast<uintptr_t>(at) % (dtype == PF_F32 ? 4 : 2)) return -2;
   if (N < 0 || T < 0 || V < 1 || N * T > 0x7fffffffll) return -3;
-  z = {at, (const long long*)labels, n, t, N * T, ignore, T, V, 1.44269504088896341f * inv_temperature};
+  z = {at, (const long long*)labels, n, t, N * T, ignore, T, V, (float)(1.44269504088896341 * inv_temperature)};
   return 0;
 }
 
@@ -616,10 +614,10 @@ PF_API int pf_token_loss_scratch(long long N, int T, int V, int dtype, int sm_co
 // backward stats (two floats a row) and coef fp32 [N].  N is even: the chosen sequences, then the rejected ones.
 PF_API int pf_preference_fwd(const void* logits, const void* labels, const void* ref, void* loss, void* rewards,
                              void* stats, void* coef, void* scratch, long long N, int T, int V, long long n,
-                             long long t, long long ignore_index, float beta, float smoothing, int dtype,
+                             long long t, long long ignore_index, double beta, double smoothing, int dtype,
                              int sm_count, void* stream) {
   Logits z;
-  int code = logits_of(z, logits, labels, N, T, V, n, t, ignore_index, 1.f, dtype);
+  int code = logits_of(z, logits, labels, N, T, V, n, t, ignore_index, 1.0, dtype);
   if (code) return code;
   if (N < 2 || N % 2) return -3;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -638,14 +636,14 @@ PF_API int pf_preference_fwd(const void* logits, const void* labels, const void*
 PF_API int pf_policy_fwd(const void* logits, const void* actions, const void* old, const void* ref, const void* adv,
                          void* loss, void* kl, void* clipped, void* inv, void* logp, void* coef, void* stats,
                          void* scratch, long long N, int T, int V, long long n, long long t, long long adv_n,
-                         long long adv_t, long long ignore_index, float low, float high, float kl_coef,
-                         float inv_temperature, int dtype, int sm_count, void* stream) {
+                         long long adv_t, long long ignore_index, double low, double high, double kl_coef,
+                         double inv_temperature, int dtype, int sm_count, void* stream) {
   Logits z;
   int code = logits_of(z, logits, actions, N, T, V, n, t, ignore_index, inv_temperature, dtype);
   if (code) return code;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const PolicyArgs p{(const float*)old, (const float*)ref, (const float*)adv, adv_n, adv_t, low, high, kl_coef,
-                     (double)inv_temperature, (float*)logp, (float*)coef, (float*)loss, (float*)kl, (float*)clipped,
+                     inv_temperature, (float*)logp, (float*)coef, (float*)loss, (float*)kl, (float*)clipped,
                      (float*)inv};
   const int n_parts = row_parts(z.rows, V, dtype, sm_count);
   const Scratch s(scratch, N, z.rows, n_parts);
@@ -661,7 +659,7 @@ PF_API int pf_policy_fwd(const void* logits, const void* actions, const void* ol
 PF_API int pf_token_loss_bwd(const void* logits, const void* labels, const void* stats, const void* coef,
                              const void* gout, const void* inv, void* dlogits, long long dlogits_row,
                              long long N, int T, int V, long long n, long long t, long long ignore_index, int per,
-                             float inv_temperature, int dtype, int sm_count, void* stream) {
+                             double inv_temperature, int dtype, int sm_count, void* stream) {
   Logits z;
   const int code = logits_of(z, logits, labels, N, T, V, n, t, ignore_index, inv_temperature, dtype);
   if (code) return code;

@@ -77,7 +77,7 @@ class _CtypesCalls:
         header = (_PKG / "csrc" / "api.h").read_text()
         for name, params in re.findall(r"PF_DECL int (pf_\w+)\(([^)]*)\)", header):
             kinds = [None if "*" in p else ctypes.c_longlong if "long long" in p
-                     else ctypes.c_float if "float" in p else ctypes.c_int
+                     else ctypes.c_double if "double" in p else ctypes.c_float if "float" in p else ctypes.c_int
                      for p in params.split(",") if p.strip()]
             setattr(self, name, self._entry(getattr(library, name), kinds))
 

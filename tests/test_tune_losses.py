@@ -703,3 +703,27 @@ def test_rows_far_from_zero_hide_nothing(V, device):
         assert ((logps[:, 0].double() + math.log(V)).abs() <= 2.0 ** (math.floor(math.log2(math.log(V))) - 24) + 1e-12).all()
         rewards = ops.preference_loss(z[:, 1:], labels[:, 1:], torch.zeros(2, device=device)).rewards
         assert not rewards.any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_borders_of_the_clipping_in_64_bits(device):
+    """A certain word has a log-probability of 0 and a ratio of exp(-old), which 64 bits place on the right side of a
+    border 1e-9 away; the borders, which have no 32 bits, are not rounded to them, nor are coefficients below their
+    range taken for 0."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    z = torch.full((1, 1, 40), -1e30, device=device)
+    z[..., 3] = -1e29
+    z, actions = z.to(dtype), torch.full((1, 1), 3, dtype=torch.int64, device=device)
+    for i in range(32):
+        old = torch.tensor([[(-1) ** i * (0.05 + 0.005 * i)]], dtype=torch.float32)
+        ratio = math.exp(-float(old))
+        for off in (-1e-9, 1e-9):
+            if ratio > 1:
+                a, clip, held = 1.0, dict(clip_low=0.5, clip_high=ratio - 1 + off), off < 0
+            else:
+                a, clip, held = -1.0, dict(clip_low=1 - ratio + off, clip_high=0.5), off < 0
+            adv = torch.full((1, 1), a, device=device)
+            assert float(ops.policy_loss(z, actions, old.to(device), adv, **clip).clipped) == held, (i, off)
+    adv = torch.ones(1, 1, device=device)
+    far = ops.policy_loss(z, actions, adv * 0, adv * 0, adv * 60, kl_coef=1e-50).loss         # 1e-50 exp(60)
+    assert float(far) == pytest.approx(1e-50 * math.exp(60), rel=1e-6)
