@@ -1079,6 +1079,9 @@ def preference_loss(logits: Tensor, labels: Tensor, ref_logps: Tensor, beta: flo
     read in 32 bits.
     With l the sum of a sequence's log-probabilities and m = beta ((l - ref of the chosen) - (l - ref of the
     rejected)) the loss is the mean of -(1 - label_smoothing) log sig(m) - label_smoothing log sig(-m).
+    Runners cut a batch on dim 0 before it is called, and nothing here could tell a chosen sequence from a rejected one:
+    each micro-batch and each data-parallel rank has to hold whole pairs in this order.  Cut [P, 2, T] between pairs and
+    lay out each part by ``transpose(0, 1).flatten(0, 1)``, or order the batch so that each part is in this order.
     Rows that do not count are not read and get a gradient of zero, whatever their logits."""
     out = _native_call("preference_loss", logits, labels, ref_logps, float(beta), float(label_smoothing), ignore_index)
     if out is not None:
@@ -1157,7 +1160,8 @@ def policy_loss(logits: Tensor, actions: Tensor, old_logps: Tensor, advantages: 
     when it was sampled; advantages: of the shape of the actions or one that expands to it ([N, 1]: one for each
     sequence), all read in 32 bits.  With l = log softmax(logits / temperature)[action] and r = exp(l - old) a token's
     term is -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(ref - l) - (ref - l) - 1), the last with
-    ``ref_logps`` [...] only; the loss is the mean over the tokens that count, 0 if there are none.
+    ``ref_logps`` [...] only; the loss is the mean over the tokens that count, 0 if there are none.  Micro-batches are
+    calls of their own: each is the mean over its own tokens, whatever their number.
     Rows that do not count are not read and get a gradient of zero, whatever their logits."""
     out = _native_call("policy_loss", logits, actions, old_logps, advantages, ref_logps, float(clip_low),
                        float(clip_high), float(kl_coef), float(temperature), ignore_index)

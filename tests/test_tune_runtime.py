@@ -2,6 +2,7 @@
 by the planner on CPU devices, and mixed precision with registered weights, eager and under CUDA graphs, on one
 GPU, against plain training of the same model."""
 import copy
+import math
 import os
 
 import pytest
@@ -121,3 +122,121 @@ def test_mixed_precision_on_one_gpu(cuda_graphs):
         moved = (q.detach() - s).norm()
         assert float((p.detach().float() - q.detach()).norm()) <= 0.1 * float(moved) + 1e-6, name
         assert moved > 0
+
+
+# ------------------------------------------------------------------------------ pairs and micro-batches
+def _documented(name, **names):
+    """The function of that name in the user's guide, over the objects given."""
+    import re
+    from pathlib import Path
+    guide = (Path(__file__).resolve().parent.parent / "README.md").read_text()
+    for block in re.findall(r"```python\n(.*?)```", guide, re.S):
+        if f"def {name}(" in block:
+            scope = {"llama_config": llama_config, **names}
+            exec(block, scope)
+            return scope[name]
+    raise AssertionError(f"no {name} in the guide")
+
+
+def _pairs(P, T, g):
+    """[P, 2, T] ids and labels, [P, 2] log-probabilities that lie around those of some 5.5 nats a token."""
+    ids, labels = _batch(2 * P, T, g)
+    return ids.view(P, 2, T), labels.view(P, 2, T), torch.randn(P, 2, generator=g) * 4 - 5.5 * T
+
+
+def _pair_loss(logits, labels, ref):
+    """Of each pair, from the definition: logits [P, 2, T, V]"""
+    l = torch.log_softmax(logits.double(), -1).gather(-1, labels.clamp(min=0).unsqueeze(-1))[..., 0] * (labels >= 0)
+    r = 0.1 * (l.sum(-1) - ref.double())
+    return -torch.nn.functional.logsigmoid(r[:, 0] - r[:, 1])
+
+
+class Unscaled:
+    """A runner's loss scale where nothing is scaled."""
+
+    class scaler:
+        scale = staticmethod(lambda loss: loss)
+
+
+@pytest.mark.parametrize("parts", [1, 2, 3, 4])
+def test_pairs_stay_together_in_micro_batches(parts):
+    """The documented function, over what a runner's cut leaves of a batch: each part's loss is the mean over its own
+    pairs, and the sum of the gradients that of the sum."""
+    from pfeife_b200.utils.batch import split_args_kwargs
+    model = _model()
+    prefer = _documented("prefer", model=model, runner=Unscaled)
+    pairs, labels, ref = _pairs(6, 12, torch.Generator().manual_seed(parts))
+    each = _pair_loss(model(pairs.flatten(0, 1)).view(6, 2, 12, -1), labels, ref)
+    want = [c.mean() for c in torch.tensor_split(each, parts)]
+    grads = torch.autograd.grad(sum(want), list(model.parameters()))
+    got = [prefer(*args) for args in split_args_kwargs((pairs, labels, ref), {}, parts)[0]]
+    # rewards of some 0.1 * 66 nats, each 1e-6 of their value off, and a loss that moves no faster than they do
+    assert [float(l.detach()) for l in got] == pytest.approx([float(l.detach()) for l in want], abs=2e-5)
+    for p, d in zip(model.parameters(), grads):
+        assert float((p.grad - d).norm()) <= 1e-4 * float(d.norm()) + 1e-9
+
+
+def test_a_policy_loss_is_the_mean_of_its_micro_batch():
+    from pfeife_b200.utils.batch import split_args_kwargs
+    model = _model()
+    reinforce = _documented("reinforce", model=model, runner=Unscaled)
+    ids, labels = _batch(4, 12, torch.Generator().manual_seed(9))
+    labels[2:, 6:] = -100                                  # fewer tokens in the second half
+    old, adv = torch.full((4, 12), -5.5), torch.tensor([[1.0], [-1.0], [0.5], [2.0]])
+    got = [reinforce(*args) for args in split_args_kwargs((ids, labels, old, adv, old), {}, 2)[0]]
+    l = torch.log_softmax(model(ids).double(), -1).gather(-1, labels.clamp(min=0).unsqueeze(-1))[..., 0]
+    ratio, d = (l - old).exp(), old - l
+    term = -torch.minimum(ratio * adv, ratio.clamp(0.8, 1.2) * adv) + 0.04 * (d.exp() - d - 1)
+    for loss, t, n in zip(got, term.chunk(2), (labels >= 0).chunk(2)):
+        assert float(loss.detach()) == pytest.approx(float((t * n).sum().detach() / n.sum()), abs=1e-5)
+    assert (labels >= 0)[:2].sum() != (labels >= 0)[2:].sum()
+
+
+def test_pairs_of_a_manager_whose_parts_are_in_order():
+    """Sequences ordered so that each part holds its chosen ones, then their rejected ones."""
+    from pfeife_b200.runtime.manager import LocalPipeManager
+    torch._dynamo.reset()
+    model = _model()
+    option = PipeOption(device_cnt=2, batch_size=4, batch_cnt=2, cpu_test=True, no_bench_optimizer=True,
+                        verbosity="warning", ctrl_timeout=60, optimizer={"type": "sgd", "lr": 0.05})
+    pairs, labels, _ = _pairs(4, 16, torch.Generator().manual_seed(4))
+    each = _pair_loss(model(pairs.flatten(0, 1)).view(4, 2, 16, -1), labels, torch.zeros(4, 2))
+    ordered = lambda t: torch.cat([c.transpose(0, 1).flatten(0, 1) for c in t.chunk(2)])
+
+    class Loss(LossWrapper):
+        def forward(self, input, target, model=None):
+            return ops.preference_loss(input, target, input.new_zeros(len(target)), beta=0.1).loss
+    mgr = LocalPipeManager(model, Loss(), option)
+    try:
+        losses = mgr.run(ordered(labels), ordered(pairs))
+        assert [float(l) for l in losses] == pytest.approx([float(c.detach().mean()) for c in each.chunk(2)], abs=2e-5)
+    finally:
+        mgr.close()
+
+
+@pytest.mark.gpu
+def test_pairs_through_a_runner():
+    """The documented function as the step of a runner, two micro-batches of two pairs."""
+    os.environ.setdefault("WORLD_SIZE", "1")
+    os.environ.setdefault("RANK", "0")
+    os.environ.setdefault("MASTER_PORT", "29879")
+    from pfeife_b200 import PartialRunner, initialize_pfeife, partial_compiler
+    dev = initialize_pfeife().device
+    model = _model(num_layers=2).to(dev)
+    ref_model = copy.deepcopy(model)
+    option = PipeOption(device_cnt=1, batch_size=2, batch_cnt=2, mixed_precision="bf16", no_bench_optimizer=True,
+                        verbosity="warning")
+    runner = PartialRunner(option, torch.optim.SGD(model.parameters(), lr=0.0))
+    torch._dynamo.reset()
+    runner.set_exec_fn(_documented("prefer", model=torch.compile(model, backend=partial_compiler), runner=runner))
+    pairs, labels, ref = (t.to(dev) for t in _pairs(4, 16, torch.Generator().manual_seed(7)))
+    out = runner.step(pairs, labels, ref)
+    torch.cuda.synchronize()
+    runner.close()
+    ops.unregister_params()
+    with torch.no_grad():
+        each = _pair_loss(ref_model(pairs.flatten(0, 1)).view(4, 2, 16, -1), labels, ref)
+    # a log-probability by logits of some 1, rounded to 8 bits behind 40 roundings that add up at random: 0.03 each,
+    # of 24 tokens or fewer, times beta
+    for loss, want in zip(out, each.chunk(2)):
+        assert float(loss.detach()) == pytest.approx(float(want.mean()), abs=0.1 * 0.03 * math.sqrt(24) * 2)
