@@ -462,7 +462,7 @@ heads_kernel(const __grid_constant__ HeadsArgs p) {
   }
 
   if constexpr (BACK) {
-    if (!part.dw) return;                            // the same for the whole CTA
+    if (!part.turn) return;                          // the same for the whole CTA
     float(*sums)[MAX_HEAD_DIM] = reinterpret_cast<float(*)[MAX_HEAD_DIM]>(heads_smem);
     __syncwarp();
     if constexpr (R::ASYNC) cp_async_wait<0>();
@@ -500,7 +500,7 @@ heads_kernel(const __grid_constant__ HeadsArgs p) {
   }
 }
 
-// dw[part] (+)= the CTAs' sums, in their order.  blockIdx.y: the part; 32 columns and 32 shares of the rows a CTA.
+// dw of each part (+)= its CTAs' sums, in their order.  blockIdx.y: the part; 32 columns and 32 shares of the rows a CTA.
 __global__ void __launch_bounds__(1024)
 heads_fold_kernel(const float* __restrict__ part0, const float* __restrict__ part1, float* __restrict__ dw0,
                   float* __restrict__ dw1, int ctas0, int ctas1, int D, int accumulate) {
@@ -511,14 +511,14 @@ heads_fold_kernel(const float* __restrict__ part0, const float* __restrict__ par
   const int n = blockIdx.y ? ctas1 : ctas0, lane = threadIdx.x & 31, share = threadIdx.x >> 5;
   int col = blockIdx.x * 32 + lane;
   float t = 0.f;
-  if (out && col < D)
+  if (col < D)
 #pragma unroll 4
     for (int i = share; i < n; i += 32) t += in[(long long)i * D + col];
   sums[share][lane] = t;
   __syncthreads();
   t = warp_sum(sums[lane][share]);                   // a warp a column
   col = blockIdx.x * 32 + share;
-  if (out && lane == 0 && col < D) out[col] = accumulate ? out[col] + t : t;
+  if (lane == 0 && col < D) out[col] = accumulate ? out[col] + t : t;
 }
 
 }  // namespace pf
@@ -678,11 +678,12 @@ PF_API int pf_heads_fwd(const void* q, const void* k, const void* v, void* yq, v
   return 0;
 }
 
-// Rows of partial sums that pf_heads_bwd needs: floats [that many][D].  No part gets less than one CTA.
-PF_API int pf_heads_bwd_rows(int Hq, int Hk, int sm_count) { return BACK_CTAS * sm_count + 2; }
+// Rows of partial sums that pf_heads_bwd needs: floats [that many][D].  A part that has heads gets a CTA though its
+// share of them be less.
+PF_API int pf_heads_bwd_rows(int Hq, int Hk, int sm_count) { return BACK_CTAS * sm_count + (Hq > 0) + (Hk > 0); }
 
-// Gradients of pf_heads_fwd with a norm: gq, gk, gv (the outputs') -> dq, dk, dv and dwq, dwk fp32 [D] (null: not
-// needed; accumulate: added to what is there).  gv null: there are no values.
+// Gradients of pf_heads_fwd with a norm: gq, gk, gv (the outputs') -> dq, dk, dv and dwq, dwk fp32 [D]
+// (accumulate: added to what is there).  gv null: there are no values.
 PF_API int pf_heads_bwd(const void* gq, const void* gk, const void* gv, const void* q, const void* k, void* dq,
                         void* dk, void* dv, const void* wq, const void* wk, void* dwq, void* dwk, void* scratch,
                         const void* cos_t, const void* sin_t, const void* pos, long long B, int S, int Hq, int Hk,
@@ -697,18 +698,16 @@ PF_API int pf_heads_bwd(const void* gq, const void* gk, const void* gv, const vo
   if (gv) p.part[parts++] = {{}, view(dv, sdk), view(gv, sgk), nullptr, nullptr, Hk, 0, 0, 0, 0};
   const int vw = prepare(p, parts, cos_t, sin_t, pos, spos, B, S, D, R, rows, eps, dtype);
   if (vw < 0) return vw;
-  if ((long long)B * S * (Hq + 2ll * Hk) > 0x7fffffffll || !wq || !wk) return -3;
+  if ((long long)B * S * (Hq + 2ll * Hk) > 0x7fffffffll || !wq || !wk || !dwq || !dwk || !scratch) return -3;
   // the sums' rows lie where the parts' CTAs do, at most BACK_CTAS an SM and one more for each of two parts
   const int weight[3] = {3, 3, 2};
-  if (dwq) p.part[0].dw = (float*)scratch;
-  if (dwk) p.part[1].dw = (float*)scratch;
+  p.part[0].dw = p.part[1].dw = (float*)scratch;
   const int code = launch<NORM_BACK>(p, parts, weight, interleaved, dtype, vw, sm_count, stream);
   if (code) return code;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dwq || dwk)
-    after(heads_fold_kernel, dim3((D + 31) / 32, 2), 1024, 0, st)(
-        (const float*)scratch, (const float*)scratch + (long long)p.part[1].cta0 * D, (float*)dwq, (float*)dwk,
-        p.part[0].ctas, p.part[1].ctas, D, accumulate);
+  after(heads_fold_kernel, dim3((D + 31) / 32, 2), 1024, 0, st)(
+      (const float*)scratch, (const float*)scratch + (long long)p.part[1].cta0 * D, (float*)dwq, (float*)dwk,
+      p.part[0].ctas, p.part[1].ctas, D, accumulate);
   PF_CHECK_LAUNCH();
   return 0;
 }

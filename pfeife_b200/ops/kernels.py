@@ -533,10 +533,9 @@ def heads_fwd(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Tens
 
 def heads_bwd(gq: torch.Tensor, gk: torch.Tensor, gv: Optional[torch.Tensor], q: torch.Tensor, k: torch.Tensor,
               dq: torch.Tensor, dk: torch.Tensor, dv: Optional[torch.Tensor], wq: torch.Tensor, wk: torch.Tensor,
-              cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor], dwq: Optional[torch.Tensor],
-              dwk: Optional[torch.Tensor], *, eps: float, interleaved: bool = False, accumulate: bool = False
-              ) -> None:
-    """Gradients of the outputs of ``heads_fwd`` with norms -> dq, dk, dv and (None: not needed) dwq, dwk fp32 [D]."""
+              cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor], dwq: torch.Tensor,
+              dwk: torch.Tensor, *, eps: float, interleaved: bool = False, accumulate: bool = False) -> None:
+    """Gradients of the outputs of ``heads_fwd`` with norms -> dq, dk, dv and dwq, dwk fp32 [D]."""
     L = _lib.calls()
     cos, sin, positions, steps = _turns(q, cos, sin, positions)
     q, k = _heads(q), _heads(k)
@@ -550,12 +549,10 @@ def heads_bwd(gq: torch.Tensor, gk: torch.Tensor, gv: Optional[torch.Tensor], q:
     for w in (wq, wk):
         assert w.shape == (D,)
     for w in (dwq, dwk):
-        assert w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() == D)
-    assert dwq is None or dwk is None or dwq.data_ptr() != dwk.data_ptr()
+        assert w.dtype == torch.float32 and w.is_contiguous() and w.numel() == D
+    assert dwq.data_ptr() != dwk.data_ptr()
     sms, Hk = sm_count(q.device), k.shape[2]
-    scratch = None
-    if dwq is not None or dwk is not None:
-        scratch = torch.empty(L.pf_heads_bwd_rows(H, Hk, sms) * D, dtype=torch.float32, device=q.device)
+    scratch = torch.empty(L.pf_heads_bwd_rows(H, Hk, sms) * D, dtype=torch.float32, device=q.device)
     check(L.pf_heads_bwd(gq, gk, gv, q, k, dq, dk, dv, _floats(wq), _floats(wk), dwq, dwk, scratch, cos, sin,
                          positions, B, S, H, Hk, D, 2 * cos.shape[1], _steps(gq), _steps(gk), _steps(q), _steps(k),
                          _steps(dq), _steps(dk), steps, cos.shape[0], int(interleaved), eps, int(accumulate),

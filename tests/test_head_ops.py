@@ -668,3 +668,24 @@ def test_tables_that_want_a_gradient(device):
                 got, want = call(*wanted), call(*tables)
             for a, b in zip(got, want):
                 assert torch.equal(a, b) and not a.requires_grad
+
+
+def test_the_backward_entry_point_refuses_what_it_cannot_write():
+    """Both gains' gradients and the rows that their sums need are the caller's; a part without heads has no row."""
+    import ctypes
+    from pfeife_b200.csrc import build
+    from pfeife_b200.ops import _lib
+    if not build.KERNEL_LIB.exists():
+        pytest.skip("the kernel library is not built")
+    calls = _lib.load_calls(ctypes.CDLL(str(build.KERNEL_LIB), mode=ctypes.RTLD_GLOBAL))
+    t = torch.zeros(64).data_ptr()
+    z = (64, 64, 16)
+
+    def bwd(wq=t, wk=t, dwq=t, dwk=t, scratch=t, D=16, R=16, q=t, dtype=2):
+        return calls.pf_heads_bwd(t, t, None, q, t, t, t, None, wq, wk, dwq, dwk, scratch, t, t, None, 1, 1, 1, 1, D, R,
+                                  z, z, z, z, z, z, (0, 1), 1, 0, 1e-6, 0, dtype, 148, None)
+    for missing in ("wq", "wk", "dwq", "dwk", "scratch"):
+        assert bwd(**{missing: None}) == -3, missing
+    assert bwd(dtype=4) == -1 and bwd(q=t + 1) == -2 and bwd(R=18) == -3 and bwd(D=258, R=2) == -3
+    rows = [calls.pf_heads_bwd_rows(h, k, 148) for h, k in ((32, 8), (32, 0), (0, 0))]
+    assert rows == [rows[2] + 2, rows[2] + 1, 2 * 148]
