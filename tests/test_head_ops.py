@@ -689,3 +689,46 @@ def test_the_backward_entry_point_refuses_what_it_cannot_write():
     assert bwd(dtype=4) == -1 and bwd(q=t + 1) == -2 and bwd(R=18) == -3 and bwd(D=258, R=2) == -3
     rows = [calls.pf_heads_bwd_rows(h, k, 148) for h, k in ((32, 8), (32, 0), (0, 0))]
     assert rows == [rows[2] + 2, rows[2] + 1, 2 * 148]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,hq,hk,D,R,dtype,interleaved,packed", [
+    (131072, 1, 1, 16, 16, torch.bfloat16, False, False), (4097, 33, 1, 16, 16, torch.bfloat16, True, False),
+    (2048, 32, 8, 128, 128, torch.bfloat16, False, False), (2049, 24, 6, 128, 64, torch.float16, True, False),
+    (5003, 6, 2, 72, 72, torch.float32, False, False), (3001, 16, 16, 64, 64, torch.bfloat16, False, True),
+    (1777, 9, 9, 90, 90, torch.float16, True, True)], ids=str)
+def test_gains_gradients_over_many_rows(tokens, hq, hk, D, R, dtype, interleaved, packed):
+    """The sums over all heads of long sequences, whose rounding grows with their depth and not with the number of
+    rows.  A lane adds up its group's heads: at most two CTAs an SM, shared by queries and keys by their numbers, of 8
+    groups or more; then 5 sums across a warp, 8 of warps, one for each 32 CTAs and 5 across a warp.  A term is off by
+    D + 32 parts of 2^-24 of its magnitude, as elsewhere.  Rows are normal, so that a sum lies as far from 0 as the
+    root of their number, beyond the bound: one that misses a CTA or a share of the fold does not pass."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    cos, sin = angles(tokens, R // 2, "cuda")
+    torch.manual_seed(tokens)
+    new = lambda *s: torch.randn(*s, device="cuda").to(dtype)
+    wq, wk = ((1 + 0.3 * torch.randn(D, device="cuda")).requires_grad_() for _ in range(2))
+    if packed:
+        qkv, g = new(1, tokens, 3, hq, D), new(1, tokens, 3, hq, D)
+        y = ops.qk_norm_rope_qkv(qkv, wq, wk, cos, sin, EPS, interleaved=interleaved)
+        got = torch.autograd.grad(y, [wq, wk], g)
+        parts = [(qkv[:, :, i], g[:, :, i]) for i in range(2)]
+    else:
+        parts = [(new(1, tokens, h, D), new(1, tokens, h, D)) for h in (hq, hk)]
+        out = ops.qk_norm_rope(parts[0][0], parts[1][0], wq, wk, cos, sin, EPS, interleaved=interleaved)
+        got = torch.autograd.grad(out, [wq, wk], [g for _, g in parts])
+    total = hq + hk + (2 / 3 * hk if packed else 0)              # the values of a projection take CTAs too
+    at = torch.arange(tokens, device="cuda")
+    for (x, g), w, d in zip(parts, (wq, wk), got):
+        want, most = norm_turn(x, w.detach(), g, cos, sin, at, interleaved)[4:]
+        heads_here = x.shape[2]
+        ctas = max(1.0, 2 * sms * heads_here / total - 1)
+        depth = tokens * heads_here / (ctas * 8) + 1 + 5 + 8 + 2 * sms / 32 + 1 + 5
+        within(d, want, most, depth + D + 32)
+        # what would not pass: nothing at all, the other sign, and the sum without one token in six hundred
+        bound = U[d.dtype] * want.abs() + (1 + U[d.dtype]) * (depth + D + 32) * E * most
+        few = slice(0, max(1, tokens // 600))
+        where = tuple(t[few] for t in (cos, sin, at)) + (interleaved,)
+        missing = norm_turn(x[:, few], w.detach(), g[:, few], *where)[4]
+        assert float((want.abs() > bound).double().mean()) > 0.8
+        assert float((missing.abs() > 2 * bound).double().mean()) > 0.5
