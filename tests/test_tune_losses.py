@@ -727,3 +727,62 @@ def test_borders_of_the_clipping_in_64_bits(device):
     adv = torch.ones(1, 1, device=device)
     far = ops.policy_loss(z, actions, adv * 0, adv * 0, adv * 60, kl_coef=1e-50).loss         # 1e-50 exp(60)
     assert float(far) == pytest.approx(1e-50 * math.exp(60), rel=1e-6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V,T", [(32000, 2048), (2000, 4096), (256, 16384)])
+def test_errors_of_rows_that_have_one_sign(V, T, dtype):
+    """A reward is a sum over a sequence less another, which keeps what is off by the same part in every row: over rows
+    of normal logits that may be 1e-8 a row, 1e-5 in a thousand tokens, beside
+      * k = log2(e) to 24 bits, a temperature that is off by 1.3e-8: the sums are those of that temperature, whose
+        log-probability lies 1.3e-8 (z_label - mean of z) from the other;
+      * what is left of the rows' own errors in the mean of 2 T of them, five times 8e-8 / sqrt(2 T): a row's sum is off
+        by 4e-8 (one standard deviation) around its average, by twice that where a few words make it up.
+    The exponential's average error alone is 3.7e-8."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    z = (torch.randn(2, T, V, device="cuda", generator=g) * 2.5).to(dtype)
+    labels = torch.randint(0, V, (2, T), device="cuda", generator=g)
+    k = float(torch.tensor(1.44269504088896341, dtype=torch.float32)) * math.log(2)
+    l, lk, mean = (torch.stack(t) for t in zip(*(
+        (torch.log_softmax(x, -1).gather(-1, t[:, None])[:, 0], torch.log_softmax(x * k, -1).gather(-1, t[:, None])[:, 0],
+         (torch.softmax(x, -1) * x).sum(-1)) for x, t in ((z[i].double(), labels[i]) for i in range(2)))))
+    ref = l.sum(1).float()
+    rewards = ops.preference_loss(z, labels, ref, beta=1.0).rewards.double() + ref.double()
+    bound = 1e-8 + 5 * 8e-8 / math.sqrt(2 * T)
+    assert abs(float((rewards - lk.sum(1)).mean())) / T < bound
+    far = (z.double().gather(-1, labels.unsqueeze(-1))[..., 0] - mean).sum() / (2 * T)
+    assert abs(float((rewards - l.sum(1)).mean()) / T - (k - 1) * float(far)) < bound
+    assert bound < 2e-8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V,T", [(1, 4096), (256, 8192), (32000, 1024)])
+def test_certain_words_over_a_sequence(V, T, dtype):
+    """One exponential is the whole sum, and what is above 0 is cut off: a log-probability of 0 comes out below it by
+    less than half a step of 1 in fp32 on average."""
+    g = torch.Generator(device="cuda").manual_seed(V + 1)
+    z = torch.full((2, T, V), -math.inf, device="cuda", dtype=dtype)
+    labels = torch.randint(0, V, (2, T), device="cuda", generator=g)
+    z.scatter_(2, labels.unsqueeze(-1), (torch.rand(2, T, 1, device="cuda", generator=g) * 40 - 20).to(dtype))
+    rewards = ops.preference_loss(z, labels, torch.zeros(2, device="cuda"), beta=1.0).rewards.double()
+    assert (rewards <= 0).all() and (rewards / T > -2.0 ** -24).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [32000, 256])
+def test_rows_of_two_values(V, dtype):
+    """All of a row's exponentials have one of two errors, which nothing but references that differ from lane to lane
+    averages: in 128 sequences of four such rows each, a log-probability is off by less than half a step of 1 in fp32
+    (root mean square; with one reference for all lanes 7.6e-8 in bf16)."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    values = torch.rand(128, 1, 2, device="cuda", generator=g) * 2
+    pick = torch.randint(0, 2, (1, 4, V), device="cuda", generator=g).expand(128, 4, V)
+    z = torch.gather(values.expand(128, 4, 2), 2, pick).to(dtype)
+    labels = torch.zeros(128, 4, dtype=torch.int64, device="cuda")
+    l = torch.log_softmax(z.double(), -1)[..., 0].sum(1)          # k's 24 bits: 1.3e-8 of 2 and less
+    rewards = ops.preference_loss(z, labels, l.float(), beta=1.0).rewards.double()
+    off = (rewards - (l - l.float().double())) / 4
+    assert float(off.square().mean().sqrt()) < 2.0 ** -24
