@@ -281,12 +281,14 @@ struct HeadsRing {
 // ROTATE and NORM: x -> y; UNROTATE is the backward of a rotation alone.  NORM_BACK: x and the gradient g of the
 // result -> y and the sums for dw, one row a CTA, which heads_fold_kernel adds in order.
 // A CTA stays with one part.  Its groups take `per` heads each, one after the other, token by token: the parts of a
-// call and the heads of a part need not divide anything, and no group has more than one head above another.
-// What bounds it is HBM behind some 220 instructions a head and lane, half of them conversions and packed arithmetic:
-// [1, 2048, 3, 32, 128] bf16 21 us forward (4.8 TB/s) and 30 backward with the fold (4.5), a rotation of
-// [1, 32768, 8, 128] 25 (5.3), where an element-wise pass over as many bytes takes 17, 28 and 22.  Heads loaded into
-// registers by the four took 24 and 40 us; all groups going through memory together, 4 or 8 heads each at a time, 30
-// and 43 (angles are loaded more often); the next token's angles in registers 23 (fewer CTAs an SM).
+// call and the heads of a part need not divide anything.  `per` is rounded up, so the last groups of a part have what is
+// left, or nothing.
+// What bounds it is HBM behind some 200 (a rotation) to 350 instructions (a backward) a head and lane, half of them
+// conversions and packed arithmetic: [1, 2048, 3, 32, 128] bf16 21 us forward (4.8 TB/s) and 30 backward with the fold
+// (4.5), a rotation of [1, 32768, 8, 128] 25 (5.3), where an element-wise pass over as many bytes takes 17, 22 and 22.
+// The backward's 122 registers leave two CTAs an SM, less than what hides its loads.  Heads loaded into registers by
+// the four took 24 and 40 us; all groups going through memory together, 4 or 8 heads each at a time, 30 and 43 (angles
+// are loaded more often); the next token's angles in registers 23 (fewer CTAs an SM).
 template <typename T, int VW, int NS, int MODE, bool INTER, bool FIT>
 __global__ void __launch_bounds__(256, HeadsRing<T, VW, NS, MODE>::CTAS)
 heads_kernel(const __grid_constant__ HeadsArgs p) {

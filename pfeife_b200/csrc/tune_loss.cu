@@ -22,9 +22,13 @@
 namespace pf {
 
 constexpr double LN2 = 0.693147180559945309417;
-// ex2.approx cuts its last bits off, and s is low by this part of its value on average (over 2048 rows of 32000
-// normal logits, bf16 and fp32 alike; a row's own s is off by 4e-8 around that).  A single probability hides it in
-// its rounding, a sum over a sequence does not.  The backward divides such values by such sums, where it cancels.
+// ex2.approx cuts its last bits off: one exponential is low by 5.1e-8 of its value on average over all fractions, and s
+// by this part (over 2048 rows of 32000 normal logits, bf16 and fp32 alike; a row's own s is off by 4e-8 around that).
+// A single probability hides it in its rounding, a sum over a sequence does not.  The backward divides such values by
+// such sums, where it cancels.  What is left, a row on average: below 1e-8 over normal logits; -2.5e-8 for a word that has
+// all the probability, since what comes out above 0 is cut off; and k's 24 bits, a temperature that is off by 1.3e-8:
+// 1.3e-8 (mean of z - z_label), 8e-8 for words taken at random among logits of 2.5 sigma.  The reference's sum over a
+// thousand such rows, some 1e4, is fp32: half a step of it is 5e-7 a row.
 constexpr double EXP2_LOW = 3.7e-8;
 
 constexpr float FAR = 4194304.f;
@@ -73,8 +77,8 @@ __device__ __forceinline__ void part_merge(float& m, float& s, float m2, float s
 }
 
 // 16 bytes of a row: its largest value, and its values two by two in fp32.  16-bit maxima are taken two at a time
-// before anything is widened, as fp32 sums and products are: ten instructions a value became six.  What is left are
-// the loads: without its exponentials, 16 a cycle and SM, the pass takes 38 us for 41 (2797 of 4096 rows of 32000
+// before anything is widened, as fp32 sums and products are: ten instructions a value became five.  What is left are
+// the loads: without its exponentials, 16 a cycle and SM, the pass takes 38 us for 41 (2787 of 4096 rows of 32000
 // bf16; 27 at the copy rate).  Batches of 4 vectors and twelve CTAs an SM take 41 too, the next batch in registers
 // 42 and several in shared memory 54.
 template <typename T> struct Words;
@@ -534,8 +538,9 @@ int back_lanes(long long rows, int nvec, int sm_count) {
   return nvec <= 256 && rows >= 4ll * sm_count ? 32 : 0;
 }
 
-// Parts of a row: enough for the CTAs that the SMs hold, and none of less than a batch (16 rows of 32000 fp32: 6.7 ->
-// 5.7 us; four times as many are slower by 1 to 3 us where rows fill the SMs as they are).
+// Parts of a row: enough for the CTAs that the SMs hold, but no more than batches, so that a part has a batch or, since
+// they are equal, somewhat less (16 rows of 32000 fp32: 7.7 us in one part, 6.1 in 8; four times as many are slower by
+// 1 to 3 us where rows fill the SMs as they are).
 int row_parts(long long rows, int V, int dtype, int sm_count) {
   const int batch = ROW_THREADS * ROW_BATCH * (dtype == PF_F32 ? 4 : 8);
   if (rows == 0 || row_lanes(rows, V, sm_count)) return 1;

@@ -1299,7 +1299,8 @@ def rope(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None
     """Rotates the heads of x [B, S, H, D] by their positions: pairs (i, i + R/2), or (2i, 2i + 1) when
     ``interleaved``, of the first R values, R twice the width of the tables cos / sin (``rope_tables``); values
     beyond R stay.  ``positions``, integers [S] or [B, S], are the rows of the tables to turn by (default: row s
-    for token s).  A row that the tables do not have makes the token's rotated values NaN on CUDA, where looking
+    for token s).  They turn and do nothing else: documents in one row still attend to those before them, as ``attention``
+    has the causal mask only.  A row that the tables do not have makes the token's rotated values NaN on CUDA, where looking
     for it would wait for the device, and an IndexError on the CPU."""
     if positions is None and not interleaved and not _narrow(cos, x):
         return _call(rope_apply, x, cos, sin, False)
