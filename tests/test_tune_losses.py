@@ -786,3 +786,25 @@ def test_rows_of_two_values(V, dtype):
     rewards = ops.preference_loss(z, labels, l.float(), beta=1.0).rewards.double()
     off = (rewards - (l - l.float().double())) / 4
     assert float(off.square().mean().sqrt()) < 2.0 ** -24
+
+
+@pytest.mark.gpu
+def test_numbers_arrive_through_ctypes_too(monkeypatch):
+    """Where there is no module of the entry points, numbers in 64 bits reach them by the same declarations."""
+    import ctypes
+    from pfeife_b200.csrc import build
+    from pfeife_b200.ops import _lib
+    z, labels = batch(4, 7, 300, "cuda", torch.bfloat16, 3)
+    z.requires_grad_()
+    v = torch.full((4, 7), -5.0, device="cuda")
+
+    def values():
+        with Watch():                              # through the registered ops, not the eager module
+            a = ops.preference_loss(z, labels, v[:, 0], 0.3, 0.1)
+            b = ops.policy_loss(z, labels, v, v[:, :1] + 6, v + 1, 0.1, 0.3, kl_coef=0.2, temperature=1.3)
+            return [*a, *b, *torch.autograd.grad(a.loss + b.loss, z)]
+    want = values()
+    through = _lib._CtypesCalls(ctypes.CDLL(str(build.KERNEL_LIB), mode=ctypes.RTLD_GLOBAL))
+    monkeypatch.setattr(_lib, "_calls", through)
+    assert _lib.calls() is through
+    assert all(torch.equal(a, b) for a, b in zip(values(), want))
