@@ -1302,6 +1302,8 @@ def rope(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None
     for token s).  They turn and do nothing else: documents in one row still attend to those before them, as ``attention``
     has the causal mask only.  A row that the tables do not have makes the token's rotated values NaN on CUDA, where looking
     for it would wait for the device, and an IndexError on the CPU."""
+    # whole heads of the half layout in their places: the kernel and the registered op that stage graphs have had; the
+    # others give the same bits for them, and take an eager caller less time
     if positions is None and not interleaved and not _narrow(cos, x):
         return _call(rope_apply, x, cos, sin, False)
     if isinstance(x, Tensor) and x.dim() != 4:

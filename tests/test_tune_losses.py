@@ -808,3 +808,26 @@ def test_numbers_arrive_through_ctypes_too(monkeypatch):
     monkeypatch.setattr(_lib, "_calls", through)
     assert _lib.calls() is through
     assert all(torch.equal(a, b) for a, b in zip(values(), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,T", [(131072, 2), (151936, 40), (200019, 3)])
+def test_large_vocabularies(V, T, dtype):
+    """Rows of 128 thousand words and more, in many parts where they are few, some of them masked."""
+    z, labels = batch(2, T, V, "cuda", dtype, 6, masked=0.2)
+    z[0, 0, 1000:] = torch.finfo(dtype).min
+    labels[0, 0], labels[1, 0] = 17, V - 1
+    z.requires_grad_()
+    l, dl, p, rel, counted = rows64(z.detach(), labels, 1.0)
+    l0 = torch.log_softmax(z.detach()[0, 0, :1000].double(), -1)[17]     # the masked row's bound is that of its words
+    R = (V / 32 + 68 + 4 * 24) * E + 2.0 ** -22
+    dl[0, 0], rel[0, 0] = R + 2 * E * l0.abs(), 2 * R
+    out = ops.policy_loss(z, labels, l.float(), torch.ones(2, 1, device="cuda"))
+    near(out.logps, l, dl)
+    (dz,) = torch.autograd.grad(out.loss, z)
+    n = int(counted.sum())
+    g = torch.full_like(l, -1.0 / n)
+    near(dz, *gradient(g, (1.1 * dl + 8 * E * l.abs().clamp(min=1)) / n, p, rel, labels, counted))
+    pref = ops.preference_loss(z, labels, l.sum(1).float(), beta=0.5)
+    near(pref.rewards, 0.5 * (l.sum(1) - l.sum(1).float().double()), 0.5 * dl.sum(1) + 4 * E * l.sum(1).abs())
