@@ -25,6 +25,34 @@ PF_DECL int pf_gemm(const void* A, const void* B, void* C, int M, int N, int K, 
 PF_DECL int pf_gemm_workspace(int M, int N, int K, int accumulate, int conv, int sm_count,
                               int tile_n);
 
+// ---- fused_gemm_sm100.cu
+PF_DECL int pf_glu_linear_fwd(const void* x, const void* w, const void* bias, int bias_dtype, void* h, void* gu, int M,
+                              int H, int K, long long ldx, long long ldw, int act, int dtype, int* status, int sm_count,
+                              void* stream);
+PF_DECL int pf_glu_linear_bwd(const void* dy, const void* w2, const void* gu, void* dgu, void* h, int M, int H, int K,
+                              long long lddy, long long ldw2, int act, int dtype, int* status, int sm_count,
+                              void* stream);
+
+// ---- head_loss.cu
+PF_DECL int pf_head_index(long long N);
+PF_DECL int pf_head_scratch(long long N, long long V);
+PF_DECL int pf_head_words(long long N, long long V);
+PF_DECL int pf_head_parts(long long N, long long V, int D, int sm_count);
+PF_DECL int pf_head_fwd(const void* x, const void* w, const void* target, void* xc, void* index, void* stats, void* loss,
+                        void* inv, void* scratch, long long N, long long V, int D, int Dp, long long ldx, long long ldw,
+                        long long ignore_index, int reduction, int dtype, int* status, int sm_count, void* stream);
+PF_DECL int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const void* w, void* index,
+                        const void* stats, void* dx, void* dw, void* dz, void* acc, void* factor, long long N,
+                        long long V, int D, int Dp, long long dloss_step, long long ldw, long long lddw, int by_row,
+                        int accumulate, int dtype, int dw_dtype, int* status, int sm_count, void* stream);
+
+// ---- embed_sorted.cu
+PF_DECL int pf_scaled_embed_fwd(const void* table, const void* ids, void* out, long long tokens, int D, long long words,
+                                float scale, int table_dtype, int out_dtype, void* stream);
+PF_DECL int pf_scaled_embed_scratch(long long tokens, int D, long long words);
+PF_DECL int pf_scaled_embed_bwd(const void* dout, const void* ids, void* dtable, void* scratch, long long tokens, int D,
+                                long long words, float scale, int accumulate, int dtype, int table_dtype, void* stream);
+
 // ---- elementwise.cu
 PF_DECL int pf_elementwise(const void* a, const void* b, void* out, long long n, int op, int dtype,
                            int sm_count, void* stream);

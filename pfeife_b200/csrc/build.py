@@ -57,9 +57,9 @@ NVCC_FLAGS = [
 ]
 # Approximate division / square root / transcendentals are fine for activations and softmax,
 # not for the optimizer update: those two files are bandwidth-bound and keep IEEE arithmetic, as do
-# the head norms and the token losses, which name the approximations that they use.
+# the head norms and the token losses, which name the approximations that they use, and sums of embedded tokens.
 FAST_MATH = ["--use_fast_math"]
-PRECISE_SOURCES = {"optim.cu", "dp_fused.cu", "qk_rope.cu", "tune_loss.cu"}
+PRECISE_SOURCES = {"optim.cu", "dp_fused.cu", "qk_rope.cu", "tune_loss.cu", "head_loss.cu", "embed_sorted.cu"}
 CXX_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-pthread"]
 
 

@@ -1,0 +1,62 @@
+// Products whose epilogues are more than a store (fused_gemm_sm100.cu), for the entry points of the gated
+// feed-forward block and of the head with its loss.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace pf {
+
+enum Job : int {
+  GLU_FWD,      // h = act(x Wg^T + bg) * (x Wu^T + bu), gate and up kept where asked for
+  GLU_BWD,      // dh = dy W2, then d(gate), d(up) and h from the kept gate and up
+  HEAD_STATS,   // per row and half a tile of z = x W^T: a reference and the sum of 2^(z log2 e - reference)
+  HEAD_DZ,      // (softmax(z) - onehot) * factor of some words, in 16 bits
+  HEAD_DX,      // parts of dz W, in fp32
+  HEAD_DW,      // dz^T x
+};
+
+// What a row of the product has of the loss: reference and one over the sum; its label.
+struct RowStat { float ref, inv; };
+
+struct FusedCall {
+  // product [M, N] over K.  GLU_FWD: N hidden values, each of two columns
+  int M = 0, N = 0, K = 0;
+  const void* A = nullptr;     // 16-bit; K innermost, but HEAD_DW: M innermost
+  const void* B = nullptr;     // GLU_FWD, HEAD_STATS, HEAD_DZ: K innermost, else N innermost
+  long long lda = 0, ldb = 0;
+  const int* rows = nullptr;   // device: how many rows there are (HEAD_DW: what to reduce over); M (K) is the most
+  int dtype = 0, out_dtype = 0;
+  void* C = nullptr;           // h | h | - | dz | fp32 parts | dW
+  long long ldc = 0;
+  // GLU
+  void* gu = nullptr;          // gate and up [M, 2 N]: written (forward, may be null) or read
+  void* dgu = nullptr;         // [M, 2 N]
+  const void* bias = nullptr;  // [2 N]
+  int bias_dtype = 0;
+  int act = 0;
+  // head
+  const int* labels = nullptr;
+  int first = 0;               // word of the first column
+  RowStat* parts = nullptr;    // [HEAD_PARTS_OF(N)][part_pitch]: reference and sum
+  long long part_pitch = 0;
+  float* picked = nullptr;     // z at the label
+  const RowStat* stats = nullptr;
+  const float* factor = nullptr;   // of each row; null: `unit` for all
+  float unit = 1.f;
+  int split = 1;               // HEAD_DX: parts of the reduction, part i in rows i * part_rows of C on
+  int part_rows = 0;
+  int accumulate = 0;          // HEAD_DX, HEAD_DW in fp32: add to C
+  const float* scale = nullptr;    // HEAD_DW: *scale times *scale2 (where given) times scale3
+  const float* scale2 = nullptr;
+  float scale3 = 1.f;
+  int* status = nullptr;
+  int sm_count = 148;
+  cudaStream_t stream = nullptr;
+};
+
+constexpr int HEAD_PART = 64;      // words of a part of HEAD_STATS; a tile of a CTA pair has twice as many in each
+
+// 256 x 256 tiles of CTA pairs instead of 128 x 128 ones
+bool fused_pairs(Job job, long long M, long long N, int sm_count);
+int fused_gemm(Job job, const FusedCall& c);
+
+}  // namespace pf

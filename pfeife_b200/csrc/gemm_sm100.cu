@@ -786,7 +786,7 @@ int make_tmap_2d_16bit(CUtensorMap* map, const void* base, int fmt, long long in
 
 // [rows, cols] output map with a 32 x 32 box; 16-bit: 64 B rows (SWIZZLE_64B), fp32: 128 B rows
 // (SWIZZLE_128B)
-static int make_tmap_out(CUtensorMap* map, const void* base, int out_dtype, long long cols,
+int make_tmap_out(CUtensorMap* map, const void* base, int out_dtype, long long cols,
                          long long rows, long long ld) {
   EncodeTiledFn enc = get_encode();
   if (!enc) return -100;

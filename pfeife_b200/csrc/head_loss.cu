@@ -1,0 +1,435 @@
+// Cross entropy of an output head, z = x W^T, without the logits.
+//
+// loss = log sum_v e^(z_v) - z_label over the rows that count, and with p = softmax(z), dz = g (p - onehot):
+// dx = dz W, dW = dz^T x.
+//
+// Forward: the rows that count are gathered (prompts, padding and last tokens then cost nothing, and what they hold
+// reaches nothing), one product whose epilogue keeps a reference and a sum of exponentials of each row and part of
+// the words, and a fold over the parts.  Backward, piece by piece of the vocabulary: the product again, now with
+// the sums at hand, leaves dz of a piece in 16 bits; from it come the piece's rows of dW, complete, and its share of
+// dx, which adds up in fp32.  Four products of 2 rows D V operations where keeping the logits takes three: what is kept
+// from forward to backward is the rows and 8 bytes of each, and what is alive at one time PIECE values.
+//
+// dz is rounded to 16 bits as p - onehot, times 2^15 for fp16: from 6e-5 / 2^15 on the probabilities keep all
+// their bits, whatever the gradient of the loss is; that and the mean's factor come in 32 bits behind the products.
+#include "common.cuh"
+#include "api.h"
+#include "fused_gemm.h"
+
+namespace pf {
+
+// index: [0] rows that count, [1] CTAs of the fold that have finished, then the rows that count, their labels, and
+// where each row is among them (or -1)
+constexpr int HEAD_HEADER = 4;
+struct HeadIndex {
+  int *count, *list, *labels, *at;
+};
+static long long padded_rows(long long N) { return (N + 255) / 256 * 256; }
+static HeadIndex head_index(int* index, long long N) {
+  const long long Mp = padded_rows(N);
+  return {index, index + HEAD_HEADER, index + HEAD_HEADER + Mp, index + HEAD_HEADER + 2 * Mp};
+}
+
+// One CTA: ranks of the rows that count, 4 rows a thread at a time.  8192 rows take two rounds.
+__global__ void __launch_bounds__(1024)
+head_rows_kernel(const long long* __restrict__ target, HeadIndex ix, float* __restrict__ loss_of_row, int N,
+                 long long V, long long ignore_index) {
+  after_previous();
+  __shared__ int sums[32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int base = 0;
+  for (int n0 = 0; n0 < N; n0 += 4096) {
+    const int n = n0 + threadIdx.x * 4;
+    int label[4], mine = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long long t = n + j < N ? target[n + j] : -1;
+      label[j] = t >= 0 && t < V && t != ignore_index ? (int)t : -1;
+      mine += label[j] >= 0;
+    }
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += up;
+    }
+    if (lane == 31) sums[warp] = before;
+    __syncthreads();
+    const int other = sums[lane];
+    const int ahead = __reduce_add_sync(0xffffffffu, lane < warp ? other : 0);
+    const int all = __reduce_add_sync(0xffffffffu, other);
+    int at = base + ahead + before - mine;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (n + j >= N) break;
+      const bool in = label[j] >= 0;
+      ix.at[n + j] = in ? at : -1;
+      if (in) {
+        ix.list[at] = n + j;
+        ix.labels[at] = label[j];
+        ++at;
+      } else if (loss_of_row) {
+        loss_of_row[n + j] = 0.f;
+      }
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    ix.count[0] = base;
+    ix.count[1] = 0;
+  }
+}
+
+// xc[i] = x[list[i]], a warp per row; zeros behind the last row to the end of its block of 64, as far as a reduction over
+// rows reads, and in the columns that fill D up to Dp.
+template <typename T>
+__global__ void __launch_bounds__(256)
+head_gather_kernel(const T* __restrict__ x, T* __restrict__ xc, HeadIndex ix, int Mp, int D, int Dp, long long ldx,
+                   int vec) {
+  after_previous();
+  const int count = *ix.count, end = min(Mp, (count + 63) / 64 * 64), lane = threadIdx.x & 31;
+  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= end) return;
+  T* dst = xc + (long long)i * Dp;
+  const T* src = i < count ? x + ix.list[i] * ldx : nullptr;
+  if (vec) {
+    uint4* dv = reinterpret_cast<uint4*>(dst);
+    const uint4* sv = reinterpret_cast<const uint4*>(src);
+    const int nv = Dp / 8;
+    for (int c = lane; c < nv; c += 128) {
+      uint4 q[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c + u * 32 < nv) q[u] = src ? __ldg(sv + c + u * 32) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c + u * 32 < nv) dv[c + u * 32] = q[u];
+    }
+  } else {
+    for (int c = lane; c < Dp; c += 32) dst[c] = src && c < D ? src[c] : from_f32<T>(0.f);
+  }
+}
+
+// Joins the parts of 32 rows: 32 threads share the parts of a row, with lanes on neighbouring rows; then a warp has a row.
+// References are integers: 2^(a - b) is exact.  The row's loss is formed in 64 bits; `sums` gets a CTA's sum of them, and
+// the CTA that finishes last adds those up in their order.
+__global__ void __launch_bounds__(1024)
+head_fold_kernel(const RowStat* __restrict__ parts, long long pitch, int n_parts, const float* __restrict__ picked,
+                 HeadIndex ix, RowStat* __restrict__ stats, float* __restrict__ loss_of_row, float* __restrict__ loss,
+                 float* __restrict__ inv, double* __restrict__ sums, int mean) {
+  after_previous();
+  __shared__ RowStat all[32][33];
+  __shared__ double rows[32];
+  __shared__ int last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int count = *ix.count, row0 = blockIdx.x * 32;
+  if (row0 < count) {
+    const int row = row0 + lane;
+    float ref = -INFINITY, sum = 0.f;
+    if (row < count) {
+      const RowStat* src = parts + row;
+      for (int k = warp; k < n_parts; k += 256) {
+        RowStat q[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (k + 32 * u < n_parts) q[u] = src[(k + 32 * u) * pitch];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (k + 32 * u < n_parts) {
+            const float m = fmaxf(ref, q[u].ref), sub = m == -INFINITY ? 0.f : m;
+            sum = sum * exp2f(ref - sub) + q[u].inv * exp2f(q[u].ref - sub);
+            ref = m;
+          }
+      }
+    }
+    all[warp][lane] = {ref, sum};
+  }
+  __syncthreads();
+  const int row = row0 + warp;                          // the warp's row, over whose parts its lanes lie
+  if (lane == 0) rows[warp] = 0.0;
+  if (row < count) {
+    RowStat q = all[lane][warp];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float ref = __shfl_xor_sync(0xffffffffu, q.ref, o), sum = __shfl_xor_sync(0xffffffffu, q.inv, o);
+      const float m = fmaxf(q.ref, ref), sub = m == -INFINITY ? 0.f : m;
+      // the same sum in both lanes of a pair, whichever has the first half
+      const float a = q.inv * exp2f(q.ref - sub), b = sum * exp2f(ref - sub);
+      q = {m, a + b};
+    }
+    if (lane == 0) {
+      const float ref = q.ref == -INFINITY ? 0.f : q.ref;
+      stats[row] = {ref, 1.f / q.inv};
+      constexpr double ln2 = 0.69314718055994531;
+      const double l = (log2((double)q.inv) + (double)ref - (double)picked[row] * (double)1.4426950408889634f) * ln2;
+      rows[warp] = l;
+      if (loss_of_row) loss_of_row[ix.list[row]] = (float)l;
+    }
+  }
+  if (loss_of_row) return;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int i = 0; i < 32; ++i) s += rows[i];
+    sums[blockIdx.x] = s;
+    __threadfence();
+    last = atomicAdd(ix.count + 1, 1) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double s = 0.0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += 1024) s += reinterpret_cast<volatile double*>(sums)[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) rows[warp] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int i = 0; i < 32; ++i) s += rows[i];
+    const double n = mean ? (double)max(count, 1) : 1.0;
+    *loss = (float)(s / n);
+    *inv = (float)(1.0 / n);
+  }
+}
+
+// Gradients that arrive row by row, of the rows that count: divided by a power of two near their largest, which goes into
+// `scale`, so that 16 bits hold the products.
+__global__ void __launch_bounds__(1024)
+head_factor_kernel(const float* __restrict__ g, long long step, HeadIndex ix, float* __restrict__ factor,
+                   float* __restrict__ scale) {
+  after_previous();
+  __shared__ float tops[32];
+  const int count = *ix.count;
+  float top = 0.f;
+  for (int i = threadIdx.x; i < count; i += 1024) {
+    const float v = g[ix.list[i] * step];
+    factor[i] = v;
+    top = fmaxf(top, fabsf(v));
+  }
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = warp_max(tops[threadIdx.x & 31]);
+  int e = 0;
+  if (top > 0.f && top < INFINITY) {
+    frexpf(top, &e);
+    e = max(-120, min(120, e));
+  }
+  const float down = ldexpf(1.f, -e);
+  for (int i = threadIdx.x; i < count; i += 1024) factor[i] *= down;
+  if (threadIdx.x == 0) *scale = ldexpf(1.f, e);
+}
+
+// dx[n] = the sum over parts of acc at the row's place, times the scale; zeros for rows that do not count.
+template <typename T>
+__global__ void __launch_bounds__(256)
+head_dx_kernel(const float* __restrict__ acc, T* __restrict__ dx, HeadIndex ix, long long N, int D, int Dp, int parts,
+               long long part_size, const float* __restrict__ scale, const float* __restrict__ scale2, float scale3,
+               int vec) {
+  after_previous();
+  const float s = *scale * (scale2 ? *scale2 : 1.f) * scale3;
+  const int lane = threadIdx.x & 31;
+  const long long n = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  if (n >= N) return;
+  const int at = ix.at[n];
+  const float* src = acc + (long long)at * Dp;
+  T* dst = dx + n * D;
+  if (vec) {
+    for (int c = lane * 8; c < D; c += 256) {
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (at >= 0) {
+        for (int k = 0; k < parts; ++k) {
+          const float4* q = reinterpret_cast<const float4*>(src + k * part_size + c);
+          const float4 a = q[0], b = q[1];
+          v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+          v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= s;
+      }
+      uint4 q;
+      T* e = reinterpret_cast<T*>(&q);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j]);
+      *reinterpret_cast<uint4*>(dst + c) = q;
+    }
+  } else {
+    for (int c = lane; c < D; c += 32) {
+      float v = 0.f;
+      if (at >= 0) {
+        for (int k = 0; k < parts; ++k) v += src[k * part_size + c];
+        v *= s;
+      }
+      dst[c] = from_f32<T>(v);
+    }
+  }
+}
+
+// Values of dz that are alive at one time: 256 MB.  Pieces of fewer than 4096 words would have dx added to too often
+// (8 bytes of each of its values a piece, for 6 x 4096 operations).
+constexpr long long PIECE = 128ll << 20;
+constexpr int PIECE_WORDS = 4096;
+
+}  // namespace pf
+
+using namespace pf;
+
+static bool head_sizes_ok(long long N, long long V, long long D) {
+  return N >= 0 && V > 0 && D > 0 && N <= (1ll << 28) && V <= (1ll << 28) && D <= (1ll << 20);
+}
+
+// int32 values of `index`
+PF_API int pf_head_index(long long N) {
+  return N < 0 || N > (1ll << 28) ? -3 : (int)(HEAD_HEADER + 2 * padded_rows(N) + N);
+}
+
+// KiB of scratch of pf_head_fwd
+PF_API int pf_head_scratch(long long N, long long V) {
+  if (!head_sizes_ok(N, V, 1)) return -3;
+  const long long Mp = padded_rows(N), parts = (V + HEAD_PART - 1) / HEAD_PART;
+  const long long kib = (parts * Mp * 8 + Mp * 4 + Mp / 32 * 8 + 1023) / 1024 + 1;
+  return kib > 0x7fffffffll ? -3 : (int)kib;
+}
+
+// Words of a piece of the backward, all pieces as near in size as multiples of 256 allow
+PF_API int pf_head_words(long long N, long long V) {
+  if (!head_sizes_ok(N, V, 1)) return -3;
+  const long long Mp = N > 0 ? padded_rows(N) : 256;
+  long long most = PIECE / Mp / 256 * 256;
+  if (most < PIECE_WORDS) most = PIECE_WORDS;
+  const long long pieces = (V + most - 1) / most;
+  return (int)(((V + pieces - 1) / pieces + 255) / 256 * 256);
+}
+
+// Parts in which the reduction of dx over the words of the only piece is split, where few rows leave SMs idle
+PF_API int pf_head_parts(long long N, long long V, int D, int sm_count) {
+  if (!head_sizes_ok(N, V, D)) return -3;
+  if (sm_count <= 0) sm_count = 148;
+  const long long words = pf_head_words(N, V);
+  if (words < V) return 1;
+  const bool pair = fused_pairs(HEAD_DX, N, D, sm_count);
+  const long long bt = pair ? 256 : 128, tiles = ((N + bt - 1) / bt) * ((D + bt - 1) / bt);
+  const long long slots = pair ? sm_count / 2 : sm_count, kb = (V + 63) / 64;
+  int parts = 1;
+  while (parts < 16 && tiles * (parts + 1) <= slots && kb >= 8ll * (parts + 1)) ++parts;
+  return parts;
+}
+
+// x [N, D] (rows ldx apart), w [V, Dp] (Dp: D up to a multiple of 8, filled with zeros; rows ldw apart), target [N].
+// xc [Mp, Dp] (Mp: N up to a multiple of 256), index: pf_head_index, stats [Mp, 2] are for the backward.
+// reduction 0: loss [N], 0 where no label counts; 1: mean over the rows that count, 2: their sum, both with inv.
+PF_API int pf_head_fwd(const void* x, const void* w, const void* target, void* xc, void* index, void* stats, void* loss,
+                       void* inv, void* scratch, long long N, long long V, int D, int Dp, long long ldx, long long ldw,
+                       long long ignore_index, int reduction, int dtype, int* status, int sm_count, void* stream) {
+  if (dtype != PF_F16 && dtype != PF_BF16) return -1;
+  if (!head_sizes_ok(N, V, D)) return -3;
+  if (Dp % 8 || Dp < D || !on_vectors(w, xc, scratch) || ldw % 8) return -2;
+  if (sm_count <= 0) sm_count = 148;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const long long Mp = padded_rows(N);
+  const HeadIndex ix = head_index(static_cast<int*>(index), N);
+  const bool pair = fused_pairs(HEAD_STATS, N, V, sm_count);
+  const int width = pair ? 2 * HEAD_PART : HEAD_PART;
+  const int n_parts = (int)((V + width - 1) / width);
+  RowStat* parts = static_cast<RowStat*>(scratch);
+  double* sums = reinterpret_cast<double*>(parts + n_parts * Mp);
+  float* picked = reinterpret_cast<float*>(sums + Mp / 32);
+  float* each = reduction == 0 ? static_cast<float*>(loss) : nullptr;
+  after(head_rows_kernel, 1, 1024, 0, st)((const long long*)target, ix, each, (int)N, V, ignore_index);
+  PF_CHECK_LAUNCH();
+  if (N > 0) {
+    const int vec = D == Dp && ldx % 8 == 0 && on_vectors(x);
+    const unsigned grid = (unsigned)(Mp / 8);
+    if (dtype == PF_F16)
+      after(head_gather_kernel<__half>, grid, 256, 0, st)((const __half*)x, (__half*)xc, ix, (int)Mp, D, Dp, ldx, vec);
+    else
+      after(head_gather_kernel<__nv_bfloat16>, grid, 256, 0, st)((const __nv_bfloat16*)x, (__nv_bfloat16*)xc, ix,
+                                                                 (int)Mp, D, Dp, ldx, vec);
+    PF_CHECK_LAUNCH();
+    FusedCall c;
+    c.M = (int)N; c.N = (int)V; c.K = Dp; c.A = xc; c.B = w; c.lda = Dp; c.ldb = ldw; c.dtype = dtype;
+    c.rows = ix.count; c.labels = ix.labels; c.parts = parts; c.part_pitch = Mp; c.picked = picked;
+    c.status = status; c.sm_count = sm_count; c.stream = st;
+    const int r = fused_gemm(HEAD_STATS, c);
+    if (r) return r;
+  }
+  const unsigned grid = (unsigned)(Mp > 0 ? Mp / 32 : 1);
+  after(head_fold_kernel, grid, 1024, 0, st)((const RowStat*)parts, Mp, n_parts, (const float*)picked, ix,
+                                             (RowStat*)stats, each, each ? nullptr : (float*)loss, (float*)inv, sums,
+                                             (int)(reduction == 1));
+  PF_CHECK_LAUNCH();
+  return 0;
+}
+
+// dloss: one value, or with by_row the rows' dloss[n * dloss_step]; inv as the forward left it.
+// dx [N, D] packed, dw [V, Dp] (rows lddw apart, added to where accumulate); either may be null.
+// dz [Mp, pf_head_words], acc [pf_head_parts * Mp, Dp] (with dx), factor [Mp + 1] (with by_row) are scratch.
+PF_API int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const void* w, void* index, const void* stats,
+                       void* dx, void* dw, void* dz, void* acc, void* factor, long long N, long long V, int D, int Dp,
+                       long long dloss_step, long long ldw, long long lddw, int by_row, int accumulate, int dtype,
+                       int dw_dtype, int* status, int sm_count, void* stream) {
+  if (dtype != PF_F16 && dtype != PF_BF16) return -1;
+  if (dw && dw_dtype != dtype && dw_dtype != PF_F32) return -1;
+  if (!head_sizes_ok(N, V, D)) return -3;
+  if (Dp % 8 || Dp < D || !on_vectors(w, xc, dw, dz, acc) || ldw % 8 || (dw && lddw % 8)) return -2;
+  if (accumulate && dw && dw_dtype != PF_F32) return -1;
+  if (sm_count <= 0) sm_count = 148;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const long long Mp = padded_rows(N);
+  const HeadIndex ix = head_index(static_cast<int*>(index), N);
+  const int words = pf_head_words(N, V), parts = pf_head_parts(N, V, D, sm_count);
+  const float unit = dtype == PF_F16 ? 32768.f : 1.f;
+  const float* scale = static_cast<const float*>(dloss);
+  const float* scale2 = static_cast<const float*>(inv);
+  float* each = nullptr;
+  if (by_row) {
+    each = static_cast<float*>(factor);
+    scale = each + Mp;
+    scale2 = nullptr;
+    after(head_factor_kernel, 1, 1024, 0, st)((const float*)dloss, dloss_step, ix, each, each + Mp);
+    PF_CHECK_LAUNCH();
+  }
+  FusedCall base;
+  base.dtype = dtype; base.rows = ix.count; base.status = status; base.sm_count = sm_count; base.stream = st;
+  const size_t es = dw_dtype == PF_F32 ? 4 : 2;
+  if (N == 0) {                                         // nothing to add up, and no rows for a tensor map
+    return dw && !accumulate ? (int)cudaMemsetAsync(dw, 0, (size_t)V * lddw * es, st) : 0;
+  }
+  for (long long v0 = 0; v0 < V; v0 += words) {
+    const int n = (int)(V - v0 < words ? V - v0 : words);
+    const char* wp = static_cast<const char*>(w) + v0 * ldw * 2;
+    int r;
+    FusedCall z = base;
+    z.M = (int)N; z.N = n; z.K = Dp; z.A = xc; z.B = wp; z.lda = Dp; z.ldb = ldw; z.C = dz; z.ldc = words;
+    z.labels = ix.labels; z.first = (int)v0; z.stats = static_cast<const RowStat*>(stats); z.factor = each;
+    z.unit = unit;
+    if ((r = fused_gemm(HEAD_DZ, z))) return r;
+    if (dx) {
+      FusedCall c = base;
+      c.M = (int)N; c.N = Dp; c.K = n; c.A = dz; c.B = wp; c.lda = words; c.ldb = ldw; c.C = acc; c.ldc = Dp;
+      c.out_dtype = PF_F32; c.split = parts; c.part_rows = (int)Mp; c.accumulate = v0 > 0;
+      if ((r = fused_gemm(HEAD_DX, c))) return r;
+    }
+    if (dw) {
+      FusedCall c = base;
+      c.M = n; c.N = Dp; c.K = (int)N; c.A = dz; c.B = xc; c.lda = words; c.ldb = Dp;
+      c.C = static_cast<char*>(dw) + v0 * lddw * es; c.ldc = lddw; c.out_dtype = dw_dtype; c.accumulate = accumulate;
+      c.scale = scale; c.scale2 = scale2; c.scale3 = 1.f / unit;
+      if ((r = fused_gemm(HEAD_DW, c))) return r;
+    }
+  }
+  if (dx) {
+    const int vec = D == Dp && on_vectors(dx);
+    const unsigned grid = (unsigned)((N + 7) / 8);
+    if (dtype == PF_F16)
+      after(head_dx_kernel<__half>, grid, 256, 0, st)((const float*)acc, (__half*)dx, ix, N, D, Dp, parts, Mp * Dp, scale,
+                                                      scale2, 1.f / unit, vec);
+    else
+      after(head_dx_kernel<__nv_bfloat16>, grid, 256, 0, st)((const float*)acc, (__nv_bfloat16*)dx, ix, N, D, Dp, parts,
+                                                             Mp * Dp, scale, scale2, 1.f / unit, vec);
+    PF_CHECK_LAUNCH();
+  }
+  return 0;
+}

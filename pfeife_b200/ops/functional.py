@@ -608,6 +608,162 @@ def mlp(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: Optional[Te
     return _call(mlp_fwd, x, w1, b1, w2, b2, residual, _ACT_NAMES[activation])
 
 
+# --------------------------------------------------------------------------- gated feed-forward block
+def _act_slope(z: Tensor, act: int) -> Tuple[Tensor, Tensor]:
+    """(activation, derivative) in z's own type"""
+    if act == ACT_GELU:
+        cdf = 0.5 * (1.0 + torch.erf(z * math.sqrt(0.5)))
+        return z * cdf, cdf + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    if act == ACT_GELU_TANH:
+        c = math.sqrt(2 / math.pi)
+        t = torch.tanh(c * (z + 0.044715 * z ** 3))
+        return 0.5 * z * (1.0 + t), 0.5 * (1.0 + t) + 0.5 * z * (1.0 - t * t) * c * (1.0 + 3 * 0.044715 * z * z)
+    sg = torch.sigmoid(z)
+    return z * sg, sg * (1.0 + z * (1.0 - sg))
+
+
+def _glu_native(x: Tensor, cd: torch.dtype, w1: Tensor, w2: Tensor) -> bool:
+    """The kernels that have the activation in the products' epilogue: whole vectors of every width."""
+    return x.is_cuda and cd in (torch.float16, torch.bfloat16) and w1.shape[1] % 8 == 0 and w2.shape[0] % 8 == 0 \
+        and w2.shape[1] % 8 == 0
+
+
+def _aligned(w: Tensor) -> Tensor:
+    return w if w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.data_ptr() % 16 == 0 else \
+        w.clone(memory_format=torch.contiguous_format)
+
+
+@_custom_op("pfeife::gated_mlp_fwd")
+def gated_mlp_fwd(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: Optional[Tensor],
+                  residual: Optional[Tensor], act: int, keep: bool) -> Tuple[Tensor, Tensor]:
+    """-> (y, gate and up [..., 2H], empty unless they are to be kept for a backward)"""
+    cd = compute_dtype(x)
+    shape, H = x.shape[:-1], w2.shape[1]
+    if _glu_native(x, cd, w1, w2):
+        x2 = _rows(x if x.dtype == cd else kx.cast(x, cd))
+        h, gu = kx.glu_linear_fwd(x2, _aligned(_weight_as(w1, cd)), b1, act, keep)
+        y, _ = linear_fwd.plain(h.view(shape + (H,)), w2, b2, residual, ACT_NONE)
+        return y, (gu.view(shape + (2 * H,)) if keep else x.new_empty(0))
+    if x.is_cuda and cd in (torch.float16, torch.bfloat16):      # odd widths, product by product
+        gu, _ = linear_fwd.plain(x, w1, b1, None, ACT_NONE)
+    else:
+        gu = F.linear(x.to(cd), w1.to(cd), None if b1 is None else b1.to(cd))
+    wide = _wide(gu)
+    h = (_act_slope(wide[..., :H], act)[0] * wide[..., H:]).to(cd)
+    y, _ = linear_fwd.plain(h, w2, b2, residual, ACT_NONE)
+    return y, (gu if keep else x.new_empty(0))
+
+
+@gated_mlp_fwd.register_fake
+def _(x, w1, b1, w2, b2, residual, act, keep):
+    cd = compute_dtype(x)
+    gu = x.new_empty(x.shape[:-1] + (w1.shape[0],), dtype=cd) if keep else x.new_empty(0)
+    return x.new_empty(x.shape[:-1] + (w2.shape[0],), dtype=cd), gu
+
+
+@_custom_op("pfeife::gated_mlp_bwd")
+def gated_mlp_bwd(dy: Tensor, x: Tensor, w1: Tensor, w2: Tensor, gu: Tensor, act: int, need_dx: bool, need_dw1: bool,
+                  need_db1: bool, need_dw2: bool, need_db2: bool, b1: Optional[Tensor] = None,
+                  b2: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """-> (dx, dw1, db1, dw2, db2); what is not needed, or went into a registered gradient bucket, comes back empty.
+    The gradient of h is formed in the epilogue of its product, where the kept gate and up turn it into their
+    gradients and into h itself, which the forward did not keep."""
+    cd = dy.dtype
+    H = w2.shape[1]
+    empty = dy.new_empty(0)
+    if not dy.numel():                   # no rows: the products would leave the weights' gradients as they are
+        zeros = lambda t, need: torch.zeros_like(t) if need else dy.new_empty(0)
+        return (dy.new_zeros(x.shape), zeros(w1, need_dw1), dy.new_zeros(2 * H if need_db1 else 0, dtype=torch.float32),
+                zeros(w2, need_dw2), dy.new_zeros(w2.shape[0] if need_db2 else 0, dtype=torch.float32))
+    if _glu_native(dy, cd, w1, w2):
+        dgu, h = kx.glu_linear_bwd(_rows(dy), _aligned(_weight_as(w2, cd)), _rows(gu), act)
+        dgu, h = dgu.view(gu.shape), h.view(gu.shape[:-1] + (H,))
+    else:
+        dh = linear_bwd.plain(dy, gu[..., :H], w2, empty, ACT_NONE, True, False, False)[0] \
+            if dy.is_cuda and cd in (torch.float16, torch.bfloat16) else dy @ w2.to(cd)
+        gate, up, dh = _wide(gu[..., :H]), _wide(gu[..., H:]), _wide(dh)
+        a, slope = _act_slope(gate, act)
+        dgu, h = torch.cat([dh * up * slope, dh * a], -1).to(cd), (a * up).to(cd)
+    if dy.is_cuda and cd in (torch.float16, torch.bfloat16):
+        _, dw2, db2 = linear_bwd.plain(dy, h, w2, empty, ACT_NONE, False, need_dw2, need_db2, b2)
+        dx, dw1, db1 = linear_bwd.plain(dgu, x, w1, empty, ACT_NONE, need_dx, need_dw1, need_db1, b1)
+        return dx, dw1, db1, dw2, db2
+    K, N = w1.shape[1], w2.shape[0]
+    d1, d2 = _wide(dgu).reshape(-1, 2 * H), _wide(dy).reshape(-1, N)
+    x2, h2 = x.to(d1.dtype).reshape(-1, K), h.to(d2.dtype).reshape(-1, H)
+    return tuple(f() if need else dy.new_empty(0) for need, f in (
+        (need_dx, lambda: dgu @ w1.to(cd)), (need_dw1, lambda: (d1.t() @ x2).to(w1.dtype)),
+        (need_db1, lambda: d1.sum(0)), (need_dw2, lambda: (d2.t() @ h2).to(w2.dtype)), (need_db2, lambda: d2.sum(0))))
+
+
+@gated_mlp_bwd.register_fake
+def _(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1=None, b2=None):
+    e, f32 = dy.new_empty(0), torch.float32
+    return (dy.new_empty(x.shape) if need_dx else e, torch.empty_like(w1) if need_dw1 else e,
+            dy.new_empty(w1.shape[0] if need_db1 else 0, dtype=f32), torch.empty_like(w2) if need_dw2 else e,
+            dy.new_empty(w2.shape[0] if need_db2 else 0, dtype=f32))
+
+
+def _gated_mlp_setup(ctx, inputs, output):
+    x, w1, b1, w2, b2, residual, act, _ = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, w1, w2, output[1], b1, b2)
+    ctx.act = act
+    ctx.res_dtype = None if residual is None else residual.dtype
+
+
+def _gated_mlp_backward(ctx, dy, dgu_unused):
+    x, w1, w2, gu, b1, b2 = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    if dy is None:
+        return (None,) * 8
+    out = [None] * 8
+    if any(need[:5]):
+        dy = dy.contiguous()
+        dx, dw1, db1, dw2, db2 = _bwd(ctx, gated_mlp_bwd)(dy, x, w1, w2, gu, ctx.act, need[0], need[1], need[2],
+                                                          need[3], need[4], b1, b2)
+        for i, g, t in ((0, dx, x), (1, dw1, w1), (2, db1, b1), (3, dw2, w2), (4, db2, b2)):
+            if need[i] and (g.numel() or not t.numel()):
+                out[i] = g.view(t.shape).to(t.dtype)
+    if need[5]:
+        out[5] = dy.to(ctx.res_dtype)
+    return tuple(out)
+
+
+_autograd(gated_mlp_fwd, 1, _gated_mlp_backward, setup=_gated_mlp_setup)
+
+
+def _for_backward(*tensors) -> bool:
+    """Whether a backward may follow: what a trace sees may be run again with gradients."""
+    return not _unobserved() or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
+
+
+def gated_mlp(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: Optional[Tensor],
+              activation: str = "silu", residual: Optional[Tensor] = None) -> Tensor:
+    """Gated feed-forward block: (act(x Wg^T + bg) * (x Wu^T + bu)) W2^T + b2 + residual for x [..., D], w1 [2H, D]
+    with Wg its first and Wu its last H rows (as ``swiglu`` and ``geglu`` have them), b1 [2H], w2 [N, H], b2 [N] and
+    residual [..., N].  Activations: silu, gelu, gelu_tanh.  One product computes both projections, the activation and
+    their product; gate and up are kept for the backward, which computes the values that W2 reads from them again.
+    Gate and up are rounded to x's type where they are kept, not on their way into the activation."""
+    if activation not in ("silu", "gelu", "gelu_tanh", "gelu_pytorch_tanh"):
+        raise ValueError(f"gated_mlp: unknown activation {activation!r}")
+    act = _ACT_NAMES[activation]
+    if isinstance(x, Tensor):
+        D, rows, N = x.shape[-1] if x.dim() else 0, w1.shape[0], w2.shape[0]
+        if w1.dim() != 2 or w2.dim() != 2 or x.dim() < 1 or w1.shape[1] != D or rows != 2 * w2.shape[1] or rows < 2 \
+                or D < 1 or N < 1:
+            raise ValueError(f"gated_mlp: x [..., D], w1 [2H, D] and w2 [N, H] are needed, not {tuple(x.shape)}, "
+                             f"{tuple(w1.shape)} and {tuple(w2.shape)}")
+        for name, t, shape in (("b1", b1, (rows,)), ("b2", b2, (N,)), ("residual", residual, x.shape[:-1] + (N,))):
+            if t is not None and t.shape != shape:
+                raise ValueError(f"gated_mlp: {name} {tuple(shape)} is needed, not {tuple(t.shape)}")
+        for t in (w1, w2, b1, b2, residual):
+            if t is not None and t.device != x.device:
+                raise ValueError(f"gated_mlp: x on {x.device}, an operand on {t.device}")
+    keep = _for_backward(x, w1, b1, w2, b2)
+    return _call(gated_mlp_fwd, x, w1, b1, w2, b2, residual, act, keep)
+
+
 # =========================================================================== norms
 @_custom_op("pfeife::norm_fwd")
 def norm_fwd(x: Tensor, gamma: Tensor, beta: Optional[Tensor], residual: Optional[Tensor],
@@ -1197,6 +1353,141 @@ def policy_loss(logits: Tensor, actions: Tensor, old_logps: Tensor, advantages: 
     return PolicyLoss(loss, logps.detach().view(shape), kl.detach(), clipped.detach())
 
 
+# --------------------------------------------------------------------------- output head with its cross entropy
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _head_kept(N: int, D: int) -> Tuple[int, int, int]:
+    """Rows and width of what is kept of the rows that count, and the size of their index"""
+    Mp = kx.head_padded(N)
+    return Mp, _pad_to8(D), 4 + 2 * Mp + N
+
+
+@_custom_op("pfeife::head_loss_fwd")
+def head_loss_fwd(x: Tensor, w: Tensor, target: Tensor, ignore_index: int, reduction: int
+                  ) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """x [N, D], w [V, D], target [N] -> (loss, and for the backward: the rows that count, packed; how many they are,
+    which, their labels and where each row is among them; two statistics of each; what the sum is multiplied by)"""
+    cd = compute_dtype(x)
+    if x.is_cuda and cd in (torch.float16, torch.bfloat16):
+        x2 = x if x.dtype == cd else kx.cast(x, cd)
+        return kx.head_fwd(x2, _weight_as(w, cd), target, ignore_index, reduction)
+    N, D = x.shape
+    Mp, Dp, size = _head_kept(N, D)
+    target = target.long()
+    counted = _tokens_counted(target, w.shape[0], ignore_index)
+    rows = counted.nonzero().squeeze(1)
+    M = rows.shape[0]
+    xc = x.new_zeros((Mp, Dp), dtype=cd)
+    xc[:M, :D] = x[rows]
+    index = torch.zeros(size, dtype=torch.int32, device=x.device)
+    index[0] = M
+    index[4:4 + M] = rows
+    index[4 + Mp:4 + Mp + M] = target[rows]
+    index[4 + 2 * Mp:] = torch.where(counted, counted.cumsum(0) - 1, -1)
+    z = _wide(F.linear(_wide(xc[:M, :D]), _wide(w.to(cd))))
+    each = torch.logsumexp(z, -1) - z.gather(1, target[rows].unsqueeze(1)).squeeze(1)
+    inv = x.new_tensor(1.0 / max(M, 1) if reduction == 1 else 1.0, dtype=torch.float32)
+    if reduction == 0:
+        loss = z.new_zeros(N).index_copy(0, rows, each)
+    else:
+        loss = each.double().sum() / (max(M, 1) if reduction == 1 else 1)
+    return loss.to(_loss_dtype(x)), xc, index, x.new_zeros((Mp, 2), dtype=torch.float32), inv
+
+
+def _loss_dtype(x: Tensor) -> torch.dtype:
+    return torch.float64 if x.dtype == torch.float64 else torch.float32
+
+
+@head_loss_fwd.register_fake
+def _(x, w, target, ignore_index, reduction):
+    N, D = x.shape
+    Mp, Dp, size = _head_kept(N, D)
+    f32 = lambda *shape: x.new_empty(shape, dtype=torch.float32)
+    return (x.new_empty((N,) if reduction == 0 else (), dtype=_loss_dtype(x)),
+            x.new_empty((Mp, Dp), dtype=compute_dtype(x)), x.new_empty(size, dtype=torch.int32), f32(Mp, 2), f32())
+
+
+@_custom_op("pfeife::head_loss_bwd")
+def head_loss_bwd(dloss: Tensor, xc: Tensor, index: Tensor, stats: Tensor, inv: Tensor, w: Tensor, N: int,
+                  by_row: bool, need_dx: bool, need_dw: bool) -> Tuple[Tensor, Tensor]:
+    """-> (dx [N, D], dw [V, D]); empty where not needed, or added to a registered gradient bucket"""
+    V, D = w.shape
+    if xc.is_cuda and xc.dtype in (torch.float16, torch.bfloat16):
+        slot = _slot(w) if need_dw else None
+        bucket = None
+        if slot is not None and slot.main_grad is not None:
+            bucket = slot.main_grad.view(V, D)
+        direct = bucket is not None and D % 8 == 0 and bucket.data_ptr() % 16 == 0
+        dtype = w.dtype if bucket is None and w.dtype == xc.dtype else torch.float32
+        dx, dw = kx.head_bwd(dloss, xc, index, stats, inv, _weight_as(w, xc.dtype), N, by_row, need_dx, need_dw, dtype,
+                             bucket if direct else None)
+        if bucket is not None and not direct:
+            bucket.add_(dw)
+        if bucket is not None or not need_dw:
+            dw = xc.new_empty(0, dtype=w.dtype)
+        return dx if need_dx else xc.new_empty(0), dw.to(w.dtype)
+    Mp, M = kx.head_padded(N), int(index[0])
+    rows, labels = (index[i:i + M].long() for i in (4, 4 + Mp))
+    x, wide = _wide(xc[:M, :D]), _wide(w.to(xc.dtype))
+    p = torch.softmax(F.linear(x, wide), -1)
+    p[torch.arange(M, device=p.device), labels] -= 1
+    g = dloss.to(p.dtype)
+    p = p * (g[rows].unsqueeze(1) if by_row else g * inv.to(p.dtype))
+    dx = xc.new_empty(0)
+    if need_dx:
+        dx = p.new_zeros(N, D).index_copy(0, rows, p @ wide).to(xc.dtype)
+    return dx, (p.t() @ x).to(w.dtype) if need_dw else xc.new_empty(0, dtype=w.dtype)
+
+
+@head_loss_bwd.register_fake
+def _(dloss, xc, index, stats, inv, w, N, by_row, need_dx, need_dw):
+    e = xc.new_empty(0)
+    return (xc.new_empty((N, w.shape[1])) if need_dx else e,
+            torch.empty_like(w) if need_dw else xc.new_empty(0, dtype=w.dtype))
+
+
+def _head_loss_setup(ctx, inputs, output):
+    x, w, _, _, reduction = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(w, *output[1:])
+    ctx.rows, ctx.by_row, ctx.x_dtype = x.shape[0], reduction == 0, x.dtype
+
+
+def _head_loss_backward(ctx, dloss, *unused):
+    if dloss is None:
+        return (None,) * 5
+    w, xc, index, stats, inv = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dx, dw = _bwd(ctx, head_loss_bwd)(dloss, xc, index, stats, inv, w, ctx.rows, ctx.by_row, need[0], need[1])
+    return (dx.to(ctx.x_dtype) if need[0] else None, dw if need[1] and dw.numel() else None) + (None,) * 3
+
+
+_autograd(head_loss_fwd, 1, _head_loss_backward, setup=_head_loss_setup)
+
+
+def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int = -100,
+                         reduction: str = "mean") -> Tensor:
+    """``cross_entropy(linear(x, weight), target)`` of x [..., D], weight [V, D] and target [...], without the logits:
+    neither they nor their gradient are ever whole in memory, and no more than x's rows and two numbers of each are kept
+    for the backward.  Logits are fp32 sums that are not rounded.  Rows whose target is ``ignore_index`` or outside
+    the vocabulary do not count: they are not read, cost no products, have a loss of 0 and a gradient of zeros,
+    whatever x holds there.  ``reduction``: mean over the rows that count (0 if there are none), sum, or none
+    (fp32 [...])."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
+    if isinstance(x, Tensor):
+        if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
+            raise ValueError(f"linear_cross_entropy: x [..., D] and a weight [V, D] are needed, not {tuple(x.shape)} "
+                             f"and {tuple(weight.shape)}")
+        if weight.device != x.device:
+            raise ValueError(f"linear_cross_entropy: x on {x.device}, the weight on {weight.device}")
+        _check_tokens("linear_cross_entropy", x, target)
+    loss = _call(head_loss_fwd, x.reshape(-1, x.shape[-1]), weight, target.reshape(-1), ignore_index,
+                 _REDUCTIONS[reduction])
+    return loss.view(target.shape) if reduction == "none" else loss
+
+
 # =========================================================================== embedding / rope
 @_custom_op("pfeife::embed_fwd")
 def embed_fwd(ids: Tensor, table: Tensor, out_dtype: torch.dtype) -> Tensor:
@@ -1251,6 +1542,86 @@ def embedding(ids: Tensor, table: Tensor, out_dtype: Optional[torch.dtype] = Non
     if out_dtype is None:
         out_dtype = compute_dtype(table)
     return _call(embed_fwd, ids, table, out_dtype)
+
+
+# --------------------------------------------------------------------------- scaled embedding
+@_custom_op("pfeife::scaled_embed_fwd")
+def scaled_embed_fwd(ids: Tensor, table: Tensor, scale: float, out_dtype: torch.dtype) -> Tensor:
+    if table.is_cuda and table.dtype in _EMBED_TYPES and out_dtype in _EMBED_TYPES:
+        t = table
+        s = _slot(table)
+        if s is not None and s.lp is not None and s.lp.dtype == out_dtype:
+            t = _weight_as(table, out_dtype)
+        elif t.dtype != out_dtype and t.dtype != torch.float32:
+            t = t.float()
+        return kx.scaled_embed_fwd(t, ids, scale, out_dtype)
+    inside = (ids >= 0) & (ids < table.shape[0])
+    if not table.shape[0]:
+        return table.new_zeros(ids.shape + table.shape[1:], dtype=out_dtype)
+    rows = _wide(table[ids.long().masked_fill(~inside, 0)]) * scale
+    return rows.masked_fill(~inside.unsqueeze(-1), 0.0).to(out_dtype)
+
+
+_EMBED_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+@scaled_embed_fwd.register_fake
+def _(ids, table, scale, out_dtype):
+    return table.new_empty(ids.shape + (table.shape[1],), dtype=out_dtype)
+
+
+@_custom_op("pfeife::scaled_embed_bwd")
+def scaled_embed_bwd(dout: Tensor, ids: Tensor, table: Tensor, scale: float) -> Tensor:
+    """-> the table's gradient (empty when it was added to a registered bucket)"""
+    if table.is_cuda and table.dtype in _EMBED_TYPES and dout.dtype in _EMBED_TYPES:
+        slot = _slot(table)
+        if slot is not None and slot.main_grad is not None:
+            kx.scaled_embed_bwd(dout, ids, table.shape[0], scale, torch.float32, slot.main_grad.view(table.shape))
+            return table.new_empty(0)
+        same = table.dtype == dout.dtype
+        g = kx.scaled_embed_bwd(dout, ids, table.shape[0], scale, table.dtype if same else torch.float32)
+        return g.to(table.dtype)
+    inside = ((ids >= 0) & (ids < table.shape[0])).reshape(-1)
+    g = torch.zeros(table.shape, dtype=_wide(table).dtype, device=table.device)
+    g.index_add_(0, ids.reshape(-1)[inside].long(), dout.reshape(-1, table.shape[1])[inside].to(g.dtype))
+    return (g * scale).to(table.dtype)
+
+
+@scaled_embed_bwd.register_fake
+def _(dout, ids, table, scale):
+    return table.new_empty(table.shape)
+
+
+def _scaled_embed_setup(ctx, inputs, output):
+    ctx.save_for_backward(inputs[0], inputs[1])
+    ctx.scale = inputs[2]
+
+
+def _scaled_embed_backward(ctx, dout):
+    ids, table = ctx.saved_tensors
+    g = _bwd(ctx, scaled_embed_bwd)(dout.contiguous(), ids, table, ctx.scale)
+    return None, (g if g.numel() or not table.numel() else None), None, None
+
+
+_autograd(scaled_embed_fwd, 1, _scaled_embed_backward, setup=_scaled_embed_setup)
+
+
+def scaled_embedding(ids: Tensor, table: Tensor, scale: float = 1.0, out_dtype: Optional[torch.dtype] = None) -> Tensor:
+    """scale * table[ids] for integers ids [...] and a table [V, D], rounded once to ``out_dtype`` (default: as
+    ``embedding``).  Ids outside the table, such as -1 for padding, have zeros and no gradient.  The table's gradient
+    adds up each row's tokens in their order, in 32 bits, rounded once: the same call gives the same bits, unlike
+    ``embedding``'s, whose sums are atomic."""
+    if out_dtype is None:
+        out_dtype = compute_dtype(table)
+    if isinstance(ids, Tensor):
+        if table.dim() != 2 or ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool \
+                or ids.device != table.device:
+            raise ValueError(f"scaled_embedding: integers on {table.device} and a table [V, D] are needed, not "
+                             f"{ids.dtype} on {ids.device} and {tuple(table.shape)}")
+        if not math.isfinite(scale) or not out_dtype.is_floating_point:
+            raise ValueError(f"scaled_embedding: a finite scale and a floating type are needed, not {scale} and "
+                             f"{out_dtype}")
+    return _call(scaled_embed_fwd, ids, table, float(scale), out_dtype)
 
 
 def _narrow(cos: Tensor, x: Tensor) -> bool:

@@ -627,6 +627,147 @@ def token_loss_bwd(gout: torch.Tensor, logits: torch.Tensor, labels: torch.Tenso
     return d
 
 
+# --------------------------------------------------------------------------- gated feed-forward blocks
+def glu_linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], act: int, keep: bool
+                   ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """x [M, K], w [2H, K] (gate first) -> (h [M, H] = act(gate) * up, both projections [M, 2H] when ``keep``)."""
+    L = _lib.calls()
+    assert x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1] and w.shape[0] % 2 == 0
+    assert x.dtype == w.dtype and x.stride(1) == 1 and w.stride(1) == 1 and w.device == x.device
+    M, H = x.shape[0], w.shape[0] // 2
+    if bias is not None:
+        bias = bias.contiguous()
+        assert bias.shape == (2 * H,) and bias.device == x.device
+    h = torch.empty((M, H), dtype=x.dtype, device=x.device)
+    gu = torch.empty((M, 2 * H), dtype=x.dtype, device=x.device) if keep else None
+    check(L.pf_glu_linear_fwd(x, w, bias, dt(bias.dtype) if bias is not None else 0, h, gu, M, H, x.shape[1],
+                              x.stride(0), w.stride(0), act, dt(x.dtype), status_word(x.device), sm_count(x.device),
+                              stream_of(x)), "pf_glu_linear_fwd")
+    return h, gu
+
+
+def glu_linear_bwd(dy: torch.Tensor, w2: torch.Tensor, gu: torch.Tensor, act: int
+                   ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """dy [M, K], w2 [K, H], gu [M, 2H] -> (the gradient of gu, h = act(gate) * up once more)"""
+    L = _lib.calls()
+    gu = _vectors(_like(gu, dy))
+    M, H = gu.shape[0], gu.shape[1] // 2
+    assert dy.shape == (M, w2.shape[0]) and w2.shape[1] == H and w2.dtype == dy.dtype
+    assert dy.stride(1) == 1 and w2.stride(1) == 1
+    dgu, h = torch.empty_like(gu), torch.empty((M, H), dtype=dy.dtype, device=dy.device)
+    check(L.pf_glu_linear_bwd(dy, w2, gu, dgu, h, M, H, dy.shape[1], dy.stride(0), w2.stride(0), act, dt(dy.dtype),
+                              status_word(dy.device), sm_count(dy.device), stream_of(dy)), "pf_glu_linear_bwd")
+    return dgu, h
+
+
+# --------------------------------------------------------------------------- output head with its cross entropy
+def head_padded(N: int) -> int:
+    """Rows of what the head's kernels keep of N rows."""
+    return (N + 255) // 256 * 256
+
+
+def _count(n: int, what: str) -> int:
+    if n < 0:
+        check(n, what)
+    return n
+
+
+def _head_weight(w: torch.Tensor) -> torch.Tensor:
+    """[V, D] -> rows on 16 bytes, D filled up with zeros to a multiple of 8"""
+    if w.shape[1] % 8:
+        return torch.nn.functional.pad(w, (0, -w.shape[1] % 8))
+    return w if w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.data_ptr() % 16 == 0 else \
+        w.clone(memory_format=torch.contiguous_format)
+
+
+def head_fwd(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, ignore_index: int, reduction: int
+             ) -> Tuple[torch.Tensor, ...]:
+    """x [N, D], w [V, D], target [N] -> (loss: [N] for reduction 0, the mean for 1, the sum for 2; then for the
+    backward the rows that count, where they come from, two statistics of each, what a sum is multiplied by)"""
+    L = _lib.calls()
+    assert x.dim() == 2 and x.dtype == w.dtype and x.shape[1] == w.shape[1] and target.shape == x.shape[:1]
+    assert w.device == x.device and target.device == x.device
+    if x.stride(1) != 1 or x.stride(0) % 8:
+        x = x.contiguous()
+    N, D = x.shape
+    w, target = _head_weight(w), target.long().contiguous()
+    V, Dp, Mp = w.shape[0], w.shape[1], head_padded(N)
+    new = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=x.device)
+    xc, stats, inv = new(Mp, Dp, dtype=x.dtype), new(Mp, 2), new()
+    loss = new(N) if reduction == 0 else new()
+    index = new(_count(L.pf_head_index(N), "pf_head_index"), dtype=torch.int32)
+    scratch = new(_count(L.pf_head_scratch(N, V), "pf_head_scratch") * 256)
+    check(L.pf_head_fwd(x, w, target, xc, index, stats, loss, inv, scratch, N, V, D, Dp, x.stride(0) if N > 1 else D,
+                        w.stride(0), ignore_index, reduction, dt(x.dtype), status_word(x.device), sm_count(x.device),
+                        stream_of(x)), "pf_head_fwd")
+    return loss, xc, index, stats, inv
+
+
+def head_bwd(dloss: torch.Tensor, xc: torch.Tensor, index: torch.Tensor, stats: torch.Tensor, inv: torch.Tensor,
+             w: torch.Tensor, N: int, by_row: bool, need_dx: bool, need_dw: bool,
+             dw_dtype: torch.dtype = torch.float32, dw: Optional[torch.Tensor] = None
+             ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """-> (dx [N, D], dw [V, D]); ``dw`` in fp32 is added to when given."""
+    L = _lib.calls()
+    w = _like(w, xc)
+    V, D = w.shape
+    w = _head_weight(w)
+    Dp, Mp, sms = w.shape[1], head_padded(N), sm_count(xc.device)
+    assert xc.shape == (Mp, Dp) and stats.shape == (Mp, 2) and w.device == xc.device
+    xc, stats, inv = _vectors(xc), _vectors(_floats(stats)), _floats(inv)
+    dloss = dloss if dloss.dtype == torch.float32 else dloss.float()
+    assert dloss.shape == ((N,) if by_row else ())
+    new = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=xc.device)
+    add = dw is not None
+    if add:
+        assert dw.dtype == torch.float32 and dw.shape == (V, D) and D == Dp and dw.is_contiguous()
+    elif need_dw:
+        dw = new(V, Dp, dtype=dw_dtype)
+    dx = new(N, D, dtype=xc.dtype) if need_dx else None
+    words = _count(L.pf_head_words(N, V), "pf_head_words")
+    dz = new(Mp, words, dtype=xc.dtype)
+    acc = new(_count(L.pf_head_parts(N, V, D, sms), "pf_head_parts") * Mp, Dp) if need_dx else None
+    factor = new(Mp + 1) if by_row else None
+    check(L.pf_head_bwd(dloss, inv, xc, w, index, stats, dx, dw, dz, acc, factor, N, V, D, Dp,
+                        dloss.stride(0) if by_row else 0, w.stride(0), Dp, int(by_row), int(add), dt(xc.dtype),
+                        dt(dw.dtype) if dw is not None else 0, status_word(xc.device), sms, stream_of(xc)),
+          "pf_head_bwd")
+    if need_dw and Dp != D:
+        dw = dw[:, :D].contiguous()
+    return dx, dw
+
+
+# --------------------------------------------------------------------------- embedded tokens
+def scaled_embed_fwd(table: torch.Tensor, ids: torch.Tensor, scale: float, out_dtype: torch.dtype) -> torch.Tensor:
+    L = _lib.calls()
+    table, ids = table.contiguous(), ids.long().contiguous()
+    V, D = table.shape
+    assert ids.device == table.device
+    out = torch.empty(ids.shape + (D,), dtype=out_dtype, device=table.device)
+    check(L.pf_scaled_embed_fwd(table, ids, out, ids.numel(), D, V, scale, dt(table.dtype), dt(out_dtype),
+                                stream_of(table)), "pf_scaled_embed_fwd")
+    return out
+
+
+def scaled_embed_bwd(dout: torch.Tensor, ids: torch.Tensor, words: int, scale: float, dtype: torch.dtype,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The table's gradient [words, D] in `dtype`; ``out`` in fp32 is added to when given."""
+    L = _lib.calls()
+    dout, ids = dout.contiguous(), ids.long().contiguous()
+    D, N = dout.shape[-1], ids.numel()
+    assert ids.device == dout.device and dout.shape[:-1] == ids.shape
+    add = out is not None
+    if add:
+        assert out.dtype == torch.float32 and out.shape == (words, D) and out.is_contiguous()
+    else:
+        out = torch.empty((words, D), dtype=dtype, device=dout.device)
+    scratch = torch.empty(_count(L.pf_scaled_embed_scratch(N, D, words), "pf_scaled_embed_scratch") * 256,
+                          dtype=torch.float32, device=dout.device)
+    check(L.pf_scaled_embed_bwd(dout, ids, out, scratch, N, D, words, scale, int(add), dt(dout.dtype), dt(out.dtype),
+                                stream_of(dout)), "pf_scaled_embed_bwd")
+    return out
+
+
 # --------------------------------------------------------------------------- attention
 def attention_supported(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bool:
     """True when the native flash-attention kernels cover this problem."""
