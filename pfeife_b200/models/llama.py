@@ -34,6 +34,9 @@ class LlamaConfig:
     rope_dim: Optional[int] = None                 # values of a head that rotate (default: all)
     rope_interleaved: bool = False                 # pairs (2i, 2i + 1)
     rope_scaling: Optional[ops.RopeScaling] = None
+    embed_scale: Optional[float] = None            # what embedded tokens are multiplied by; their gradient is then
+                                                   # summed in the order of the tokens
+    fused_mlp: bool = False                        # ops.gated_mlp instead of two products around a SwiGLU
 
 
 LLAMA_CONFIGS = {
@@ -64,6 +67,7 @@ class LlamaBlock(nn.Module):
         self.post_norm = nn.Parameter(torch.ones(d))
         self.gate_up = nn.Linear(d, 2 * cfg.intermediate_size, bias=False)
         self.down = nn.Linear(cfg.intermediate_size, d, bias=False)
+        self.fused_mlp = cfg.fused_mlp
 
     def forward(self, x: torch.Tensor, delta, cos: torch.Tensor, sin: torch.Tensor):
         """(x, delta) -> (x', delta'): the residual stream is x + delta, summed inside the next
@@ -88,6 +92,8 @@ class LlamaBlock(nn.Module):
         a = a.view(B, S, d)
         delta = ops.linear(a, self.o_proj.weight)
         y, x = ops.rms_norm(delta, self.post_norm, self.eps, residual=x)
+        if self.fused_mlp:
+            return x, ops.gated_mlp(y, self.gate_up.weight, None, self.down.weight, None, "silu")
         g = ops.swiglu(ops.linear(y, self.gate_up.weight))
         return x, ops.linear(g, self.down.weight)
 
@@ -113,9 +119,14 @@ class Llama(nn.Module):
             if isinstance(m, (nn.Linear, nn.Embedding)):
                 nn.init.normal_(m.weight, std=0.02)
 
-    def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
+    def forward(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Logits [B, S, V]; with ``labels`` [B, S], the token that each row predicts (-100 where none counts), the mean
+        loss over the rows that count instead, for which no logits are kept (``ops.linear_cross_entropy``)."""
         S = input_ids.shape[1]
-        x = ops.embedding(input_ids, self.embed.weight)
+        if self.cfg.embed_scale is None:
+            x = ops.embedding(input_ids, self.embed.weight)
+        else:
+            x = ops.scaled_embedding(input_ids, self.embed.weight, self.cfg.embed_scale)
         cos, sin = self.rope_cos[:S], self.rope_sin[:S]
         delta = None
         for layer in self.layers:
@@ -124,7 +135,14 @@ class Llama(nn.Module):
             y = ops.rms_norm(x, self.norm, self.cfg.rms_eps)
         else:
             y, _ = ops.rms_norm(delta, self.norm, self.cfg.rms_eps, residual=x)
+        if labels is not None:
+            return ops.linear_cross_entropy(y, self.lm_head.weight, labels)
         return ops.linear(y, self.lm_head.weight)
+
+
+def next_tokens(input_ids: torch.Tensor) -> torch.Tensor:
+    """Labels of next-token prediction for ``Llama.forward``: the ids shifted by one, none for the last row."""
+    return torch.cat([input_ids[:, 1:], torch.full_like(input_ids[:, :1], -100)], 1)
 
 
 def causal_lm_loss(logits: torch.Tensor, input_ids: torch.Tensor) -> torch.Tensor:

@@ -629,6 +629,7 @@ def _glu_native(x: Tensor, cd: torch.dtype, w1: Tensor, w2: Tensor) -> bool:
 
 
 def _aligned(w: Tensor) -> Tensor:
+    """`w` with rows on 16 bytes, as the products read them"""
     return w if w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.data_ptr() % 16 == 0 else \
         w.clone(memory_format=torch.contiguous_format)
 
@@ -639,19 +640,24 @@ def gated_mlp_fwd(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: O
     """-> (y, gate and up [..., 2H], empty unless they are to be kept for a backward)"""
     cd = compute_dtype(x)
     shape, H = x.shape[:-1], w2.shape[1]
+    if w2.is_cuda and w2.dtype == cd and H % 8 == 0:
+        w2 = _aligned(w2)
     if _glu_native(x, cd, w1, w2):
         x2 = _rows(x if x.dtype == cd else kx.cast(x, cd))
         h, gu = kx.glu_linear_fwd(x2, _aligned(_weight_as(w1, cd)), b1, act, keep)
         y, _ = linear_fwd.plain(h.view(shape + (H,)), w2, b2, residual, ACT_NONE)
         return y, (gu.view(shape + (2 * H,)) if keep else x.new_empty(0))
     if x.is_cuda and cd in (torch.float16, torch.bfloat16):      # odd widths, product by product
-        gu, _ = linear_fwd.plain(x, w1, b1, None, ACT_NONE)
+        x2, w = _rows(x if x.dtype == cd else kx.cast(x, cd)), _weight_as(w1, cd)
+        wide = kx.gemm(_aligned(_pad_k(x2)), _aligned(_pad_k(w)), out_dtype=torch.float32, bias=b1).view(
+            shape + (2 * H,))
     else:
-        gu = F.linear(x.to(cd), w1.to(cd), None if b1 is None else b1.to(cd))
-    wide = _wide(gu)
+        wide = F.linear(_wide(x.to(cd)), _wide(w1.to(cd)))
+        if b1 is not None:
+            wide = wide + b1.to(cd)
     h = (_act_slope(wide[..., :H], act)[0] * wide[..., H:]).to(cd)
     y, _ = linear_fwd.plain(h, w2, b2, residual, ACT_NONE)
-    return y, (gu if keep else x.new_empty(0))
+    return y, (wide.to(cd) if keep else x.new_empty(0))
 
 
 @gated_mlp_fwd.register_fake
@@ -675,6 +681,10 @@ def gated_mlp_bwd(dy: Tensor, x: Tensor, w1: Tensor, w2: Tensor, gu: Tensor, act
         zeros = lambda t, need: torch.zeros_like(t) if need else dy.new_empty(0)
         return (dy.new_zeros(x.shape), zeros(w1, need_dw1), dy.new_zeros(2 * H if need_db1 else 0, dtype=torch.float32),
                 zeros(w2, need_dw2), dy.new_zeros(w2.shape[0] if need_db2 else 0, dtype=torch.float32))
+    if w2.is_cuda and w1.dtype == cd and w1.shape[1] % 8 == 0:
+        w1 = _aligned(w1)
+    if w2.is_cuda and w2.dtype == cd and H % 8 == 0:
+        w2 = _aligned(w2)
     if _glu_native(dy, cd, w1, w2):
         dgu, h = kx.glu_linear_bwd(_rows(dy), _aligned(_weight_as(w2, cd)), _rows(gu), act)
         dgu, h = dgu.view(gu.shape), h.view(gu.shape[:-1] + (H,))

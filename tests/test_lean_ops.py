@@ -1,0 +1,618 @@
+"""Scaled embeddings, the gated feed-forward block and the head with its loss against their formulas in 64 bits.
+
+Bounds.  u is half a step of the result's type, 2^-24 half a step of fp32.  The tensor cores' sums of n products are off by
+a whole step (2^-23) of the sum of magnitudes for each of the n + 16 additions at most (they may cut bits off instead
+of rounding).  An activation is off by 1e-6 (1 + |z|), and changes by no more than 1.2 times its argument's error, its
+derivative by no more than 0.8 times.  Errors go through each formula by its partial derivatives, in magnitudes."""
+import math
+import threading
+
+import pytest
+import torch
+
+from pfeife_b200 import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+TINY = {torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -126}
+E = 2.0 ** -24
+
+
+def within(got, want, error):
+    """|got - want| <= error in the values, and half a step of got's type"""
+    bound = error + U[got.dtype] * (want.abs() + error) + TINY[got.dtype]
+    off = (got.double() - want).abs()
+    assert got.shape == want.shape and torch.isfinite(got).all()
+    assert (off <= bound).all(), float((off / bound).max())
+
+
+def sums(n):
+    return (n + 16) * 2.0 ** -23
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def normal(*shape, device, dtype, seed, std=1.0):
+    return (torch.randn(*shape, generator=gen(seed)) * std).to(device=device, dtype=dtype)
+
+
+# ------------------------------------------------------------------------------ embedding
+def tokens(kind, N, V, seed=0):
+    ids = torch.randint(0, V, (N,), generator=gen(seed))
+    if kind == "one":
+        ids[:] = V - 1
+    elif kind == "padded":
+        ids[N // 3:] = 0
+        ids[: N // 5] = -1
+    elif kind == "outside":
+        ids[::3] = V
+        ids[1::7] = -(1 << 40)
+        ids[2::11] = 1 << 40
+    elif kind == "few":
+        ids %= 3
+    return ids
+
+
+EMBED = [(1, 1, 1, "any"), (5, 7, 16, "any"), (64, 256, 64, "any"), (33, 9, 13, "few"), (1027, 3001, 77, "padded"),
+         (2049, 512, 1032, "any"), (300, 4, 8, "one"), (4096, 40, 24, "few"), (4097, 33000, 8, "outside"),
+         (9001, 300, 136, "padded"), (70001, 262145, 8, "any"), (20000, 70000, 5, "one")]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,wide", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32),
+                                        (torch.bfloat16, torch.float32), (torch.float32, torch.float32),
+                                        (torch.float16, torch.float16)], ids=str)
+@pytest.mark.parametrize("N,V,D,kind", EMBED, ids=str)
+def test_scaled_embedding(N, V, D, kind, dtype, wide, device):
+    scale = 1.0 if N == 64 else 5.37
+    ids = tokens(kind, N, V).to(device)
+    table = normal(V, D, device=device, dtype=wide, seed=1).requires_grad_()
+    dy = normal(N, D, device=device, dtype=dtype, seed=2)
+    y = ops.scaled_embedding(ids, table, scale, out_dtype=dtype)
+    (g,) = torch.autograd.grad(y, table, dy)
+    assert y.dtype == dtype and g.dtype == wide
+    inside = (ids >= 0) & (ids < V)
+    at = ids.masked_fill(~inside, 0)
+    want = table.detach().double()[at].masked_fill(~inside[:, None], 0.0) * scale
+    within(y.detach(), want, E * want.abs())
+    total, mag = (torch.zeros(V, D, dtype=torch.float64, device=device) for _ in range(2))
+    total.index_add_(0, ids[inside], dy[inside].double())
+    mag.index_add_(0, ids[inside], dy[inside].double().abs())
+    times = torch.zeros(V, dtype=torch.float64, device=device).index_add_(0, ids[inside], torch.ones(
+        int(inside.sum()), dtype=torch.float64, device=device))
+    within(g, total * scale, (times[:, None] + 2) * E * mag * scale)
+    assert not g[times == 0].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [130, 4096, 50000])
+def test_sums_of_tokens_go_in_their_order(N):
+    """In the order of the tokens, in windows: the same bits every time, and exact sums where all partial sums are."""
+    ids = tokens("padded", N, 50).cuda()
+    table = torch.zeros(50, 32, device="cuda", requires_grad=True)
+    dy = torch.randint(-8, 9, (N, 32), generator=gen(3)).cuda().to(torch.bfloat16)
+    g = [torch.autograd.grad(ops.scaled_embedding(ids, table, 2.0, out_dtype=dy.dtype), table, dy)[0] for _ in range(3)]
+    want = torch.zeros(50, 32, dtype=torch.float64, device="cuda").index_add_(0, ids.clamp(min=0), torch.where(
+        ids[:, None] >= 0, dy.double(), 0.0)) * 2.0
+    assert torch.equal(g[0].double(), want) and torch.equal(g[0], g[1]) and torch.equal(g[0], g[2])
+    dy = normal(N, 32, device="cuda", dtype=torch.bfloat16, seed=4)
+    g = [torch.autograd.grad(ops.scaled_embedding(ids, table, 2.0, out_dtype=dy.dtype), table, dy)[0] for _ in range(3)]
+    assert torch.equal(g[0], g[1]) and torch.equal(g[0], g[2])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_embedded_tokens_of_any_shape(device):
+    """Ids of several dimensions, types and strides, a table and a gradient that are views."""
+    big = normal(40, 48, device=device, dtype=torch.bfloat16, seed=1)
+    for table in (big[:, 8:40], big[::2], big.t()):
+        V, D = table.shape
+        table = table.detach().requires_grad_()
+        ids = torch.randint(0, V, (6, 10), generator=gen(1)).to(device)
+        for i in (ids, ids.t(), ids.int(), ids.to(torch.int16)[:, 1::2], ids[:0], ids[0, 0]):
+            y = ops.scaled_embedding(i, table, 0.5)
+            assert y.shape == i.shape + (D,) and torch.equal(y, (table[i.long()] * 0.5).detach())
+            dy = normal(*i.shape, 2 * D, device=device, dtype=y.dtype, seed=2)[..., ::2]
+            (g,) = torch.autograd.grad(y, table, dy)
+            n = max(1, i.numel())
+            want, mag = (torch.zeros(V, D, dtype=torch.float64, device=device) for _ in range(2))
+            want.index_add_(0, i.long().reshape(-1), dy.double().reshape(-1, D))
+            mag.index_add_(0, i.long().reshape(-1), dy.double().abs().reshape(-1, D))
+            within(g, want * 0.5, (n + 2) * E * mag)
+    y = ops.scaled_embedding(ids, table, 0.5)
+    (g,) = torch.autograd.grad(y.sum(), table)            # a gradient that is broadcast
+    assert torch.equal(g[:, 0].float(), torch.bincount(ids.reshape(-1), minlength=V).to(g.dtype).float() * 0.5)
+
+
+# ------------------------------------------------------------------------------ gated feed-forward block
+def act64(z, kind):
+    if kind == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s + z * s * (1 - s)
+    if kind == "gelu":
+        phi = 0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+        return z * phi, phi + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    q = 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+    s = torch.sigmoid(q)
+    return z * s, s + z * s * (1 - s) * 2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * z * z)
+
+
+def mlp64(x, w1, b1, w2, b2, res, dy, kind, u):
+    """((value, its error) of y, dx, dw1, db1, dw2, db2) with 16-bit values of half a step u in between"""
+    x, w1, w2, dy = (t.detach().double() for t in (x, w1, w2, dy))
+    K, H, N, M = x.shape[1], w2.shape[1], w2.shape[0], x.shape[0]
+    z, zm = x @ w1.t(), x.abs() @ w1.abs().t()
+    if b1 is not None:
+        z, zm = z + b1.detach().double(), zm + b1.detach().double().abs()
+    ez = sums(K) * zm
+    gate, up, eg, eu = z[:, :H], z[:, H:], ez[:, :H], ez[:, H:]
+    a, slope = act64(gate, kind)
+
+    def hidden(eg, eu):
+        ea = 1.2 * eg + 1e-6 * (1 + gate.abs())
+        e = ea * (up.abs() + eu) + a.abs() * eu
+        return e + u * (a * up).abs() + u * e
+    h, eh = a * up, hidden(eg, eu)
+    y, ey = h @ w2.t(), eh @ w2.abs().t() + sums(H) * (h.abs() + eh) @ w2.abs().t()
+    for t in (b2, res):
+        if t is not None:
+            y, ey = y + t.detach().double(), ey + E * (y.abs() + t.detach().double().abs())
+    eg, eu = (e + u * (t.abs() + e) for e, t in ((eg, gate), (eu, up)))       # as they were kept
+    dh, dhm = dy @ w2, dy.abs() @ w2.abs()
+    edh = sums(N) * dhm
+    dg, du = dh * up * slope, dh * a
+    es = 0.8 * eg + 1e-6 * (1 + gate.abs())
+    ea = 1.2 * eg + 1e-6 * (1 + gate.abs())
+    edg = edh * ((up.abs() + eu) * 1.2) + (dh.abs() + edh) * (eu * 1.2 + (up.abs() + eu) * es)
+    edu = edh * a.abs() + (dh.abs() + edh) * ea
+    d = torch.cat([dg, du], 1)
+    ed = torch.cat([edg, edu], 1)
+    ed = ed + u * (d.abs() + ed)
+    eh = hidden(eg, eu)
+    dx, edx = d @ w1, ed @ w1.abs() + sums(2 * H) * (d.abs() + ed) @ w1.abs()
+    dw1, edw1 = d.t() @ x, ed.t() @ x.abs() + sums(M) * (d.abs() + ed).t() @ x.abs()
+    dw2, edw2 = dy.t() @ h, dy.abs().t() @ eh + sums(M) * dy.abs().t() @ (h.abs() + eh)
+    return ((y, ey), (dx, edx), (dw1, edw1), (dw2, edw2), (d.sum(0), ed.sum(0) + sums(M) * (d.abs() + ed).sum(0)),
+            (dy.sum(0), sums(M) * dy.abs().sum(0)))
+
+
+MLP = [(1, 8, 8, 8, "silu", False, False), (3, 16, 24, 8, "gelu", True, False), (64, 64, 128, 64, "silu", False, True),
+       (129, 72, 136, 40, "gelu_tanh", True, True), (257, 264, 520, 264, "gelu", True, True),
+       (7, 128, 1000, 72, "silu", True, False), (300, 40, 64, 1032, "gelu_tanh", False, False),
+       (2500, 128, 648, 128, "silu", False, True),       # tiles of pairs, the last of them ragged
+       (5, 20, 30, 12, "silu", True, True), (33, 24, 27, 16, "gelu", False, True), (2, 3, 1, 1, "silu", False, False)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("M,K,H,N,kind,biases,residual", MLP, ids=str)
+def test_gated_mlp(M, K, H, N, kind, biases, residual, dtype, device):
+    new = lambda *s, seed, std=1.0: normal(*s, device=device, dtype=dtype, seed=seed, std=std)
+    x, w1 = new(M, K, seed=1), new(2 * H, K, seed=2, std=1.5 * K ** -0.5)
+    w2, dy = new(N, H, seed=3, std=H ** -0.5), new(M, N, seed=4)
+    b1, b2 = (new(2 * H, seed=5, std=0.3), new(N, seed=6)) if biases else (None, None)
+    res = new(M, N, seed=7) if residual else None
+    leaves = [t.requires_grad_() for t in (x, w1, w2, b1, b2, res) if t is not None]
+    y = ops.gated_mlp(x, w1, b1, w2, b2, kind, res)
+    grads = dict(zip(map(id, leaves), torch.autograd.grad(y, leaves, dy)))
+    want = mlp64(x, w1, b1, w2, b2, res, dy, kind, U[dtype])
+    within(y.detach(), *want[0])
+    for t, w in zip((x, w1, w2, b1, b2), want[1:]):
+        if t is not None:
+            assert grads[id(t)].dtype == dtype
+            within(grads[id(t)], *w)
+    if residual:
+        assert torch.equal(grads[id(res)], dy)
+    with torch.no_grad():
+        assert torch.equal(ops.gated_mlp(x, w1, b1, w2, b2, kind, res), y)
+    again = torch.autograd.grad(ops.gated_mlp(x, w1, b1, w2, b2, kind, res), leaves[:3], dy)
+    assert all(torch.equal(a, grads[id(t)]) for a, t in zip(again, leaves))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gated_mlp_of_views(device):
+    """Rows, weights and gradients that are slices, transposed or off their vectors; dims in front; some gradients."""
+    new = lambda *s, seed: normal(*s, device=device, dtype=torch.bfloat16, seed=seed, std=0.3)
+    x = new(2, 5, 72, seed=1)[:, 1:4, 4:36]
+    w1 = new(65, 32, seed=2)[1:].requires_grad_()
+    w2 = new(32, 24, seed=3).t().requires_grad_()
+    off = new(24 * 32 + 1, seed=3)[1:].view(24, 32)
+    dy = new(3, 2, 24, seed=4).transpose(0, 1)
+    for second in (w2, off):
+        y = ops.gated_mlp(x, w1, None, second, None)
+        want = mlp64(x.reshape(-1, 32), w1, None, second, None, None, dy.reshape(-1, 24), "silu", U[torch.bfloat16])
+        within(y.detach().reshape(-1, 24), *want[0])
+        (dw1,) = torch.autograd.grad(y, w1, dy)
+        within(dw1, *want[2])
+    x = x.detach().requires_grad_()
+    y = ops.gated_mlp(x, w1.detach(), None, w2.detach(), None)
+    within(torch.autograd.grad(y, x, dy)[0].reshape(-1, 32), *mlp64(
+        x.reshape(-1, 32), w1, None, w2, None, None, dy.reshape(-1, 24), "silu", U[torch.bfloat16])[1])
+    y = ops.gated_mlp(x[:, :0], w1, None, w2, None)
+    dx, dw1, dw2 = torch.autograd.grad(y, [x, w1, w2], y)
+    assert y.shape == (2, 0, 24) and not dx.any() and not dw1.any() and not dw2.any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_large_gates(device):
+    """Gates far out: the activation is the gate or nothing, its derivative one or nothing, and nothing is a NaN."""
+    for dtype, far in ((torch.bfloat16, 1e18), (torch.float16, 6e4)):
+        for kind in ("silu", "gelu", "gelu_tanh"):
+            if device == "cpu" and kind == "gelu_tanh":
+                far = min(far, 1e12)                  # whose cube fp32 has
+            gates = torch.tensor([far, -far, 200.0, -200.0, 88.5, -88.5, -12.0, 0.0])
+            x = torch.ones(1, 8, device=device, dtype=dtype, requires_grad=True)
+            w1 = torch.zeros(16, 8, device=device, dtype=dtype)
+            w1[:8, 0], w1[8:, 1] = gates.to(device, dtype), 1.0
+            w1.requires_grad_()
+            y = ops.gated_mlp(x, w1, None, torch.eye(8, device=device, dtype=dtype), None, kind)
+            (dw1,) = torch.autograd.grad(y, w1, torch.ones_like(y))
+            a, slope = act64(w1[:8, 0].detach().double().clamp(-1e4, 1e4), kind)
+            a = torch.where(w1[:8, 0] > 1e4, w1[:8, 0].double(), a)
+            within(y.detach()[0], a, 1e-6 * (1 + a.abs()) + U[dtype] * a.abs())
+            within(dw1[:8, 0], slope, 1e-5 + U[dtype] * slope.abs())
+
+
+# ------------------------------------------------------------------------------ head and loss
+def head64(x, w, target, g, reduction, u, unit, ignore=-100):
+    """((value, error) of the loss, dx, dw), rows that count only"""
+    x, w, g = x.detach().double(), w.detach().double(), g.double()
+    counted = (target >= 0) & (target < w.shape[0]) & (target != ignore)
+    rows = counted.nonzero().squeeze(1)
+    xr, t, at = x[rows], target[rows].long(), torch.arange(len(rows), device=x.device)
+    z, ez = xr @ w.t(), sums(x.shape[1]) * (xr.abs() @ w.abs().t())
+    logp = torch.log_softmax(z, -1)
+    p, most = logp.exp(), ez.amax(-1, keepdim=True) if len(rows) else ez.new_zeros(0, 1)
+    each = -logp[at, t]
+    e_each = 2 * most.squeeze(1) + 1e-6 + 2 * E * (z.abs().amax(-1) if len(rows) else 0)
+    n = max(1, len(rows)) if reduction == "mean" else 1
+    if reduction == "none":
+        loss, e_loss = (torch.zeros(len(x), dtype=torch.float64, device=x.device).index_copy(0, rows, v)
+                        for v in (each, e_each))
+        coef = g[rows][:, None]
+    else:
+        loss, e_loss = each.sum() / n, e_each.sum() / n
+        coef = g / n
+    d = p.clone()
+    d[at, t] -= 1
+    ed = p * (2 * (most + ez) + 4e-6)
+    ed = ed + u * (d.abs() + ed) + 2.0 ** -25 / unit       # 16 bits of dz, before its factor
+    c = coef.abs() * (1 + 4 * E)
+    dx, dw = torch.zeros_like(x), (coef * d).t() @ xr
+    edx = torch.zeros_like(x)
+    dx[rows] = coef * d @ w
+    edx[rows] = c * (ed + sums(w.shape[0]) * (d.abs() + ed)) @ w.abs()
+    edw = (c * (ed + sums(len(rows)) * (d.abs() + ed))).t() @ xr.abs()
+    return (loss, e_loss), (dx, edx), (dw, edw)
+
+
+HEAD = [(1, 8, 1, 1.0, "mean"), (3, 16, 9, 1.0, "none"), (64, 64, 256, 0.7, "mean"), (300, 264, 1001, 0.7, "none"),
+        (130, 100, 129, 0.5, "sum"), (257, 72, 5000, 0.9, "mean"), (1000, 40, 301, 0.2, "none"), (9, 3, 65, 1.0, "sum"),
+        (100, 64, 70, 0.0, "mean"), (700, 136, 4097, 1.0, "mean")]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("N,D,V,part,reduction", HEAD, ids=str)
+def test_head(N, D, V, part, reduction, dtype, device):
+    x = normal(N, D, device=device, dtype=dtype, seed=1).requires_grad_()
+    w = normal(V, D, device=device, dtype=dtype, seed=2, std=2.0 * D ** -0.5).requires_grad_()
+    target = torch.randint(0, V, (N,), generator=gen(3))
+    target[torch.rand(N, generator=gen(4)) >= part] = -100
+    target[N // 2:: 17] = V                               # outside the vocabulary
+    target = target.to(device)
+    g = torch.randn(N, generator=gen(5)).to(device) if reduction == "none" else torch.tensor(0.37, device=device)
+    loss = ops.linear_cross_entropy(x, w, target, reduction=reduction)
+    dx, dw = torch.autograd.grad(loss, [x, w], g)
+    unit = 2.0 ** 15 if dtype == torch.float16 else 2.0 ** 100
+    if reduction == "none":
+        unit /= 2 * float(g.abs().max())                  # rows' factors are divided by a power of two near the largest
+        unit = unit * float(g.abs().min())
+    want = head64(x, w, target, g, reduction, U[dtype], unit)
+    assert loss.dtype == torch.float32 and dx.dtype == dw.dtype == dtype
+    within(loss.detach(), *want[0])
+    within(dx, *want[1])
+    within(dw, *want[2])
+    counted = (target >= 0) & (target < V)
+    assert not dx[~counted].any()
+    if reduction == "none":
+        assert not loss[~counted].any()
+    again = torch.autograd.grad(ops.linear_cross_entropy(x, w, target, reduction=reduction), [x, w], g)
+    assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
+    with torch.no_grad():
+        assert torch.equal(ops.linear_cross_entropy(x, w, target, reduction=reduction), loss)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_head_in_pieces(reduction):
+    """More rows and words than one piece of the backward has: the last piece is ragged."""
+    N, D, V = 33000, 16, 9000
+    x = normal(N, D, device="cuda", dtype=torch.bfloat16, seed=1).requires_grad_()
+    w = normal(V, D, device="cuda", dtype=torch.bfloat16, seed=2, std=0.5).requires_grad_()
+    target = torch.randint(0, V, (N,), generator=gen(3)).cuda()
+    g = torch.rand(N, generator=gen(5)).cuda() + 0.1 if reduction == "none" else torch.tensor(1.0, device="cuda")
+    dx, dw = torch.autograd.grad(ops.linear_cross_entropy(x, w, target, reduction=reduction), [x, w], g)
+    want = head64(x, w, target, g, reduction, U[torch.bfloat16], 2.0 ** 100)
+    within(dx, *want[1])
+    within(dw, *want[2])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_that_do_not_count_reach_nothing(device):
+    """Whatever they hold: infinities and NaN, in rows between others and behind the last."""
+    N, D, V = 150, 24, 40
+    target = torch.randint(0, V, (N,), generator=gen(1))
+    target[::3], target[140:] = -100, -1
+    target = target.to(device)
+    x = normal(N, D, device=device, dtype=torch.bfloat16, seed=1)
+    w = normal(V, D, device=device, dtype=torch.bfloat16, seed=2).requires_grad_()
+    bad = x.clone()
+    bad[target < 0] = torch.tensor([math.nan, math.inf, -math.inf], device=device).repeat(8).to(x.dtype)
+    out = []
+    for t in (x, bad):
+        t = t.requires_grad_()
+        loss = ops.linear_cross_entropy(t, w, target)
+        out.append((loss.detach(), *torch.autograd.grad(loss, [t, w])))
+    assert all(torch.equal(a, b) for a, b in zip(*out)) and torch.isfinite(out[0][0])
+    assert not out[1][1][target < 0].any()
+    # a row that counts keeps its NaN to itself, but for the weights
+    bad = x.detach().clone()
+    bad[1, 0] = math.nan
+    bad.requires_grad_()
+    each = ops.linear_cross_entropy(bad, w, target, reduction="none")
+    (dx,) = torch.autograd.grad(each.sum(), bad)
+    assert each.isnan().nonzero().squeeze(1).tolist() == [1]
+    assert torch.equal(dx[2:], out[0][1][2:] * 0 + torch.autograd.grad(ops.linear_cross_entropy(
+        x, w, target, reduction="none").sum(), x)[0][2:])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_head_of_views_and_frozen_parts(device):
+    x = normal(4, 9, 48, device=device, dtype=torch.float16, seed=1)[:, 1:, 3:35].requires_grad_()
+    wide = normal(60, 41, device=device, dtype=torch.float16, seed=2, std=0.4)
+    target = torch.randint(0, 60, (8, 4), generator=gen(3)).to(device).t()
+    g = torch.tensor(0.5, device=device)
+    for w in (wide[:, 1:33], wide[:, :32].t().contiguous().t(), wide[::2, 8:40].detach()):
+        w = w.detach().requires_grad_()
+        flat = (x.reshape(-1, 32), w, target.reshape(-1))
+        want = head64(*flat, g, "mean", U[torch.float16], 2.0 ** 15)
+        loss = ops.linear_cross_entropy(x, w, target.to(torch.int32))
+        within(loss.detach(), *want[0])
+        dx, dw = torch.autograd.grad(loss, [x, w], g)
+        within(dx.reshape(-1, 32), *want[1])
+        within(dw, *want[2])
+        (only,) = torch.autograd.grad(ops.linear_cross_entropy(x.detach(), w, target), w, g)
+        assert torch.equal(only, dw)
+        (only,) = torch.autograd.grad(ops.linear_cross_entropy(x, w.detach(), target), x, g)
+        assert torch.equal(only, dx)
+    each = ops.linear_cross_entropy(x, w, target, reduction="none")
+    assert each.shape == target.shape
+    (a,) = torch.autograd.grad(each.sum(), x, retain_graph=True)      # one value for all rows
+    (b,) = torch.autograd.grad(each, x, torch.ones_like(each))
+    assert torch.equal(a, b)
+    other = ops.linear_cross_entropy(x, w, target.where(target != 7, -5), ignore_index=3)
+    want = head64(x.reshape(-1, 32), w, target.where(target != 7, -5).reshape(-1), g, "mean", U[torch.float16],
+                  2.0 ** 15, ignore=3)
+    within(other.detach(), *want[0])
+    none = x.detach()[:, :0].requires_grad_()
+    loss = ops.linear_cross_entropy(none, w, target[:, :0])
+    dx, dw = torch.autograd.grad(loss, [none, w])
+    assert float(loss.detach()) == 0.0 and dx.shape == none.shape and not dw.any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_small_gradients_of_a_loss(device):
+    """The mean over many rows and a vocabulary of small probabilities: fp16 would lose them without their factor."""
+    N, D, V = 2048, 64, 3000
+    x = normal(N, D, device=device, dtype=torch.float16, seed=1).requires_grad_()
+    w = normal(V, D, device=device, dtype=torch.float16, seed=2, std=0.02).requires_grad_()
+    target = torch.zeros(N, dtype=torch.int64, device=device)
+    g = torch.tensor(65536.0, device=device)
+    loss = ops.linear_cross_entropy(x, w, target)
+    dx, dw = torch.autograd.grad(loss, [x, w], g)
+    want = head64(x, w, target, g, "mean", U[torch.float16], 2.0 ** 15)
+    within(dw, *want[2])
+    rest = want[2][0][1:]                                  # words that are no label
+    assert float((dw[1:].double() - rest).norm() / rest.norm()) < 2e-3
+
+
+# ------------------------------------------------------------------------------ differences, refusals
+def test_gradients_are_those_of_differences():
+    """In 64 bits, where the formulas are the kernels' (the kernels have no such type)."""
+    f64 = lambda *s, seed: torch.randn(*s, dtype=torch.float64, generator=gen(seed)).requires_grad_()
+    x, w1, w2, res = f64(3, 4, 6, seed=1), f64(14, 6, seed=2), f64(5, 7, seed=3), f64(3, 4, 5, seed=4)
+    b1, b2 = f64(14, seed=5), f64(5, seed=6)
+    for kind in ("silu", "gelu", "gelu_tanh"):
+        assert torch.autograd.gradcheck(lambda *a: ops.gated_mlp(*a[:5], kind, a[5]), [x, w1, b1, w2, b2, res])
+    w, target = f64(9, 6, seed=7), torch.randint(0, 9, (3, 4), generator=gen(8))
+    target[0, 1], target[2, 2] = -100, 9
+    for reduction in ("mean", "sum", "none"):
+        assert torch.autograd.gradcheck(lambda a, b: ops.linear_cross_entropy(a, b, target, reduction=reduction), [x, w])
+    ids = torch.tensor([[0, 2, 2], [4, -1, 7]])
+    assert torch.autograd.gradcheck(lambda t: ops.scaled_embedding(ids, t, 1.7), [f64(5, 4, seed=9)])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    new = lambda *s: torch.zeros(*s, device=device, dtype=torch.bfloat16)
+    for bad in (lambda: ops.gated_mlp(new(4, 8), new(16, 9), None, new(8, 8), None),
+                lambda: ops.gated_mlp(new(4, 8), new(15, 8), None, new(8, 8), None),
+                lambda: ops.gated_mlp(new(4, 8), new(16, 8), None, new(8, 9), None),
+                lambda: ops.gated_mlp(new(4, 8), new(16, 8), new(8), new(8, 8), None),
+                lambda: ops.gated_mlp(new(4, 8), new(16, 8), None, new(8, 8), new(4)),
+                lambda: ops.gated_mlp(new(4, 8), new(16, 8), None, new(8, 8), None, residual=new(8)),
+                lambda: ops.gated_mlp(new(4, 8), new(16, 8), None, new(8, 8), None, "relu"),
+                lambda: ops.gated_mlp(new(4, 8), new(0, 8), None, new(8, 0), None),
+                lambda: ops.linear_cross_entropy(new(4, 8), new(9, 7), new(4).long()),
+                lambda: ops.linear_cross_entropy(new(4, 8), new(0, 8), new(4).long()),
+                lambda: ops.linear_cross_entropy(new(4, 8), new(9, 8), new(5).long()),
+                lambda: ops.linear_cross_entropy(new(4, 8), new(9, 8), new(4)),
+                lambda: ops.linear_cross_entropy(new(4, 8), new(9, 8), new(4).long(), reduction="max"),
+                lambda: ops.scaled_embedding(new(4), new(9, 8)),
+                lambda: ops.scaled_embedding(new(4) > 0, new(9, 8)),
+                lambda: ops.scaled_embedding(new(4).long(), new(9)),
+                lambda: ops.scaled_embedding(new(4).long(), new(9, 8), math.inf),
+                lambda: ops.scaled_embedding(new(4).long(), new(9, 8), out_dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@pytest.mark.gpu
+def test_operands_of_two_devices_are_refused():
+    new = lambda *s, d="cuda": torch.zeros(*s, device=d, dtype=torch.bfloat16)
+    for bad in (lambda: ops.gated_mlp(new(4, 8), new(16, 8, d="cpu"), None, new(8, 8), None),
+                lambda: ops.gated_mlp(new(4, 8), new(16, 8), None, new(8, 8), None, residual=new(4, 8, d="cpu")),
+                lambda: ops.linear_cross_entropy(new(4, 8), new(9, 8, d="cpu"), new(4).long()),
+                lambda: ops.linear_cross_entropy(new(4, 8), new(9, 8), new(4, d="cpu").long()),
+                lambda: ops.scaled_embedding(new(4, d="cpu").long(), new(9, 8))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+# ------------------------------------------------------------------------------ how a program uses them
+def _all(device, dtype, seed=0, N=70):
+    """(leaves, a function that takes them through embedding, block and head to a loss)"""
+    table = normal(50, 32, device=device, dtype=dtype, seed=seed + 1)
+    w1, w2 = (normal(*s, device=device, dtype=dtype, seed=seed + i, std=0.2) for s, i in (((96, 32), 2), ((32, 48), 3)))
+    head = normal(50, 32, device=device, dtype=dtype, seed=seed + 4, std=0.3)
+    leaves = [t.requires_grad_() for t in (table, w1, w2, head)]
+
+    def run(ids, labels):
+        h = ops.scaled_embedding(ids, leaves[0], 1.5)
+        h = ops.gated_mlp(h, leaves[1], None, leaves[2], None, residual=h)
+        return ops.linear_cross_entropy(h, leaves[3], labels)
+    return leaves, run
+
+
+def _data(device, seed, N=70):
+    ids = torch.randint(0, 50, (N,), generator=gen(seed))
+    labels = torch.randint(0, 50, (N,), generator=gen(seed + 1))
+    labels[::5] = -100
+    return ids.to(device), labels.to(device)
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed():
+    """A forward and backward in a graph, replayed on other data beside a second graph and eager calls."""
+    leaves, run = _all("cuda", torch.bfloat16)
+    graphs = []
+    for seed in (10, 20):
+        ids, labels = _data("cuda", seed)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for _ in range(2):
+                torch.autograd.grad(run(ids, labels), leaves)
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            loss = run(ids, labels)
+            grads = torch.autograd.grad(loss, leaves)
+        graphs.append((graph, ids, labels, loss, grads))
+    for seed in (30, 40, 50):
+        for i, (graph, ids, labels, loss, grads) in enumerate(graphs):
+            new = _data("cuda", seed + 5 * i)
+            ids.copy_(new[0])
+            labels.copy_(new[1] if seed != 40 else torch.full_like(new[1], -100))
+            graph.replay()
+        for graph, ids, labels, loss, grads in graphs:
+            want = run(ids, labels)
+            assert torch.equal(want, loss)
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(want, leaves), grads))
+
+
+@pytest.mark.gpu
+def test_streams_and_threads():
+    leaves, run = _all("cuda", torch.bfloat16)
+    data = [_data("cuda", 10 * i, N=70 + 300 * i) for i in range(4)]
+    want = [(l, torch.autograd.grad(l, leaves)) for l in (run(*d) for d in data)]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                loss = run(*data[i])
+                got[i] = (loss, torch.autograd.grad(loss, leaves))
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for (a, ga), (b, gb) in zip(want, got):
+        assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(ga, gb))
+
+
+@pytest.mark.gpu
+def test_registered_weights_get_their_gradients_in_their_buckets():
+    """16-bit shadows are read and fp32 buckets added to, tied weights included, as gradients of autograd would be."""
+    leaves, run = _all("cuda", torch.float32)
+    ids, labels = _data("cuda", 10)
+    try:
+        low = [t.detach().to(torch.bfloat16).requires_grad_() for t in leaves]
+        h = ops.scaled_embedding(ids, low[0], 1.5)
+        h = ops.gated_mlp(h, low[1], None, low[2], None, residual=h)
+        want = torch.autograd.grad(ops.linear_cross_entropy(h, low[3], labels), low)
+        buckets = [torch.full(t.shape, 3.0, device="cuda") for t in leaves]
+        for t, b in zip(leaves, buckets):
+            ops.register_param(t, t.detach().to(torch.bfloat16), b)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            loss = run(ids, labels)
+        grads = torch.autograd.grad(loss, leaves, allow_unused=True)
+        assert all(g is None for g in grads)
+        for b, w in zip(buckets, want):
+            # the bucket's 3.0 takes bits of small gradients; the 16-bit gradient is rounded
+            assert ((b - 3.0).double() - w.double()).abs().le(2.0 ** -8 * w.double().abs() + 2.0 ** -21).all()
+        ops.unregister_params()
+        tied = normal(50, 32, device="cuda", dtype=torch.float32, seed=9, std=0.3).requires_grad_()
+        bucket = torch.zeros_like(tied)
+        low = tied.detach().to(torch.bfloat16)
+        ops.register_param(tied, low, bucket)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            loss = ops.linear_cross_entropy(ops.scaled_embedding(ids, tied, 2.0), tied, labels)
+        torch.autograd.grad(loss, tied, allow_unused=True)
+        ops.unregister_params()
+        low = low.requires_grad_()
+        (w,) = torch.autograd.grad(ops.linear_cross_entropy(ops.scaled_embedding(ids, low, 2.0), low, labels), low)
+        # autograd adds two 16-bit gradients in 16 bits
+        assert (bucket.double() - w.double()).abs().max() <= 2.0 ** -7 * float(w.abs().max())
+    finally:
+        ops.unregister_params()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+def test_autocast_and_full_precision(device, dtype):
+    """fp32 leaves under autocast, or without it in PyTorch's own products."""
+    leaves, run = _all(device, torch.float32)
+    ids, labels = _data(device, 10)
+    with torch.autocast(device, dtype=dtype, enabled=dtype != torch.float32):
+        loss = run(ids, labels)
+    grads = torch.autograd.grad(loss, leaves)
+    wide = [t.detach().double().cpu().requires_grad_() for t in leaves]
+    h = ops.scaled_embedding(ids.cpu(), wide[0], 1.5)
+    h = ops.gated_mlp(h, wide[1], None, wide[2], None, residual=h)
+    want = ops.linear_cross_entropy(h, wide[3], labels.cpu())
+    # some ten roundings lie between a leaf and its gradient; a gradient as a whole is off by no more than they add up to
+    assert abs(float(loss) - float(want)) <= 16 * U[dtype] * float(want) + 2e-6
+    for g, w in zip(grads, torch.autograd.grad(want, wide)):
+        assert g.dtype == torch.float32 and float((g.cpu().double() - w).norm() / w.norm()) <= 16 * U[dtype] + 2e-5
+
+
+def test_shapes_without_data():
+    """What a trace sees: shapes and types of every output, and a gradient through the registered ops."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    leaves, run = _all("cpu", torch.bfloat16)
+    ids, labels = _data("cpu", 10)
+    with FakeTensorMode() as mode:
+        low = [mode.from_tensor(t) for t in leaves]
+        h = ops.scaled_embedding(mode.from_tensor(ids), low[0], 1.5)
+        h = ops.gated_mlp(h, low[1], None, low[2], None, residual=h)
+        loss = ops.linear_cross_entropy(h, low[3], mode.from_tensor(labels))
+        assert h.shape == (70, 32) and loss.shape == () and loss.dtype == torch.float32
+    compiled = torch.compile(run, backend="eager")
+    a, b = run(ids, labels), compiled(ids, labels)
+    assert torch.equal(a, b)
+    for x, y in zip(torch.autograd.grad(a, leaves), torch.autograd.grad(b, leaves)):
+        assert torch.equal(x, y)

@@ -1,0 +1,146 @@
+"""A decoder whose embedding, feed-forward blocks and head with its loss keep less, through the runtimes: stages cut by the
+planner on CPU devices, and mixed precision with registered weights, eager and under CUDA graphs, on one GPU, against
+plain training of the same model and against the model of separate operators."""
+import copy
+import os
+
+import pytest
+import torch
+
+from pfeife_b200 import ops
+from pfeife_b200.loss import LossWrapper
+from pfeife_b200.models.llama import Llama, llama_config, next_tokens
+from pfeife_b200.option import PipeOption
+
+
+def _model(**overrides):
+    torch.manual_seed(0)
+    cfg = llama_config("llama_tiny", **{"embed_scale": 2.0, "fused_mlp": True, **overrides})
+    return Llama(cfg)
+
+
+def _batch(n, T, g):
+    ids = torch.randint(0, 256, (n, T), generator=g)
+    labels = next_tokens(ids)
+    labels[::2, :5] = -100
+    return ids, labels
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("tied", [False, True])
+def test_the_same_model_of_separate_operators(device, tied):
+    model = _model(tie_embeddings=tied).to(device)
+    other = Llama(llama_config("llama_tiny", tie_embeddings=tied)).to(device)
+    other.load_state_dict(model.state_dict())
+    ids, labels = (t.to(device) for t in _batch(3, 24, torch.Generator().manual_seed(1)))
+    with torch.autocast(device, dtype=torch.bfloat16):
+        loss = model(ids, labels)
+        x = ops.embedding(ids, other.embed.weight) * 2.0
+        cos, sin = other.rope_cos[:24], other.rope_sin[:24]
+        delta = None
+        for layer in other.layers:
+            x, delta = layer(x, delta, cos, sin)
+        y, _ = ops.rms_norm(delta, other.norm, other.cfg.rms_eps, residual=x)
+        want = ops.cross_entropy(ops.linear(y, other.lm_head.weight).reshape(-1, 256), labels.reshape(-1))
+    loss.backward()
+    want.backward()
+    # some thirty roundings to 8 bits on the way to a logit and back
+    assert float(loss.detach()) == pytest.approx(float(want.detach()), rel=2e-2)
+    for (name, p), q in zip(model.named_parameters(), other.parameters()):
+        assert float((p.grad - q.grad).norm()) <= 30 * 2.0 ** -8 * float(q.grad.norm()), name
+
+
+def test_logits_and_losses_are_of_one_model():
+    model = _model()
+    ids, labels = _batch(2, 16, torch.Generator().manual_seed(1))
+    logits = model(ids)
+    each = torch.nn.functional.cross_entropy(logits.reshape(-1, 256), labels.reshape(-1))
+    assert float(model(ids, labels).detach()) == pytest.approx(float(each.detach()), abs=1e-6)
+    assert next_tokens(ids)[:, :-1].equal(ids[:, 1:]) and (next_tokens(ids)[:, -1] == -100).all()
+
+
+class Given(LossWrapper):
+    """The model gives the loss."""
+
+    def forward(self, input, target, model=None):
+        return input
+
+
+def test_stages_on_the_cpu():
+    from pfeife_b200.runtime.manager import LocalPipeManager
+    torch._dynamo.reset()
+    model = _model()
+    ref = copy.deepcopy(model)
+    option = PipeOption(device_cnt=2, batch_size=4, batch_cnt=2, cpu_test=True, no_bench_optimizer=True,
+                        verbosity="warning", ctrl_timeout=60, optimizer={"type": "sgd", "lr": 0.05})
+    mgr = LocalPipeManager(model, Given(), option)
+    ropt = torch.optim.SGD(ref.parameters(), lr=0.05)
+    g = torch.Generator().manual_seed(1)
+    try:
+        for _ in range(2):
+            ids, labels = _batch(8, 16, g)
+            losses = mgr.run(labels, ids, labels)
+            ropt.zero_grad()
+            want = []
+            for i, l in zip(ids.chunk(2), labels.chunk(2)):
+                loss = ref(i, l)
+                loss.backward()
+                want.append(float(loss.detach()))
+            ropt.step()
+            assert [float(l) for l in losses] == pytest.approx(want, abs=1e-5)
+        mgr.gather_params()
+        for p, q in zip(model.parameters(), ref.parameters()):
+            assert torch.allclose(p, q, atol=1e-5)
+    finally:
+        mgr.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cuda_graphs", [False, True])
+def test_mixed_precision_on_one_gpu(cuda_graphs):
+    os.environ.setdefault("WORLD_SIZE", "1")
+    os.environ.setdefault("RANK", "0")
+    os.environ.setdefault("MASTER_PORT", "29881")
+    from pfeife_b200 import PartialRunner, initialize_pfeife, partial_compiler
+    from pfeife_b200.ops import kernels as kx
+    dev = initialize_pfeife().device
+    model = _model(num_layers=2).to(dev)
+    ref = copy.deepcopy(model)
+    opt, ropt = (torch.optim.SGD(m.parameters(), lr=0.1) for m in (model, ref))
+    option = PipeOption(device_cnt=1, batch_size=4, batch_cnt=2, mixed_precision="bf16", no_bench_optimizer=True,
+                        cuda_graphs=cuda_graphs, verbosity="warning")
+    runner = PartialRunner(option, opt)
+    torch._dynamo.reset()
+    cm = torch.compile(model, backend=partial_compiler)
+
+    def fn(ids, labels):
+        loss = cm(ids, labels)
+        runner.scaler.scale(loss).backward()
+        return loss.detach()
+
+    runner.set_exec_fn(fn)
+    g = torch.Generator().manual_seed(3)
+    start = [p.detach().clone() for p in ref.parameters()]
+    try:
+        for _ in range(4):
+            ids, labels = (t.to(dev) for t in _batch(8, 16, g))
+            out = runner.step(ids, labels)
+            ropt.zero_grad()
+            for i, (a, b) in enumerate(zip(ids.chunk(2), labels.chunk(2))):
+                loss = ref(a, b)
+                loss.backward()
+                assert float(out[i]) == pytest.approx(float(loss.detach()), rel=1e-2)
+            ropt.step()
+        torch.cuda.synchronize()
+        kx.check_status()
+        runner.gather_params()
+        graphs = len(runner.worker.graphs)
+    finally:
+        runner.close()
+        ops.unregister_params()              # later calls of this process are of plain tensors again
+    assert (graphs > 0) == cuda_graphs
+    for (name, p), q, s in zip(model.named_parameters(), ref.parameters(), start):
+        # the way that a weight went: some 40 roundings of 2^-9 lie between it and its gradient, four steps
+        moved = (q.detach() - s).norm()
+        assert float((p.detach().float() - q.detach()).norm()) <= 0.1 * float(moved) + 1e-6, name
+        assert moved > 0
