@@ -10,7 +10,8 @@ enum Job : int {
   GLU_BWD,      // dh = dy W2, then d(gate), d(up) and h from the kept gate and up
   HEAD_STATS,   // per row and half a tile of z = x W^T: a reference and the sum of 2^(z log2 e - reference)
   HEAD_DZ,      // (softmax(z) - onehot) * factor of some words, in 16 bits
-  HEAD_DX,      // parts of dz W, in fp32
+  PARTS_K,      // parts of A B^T in fp32, B with K innermost: products of few rows, split over their reduction
+  PARTS_N,      // the same, B with N innermost
   HEAD_DW,      // dz^T x
 };
 
@@ -21,7 +22,7 @@ struct FusedCall {
   // product [M, N] over K.  GLU_FWD: N hidden values, each of two columns
   int M = 0, N = 0, K = 0;
   const void* A = nullptr;     // 16-bit; K innermost, but HEAD_DW: M innermost
-  const void* B = nullptr;     // GLU_FWD, HEAD_STATS, HEAD_DZ: K innermost, else N innermost
+  const void* B = nullptr;     // GLU_FWD, HEAD_STATS, HEAD_DZ, PARTS_K: K innermost, else N innermost
   long long lda = 0, ldb = 0;
   const int* rows = nullptr;   // device: how many rows there are (HEAD_DW: what to reduce over); M (K) is the most
   int dtype = 0, out_dtype = 0;
@@ -36,15 +37,15 @@ struct FusedCall {
   // head
   const int* labels = nullptr;
   int first = 0;               // word of the first column
-  RowStat* parts = nullptr;    // [HEAD_PARTS_OF(N)][part_pitch]: reference and sum
+  RowStat* parts = nullptr;    // [N / HEAD_PART][part_pitch]: reference and sum
   long long part_pitch = 0;
   float* picked = nullptr;     // z at the label
   const RowStat* stats = nullptr;
   const float* factor = nullptr;   // of each row; null: `unit` for all
   float unit = 1.f;
-  int split = 1;               // HEAD_DX: parts of the reduction, part i in rows i * part_rows of C on
+  int split = 1;               // PARTS: parts of the reduction, part i in rows i * part_rows of C on
   int part_rows = 0;
-  int accumulate = 0;          // HEAD_DX, HEAD_DW in fp32: add to C
+  int accumulate = 0;          // PARTS, HEAD_DW in fp32: add to C
   const float* scale = nullptr;    // HEAD_DW: *scale times *scale2 (where given) times scale3
   const float* scale2 = nullptr;
   float scale3 = 1.f;
@@ -53,7 +54,7 @@ struct FusedCall {
   cudaStream_t stream = nullptr;
 };
 
-constexpr int HEAD_PART = 64;      // words of a part of HEAD_STATS; a tile of a CTA pair has twice as many in each
+constexpr int HEAD_PART = 64;      // words of a part of HEAD_STATS
 
 // 256 x 256 tiles of CTA pairs instead of 128 x 128 ones
 bool fused_pairs(Job job, long long M, long long N, int sm_count);

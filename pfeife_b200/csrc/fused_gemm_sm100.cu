@@ -21,33 +21,44 @@ namespace pf {
 
 int make_tmap_2d_16bit(CUtensorMap* map, const void* base, int fmt, long long inner, long long outer, long long ld,
                        int box_inner, int box_outer);
-int make_tmap_out(CUtensorMap* map, const void* base, int out_dtype, long long cols, long long rows, long long ld);
+int make_tmap_out(CUtensorMap* map, const void* base, int out_dtype, long long cols, long long rows, long long ld,
+                  int box_cols);
 
 constexpr int FG_BM = 128, FG_BN = 128, FG_BK = 64;      // per CTA and k-block
-constexpr int FG_EPI_WARPS = 8;
-constexpr int FG_THREADS = 64 + 32 * FG_EPI_WARPS;
+// Epilogue warps: a warp has 32 rows and, of a pair's tile, a fourth of its columns, of a single tile's a half.  With half
+// as many, two a scheduler that each wait for their own results, an epilogue shows behind reductions of up to 1280 values.
+constexpr int epi_warps(bool pair) { return pair ? 16 : 8; }
+constexpr int fg_threads(bool pair) { return 64 + 32 * epi_warps(pair); }
 constexpr int FG_STAGE_BYTES = (FG_BM + FG_BN) * FG_BK * 2;
 constexpr int FG_GROUP_ROWS = 4096;                      // see GROUP_ROWS in gemm_sm100.cu
-constexpr int FG_BOX16 = 2048, FG_BOX32 = 4096;          // staged [32 x 32] boxes
+constexpr long long FG_B_STAYS = 48ll << 20;
 
-// Shared memory of a job: stages of operands, barriers, and what each epilogue warp stages its stores in.
-template <int JOB, typename OutT>
+// Shared memory of a job: stages of operands, barriers, and the boxes (32 rows of BW columns) in which an epilogue warp
+// turns its rows of the accumulator into lines of the output.
+template <int JOB, typename OutT, bool PAIR>
 struct FusedSmem {
-  static constexpr int BOX = sizeof(OutT) == 4 ? FG_BOX32 : FG_BOX16;
-  static constexpr int BOXES = JOB == GLU_FWD || JOB == GLU_BWD ? 3 : JOB == HEAD_STATS ? 0 : 1;
-  static constexpr int SETS = BOXES == 1 ? 2 : 1;
-  static constexpr int PER_WARP = SETS * BOXES * BOX;
-  static constexpr int STAGES = BOXES ? 5 : 6;
+  static constexpr int HC = JOB == GLU_FWD ? 32 : 64;               // output columns of a warp
+  static constexpr int BW = sizeof(OutT) == 4 || JOB == GLU_FWD || JOB == GLU_BWD ? 32 : 64;
+  static constexpr int BOX = 32 * BW * sizeof(OutT);
+  static constexpr int BOXES = JOB == GLU_BWD ? 2 : JOB == HEAD_STATS ? 0 : 1;
+  static constexpr int PER_WARP = BOXES * BOX;
+  static constexpr int STAGING = epi_warps(PAIR) * PER_WARP;
+  static constexpr int STAGES = STAGING <= 32768 ? 6 : 5;
   static constexpr int BAR_OFFSET = STAGES * FG_STAGE_BYTES;
   static constexpr int STAGING_OFFSET = BAR_OFFSET + 1024;
-  static constexpr int TOTAL = STAGING_OFFSET + FG_EPI_WARPS * PER_WARP + 1024;
+  static constexpr int TOTAL = STAGING_OFFSET + STAGING + 1024;
   static_assert(TOTAL <= 232448, "more than a CTA may have");
 };
 
-struct FusedMaps { CUtensorMap a, b, b2, c0, c1, c2; };
+struct FusedMaps { CUtensorMap a, b, b2, c; };          // c: of an output that is added to
 
 struct FusedParams {
   int M, N, K, fmt, group_m;
+  void* C;                       // h | h | - | dz | parts | parts | dW
+  void* two;                     // gate and up [M, 2 N], or their gradients
+  long long ldc;
+  int c_rows;                    // rows of C that may be written
+  int a_rows;                    // rows of A that a CTA loads: all of a tile's, or as many as there are
   const int* rows;
   int* status;
   const void* gu;
@@ -78,67 +89,116 @@ __device__ __forceinline__ float ex2(float x) {
 // s + z s (1 - s) q'.  e^-q overflows to infinity for large negative q, where s is 0.  q' is held to |z| <= 1e3, beyond
 // which s (1 - s) is 0 and z^2 may not be finite.
 template <bool SLOPE>
-__device__ __forceinline__ void sigmoid_act(float z, float q, float dq, float& a, float& d) {
-  const float s = rcp_approx(1.f + ex2(-LOG2E * q));
-  a = z * s;
-  if (SLOPE) d = fmaf(a * (1.f - s), dq, s);
+__device__ __forceinline__ void sigmoid_act2(uint64_t z, uint64_t q, uint64_t dq, uint64_t& a, uint64_t& d) {
+  float q0, q1, d0, d1;
+  f2_unpack(mul2(q, f2_pack(-LOG2E, -LOG2E)), q0, q1);
+  f2_unpack(add2(f2_pack(ex2(q0), ex2(q1)), f2_pack(1.f, 1.f)), d0, d1);
+  const uint64_t s = f2_pack(rcp_approx(d0), rcp_approx(d1));
+  a = mul2(z, s);
+  if (SLOPE) d = fma2(fma2(mul2(a, f2_pack(-1.f, -1.f)), s, a), dq, s);      // s + (a - a s) q'
 }
-template <bool SLOPE>
-__device__ __forceinline__ void act2(int act, float z0, float z1, float& a0, float& a1, float& d0, float& d1) {
-  if (act == 1) {                                       // GELU with erf
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void act2(float z0, float z1, uint64_t& a, uint64_t& d) {
+  if constexpr (ACT == 1) {                             // GELU with erf
     uint64_t e;
-    const uint64_t ny = gelu_neg_tail2(f2_pack(fabsf(z0), fabsf(z1)), e);
-    float y0, y1, e0, e1;
-    f2_unpack(ny, y0, y1);
-    a0 = fmaf(fabsf(z0), y0, fmaxf(z0, 0.f));
-    a1 = fmaf(fabsf(z1), y1, fmaxf(z1, 0.f));
+    const uint64_t az = f2_pack(fabsf(z0), fabsf(z1));
+    const uint64_t ny = gelu_neg_tail2(az, e);
+    a = fma2(az, ny, f2_pack(fmaxf(z0, 0.f), fmaxf(z1, 0.f)));
     if (SLOPE) {
-      f2_unpack(e, e0, e1);
-      d0 = fmaf(z0 * 0.3989422804014327f, e0, z0 >= 0.f ? 1.f + y0 : -y0);
-      d1 = fmaf(z1 * 0.3989422804014327f, e1, z1 >= 0.f ? 1.f + y1 : -y1);
+      float y0, y1, c0, c1;
+      f2_unpack(ny, y0, y1);
+      f2_unpack(add2(ny, f2_pack(1.f, 1.f)), c0, c1);
+      d = fma2(mul2(f2_pack(z0, z1), f2_pack(0.3989422804014327f, 0.3989422804014327f)), e,
+               f2_pack(z0 >= 0.f ? c0 : -y0, z1 >= 0.f ? c1 : -y1));
     }
-  } else if (act == 2) {                                // GELU with tanh
+  } else if constexpr (ACT == 2) {                      // GELU with tanh
     constexpr float c = 2.f * 0.7978845608028654f;
-    auto one = [](float z, float& a, float& d) {
-      const float z2 = z * z, zc = fminf(z2, 1e6f);
-      sigmoid_act<SLOPE>(z, c * fmaf(0.044715f * z2, z, z), c * fmaf(3.f * 0.044715f, zc, 1.f), a, d);
-    };
-    one(z0, a0, d0);
-    one(z1, a1, d1);
+    const uint64_t z = f2_pack(z0, z1), z2 = mul2(z, z);
+    const uint64_t q = mul2(mul2(z, f2_pack(c, c)), fma2(z2, f2_pack(0.044715f, 0.044715f), f2_pack(1.f, 1.f)));
+    uint64_t dq = 0;
+    if (SLOPE) {
+      float s0, s1;
+      f2_unpack(z2, s0, s1);
+      dq = fma2(f2_pack(fminf(s0, 1e6f), fminf(s1, 1e6f)), f2_pack(3.f * 0.044715f * c, 3.f * 0.044715f * c),
+                f2_pack(c, c));
+    }
+    sigmoid_act2<SLOPE>(z, q, dq, a, d);
   } else {                                              // SiLU
-    sigmoid_act<SLOPE>(z0, z0, 1.f, a0, d0);
-    sigmoid_act<SLOPE>(z1, z1, 1.f, a1, d1);
+    const uint64_t z = f2_pack(z0, z1);
+    sigmoid_act2<SLOPE>(z, z, f2_pack(1.f, 1.f), a, d);
   }
 }
 
-__device__ __forceinline__ float bias_at(const void* b, int dtype, int i) {
-  if (dtype == PF_F32) return __ldg(reinterpret_cast<const float*>(b) + i);
-  if (dtype == PF_F16) return __half2float(__ldg(reinterpret_cast<const __half*>(b) + i));
-  return __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(b) + i));
+// The values of an accumulator are in registers (tcgen05.wait::ld) and nothing else is handed over with this arrival: a
+// release would first wait for the stores that are on their way to memory, a tenth of a small reduction's time.
+__device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// Row r (32 values) of a [32 x 32] box as a TMA store reads it: 64-byte rows swizzled over 64 bytes (16-bit values),
-// 128-byte rows over 128 (fp32).  No two lanes of a warp meet in a bank.
-template <typename OutT>
-__device__ __forceinline__ void fill_box(uint8_t* box, int r, const float (&v)[32]) {
-  constexpr int PER = 16 / sizeof(OutT), NCH = 32 / PER;
+// W values of a bias, of which n exist
+template <typename B, int W>
+__device__ __forceinline__ void add_bias_of(const B* b, int n, float (&v)[W]) {
+  constexpr int PER = 16 / sizeof(B);
+  if (n >= W && (reinterpret_cast<uintptr_t>(b) & 15) == 0) {
 #pragma unroll
-  for (int c = 0; c < NCH; ++c) {
+    for (int c = 0; c < W / PER; ++c) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(b) + c);
+      const B* e = reinterpret_cast<const B*>(&q);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) v[c * PER + j] += to_f32<B>(e[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      if (j < n) v[j] += to_f32<B>(b[j]);
+  }
+}
+template <int W>
+__device__ __forceinline__ void add_bias(const void* b, int dtype, int i, int n, float (&v)[W]) {
+  if (!b) return;
+  if (dtype == PF_F32) add_bias_of(static_cast<const float*>(b) + i, n, v);
+  else if (dtype == PF_F16) add_bias_of(static_cast<const __half*>(b) + i, n, v);
+  else add_bias_of(static_cast<const __nv_bfloat16*>(b) + i, n, v);
+}
+// see tmem_ld_wait_for in common.cuh
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+        "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+        "+r"(r[14]), "+r"(r[15])
+      :
+      : "memory");
+}
+
+// Where 16 bytes lie in a box as TMA reads it: chunk c of row r, rows of 128 bytes swizzled over 128 or of 64 over 64.
+// The 16-byte accesses of eight lanes, of one row or one chunk, meet no bank twice.
+template <int ROW_BYTES>
+__device__ __forceinline__ uint4* box_at(uint8_t* box, int r, int c) {
+  const int at = ROW_BYTES == 128 ? (c ^ (r & 7)) : (c ^ ((r >> 1) & 3));
+  return reinterpret_cast<uint4*>(box + r * ROW_BYTES + at * 16);
+}
+// 32 columns of a row, from the box's column `c0` on
+template <typename OutT, int ROW_BYTES>
+__device__ __forceinline__ void fill_box(uint8_t* box, int r, int c0, const float (&v)[32]) {
+  constexpr int PER = 16 / sizeof(OutT);
+#pragma unroll
+  for (int c = 0; c < 32 / PER; ++c) {
     uint4 q;
     OutT* e = reinterpret_cast<OutT*>(&q);
 #pragma unroll
     for (int j = 0; j < PER; ++j) e[j] = from_f32<OutT>(v[c * PER + j]);
-    const int at = NCH == 4 ? (c ^ ((r >> 1) & 3)) : (c ^ (r & 7));
-    *reinterpret_cast<uint4*>(box + r * (NCH * 16) + at * 16) = q;
+    *box_at<ROW_BYTES>(box, r, c0 / PER + c) = q;
   }
 }
 
 template <typename T, typename OutT, int JOB, bool PAIR>
-__global__ void __launch_bounds__(FG_THREADS, 1)
+__global__ void __launch_bounds__(fg_threads(PAIR), 1)
 fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
-  using S = FusedSmem<JOB, OutT>;
+  using S = FusedSmem<JOB, OutT, PAIR>;
   constexpr bool A_MN = JOB == HEAD_DW;
-  constexpr bool B_MN = JOB == GLU_BWD || JOB == HEAD_DX || JOB == HEAD_DW;
+  constexpr bool B_MN = JOB == GLU_BWD || JOB == PARTS_N || JOB == HEAD_DW;
+  constexpr bool PARTS = JOB == PARTS_K || JOB == PARTS_N;
   constexpr int BMT = PAIR ? 2 * FG_BM : FG_BM;
   constexpr int BNT = PAIR ? 2 * FG_BN : FG_BN;           // accumulator columns of a tile
   constexpr int NT = JOB == GLU_FWD ? BNT / 2 : BNT;      // output columns of a tile
@@ -166,7 +226,7 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tmem_full[i], 1);
-      mbar_init(&tmem_empty[i], (PAIR ? 2 : 1) * FG_EPI_WARPS);      // lane 0 of every epilogue warp
+      mbar_init(&tmem_empty[i], (PAIR ? 2 : 1) * epi_warps(PAIR));      // lane 0 of every epilogue warp
     }
     mbar_fence_init();
   }
@@ -191,7 +251,7 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
   const int M = p.rows && JOB != HEAD_DW ? count : p.M;
   const int K = p.rows && JOB == HEAD_DW ? count : p.K;
   const int num_m = (M + BMT - 1) / BMT, num_n = (p.N + NT - 1) / NT, num_mn = num_m * num_n;
-  const int split = JOB == HEAD_DX ? p.split : 1;
+  const int split = PARTS ? p.split : 1;
   const int num_items = num_mn * split;
   const int num_kb = (K + FG_BK - 1) / FG_BK;
   // Items are dealt in rounds, every other one in reverse; tiles in bands of group_m rows of tiles, column by column.
@@ -225,7 +285,8 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
           uint8_t* sa = smem + stage * FG_STAGE_BYTES;
           uint8_t* sb = sa + FG_BM * FG_BK * 2;
           const int k0 = kb * FG_BK;
-          if (!PAIR || cta_rank == 0) mbar_expect_tx(&full_bar[stage], (PAIR ? 2 : 1) * FG_STAGE_BYTES);
+          if (!PAIR || cta_rank == 0)
+            mbar_expect_tx(&full_bar[stage], (PAIR ? 2 : 1) * ((A_MN ? FG_BM : p.a_rows) + FG_BN) * FG_BK * 2);
           auto load = [&](uint8_t* to, const CUtensorMap* map, int x, int y) {
             if (PAIR) tma_load_2d_pair(to, map, full_leader + stage * 8, x, y);
             else tma_load_2d(to, map, &full_bar[stage], x, y);
@@ -299,31 +360,68 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
   } else {
     // ------------------------------------------------------------------ epilogue
     const int quad = warp & 3, side = (warp - 2) >> 2;
-    constexpr int HC = NT / 2;                          // output columns of a warp
+    constexpr int HC = S::HC, BW = S::BW, RB = BW * sizeof(OutT);        // columns of a warp, of a box; bytes of a row
+    static_assert(HC * epi_warps(PAIR) == 4 * NT, "the warps share a tile's columns");
     const int c_begin = side * HC, c_end = c_begin + HC;
     uint8_t* boxes = smem + S::STAGING_OFFSET + (warp - 2) * S::PER_WARP;
-    int set = 0, staged = 0, acc = 0;
+    int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    // the boxes about to be filled: stores that last read them are done with them
-    auto free_boxes = [&]() {
-      if (staged >= S::SETS) {
-        if (lane == 0) {
-          if (S::SETS == 2) tma_store_wait_read_but_one();
-          else tma_store_wait_read();
-        }
-        __syncwarp();
+    // A box that the warp has filled, to memory: 16 bytes a lane, whole rows of the box behind one another.  (As TMA
+    // stores the boxes take about 13 bytes a clock of each SM: 262 MB of dW of few rows 72 us.)
+    constexpr int CPR = RB / 16, RPI = 32 / CPR, PER = 16 / sizeof(OutT);      // chunks of a row, rows of an access
+    auto store = [&](uint8_t* box, void* C, long long ldc, int col, int row0, int rows) {
+      __syncwarp();
+      const int r = lane / CPR, c = col + (lane % CPR) * PER;
+      OutT* dst = static_cast<OutT*>(C) + (long long)(row0 + r) * ldc + c;
+      const long long step = RPI * ldc;
+      if (row0 + 32 <= rows && col + BW <= p.N) {
+#pragma unroll
+        for (int i = 0; i < CPR; ++i, dst += step)
+          *reinterpret_cast<uint4*>(dst) = *box_at<RB>(box, i * RPI + r, lane % CPR);
+      } else {
+#pragma unroll
+        for (int i = 0; i < CPR; ++i, dst += step)
+          if (row0 + i * RPI + r < rows && c < p.N)
+            *reinterpret_cast<uint4*>(dst) = *box_at<RB>(box, i * RPI + r, lane % CPR);
       }
-      return boxes + set * (S::BOXES * S::BOX);
-    };
-    auto boxes_sent = [&]() {
-      if (lane == 0) tma_store_commit();
-      if (staged < S::SETS) ++staged;
-      if (S::SETS == 2) set ^= 1;
+      __syncwarp();
     };
     float alpha = 1.f;
     if (JOB == HEAD_DW) alpha = (p.scale ? *p.scale : 1.f) * (p.scale2 ? *p.scale2 : 1.f) * p.scale3;
 
+    // GLU backward: gate and up of one of the warp's two chunks of 32 columns, in boxes whose places their gradients take.
+    // The next is asked for as soon as a chunk has left its boxes, 16 bytes a lane and whole rows of a box behind one
+    // another: a lane that read its own row would touch 32 lines with every load.  (Two sets of boxes, for both chunks, and
+    // three stages of operands: 84 us for 87 over 8192 x 4096 at a reduction of 640, 124 for 115 at 1536, 256 for 228 at
+    // 4096.)
+    auto fetch = [&](int chunk, int round) {
+      if constexpr (JOB == GLU_BWD) {
+        const int item = item_of(round);
+        if (item < num_items) {
+          int mt, nt, kb0, kb1;
+          place(item, mt, nt, kb0, kb1);
+          const int row0 = mt * BMT + int(cta_rank) * FG_BM + quad * 32;
+          const int c = nt * NT + c_begin + 32 * chunk + (lane % CPR) * 8;
+          uint8_t* box = boxes;
+#pragma unroll
+          for (int i = 0; i < CPR; ++i) {
+            const int r = i * RPI + lane / CPR;
+            uint4 *g = box_at<RB>(box, r, lane % CPR), *u = box_at<RB>(box + S::BOX, r, lane % CPR);
+            if (row0 + r < M && c < p.N) {              // N is a multiple of 8
+              const T* at = reinterpret_cast<const T*>(p.gu) + (long long)(row0 + r) * 2 * p.N + c;
+              cp_async16(g, at);
+              cp_async16(u, at + p.N);
+            } else {
+              *g = *u = make_uint4(0, 0, 0, 0);
+            }
+          }
+        }
+        cp_async_commit();
+      }
+    };
+    auto fetch_next = [&](int c, int round) { fetch(c == c_begin, c == c_begin ? round : round + 1); };
+    fetch(0, 0);
     for (int round = 0, item = item_of(0); item < num_items && ok; item = item_of(++round)) {
       int mt, nt, kb0, kb1;
       const int ks = place(item, mt, nt, kb0, kb1);
@@ -331,20 +429,6 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
       const int n0 = nt * NT;
       const bool row_ok = row < M;
 
-      // what the epilogue reads travels while the products are computed
-      [[maybe_unused]] uint4 kept[8];
-      auto fetch = [&](int col) {
-        if constexpr (JOB == GLU_BWD) {
-          const T* g = reinterpret_cast<const T*>(p.gu) + (long long)row * 2 * p.N + col;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool there = row_ok && col + 8 * i < p.N;              // N is a multiple of 8
-            kept[i] = there ? __ldg(reinterpret_cast<const uint4*>(g) + i) : make_uint4(0, 0, 0, 0);
-            kept[4 + i] = there ? __ldg(reinterpret_cast<const uint4*>(g + p.N) + i) : make_uint4(0, 0, 0, 0);
-          }
-        }
-      };
-      fetch(n0 + c_begin);
       [[maybe_unused]] int label = -1;                  // as a column of this product
       [[maybe_unused]] float ref = 0.f, inv = 0.f, factor = 0.f, total = 0.f;
       if constexpr (JOB == HEAD_STATS || JOB == HEAD_DZ) {
@@ -365,174 +449,223 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
         tc_fence_after();
       }
       const uint32_t t_row = tmem_base + (uint32_t(quad * 32) << 16) + acc * BNT;
+      // the accumulator may be written again: called once its last columns are in registers
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) arrive_relaxed(mapa_u32(&tmem_empty[acc], 0));
+          else mbar_arrive(&tmem_empty[acc]);
+        }
+      };
+      const int last = min(c_end, (p.N - n0 + 31) / 32 * 32) - 32;      // first of the last 32 columns there are
+      if (!empty && last < c_begin) release();          // none: the whole warp is behind the last column
+      auto values = [&](const uint32_t (&raw)[32], float (&v)[32]) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
+      };
 #pragma unroll 1
-      for (int c = c_begin; c < c_end; c += 32) {
+      for (int c = c_begin; c < c_end; c += BW) {
         const int col = n0 + c;
-        if (col >= p.N) break;                          // uniform across the warp
+        if (col >= p.N) {                               // uniform across the warp
+          if (JOB == GLU_BWD) fetch_next(c, round);
+          continue;
+        }
         uint32_t raw[32];
         float v[32];
-        if (!empty) {
-          tmem_ld32(t_row + c, raw);
-          if constexpr (JOB == GLU_FWD) {
-            uint32_t raw_up[32];
-            float u[32], h[32];
-            tmem_ld32(t_row + NT + c, raw_up);
-            tmem_ld_wait_for(raw);
-            tmem_ld_wait_for(raw_up);
+        if constexpr (JOB == GLU_FWD) {
+          // to be kept: gate, then up, as they are; registers hold no more than 32 columns of both at a time
+          if (p.save) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              v[i] = __uint_as_float(raw[i]);
-              u[i] = __uint_as_float(raw_up[i]);
+            for (int half = 0; half < 2; ++half) {
+              tmem_ld32(t_row + half * NT + c, raw);
+              tmem_ld_wait_for(raw);
+              values(raw, v);
+              add_bias(p.bias, p.bias_dtype, half * p.N + col, p.N - col, v);
+              fill_box<OutT, RB>(boxes, lane, 0, v);
+              store(boxes, static_cast<OutT*>(p.two) + half * p.N, 2ll * p.N, col, row0, M);
             }
-            if (p.bias) {
+          }
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (col + i < p.N) {
-                  v[i] += bias_at(p.bias, p.bias_dtype, col + i);
-                  u[i] += bias_at(p.bias, p.bias_dtype, p.N + col + i);
-                }
+          for (int s = 0; s < 32; s += 16) {
+            uint32_t gate[16], up[16];
+            float g[16], u[16];
+            tmem_ld16(t_row + c + s, gate);
+            tmem_ld16(t_row + NT + c + s, up);
+            tmem_ld_wait_for(gate);
+            tmem_ld_wait_for(up);
+            if (s) release();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              g[i] = __uint_as_float(gate[i]);
+              u[i] = __uint_as_float(up[i]);
             }
-            uint8_t* box = free_boxes();
-            if (p.save) {
-              fill_box<OutT>(box + FG_BOX16, lane, v);
-              fill_box<OutT>(box + 2 * FG_BOX16, lane, u);
-            }
-            float none;
+            add_bias(p.bias, p.bias_dtype, col + s, p.N - col - s, g);
+            add_bias(p.bias, p.bias_dtype, p.N + col + s, p.N - col - s, u);
             auto all = [&](auto kind) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                act2<false>(kind, v[i], v[i + 1], h[i], h[i + 1], none, none);
-                h[i] *= u[i];
-                h[i + 1] *= u[i + 1];
+              for (int i = 0; i < 16; i += 2) {
+                uint64_t a, none;
+                act2<decltype(kind)::value, false>(g[i], g[i + 1], a, none);
+                f2_unpack(mul2(a, f2_pack(u[i], u[i + 1])), g[i], g[i + 1]);
               }
             };
             if (p.act == 1) all(std::integral_constant<int, 1>());
             else if (p.act == 2) all(std::integral_constant<int, 2>());
             else all(std::integral_constant<int, 3>());
-            fill_box<OutT>(box, lane, h);
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0 && row0 < M) {                // rows and columns that do not exist are clipped
-              tma_store_2d(&maps.c0, box, col, row0);
-              if (p.save) {
-                tma_store_2d(&maps.c1, box + FG_BOX16, col, row0);
-                tma_store_2d(&maps.c2, box + 2 * FG_BOX16, col, row0);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              uint4 q;
+              OutT* e = reinterpret_cast<OutT*>(&q);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) e[j] = from_f32<OutT>(g[8 * k + j]);
+              *box_at<RB>(boxes, lane, s / 8 + k) = q;
+            }
+          }
+          store(boxes, p.C, p.ldc, col, row0, M);
+        } else if constexpr (JOB == GLU_BWD) {
+          uint8_t *gbox = boxes, *ubox = boxes + S::BOX;
+          uint4 hq[BW / 8];                             // h, which takes the place of d(gate) once that is stored
+          cp_async_wait<0>();
+          __syncwarp();
+#pragma unroll
+          for (int s = 0; s < BW; s += 16) {
+            uint32_t part[16];
+            tmem_ld16(t_row + c + s, part);
+            tmem_ld_wait_for(part);
+            if (c + s == last + 16) release();
+            auto all = [&](auto kind) {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                uint4 *gp = box_at<RB>(gbox, lane, s / 8 + k), *up = box_at<RB>(ubox, lane, s / 8 + k);
+                uint4 g4 = *gp, u4 = *up;
+                T *g = reinterpret_cast<T*>(&g4), *u = reinterpret_cast<T*>(&u4), *h = reinterpret_cast<T*>(&hq[s / 8 + k]);
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                  const uint64_t dh = f2_pack(__uint_as_float(part[8 * k + j]), __uint_as_float(part[8 * k + j + 1]));
+                  const uint64_t uu = f2_pack(to_f32<T>(u[j]), to_f32<T>(u[j + 1]));
+                  uint64_t a, slope;
+                  act2<decltype(kind)::value, true>(to_f32<T>(g[j]), to_f32<T>(g[j + 1]), a, slope);
+                  float x0, x1;
+                  f2_unpack(mul2(mul2(dh, uu), slope), x0, x1);        // d(gate) = dh up act'(gate)
+                  g[j] = from_f32<T>(x0);
+                  g[j + 1] = from_f32<T>(x1);
+                  f2_unpack(mul2(a, uu), x0, x1);
+                  h[j] = from_f32<T>(x0);
+                  h[j + 1] = from_f32<T>(x1);
+                  f2_unpack(mul2(dh, a), x0, x1);                      // d(up) = dh act(gate)
+                  u[j] = from_f32<T>(x0);
+                  u[j + 1] = from_f32<T>(x1);
+                }
+                *gp = g4;
+                *up = u4;
               }
-            }
-            boxes_sent();
-            continue;
-          } else {
+            };
+            if (p.act == 1) all(std::integral_constant<int, 1>());
+            else if (p.act == 2) all(std::integral_constant<int, 2>());
+            else all(std::integral_constant<int, 3>());
+          }
+          store(gbox, p.two, 2ll * p.N, col, row0, M);
+          store(ubox, static_cast<OutT*>(p.two) + p.N, 2ll * p.N, col, row0, M);
+#pragma unroll
+          for (int k = 0; k < BW / 8; ++k) *box_at<RB>(gbox, lane, k) = hq[k];
+          store(gbox, p.C, p.ldc, col, row0, M);
+          fetch_next(c, round);
+        } else if constexpr (JOB == HEAD_STATS) {
+#pragma unroll
+          for (int s = 0; s < BW; s += 32) {
+            const int at = col + s, nvalid = p.N - at;
+            if (s && nvalid <= 0) break;
+            tmem_ld32(t_row + c + s, raw);
             tmem_ld_wait_for(raw);
+            if (c + s == last) release();
+            values(raw, v);
+            if (nvalid < 32) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0.f;
-        }
-
-        if constexpr (JOB == GLU_BWD) {
-          float g[32], u[32];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const T* eg = reinterpret_cast<const T*>(&kept[i]);
-            const T* eu = reinterpret_cast<const T*>(&kept[4 + i]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              g[i * 8 + j] = to_f32<T>(eg[j]);
-              u[i * 8 + j] = to_f32<T>(eu[j]);
+              for (int i = 0; i < 32; ++i)
+                if (i >= nvalid) v[i] = -INFINITY;
             }
-          }
-          if (c + 32 < c_end) fetch(col + 32);
-          // v: dh -> d(up) = dh act(gate); u: up -> h = act(gate) up; g: gate -> d(gate) = dh up act'(gate)
-          auto all = [&](auto kind) {
+            if ((unsigned)(label - at) < 32u) {
+              float z = 0.f;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (i == label - at) z = v[i];
+              p.picked[row] = z;
+            }
+            // a NaN does not move the maximum but reaches the sum; a part that is -inf so far subtracts 0
+            float top = v[0];
+#pragma unroll
+            for (int i = 1; i < 32; ++i) top = fmaxf(top, v[i]);
+            const float now = fmaxf(ref, ceilf(top * LOG2E)), sub = now == -INFINITY ? 0.f : now;
+            total *= ex2(ref - sub);
+            uint64_t sum = 0;
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              float a0, a1, d0, d1;
-              act2<true>(kind, g[i], g[i + 1], a0, a1, d0, d1);
-              g[i] = v[i] * u[i] * d0;
-              g[i + 1] = v[i + 1] * u[i + 1] * d1;
-              v[i] *= a0;
-              v[i + 1] *= a1;
-              u[i] *= a0;
-              u[i + 1] *= a1;
+              float e0, e1;
+              f2_unpack(fma2(f2_pack(v[i], v[i + 1]), f2_pack(LOG2E, LOG2E), f2_pack(-sub, -sub)), e0, e1);
+              sum = add2(sum, f2_pack(ex2(e0), ex2(e1)));
             }
-          };
-          if (p.act == 1) all(std::integral_constant<int, 1>());
-          else if (p.act == 2) all(std::integral_constant<int, 2>());
-          else all(std::integral_constant<int, 3>());
-          uint8_t* box = free_boxes();
-          fill_box<OutT>(box, lane, u);
-          fill_box<OutT>(box + FG_BOX16, lane, g);
-          fill_box<OutT>(box + 2 * FG_BOX16, lane, v);
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0 && row0 < M) {
-            tma_store_2d(&maps.c0, box, col, row0);
-            tma_store_2d(&maps.c1, box + FG_BOX16, col, row0);
-            tma_store_2d(&maps.c2, box + 2 * FG_BOX16, col, row0);
+            float s0, s1;
+            f2_unpack(sum, s0, s1);
+            total += s0 + s1;
+            ref = now;
           }
-          boxes_sent();
-        } else if constexpr (JOB == HEAD_STATS) {
-          const int nvalid = p.N - col;
-          if (nvalid < 32) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i >= nvalid) v[i] = -INFINITY;
-          }
-          if ((unsigned)(label - col) < 32u) {
-            float z = 0.f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i == label - col) z = v[i];
-            p.picked[row] = z;
-          }
-          // a NaN does not move the maximum but reaches the sum; a part that is -inf so far subtracts 0
-          float top = v[0];
-#pragma unroll
-          for (int i = 1; i < 32; ++i) top = fmaxf(top, v[i]);
-          const float now = fmaxf(ref, ceilf(top * LOG2E)), sub = now == -INFINITY ? 0.f : now;
-          total *= ex2(ref - sub);
-          float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            s0 += ex2(fmaf(v[i], LOG2E, -sub));
-            s1 += ex2(fmaf(v[i + 1], LOG2E, -sub));
-          }
-          total += s0 + s1;
-          ref = now;
-        } else if constexpr (JOB == HEAD_DZ) {
-          // rows behind the last have neither a sum nor a factor: their gradients are zeros, which the reduction
-          // over rows may read
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float pr = ex2(fmaf(v[i], LOG2E, -ref)) * inv;
-            v[i] = (pr - (i == label - col ? 1.f : 0.f)) * factor;
-          }
-          if (!row_ok) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.f;
-          }
-          uint8_t* box = free_boxes();
-          fill_box<OutT>(box, lane, v);
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) tma_store_2d(&maps.c0, box, col, row0);
-          boxes_sent();
         } else {
-          if (JOB == HEAD_DW) {
+          if (sizeof(OutT) == 4 && p.accumulate) {      // the last box is read before it is filled again
+            if (lane == 0) tma_store_wait_read();
+            __syncwarp();
+          }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = empty ? 0.f : v[i] * alpha;
+          for (int s = 0; s < BW; s += 32) {
+            if (s && col + s >= p.N) break;
+            if (!empty) {
+              tmem_ld32(t_row + c + s, raw);
+              tmem_ld_wait_for(raw);
+              if (c + s == last) release();
+              values(raw, v);
+            }
+            if (JOB == HEAD_DZ) {
+              // (p - onehot) factor; rows behind the last have zeros, which the reduction over rows may read
+              const uint64_t times = f2_pack(inv * factor, inv * factor);
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float e0, e1;
+                f2_unpack(fma2(f2_pack(v[i], v[i + 1]), f2_pack(LOG2E, LOG2E), f2_pack(-ref, -ref)), e0, e1);
+                f2_unpack(mul2(f2_pack(ex2(e0), ex2(e1)), times), v[i], v[i + 1]);
+              }
+              const int at = label - col - s;
+              if ((unsigned)at < 32u) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (i == at) v[i] -= factor;
+              }
+              if (row0 + 32 > M && !row_ok) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = 0.f;
+              }
+            } else if (JOB == HEAD_DW) {
+              if (empty) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = 0.f;
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 2)
+                  f2_unpack(mul2(f2_pack(v[i], v[i + 1]), f2_pack(alpha, alpha)), v[i], v[i + 1]);
+              }
+            }
+            fill_box<OutT, RB>(boxes, lane, s, v);
           }
-          uint8_t* box = free_boxes();
-          fill_box<OutT>(box, lane, v);
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0 && row0 < M) {
-            if (sizeof(OutT) == 4 && p.accumulate) tma_reduce_add_2d(&maps.c0, box, col, row0);
-            else tma_store_2d(&maps.c0, box, col, row0 + ks * p.part_rows);
+          if (sizeof(OutT) == 4 && p.accumulate) {      // rows and columns that do not exist are clipped
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (row0 < M) tma_reduce_add_2d(&maps.c, boxes, col, row0);
+              tma_store_commit();
+            }
+          } else {
+            const int part = PARTS ? ks * p.part_rows : 0;
+            store(boxes, p.C, p.ldc, col, row0 + part, JOB == HEAD_DZ ? p.c_rows : M + part);
           }
-          boxes_sent();
         }
       }
       if constexpr (JOB == HEAD_STATS) {
@@ -540,17 +673,11 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
         if (row_ok && n0 + c_begin < p.N) p.parts[part * p.part_pitch + row] = {ref, total};
       }
       if (!empty) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (PAIR) mbar_arrive_cluster(mapa_u32(&tmem_empty[acc], 0));
-          else mbar_arrive(&tmem_empty[acc]);
-        }
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
     }
-    if (lane == 0 && S::BOXES) tma_store_wait_all();
+    if (lane == 0 && p.accumulate) tma_store_wait_all();
   }
 
   // every role reaches this point: all waits are bounded
@@ -567,7 +694,7 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
 // ------------------------------------------------------------------------------- host side
 template <typename T, typename OutT, int JOB, bool PAIR>
 static int launch_fused(const FusedMaps& maps, const FusedParams& p, int sm_count, cudaStream_t stream) {
-  using S = FusedSmem<JOB, OutT>;
+  using S = FusedSmem<JOB, OutT, PAIR>;
   auto kern = fused_gemm_kernel<T, OutT, JOB, PAIR>;
   static bool configured[64] = {};
   static int resident_pairs[64] = {};
@@ -583,7 +710,7 @@ static int launch_fused(const FusedMaps& maps, const FusedParams& p, int sm_coun
   const long long items = (long long)((p.M + BMT - 1) / BMT) * ((p.N + NT - 1) / NT) * p.split;
   if (items > 0x7fffffffll) return -3;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(FG_THREADS);
+  cfg.blockDim = dim3(fg_threads(PAIR));
   cfg.dynamicSmemBytes = S::TOTAL;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -635,7 +762,8 @@ static int fused_by_job(Job job, const FusedMaps& maps, const FusedParams& p, bo
     case GLU_BWD: return fused_by_tile<T, T, GLU_BWD>(maps, p, pair, c);
     case HEAD_STATS: return fused_by_tile<T, T, HEAD_STATS>(maps, p, pair, c);
     case HEAD_DZ: return fused_by_tile<T, T, HEAD_DZ>(maps, p, pair, c);
-    case HEAD_DX: return fused_by_tile<T, float, HEAD_DX>(maps, p, pair, c);
+    case PARTS_K: return fused_by_tile<T, float, PARTS_K>(maps, p, pair, c);
+    case PARTS_N: return fused_by_tile<T, float, PARTS_N>(maps, p, pair, c);
     case HEAD_DW:
       if (c.out_dtype == PF_F32) return fused_by_tile<T, float, HEAD_DW>(maps, p, pair, c);
       return fused_by_tile<T, T, HEAD_DW>(maps, p, pair, c);
@@ -646,51 +774,46 @@ static int fused_by_job(Job job, const FusedMaps& maps, const FusedParams& p, bo
 int fused_gemm(Job job, const FusedCall& c) {
   if (c.M <= 0 || c.N <= 0) return 0;
   if (c.dtype != PF_F16 && c.dtype != PF_BF16) return -1;
-  if (c.lda % 8 || c.ldb % 8 || !on_vectors(c.A, c.B, c.C, c.gu, c.dgu)) return -2;
+  if (c.lda % 8 || c.ldb % 8 || c.ldc % 8 || c.N % 8 && job != HEAD_STATS && job != HEAD_DZ ||
+      !on_vectors(c.A, c.B, c.C, c.gu, c.dgu))
+    return -2;
   const int fmt = c.dtype == PF_BF16;
   const bool pair = fused_pairs(job, c.M, c.N, c.sm_count);
+  // Fewer rows than a tile has are loaded as what they are: rows of accumulators that no row of A fills are not read.
+  const int a_rows = pair || c.M >= FG_BM ? FG_BM : (c.M + 7) / 8 * 8;
   FusedMaps maps;
   memset(&maps, 0, sizeof(maps));
   int r;
   const char* B = static_cast<const char*>(c.B);
   if (job == HEAD_DW) r = make_tmap_2d_16bit(&maps.a, c.A, fmt, c.M, c.K, c.lda, 64, FG_BK);
-  else r = make_tmap_2d_16bit(&maps.a, c.A, fmt, c.K, c.M, c.lda, FG_BK, FG_BM);
+  else r = make_tmap_2d_16bit(&maps.a, c.A, fmt, c.K, c.M, c.lda, FG_BK, a_rows);
   if (r) return r;
   if (job == GLU_FWD) {
     const int rows = pair ? FG_BN : FG_BN / 2;
     if ((r = make_tmap_2d_16bit(&maps.b, B, fmt, c.K, c.N, c.ldb, FG_BK, rows)) ||
         (r = make_tmap_2d_16bit(&maps.b2, B + c.ldb * 2 * c.N, fmt, c.K, c.N, c.ldb, FG_BK, rows)))
       return r;
-  } else if (job == HEAD_STATS || job == HEAD_DZ) {
+  } else if (job == HEAD_STATS || job == HEAD_DZ || job == PARTS_K) {
     if ((r = make_tmap_2d_16bit(&maps.b, B, fmt, c.K, c.N, c.ldb, FG_BK, FG_BN))) return r;
   } else {
     if ((r = make_tmap_2d_16bit(&maps.b, B, fmt, c.N, c.K, c.ldb, 64, FG_BK))) return r;
   }
-  if (job == GLU_FWD || job == GLU_BWD) {
-    char* two = static_cast<char*>(job == GLU_FWD ? c.gu : c.dgu);
-    if ((r = make_tmap_out(&maps.c0, c.C, c.dtype, c.N, c.M, c.ldc))) return r;
-    if (two && ((r = make_tmap_out(&maps.c1, two, c.dtype, c.N, c.M, 2ll * c.N)) ||
-                (r = make_tmap_out(&maps.c2, two + 2ll * c.N, c.dtype, c.N, c.M, 2ll * c.N))))
-      return r;
-  } else if (job == HEAD_DZ) {
-    // rows up to the end of the last tile are written
-    const int rows = (c.M + 2 * FG_BM - 1) / (2 * FG_BM) * (2 * FG_BM);
-    if ((r = make_tmap_out(&maps.c0, c.C, c.dtype, c.N, rows, c.ldc))) return r;
-  } else if (job == HEAD_DX) {
-    const long long rows = c.split > 1 ? (long long)c.split * c.part_rows : c.M;
-    if ((r = make_tmap_out(&maps.c0, c.C, PF_F32, c.N, rows, c.ldc))) return r;
-  } else if (job == HEAD_DW) {
-    if ((r = make_tmap_out(&maps.c0, c.C, c.out_dtype, c.N, c.M, c.ldc))) return r;
-  }
+  if (c.accumulate && (r = make_tmap_out(&maps.c, c.C, PF_F32, c.N, c.M, c.ldc, 32))) return r;
   FusedParams p;
   memset(&p, 0, sizeof(p));
   p.M = c.M; p.N = c.N; p.K = c.K; p.fmt = fmt;
   p.group_m = FG_GROUP_ROWS / (pair ? 2 * FG_BM : FG_BM);
+  // Where all of B stays in L2, the tiles in flight are whole rows of the output instead, which DRAM takes better.
+  const int bt = pair ? 2 * FG_BM : FG_BM, nt = job == GLU_FWD ? bt / 2 : bt;
+  const int columns = (c.N + nt - 1) / nt, workers = pair ? c.sm_count / 2 : c.sm_count;
+  if ((long long)c.N * c.K * (job == GLU_FWD ? 4 : 2) <= FG_B_STAYS) p.group_m = (workers + columns - 1) / columns;
   p.rows = c.rows; p.status = c.status;
   p.gu = c.gu; p.bias = c.bias; p.bias_dtype = c.bias_dtype; p.act = c.act; p.save = job == GLU_FWD && c.gu;
   p.labels = c.labels; p.parts = c.parts; p.part_pitch = c.part_pitch; p.picked = c.picked; p.stats = c.stats;
   p.factor = c.factor; p.unit = c.unit;
-  p.first = c.first; p.split = job == HEAD_DX ? c.split : 1; p.part_rows = c.part_rows; p.accumulate = c.accumulate;
+  p.a_rows = a_rows;
+  p.C = c.C; p.ldc = c.ldc; p.two = job == GLU_FWD ? c.gu : c.dgu; p.c_rows = (c.M + 255) / 256 * 256;
+  p.first = c.first; p.split = job == PARTS_K || job == PARTS_N ? c.split : 1; p.part_rows = c.part_rows; p.accumulate = c.accumulate;
   p.scale = c.scale; p.scale2 = c.scale2; p.scale3 = c.scale3;
   return c.dtype == PF_F16 ? fused_by_job<__half>(job, maps, p, pair, c)
                            : fused_by_job<__nv_bfloat16>(job, maps, p, pair, c);

@@ -309,7 +309,7 @@ PF_API int pf_head_parts(long long N, long long V, int D, int sm_count) {
   if (sm_count <= 0) sm_count = 148;
   const long long words = pf_head_words(N, V);
   if (words < V) return 1;
-  const bool pair = fused_pairs(HEAD_DX, N, D, sm_count);
+  const bool pair = fused_pairs(PARTS_N, N, D, sm_count);
   const long long bt = pair ? 256 : 128, tiles = ((N + bt - 1) / bt) * ((D + bt - 1) / bt);
   const long long slots = pair ? sm_count / 2 : sm_count, kb = (V + 63) / 64;
   int parts = 1;
@@ -330,9 +330,7 @@ PF_API int pf_head_fwd(const void* x, const void* w, const void* target, void* x
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const long long Mp = padded_rows(N);
   const HeadIndex ix = head_index(static_cast<int*>(index), N);
-  const bool pair = fused_pairs(HEAD_STATS, N, V, sm_count);
-  const int width = pair ? 2 * HEAD_PART : HEAD_PART;
-  const int n_parts = (int)((V + width - 1) / width);
+  const int n_parts = (int)((V + HEAD_PART - 1) / HEAD_PART);
   RowStat* parts = static_cast<RowStat*>(scratch);
   double* sums = reinterpret_cast<double*>(parts + n_parts * Mp);
   float* picked = reinterpret_cast<float*>(sums + Mp / 32);
@@ -410,7 +408,7 @@ PF_API int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const
       FusedCall c = base;
       c.M = (int)N; c.N = Dp; c.K = n; c.A = dz; c.B = wp; c.lda = words; c.ldb = ldw; c.C = acc; c.ldc = Dp;
       c.out_dtype = PF_F32; c.split = parts; c.part_rows = (int)Mp; c.accumulate = v0 > 0;
-      if ((r = fused_gemm(HEAD_DX, c))) return r;
+      if ((r = fused_gemm(PARTS_N, c))) return r;
     }
     if (dw) {
       FusedCall c = base;
