@@ -25,13 +25,17 @@ PF_DECL int pf_gemm(const void* A, const void* B, void* C, int M, int N, int K, 
 PF_DECL int pf_gemm_workspace(int M, int N, int K, int accumulate, int conv, int sm_count,
                               int tile_n);
 
-// ---- fused_gemm_sm100.cu
-PF_DECL int pf_glu_linear_fwd(const void* x, const void* w, const void* bias, int bias_dtype, void* h, void* gu, int M,
-                              int H, int K, long long ldx, long long ldw, int act, int dtype, int* status, int sm_count,
-                              void* stream);
-PF_DECL int pf_glu_linear_bwd(const void* dy, const void* w2, const void* gu, void* dgu, void* h, int M, int H, int K,
-                              long long lddy, long long ldw2, int act, int dtype, int* status, int sm_count,
-                              void* stream);
+// ---- gated_mlp.cu
+PF_DECL int pf_gated_mlp_scratch(int M, int D, int H, int N, int sm_count);
+PF_DECL int pf_gated_mlp_fwd(const void* x, const void* w1, const void* b1, int b1_dtype, const void* w2,
+                             const void* b2, int b2_dtype, const void* residual, void* h, void* gu, void* y, void* ws,
+                             int ws_kib, int M, int D, int H, int N, long long ldx, long long ldw1, long long ldw2,
+                             long long ldr, int act, int dtype, int* status, int sm_count, void* stream);
+PF_DECL int pf_gated_mlp_bwd(const void* dy, const void* x, const void* w1, const void* w2, const void* gu, void* dgu,
+                             void* h, void* dx, void* dw1, void* dw2, void* db1, void* db2, void* ws, int ws_kib, int M,
+                             int D, int H, int N, long long lddy, long long ldx, long long ldw1, long long ldw2,
+                             int act, int dtype, int dw1_dtype, int dw2_dtype, int add1, int add2, int* status,
+                             int sm_count, void* stream);
 
 // ---- head_loss.cu
 PF_DECL int pf_head_index(long long N);

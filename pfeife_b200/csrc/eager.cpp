@@ -1147,6 +1147,246 @@ struct DirectConv2d : torch::autograd::Function<DirectConv2d> {
   }
 };
 
+// ------------------------------------------------------------------------------ gated feed-forward block
+// 3 activations of gated_mlp.cu; weights [2H, D] and [N, H] of whole vectors
+bool gated_fits(const Tensor& x, const Tensor& w1, const Tensor& w2) {
+  return layer_fits(x, w1, {}) && w2.scalar_type() == x.scalar_type() && readable(w2) && w1.size(0) == 2 * w2.size(1) &&
+         w2.size(1) > 0 && w2.size(1) % 8 == 0 && w2.size(0) > 0 && w2.size(0) % 8 == 0 && w2.size(0) < (1ll << 31);
+}
+struct GatedSizes {
+  int M, D, H, N;
+  GatedSizes(const Tensor& x2, const Tensor& w2)
+      : M((int)x2.size(0)), D((int)x2.size(1)), H((int)w2.size(1)), N((int)w2.size(0)) {}
+};
+Tensor gated_workspace(const GatedSizes& g, const Env& e, const Tensor& like, int& kib) {
+  kib = pf_gated_mlp_scratch(g.M, g.D, g.H, g.N, e.sms);
+  return kib ? floats(kib * 256ll, like) : Tensor();
+}
+std::pair<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& w1, const Tensor& b1, const Tensor& w2,
+                                        const Tensor& b2, const Tensor& res, int act, bool keep) {
+  const Env e(x);
+  const Tensor x2 = rows(x), r2 = res.defined() ? rows(res) : Tensor();
+  const GatedSizes g(x2, w2);
+  const Tensor h = empty({g.M, g.H}, x), gu = keep ? empty({g.M, 2 * g.H}, x) : Tensor(), y = empty({g.M, g.N}, x);
+  int kib;
+  const Tensor ws = gated_workspace(g, e, x, kib);
+  ok(pf_gated_mlp_fwd(x2.data_ptr(), w1.data_ptr(), at_or_null(b1), b1.defined() ? code_of(b1) : 0, w2.data_ptr(),
+                      at_or_null(b2), b2.defined() ? code_of(b2) : 0, at_or_null(r2), h.data_ptr(),
+                      const_cast<void*>(at_or_null(gu)), y.data_ptr(), const_cast<void*>(at_or_null(ws)), kib, g.M, g.D,
+                      g.H, g.N, x2.stride(0), w1.stride(0), w2.stride(0), r2.defined() ? r2.stride(0) : 0, act,
+                      code_of(x), e.status, e.sms, e.stream),
+     "pf_gated_mlp_fwd");
+  return {y.view(with_last(x, g.N)), keep ? gu.view(with_last(x, 2 * g.H)) : gu};
+}
+
+struct DirectGatedMlp : torch::autograd::Function<DirectGatedMlp> {
+  static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w1, Maybe bias1, Tensor w2, Maybe bias2,
+                        Maybe residual, int64_t act) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const Tensor b1 = value(bias1), b2 = value(bias2), res = value(residual);
+    // gate and up are for any gradient but the residual's
+    bool keep = x.requires_grad() || w1.requires_grad() || w2.requires_grad();
+    for (const Tensor* t : {&b1, &b2}) keep = keep || (t->defined() && t->requires_grad());
+    auto [y, gu] = gated_forward(x, w1, b1, w2, b2, res, (int)act, keep);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, w1, w2, gu, b1, b2});
+    ctx->saved_data["act"] = act;
+    if (bias1) ctx->saved_data["type1"] = (int64_t)b1.scalar_type();
+    if (bias2) ctx->saved_data["type2"] = (int64_t)b2.scalar_type();
+    ctx->saved_data["res"] = res.defined();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &w1 = s[1], &w2 = s[2], &gu = s[3], &b1 = s[4], &b2 = s[5];
+    if (!grads[0].defined()) return variable_list(7);
+    const Tensor dy = grads[0].contiguous();
+    const int act = (int)ctx->saved_data["act"].toInt();
+    const int i1 = 2, i2 = i1 + b1.defined(), i3 = i2 + 1, ir = i3 + b2.defined();     // inputs that were given
+    const bool nx = ctx->needs_input_grad(0), nw1 = ctx->needs_input_grad(1),
+               nb1 = b1.defined() && ctx->needs_input_grad(i1), nw2 = ctx->needs_input_grad(i2),
+               nb2 = b2.defined() && ctx->needs_input_grad(i3),
+               nr = ctx->saved_data["res"].toBool() && ctx->needs_input_grad(ir);
+    Tensor dx, dw1, db1, dw2, db2;
+    if (!(nx || nw1 || nb1 || nw2 || nb2)) {
+      // the residual's alone
+    } else if (gu.defined() && direct(dy, x, w1, w2, gu, b1, b2) && gated_fits(x, w1, w2) &&
+               dy.scalar_type() == x.scalar_type() && dy.size(-1) == w2.size(0) &&
+               dy.numel() / dy.size(-1) == x.numel() / x.size(-1) && gu.scalar_type() == x.scalar_type() &&
+               gu.size(-1) == w1.size(0) && gu.numel() / gu.size(-1) == x.numel() / x.size(-1)) {
+      below([&] {
+        const Env e(dy);
+        const Tensor x2 = rows(x), dy2 = rows(dy);
+        Tensor kept = gu.contiguous();
+        if (!aligned(kept)) kept = kept.clone();
+        const GatedSizes g(x2, w2);
+        const Tensor dgu = empty({g.M, 2 * g.H}, dy), h = empty({g.M, g.H}, dy);
+        int kib;
+        const Tensor ws = gated_workspace(g, e, dy, kib);
+        if (nx) dx = empty(x.sizes(), dy);
+        if (nw1) dw1 = empty(w1.sizes(), dy);
+        if (nw2) dw2 = empty(w2.sizes(), dy);
+        if (nb1) db1 = at::zeros({2 * g.H}, dy.options().dtype(at::kFloat));
+        if (nb2) db2 = at::zeros({g.N}, dy.options().dtype(at::kFloat));
+        auto out = [](const Tensor& t) { return const_cast<void*>(at_or_null(t)); };
+        ok(pf_gated_mlp_bwd(dy2.data_ptr(), x2.data_ptr(), w1.data_ptr(), w2.data_ptr(), kept.data_ptr(),
+                            dgu.data_ptr(), h.data_ptr(), out(dx), out(dw1), out(dw2), out(db1), out(db2), out(ws), kib,
+                            g.M, g.D, g.H, g.N, dy2.stride(0), x2.stride(0), w1.stride(0), w2.stride(0), act,
+                            code_of(dy), code_of(dy), code_of(dy), 0, 0, e.status, e.sms, e.stream),
+           "pf_gated_mlp_bwd");
+        return 0;
+      });
+    } else {
+      auto out = dispatched("pfeife::gated_mlp_bwd", {dy, x, w1, w2, gu, (int64_t)act, nx, nw1, nb1, nw2, nb2, opt(b1),
+                                                      opt(b2)});
+      dx = given(out[0]); dw1 = given(out[1]); db1 = given(out[2]); dw2 = given(out[3]); db2 = given(out[4]);
+    }
+    return {dx, dw1, nb1 ? as(db1, ctx->saved_data["type1"]) : Tensor(), dw2,
+            nb2 ? as(db2, ctx->saved_data["type2"]) : Tensor(), nr ? dy : Tensor(), Tensor()};
+  }
+};
+
+// ------------------------------------------------------------------------------ output head with its cross entropy
+bool head_fits(const Tensor& x, const Tensor& w, const Tensor& target) {
+  return x.dim() >= 2 && half(x) && x.numel() > 0 && w.scalar_type() == x.scalar_type() && readable(w) &&
+         w.size(1) == x.size(-1) && w.size(1) % 8 == 0 && w.size(0) > 0 && w.size(0) <= (1ll << 28) &&
+         target.scalar_type() == at::kLong && target.sizes() == x.sizes().slice(0, x.dim() - 1) &&
+         target.numel() <= (1ll << 28) && w.size(1) <= (1ll << 20);
+}
+int64_t padded_rows(int64_t n) { return (n + 255) / 256 * 256; }
+Tensor counted(int n, const char* what, at::ScalarType type, const Tensor& like) {
+  if (n < 0) throw Failed{n, what};
+  return empty({n}, type, like);
+}
+// loss, and for the backward: rows that count, index, statistics, what a sum is multiplied by
+struct HeadOut { Tensor loss, xc, index, stats, inv; };
+HeadOut head_forward(const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore, int reduction) {
+  const Env e(x);
+  Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  if (x2.stride(1) != 1 || x2.stride(0) % 8) x2 = x2.contiguous();
+  const Tensor t = target.contiguous();
+  const int64_t N = x2.size(0), V = w.size(0), D = x2.size(1), Mp = padded_rows(N);
+  HeadOut o;
+  o.loss = reduction ? empty({}, at::kFloat, x) : empty(target.sizes(), at::kFloat, x);
+  o.xc = empty({Mp, D}, x);
+  o.index = counted(pf_head_index(N), "pf_head_index", at::kInt, x);
+  o.stats = empty({Mp, 2}, at::kFloat, x);
+  o.inv = empty({}, at::kFloat, x);
+  const int kib = pf_head_scratch(N, V);
+  if (kib < 0) throw Failed{kib, "pf_head_scratch"};
+  const Tensor scratch = floats(kib * 256ll, x);
+  ok(pf_head_fwd(x2.data_ptr(), w.data_ptr(), t.data_ptr(), o.xc.data_ptr(), o.index.data_ptr(), o.stats.data_ptr(),
+                 o.loss.data_ptr(), o.inv.data_ptr(), scratch.data_ptr(), N, V, (int)D, (int)D,
+                 N > 1 ? x2.stride(0) : D, w.stride(0), ignore, reduction, code_of(x), e.status, e.sms, e.stream),
+     "pf_head_fwd");
+  return o;
+}
+
+struct DirectHeadLoss : torch::autograd::Function<DirectHeadLoss> {
+  static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w, Tensor target, int64_t ignore, int64_t reduction) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const HeadOut o = head_forward(x, w, target, ignore, (int)reduction);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({w, o.xc, o.index, o.stats, o.inv});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["by_row"] = reduction == 0;
+    return o.loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &w = s[0], &xc = s[1], &index = s[2], &stats = s[3], &inv = s[4];
+    if (!grads[0].defined()) return variable_list(5);
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const bool by_row = ctx->saved_data["by_row"].toBool();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
+    int64_t N = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) N *= shape[i];
+    const Tensor g = by_row ? grads[0].reshape({-1}) : grads[0];
+    const int64_t D = shape.back(), Mp = padded_rows(N);
+    Tensor dx, dw;
+    if (direct(g, w, xc, index, stats, inv) && half(xc) && w.scalar_type() == xc.scalar_type() && readable(w) &&
+        w.size(1) == D && xc.dim() == 2 && xc.size(0) == Mp && xc.size(1) == D && xc.is_contiguous() && aligned(xc) &&
+        packed_floats(stats, 2 * Mp) && packed_floats(inv, 1) && index.scalar_type() == at::kInt &&
+        index.is_contiguous() && index.numel() == pf_head_index(N) && g.scalar_type() == at::kFloat &&
+        g.numel() == (by_row ? N : 1)) {
+      below([&] {
+        const Env e(g);
+        const int64_t V = w.size(0);
+        if (nx) dx = empty(shape, xc);
+        if (nw) dw = empty(w.sizes(), xc);
+        const int words = pf_head_words(N, V), parts = pf_head_parts(N, V, (int)D, e.sms);
+        if (words < 0 || parts < 0) throw Failed{words < 0 ? words : parts, "pf_head_words"};
+        const Tensor dz = empty({Mp, words}, xc), acc = nx ? floats(parts * Mp * D, xc) : Tensor();
+        const Tensor factor = by_row ? floats(Mp + 1, xc) : Tensor();
+        auto out = [](const Tensor& t) { return const_cast<void*>(at_or_null(t)); };
+        ok(pf_head_bwd(g.data_ptr(), inv.data_ptr(), xc.data_ptr(), w.data_ptr(), index.data_ptr(), stats.data_ptr(),
+                       out(dx), out(dw), dz.data_ptr(), out(acc), out(factor), N, V, (int)D, (int)D,
+                       by_row ? g.stride(0) : 0, w.stride(0), D, by_row, 0, code_of(xc), code_of(xc), e.status, e.sms,
+                       e.stream),
+           "pf_head_bwd");
+        return 0;
+      });
+    } else {
+      auto out = dispatched("pfeife::head_loss_bwd", {g, xc, index, stats, inv, w, N, by_row, nx, nw});
+      if (nx) dx = out[0].toTensor().view(shape);
+      dw = given(out[1]);
+    }
+    return {dx, nw ? dw : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// ------------------------------------------------------------------------------ scaled embedding
+bool table_type_fits(const Tensor& table, at::ScalarType out) {
+  return table.scalar_type() == at::kFloat || (half(table) && table.scalar_type() == out);
+}
+Tensor embed_forward(const Tensor& ids, const Tensor& table, double scale, at::ScalarType type) {
+  const Env e(table);
+  const Tensor ic = ids.contiguous();
+  auto shape = ids.sizes().vec();
+  shape.push_back(table.size(1));
+  const Tensor out = empty(shape, type, table);
+  ok(pf_scaled_embed_fwd(table.data_ptr(), ic.data_ptr(), out.data_ptr(), ids.numel(), (int)table.size(1),
+                         table.size(0), (float)scale, code_of(table), code_of(type), e.stream),
+     "pf_scaled_embed_fwd");
+  return out;
+}
+struct DirectScaledEmbed : torch::autograd::Function<DirectScaledEmbed> {
+  static Tensor forward(AutogradContext* ctx, Tensor ids, Tensor table, double scale, int64_t type) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const Tensor y = embed_forward(ids, table, scale, static_cast<at::ScalarType>(type));
+    ctx->save_for_backward({ids, table});
+    ctx->saved_data["scale"] = scale;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &ids = s[0], &table = s[1];
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const Tensor dout = grads[0].contiguous();
+    Tensor d;
+    if (direct(dout, ids, table) && ids.scalar_type() == at::kLong && table.dim() == 2 &&
+        (half(dout) || dout.scalar_type() == at::kFloat) && table_type_fits(table, dout.scalar_type()) &&
+        dout.numel() == ids.numel() * table.size(1)) {
+      below([&] {
+        const Env e(dout);
+        const Tensor ic = ids.contiguous();
+        const int64_t V = table.size(0), D = table.size(1);
+        d = empty(table.sizes(), table);
+        const int kib = pf_scaled_embed_scratch(ids.numel(), (int)D, V);
+        if (kib < 0) throw Failed{kib, "pf_scaled_embed_scratch"};
+        const Tensor scratch = floats(kib * 256ll, table);
+        ok(pf_scaled_embed_bwd(dout.data_ptr(), ic.data_ptr(), d.data_ptr(), scratch.data_ptr(), ids.numel(), (int)D, V,
+                               (float)scale, 0, code_of(dout), code_of(table), e.stream),
+           "pf_scaled_embed_bwd");
+        return 0;
+      });
+    } else {
+      d = dispatched("pfeife::scaled_embed_bwd", {dout, ids, table, scale})[0].toTensor();
+    }
+    return {Tensor(), d, Tensor(), Tensor()};
+  }
+};
+
 // ------------------------------------------------------------------------------ Python
 // Arguments of one call.  `fits` turns false at the first that is not what the usual call has.
 struct Args {
@@ -1475,6 +1715,55 @@ PF_OP(conv2d) {
   END_HANDLE_TH_ERRORS
 }
 
+PF_OP(gated_mlp) {
+  HANDLE_TH_ERRORS
+  Args a(args, n, 7);
+  if (PyErr_Occurred()) return nullptr;
+  const Tensor x = a.tensor(0), w1 = a.tensor(1), b1 = a.tensor(2, true), w2 = a.tensor(3), b2 = a.tensor(4, true),
+               r = a.tensor(5, true);
+  const int64_t act = a.integer(6);
+  if (!a.fits || act < 1 || act > 3 || !all_plain(x, w1, b1, w2, b2, r) || !gated_fits(x, w1, w2) ||
+      !bias_fits(b1, w1.size(0)) || !bias_fits(b2, w2.size(0)) ||
+      (r.defined() && (r.scalar_type() != x.scalar_type() || r.sizes() != at::IntArrayRef(with_last(x, w2.size(0))))))
+    Py_RETURN_NONE;
+  if (!recorded(x, w1, b1, w2, b2, r))
+    return run(x, [&] { return unrecorded([&] { return gated_forward(x, w1, b1, w2, b2, r, (int)act, false).first; }); });
+  return run(x, [&] { return DirectGatedMlp::apply(x, w1, maybe(b1), w2, maybe(b2), maybe(r), act); });
+  END_HANDLE_TH_ERRORS
+}
+
+PF_OP(linear_cross_entropy) {
+  HANDLE_TH_ERRORS
+  Args a(args, n, 5);
+  if (PyErr_Occurred()) return nullptr;
+  const Tensor x = a.tensor(0), w = a.tensor(1), t = a.tensor(2);
+  const int64_t ignore = a.integer(3), reduction = a.integer(4);
+  if (!a.fits || !all_plain(x, w, t) || !head_fits(x, w, t)) Py_RETURN_NONE;
+  if (!recorded(x, w))
+    return run(x, [&] { return unrecorded([&] { return head_forward(x, w, t, ignore, (int)reduction).loss; }); });
+  return run(x, [&] { return DirectHeadLoss::apply(x, w, t, ignore, reduction); });
+  END_HANDLE_TH_ERRORS
+}
+
+// the type of the result as the kernels' code for it
+PF_OP(scaled_embedding) {
+  HANDLE_TH_ERRORS
+  Args a(args, n, 4);
+  if (PyErr_Occurred()) return nullptr;
+  const Tensor ids = a.tensor(0), table = a.tensor(1);
+  const double scale = a.real(2);
+  const int64_t code = a.integer(3);
+  if (!a.fits || code < 0 || code > 2) Py_RETURN_NONE;
+  const at::ScalarType type = code == 0 ? at::kFloat : code == 1 ? at::kHalf : at::kBFloat16;
+  if (!all_plain(ids, table) || ids.scalar_type() != at::kLong || table.dim() != 2 || !table.is_contiguous() ||
+      !table_type_fits(table, type) || table.size(0) >= (1ll << 30) || ids.numel() > (1ll << 30) || !std::isfinite(scale))
+    Py_RETURN_NONE;
+  if (!recorded(table))
+    return run(table, [&] { return unrecorded([&] { return embed_forward(ids, table, scale, type); }); });
+  return run(table, [&] { return DirectScaledEmbed::apply(ids, table, scale, (int64_t)type); });
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* setup(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 2) return PyErr_Format(PyExc_TypeError, "setup(status_word, check)");
   Py_INCREF(args[0]);
@@ -1491,7 +1780,7 @@ PyMethodDef methods[] = {
     PF_ENTRY(linear), PF_ENTRY(mlp), PF_ENTRY(norm), PF_ENTRY(attention), PF_ENTRY(attention_qkv),
     PF_ENTRY(rope_qkv), PF_ENTRY(glu), PF_ENTRY(cross_entropy), PF_ENTRY(group_norm), PF_ENTRY(conv2d),
     PF_ENTRY(rotate_heads), PF_ENTRY(norm_rotate_heads), PF_ENTRY(preference_loss), PF_ENTRY(policy_loss),
-    PF_ENTRY(setup), {"launches", launches, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+    PF_ENTRY(gated_mlp), PF_ENTRY(linear_cross_entropy), PF_ENTRY(scaled_embedding), PF_ENTRY(setup), {"launches", launches, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "pfeife_b200_eager", "eager calls of the ops", -1, methods,
                           nullptr, nullptr, nullptr, nullptr};
 

@@ -13,6 +13,7 @@
 
 namespace pf {
 
+// V values of a row; 8 of fp32 move as one access of 32 bytes: two of 16 at a distance of 32 would write each sector twice.
 template <typename T, int V> struct Vec {
   float v[V];
   __device__ __forceinline__ void load(const T* p) {
@@ -22,8 +23,9 @@ template <typename T, int V> struct Vec {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(e[j]);
     } else if constexpr (V == 8) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                   : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                   : "l"(p) : "memory");
     } else {
       v[0] = to_f32<T>(p[0]);
     }
@@ -36,13 +38,17 @@ template <typename T, int V> struct Vec {
       for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j]);
       *reinterpret_cast<uint4*>(p) = q;
     } else if constexpr (V == 8) {
-      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                   "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
     } else {
       p[0] = from_f32<T>(v[0]);
     }
   }
 };
+// whether rows of D values start on the 8-value accesses of their type
+static bool on_rows(const void* p, int D, int dtype) {
+  return D % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & (dtype == PF_F32 ? 31 : 15)) == 0;
+}
 
 // Four vectors of V values a thread, requested before any is written.
 template <typename TT, typename T, int V>
@@ -122,13 +128,28 @@ sort_tokens_kernel(const long long* __restrict__ ids, int N, int words, int bits
     int* mine = counts + warp * SORT_BINS;
     for (int b = lane; b < bins; b += 32) mine[b] = 0;
     __syncwarp();
-    for (int i = begin; i < end; i += 32) {
-      const bool in = i + lane < end;
-      const int t = !in ? 0 : pass ? __ldcg(src + i + lane) : i + lane;
-      const int digit = in ? (key_of(t) >> shift) & (bins - 1) : bins;
-      const unsigned same = __match_any_sync(0xffffffffu, digit);
-      if (in && lane == __ffs(same) - 1) mine[digit] += __popc(same);
-      __syncwarp();
+    // rounds of 32 tokens, 8 at a time so that their loads overlap; a stretch of no more keeps them for the second turn
+    int tok[8], key[8];
+    auto load = [&](int i0) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + 32 * u + lane;
+        tok[u] = i < end ? (pass ? __ldcg(src + i) : i) : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) key[u] = tok[u] >= 0 ? key_of(tok[u]) : -1;
+    };
+    for (int i0 = begin; i0 < end; i0 += 256) {
+      load(i0);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (i0 + 32 * u >= end) break;                  // uniform across the warp
+        const bool in = tok[u] >= 0;
+        const int digit = in ? (key[u] >> shift) & (bins - 1) : bins;
+        const unsigned same = __match_any_sync(0xffffffffu, digit);
+        if (in && lane == __ffs(same) - 1) mine[digit] += __popc(same);
+        __syncwarp();
+      }
     }
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += SORT_THREADS) {
@@ -168,23 +189,26 @@ sort_tokens_kernel(const long long* __restrict__ ids, int N, int words, int bits
     __syncthreads();
     for (int b = lane; b < bins; b += 32) mine[b] += starts[b];
     __syncwarp();
-    for (int i = begin; i < end; i += 32) {
-      const bool in = i + lane < end;
-      const int t = !in ? 0 : pass ? __ldcg(src + i + lane) : i + lane;
-      const int key = in ? key_of(t) : 0;
-      const int digit = in ? (key >> shift) & (bins - 1) : bins;
-      const unsigned same = __match_any_sync(0xffffffffu, digit);
-      if (in) {
-        const int to = mine[digit] + __popc(same & ((1u << lane) - 1));
-        __stcg(dst + to, t);
-        if (pass == passes - 1) {
-          keys[to] = key;
-          if (key < words) atomicOr(present + (key >> 5), 1u << (key & 31));
+    for (int i0 = begin; i0 < end; i0 += 256) {
+      if (end - begin > 256) load(i0);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (i0 + 32 * u >= end) break;
+        const bool in = tok[u] >= 0;
+        const int digit = in ? (key[u] >> shift) & (bins - 1) : bins;
+        const unsigned same = __match_any_sync(0xffffffffu, digit);
+        if (in) {
+          const int to = mine[digit] + __popc(same & ((1u << lane) - 1));
+          __stcg(dst + to, tok[u]);
+          if (pass == passes - 1) {
+            keys[to] = key[u];
+            if (key[u] < words) atomicOr(present + (key[u] >> 5), 1u << (key[u] & 31));
+          }
         }
+        __syncwarp();
+        if (in && lane == __ffs(same) - 1) mine[digit] += __popc(same);
+        __syncwarp();
       }
-      __syncwarp();
-      if (in && lane == __ffs(same) - 1) mine[digit] += __popc(same);
-      __syncwarp();
     }
     all_sync();
   }
@@ -211,8 +235,7 @@ __device__ __forceinline__ void put_row(TT* dtable, const TableGrad& p, int key,
   for (int j = 0; j < V; ++j) r.v[j] *= p.scale;
   if (p.accumulate) {
     Vec<TT, V> old;
-#pragma unroll
-    for (int j = 0; j < V; ++j) old.v[j] = to_f32<TT>(dst[j]);
+    old.load(dst);
 #pragma unroll
     for (int j = 0; j < V; ++j) r.v[j] += old.v[j];
   }
@@ -299,46 +322,69 @@ table_grad_kernel(const T* __restrict__ dout, TT* __restrict__ dtable, const Tab
   }
 }
 
-// Runs that cross windows: the window in which one starts adds up its parts.
+// Runs that cross windows: the window in which one starts adds up its parts, JOIN_GROUPS neighbouring stretches of them
+// side by side and then those.  A CTA has one window's slice of a row.
+constexpr int JOIN_GROUPS = 8;
 template <typename TT, int V>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128 * JOIN_GROUPS)
 table_join_kernel(TT* __restrict__ dtable, const TableGrad p) {
   after_previous();
-  const int lanes = 1 << p.lanes_log;
-  const int slice = blockIdx.x % p.slices;
-  const long long w = (long long)(blockIdx.x / p.slices) * (128 >> p.lanes_log) + (threadIdx.x >> p.lanes_log);
-  const long long b = w * p.window, e = b + p.window;
-  const int c = (slice * lanes + (threadIdx.x & (lanes - 1))) * V;
-  if (e >= p.N || c >= p.D) return;
+  __shared__ float sums[JOIN_GROUPS][128 * V];
+  const int slice = blockIdx.x % p.slices, w = blockIdx.x / p.slices;
+  const int b = w * p.window, e = b + p.window;         // in range: only windows before the last are dealt
   const int run = p.keys[e - 1];
   if (run >= p.words || p.keys[e] != run) return;
   if (b > 0 && p.keys[b] == run && p.keys[b - 1] == run) return;         // it started further ahead
-  int lo = (int)e, hi = p.N;                            // the first token behind the run
+  // the first token behind the run, by 32 looks at a time
+  const int lane = threadIdx.x & 31;
+  int lo = e, hi = p.N;
   while (lo < hi) {
-    const int mid = lo + ((hi - lo) >> 1);
-    if (p.keys[mid] == run) lo = mid + 1;
-    else hi = mid;
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const int n = __popc(__ballot_sync(0xffffffffu, at < hi && p.keys[at] == run));
+    if (n == 0) break;
+    hi = min(hi, lo + n * step);
+    lo = lo + (n - 1) * step + 1;
   }
-  const long long last = (lo - 1) / p.window;
+  const int last = (lo - 1) / p.window;
+  const int group = threadIdx.x >> 7, x = threadIdx.x & 127, c = (slice * 128 + x) * V;
+  const int n = last - w, each = (n + JOIN_GROUPS - 1) / JOIN_GROUPS;
+  const bool mine = c < p.D;
+  float s[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[j] = 0.f;
+  if (mine) {
+    const float* src = p.parts + c;
+    const long long size = 2ll * p.D;
+    if (group == 0) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[j] = src[w * size + p.D + j];
+    }
+    const int k1 = w + 1 + min(n, (group + 1) * each);
+    for (int k = w + 1 + group * each; k < k1; k += 4) {
+      float q[4][V];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (k + u < k1) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) q[u][j] = src[(k + u) * size + j];
+        }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (k + u < k1) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) s[j] += q[u][j];
+        }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) sums[group][j * 128 + x] = s[j];
+  __syncthreads();
+  if (group || !mine) return;
   Vec<TT, V> r;
-  const float* own = p.parts + (w * 2 + 1) * p.D + c;
 #pragma unroll
-  for (int j = 0; j < V; ++j) r.v[j] = own[j];
-  const float* src = p.parts + c;
-  for (long long k = w + 1; k <= last; k += 8) {
-    float q[8][V];
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (k + u <= last) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) q[u][j] = src[(k + u) * 2 * p.D + j];
-      }
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (k + u <= last) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) r.v[j] += q[u][j];
-      }
+  for (int j = 0; j < V; ++j) {
+    r.v[j] = sums[0][j * 128 + x];
+    for (int k = 1; k < JOIN_GROUPS; ++k) r.v[j] += sums[k][j * 128 + x];
   }
   put_row<TT, V>(dtable, p, run, c, r);
 }
@@ -412,7 +458,7 @@ PF_API int pf_scaled_embed_fwd(const void* table, const void* ids, void* out, lo
   if (!embed_sizes_ok(tokens, words, D)) return -3;
   if (tokens == 0 || D == 0) return 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const bool vec = D % 8 == 0 && on_vectors(table, out);
+  const bool vec = on_rows(table, D, table_dtype) && on_rows(out, D, out_dtype);
   const int per_row = vec ? D / 8 : D;
   const long long total = tokens * per_row, ctas = (total + 1023) / 1024;
   if (ctas > 0x7fffffffll) return -3;
@@ -455,7 +501,7 @@ PF_API int pf_scaled_embed_bwd(const void* dout, const void* ids, void* dtable, 
   if (!on_vectors(scratch)) return -2;
   if (D == 0 || words == 0 || (accumulate && tokens == 0)) return 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const bool vec = D % 8 == 0 && on_vectors(dout, dtable);
+  const bool vec = on_rows(dout, D, dtype) && on_rows(dtable, D, table_dtype);
   const EmbedPlan g = embed_plan(tokens, D, vec);
   TableGrad p;
   const int N = (int)tokens;
@@ -473,19 +519,24 @@ PF_API int pf_scaled_embed_bwd(const void* dout, const void* ids, void* dtable, 
   p.scale = scale; p.accumulate = accumulate;
   const int per_cta = 128 >> g.lanes_log;
   const long long work = (g.windows + per_cta - 1) / per_cta * g.slices;
-  p.zero_rows = D >= 1024 ? 8 : D >= 128 ? 64 : 256;
+  p.zero_rows = (int)(words / 2048 < 4 ? 4 : words / 2048);
   const long long zeros = accumulate ? 0 : (words + p.zero_rows - 1) / p.zero_rows;
   if (work + zeros > 0x7fffffffll) return -3;
   p.work_ctas = (unsigned)work;
   const unsigned grid = (unsigned)(work + zeros);
+  const int join_slices = (D + 128 * g.V - 1) / (128 * g.V);
+  const long long joins = (g.windows - 1) * join_slices;         // a run that crosses starts before the last window
+  if (joins > 0x7fffffffll) return -3;
+  TableGrad pj = p;
+  pj.slices = join_slices;
 #define PF_BWD(ID, T_, TD, TT_)                                                                                        \
   if (dtype == ID && table_dtype == TD) {                                                                              \
     if (vec) {                                                                                                         \
       after(table_grad_kernel<T_, TT_, 8>, grid, 128, 0, st)((const T_*)dout, (TT_*)dtable, p);                        \
-      if (g.windows > 1) after(table_join_kernel<TT_, 8>, (unsigned)work, 128, 0, st)((TT_*)dtable, p);                \
+      if (joins > 0) after(table_join_kernel<TT_, 8>, (unsigned)joins, 128 * JOIN_GROUPS, 0, st)((TT_*)dtable, pj);                \
     } else {                                                                                                           \
       after(table_grad_kernel<T_, TT_, 1>, grid, 128, 0, st)((const T_*)dout, (TT_*)dtable, p);                        \
-      if (g.windows > 1) after(table_join_kernel<TT_, 1>, (unsigned)work, 128, 0, st)((TT_*)dtable, p);                \
+      if (joins > 0) after(table_join_kernel<TT_, 1>, (unsigned)joins, 128 * JOIN_GROUPS, 0, st)((TT_*)dtable, pj);                \
     }                                                                                                                  \
   } else
   PF_BWD(PF_F32, float, PF_F32, float)

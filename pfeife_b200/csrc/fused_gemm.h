@@ -12,7 +12,7 @@ enum Job : int {
   HEAD_DZ,      // (softmax(z) - onehot) * factor of some words, in 16 bits
   PARTS_K,      // parts of A B^T in fp32, B with K innermost: products of few rows, split over their reduction
   PARTS_N,      // the same, B with N innermost
-  HEAD_DW,      // dz^T x
+  HEAD_DW,      // dz^T x, and any weight's gradient
 };
 
 // What a row of the product has of the loss: reference and one over the sum; its label.

@@ -820,33 +820,3 @@ int fused_gemm(Job job, const FusedCall& c) {
 }
 
 }  // namespace pf
-
-using namespace pf;
-
-// h [M, H] = act(x Wg^T + bg) * (x Wu^T + bu) with Wg, Wu the first and the last H rows of w [2H, K]; gu [M, 2H], where
-// given, keeps both projections for the backward.  act: 1 GELU (erf), 2 GELU (tanh), 3 SiLU.  K and H are multiples of
-// 8, rows of x and w start on 16 bytes; h and gu are packed.
-PF_API int pf_glu_linear_fwd(const void* x, const void* w, const void* bias, int bias_dtype, void* h, void* gu, int M,
-                             int H, int K, long long ldx, long long ldw, int act, int dtype, int* status, int sm_count,
-                             void* stream) {
-  if (act < 1 || act > 3) return -1;
-  if (H % 8 || K % 8) return -2;
-  FusedCall c;
-  c.M = M; c.N = H; c.K = K; c.A = x; c.B = w; c.lda = ldx; c.ldb = ldw; c.dtype = dtype;
-  c.C = h; c.ldc = H; c.gu = gu; c.bias = bias; c.bias_dtype = bias_dtype; c.act = act; c.status = status;
-  c.sm_count = sm_count > 0 ? sm_count : 148; c.stream = reinterpret_cast<cudaStream_t>(stream);
-  return fused_gemm(GLU_FWD, c);
-}
-
-// From dy [M, K], w2 [K, H] and the kept gu [M, 2H]: dgu [M, 2H], the gradient of gu, and h [M, H] once more.
-PF_API int pf_glu_linear_bwd(const void* dy, const void* w2, const void* gu, void* dgu, void* h, int M, int H, int K,
-                             long long lddy, long long ldw2, int act, int dtype, int* status, int sm_count,
-                             void* stream) {
-  if (act < 1 || act > 3) return -1;
-  if (H % 8 || K % 8) return -2;
-  FusedCall c;
-  c.M = M; c.N = H; c.K = K; c.A = dy; c.B = w2; c.lda = lddy; c.ldb = ldw2; c.dtype = dtype;
-  c.C = h; c.ldc = H; c.gu = const_cast<void*>(gu); c.dgu = dgu; c.act = act; c.status = status;
-  c.sm_count = sm_count > 0 ? sm_count : 148; c.stream = reinterpret_cast<cudaStream_t>(stream);
-  return fused_gemm(GLU_BWD, c);
-}

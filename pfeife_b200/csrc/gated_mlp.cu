@@ -1,0 +1,325 @@
+// The gated feed-forward block, y = (act(x Wg^T + bg) * (x Wu^T + bu)) W2^T + b2 + residual, and its gradients, as the
+// products of fused_gemm_sm100.cu and gemm_sm100.cu.
+//
+// Forward 6 M D H operations in two products (the first with both projections, the activation and their product in its
+// epilogue), backward 12 M D H in five: dh with everything that follows from it in the epilogue, dx and the weights'
+// gradients.  Up to 128 rows the weights are what moves, 6 bytes of each of the 3 D H read or written per direction:
+// a product is then split over its reduction into as many parts as keep all SMs reading, and what its epilogue does is done
+// by the kernels here, which add the parts up in their order.
+#include "common.cuh"
+#include "api.h"
+#include "fused_gemm.h"
+
+namespace pf {
+
+// Parts that a product of few rows is split into; 1: it stays whole.  In units of the time of a k-block of 64: an item
+// costs its k-blocks and one more or two, parts a launch and a read of some 20.
+static int row_parts(long long M, long long N, long long K, int sm_count) {
+  if (M > 128) return 1;
+  const long long tiles = (N + 127) / 128, kb = (K + 63) / 64;
+  int best = 1;
+  double least = 1e30;
+  for (int p = 1; p <= 32 && (p == 1 || p * 4 <= kb); ++p) {
+    const double rounds = (double)((tiles * p + sm_count - 1) / sm_count);
+    double t = rounds * ((double)((kb + p - 1) / p) + 1.5);
+    if (p > 1) t += 20 + (double)p * M * N * 8 / 6e12 / 0.15e-6;
+    if (t < least - 1e-9) {
+      least = t;
+      best = p;
+    }
+  }
+  return best;
+}
+constexpr int PART_ROWS = 128;
+
+struct Parts {
+  const float* at;
+  int parts;
+  long long size;               // floats of a part
+};
+__device__ __forceinline__ void sum_parts(const Parts& p, long long i, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < p.parts; ++k) {
+    const float4* q = reinterpret_cast<const float4*>(p.at + k * p.size + i);
+    const float4 a = __ldg(q), b = __ldg(q + 1);
+    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+  }
+}
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  const uint4 q = *reinterpret_cast<const uint4*>(p);
+  const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(e[j]);
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  uint4 q;
+  T* e = reinterpret_cast<T*>(&q);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j]);
+  *reinterpret_cast<uint4*>(p) = q;
+}
+__device__ __forceinline__ void add_bias8(const void* b, int dtype, int i, float (&v)[8]) {
+  if (!b) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    v[j] += dtype == PF_F32 ? static_cast<const float*>(b)[i + j]
+            : dtype == PF_F16 ? __half2float(static_cast<const __half*>(b)[i + j])
+                              : __bfloat162float(static_cast<const __nv_bfloat16*>(b)[i + j]);
+}
+__device__ __forceinline__ void act_of(int act, float z, float& a, float& slope) {
+  if (act == 1) {
+    a = gelu_erf(z);
+    slope = dgelu_erf(z);
+  } else {
+    // z s(q), see fused_gemm_sm100.cu
+    const float z2 = z * z, c = 2.f * 0.7978845608028654f;
+    const float q = act == 2 ? c * z * fmaf(z2, 0.044715f, 1.f) : z;
+    const float dq = act == 2 ? fmaf(fminf(z2, 1e6f), 3.f * 0.044715f * c, c) : 1.f;
+    const float s = 1.f / (1.f + __expf(-q));
+    a = z * s;
+    slope = fmaf(a - a * s, dq, s);
+  }
+}
+
+// Gate and up of 8 hidden values a thread -> h, and both kept.
+template <typename T>
+__global__ void __launch_bounds__(128)
+glu_join_kernel(const Parts p, const void* __restrict__ bias, int bias_dtype, T* __restrict__ gu, T* __restrict__ h,
+                int M, int H, int act) {
+  after_previous();
+  const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
+  const int nv = H / 8, m = (int)(i / nv), c = (int)(i - (long long)m * nv) * 8;
+  if (m >= M) return;
+  float g[8], u[8];
+  sum_parts(p, (long long)m * 2 * H + c, g);
+  sum_parts(p, (long long)m * 2 * H + H + c, u);
+  add_bias8(bias, bias_dtype, c, g);
+  add_bias8(bias, bias_dtype, H + c, u);
+  if (gu) {
+    store8(gu + (long long)m * 2 * H + c, g);
+    store8(gu + (long long)m * 2 * H + H + c, u);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float a, slope;
+    act_of(act, g[j], a, slope);
+    g[j] = a * u[j];
+  }
+  store8(h + (long long)m * H + c, g);
+}
+
+// dh of 8 hidden values a thread -> the gradients of gate and up, and h.
+template <typename T>
+__global__ void __launch_bounds__(128)
+glu_join_bwd_kernel(const Parts p, const T* __restrict__ gu, T* __restrict__ dgu, T* __restrict__ h, int M, int H,
+                    int act) {
+  after_previous();
+  const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
+  const int nv = H / 8, m = (int)(i / nv), c = (int)(i - (long long)m * nv) * 8;
+  if (m >= M) return;
+  float d[8], g[8], u[8];
+  const long long at = (long long)m * 2 * H + c;
+  load8(gu + at, g);
+  load8(gu + at + H, u);
+  sum_parts(p, (long long)m * H + c, d);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float a, slope;
+    act_of(act, g[j], a, slope);
+    g[j] = d[j] * u[j] * slope;
+    d[j] *= a;
+    u[j] *= a;
+  }
+  store8(dgu + at, g);
+  store8(dgu + at + H, d);
+  store8(h + (long long)m * H + c, u);
+}
+
+// The sum of the parts, with a bias and a residual
+template <typename T>
+__global__ void __launch_bounds__(128)
+row_join_kernel(const Parts p, const void* __restrict__ bias, int bias_dtype, const T* __restrict__ residual,
+                long long ldr, T* __restrict__ out, int M, int N) {
+  after_previous();
+  const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
+  const int nv = N / 8, m = (int)(i / nv), c = (int)(i - (long long)m * nv) * 8;
+  if (m >= M) return;
+  float v[8];
+  sum_parts(p, (long long)m * N + c, v);
+  add_bias8(bias, bias_dtype, c, v);
+  if (residual) {
+    float r[8];
+    load8(residual + m * ldr + c, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += r[j];
+  }
+  store8(out + (long long)m * N + c, v);
+}
+
+}  // namespace pf
+
+using namespace pf;
+
+// KiB of workspace of both directions for M rows; 0 where no product is split
+PF_API int pf_gated_mlp_scratch(int M, int D, int H, int N, int sm_count) {
+  if (sm_count <= 0) sm_count = 148;
+  long long most = 0;
+  auto need = [&](long long n, long long k) {
+    const int p = row_parts(M, n, k, sm_count);
+    if (p > 1 && p * n > most) most = p * n;
+  };
+  need(2ll * H, D);
+  need(N, H);
+  need(H, N);
+  need(D, 2ll * H);
+  return (int)((most * PART_ROWS * 4 + 1023) / 1024);
+}
+
+namespace pf {
+struct Block {
+  int M, D, H, N, act, dtype, sms;
+  int* status;
+  float* ws;
+  cudaStream_t st;
+  FusedCall call(int n, int k, const void* a, long long lda, const void* b, long long ldb) const {
+    FusedCall c;
+    c.M = M; c.N = n; c.K = k; c.A = a; c.lda = lda; c.B = b; c.ldb = ldb;
+    c.dtype = dtype; c.status = status; c.sm_count = sms; c.stream = st;
+    return c;
+  }
+  // A B^T in parts; n > 1
+  int in_parts(Job job, FusedCall c, int n, Parts& p) const {
+    c.C = ws; c.ldc = c.N; c.out_dtype = PF_F32; c.split = n; c.part_rows = PART_ROWS;
+    p = {ws, n, (long long)PART_ROWS * c.N};
+    return fused_gemm(job, c);
+  }
+  unsigned grid(int width) const { return (unsigned)(((long long)M * (width / 8) + 127) / 128); }
+  // dst [rows, cols] (+)= a^T b over the M rows
+  int weight_grad(const void* a, long long lda, const void* b, long long ldb, void* dst, int rows, int cols,
+                  int dst_dtype, int add) const {
+    FusedCall c = call(cols, M, a, lda, b, ldb);
+    c.M = rows; c.C = dst; c.ldc = cols; c.out_dtype = dst_dtype; c.accumulate = add;
+    return fused_gemm(HEAD_DW, c);
+  }
+};
+
+template <typename T>
+static int mlp_forward(const Block& b, const void* x, const void* w1, const void* b1, int b1_dtype, const void* w2,
+                       const void* b2, int b2_dtype, const void* residual, void* h, void* gu, void* y, long long ldx,
+                       long long ldw1, long long ldw2, long long ldr) {
+  int r;
+  const int p1 = b.ws ? row_parts(b.M, 2ll * b.H, b.D, b.sms) : 1, p2 = b.ws ? row_parts(b.M, b.N, b.H, b.sms) : 1;
+  Parts p;
+  if (p1 > 1) {
+    if ((r = b.in_parts(PARTS_K, b.call(2 * b.H, b.D, x, ldx, w1, ldw1), p1, p))) return r;
+    after(glu_join_kernel<T>, b.grid(b.H), 128, 0, b.st)(p, b1, b1_dtype, (T*)gu, (T*)h, b.M, b.H, b.act);
+    PF_CHECK_LAUNCH();
+  } else {
+    FusedCall c = b.call(b.H, b.D, x, ldx, w1, ldw1);
+    c.C = h; c.ldc = b.H; c.gu = gu; c.bias = b1; c.bias_dtype = b1_dtype; c.act = b.act;
+    if ((r = fused_gemm(GLU_FWD, c))) return r;
+  }
+  if (p2 > 1) {
+    if ((r = b.in_parts(PARTS_K, b.call(b.N, b.H, h, b.H, w2, ldw2), p2, p))) return r;
+    after(row_join_kernel<T>, b.grid(b.N), 128, 0, b.st)(p, b2, b2_dtype, (const T*)residual, ldr, (T*)y, b.M, b.N);
+    PF_CHECK_LAUNCH();
+    return 0;
+  }
+  return pf_gemm(h, w2, y, b.M, b.N, b.H, b.H, ldw2, b.N, 0, 0, b.dtype, b.dtype, b2, b2_dtype, residual, ldr, nullptr,
+                 0, 0, 0, 1.0f, b.status, b.sms, 0, nullptr, 0, b.st);
+}
+
+template <typename T>
+static int mlp_backward(const Block& b, const void* dy, const void* x, const void* w1, const void* w2, const void* gu,
+                        void* dgu, void* h, void* dx, void* dw1, void* dw2, void* db1, void* db2, long long lddy,
+                        long long ldx, long long ldw1, long long ldw2, int dw1_dtype, int dw2_dtype, int add1,
+                        int add2) {
+  int r;
+  const int p1 = b.ws ? row_parts(b.M, b.H, b.N, b.sms) : 1, p2 = b.ws ? row_parts(b.M, b.D, 2ll * b.H, b.sms) : 1;
+  Parts p;
+  if (p1 > 1) {
+    if ((r = b.in_parts(PARTS_N, b.call(b.H, b.N, dy, lddy, w2, ldw2), p1, p))) return r;
+    after(glu_join_bwd_kernel<T>, b.grid(b.H), 128, 0, b.st)(p, (const T*)gu, (T*)dgu, (T*)h, b.M, b.H, b.act);
+    PF_CHECK_LAUNCH();
+  } else {
+    FusedCall c = b.call(b.H, b.N, dy, lddy, w2, ldw2);
+    c.C = h; c.ldc = b.H; c.gu = const_cast<void*>(gu); c.dgu = dgu; c.act = b.act;
+    if ((r = fused_gemm(GLU_BWD, c))) return r;
+  }
+  if (dw2 && (r = b.weight_grad(dy, lddy, h, b.H, dw2, b.N, b.H, dw2_dtype, add2))) return r;
+  if (db2 && (r = pf_colsum(dy, db2, b.M, b.N, lddy, b.dtype, b.sms, b.st))) return r;
+  const long long ldgu = 2ll * b.H;
+  if (dx) {
+    if (p2 > 1) {
+      if ((r = b.in_parts(PARTS_N, b.call(b.D, 2 * b.H, dgu, ldgu, w1, ldw1), p2, p))) return r;
+      after(row_join_kernel<T>, b.grid(b.D), 128, 0, b.st)(p, (const void*)nullptr, 0, (const T*)nullptr, 0ll, (T*)dx,
+                                                           b.M, b.D);
+      PF_CHECK_LAUNCH();
+    } else if ((r = pf_gemm(dgu, w1, dx, b.M, b.D, 2 * b.H, ldgu, ldw1, b.D, 0, 1, b.dtype, b.dtype, nullptr, 0,
+                            nullptr, 0, nullptr, 0, 0, 0, 1.0f, b.status, b.sms, 0, nullptr, 0, b.st))) {
+      return r;
+    }
+  }
+  if (dw1 && (r = b.weight_grad(dgu, ldgu, x, ldx, dw1, 2 * b.H, b.D, dw1_dtype, add1))) return r;
+  if (db1 && (r = pf_colsum(dgu, db1, b.M, 2 * b.H, ldgu, b.dtype, b.sms, b.st))) return r;
+  return 0;
+}
+
+static int mlp_block(Block& b, int M, int D, int H, int N, int act, int dtype, void* ws, int ws_kib, int* status,
+                     int sm_count, void* stream) {
+  if (dtype != PF_F16 && dtype != PF_BF16) return -1;
+  if (act < 1 || act > 3) return -1;
+  if (M < 0 || D <= 0 || H <= 0 || N <= 0 || H > (1 << 29)) return -3;
+  if (D % 8 || H % 8 || N % 8 || !on_vectors(ws)) return -2;
+  b = {M, D, H, N, act, dtype, sm_count > 0 ? sm_count : 148, status, static_cast<float*>(ws),
+       reinterpret_cast<cudaStream_t>(stream)};
+  if (!ws || ws_kib < pf_gated_mlp_scratch(M, D, H, N, b.sms)) b.ws = nullptr;       // every product stays whole
+  return 0;
+}
+}  // namespace pf
+
+// x [M, D], w1 [2H, D], w2 [N, H], all with rows on 16 bytes, b1 [2H], b2 [N] and residual [M, N] may be null; D, H and N
+// are multiples of 8.  h [M, H], gu [M, 2H] (null: gate and up are not kept) and y [M, N] are packed.
+// act: 1 GELU (erf), 2 GELU (tanh), 3 SiLU.  ws: pf_gated_mlp_scratch.
+PF_API int pf_gated_mlp_fwd(const void* x, const void* w1, const void* b1, int b1_dtype, const void* w2, const void* b2,
+                            int b2_dtype, const void* residual, void* h, void* gu, void* y, void* ws, int ws_kib, int M,
+                            int D, int H, int N, long long ldx, long long ldw1, long long ldw2, long long ldr, int act,
+                            int dtype, int* status, int sm_count, void* stream) {
+  Block b;
+  const int r = mlp_block(b, M, D, H, N, act, dtype, ws, ws_kib, status, sm_count, stream);
+  if (r || M == 0) return r;
+  if (ldx % 8 || ldw1 % 8 || ldw2 % 8 || (residual && ldr % 8) || !on_vectors(x, w1, w2, residual, h, gu, y)) return -2;
+  return dtype == PF_F16 ? mlp_forward<__half>(b, x, w1, b1, b1_dtype, w2, b2, b2_dtype, residual, h, gu, y, ldx, ldw1,
+                                               ldw2, ldr)
+                         : mlp_forward<__nv_bfloat16>(b, x, w1, b1, b1_dtype, w2, b2, b2_dtype, residual, h, gu, y, ldx,
+                                                      ldw1, ldw2, ldr);
+}
+
+// From dy [M, N] and the kept gu: dx [M, D], dw1 [2H, D], dw2 [N, H] (packed, 16 bits or fp32; add1, add2: added to fp32),
+// db1 [2H] and db2 [N] (fp32, added to); any of these may be null.  dgu [M, 2H] and h [M, H] are scratch.
+PF_API int pf_gated_mlp_bwd(const void* dy, const void* x, const void* w1, const void* w2, const void* gu, void* dgu,
+                            void* h, void* dx, void* dw1, void* dw2, void* db1, void* db2, void* ws, int ws_kib, int M,
+                            int D, int H, int N, long long lddy, long long ldx, long long ldw1, long long ldw2, int act,
+                            int dtype, int dw1_dtype, int dw2_dtype, int add1, int add2, int* status, int sm_count,
+                            void* stream) {
+  Block b;
+  const int r = mlp_block(b, M, D, H, N, act, dtype, ws, ws_kib, status, sm_count, stream);
+  if (r) return r;
+  if ((add1 && dw1_dtype != PF_F32) || (add2 && dw2_dtype != PF_F32)) return -1;
+  if ((dw1 && dw1_dtype != dtype && dw1_dtype != PF_F32) || (dw2 && dw2_dtype != dtype && dw2_dtype != PF_F32)) return -1;
+  if (M == 0) {                                         // nothing to add up
+    const size_t s1 = dw1_dtype == PF_F32 ? 4 : 2, s2 = dw2_dtype == PF_F32 ? 4 : 2;
+    cudaError_t e = cudaSuccess;
+    if (dw1 && !add1) e = cudaMemsetAsync(dw1, 0, 2 * (size_t)H * D * s1, b.st);
+    if (dw2 && !add2 && e == cudaSuccess) e = cudaMemsetAsync(dw2, 0, (size_t)N * H * s2, b.st);
+    return (int)e;
+  }
+  if (lddy % 8 || ldx % 8 || ldw1 % 8 || ldw2 % 8 || !on_vectors(dy, x, w1, w2, gu, dgu, h, dx, dw1, dw2)) return -2;
+  return dtype == PF_F16 ? mlp_backward<__half>(b, dy, x, w1, w2, gu, dgu, h, dx, dw1, dw2, db1, db2, lddy, ldx, ldw1,
+                                                ldw2, dw1_dtype, dw2_dtype, add1, add2)
+                         : mlp_backward<__nv_bfloat16>(b, dy, x, w1, w2, gu, dgu, h, dx, dw1, dw2, db1, db2, lddy, ldx,
+                                                       ldw1, ldw2, dw1_dtype, dw2_dtype, add1, add2);
+}

@@ -111,58 +111,57 @@ head_gather_kernel(const T* __restrict__ x, T* __restrict__ xc, HeadIndex ix, in
   }
 }
 
-// Joins the parts of 32 rows: 32 threads share the parts of a row, with lanes on neighbouring rows; then a warp has a row.
-// References are integers: 2^(a - b) is exact.  The row's loss is formed in 64 bits; `sums` gets a CTA's sum of them, and
-// the CTA that finishes last adds those up in their order.
+// Joins the parts of FOLD_ROWS rows: 128 threads share the parts of a row, with lanes on neighbouring rows; then a warp
+// has a row.  References are integers: 2^(a - b) is exact.  The row's loss is formed in 64 bits; `sums` gets a CTA's sum
+// of them, and the CTA that finishes last adds those up in their order.
+constexpr int FOLD_ROWS = 8, FOLD_LANES = 1024 / FOLD_ROWS;
+__device__ __forceinline__ void join(float& ref, float& sum, float ref2, float sum2) {
+  const float m = fmaxf(ref, ref2), sub = m == -INFINITY ? 0.f : m;
+  sum = sum * exp2f(ref - sub) + sum2 * exp2f(ref2 - sub);
+  ref = m;
+}
 __global__ void __launch_bounds__(1024)
 head_fold_kernel(const RowStat* __restrict__ parts, long long pitch, int n_parts, const float* __restrict__ picked,
                  HeadIndex ix, RowStat* __restrict__ stats, float* __restrict__ loss_of_row, float* __restrict__ loss,
                  float* __restrict__ inv, double* __restrict__ sums, int mean) {
   after_previous();
-  __shared__ RowStat all[32][33];
+  __shared__ RowStat all[FOLD_ROWS][FOLD_LANES + 1];
   __shared__ double rows[32];
   __shared__ int last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int count = *ix.count, row0 = blockIdx.x * 32;
+  const int count = *ix.count, row0 = blockIdx.x * FOLD_ROWS;
   if (row0 < count) {
-    const int row = row0 + lane;
+    const int r = threadIdx.x % FOLD_ROWS, l = threadIdx.x / FOLD_ROWS, row = row0 + r;
     float ref = -INFINITY, sum = 0.f;
     if (row < count) {
       const RowStat* src = parts + row;
-      for (int k = warp; k < n_parts; k += 256) {
+      for (int k = l; k < n_parts; k += 8 * FOLD_LANES) {
         RowStat q[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-          if (k + 32 * u < n_parts) q[u] = src[(k + 32 * u) * pitch];
+          if (k + FOLD_LANES * u < n_parts) q[u] = src[(k + FOLD_LANES * u) * pitch];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-          if (k + 32 * u < n_parts) {
-            const float m = fmaxf(ref, q[u].ref), sub = m == -INFINITY ? 0.f : m;
-            sum = sum * exp2f(ref - sub) + q[u].inv * exp2f(q[u].ref - sub);
-            ref = m;
-          }
+          if (k + FOLD_LANES * u < n_parts) join(ref, sum, q[u].ref, q[u].inv);
       }
     }
-    all[warp][lane] = {ref, sum};
+    all[r][l] = {ref, sum};
   }
   __syncthreads();
-  const int row = row0 + warp;                          // the warp's row, over whose parts its lanes lie
+  const int row = row0 + warp;
   if (lane == 0) rows[warp] = 0.0;
-  if (row < count) {
-    RowStat q = all[lane][warp];
+  if (warp < FOLD_ROWS && row < count) {
+    float ref = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float ref = __shfl_xor_sync(0xffffffffu, q.ref, o), sum = __shfl_xor_sync(0xffffffffu, q.inv, o);
-      const float m = fmaxf(q.ref, ref), sub = m == -INFINITY ? 0.f : m;
-      // the same sum in both lanes of a pair, whichever has the first half
-      const float a = q.inv * exp2f(q.ref - sub), b = sum * exp2f(ref - sub);
-      q = {m, a + b};
-    }
+    for (int k = 0; k < FOLD_LANES / 32; ++k) join(ref, sum, all[warp][lane + 32 * k].ref, all[warp][lane + 32 * k].inv);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      join(ref, sum, __shfl_xor_sync(0xffffffffu, ref, o), __shfl_xor_sync(0xffffffffu, sum, o));
     if (lane == 0) {
-      const float ref = q.ref == -INFINITY ? 0.f : q.ref;
-      stats[row] = {ref, 1.f / q.inv};
+      if (ref == -INFINITY) ref = 0.f;
+      stats[row] = {ref, 1.f / sum};
       constexpr double ln2 = 0.69314718055994531;
-      const double l = (log2((double)q.inv) + (double)ref - (double)picked[row] * (double)1.4426950408889634f) * ln2;
+      const double l = (log2((double)sum) + (double)ref - (double)picked[row] * (double)1.4426950408889634f) * ln2;
       rows[warp] = l;
       if (loss_of_row) loss_of_row[ix.list[row]] = (float)l;
     }
@@ -171,7 +170,7 @@ head_fold_kernel(const RowStat* __restrict__ parts, long long pitch, int n_parts
   __syncthreads();
   if (threadIdx.x == 0) {
     double s = 0.0;
-    for (int i = 0; i < 32; ++i) s += rows[i];
+    for (int i = 0; i < FOLD_ROWS; ++i) s += rows[i];
     sums[blockIdx.x] = s;
     __threadfence();
     last = atomicAdd(ix.count + 1, 1) == (int)gridDim.x - 1;
@@ -180,7 +179,8 @@ head_fold_kernel(const RowStat* __restrict__ parts, long long pitch, int n_parts
   if (!last) return;
   __threadfence();
   double s = 0.0;
-  for (int i = threadIdx.x; i < (int)gridDim.x; i += 1024) s += reinterpret_cast<volatile double*>(sums)[i];
+  for (int i = threadIdx.x; i < (count + FOLD_ROWS - 1) / FOLD_ROWS; i += 1024)
+    s += reinterpret_cast<volatile double*>(sums)[i];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) rows[warp] = s;
@@ -222,7 +222,9 @@ head_factor_kernel(const float* __restrict__ g, long long step, HeadIndex ix, fl
   if (threadIdx.x == 0) *scale = ldexpf(1.f, e);
 }
 
-// dx[n] = the sum over parts of acc at the row's place, times the scale; zeros for rows that do not count.
+// dx[n] = the sum over parts of acc at the row's place, times the scale; zeros for rows that do not count.  A warp has
+// DX_COLUMNS of a row.
+constexpr int DX_COLUMNS = 512;
 template <typename T>
 __global__ void __launch_bounds__(256)
 head_dx_kernel(const float* __restrict__ acc, T* __restrict__ dx, HeadIndex ix, long long N, int D, int Dp, int parts,
@@ -233,13 +235,14 @@ head_dx_kernel(const float* __restrict__ acc, T* __restrict__ dx, HeadIndex ix, 
   const int lane = threadIdx.x & 31;
   const long long n = blockIdx.x * 8ll + (threadIdx.x >> 5);
   if (n >= N) return;
-  const int at = ix.at[n];
+  const int at = ix.at[n], begin = blockIdx.y * DX_COLUMNS, end = min(D, begin + DX_COLUMNS);
   const float* src = acc + (long long)at * Dp;
   T* dst = dx + n * D;
   if (vec) {
-    for (int c = lane * 8; c < D; c += 256) {
+    for (int c = begin + lane * 8; c < end; c += 256) {
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (at >= 0) {
+#pragma unroll 4
         for (int k = 0; k < parts; ++k) {
           const float4* q = reinterpret_cast<const float4*>(src + k * part_size + c);
           const float4 a = q[0], b = q[1];
@@ -256,7 +259,7 @@ head_dx_kernel(const float* __restrict__ acc, T* __restrict__ dx, HeadIndex ix, 
       *reinterpret_cast<uint4*>(dst + c) = q;
     }
   } else {
-    for (int c = lane; c < D; c += 32) {
+    for (int c = begin + lane; c < end; c += 32) {
       float v = 0.f;
       if (at >= 0) {
         for (int k = 0; k < parts; ++k) v += src[k * part_size + c];
@@ -289,7 +292,7 @@ PF_API int pf_head_index(long long N) {
 PF_API int pf_head_scratch(long long N, long long V) {
   if (!head_sizes_ok(N, V, 1)) return -3;
   const long long Mp = padded_rows(N), parts = (V + HEAD_PART - 1) / HEAD_PART;
-  const long long kib = (parts * Mp * 8 + Mp * 4 + Mp / 32 * 8 + 1023) / 1024 + 1;
+  const long long kib = (parts * Mp * 8 + Mp * 4 + (Mp / FOLD_ROWS + 1) * 8 + 1023) / 1024 + 1;
   return kib > 0x7fffffffll ? -3 : (int)kib;
 }
 
@@ -333,7 +336,7 @@ PF_API int pf_head_fwd(const void* x, const void* w, const void* target, void* x
   const int n_parts = (int)((V + HEAD_PART - 1) / HEAD_PART);
   RowStat* parts = static_cast<RowStat*>(scratch);
   double* sums = reinterpret_cast<double*>(parts + n_parts * Mp);
-  float* picked = reinterpret_cast<float*>(sums + Mp / 32);
+  float* picked = reinterpret_cast<float*>(sums + Mp / FOLD_ROWS + 1);
   float* each = reduction == 0 ? static_cast<float*>(loss) : nullptr;
   after(head_rows_kernel, 1, 1024, 0, st)((const long long*)target, ix, each, (int)N, V, ignore_index);
   PF_CHECK_LAUNCH();
@@ -353,7 +356,7 @@ PF_API int pf_head_fwd(const void* x, const void* w, const void* target, void* x
     const int r = fused_gemm(HEAD_STATS, c);
     if (r) return r;
   }
-  const unsigned grid = (unsigned)(Mp > 0 ? Mp / 32 : 1);
+  const unsigned grid = (unsigned)(N > 0 ? (N + FOLD_ROWS - 1) / FOLD_ROWS : 1);
   after(head_fold_kernel, grid, 1024, 0, st)((const RowStat*)parts, Mp, n_parts, (const float*)picked, ix,
                                              (RowStat*)stats, each, each ? nullptr : (float*)loss, (float*)inv, sums,
                                              (int)(reduction == 1));
@@ -420,7 +423,7 @@ PF_API int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const
   }
   if (dx) {
     const int vec = D == Dp && on_vectors(dx);
-    const unsigned grid = (unsigned)((N + 7) / 8);
+    const dim3 grid((unsigned)((N + 7) / 8), (unsigned)((D + DX_COLUMNS - 1) / DX_COLUMNS));
     if (dtype == PF_F16)
       after(head_dx_kernel<__half>, grid, 256, 0, st)((const float*)acc, (__half*)dx, ix, N, D, Dp, parts, Mp * Dp, scale,
                                                       scale2, 1.f / unit, vec);

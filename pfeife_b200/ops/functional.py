@@ -640,13 +640,11 @@ def gated_mlp_fwd(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: O
     """-> (y, gate and up [..., 2H], empty unless they are to be kept for a backward)"""
     cd = compute_dtype(x)
     shape, H = x.shape[:-1], w2.shape[1]
-    if w2.is_cuda and w2.dtype == cd and H % 8 == 0:
-        w2 = _aligned(w2)
     if _glu_native(x, cd, w1, w2):
-        x2 = _rows(x if x.dtype == cd else kx.cast(x, cd))
-        h, gu = kx.glu_linear_fwd(x2, _aligned(_weight_as(w1, cd)), b1, act, keep)
-        y, _ = linear_fwd.plain(h.view(shape + (H,)), w2, b2, residual, ACT_NONE)
-        return y, (gu.view(shape + (2 * H,)) if keep else x.new_empty(0))
+        cast = lambda t: _rows(t if t.dtype == cd else kx.cast(t, cd))
+        y, gu = kx.gated_mlp_fwd(cast(x), _aligned(_weight_as(w1, cd)), b1, _aligned(_weight_as(w2, cd)), b2,
+                                 None if residual is None else cast(residual), act, keep)
+        return y.view(shape + (w2.shape[0],)), (gu.view(shape + (2 * H,)) if keep else x.new_empty(0))
     if x.is_cuda and cd in (torch.float16, torch.bfloat16):      # odd widths, product by product
         x2, w = _rows(x if x.dtype == cd else kx.cast(x, cd)), _weight_as(w1, cd)
         wide = kx.gemm(_aligned(_pad_k(x2)), _aligned(_pad_k(w)), out_dtype=torch.float32, bias=b1).view(
@@ -656,7 +654,8 @@ def gated_mlp_fwd(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: O
         if b1 is not None:
             wide = wide + b1.to(cd)
     h = (_act_slope(wide[..., :H], act)[0] * wide[..., H:]).to(cd)
-    y, _ = linear_fwd.plain(h, w2, b2, residual, ACT_NONE)
+    w = _aligned(_pad_k(w2)) if w2.is_cuda and w2.dtype == cd else w2
+    y, _ = linear_fwd.plain(h if w.shape[1] == H else _pad_k(h), w, b2, residual, ACT_NONE)
     return y, (wide.to(cd) if keep else x.new_empty(0))
 
 
@@ -681,20 +680,14 @@ def gated_mlp_bwd(dy: Tensor, x: Tensor, w1: Tensor, w2: Tensor, gu: Tensor, act
         zeros = lambda t, need: torch.zeros_like(t) if need else dy.new_empty(0)
         return (dy.new_zeros(x.shape), zeros(w1, need_dw1), dy.new_zeros(2 * H if need_db1 else 0, dtype=torch.float32),
                 zeros(w2, need_dw2), dy.new_zeros(w2.shape[0] if need_db2 else 0, dtype=torch.float32))
-    if w2.is_cuda and w1.dtype == cd and w1.shape[1] % 8 == 0:
-        w1 = _aligned(w1)
-    if w2.is_cuda and w2.dtype == cd and H % 8 == 0:
-        w2 = _aligned(w2)
+    native = dy.is_cuda and cd in (torch.float16, torch.bfloat16)
     if _glu_native(dy, cd, w1, w2):
-        dgu, h = kx.glu_linear_bwd(_rows(dy), _aligned(_weight_as(w2, cd)), _rows(gu), act)
-        dgu, h = dgu.view(gu.shape), h.view(gu.shape[:-1] + (H,))
-    else:
-        dh = linear_bwd.plain(dy, gu[..., :H], w2, empty, ACT_NONE, True, False, False)[0] \
-            if dy.is_cuda and cd in (torch.float16, torch.bfloat16) else dy @ w2.to(cd)
-        gate, up, dh = _wide(gu[..., :H]), _wide(gu[..., H:]), _wide(dh)
-        a, slope = _act_slope(gate, act)
-        dgu, h = torch.cat([dh * up * slope, dh * a], -1).to(cd), (a * up).to(cd)
-    if dy.is_cuda and cd in (torch.float16, torch.bfloat16):
+        return _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1, b2)
+    dh = linear_bwd.plain(dy, gu[..., :H], w2, empty, ACT_NONE, True, False, False)[0] if native else dy @ w2.to(cd)
+    gate, up, dh = _wide(gu[..., :H]), _wide(gu[..., H:]), _wide(dh)
+    a, slope = _act_slope(gate, act)
+    dgu, h = torch.cat([dh * up * slope, dh * a], -1).to(cd), (a * up).to(cd)
+    if native:
         _, dw2, db2 = linear_bwd.plain(dy, h, w2, empty, ACT_NONE, False, need_dw2, need_db2, b2)
         dx, dw1, db1 = linear_bwd.plain(dgu, x, w1, empty, ACT_NONE, need_dx, need_dw1, need_db1, b1)
         return dx, dw1, db1, dw2, db2
@@ -704,6 +697,41 @@ def gated_mlp_bwd(dy: Tensor, x: Tensor, w1: Tensor, w2: Tensor, gu: Tensor, act
     return tuple(f() if need else dy.new_empty(0) for need, f in (
         (need_dx, lambda: dgu @ w1.to(cd)), (need_dw1, lambda: (d1.t() @ x2).to(w1.dtype)),
         (need_db1, lambda: d1.sum(0)), (need_dw2, lambda: (d2.t() @ h2).to(w2.dtype)), (need_db2, lambda: d2.sum(0))))
+
+
+def _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1, b2):
+    """``gated_mlp_bwd`` by its kernels"""
+    cd, dev = dy.dtype, dy.device
+    x2 = _rows(x if x.dtype == cd else kx.cast(x, cd))
+    out, filled, late = {}, {}, []
+    if need_dx:
+        out["dx"] = torch.empty(x2.shape, dtype=cd, device=dev)
+    for name, w, need, add in (("dw1", w1, need_dw1, "add1"), ("dw2", w2, need_dw2, "add2")):
+        if need:
+            slot = _slot(w)
+            bucket = None if slot is None or slot.main_grad is None else slot.main_grad.view(w.shape)
+            if bucket is not None and bucket.data_ptr() % 16 == 0:
+                out[name], filled[add] = bucket, True
+            else:
+                out[name] = torch.empty(w.shape, dtype=cd if w.dtype == cd and bucket is None else torch.float32,
+                                        device=dev)
+                late.append((name, add, bucket))
+    for name, b, n, need in (("db1", b1, w1.shape[0], need_db1), ("db2", b2, w2.shape[0], need_db2)):
+        if need:
+            bucket = _grad_bucket(b)
+            filled[name] = bucket is not None
+            out[name] = bucket if bucket is not None else torch.zeros(n, dtype=torch.float32, device=dev)
+    kx.gated_mlp_bwd(_rows(dy), x2, _aligned(_weight_as(w1, cd)), _aligned(_weight_as(w2, cd)), _rows(gu), act,
+                     add1=filled.get("add1", False), add2=filled.get("add2", False), **out)
+    for name, add, bucket in late:
+        if bucket is not None:               # a bucket off the 16 bytes that the kernels write
+            bucket.add_(out[name])
+            filled[add] = True
+    kept = lambda name, gone: out[name] if name in out and not gone else dy.new_empty(0)
+    dx = out["dx"].view(x.shape) if need_dx else dy.new_empty(0)
+    dw1, dw2 = (kept(n, filled.get(a, False)) for n, a in (("dw1", "add1"), ("dw2", "add2")))
+    return (dx, dw1.to(w1.dtype), kept("db1", filled.get("db1", False)), dw2.to(w2.dtype),
+            kept("db2", filled.get("db2", False)))
 
 
 @gated_mlp_bwd.register_fake
@@ -758,6 +786,9 @@ def gated_mlp(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: Optio
     if activation not in ("silu", "gelu", "gelu_tanh", "gelu_pytorch_tanh"):
         raise ValueError(f"gated_mlp: unknown activation {activation!r}")
     act = _ACT_NAMES[activation]
+    y = _native_layer("gated_mlp", x, w1, b1, w2, b2, residual, act)
+    if y is not None:
+        return y
     if isinstance(x, Tensor):
         D, rows, N = x.shape[-1] if x.dim() else 0, w1.shape[0], w2.shape[0]
         if w1.dim() != 2 or w2.dim() != 2 or x.dim() < 1 or w1.shape[1] != D or rows != 2 * w2.shape[1] or rows < 2 \
@@ -1486,6 +1517,9 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index
     (fp32 [...])."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
+    loss = _native_layer("linear_cross_entropy", x, weight, target, ignore_index, _REDUCTIONS[reduction])
+    if loss is not None:
+        return loss
     if isinstance(x, Tensor):
         if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
             raise ValueError(f"linear_cross_entropy: x [..., D] and a weight [V, D] are needed, not {tuple(x.shape)} "
@@ -1623,6 +1657,10 @@ def scaled_embedding(ids: Tensor, table: Tensor, scale: float = 1.0, out_dtype: 
     ``embedding``'s, whose sums are atomic."""
     if out_dtype is None:
         out_dtype = compute_dtype(table)
+    if out_dtype in _EMBED_TYPES:
+        y = _native_layer("scaled_embedding", ids, table, float(scale), _lib.dt(out_dtype))
+        if y is not None:
+            return y
     if isinstance(ids, Tensor):
         if table.dim() != 2 or ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool \
                 or ids.device != table.device:

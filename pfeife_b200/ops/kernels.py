@@ -628,36 +628,61 @@ def token_loss_bwd(gout: torch.Tensor, logits: torch.Tensor, labels: torch.Tenso
 
 
 # --------------------------------------------------------------------------- gated feed-forward blocks
-def glu_linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], act: int, keep: bool
-                   ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """x [M, K], w [2H, K] (gate first) -> (h [M, H] = act(gate) * up, both projections [M, 2H] when ``keep``)."""
-    L = _lib.calls()
-    assert x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1] and w.shape[0] % 2 == 0
-    assert x.dtype == w.dtype and x.stride(1) == 1 and w.stride(1) == 1 and w.device == x.device
-    M, H = x.shape[0], w.shape[0] // 2
-    if bias is not None:
-        bias = bias.contiguous()
-        assert bias.shape == (2 * H,) and bias.device == x.device
-    h = torch.empty((M, H), dtype=x.dtype, device=x.device)
-    gu = torch.empty((M, 2 * H), dtype=x.dtype, device=x.device) if keep else None
-    check(L.pf_glu_linear_fwd(x, w, bias, dt(bias.dtype) if bias is not None else 0, h, gu, M, H, x.shape[1],
-                              x.stride(0), w.stride(0), act, dt(x.dtype), status_word(x.device), sm_count(x.device),
-                              stream_of(x)), "pf_glu_linear_fwd")
-    return h, gu
+def _mlp_workspace(L, M: int, D: int, H: int, N: int, device) -> Tuple[Optional[torch.Tensor], int]:
+    kib = L.pf_gated_mlp_scratch(M, D, H, N, sm_count(device))
+    return (torch.empty(kib * 256, dtype=torch.float32, device=device) if kib else None), kib
 
 
-def glu_linear_bwd(dy: torch.Tensor, w2: torch.Tensor, gu: torch.Tensor, act: int
-                   ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """dy [M, K], w2 [K, H], gu [M, 2H] -> (the gradient of gu, h = act(gate) * up once more)"""
+def _packed_bias(b: Optional[torch.Tensor], n: int) -> Tuple[Optional[torch.Tensor], int]:
+    if b is None:
+        return None, 0
+    assert b.shape == (n,)
+    return b.contiguous(), dt(b.dtype)
+
+
+def gated_mlp_fwd(x: torch.Tensor, w1: torch.Tensor, b1: Optional[torch.Tensor], w2: torch.Tensor,
+                  b2: Optional[torch.Tensor], residual: Optional[torch.Tensor], act: int, keep: bool
+                  ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """x [M, D], w1 [2H, D] (gate first), w2 [N, H], residual [M, N], rows on 16 bytes -> (y [M, N], gate and up
+    [M, 2H] when ``keep``)."""
     L = _lib.calls()
+    M, D = x.shape
+    N, H = w2.shape
+    assert w1.shape == (2 * H, D) and x.dtype == w1.dtype == w2.dtype
+    for t in (x, w1, w2, residual):
+        assert t is None or (t.dim() == 2 and t.stride(1) == 1 and t.dtype == x.dtype and t.device == x.device)
+    assert residual is None or residual.shape == (M, N)
+    (b1, t1), (b2, t2) = _packed_bias(b1, 2 * H), _packed_bias(b2, N)
+    new = lambda width: torch.empty((M, width), dtype=x.dtype, device=x.device)
+    h, gu, y = new(H), new(2 * H) if keep else None, new(N)
+    ws, kib = _mlp_workspace(L, M, D, H, N, x.device)
+    check(L.pf_gated_mlp_fwd(x, w1, b1, t1, w2, b2, t2, residual, h, gu, y, ws, kib, M, D, H, N, x.stride(0),
+                             w1.stride(0), w2.stride(0), residual.stride(0) if residual is not None else 0, act,
+                             dt(x.dtype), status_word(x.device), sm_count(x.device), stream_of(x)), "pf_gated_mlp_fwd")
+    return y, gu
+
+
+def gated_mlp_bwd(dy: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, gu: torch.Tensor, act: int, *,
+                  dx: Optional[torch.Tensor] = None, dw1: Optional[torch.Tensor] = None,
+                  dw2: Optional[torch.Tensor] = None, db1: Optional[torch.Tensor] = None,
+                  db2: Optional[torch.Tensor] = None, add1: bool = False, add2: bool = False) -> None:
+    """Writes the gradients whose tensors are given: dx [M, D], dw1 [2H, D] and dw2 [N, H] (added to with add1 and add2,
+    fp32), db1 [2H] and db2 [N] (fp32, added to)."""
+    L = _lib.calls()
+    M, D = x.shape
+    N, H = w2.shape
     gu = _vectors(_like(gu, dy))
-    M, H = gu.shape[0], gu.shape[1] // 2
-    assert dy.shape == (M, w2.shape[0]) and w2.shape[1] == H and w2.dtype == dy.dtype
-    assert dy.stride(1) == 1 and w2.stride(1) == 1
+    assert dy.shape == (M, N) and gu.shape == (M, 2 * H) and w1.shape == (2 * H, D)
+    for t in (dy, x, w1, w2):
+        assert t.dim() == 2 and t.stride(1) == 1 and t.dtype == dy.dtype and t.device == dy.device
+    for t, shape in ((dx, (M, D)), (dw1, (2 * H, D)), (dw2, (N, H)), (db1, (2 * H,)), (db2, (N,))):
+        assert t is None or (t.shape == shape and t.is_contiguous())
     dgu, h = torch.empty_like(gu), torch.empty((M, H), dtype=dy.dtype, device=dy.device)
-    check(L.pf_glu_linear_bwd(dy, w2, gu, dgu, h, M, H, dy.shape[1], dy.stride(0), w2.stride(0), act, dt(dy.dtype),
-                              status_word(dy.device), sm_count(dy.device), stream_of(dy)), "pf_glu_linear_bwd")
-    return dgu, h
+    ws, kib = _mlp_workspace(L, M, D, H, N, dy.device)
+    check(L.pf_gated_mlp_bwd(dy, x, w1, w2, gu, dgu, h, dx, dw1, dw2, db1, db2, ws, kib, M, D, H, N, dy.stride(0),
+                             x.stride(0), w1.stride(0), w2.stride(0), act, dt(dy.dtype),
+                             dt(dw1.dtype) if dw1 is not None else 0, dt(dw2.dtype) if dw2 is not None else 0, int(add1),
+                             int(add2), status_word(dy.device), sm_count(dy.device), stream_of(dy)), "pf_gated_mlp_bwd")
 
 
 # --------------------------------------------------------------------------- output head with its cross entropy

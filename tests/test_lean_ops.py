@@ -616,3 +616,83 @@ def test_shapes_without_data():
     assert torch.equal(a, b)
     for x, y in zip(torch.autograd.grad(a, leaves), torch.autograd.grad(b, leaves)):
         assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", ["embedding", "wide table", "block", "biases", "head", "rows"])
+def test_native_calls_equal_those_through_python(case, monkeypatch):
+    """Eager calls and their backwards in C++: the same bits, and no Python on the way."""
+    from pfeife_b200.ops import _lib
+    if _lib.eager() is None:
+        pytest.skip("the module of eager calls is not built")
+    new = lambda *s, seed: normal(*s, device="cuda", dtype=torch.bfloat16, seed=seed, std=0.5)
+    ids, labels = _data("cuda", 3)
+    if case in ("embedding", "wide table"):
+        table = new(50, 24, seed=1).to(torch.float32 if case == "wide table" else torch.bfloat16).requires_grad_()
+        leaves, call = [table], lambda: ops.scaled_embedding(ids.view(7, 10), table, 3.0, out_dtype=torch.bfloat16)
+    elif case in ("block", "biases"):
+        leaves = [new(*s, seed=i).requires_grad_() for i, s in enumerate(((7, 10, 32), (96, 32), (40, 48), (7, 10, 40)))]
+        b1, b2 = (new(n, seed=n).requires_grad_() if case == "biases" else None for n in (96, 40))
+        x, w1, w2, res = leaves
+        leaves = leaves + [b for b in (b1, b2) if b is not None]
+        call = lambda: ops.gated_mlp(x, w1, b1, w2, b2, "gelu", res)
+    else:
+        leaves = [new(*s, seed=i).requires_grad_() for i, s in enumerate(((7, 10, 32), (50, 32)))]
+        call = lambda: ops.linear_cross_entropy(*leaves, labels.view(7, 10),
+                                                reduction="none" if case == "rows" else "mean")
+
+    def both():
+        y = call()
+        return (y, *torch.autograd.grad(y, leaves, torch.ones_like(y)))
+    before = _lib._eager.launches()
+    native = both()
+    assert _lib._eager.launches() > before + 1
+    launches = _lib._launches
+    both()
+    assert _lib._launches == launches                     # none went through Python
+    with torch.no_grad():
+        assert torch.equal(call(), native[0])
+    monkeypatch.setattr(_lib, "_eager", None)
+    monkeypatch.setattr(_lib, "eager", lambda: None)
+    for a, b in zip(native, both()):
+        assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_saved_tensors_may_come_back_otherwise():
+    """Hooks that unpack what was saved in another place or order of memory, in C++ and through Python."""
+    from pfeife_b200.ops import _lib
+    leaves, run = _all("cuda", torch.bfloat16)
+    ids, labels = _data("cuda", 10)
+    want = torch.autograd.grad(run(ids, labels), leaves)
+
+    def moved(t):
+        if t.dim() == 2 and t.is_floating_point():
+            big = torch.empty(t.shape[1], t.shape[0] + 1, dtype=t.dtype, device=t.device)
+            big[:, 1:] = t.t()
+            return big[:, 1:].t()                         # the same values, columns innermost and off their vectors
+        return t.clone()
+    for through in ("C++", "Python"):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, moved):
+            if through == "Python":
+                held, _lib._eager = _lib._eager, None
+                tried, _lib.eager = _lib.eager, lambda: None
+            try:
+                got = torch.autograd.grad(run(ids, labels), leaves)
+            finally:
+                if through == "Python":
+                    _lib._eager, _lib.eager = held, tried
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_checkpoints_and_second_backwards():
+    from torch.utils.checkpoint import checkpoint
+    leaves, run = _all("cuda", torch.bfloat16)
+    ids, labels = _data("cuda", 10)
+    loss = run(ids, labels)
+    want = torch.autograd.grad(loss, leaves, retain_graph=True)
+    again = torch.autograd.grad(loss, leaves)
+    through = torch.autograd.grad(checkpoint(run, ids, labels, use_reentrant=False), leaves)
+    for a, b, c in zip(want, again, through):
+        assert torch.equal(a, b) and torch.equal(a, c)
