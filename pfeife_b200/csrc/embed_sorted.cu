@@ -4,10 +4,12 @@
 //
 // Both are bound by memory: forward the rows that are named and the output, backward dout and the whole gradient
 // table, most of whose rows are zeros.  Sums go over the tokens in their order (the sort is stable) in 32 bits, in
-// windows of the sorted tokens: a run of one id inside a window is written at once, one that crosses windows
-// leaves a part in each, which are added in their order.  So the same tokens give the same bits, a row is written
-// once and rounded once, and a padding token that a third of the batch shares is summed by as many CTAs as it has
-// windows.  Ids outside the table have zeros and no gradient.
+// windows of the sorted tokens: a run of one id is summed and written by the window in which it starts, unless it is
+// longer than several windows; then every window leaves its part, and the parts are added in their order.  So the same
+// tokens give the same bits, a row is written once and rounded once, and a padding token that a third of the batch
+// shares is summed by as many CTAs as it has windows.  Ids outside the table have zeros and no gradient.
+#include <algorithm>
+#include <type_traits>
 #include "common.cuh"
 #include "api.h"
 
@@ -45,43 +47,54 @@ template <typename T, int V> struct Vec {
     }
   }
 };
+// the same as it was loaded: 16-bit values stay packed until they are added
+template <typename T, int V> struct Raw {
+  static constexpr bool PACKED = V == 8 && sizeof(T) == 2;
+  typename std::conditional<PACKED, uint4, Vec<T, V>>::type q;
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (PACKED) q = __ldg(reinterpret_cast<const uint4*>(p));
+    else q.load(p);
+  }
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (PACKED) return to_f32<T>(reinterpret_cast<const T*>(&q)[j]);
+    else return q.v[j];
+  }
+};
 // whether rows of D values start on the 8-value accesses of their type
 static bool on_rows(const void* p, int D, int dtype) {
   return D % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & (dtype == PF_F32 ? 31 : 15)) == 0;
 }
 
-// Four vectors of V values a thread, requested before any is written.
+// 2^lanes_log threads a row, up to eight vectors of V values each requested before any is written.
 template <typename TT, typename T, int V>
 __global__ void __launch_bounds__(256)
 scaled_embed_kernel(const TT* __restrict__ table, const long long* __restrict__ ids, T* __restrict__ out,
-                    long long total, int per_row, int D, long long words, float scale) {
+                    long long tokens, int lanes_log, int D, long long words, float scale) {
   after_previous();
-  constexpr int U = 4;
-  const long long i0 = blockIdx.x * (256ll * U) + threadIdx.x;
-  Vec<TT, V> q[U];
+  constexpr int U = V == 8 && sizeof(TT) == 4 ? 4 : 8;
+  const long long t = ((long long)blockIdx.x * 256 + threadIdx.x) >> lanes_log;
+  if (t >= tokens) return;
+  const long long id = __ldg(ids + t);
+  const bool there = id >= 0 && id < words;
+  const int step = V << lanes_log;
+  const TT* src = table + (there ? id : 0) * D;
+  T* dst = out + t * D;
+  for (int c0 = (threadIdx.x & ((1 << lanes_log) - 1)) * V; c0 < D; c0 += U * step) {
+    Raw<TT, V> q[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const long long i = i0 + u * 256;
-    if (i < total) {
-      const long long t = total <= 0x7fffffffll ? (unsigned)i / (unsigned)per_row : i / per_row;
-      const long long id = ids[t];
-      const int c = (int)(i - t * per_row) * V;
-      if (id >= 0 && id < words) {
-        q[u].load(table + id * D + c);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) q[u].v[j] = 0.f;
-      }
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * step;
+      if (c < D && there) q[u].load(src + c);
     }
-  }
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const long long i = i0 + u * 256;
-    if (i < total) {
-      Vec<T, V> r;
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * step;
+      if (c < D) {
+        Vec<T, V> r;
 #pragma unroll
-      for (int j = 0; j < V; ++j) r.v[j] = q[u].v[j] * scale;
-      r.store(out + i * V);                             // rows of D = per_row V values, packed
+        for (int j = 0; j < V; ++j) r.v[j] = there ? q[u].at(j) * scale : 0.f;
+        r.store(dst + c);
+      }
     }
   }
 }
@@ -95,13 +108,14 @@ constexpr int SORT_SMEM = (SORT_WARPS * SORT_BINS + 2 * SORT_BINS + 64) * 4;
 template <int CTAS>
 __global__ void __launch_bounds__(SORT_THREADS)
 sort_tokens_kernel(const long long* __restrict__ ids, int N, int words, int bits, int passes, int* __restrict__ order,
-                   int* __restrict__ other, int* __restrict__ keys, unsigned* __restrict__ present) {
+                   int* __restrict__ other, int* __restrict__ keys, int2* __restrict__ runs) {
   extern __shared__ int sort_smem[];
   int* counts = sort_smem;                              // [warp][bin]
   int* totals = counts + SORT_WARPS * SORT_BINS;        // [bin], read by the other CTAs
   int* starts = totals + SORT_BINS;
   int* sums = starts + SORT_BINS;
   after_previous();
+  let_next_start();                                     // zeros for the table, which need nothing of this
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CTAS > 1 ? (int)cluster_ctarank() : 0;
   const int bins = 1 << bits;
@@ -109,7 +123,6 @@ sort_tokens_kernel(const long long* __restrict__ ids, int N, int words, int bits
   const int per_warp = ((N + CTAS * SORT_WARPS - 1) / (CTAS * SORT_WARPS) + 31) / 32 * 32;
   const long long lo = (long long)(rank * SORT_WARPS + warp) * per_warp;
   const int begin = (int)(lo < N ? lo : N), end = (int)(lo + per_warp < N ? lo + per_warp : N);
-  for (int i = rank * SORT_THREADS + threadIdx.x; i < (words + 31) / 32; i += CTAS * SORT_THREADS) present[i] = 0;
   auto key_of = [&](int t) {
     const long long id = __ldg(ids + t);
     return id >= 0 && id < words ? (int)id : words;     // ids outside the table come last
@@ -200,10 +213,7 @@ sort_tokens_kernel(const long long* __restrict__ ids, int N, int words, int bits
         if (in) {
           const int to = mine[digit] + __popc(same & ((1u << lane) - 1));
           __stcg(dst + to, tok[u]);
-          if (pass == passes - 1) {
-            keys[to] = key[u];
-            if (key[u] < words) atomicOr(present + (key[u] >> 5), 1u << (key[u] & 31));
-          }
+          if (pass == passes - 1) __stcg(keys + to, key[u]);
         }
         __syncwarp();
         if (in && lane == __ffs(same) - 1) mine[digit] += __popc(same);
@@ -212,20 +222,39 @@ sort_tokens_kernel(const long long* __restrict__ ids, int N, int words, int bits
     }
     all_sync();
   }
+  // where the run of each id starts and ends
+#pragma unroll 4
+  for (int i = rank * SORT_THREADS + threadIdx.x; i < N; i += CTAS * SORT_THREADS) {
+    const int key = __ldcg(keys + i);
+    const int left = i > 0 ? __ldcg(keys + i - 1) : -1, right = i < N - 1 ? __ldcg(keys + i + 1) : -1;
+    if (key < words && left != key) runs[key].x = i;
+    if (key < words && right != key) runs[key].y = i + 1;
+  }
+}
+
+// Zeros for a table's gradient, 16 bytes a thread and store, beside the sort: rows that tokens name are written again
+// behind both.
+__global__ void __launch_bounds__(512)
+table_zeros_kernel(uint4* __restrict__ dst, long long n, unsigned char* __restrict__ tail, int bytes) {
+  const long long i0 = (long long)blockIdx.x * (512 * 8) + threadIdx.x;
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+    if (i0 + u * 512 < n) dst[i0 + u * 512] = make_uint4(0, 0, 0, 0);
+  if (blockIdx.x == 0 && (int)threadIdx.x < bytes) tail[threadIdx.x] = 0;
+  if (blockIdx.x == gridDim.x - 1) after_previous();    // what comes next finds the sort completed, too
 }
 
 // Sums of windows of the sorted tokens.  `lanes` threads (a power of two) share a row of V-wide vectors, 128 / lanes
-// windows a CTA; CTAs behind those of the windows write zeros to rows that no token names.
+// windows a CTA.
 struct TableGrad {
   const int* keys;
   const int* order;
-  const unsigned* present;
+  const int2* runs;
   int N, words, D, window, lanes_log, slices;
-  unsigned work_ctas;
-  int zero_rows;                // rows of a CTA that writes zeros
   float scale;
   int accumulate;
-  float* parts;                 // [window][2][D]: of the run that came in, of the run that goes on
+  float* parts;                 // [window][2][D]: of a long run that came in, of one that goes on
+  int most;                     // tokens of a run that is not long
 };
 
 template <typename TT, int V>
@@ -246,39 +275,43 @@ template <typename T, typename TT, int V>
 __global__ void __launch_bounds__(128)
 table_grad_kernel(const T* __restrict__ dout, TT* __restrict__ dtable, const TableGrad p) {
   after_previous();
-  constexpr int U = V == 1 ? 8 : 4;
-  if (blockIdx.x >= p.work_ctas) {
-    const long long r0 = (blockIdx.x - p.work_ctas) * (long long)p.zero_rows;
-    const long long r1 = r0 + p.zero_rows < p.words ? r0 + p.zero_rows : p.words;
-    Vec<TT, V> zero;
-#pragma unroll
-    for (int j = 0; j < V; ++j) zero.v[j] = 0.f;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (long long r = r0 + warp; r < r1; r += 4) {
-      if (p.present[r >> 5] >> (r & 31) & 1) continue;
-      TT* dst = dtable + r * p.D;
-      for (int c = lane * V; c < p.D; c += 32 * V) zero.store(dst + c);
-    }
-    return;
-  }
+  constexpr int U = V == 8 && sizeof(T) == 4 ? 4 : 8;
   const int lanes = 1 << p.lanes_log;
   const int slice = blockIdx.x % p.slices;
   const long long w = (long long)(blockIdx.x / p.slices) * (128 >> p.lanes_log) + (threadIdx.x >> p.lanes_log);
   const long long b = w * p.window;
   const int c = (slice * lanes + (threadIdx.x & (lanes - 1))) * V;
   if (b >= p.N || c >= p.D) return;
-  const int begin = (int)b, end = min(p.N, begin + p.window);
+  int begin = (int)b, end = min(p.N, begin + p.window);
+  int run = p.keys[begin];
+  if (run >= p.words) return;                           // ids outside the table come last
+  bool came_in = false, goes_on = false;                // a long run that another window starts, or ends
+  const int2 first = p.runs[run];
+  if (first.x < begin) {
+    if (first.y - first.x > p.most) came_in = true;
+    else begin = first.y;                               // summed where it starts
+    if (begin >= end) return;
+    run = p.keys[begin];
+  }
+  const int tail = p.keys[end - 1];
+  if (tail < p.words) {
+    const int2 last = p.runs[tail];
+    if (last.y > end && (last.x >= begin || came_in)) {
+      if (last.y - last.x > p.most) goes_on = true;
+      else end = last.y;
+    }
+  }
   float acc[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
-  int run = p.keys[begin];
-  bool came_in = begin > 0 && p.keys[begin - 1] == run;
   float* part = p.parts + w * 2 * p.D + c;
   auto done = [&]() {                                   // the run has ended inside the window
     if (run >= p.words) return;
     if (came_in) {
+      Vec<float, V> r;
 #pragma unroll
-      for (int j = 0; j < V; ++j) part[j] = acc[j];
+      for (int j = 0; j < V; ++j) r.v[j] = acc[j];
+      r.store(part);
     } else {
       Vec<TT, V> r;
 #pragma unroll
@@ -288,7 +321,7 @@ table_grad_kernel(const T* __restrict__ dout, TT* __restrict__ dtable, const Tab
   };
   for (int e = begin; e < end; e += U) {
     int key[U];
-    Vec<T, V> q[U];
+    Raw<T, V> q[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       key[u] = e + u < end ? p.keys[e + u] : p.words;
@@ -306,46 +339,35 @@ table_grad_kernel(const T* __restrict__ dout, TT* __restrict__ dtable, const Tab
         }
         if (run < p.words) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) acc[j] += q[u].v[j];
+          for (int j = 0; j < V; ++j) acc[j] += q[u].at(j);
         }
       }
     }
   }
-  const bool goes_on = end < p.N && p.keys[end] == run;
   if (goes_on && !came_in) {
-    if (run < p.words) {
+    Vec<float, V> r;
 #pragma unroll
-      for (int j = 0; j < V; ++j) part[p.D + j] = acc[j];
-    }
+    for (int j = 0; j < V; ++j) r.v[j] = acc[j];
+    r.store(part + p.D);
   } else {
     done();                                             // a run through the whole window leaves its part as one that came in
   }
 }
 
-// Runs that cross windows: the window in which one starts adds up its parts, JOIN_GROUPS neighbouring stretches of them
-// side by side and then those.  A CTA has one window's slice of a row.
+// Long runs: their parts are added up, JOIN_GROUPS neighbouring stretches of them side by side and then those.  A long
+// run holds a multiple of `most`, and is found by the first that it holds.  A CTA has a slice of a row.
 constexpr int JOIN_GROUPS = 8;
 template <typename TT, int V>
 __global__ void __launch_bounds__(128 * JOIN_GROUPS)
 table_join_kernel(TT* __restrict__ dtable, const TableGrad p) {
   after_previous();
   __shared__ float sums[JOIN_GROUPS][128 * V];
-  const int slice = blockIdx.x % p.slices, w = blockIdx.x / p.slices;
-  const int b = w * p.window, e = b + p.window;         // in range: only windows before the last are dealt
-  const int run = p.keys[e - 1];
-  if (run >= p.words || p.keys[e] != run) return;
-  if (b > 0 && p.keys[b] == run && p.keys[b - 1] == run) return;         // it started further ahead
-  // the first token behind the run, by 32 looks at a time
-  const int lane = threadIdx.x & 31;
-  int lo = e, hi = p.N;
-  while (lo < hi) {
-    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-    const int n = __popc(__ballot_sync(0xffffffffu, at < hi && p.keys[at] == run));
-    if (n == 0) break;
-    hi = min(hi, lo + n * step);
-    lo = lo + (n - 1) * step + 1;
-  }
-  const int last = (lo - 1) / p.window;
+  const int slice = blockIdx.x % p.slices, at = blockIdx.x / p.slices * p.most;         // at < N
+  const int run = p.keys[at];
+  if (run >= p.words) return;
+  const int2 range = p.runs[run];
+  if (range.y - range.x <= p.most || at - range.x >= p.most) return;
+  const int w = range.x / p.window, last = (range.y - 1) / p.window;
   const int group = threadIdx.x >> 7, x = threadIdx.x & 127, c = (slice * 128 + x) * V;
   const int n = last - w, each = (n + JOIN_GROUPS - 1) / JOIN_GROUPS;
   const bool mine = c < p.D;
@@ -355,24 +377,22 @@ table_join_kernel(TT* __restrict__ dtable, const TableGrad p) {
   if (mine) {
     const float* src = p.parts + c;
     const long long size = 2ll * p.D;
+    Vec<float, V> q[8];
     if (group == 0) {
+      q[0].load(src + w * size + p.D);
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[j] = src[w * size + p.D + j];
+      for (int j = 0; j < V; ++j) s[j] = q[0].v[j];
     }
     const int k1 = w + 1 + min(n, (group + 1) * each);
-    for (int k = w + 1 + group * each; k < k1; k += 4) {
-      float q[4][V];
+    for (int k = w + 1 + group * each; k < k1; k += 8) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 8; ++u)
+        if (k + u < k1) q[u].load(src + (k + u) * size);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
         if (k + u < k1) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) q[u][j] = src[(k + u) * size + j];
-        }
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (k + u < k1) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) s[j] += q[u][j];
+          for (int j = 0; j < V; ++j) s[j] += q[u].v[j];
         }
     }
   }
@@ -390,7 +410,7 @@ table_join_kernel(TT* __restrict__ dtable, const TableGrad p) {
 }
 
 template <int CTAS>
-static int launch_sort(const long long* ids, int N, int words, int* order, int* other, int* keys, unsigned* present,
+static int launch_sort(const long long* ids, int N, int words, int* order, int* other, int* keys, int2* runs,
                        cudaStream_t st) {
   auto kern = sort_tokens_kernel<CTAS>;
   static bool configured[64] = {};
@@ -417,8 +437,8 @@ static int launch_sort(const long long* ids, int N, int words, int* order, int* 
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return (int)LaunchAfter<const long long*, int, int, int, int, int*, int*, int*, unsigned*>{kern, cfg}(
-      ids, N, words, per_pass, passes, order, other, keys, present);
+  return (int)LaunchAfter<const long long*, int, int, int, int, int*, int*, int*, int2*>{kern, cfg}(
+      ids, N, words, per_pass, passes, order, other, keys, runs);
 }
 
 }  // namespace pf
@@ -429,10 +449,10 @@ static bool embed_sizes_ok(long long N, long long words, int D) {
   return N >= 0 && N <= (1ll << 30) && words >= 0 && words < (1ll << 30) && D >= 0;
 }
 
-// tokens of a window: some 2000 CTAs' worth, at least 8 and at most 256
+// tokens of a window: some 4000 CTAs' worth, at least 8 and at most 128
 static int window_of(long long N, int per_cta_slices) {
-  long long w = N * per_cta_slices / 2048;
-  return (int)(w < 8 ? 8 : w > 256 ? 256 : w);
+  long long w = N * per_cta_slices / 4096;
+  return (int)(w < 8 ? 8 : w > 128 ? 128 : w);
 }
 
 struct EmbedPlan {
@@ -460,17 +480,19 @@ PF_API int pf_scaled_embed_fwd(const void* table, const void* ids, void* out, lo
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool vec = on_rows(table, D, table_dtype) && on_rows(out, D, out_dtype);
   const int per_row = vec ? D / 8 : D;
-  const long long total = tokens * per_row, ctas = (total + 1023) / 1024;
+  int lanes_log = 0;
+  while (lanes_log < 5 && (1 << lanes_log) < per_row) ++lanes_log;
+  const long long ctas = ((tokens << lanes_log) + 255) / 256;
   if (ctas > 0x7fffffffll) return -3;
   const long long* I = (const long long*)ids;
 #define PF_FWD(TD, TT_, OD, OT_)                                                                                       \
   if (table_dtype == TD && out_dtype == OD) {                                                                          \
     if (vec)                                                                                                           \
-      after(scaled_embed_kernel<TT_, OT_, 8>, (unsigned)ctas, 256, 0, st)((const TT_*)table, I, (OT_*)out, total,      \
-                                                                          per_row, D, words, scale);                   \
+      after(scaled_embed_kernel<TT_, OT_, 8>, (unsigned)ctas, 256, 0, st)((const TT_*)table, I, (OT_*)out, tokens,     \
+                                                                          lanes_log, D, words, scale);                 \
     else                                                                                                               \
-      after(scaled_embed_kernel<TT_, OT_, 1>, (unsigned)ctas, 256, 0, st)((const TT_*)table, I, (OT_*)out, total,      \
-                                                                          per_row, D, words, scale);                   \
+      after(scaled_embed_kernel<TT_, OT_, 1>, (unsigned)ctas, 256, 0, st)((const TT_*)table, I, (OT_*)out, tokens,     \
+                                                                          lanes_log, D, words, scale);                 \
   } else
   PF_FWD(PF_F32, float, PF_F32, float)
   PF_FWD(PF_F32, float, PF_F16, __half)
@@ -488,7 +510,7 @@ PF_API int pf_scaled_embed_scratch(long long tokens, int D, long long words) {
   if (!embed_sizes_ok(tokens, words, D)) return -3;
   const EmbedPlan a = embed_plan(tokens, D, true), b = embed_plan(tokens, D, false);
   const long long windows = a.windows > b.windows ? a.windows : b.windows;
-  const long long bytes = tokens * 12 + (words + 31) / 32 * 4 + windows * 2 * D * 4 + 64;
+  const long long bytes = tokens * 12 + (words + 3) / 4 * 32 + windows * 2 * D * 4 + 64;
   const long long kib = (bytes + 1023) / 1024;
   return kib > 0x7fffffffll ? -3 : (int)kib;
 }
@@ -505,27 +527,40 @@ PF_API int pf_scaled_embed_bwd(const void* dout, const void* ids, void* dtable, 
   const EmbedPlan g = embed_plan(tokens, D, vec);
   TableGrad p;
   const int N = (int)tokens;
-  p.parts = static_cast<float*>(scratch);
+  int2* runs = static_cast<int2*>(scratch);
+  p.parts = reinterpret_cast<float*>(runs + (words + 3) / 4 * 4);       // 32 bytes for vectors of 8
   int* keys = reinterpret_cast<int*>(p.parts + g.windows * 2 * D);
   int* order = keys + N;
   int* other = order + N;
-  unsigned* present = reinterpret_cast<unsigned*>(other + N);
   // one CTA where a second or two of its rounds are all there is
-  const int r = N <= 4096 ? launch_sort<1>((const long long*)ids, N, (int)words, order, other, keys, present, st)
-                          : launch_sort<8>((const long long*)ids, N, (int)words, order, other, keys, present, st);
+  const int r = N <= 4096 ? launch_sort<1>((const long long*)ids, N, (int)words, order, other, keys, runs, st)
+                          : launch_sort<8>((const long long*)ids, N, (int)words, order, other, keys, runs, st);
   if (r) return r;
-  p.keys = keys; p.order = order; p.present = present;
+  p.keys = keys; p.order = order; p.runs = runs; p.most = std::max(64, 4 * g.window);
   p.N = N; p.words = (int)words; p.D = D; p.window = g.window; p.lanes_log = g.lanes_log; p.slices = g.slices;
   p.scale = scale; p.accumulate = accumulate;
   const int per_cta = 128 >> g.lanes_log;
   const long long work = (g.windows + per_cta - 1) / per_cta * g.slices;
-  p.zero_rows = (int)(words / 2048 < 4 ? 4 : words / 2048);
-  const long long zeros = accumulate ? 0 : (words + p.zero_rows - 1) / p.zero_rows;
-  if (work + zeros > 0x7fffffffll) return -3;
-  p.work_ctas = (unsigned)work;
-  const unsigned grid = (unsigned)(work + zeros);
+  if (work > 0x7fffffffll) return -3;
+  if (!accumulate) {
+    const size_t bytes = (size_t)words * D * (table_dtype == PF_F32 ? 4 : 2);
+    // up to the first 16 bytes, and behind the last: a table that is a view may start anywhere
+    char* at = static_cast<char*>(dtable);
+    const size_t head = std::min(bytes, (16 - (reinterpret_cast<uintptr_t>(at) & 15)) & 15);
+    if (head) {
+      cudaError_t e = cudaMemsetAsync(at, 0, head, st);
+      if (e != cudaSuccess) return (int)e;
+    }
+    const long long n = (long long)((bytes - head) / 16), zeros = std::max(1ll, (n + 4095) / 4096);
+    if (zeros > 0x7fffffffll) return -3;
+    after(table_zeros_kernel, (unsigned)zeros, 512, 0, st)(reinterpret_cast<uint4*>(at + head), n,
+        reinterpret_cast<unsigned char*>(at + head + n * 16), (int)((bytes - head) & 15));
+    PF_CHECK_LAUNCH();
+  }
+  if (N == 0) return 0;
+  const unsigned grid = (unsigned)work;
   const int join_slices = (D + 128 * g.V - 1) / (128 * g.V);
-  const long long joins = (g.windows - 1) * join_slices;         // a run that crosses starts before the last window
+  const long long joins = N > p.most ? (long long)((N + p.most - 1) / p.most) * join_slices : 0;
   if (joins > 0x7fffffffll) return -3;
   TableGrad pj = p;
   pj.slices = join_slices;
