@@ -377,19 +377,19 @@ table_join_kernel(TT* __restrict__ dtable, const TableGrad p) {
   if (mine) {
     const float* src = p.parts + c;
     const long long size = 2ll * p.D;
-    Vec<float, V> q[8];
+    Vec<float, V> q[4];
     if (group == 0) {
       q[0].load(src + w * size + p.D);
 #pragma unroll
       for (int j = 0; j < V; ++j) s[j] = q[0].v[j];
     }
     const int k1 = w + 1 + min(n, (group + 1) * each);
-    for (int k = w + 1 + group * each; k < k1; k += 8) {
+    for (int k = w + 1 + group * each; k < k1; k += 4) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+      for (int u = 0; u < 4; ++u)
         if (k + u < k1) q[u].load(src + (k + u) * size);
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+      for (int u = 0; u < 4; ++u)
         if (k + u < k1) {
 #pragma unroll
           for (int j = 0; j < V; ++j) s[j] += q[u].v[j];
