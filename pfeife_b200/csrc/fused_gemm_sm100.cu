@@ -40,7 +40,7 @@ struct FusedSmem {
   static constexpr int HC = JOB == GLU_FWD ? 32 : 64;               // output columns of a warp
   static constexpr int BW = sizeof(OutT) == 4 || JOB == GLU_FWD || JOB == GLU_BWD ? 32 : 64;
   static constexpr int BOX = 32 * BW * sizeof(OutT);
-  static constexpr int BOXES = JOB == GLU_BWD ? 2 : JOB == HEAD_STATS ? 0 : 1;
+  static constexpr int BOXES = JOB == GLU_FWD || JOB == GLU_BWD ? 2 : JOB == HEAD_STATS ? 0 : 1;
   static constexpr int PER_WARP = BOXES * BOX;
   static constexpr int STAGING = epi_warps(PAIR) * PER_WARP;
   static constexpr int STAGES = STAGING <= 32768 ? 6 : 5;
@@ -145,7 +145,9 @@ __device__ __forceinline__ void add_bias_of(const B* b, int n, float (&v)[W]) {
       const uint4 q = __ldg(reinterpret_cast<const uint4*>(b) + c);
       const B* e = reinterpret_cast<const B*>(&q);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) v[c * PER + j] += to_f32<B>(e[j]);
+      for (int j = 0; j < PER; j += 2)
+        f2_unpack(add2(f2_pack(v[c * PER + j], v[c * PER + j + 1]), f2_pack(to_f32<B>(e[j]), to_f32<B>(e[j + 1]))),
+                  v[c * PER + j], v[c * PER + j + 1]);
     }
   } else {
 #pragma unroll
@@ -474,18 +476,7 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
         uint32_t raw[32];
         float v[32];
         if constexpr (JOB == GLU_FWD) {
-          // to be kept: gate, then up, as they are; registers hold no more than 32 columns of both at a time
-          if (p.save) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              tmem_ld32(t_row + half * NT + c, raw);
-              tmem_ld_wait_for(raw);
-              values(raw, v);
-              add_bias(p.bias, p.bias_dtype, half * p.N + col, p.N - col, v);
-              fill_box<OutT, RB>(boxes, lane, 0, v);
-              store(boxes, static_cast<OutT*>(p.two) + half * p.N, 2ll * p.N, col, row0, M);
-            }
-          }
+          uint4 hq[4];                                  // h, which takes the place of the gate once that is stored
 #pragma unroll
           for (int s = 0; s < 32; s += 16) {
             uint32_t gate[16], up[16];
@@ -502,6 +493,20 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
             }
             add_bias(p.bias, p.bias_dtype, col + s, p.N - col - s, g);
             add_bias(p.bias, p.bias_dtype, p.N + col + s, p.N - col - s, u);
+            auto packed = [&](const float (&v)[16], int k) {
+              uint4 q;
+              OutT* e = reinterpret_cast<OutT*>(&q);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) e[j] = from_f32<OutT>(v[8 * k + j]);
+              return q;
+            };
+            if (p.save) {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                *box_at<RB>(boxes, lane, s / 8 + k) = packed(g, k);
+                *box_at<RB>(boxes + S::BOX, lane, s / 8 + k) = packed(u, k);
+              }
+            }
             auto all = [&](auto kind) {
 #pragma unroll
               for (int i = 0; i < 16; i += 2) {
@@ -513,15 +518,15 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
             if (p.act == 1) all(std::integral_constant<int, 1>());
             else if (p.act == 2) all(std::integral_constant<int, 2>());
             else all(std::integral_constant<int, 3>());
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              uint4 q;
-              OutT* e = reinterpret_cast<OutT*>(&q);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) e[j] = from_f32<OutT>(g[8 * k + j]);
-              *box_at<RB>(boxes, lane, s / 8 + k) = q;
-            }
+            hq[s / 8] = packed(g, 0);
+            hq[s / 8 + 1] = packed(g, 1);
           }
+          if (p.save) {
+            store(boxes, p.two, 2ll * p.N, col, row0, M);
+            store(boxes + S::BOX, static_cast<OutT*>(p.two) + p.N, 2ll * p.N, col, row0, M);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) *box_at<RB>(boxes, lane, k) = hq[k];
           store(boxes, p.C, p.ldc, col, row0, M);
         } else if constexpr (JOB == GLU_BWD) {
           uint8_t *gbox = boxes, *ubox = boxes + S::BOX;
