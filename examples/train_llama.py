@@ -19,7 +19,7 @@ from common import (DevicePrefetcher, SyntheticDataset, TensorFileDataset, add_t
                     make_loader, option_from_args, train_loop)
 
 from pfeife_b200 import PartialRunner, initialize_pfeife, partial_compiler
-from pfeife_b200.models.llama import Llama, causal_lm_loss, llama_config
+from pfeife_b200.models.llama import Llama, causal_lm_loss, llama_config, next_tokens
 from pfeife_b200.utils import set_seed
 
 
@@ -53,6 +53,9 @@ def main():
     parser.add_argument("--tie_embeddings", action="store_true",
                         help="share the embedding with the output projection (its gradient is then "
                              "summed across the stages that hold a copy)")
+    parser.add_argument("--lean", action="store_true",
+                        help="keep less between forward and backward: gated feed-forward blocks as one operator, and the "
+                             "head with its loss without the logits")
     parser.add_argument("--lr_scheduler_type", default="linear", choices=["linear", "constant"])
     parser.add_argument("--num_warmup_steps", type=int, default=0)
     add_train_arguments(parser)
@@ -65,7 +68,8 @@ def main():
     option = option_from_args(args)
     set_seed(args.seed)
 
-    over = {"max_seq_len": args.block_size, "tie_embeddings": args.tie_embeddings}
+    over = {"max_seq_len": args.block_size, "tie_embeddings": args.tie_embeddings,
+            "fused_mlp": args.lean}
     if args.num_layers:
         over["num_layers"] = args.num_layers
     cfg = llama_config(args.model, **over)
@@ -88,7 +92,10 @@ def main():
     cmodel = torch.compile(model, backend=partial_compiler)
 
     def iter_fn(input_ids):
-        loss = causal_lm_loss(cmodel(input_ids), input_ids)
+        if args.lean:
+            loss = cmodel(input_ids, next_tokens(input_ids))
+        else:
+            loss = causal_lm_loss(cmodel(input_ids), input_ids)
         runner.scaler.scale(loss).backward()
         return loss.detach()
 

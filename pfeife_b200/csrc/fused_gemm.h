@@ -45,6 +45,7 @@ struct FusedCall {
   float unit = 1.f;
   int split = 1;               // PARTS: parts of the reduction, part i in rows i * part_rows of C on
   int part_rows = 0;
+  int tile = -1;               // 1: tiles of CTA pairs, 0: of one CTA; -1: as fused_pairs has it
   int accumulate = 0;          // PARTS, HEAD_DW in fp32: add to C
   const float* scale = nullptr;    // HEAD_DW: *scale times *scale2 (where given) times scale3
   const float* scale2 = nullptr;
@@ -58,6 +59,10 @@ constexpr int HEAD_PART = 64;      // words of a part of HEAD_STATS
 
 // 256 x 256 tiles of CTA pairs instead of 128 x 128 ones
 bool fused_pairs(Job job, long long M, long long N, int sm_count);
+// Tiles and parts that a product [M, N] over K is best split into; `joined`: its parts are read by a pass that would
+// follow in any case.
+struct PartPlan { int pair = 0, parts = 1; };
+PartPlan plan_parts(long long M, long long N, long long K, int sm_count, bool joined);
 int fused_gemm(Job job, const FusedCall& c);
 
 }  // namespace pf

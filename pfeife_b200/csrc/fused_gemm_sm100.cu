@@ -748,10 +748,38 @@ static int launch_fused(const FusedMaps& maps, const FusedParams& p, int sm_coun
 bool fused_pairs(Job job, long long M, long long N, int sm_count) {
   if (sm_count < 2) return false;
   const long long nt = job == GLU_FWD ? 128 : 256;
-  // rounds of pair tiles over half as many pairs as SMs against rounds of single tiles, which take 0.55 of as long
+  // rounds of pair tiles over half as many pairs as SMs against rounds of single tiles (see plan_parts)
   const long long t2 = ((M + 255) / 256) * ((N + nt - 1) / nt), t1 = ((M + 127) / 128) * ((2 * N + nt - 1) / nt);
   const long long w2 = (t2 + sm_count / 2 - 1) / (sm_count / 2), w1 = (t1 + sm_count - 1) / sm_count;
-  return 93 * w2 <= 55 * w1;
+  return 37 * w2 <= 25 * w1;
+}
+
+// In microseconds, as measured: a k-block of 64 costs a pair's tile 0.37 and a single one 0.25, or what memory brings of B
+// (5.5 TB/s over all that run at once; tiles of one column share it); an item costs 1.5 more of them, parts their way
+// through memory and a launch.  (2048 x 4096 outputs never gain by it; over 22016: 512 rows whole 101, in two parts over
+// pairs 72; 256 rows 97 and in four 46; 13 rows 115 and in 13 over single tiles 43.)
+PartPlan plan_parts(long long M, long long N, long long K, int sm_count, bool joined) {
+  PartPlan best;
+  double least = 1e30;
+  const long long kb = (K + FG_BK - 1) / FG_BK;
+  for (int pair = 0; pair <= (M > FG_BM && sm_count >= 2); ++pair) {
+    const long long bt = pair ? 2 * FG_BM : FG_BM, slots = pair ? sm_count / 2 : sm_count;
+    const long long rows = (M + bt - 1) / bt, tiles = rows * ((N + bt - 1) / bt);
+    const double each = pair ? 0.37 : 0.25, fed = (double)(bt * FG_BK * 2) / rows * slots / 5.5e6;
+    for (int p = 1; p <= 16 && (p == 1 || kb >= 8ll * p) && p * M * N <= (64ll << 20); ++p) {
+      const long long items = tiles * p, full = items / slots, rest = items % slots;
+      const double blocks = (double)((kb + p - 1) / p) + 1.5;
+      double t = full * blocks * (each > fed ? each : fed);
+      const double last = fed * rest / slots;
+      if (rest) t += blocks * (each > last ? each : last);
+      if (p > 1 || joined) t += (joined ? 0.0 : 2.0) + (double)p * M * N * 8 / 6e6;
+      if (t < least * (p > 1 ? 0.97 : 1.0)) {
+        least = t;
+        best = {pair, p};
+      }
+    }
+  }
+  return best;
 }
 
 template <typename T, typename OutT, int JOB>
@@ -783,7 +811,7 @@ int fused_gemm(Job job, const FusedCall& c) {
       !on_vectors(c.A, c.B, c.C, c.gu, c.dgu))
     return -2;
   const int fmt = c.dtype == PF_BF16;
-  const bool pair = fused_pairs(job, c.M, c.N, c.sm_count);
+  const bool pair = c.tile < 0 ? fused_pairs(job, c.M, c.N, c.sm_count) : c.tile;
   // Fewer rows than a tile has are loaded as what they are: rows of accumulators that no row of A fills are not read.
   const int a_rows = pair || c.M >= FG_BM ? FG_BM : (c.M + 7) / 8 * 8;
   FusedMaps maps;

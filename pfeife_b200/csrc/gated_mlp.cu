@@ -3,34 +3,16 @@
 //
 // Forward 6 M D H operations in two products (the first with both projections, the activation and their product in its
 // epilogue), backward 12 M D H in five: dh with everything that follows from it in the epilogue, dx and the weights'
-// gradients.  Up to 128 rows the weights are what moves, 6 bytes of each of the 3 D H read or written per direction:
-// a product is then split over its reduction into as many parts as keep all SMs reading, and what its epilogue does is done
-// by the kernels here, which add the parts up in their order.
+// gradients.  For few rows the weights are what moves, and products have few tiles: one is then split over its reduction
+// into as many parts as keep all SMs reading (plan_parts), and what its epilogue does is done by the kernels here, which
+// add the parts up in their order.
 #include "common.cuh"
 #include "api.h"
 #include "fused_gemm.h"
 
 namespace pf {
 
-// Parts that a product of few rows is split into; 1: it stays whole.  In units of the time of a k-block of 64: an item
-// costs its k-blocks and one more or two, parts a launch and a read of some 20.
-static int row_parts(long long M, long long N, long long K, int sm_count) {
-  if (M > 128) return 1;
-  const long long tiles = (N + 127) / 128, kb = (K + 63) / 64;
-  int best = 1;
-  double least = 1e30;
-  for (int p = 1; p <= 32 && (p == 1 || p * 4 <= kb); ++p) {
-    const double rounds = (double)((tiles * p + sm_count - 1) / sm_count);
-    double t = rounds * ((double)((kb + p - 1) / p) + 1.5);
-    if (p > 1) t += 20 + (double)p * M * N * 8 / 6e12 / 0.15e-6;
-    if (t < least - 1e-9) {
-      least = t;
-      best = p;
-    }
-  }
-  return best;
-}
-constexpr int PART_ROWS = 128;
+static long long part_rows(long long M) { return (M + 255) / 256 * 256; }
 
 struct Parts {
   const float* at;
@@ -168,14 +150,14 @@ PF_API int pf_gated_mlp_scratch(int M, int D, int H, int N, int sm_count) {
   if (sm_count <= 0) sm_count = 148;
   long long most = 0;
   auto need = [&](long long n, long long k) {
-    const int p = row_parts(M, n, k, sm_count);
+    const int p = plan_parts(M, n, k, sm_count, false).parts;
     if (p > 1 && p * n > most) most = p * n;
   };
   need(2ll * H, D);
   need(N, H);
   need(H, N);
   need(D, 2ll * H);
-  return (int)((most * PART_ROWS * 4 + 1023) / 1024);
+  return M <= 0 ? 0 : (int)((most * part_rows(M) * 4 + 1023) / 1024);
 }
 
 namespace pf {
@@ -190,10 +172,11 @@ struct Block {
     c.dtype = dtype; c.status = status; c.sm_count = sms; c.stream = st;
     return c;
   }
-  // A B^T in parts; n > 1
-  int in_parts(Job job, FusedCall c, int n, Parts& p) const {
-    c.C = ws; c.ldc = c.N; c.out_dtype = PF_F32; c.split = n; c.part_rows = PART_ROWS;
-    p = {ws, n, (long long)PART_ROWS * c.N};
+  PartPlan plan(long long n, long long k) const { return ws ? plan_parts(M, n, k, sms, false) : PartPlan(); }
+  // A B^T in parts, more than one
+  int in_parts(Job job, FusedCall c, PartPlan g, Parts& p) const {
+    c.C = ws; c.ldc = c.N; c.out_dtype = PF_F32; c.split = g.parts; c.part_rows = (int)part_rows(M); c.tile = g.pair;
+    p = {ws, g.parts, part_rows(M) * c.N};
     return fused_gemm(job, c);
   }
   unsigned grid(int width) const { return (unsigned)(((long long)M * (width / 8) + 127) / 128); }
@@ -211,9 +194,9 @@ static int mlp_forward(const Block& b, const void* x, const void* w1, const void
                        const void* b2, int b2_dtype, const void* residual, void* h, void* gu, void* y, long long ldx,
                        long long ldw1, long long ldw2, long long ldr) {
   int r;
-  const int p1 = b.ws ? row_parts(b.M, 2ll * b.H, b.D, b.sms) : 1, p2 = b.ws ? row_parts(b.M, b.N, b.H, b.sms) : 1;
+  const PartPlan p1 = b.plan(2ll * b.H, b.D), p2 = b.plan(b.N, b.H);
   Parts p;
-  if (p1 > 1) {
+  if (p1.parts > 1) {
     if ((r = b.in_parts(PARTS_K, b.call(2 * b.H, b.D, x, ldx, w1, ldw1), p1, p))) return r;
     after(glu_join_kernel<T>, b.grid(b.H), 128, 0, b.st)(p, b1, b1_dtype, (T*)gu, (T*)h, b.M, b.H, b.act);
     PF_CHECK_LAUNCH();
@@ -222,7 +205,7 @@ static int mlp_forward(const Block& b, const void* x, const void* w1, const void
     c.C = h; c.ldc = b.H; c.gu = gu; c.bias = b1; c.bias_dtype = b1_dtype; c.act = b.act;
     if ((r = fused_gemm(GLU_FWD, c))) return r;
   }
-  if (p2 > 1) {
+  if (p2.parts > 1) {
     if ((r = b.in_parts(PARTS_K, b.call(b.N, b.H, h, b.H, w2, ldw2), p2, p))) return r;
     after(row_join_kernel<T>, b.grid(b.N), 128, 0, b.st)(p, b2, b2_dtype, (const T*)residual, ldr, (T*)y, b.M, b.N);
     PF_CHECK_LAUNCH();
@@ -238,9 +221,9 @@ static int mlp_backward(const Block& b, const void* dy, const void* x, const voi
                         long long ldx, long long ldw1, long long ldw2, int dw1_dtype, int dw2_dtype, int add1,
                         int add2) {
   int r;
-  const int p1 = b.ws ? row_parts(b.M, b.H, b.N, b.sms) : 1, p2 = b.ws ? row_parts(b.M, b.D, 2ll * b.H, b.sms) : 1;
+  const PartPlan p1 = b.plan(b.H, b.N), p2 = b.plan(b.D, 2ll * b.H);
   Parts p;
-  if (p1 > 1) {
+  if (p1.parts > 1) {
     if ((r = b.in_parts(PARTS_N, b.call(b.H, b.N, dy, lddy, w2, ldw2), p1, p))) return r;
     after(glu_join_bwd_kernel<T>, b.grid(b.H), 128, 0, b.st)(p, (const T*)gu, (T*)dgu, (T*)h, b.M, b.H, b.act);
     PF_CHECK_LAUNCH();
@@ -253,7 +236,7 @@ static int mlp_backward(const Block& b, const void* dy, const void* x, const voi
   if (db2 && (r = pf_colsum(dy, db2, b.M, b.N, lddy, b.dtype, b.sms, b.st))) return r;
   const long long ldgu = 2ll * b.H;
   if (dx) {
-    if (p2 > 1) {
+    if (p2.parts > 1) {
       if ((r = b.in_parts(PARTS_N, b.call(b.D, 2 * b.H, dgu, ldgu, w1, ldw1), p2, p))) return r;
       after(row_join_kernel<T>, b.grid(b.D), 128, 0, b.st)(p, (const void*)nullptr, 0, (const T*)nullptr, 0ll, (T*)dx,
                                                            b.M, b.D);

@@ -312,12 +312,7 @@ PF_API int pf_head_parts(long long N, long long V, int D, int sm_count) {
   if (sm_count <= 0) sm_count = 148;
   const long long words = pf_head_words(N, V);
   if (words < V) return 1;
-  const bool pair = fused_pairs(PARTS_N, N, D, sm_count);
-  const long long bt = pair ? 256 : 128, tiles = ((N + bt - 1) / bt) * ((D + bt - 1) / bt);
-  const long long slots = pair ? sm_count / 2 : sm_count, kb = (V + 63) / 64;
-  int parts = 1;
-  while (parts < 16 && tiles * (parts + 1) <= slots && kb >= 8ll * (parts + 1)) ++parts;
-  return parts;
+  return N > 0 ? plan_parts(N, (D + 7) / 8 * 8, V, sm_count, true).parts : 1;
 }
 
 // x [N, D] (rows ldx apart), w [V, Dp] (Dp: D up to a multiple of 8, filled with zeros; rows ldw apart), target [N].
@@ -381,6 +376,8 @@ PF_API int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const
   const long long Mp = padded_rows(N);
   const HeadIndex ix = head_index(static_cast<int*>(index), N);
   const int words = pf_head_words(N, V), parts = pf_head_parts(N, V, D, sm_count);
+  // where the vocabulary is one piece, with the tiles that go with its parts
+  const int tile = words >= V && N > 0 ? plan_parts(N, Dp, V, sm_count, true).pair : -1;
   const float unit = dtype == PF_F16 ? 32768.f : 1.f;
   const float* scale = static_cast<const float*>(dloss);
   const float* scale2 = static_cast<const float*>(inv);
@@ -410,7 +407,7 @@ PF_API int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const
     if (dx) {
       FusedCall c = base;
       c.M = (int)N; c.N = Dp; c.K = n; c.A = dz; c.B = wp; c.lda = words; c.ldb = ldw; c.C = acc; c.ldc = Dp;
-      c.out_dtype = PF_F32; c.split = parts; c.part_rows = (int)Mp; c.accumulate = v0 > 0;
+      c.out_dtype = PF_F32; c.split = parts; c.tile = tile; c.part_rows = (int)Mp; c.accumulate = v0 > 0;
       if ((r = fused_gemm(PARTS_N, c))) return r;
     }
     if (dw) {

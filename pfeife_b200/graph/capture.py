@@ -94,7 +94,8 @@ class CapturedGraph:
 
 
 # op name -> positions of the weight operands that the op reads through the 16-bit shadow
-_SHADOW_OPERANDS = {"linear_fwd": (1,), "mlp_fwd": (1, 3), "conv2d_fwd": (1,), "embed_fwd": (1,)}
+_SHADOW_OPERANDS = {"linear_fwd": (1,), "mlp_fwd": (1, 3), "conv2d_fwd": (1,), "embed_fwd": (1,),
+                    "gated_mlp_fwd": (1, 3), "head_loss_fwd": (1,), "scaled_embed_fwd": (1,)}
 
 
 def _reads_shadow(user: fx.Node, value: fx.Node) -> bool:

@@ -35,6 +35,7 @@ class UNetConfig:
     time_id_count: int = 6
     time_id_dim: int = 256
     groups: int = 32
+    fused_mlp: bool = False                # ops.gated_mlp instead of two products around a GEGLU
 
 
 UNET_CONFIGS = {
@@ -98,9 +99,10 @@ class ResBlock(nn.Module):
 
 
 class TransformerLayer(nn.Module):
-    def __init__(self, dim, heads, cross_dim):
+    def __init__(self, dim, heads, cross_dim, fused_mlp=False):
         super().__init__()
         self.heads = heads
+        self.fused_mlp = fused_mlp
         self.n1, self.n2, self.n3 = nn.LayerNorm(dim), nn.LayerNorm(dim), nn.LayerNorm(dim)
         self.qkv = nn.Linear(dim, 3 * dim, bias=False)
         self.o1 = nn.Linear(dim, dim)
@@ -128,16 +130,18 @@ class TransformerLayer(nn.Module):
         a = ops.attention(q, kv[:, :, 0], kv[:, :, 1])
         delta = ops.linear(a.view(B, S, d), self.o2.weight, self.o2.bias)
         y, x = ops.layer_norm(delta, self.n3.weight, self.n3.bias, 1e-5, residual=x)
+        if self.fused_mlp:
+            return x, ops.gated_mlp(y, self.ff1.weight, self.ff1.bias, self.ff2.weight, self.ff2.bias, "gelu")
         g = ops.geglu(ops.linear(y, self.ff1.weight, self.ff1.bias))
         return x, ops.linear(g, self.ff2.weight, self.ff2.bias)
 
 
 class SpatialTransformer(nn.Module):
-    def __init__(self, dim, depth, head_dim, cross_dim, groups):
+    def __init__(self, dim, depth, head_dim, cross_dim, groups, fused_mlp=False):
         super().__init__()
         self.norm = GroupNorm(groups, dim, eps=1e-6)
         self.proj_in = nn.Linear(dim, dim)
-        self.layers = nn.ModuleList([TransformerLayer(dim, dim // head_dim, cross_dim)
+        self.layers = nn.ModuleList([TransformerLayer(dim, dim // head_dim, cross_dim, fused_mlp)
                                      for _ in range(depth)])
         self.proj_out = nn.Linear(dim, dim)
 
@@ -174,7 +178,7 @@ class UNet(nn.Module):
             for _ in range(cfg.layers_per_block):
                 self.down_res.append(ResBlock(cur, c, emb, g))
                 depth = cfg.transformer_depth[lvl]
-                self.down_attn.append(SpatialTransformer(c, depth, cfg.head_dim, cfg.cross_dim, g)
+                self.down_attn.append(SpatialTransformer(c, depth, cfg.head_dim, cfg.cross_dim, g, cfg.fused_mlp)
                                       if depth else nn.Identity())
                 cur = c
                 skip_ch.append(cur)
@@ -183,7 +187,7 @@ class UNet(nn.Module):
                 skip_ch.append(cur)
         self.mid1 = ResBlock(cur, cur, emb, g)
         self.mid_attn = SpatialTransformer(cur, cfg.transformer_depth[-1], cfg.head_dim,
-                                           cfg.cross_dim, g)
+                                           cfg.cross_dim, g, cfg.fused_mlp)
         self.mid2 = ResBlock(cur, cur, emb, g)
 
         self.up_res, self.up_attn, self.up_sample = nn.ModuleList(), nn.ModuleList(), \
@@ -193,7 +197,7 @@ class UNet(nn.Module):
             for _ in range(cfg.layers_per_block + 1):
                 self.up_res.append(ResBlock(cur + skip_ch.pop(), c, emb, g))
                 depth = cfg.transformer_depth[lvl]
-                self.up_attn.append(SpatialTransformer(c, depth, cfg.head_dim, cfg.cross_dim, g)
+                self.up_attn.append(SpatialTransformer(c, depth, cfg.head_dim, cfg.cross_dim, g, cfg.fused_mlp)
                                     if depth else nn.Identity())
                 cur = c
             if lvl > 0:

@@ -144,3 +144,48 @@ def test_mixed_precision_on_one_gpu(cuda_graphs):
         moved = (q.detach() - s).norm()
         assert float((p.detach().float() - q.detach()).norm()) <= 0.1 * float(moved) + 1e-6, name
         assert moved > 0
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_a_transformer_layer_of_images(device):
+    """The feed-forward block with biases and GELU, as the UNet's transformer layers have it."""
+    from pfeife_b200.models.unet import TransformerLayer
+    torch.manual_seed(0)
+    layer, other = (TransformerLayer(64, 4, 32, fused).to(device) for fused in (True, False))
+    other.load_state_dict(layer.state_dict())
+    x, ctx = torch.randn(2, 48, 64, device=device), torch.randn(2, 7, 32, device=device)
+    out = []
+    for m in (layer, other):
+        with torch.autocast(device, dtype=torch.bfloat16):
+            h, delta = m(x, None, ctx)
+        y = h.float() + delta.float()
+        y.square().mean().backward()
+        out.append(y.detach())
+    # some twenty roundings to 8 bits
+    assert float((out[0] - out[1]).norm()) <= 20 * 2.0 ** -8 * float(out[1].norm())
+    for (name, p), q in zip(layer.named_parameters(), other.parameters()):
+        assert float((p.grad - q.grad).norm()) <= 20 * 2.0 ** -8 * float(q.grad.norm()) + 1e-6, name
+
+
+@pytest.mark.timeout(900)
+@pytest.mark.parametrize("mesh", [None, "-2,1"], ids=["stages", "replicas"])
+def test_the_trainer_with_the_lean_operators(mesh):
+    """Two ranks of the example trainer, as stages and as replicas: it runs, and the loss is a number."""
+    from test_examples import COMMON, _PORT, _launch
+    _PORT[0] += 40
+    its, loss, _ = _launch("train_llama.py", ["--model", "llama_tiny", "--block_size", "16", "--lean",
+                                             "--per_device_train_batch_size", "2", "--iter_cnt", "3"] + COMMON,
+                           mesh=mesh)
+    assert its > 0 and loss == loss
+
+
+def test_weights_that_are_read_in_16_bits_only():
+    """A replica that does not own one needs no current fp32 copy of it."""
+    from test_graph import capture
+    model = _model(num_layers=1)
+    ids, labels = _batch(2, 16, torch.Generator().manual_seed(1))
+    cap, _, _ = capture(model, ids, labels)
+    only = cap.shadow_only_inputs()
+    assert {i.qualname for i in cap.inputs if i.is_state and i.index in only} == {
+        "embed.weight", "layers.0.qkv.weight", "layers.0.o_proj.weight", "layers.0.gate_up.weight",
+        "layers.0.down.weight", "lm_head.weight"}
