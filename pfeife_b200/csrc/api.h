@@ -34,8 +34,8 @@ PF_DECL int pf_gated_mlp_fwd(const void* x, const void* w1, const void* b1, int 
 PF_DECL int pf_gated_mlp_bwd(const void* dy, const void* x, const void* w1, const void* w2, const void* gu, void* dgu,
                              void* h, void* dx, void* dw1, void* dw2, void* db1, void* db2, void* ws, int ws_kib, int M,
                              int D, int H, int N, long long lddy, long long ldx, long long ldw1, long long ldw2,
-                             int act, int dtype, int dw1_dtype, int dw2_dtype, int add1, int add2, int* status,
-                             int sm_count, void* stream);
+                             int act, int dtype, int dw1_dtype, int dw2_dtype, int db1_dtype, int db2_dtype, int add,
+                             int* status, int sm_count, void* stream);
 
 // ---- head_loss.cu
 PF_DECL int pf_head_index(long long N);

@@ -1213,7 +1213,8 @@ struct DirectGatedMlp : torch::autograd::Function<DirectGatedMlp> {
     } else if (gu.defined() && direct(dy, x, w1, w2, gu, b1, b2) && gated_fits(x, w1, w2) &&
                dy.scalar_type() == x.scalar_type() && dy.size(-1) == w2.size(0) &&
                dy.numel() / dy.size(-1) == x.numel() / x.size(-1) && gu.scalar_type() == x.scalar_type() &&
-               gu.size(-1) == w1.size(0) && gu.numel() / gu.size(-1) == x.numel() / x.size(-1)) {
+               gu.size(-1) == w1.size(0) && gu.numel() / gu.size(-1) == x.numel() / x.size(-1) &&
+               (!b1.defined() || number(b1)) && (!b2.defined() || number(b2))) {
       below([&] {
         const Env e(dy);
         const Tensor x2 = rows(x), dy2 = rows(dy);
@@ -1226,13 +1227,14 @@ struct DirectGatedMlp : torch::autograd::Function<DirectGatedMlp> {
         if (nx) dx = empty(x.sizes(), dy);
         if (nw1) dw1 = empty(w1.sizes(), dy);
         if (nw2) dw2 = empty(w2.sizes(), dy);
-        if (nb1) db1 = at::zeros({2 * g.H}, dy.options().dtype(at::kFloat));
-        if (nb2) db2 = at::zeros({g.N}, dy.options().dtype(at::kFloat));
+        if (nb1) db1 = empty({2 * g.H}, b1);
+        if (nb2) db2 = empty({g.N}, b2);
         auto out = [](const Tensor& t) { return const_cast<void*>(at_or_null(t)); };
         ok(pf_gated_mlp_bwd(dy2.data_ptr(), x2.data_ptr(), w1.data_ptr(), w2.data_ptr(), kept.data_ptr(),
                             dgu.data_ptr(), h.data_ptr(), out(dx), out(dw1), out(dw2), out(db1), out(db2), out(ws), kib,
                             g.M, g.D, g.H, g.N, dy2.stride(0), x2.stride(0), w1.stride(0), w2.stride(0), act,
-                            code_of(dy), code_of(dy), code_of(dy), 0, 0, e.status, e.sms, e.stream),
+                            code_of(dy), code_of(dy), code_of(dy), nb1 ? code_of(b1) : 0, nb2 ? code_of(b2) : 0, 0,
+                            e.status, e.sms, e.stream),
            "pf_gated_mlp_bwd");
         return 0;
       });

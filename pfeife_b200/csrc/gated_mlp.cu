@@ -141,11 +141,83 @@ row_join_kernel(const Parts p, const void* __restrict__ bias, int bias_dtype, co
   store8(out + (long long)m * N + c, v);
 }
 
+// Gradients of both biases: sums over the rows of up to two matrices, 256 columns a CTA, a row a warp and step.  Where
+// columns alone leave SMs idle the rows are dealt to `parts` CTAs, whose sums a second launch adds up in their order.
+struct BiasGrad {
+  const void* x;                // [M, cols], rows ld apart; null: none
+  long long ld;
+  int cols, dtype, add;         // of the output; add: to fp32
+  void* out;
+};
+__device__ __forceinline__ void put_bias_grad(const BiasGrad& b, int c, float v) {
+  if (b.dtype == PF_F32) {
+    float* o = static_cast<float*>(b.out) + c;
+    *o = b.add ? *o + v : v;
+  } else if (b.dtype == PF_F16) {
+    static_cast<__half*>(b.out)[c] = from_f32<__half>(v);
+  } else {
+    static_cast<__nv_bfloat16*>(b.out)[c] = from_f32<__nv_bfloat16>(v);
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(256)
+bias_grad_kernel(const BiasGrad b1, const BiasGrad b2, int blocks1, int M, int parts, float* __restrict__ ws) {
+  after_previous();
+  __shared__ float sums[8][256];
+  const bool second = (int)blockIdx.x >= blocks1;
+  const BiasGrad& b = second ? b2 : b1;
+  const int c0 = ((int)blockIdx.x - (second ? blocks1 : 0)) * 256, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = c0 + lane * 8, part = blockIdx.y;
+  const int begin = (int)((long long)M * part / parts), end = (int)((long long)M * (part + 1) / parts);
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (c < b.cols) {
+    const T* x = static_cast<const T*>(b.x) + c;
+    for (int r = begin + warp; r < end; r += 32) {
+      uint4 q[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (r + 8 * u < end) q[u] = __ldg(reinterpret_cast<const uint4*>(x + (long long)(r + 8 * u) * b.ld));
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (r + 8 * u < end) {
+          const T* e = reinterpret_cast<const T*>(&q[u]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[j] += to_f32<T>(e[j]);
+        }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sums[warp][lane * 8 + j] = s[j];
+  __syncthreads();
+  const int col = c0 + threadIdx.x;
+  if (col >= b.cols) return;
+  float v = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v += sums[k][threadIdx.x];
+  if (parts == 1) put_bias_grad(b, col, v);
+  else ws[(long long)part * (b1.cols + b2.cols) + (second ? b1.cols : 0) + col] = v;
+}
+__global__ void __launch_bounds__(256)
+bias_join_kernel(const BiasGrad b1, const BiasGrad b2, int parts, const float* __restrict__ ws) {
+  after_previous();
+  const int all = b1.cols + b2.cols, i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= all) return;
+  float v = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < parts; ++k) v += ws[(long long)k * all + i];
+  if (i < b1.cols) put_bias_grad(b1, i, v);
+  else put_bias_grad(b2, i - b1.cols, v);
+}
+static int bias_parts(long long M, long long cols, int sm_count) {
+  const long long blocks = (cols + 255) / 256 + 1, most = (M + 63) / 64, parts = (4ll * sm_count + blocks - 1) / blocks;
+  return (int)(parts < most ? parts : most);
+}
+
 }  // namespace pf
 
 using namespace pf;
 
-// KiB of workspace of both directions for M rows; 0 where no product is split
+// KiB of workspace of both directions for M rows; 0 where nothing is split
 PF_API int pf_gated_mlp_scratch(int M, int D, int H, int N, int sm_count) {
   if (sm_count <= 0) sm_count = 148;
   long long most = 0;
@@ -157,7 +229,11 @@ PF_API int pf_gated_mlp_scratch(int M, int D, int H, int N, int sm_count) {
   need(N, H);
   need(H, N);
   need(D, 2ll * H);
-  return M <= 0 ? 0 : (int)((most * part_rows(M) * 4 + 1023) / 1024);
+  if (M <= 0) return 0;
+  most *= part_rows(M);
+  const int p = bias_parts(M, 2ll * H + N, sm_count);
+  if (p > 1 && p * (2ll * H + N) > most) most = p * (2ll * H + N);
+  return (int)((most * 4 + 1023) / 1024);
 }
 
 namespace pf {
@@ -180,6 +256,21 @@ struct Block {
     return fused_gemm(job, c);
   }
   unsigned grid(int width) const { return (unsigned)(((long long)M * (width / 8) + 127) / 128); }
+  template <typename T> int bias_grads(BiasGrad b1, BiasGrad b2) const {
+    for (BiasGrad* b : {&b1, &b2})
+      if (!b->out) b->cols = 0;
+    const int all = b1.cols + b2.cols;
+    if (!all) return 0;
+    const int blocks1 = (b1.cols + 255) / 256, blocks = blocks1 + (b2.cols + 255) / 256;
+    const int parts = ws ? bias_parts(M, 2ll * H + N, sms) : 1;
+    after(bias_grad_kernel<T>, dim3(blocks, parts), 256, 0, st)(b1, b2, blocks1, M, parts, ws);
+    PF_CHECK_LAUNCH();
+    if (parts > 1) {
+      after(bias_join_kernel, (unsigned)((all + 255) / 256), 256, 0, st)(b1, b2, parts, (const float*)ws);
+      PF_CHECK_LAUNCH();
+    }
+    return 0;
+  }
   // dst [rows, cols] (+)= a^T b over the M rows
   int weight_grad(const void* a, long long lda, const void* b, long long ldb, void* dst, int rows, int cols,
                   int dst_dtype, int add) const {
@@ -215,11 +306,15 @@ static int mlp_forward(const Block& b, const void* x, const void* w1, const void
                  0, 0, 0, 1.0f, b.status, b.sms, 0, nullptr, 0, b.st);
 }
 
+// what a backward writes; `add`: bits 1 dw1, 2 dw2, 4 db1, 8 db2
+struct Grads {
+  void *dx, *dw1, *dw2, *db1, *db2;
+  int dw1_dtype, dw2_dtype, db1_dtype, db2_dtype, add;
+};
 template <typename T>
 static int mlp_backward(const Block& b, const void* dy, const void* x, const void* w1, const void* w2, const void* gu,
-                        void* dgu, void* h, void* dx, void* dw1, void* dw2, void* db1, void* db2, long long lddy,
-                        long long ldx, long long ldw1, long long ldw2, int dw1_dtype, int dw2_dtype, int add1,
-                        int add2) {
+                        void* dgu, void* h, const Grads& g, long long lddy, long long ldx, long long ldw1,
+                        long long ldw2) {
   int r;
   const PartPlan p1 = b.plan(b.H, b.N), p2 = b.plan(b.D, 2ll * b.H);
   Parts p;
@@ -232,23 +327,21 @@ static int mlp_backward(const Block& b, const void* dy, const void* x, const voi
     c.C = h; c.ldc = b.H; c.gu = const_cast<void*>(gu); c.dgu = dgu; c.act = b.act;
     if ((r = fused_gemm(GLU_BWD, c))) return r;
   }
-  if (dw2 && (r = b.weight_grad(dy, lddy, h, b.H, dw2, b.N, b.H, dw2_dtype, add2))) return r;
-  if (db2 && (r = pf_colsum(dy, db2, b.M, b.N, lddy, b.dtype, b.sms, b.st))) return r;
   const long long ldgu = 2ll * b.H;
-  if (dx) {
+  if (g.dw2 && (r = b.weight_grad(dy, lddy, h, b.H, g.dw2, b.N, b.H, g.dw2_dtype, g.add & 2))) return r;
+  if (g.dx) {
     if (p2.parts > 1) {
       if ((r = b.in_parts(PARTS_N, b.call(b.D, 2 * b.H, dgu, ldgu, w1, ldw1), p2, p))) return r;
-      after(row_join_kernel<T>, b.grid(b.D), 128, 0, b.st)(p, (const void*)nullptr, 0, (const T*)nullptr, 0ll, (T*)dx,
+      after(row_join_kernel<T>, b.grid(b.D), 128, 0, b.st)(p, (const void*)nullptr, 0, (const T*)nullptr, 0ll, (T*)g.dx,
                                                            b.M, b.D);
       PF_CHECK_LAUNCH();
-    } else if ((r = pf_gemm(dgu, w1, dx, b.M, b.D, 2 * b.H, ldgu, ldw1, b.D, 0, 1, b.dtype, b.dtype, nullptr, 0,
+    } else if ((r = pf_gemm(dgu, w1, g.dx, b.M, b.D, 2 * b.H, ldgu, ldw1, b.D, 0, 1, b.dtype, b.dtype, nullptr, 0,
                             nullptr, 0, nullptr, 0, 0, 0, 1.0f, b.status, b.sms, 0, nullptr, 0, b.st))) {
       return r;
     }
   }
-  if (dw1 && (r = b.weight_grad(dgu, ldgu, x, ldx, dw1, 2 * b.H, b.D, dw1_dtype, add1))) return r;
-  if (db1 && (r = pf_colsum(dgu, db1, b.M, 2 * b.H, ldgu, b.dtype, b.sms, b.st))) return r;
-  return 0;
+  if (g.dw1 && (r = b.weight_grad(dgu, ldgu, x, ldx, g.dw1, 2 * b.H, b.D, g.dw1_dtype, g.add & 1))) return r;
+  return b.bias_grads<T>({dgu, ldgu, 2 * b.H, g.db1_dtype, g.add & 4, g.db1}, {dy, lddy, b.N, g.db2_dtype, g.add & 8, g.db2});
 }
 
 static int mlp_block(Block& b, int M, int D, int H, int N, int act, int dtype, void* ws, int ws_kib, int* status,
@@ -281,28 +374,32 @@ PF_API int pf_gated_mlp_fwd(const void* x, const void* w1, const void* b1, int b
                                                       ldw1, ldw2, ldr);
 }
 
-// From dy [M, N] and the kept gu: dx [M, D], dw1 [2H, D], dw2 [N, H] (packed, 16 bits or fp32; add1, add2: added to fp32),
-// db1 [2H] and db2 [N] (fp32, added to); any of these may be null.  dgu [M, 2H] and h [M, H] are scratch.
+// From dy [M, N] and the kept gu: dx [M, D], dw1 [2H, D], dw2 [N, H], db1 [2H] and db2 [N], packed, each in 16 bits or fp32
+// but dx; any of these may be null.  add: bits 1 dw1, 2 dw2, 4 db1, 8 db2 are added to, in fp32.  dgu [M, 2H] and h [M, H]
+// are scratch.
 PF_API int pf_gated_mlp_bwd(const void* dy, const void* x, const void* w1, const void* w2, const void* gu, void* dgu,
                             void* h, void* dx, void* dw1, void* dw2, void* db1, void* db2, void* ws, int ws_kib, int M,
                             int D, int H, int N, long long lddy, long long ldx, long long ldw1, long long ldw2, int act,
-                            int dtype, int dw1_dtype, int dw2_dtype, int add1, int add2, int* status, int sm_count,
-                            void* stream) {
+                            int dtype, int dw1_dtype, int dw2_dtype, int db1_dtype, int db2_dtype, int add, int* status,
+                            int sm_count, void* stream) {
   Block b;
   const int r = mlp_block(b, M, D, H, N, act, dtype, ws, ws_kib, status, sm_count, stream);
   if (r) return r;
-  if ((add1 && dw1_dtype != PF_F32) || (add2 && dw2_dtype != PF_F32)) return -1;
-  if ((dw1 && dw1_dtype != dtype && dw1_dtype != PF_F32) || (dw2 && dw2_dtype != dtype && dw2_dtype != PF_F32)) return -1;
-  if (M == 0) {                                         // nothing to add up
-    const size_t s1 = dw1_dtype == PF_F32 ? 4 : 2, s2 = dw2_dtype == PF_F32 ? 4 : 2;
-    cudaError_t e = cudaSuccess;
-    if (dw1 && !add1) e = cudaMemsetAsync(dw1, 0, 2 * (size_t)H * D * s1, b.st);
-    if (dw2 && !add2 && e == cudaSuccess) e = cudaMemsetAsync(dw2, 0, (size_t)N * H * s2, b.st);
-    return (int)e;
+  const Grads g{dx, dw1, dw2, db1, db2, dw1_dtype, dw2_dtype, db1_dtype, db2_dtype, add};
+  void* const out[4] = {dw1, dw2, db1, db2};
+  const int types[4] = {dw1_dtype, dw2_dtype, db1_dtype, db2_dtype};
+  const size_t sizes[4] = {2 * (size_t)H * D, (size_t)N * H, 2 * (size_t)H, (size_t)N};
+  for (int i = 0; i < 4; ++i) {
+    if (!out[i]) continue;
+    const bool added = add >> i & 1;
+    if (types[i] != PF_F32 && (added || types[i] < 0 || types[i] > 2 || (i < 2 && types[i] != dtype))) return -1;
+    if (M == 0 && !added) {                             // nothing to add up
+      cudaError_t e = cudaMemsetAsync(out[i], 0, sizes[i] * (types[i] == PF_F32 ? 4 : 2), b.st);
+      if (e != cudaSuccess) return (int)e;
+    }
   }
+  if (M == 0) return 0;
   if (lddy % 8 || ldx % 8 || ldw1 % 8 || ldw2 % 8 || !on_vectors(dy, x, w1, w2, gu, dgu, h, dx, dw1, dw2)) return -2;
-  return dtype == PF_F16 ? mlp_backward<__half>(b, dy, x, w1, w2, gu, dgu, h, dx, dw1, dw2, db1, db2, lddy, ldx, ldw1,
-                                                ldw2, dw1_dtype, dw2_dtype, add1, add2)
-                         : mlp_backward<__nv_bfloat16>(b, dy, x, w1, w2, gu, dgu, h, dx, dw1, dw2, db1, db2, lddy, ldx,
-                                                       ldw1, ldw2, dw1_dtype, dw2_dtype, add1, add2);
+  return dtype == PF_F16 ? mlp_backward<__half>(b, dy, x, w1, w2, gu, dgu, h, g, lddy, ldx, ldw1, ldw2)
+                         : mlp_backward<__nv_bfloat16>(b, dy, x, w1, w2, gu, dgu, h, g, lddy, ldx, ldw1, ldw2);
 }

@@ -703,43 +703,47 @@ def _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_d
     """``gated_mlp_bwd`` by its kernels"""
     cd, dev = dy.dtype, dy.device
     x2 = _rows(x if x.dtype == cd else kx.cast(x, cd))
-    out, filled, late = {}, {}, []
+    out, buckets, late = {}, [], []
     if need_dx:
         out["dx"] = torch.empty(x2.shape, dtype=cd, device=dev)
-    for name, w, need, add in (("dw1", w1, need_dw1, "add1"), ("dw2", w2, need_dw2, "add2")):
+    for name, w, need in (("dw1", w1, need_dw1), ("dw2", w2, need_dw2)):
         if need:
             slot = _slot(w)
             bucket = None if slot is None or slot.main_grad is None else slot.main_grad.view(w.shape)
             if bucket is not None and bucket.data_ptr() % 16 == 0:
-                out[name], filled[add] = bucket, True
+                out[name] = bucket
+                buckets.append(name)
             else:
                 out[name] = torch.empty(w.shape, dtype=cd if w.dtype == cd and bucket is None else torch.float32,
                                         device=dev)
-                late.append((name, add, bucket))
+                if bucket is not None:       # off the 16 bytes that the kernels write
+                    late.append((name, bucket))
     for name, b, n, need in (("db1", b1, w1.shape[0], need_db1), ("db2", b2, w2.shape[0], need_db2)):
         if need:
             bucket = _grad_bucket(b)
-            filled[name] = bucket is not None
-            out[name] = bucket if bucket is not None else torch.zeros(n, dtype=torch.float32, device=dev)
+            if bucket is not None:
+                out[name] = bucket
+                buckets.append(name)
+            else:
+                dtype = b.dtype if b is not None and b.dtype in (torch.float16, torch.bfloat16) else torch.float32
+                out[name] = torch.empty(n, dtype=dtype, device=dev)
     kx.gated_mlp_bwd(_rows(dy), x2, _aligned(_weight_as(w1, cd)), _aligned(_weight_as(w2, cd)), _rows(gu), act,
-                     add1=filled.get("add1", False), add2=filled.get("add2", False), **out)
-    for name, add, bucket in late:
-        if bucket is not None:               # a bucket off the 16 bytes that the kernels write
-            bucket.add_(out[name])
-            filled[add] = True
-    kept = lambda name, gone: out[name] if name in out and not gone else dy.new_empty(0)
-    dx = out["dx"].view(x.shape) if need_dx else dy.new_empty(0)
-    dw1, dw2 = (kept(n, filled.get(a, False)) for n, a in (("dw1", "add1"), ("dw2", "add2")))
-    return (dx, dw1.to(w1.dtype), kept("db1", filled.get("db1", False)), dw2.to(w2.dtype),
-            kept("db2", filled.get("db2", False)))
+                     add=tuple(buckets), **out)
+    for name, bucket in late:
+        bucket.add_(out[name])
+        buckets.append(name)
+    dx, dw1, db1, dw2, db2 = (out[k] if k in out and k not in buckets else dy.new_empty(0)
+                              for k in ("dx", "dw1", "db1", "dw2", "db2"))
+    return dx.view(x.shape) if need_dx else dx, dw1.to(w1.dtype), db1, dw2.to(w2.dtype), db2
 
 
 @gated_mlp_bwd.register_fake
 def _(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1=None, b2=None):
     e, f32 = dy.new_empty(0), torch.float32
     return (dy.new_empty(x.shape) if need_dx else e, torch.empty_like(w1) if need_dw1 else e,
-            dy.new_empty(w1.shape[0] if need_db1 else 0, dtype=f32), torch.empty_like(w2) if need_dw2 else e,
-            dy.new_empty(w2.shape[0] if need_db2 else 0, dtype=f32))
+            dy.new_empty(w1.shape[0] if need_db1 else 0, dtype=b1.dtype if b1 is not None else f32),
+            torch.empty_like(w2) if need_dw2 else e,
+            dy.new_empty(w2.shape[0] if need_db2 else 0, dtype=b2.dtype if b2 is not None else f32))
 
 
 def _gated_mlp_setup(ctx, inputs, output):

@@ -665,9 +665,9 @@ def gated_mlp_fwd(x: torch.Tensor, w1: torch.Tensor, b1: Optional[torch.Tensor],
 def gated_mlp_bwd(dy: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, gu: torch.Tensor, act: int, *,
                   dx: Optional[torch.Tensor] = None, dw1: Optional[torch.Tensor] = None,
                   dw2: Optional[torch.Tensor] = None, db1: Optional[torch.Tensor] = None,
-                  db2: Optional[torch.Tensor] = None, add1: bool = False, add2: bool = False) -> None:
-    """Writes the gradients whose tensors are given: dx [M, D], dw1 [2H, D] and dw2 [N, H] (added to with add1 and add2,
-    fp32), db1 [2H] and db2 [N] (fp32, added to)."""
+                  db2: Optional[torch.Tensor] = None, add: Tuple[str, ...] = ()) -> None:
+    """Writes the gradients whose tensors are given: dx [M, D], dw1 [2H, D], dw2 [N, H], db1 [2H], db2 [N], in 16 bits or
+    fp32; those named in ``add`` are added to, in fp32."""
     L = _lib.calls()
     M, D = x.shape
     N, H = w2.shape
@@ -679,10 +679,12 @@ def gated_mlp_bwd(dy: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w2: torch
         assert t is None or (t.shape == shape and t.is_contiguous())
     dgu, h = torch.empty_like(gu), torch.empty((M, H), dtype=dy.dtype, device=dy.device)
     ws, kib = _mlp_workspace(L, M, D, H, N, dy.device)
+    grads = {"dw1": dw1, "dw2": dw2, "db1": db1, "db2": db2}
+    types = [0 if t is None else dt(t.dtype) for t in grads.values()]
+    bits = sum(1 << i for i, name in enumerate(grads) if name in add)
     check(L.pf_gated_mlp_bwd(dy, x, w1, w2, gu, dgu, h, dx, dw1, dw2, db1, db2, ws, kib, M, D, H, N, dy.stride(0),
-                             x.stride(0), w1.stride(0), w2.stride(0), act, dt(dy.dtype),
-                             dt(dw1.dtype) if dw1 is not None else 0, dt(dw2.dtype) if dw2 is not None else 0, int(add1),
-                             int(add2), status_word(dy.device), sm_count(dy.device), stream_of(dy)), "pf_gated_mlp_bwd")
+                             x.stride(0), w1.stride(0), w2.stride(0), act, dt(dy.dtype), *types, bits,
+                             status_word(dy.device), sm_count(dy.device), stream_of(dy)), "pf_gated_mlp_bwd")
 
 
 # --------------------------------------------------------------------------- output head with its cross entropy

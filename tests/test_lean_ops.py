@@ -206,7 +206,7 @@ def test_gated_mlp(M, K, H, N, kind, biases, residual, dtype, device):
         assert torch.equal(grads[id(res)], dy)
     with torch.no_grad():
         assert torch.equal(ops.gated_mlp(x, w1, b1, w2, b2, kind, res), y)
-    again = torch.autograd.grad(ops.gated_mlp(x, w1, b1, w2, b2, kind, res), leaves[:3], dy)
+    again = torch.autograd.grad(ops.gated_mlp(x, w1, b1, w2, b2, kind, res), leaves, dy)
     assert all(torch.equal(a, grads[id(t)]) for a, t in zip(again, leaves))
 
 
