@@ -12,8 +12,6 @@
 
 namespace pf {
 
-static long long part_rows(long long M) { return (M + 255) / 256 * 256; }
-
 struct Parts {
   const float* at;
   int parts;
@@ -219,6 +217,7 @@ using namespace pf;
 
 // KiB of workspace of both directions for M rows; 0 where nothing is split
 PF_API int pf_gated_mlp_scratch(int M, int D, int H, int N, int sm_count) {
+  if (M <= 0) return 0;
   if (sm_count <= 0) sm_count = 148;
   long long most = 0;
   auto need = [&](long long n, long long k) {
@@ -229,8 +228,7 @@ PF_API int pf_gated_mlp_scratch(int M, int D, int H, int N, int sm_count) {
   need(N, H);
   need(H, N);
   need(D, 2ll * H);
-  if (M <= 0) return 0;
-  most *= part_rows(M);
+  most *= M;
   const int p = bias_parts(M, 2ll * H + N, sm_count);
   if (p > 1 && p * (2ll * H + N) > most) most = p * (2ll * H + N);
   return (int)((most * 4 + 1023) / 1024);
@@ -251,8 +249,8 @@ struct Block {
   PartPlan plan(long long n, long long k) const { return ws ? plan_parts(M, n, k, sms, false) : PartPlan(); }
   // A B^T in parts, more than one
   int in_parts(Job job, FusedCall c, PartPlan g, Parts& p) const {
-    c.C = ws; c.ldc = c.N; c.out_dtype = PF_F32; c.split = g.parts; c.part_rows = (int)part_rows(M); c.tile = g.pair;
-    p = {ws, g.parts, part_rows(M) * c.N};
+    c.C = ws; c.ldc = c.N; c.out_dtype = PF_F32; c.split = g.parts; c.part_rows = M; c.tile = g.pair;
+    p = {ws, g.parts, (long long)M * c.N};
     return fused_gemm(job, c);
   }
   unsigned grid(int width) const { return (unsigned)(((long long)M * (width / 8) + 127) / 128); }

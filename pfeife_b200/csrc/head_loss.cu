@@ -81,18 +81,10 @@ head_rows_kernel(const long long* __restrict__ target, HeadIndex ix, float* __re
   }
 }
 
-// xc[i] = x[list[i]], a warp per row; zeros behind the last row to the end of its block of 64, as far as a reduction over
-// rows reads, and in the columns that fill D up to Dp.
+// A row of x into the packed rows, or zeros; a warp.
 template <typename T>
-__global__ void __launch_bounds__(256)
-head_gather_kernel(const T* __restrict__ x, T* __restrict__ xc, HeadIndex ix, int Mp, int D, int Dp, long long ldx,
-                   int vec) {
-  after_previous();
-  const int count = *ix.count, end = min(Mp, (count + 63) / 64 * 64), lane = threadIdx.x & 31;
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= end) return;
-  T* dst = xc + (long long)i * Dp;
-  const T* src = i < count ? x + ix.list[i] * ldx : nullptr;
+__device__ __forceinline__ void put_row(const T* src, T* dst, int D, int Dp, int vec) {
+  const int lane = threadIdx.x & 31;
   if (vec) {
     uint4* dv = reinterpret_cast<uint4*>(dst);
     const uint4* sv = reinterpret_cast<const uint4*>(src);
@@ -108,6 +100,68 @@ head_gather_kernel(const T* __restrict__ x, T* __restrict__ xc, HeadIndex ix, in
     }
   } else {
     for (int c = lane; c < Dp; c += 32) dst[c] = src && c < D ? src[c] : from_f32<T>(0.f);
+  }
+}
+// A reduction over rows reads whole blocks of 64: zeros behind the last row
+__device__ __forceinline__ int zeroed_rows(int count, int Mp) { return min(Mp, (count + 63) / 64 * 64); }
+
+// xc[i] = x[list[i]], a warp per row
+template <typename T>
+__global__ void __launch_bounds__(256)
+head_gather_kernel(const T* __restrict__ x, T* __restrict__ xc, HeadIndex ix, int Mp, int D, int Dp, long long ldx,
+                   int vec) {
+  after_previous();
+  const int count = *ix.count, i = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= zeroed_rows(count, Mp)) return;
+  put_row(i < count ? x + ix.list[i] * ldx : nullptr, xc + (long long)i * Dp, D, Dp, vec);
+}
+
+// Both at once for calls of few rows, where a launch costs more than that every CTA, of 8 rows, looks at all labels.
+constexpr int PICK_ROWS = 4096;
+template <typename T>
+__global__ void __launch_bounds__(256)
+head_pick_kernel(const long long* __restrict__ target, const T* __restrict__ x, T* __restrict__ xc, HeadIndex ix,
+                 float* __restrict__ loss_of_row, int N, int Mp, int D, int Dp, long long ldx, long long V,
+                 long long ignore_index, int vec) {
+  after_previous();
+  __shared__ int sums[2][8];
+  __shared__ int labels[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row0 = blockIdx.x * 8;
+  int before = 0, all = 0;
+  for (int n = threadIdx.x; n < N; n += 256) {
+    const long long t = target[n];
+    const bool in = t >= 0 && t < V && t != ignore_index;
+    all += in;
+    before += in && n < row0;
+    if (n >= row0 && n < row0 + 8) labels[n - row0] = in ? (int)t : -1;
+  }
+  all = __reduce_add_sync(0xffffffffu, all);
+  before = __reduce_add_sync(0xffffffffu, before);
+  if (lane == 0) { sums[0][warp] = all; sums[1][warp] = before; }
+  __syncthreads();
+  all = before = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) { all += sums[0][k]; before += sums[1][k]; }
+  const int row = row0 + warp;
+  if (row < N) {
+    const int label = labels[warp];
+    int at = before;
+    for (int k = 0; k < warp; ++k) at += labels[k] >= 0;
+    if (lane == 0) {
+      ix.at[row] = label >= 0 ? at : -1;
+      if (label >= 0) {
+        ix.list[at] = row;
+        ix.labels[at] = label;
+      } else if (loss_of_row) {
+        loss_of_row[row] = 0.f;
+      }
+    }
+    if (label >= 0) put_row(x + row * ldx, xc + (long long)at * Dp, D, Dp, vec);
+  }
+  if (row >= all && row < zeroed_rows(all, Mp)) put_row<T>(nullptr, xc + (long long)row * Dp, D, Dp, vec);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    ix.count[0] = all;
+    ix.count[1] = 0;
   }
 }
 
@@ -333,23 +387,36 @@ PF_API int pf_head_fwd(const void* x, const void* w, const void* target, void* x
   double* sums = reinterpret_cast<double*>(parts + n_parts * Mp);
   float* picked = reinterpret_cast<float*>(sums + Mp / FOLD_ROWS + 1);
   float* each = reduction == 0 ? static_cast<float*>(loss) : nullptr;
-  after(head_rows_kernel, 1, 1024, 0, st)((const long long*)target, ix, each, (int)N, V, ignore_index);
-  PF_CHECK_LAUNCH();
-  if (N > 0) {
-    const int vec = D == Dp && ldx % 8 == 0 && on_vectors(x);
-    const unsigned grid = (unsigned)(Mp / 8);
-    if (dtype == PF_F16)
-      after(head_gather_kernel<__half>, grid, 256, 0, st)((const __half*)x, (__half*)xc, ix, (int)Mp, D, Dp, ldx, vec);
-    else
-      after(head_gather_kernel<__nv_bfloat16>, grid, 256, 0, st)((const __nv_bfloat16*)x, (__nv_bfloat16*)xc, ix,
-                                                                 (int)Mp, D, Dp, ldx, vec);
+  const int vec = D == Dp && ldx % 8 == 0 && on_vectors(x);
+  const unsigned eights = (unsigned)(Mp / 8);
+  auto pick = [&](auto type) -> int {
+    using T = decltype(type);
+    after(head_pick_kernel<T>, eights, 256, 0, st)((const long long*)target, (const T*)x, (T*)xc, ix, each, (int)N,
+                                                   (int)Mp, D, Dp, ldx, V, ignore_index, vec);
     PF_CHECK_LAUNCH();
+    return 0;
+  };
+  auto gather = [&](auto type) -> int {
+    using T = decltype(type);
+    after(head_gather_kernel<T>, eights, 256, 0, st)((const T*)x, (T*)xc, ix, (int)Mp, D, Dp, ldx, vec);
+    PF_CHECK_LAUNCH();
+    return 0;
+  };
+  int r = 0;
+  if (N > 0 && N <= PICK_ROWS) {
+    r = dtype == PF_F16 ? pick(__half()) : pick(__nv_bfloat16());
+  } else {
+    after(head_rows_kernel, 1, 1024, 0, st)((const long long*)target, ix, each, (int)N, V, ignore_index);
+    PF_CHECK_LAUNCH();
+    if (N > 0) r = dtype == PF_F16 ? gather(__half()) : gather(__nv_bfloat16());
+  }
+  if (r) return r;
+  if (N > 0) {
     FusedCall c;
     c.M = (int)N; c.N = (int)V; c.K = Dp; c.A = xc; c.B = w; c.lda = Dp; c.ldb = ldw; c.dtype = dtype;
     c.rows = ix.count; c.labels = ix.labels; c.parts = parts; c.part_pitch = Mp; c.picked = picked;
     c.status = status; c.sm_count = sm_count; c.stream = st;
-    const int r = fused_gemm(HEAD_STATS, c);
-    if (r) return r;
+    if ((r = fused_gemm(HEAD_STATS, c))) return r;
   }
   const unsigned grid = (unsigned)(N > 0 ? (N + FOLD_ROWS - 1) / FOLD_ROWS : 1);
   after(head_fold_kernel, grid, 1024, 0, st)((const RowStat*)parts, Mp, n_parts, (const float*)picked, ix,

@@ -181,6 +181,8 @@ MLP = [(1, 8, 8, 8, "silu", False, False), (3, 16, 24, 8, "gelu", True, False), 
        (129, 72, 136, 40, "gelu_tanh", True, True), (257, 264, 520, 264, "gelu", True, True),
        (7, 128, 1000, 72, "silu", True, False), (300, 40, 64, 1032, "gelu_tanh", False, False),
        (2500, 128, 648, 128, "silu", False, True),       # tiles of pairs, the last of them ragged
+       (1, 2048, 1024, 2056, "gelu", True, True), (130, 1032, 2048, 520, "silu", True, False),    # products in parts
+       (300, 4096, 2560, 1024, "gelu_tanh", False, True),
        (5, 20, 30, 12, "silu", True, True), (33, 24, 27, 16, "gelu", False, True), (2, 3, 1, 1, "silu", False, False)]
 
 
@@ -337,6 +339,28 @@ def test_head_in_pieces(reduction):
     want = head64(x, w, target, g, reduction, U[torch.bfloat16], 2.0 ** 100)
     within(dx, *want[1])
     within(dw, *want[2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [4095, 4097, 9000])
+def test_many_rows_of_which_some_count(N):
+    """Beyond the calls in which every CTA looks at all labels, too."""
+    D, V = 24, 70
+    x = normal(N, D, device="cuda", dtype=torch.float16, seed=1).requires_grad_()
+    w = normal(V, D, device="cuda", dtype=torch.float16, seed=2, std=0.4).requires_grad_()
+    target = torch.randint(0, V, (N,), generator=gen(3))
+    target[torch.rand(N, generator=gen(4)) < 0.4] = -100
+    target[100:1300], target[-70:] = -1, V
+    target = target.cuda()
+    g = torch.rand(N, generator=gen(5)).cuda() + 0.1
+    loss = ops.linear_cross_entropy(x, w, target, reduction="none")
+    dx, dw = torch.autograd.grad(loss, [x, w], g)
+    want = head64(x, w, target, g, "none", U[torch.float16], 2.0 ** 15 / 2 * float(g.min() / g.max()))
+    within(loss.detach(), *want[0])
+    within(dx, *want[1])
+    within(dw, *want[2])
+    out = (target < 0) | (target >= V)
+    assert not loss[out].any() and not dx[out].any()
 
 
 @pytest.mark.parametrize("device", DEVICES)
