@@ -677,9 +677,10 @@ def gated_mlp_bwd(dy: Tensor, x: Tensor, w1: Tensor, w2: Tensor, gu: Tensor, act
     H = w2.shape[1]
     empty = dy.new_empty(0)
     if not dy.numel():                   # no rows: the products would leave the weights' gradients as they are
-        zeros = lambda t, need: torch.zeros_like(t) if need else dy.new_empty(0)
-        return (dy.new_zeros(x.shape), zeros(w1, need_dw1), dy.new_zeros(2 * H if need_db1 else 0, dtype=torch.float32),
-                zeros(w2, need_dw2), dy.new_zeros(w2.shape[0] if need_db2 else 0, dtype=torch.float32))
+        zeros = lambda n, t, need, **kw: dy.new_zeros(n if need and _grad_bucket(t) is None else 0, **kw)
+        f32 = dict(dtype=torch.float32)
+        return (dy.new_zeros(x.shape), zeros(w1.shape, w1, need_dw1, dtype=w1.dtype), zeros(2 * H, b1, need_db1, **f32),
+                zeros(w2.shape, w2, need_dw2, dtype=w2.dtype), zeros(w2.shape[0], b2, need_db2, **f32))
     native = dy.is_cuda and cd in (torch.float16, torch.bfloat16)
     if _glu_native(dy, cd, w1, w2):
         return _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1, b2)
@@ -1421,22 +1422,24 @@ def head_loss_fwd(x: Tensor, w: Tensor, target: Tensor, ignore_index: int, reduc
     Mp, Dp, size = _head_kept(N, D)
     target = target.long()
     counted = _tokens_counted(target, w.shape[0], ignore_index)
-    rows = counted.nonzero().squeeze(1)
-    M = rows.shape[0]
+    rows = counted.sort(descending=True, stable=True).indices        # the rows that count first; how many, no host knows
+    live = counted[rows]
+    labels = target[rows].masked_fill(~live, 0)
     xc = x.new_zeros((Mp, Dp), dtype=cd)
-    xc[:M, :D] = x[rows]
+    xc[:N, :D] = x[rows].masked_fill(~live.unsqueeze(1), 0)
     index = torch.zeros(size, dtype=torch.int32, device=x.device)
-    index[0] = M
-    index[4:4 + M] = rows
-    index[4 + Mp:4 + Mp + M] = target[rows]
+    index[0] = counted.sum()
+    index[4:4 + N] = rows
+    index[4 + Mp:4 + Mp + N] = labels
     index[4 + 2 * Mp:] = torch.where(counted, counted.cumsum(0) - 1, -1)
-    z = _wide(F.linear(_wide(xc[:M, :D]), _wide(w.to(cd))))
-    each = torch.logsumexp(z, -1) - z.gather(1, target[rows].unsqueeze(1)).squeeze(1)
-    inv = x.new_tensor(1.0 / max(M, 1) if reduction == 1 else 1.0, dtype=torch.float32)
+    z = _wide(F.linear(_wide(xc[:N, :D]), _wide(w.to(cd))))
+    each = (torch.logsumexp(z, -1) - z.gather(1, labels.unsqueeze(1)).squeeze(1)).masked_fill(~live, 0)
+    count = index[0].clamp(min=1) if reduction == 1 else torch.ones_like(index[0])
+    inv = 1.0 / count.float()
     if reduction == 0:
         loss = z.new_zeros(N).index_copy(0, rows, each)
     else:
-        loss = each.double().sum() / (max(M, 1) if reduction == 1 else 1)
+        loss = each.double().sum() / count
     return loss.to(_loss_dtype(x)), xc, index, x.new_zeros((Mp, 2), dtype=torch.float32), inv
 
 
@@ -1472,16 +1475,17 @@ def head_loss_bwd(dloss: Tensor, xc: Tensor, index: Tensor, stats: Tensor, inv: 
         if bucket is not None or not need_dw:
             dw = xc.new_empty(0, dtype=w.dtype)
         return dx if need_dx else xc.new_empty(0), dw.to(w.dtype)
-    Mp, M = kx.head_padded(N), int(index[0])
-    rows, labels = (index[i:i + M].long() for i in (4, 4 + Mp))
-    x, wide = _wide(xc[:M, :D]), _wide(w.to(xc.dtype))
+    Mp = kx.head_padded(N)
+    rows, labels = (index[i:i + N].long() for i in (4, 4 + Mp))
+    behind = (torch.arange(N, device=xc.device) >= index[0]).unsqueeze(1)        # rows that do not count
+    x, wide = _wide(xc[:N, :D]), _wide(w.to(xc.dtype))
     p = torch.softmax(F.linear(x, wide), -1)
-    p[torch.arange(M, device=p.device), labels] -= 1
+    p = p.scatter_add(1, labels.unsqueeze(1), p.new_full((N, 1), -1.0))
     g = dloss.to(p.dtype)
-    p = p * (g[rows].unsqueeze(1) if by_row else g * inv.to(p.dtype))
+    p = (p * (g[rows].unsqueeze(1) if by_row else g * inv.to(p.dtype))).masked_fill(behind, 0)
     dx = xc.new_empty(0)
     if need_dx:
-        dx = p.new_zeros(N, D).index_copy(0, rows, p @ wide).to(xc.dtype)
+        dx = p.new_zeros(N, D).index_copy(0, rows, (p @ wide).masked_fill(behind, 0)).to(xc.dtype)
     return dx, (p.t() @ x).to(w.dtype) if need_dw else xc.new_empty(0, dtype=w.dtype)
 
 
@@ -1629,9 +1633,11 @@ def scaled_embed_bwd(dout: Tensor, ids: Tensor, table: Tensor, scale: float) -> 
         same = table.dtype == dout.dtype
         g = kx.scaled_embed_bwd(dout, ids, table.shape[0], scale, table.dtype if same else torch.float32)
         return g.to(table.dtype)
-    inside = ((ids >= 0) & (ids < table.shape[0])).reshape(-1)
+    outside = ((ids < 0) | (ids >= table.shape[0])).reshape(-1)
     g = torch.zeros(table.shape, dtype=_wide(table).dtype, device=table.device)
-    g.index_add_(0, ids.reshape(-1)[inside].long(), dout.reshape(-1, table.shape[1])[inside].to(g.dtype))
+    if table.shape[0]:
+        rows = dout.reshape(-1, table.shape[1]).to(g.dtype).masked_fill(outside.unsqueeze(1), 0)
+        g.index_add_(0, ids.reshape(-1).long().masked_fill(outside, 0), rows)
     return (g * scale).to(table.dtype)
 
 

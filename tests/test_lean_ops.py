@@ -11,6 +11,8 @@ import pytest
 import torch
 
 from pfeife_b200 import ops
+from pfeife_b200.ops import _lib
+from test_kernel_calls import calls  # noqa: F401
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
@@ -495,6 +497,71 @@ def test_operands_of_two_devices_are_refused():
             bad()
 
 
+BF16, F32 = _lib.PF_BF16, _lib.PF_F32
+# Entry points with operands of 16 bytes a time: arguments of a call that is all right but for what is put in place of one,
+# and the positions of those operands.  None of them reaches a device: the first that is wrong is refused.
+ENTRIES = {
+    "pf_gated_mlp_fwd": (lambda t: [t, t, None, 0, t, None, 0, t, t, t, t, None, 0, 4, 8, 8, 8, 8, 8, 8, 8, 3, BF16, None,
+                                    148, None], (0, 4, 7, 8, 9, 10)),
+    "pf_gated_mlp_bwd": (lambda t: [t, t, t, t, t, t, t, t, t, t, None, None, None, 0, 4, 8, 8, 8, 8, 8, 8, 8, 3, BF16,
+                                    BF16, BF16, 0, 0, 0, None, 148, None], range(10)),
+    "pf_head_fwd": (lambda t: [t, t, t, t, t, t, t, t, t, 4, 8, 8, 8, 8, 8, -100, 1, BF16, None, 148, None], (1, 3, 8)),
+    "pf_head_bwd": (lambda t: [t, t, t, t, t, t, t, t, t, t, None, 4, 8, 8, 8, 0, 8, 8, 0, 0, BF16, BF16, None, 148, None],
+                    (2, 3, 7, 8, 9)),
+    "pf_scaled_embed_bwd": (lambda t: [t, t, t, t, 4, 8, 8, 1.0, 0, BF16, BF16, None], (3,)),
+}
+
+
+@pytest.mark.parametrize("name", ENTRIES)
+def test_operands_off_their_boundaries(name, calls):
+    make, places = ENTRIES[name]
+    t = torch.zeros(4096, dtype=torch.bfloat16)
+    for i in places:
+        args = make(t.data_ptr())
+        args[i] = t.data_ptr() + 2
+        assert getattr(calls, name)(*args) == -2, i
+
+
+def test_entry_points_refuse(calls):
+    t = torch.zeros(4096, dtype=torch.bfloat16).data_ptr()
+
+    def answer(name, **put):
+        args = ENTRIES[name][0](t)
+        for i, v in put.items():
+            args[int(i[1:])] = v
+        return getattr(calls, name)(*args)
+    fwd, bwd = "pf_gated_mlp_fwd", "pf_gated_mlp_bwd"
+    assert answer(fwd, _22=F32) == answer(bwd, _23=F32) == -1
+    assert answer(fwd, _21=0) == answer(fwd, _21=4) == answer(bwd, _22=7) == -1
+    assert answer(fwd, _14=0) == answer(fwd, _13=-1) == answer(bwd, _16=0) == -3
+    assert answer(fwd, _14=12) == answer(fwd, _15=9) == answer(bwd, _17=20) == answer(fwd, _17=12) == answer(bwd, _18=9) == -2
+    assert answer(fwd, _13=0) == 0
+    assert answer(bwd, _28=1) == -1                          # 16-bit gradients are not added to
+    assert answer(bwd, _24=_lib.PF_F16) == -1
+    for name, dtype in (("pf_head_fwd", 17), ("pf_head_bwd", 20)):
+        assert answer(name, **{f"_{dtype}": F32}) == -1
+        at = 9 if name == "pf_head_fwd" else 11
+        assert answer(name, **{f"_{at}": -1}) == answer(name, **{f"_{at + 1}": 0}) == -3
+        assert answer(name, **{f"_{at}": (1 << 28) + 1}) == -3
+        assert answer(name, **{f"_{at + 3}": 12}) == answer(name, **{f"_{at + 5}": 12}) == -2
+    assert answer("pf_head_bwd", _19=1) == -1 == answer("pf_head_bwd", _21=_lib.PF_F16)
+    assert calls.pf_head_index(-1) == calls.pf_head_scratch(4, 0) == calls.pf_head_words(-1, 4) == -3
+    assert calls.pf_head_scratch(1 << 28, 1 << 28) == -3     # more KiB than an int has
+    assert calls.pf_scaled_embed_scratch(-1, 8, 8) == calls.pf_scaled_embed_scratch(8, 8, 1 << 30) == -3
+    assert answer("pf_scaled_embed_bwd", _4=-1) == -3 and answer("pf_scaled_embed_bwd", _8=1) == -1
+    assert answer("pf_scaled_embed_bwd", _3=t + 16) == -2 and answer("pf_scaled_embed_bwd", _6=0) == 0
+
+
+@pytest.mark.parametrize("N,V", [(1, 8), (256, 32000), (8192, 32000), (4095, 128011), (1 << 20, 50257)])
+def test_pieces_of_the_vocabulary(calls, N, V):
+    """Whole tiles of words, no more of them alive than 2^27 values unless a piece would have fewer than 4096 words, and all
+    of a vocabulary of that size in one piece."""
+    words, rows = calls.pf_head_words(N, V), (N + 255) // 256 * 256
+    assert words % 256 == 0 and 0 < words
+    assert words * rows <= 2 ** 27 or words <= 4096
+    assert words >= V or words >= 2048
+
+
 # ------------------------------------------------------------------------------ how a program uses them
 def _all(device, dtype, seed=0, N=70):
     """(leaves, a function that takes them through embedding, block and head to a loss)"""
@@ -545,6 +612,50 @@ def test_captured_and_replayed():
             want = run(ids, labels)
             assert torch.equal(want, loss)
             assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(want, leaves), grads))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64], ids=str)
+def test_captured_in_full_precision(dtype):
+    """PyTorch's own products ask the host for nothing either, and which rows count may differ from replay to replay."""
+    leaves, run = _all("cuda", dtype)
+    ids, labels = _data("cuda", 10)
+    for _ in range(2):
+        torch.autograd.grad(run(ids, labels), leaves)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = run(ids, labels)
+        grads = torch.autograd.grad(loss, leaves)
+    for seed in (30, 40):
+        new = _data("cuda", seed)
+        ids.copy_(new[0].masked_fill(new[0] < 5, -1))
+        labels.copy_(new[1].masked_fill(new[1] < seed - 20, -100))
+        graph.replay()
+        want = run(ids, labels)
+        assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
+        for a, b in zip(torch.autograd.grad(want, leaves), grads):
+            assert float((a - b).norm()) <= 1e-5 * float(a.norm())
+
+
+@pytest.mark.gpu
+def test_no_rows_leave_buckets_as_they_are():
+    leaves, run = _all("cuda", torch.float32)
+    biases = [torch.randn(96, device="cuda").requires_grad_(), torch.randn(32, device="cuda").requires_grad_()]
+    every = leaves[:3] + biases
+    buckets = [torch.full(t.shape, 3.0, device="cuda") for t in every]
+    try:
+        for t, b in zip(every, buckets):
+            ops.register_param(t, t.detach().to(torch.bfloat16), b)
+        ids = torch.zeros(0, dtype=torch.long, device="cuda")
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            h = ops.scaled_embedding(ids, leaves[0], 1.5)
+            y = ops.gated_mlp(h, leaves[1], biases[0], leaves[2], biases[1])
+        assert y.shape == (0, 32)
+        assert all(g is None for g in torch.autograd.grad(y.float().sum(), every, allow_unused=True))
+        assert all((b == 3.0).all() for b in buckets)
+    finally:
+        ops.unregister_params()
 
 
 @pytest.mark.gpu

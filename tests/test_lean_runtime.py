@@ -172,7 +172,7 @@ def test_a_transformer_layer_of_images(device):
 def test_the_trainer_with_the_lean_operators(mesh):
     """Two ranks of the example trainer, as stages and as replicas: it runs, and the loss is a number."""
     from test_examples import COMMON, _PORT, _launch
-    _PORT[0] += 40
+    _PORT[0] += 40 if mesh is None else 70        # both may run at the same time
     its, loss, _ = _launch("train_llama.py", ["--model", "llama_tiny", "--block_size", "16", "--lean",
                                              "--per_device_train_batch_size", "2", "--iter_cnt", "3"] + COMMON,
                            mesh=mesh)
