@@ -2,9 +2,19 @@
 // output head with its cross entropy, whose logits stay in TMEM.
 //
 // The main loop is that of gemm_sm100.cu: persistent CTAs, warp 0 the TMA producer, warp 1 the issuer of the
-// products, warps 2..9 the epilogue (a row per thread, half the tile's columns per warp), accumulators twice in
-// TMEM so that an epilogue runs under the next tile's products.  Tiles are 256 x 256 of a CTA pair
-// (cta_group::2) or 128 x 128 of one CTA.
+// products, the other warps the epilogue (a row per thread), accumulators twice in TMEM so that an epilogue runs
+// under the next tile's products.  Tiles are 256 x 256 of a CTA pair (cta_group::2) or 128 x 128 of one CTA.
+//
+// In short runs on a B200, rows x columns x reduction, bf16:
+//   GLU_FWD     2048 x (2 x 11008) x 4096   245 us  1.51 PFLOP/s    16384 x (2 x 2560) x 640   90 us  1.19 PFLOP/s
+//   GLU_BWD     2048 x 11008 x 4096         150 us  1.23            16384 x 2560 x 640        110 us  0.49
+//   HEAD_STATS  2048 x 32000 x 4096         330 us  1.63            13 x 32000 x 4096          60 us  4.4 TB/s of W
+//   HEAD_DZ     the same                    339 us  1.58                                       49 us  5.4 TB/s
+//   PARTS_N     2048 x 4096 x 32000         370 us  1.45            13 x 4096 x 32000          44 us  6.0 TB/s
+//   HEAD_DW     32000 x 4096 x 2048         345 us  1.56            32000 x 4096 x 13          50 us  5.2 TB/s written
+// Products of many rows are bound by the tensor cores, or by rounds that tiles do not fill: PARTS_N above has 128 tiles for
+// 74 pairs, 86 % of two rounds.  GLU_BWD moves 10 bytes for each of its values (420 MB for the short reduction, 63 us) and
+// has the longest epilogue, which a reduction of 640 does not cover.  Products of few rows are bound by memory.
 //
 // GLU_FWD: a tile has as many gate columns as up columns.  B comes from two tensor maps, the gate and the up rows of
 // one weight; of a pair, the even CTA loads the gate rows and the odd one the up rows, so that the accumulator
@@ -21,8 +31,7 @@ namespace pf {
 
 int make_tmap_2d_16bit(CUtensorMap* map, const void* base, int fmt, long long inner, long long outer, long long ld,
                        int box_inner, int box_outer);
-int make_tmap_out(CUtensorMap* map, const void* base, int out_dtype, long long cols, long long rows, long long ld,
-                  int box_cols);
+int make_tmap_out(CUtensorMap* map, const void* base, int out_dtype, long long cols, long long rows, long long ld);
 
 constexpr int FG_BM = 128, FG_BN = 128, FG_BK = 64;      // per CTA and k-block
 // Epilogue warps: a warp has 32 rows and, of a pair's tile, a fourth of its columns, of a single tile's a half.  With half
@@ -31,7 +40,7 @@ constexpr int epi_warps(bool pair) { return pair ? 16 : 8; }
 constexpr int fg_threads(bool pair) { return 64 + 32 * epi_warps(pair); }
 constexpr int FG_STAGE_BYTES = (FG_BM + FG_BN) * FG_BK * 2;
 constexpr int FG_GROUP_ROWS = 4096;                      // see GROUP_ROWS in gemm_sm100.cu
-constexpr long long FG_B_STAYS = 48ll << 20;
+constexpr long long FG_B_STAYS = 48ll << 20;             // bytes of B that stay in L2 beside what streams through it
 
 // Shared memory of a job: stages of operands, barriers, and the boxes (32 rows of BW columns) in which an epilogue warp
 // turns its rows of the accumulator into lines of the output.
@@ -130,7 +139,8 @@ __device__ __forceinline__ void act2(float z0, float z1, uint64_t& a, uint64_t& 
 }
 
 // The values of an accumulator are in registers (tcgen05.wait::ld) and nothing else is handed over with this arrival: a
-// release would first wait for the stores that are on their way to memory, a tenth of a small reduction's time.
+// release would first wait for the stores that are on their way to memory.  (dW of 13 rows, 262 MB of stores, 72 us with a
+// release and 50 so; GLU_FWD over 16384 x 2560 at a reduction of 640 100 and 86.)
 __device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -173,7 +183,7 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
       : "memory");
 }
 
-// Where 16 bytes lie in a box as TMA reads it: chunk c of row r, rows of 128 bytes swizzled over 128 or of 64 over 64.
+// Where 16 bytes lie in a box, as TMA has it for outputs that are added to: chunk c of row r, rows of 128 bytes swizzled over 128 or of 64 over 64.
 // The 16-byte accesses of eight lanes, of one row or one chunk, meet no bank twice.
 template <int ROW_BYTES>
 __device__ __forceinline__ uint4* box_at(uint8_t* box, int r, int c) {
@@ -369,8 +379,7 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    // A box that the warp has filled, to memory: 16 bytes a lane, whole rows of the box behind one another.  (As TMA
-    // stores the boxes take about 13 bytes a clock of each SM: 262 MB of dW of few rows 72 us.)
+    // A box that the warp has filled, to memory: 16 bytes a lane, whole rows of the box behind one another.
     constexpr int CPR = RB / 16, RPI = 32 / CPR, PER = 16 / sizeof(OutT);      // chunks of a row, rows of an access
     auto store = [&](uint8_t* box, void* C, long long ldc, int col, int row0, int rows) {
       __syncwarp();
@@ -831,12 +840,13 @@ int fused_gemm(Job job, const FusedCall& c) {
   } else {
     if ((r = make_tmap_2d_16bit(&maps.b, B, fmt, c.N, c.K, c.ldb, 64, FG_BK))) return r;
   }
-  if (c.accumulate && (r = make_tmap_out(&maps.c, c.C, PF_F32, c.N, c.M, c.ldc, 32))) return r;
+  if (c.accumulate && (r = make_tmap_out(&maps.c, c.C, PF_F32, c.N, c.M, c.ldc))) return r;
   FusedParams p;
   memset(&p, 0, sizeof(p));
   p.M = c.M; p.N = c.N; p.K = c.K; p.fmt = fmt;
   p.group_m = FG_GROUP_ROWS / (pair ? 2 * FG_BM : FG_BM);
-  // Where all of B stays in L2, the tiles in flight are whole rows of the output instead, which DRAM takes better.
+  // Where all of B stays in L2, the tiles in flight are whole rows of the output instead, which DRAM takes better (GLU_FWD
+  // over 16384 x 2560 at a reduction of 640: 90 us, 93 in bands; over 8192 x 5120 at 1280: 154 and 156).
   const int bt = pair ? 2 * FG_BM : FG_BM, nt = job == GLU_FWD ? bt / 2 : bt;
   const int columns = (c.N + nt - 1) / nt, workers = pair ? c.sm_count / 2 : c.sm_count;
   if ((long long)c.N * c.K * (job == GLU_FWD ? 4 : 2) <= FG_B_STAYS) p.group_m = (workers + columns - 1) / columns;

@@ -784,23 +784,23 @@ int make_tmap_2d_16bit(CUtensorMap* map, const void* base, int fmt, long long in
   return r == CUDA_SUCCESS ? 0 : -(1000 + (int)r);
 }
 
-// [rows, cols] output map with a box of 32 rows x 64 or 128 bytes, swizzled over as many: 32 columns of
-// either type, or 64 16-bit ones
+// [rows, cols] output map with a 32 x 32 box; 16-bit: 64 B rows (SWIZZLE_64B), fp32: 128 B rows
+// (SWIZZLE_128B)
 int make_tmap_out(CUtensorMap* map, const void* base, int out_dtype, long long cols,
-                  long long rows, long long ld, int box_cols) {
+                         long long rows, long long ld) {
   EncodeTiledFn enc = get_encode();
   if (!enc) return -100;
   const int es = out_dtype == PF_F32 ? 4 : 2;
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)ld * es};
-  cuuint32_t box[2] = {(cuuint32_t)box_cols, 32};
+  cuuint32_t box[2] = {32, 32};
   cuuint32_t estr[2] = {1, 1};
   const CUtensorMapDataType dt = out_dtype == PF_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                  : out_dtype == PF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUresult r = enc(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   box_cols * es == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   out_dtype == PF_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                    CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -(1000 + (int)r);
 }
@@ -1087,10 +1087,10 @@ PF_API int pf_gemm(const void* A, const void* B, void* C, int M, int N, int K, l
   memset(&tc, 0, sizeof(tc));
   memset(&taux, 0, sizeof(taux));
   if (p.tma_store) {
-    if ((r = make_tmap_out(&tc, dst, out_dtype, N, dst_rows, dst_ld, 32))) return r;
+    if ((r = make_tmap_out(&tc, dst, out_dtype, N, dst_rows, dst_ld))) return r;
     const bool aux_is_out = aux && (epilogue == EPI_GELU || epilogue == EPI_GELU_TANH ||
                                     epilogue == EPI_SILU);
-    if (aux_is_out && (r = make_tmap_out(&taux, aux, out_dtype, N, M, ldaux, 32))) return r;
+    if (aux_is_out && (r = make_tmap_out(&taux, aux, out_dtype, N, M, ldaux))) return r;
   }
 
   const bool gather = g_gather.world > 1;

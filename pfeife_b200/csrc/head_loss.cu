@@ -10,6 +10,11 @@
 // dx, which adds up in fp32.  Four products of 2 rows D V operations where keeping the logits takes three: what is kept
 // from forward to backward is the rows and 8 bytes of each, and what is alive at one time PIECE values.
 //
+// On a B200, bf16, forward and backward, 4096 values a row and 32000 words: 2048 rows 1.42 ms in a short run (four
+// products 1384 us at 1.45 to 1.63 PFLOP/s, picking the rows 12, the fold 13, dx 13); 13 rows 0.23 ms, bound by what
+// memory takes for W three times and dW once.  The fold reads 8 bytes of each row and 64 words, 1/16 of what the logits
+// in 16 bits would be.
+//
 // dz is rounded to 16 bits as p - onehot, times 2^15 for fp16: from 6e-5 / 2^15 on the probabilities keep all
 // their bits, whatever the gradient of the loss is; that and the mean's factor come in 32 bits behind the products.
 #include "common.cuh"
