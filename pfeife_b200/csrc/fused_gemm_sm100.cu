@@ -8,9 +8,9 @@
 // In short runs on a B200, rows x columns x reduction, bf16:
 //   GLU_FWD     2048 x (2 x 11008) x 4096   245 us  1.51 PFLOP/s    16384 x (2 x 2560) x 640   90 us  1.19 PFLOP/s
 //   GLU_BWD     2048 x 11008 x 4096         150 us  1.23            16384 x 2560 x 640        110 us  0.49
-//   HEAD_STATS  2048 x 32000 x 4096         330 us  1.63            13 x 32000 x 4096          60 us  4.4 TB/s of W
-//   HEAD_DZ     the same                    339 us  1.58                                       49 us  5.4 TB/s
-//   PARTS_N     2048 x 4096 x 32000         370 us  1.45            13 x 4096 x 32000          44 us  6.0 TB/s
+//   HEAD_STATS  2048 x 32000 x 4096         330 us  1.63            13 x 32000 x 4096          58 us  4.5 TB/s of W
+//   HEAD_DZ     the same                    339 us  1.58                                       48 us  5.5 TB/s
+//   PARTS_N     2048 x 4096 x 32000         370 us  1.45            13 x 4096 x 32000          42 us  6.2 TB/s
 //   HEAD_DW     32000 x 4096 x 2048         345 us  1.56            32000 x 4096 x 13          50 us  5.2 TB/s written
 // Products of many rows are bound by the tensor cores, or by rounds that tiles do not fill: PARTS_N above has 128 tiles for
 // 74 pairs, 86 % of two rounds.  GLU_BWD moves 10 bytes for each of its values (420 MB for the short reduction, 63 us) and
@@ -55,6 +55,13 @@ struct FusedSmem {
   static constexpr int STAGES = STAGING <= 32768 ? 6 : 5;
   static constexpr int BAR_OFFSET = STAGES * FG_STAGE_BYTES;
   static constexpr int STAGING_OFFSET = BAR_OFFSET + 1024;
+  // With A boxes of fewer rows there are as many stages as have room.  (13 rows over 11008 x 4096 weights, 11 for 6: products
+  // with N innermost 40 us for 44, K innermost 34 for 35, GLU_BWD 26 for 30.)
+  static constexpr int MOST = PAIR ? STAGES : 12;
+  static constexpr int stages(int a_rows) {
+    const int n = BAR_OFFSET / ((a_rows + FG_BN) * FG_BK * 2);
+    return n < MOST ? n : MOST;
+  }
   static constexpr int TOTAL = STAGING_OFFSET + STAGING + 1024;
   static_assert(TOTAL <= 232448, "more than a CTA may have");
 };
@@ -67,7 +74,7 @@ struct FusedParams {
   void* two;                     // gate and up [M, 2 N], or their gradients
   long long ldc;
   int c_rows;                    // rows of C that may be written
-  int a_rows;                    // rows of A that a CTA loads: all of a tile's, or as many as there are
+  int a_rows;                    // rows of A that a CTA loads: all of a tile's, or as many as there are, in eights
   const int* rows;
   int* status;
   const void* gu;
@@ -197,13 +204,14 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
   constexpr int BMT = PAIR ? 2 * FG_BM : FG_BM;
   constexpr int BNT = PAIR ? 2 * FG_BN : FG_BN;           // accumulator columns of a tile
   constexpr int NT = JOB == GLU_FWD ? BNT / 2 : BNT;      // output columns of a tile
-  constexpr int STAGES = S::STAGES;
+  const int a_bytes = PAIR || A_MN ? FG_BM * FG_BK * 2 : p.a_rows * FG_BK * 2;
+  const int STAGES = PAIR || A_MN ? S::STAGES : S::stages(p.a_rows), stage_bytes = a_bytes + FG_BN * FG_BK * 2;
   constexpr uint32_t TMEM_COLS = 2 * BNT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::BAR_OFFSET);
-  uint64_t* empty_bar = full_bar + STAGES;
-  uint64_t* tmem_full = empty_bar + STAGES;
+  uint64_t* empty_bar = full_bar + S::MOST;
+  uint64_t* tmem_full = empty_bar + S::MOST;
   uint64_t* tmem_empty = tmem_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
 
@@ -277,11 +285,11 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = mbar_wait(&empty_bar[stage], phase ^ 1, p.status, PF_ERR_TIMEOUT_EMPTY);
           if (!ok) break;
-          uint8_t* sa = smem + stage * FG_STAGE_BYTES;
-          uint8_t* sb = sa + FG_BM * FG_BK * 2;
+          uint8_t* sa = smem + stage * stage_bytes;
+          uint8_t* sb = sa + a_bytes;
           const int k0 = kb * FG_BK;
           if (!PAIR || cta_rank == 0)
-            mbar_expect_tx(&full_bar[stage], (PAIR ? 2 : 1) * ((A_MN ? FG_BM : p.a_rows) + FG_BN) * FG_BK * 2);
+            mbar_expect_tx(&full_bar[stage], (PAIR ? 2 : 1) * stage_bytes);
           auto load = [&](uint8_t* to, const CUtensorMap* map, int x, int y) {
             if (PAIR) tma_load_2d_pair(to, map, full_leader + stage * 8, x, y);
             else tma_load_2d(to, map, &full_bar[stage], x, y);
@@ -332,8 +340,8 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
           ok = mbar_wait(&full_bar[stage], phase, p.status, PF_ERR_TIMEOUT_FULL);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * FG_STAGE_BYTES);
-          const uint32_t a_lo = desc_lo(sa, a_lbo), b_lo = desc_lo(sa + FG_BM * FG_BK * 2, b_lbo);
+          const uint32_t sa = smem_u32(smem + stage * stage_bytes);
+          const uint32_t a_lo = desc_lo(sa, a_lbo), b_lo = desc_lo(sa + a_bytes, b_lbo);
 #pragma unroll
           for (int k = 0; k < FG_BK / 16; ++k) {
             const uint32_t on = (kb != kb0) || (k != 0);
@@ -841,7 +849,8 @@ int fused_gemm(Job job, const FusedCall& c) {
     return -2;
   const int fmt = c.dtype == PF_BF16;
   const bool pair = c.tile < 0 ? fused_pairs(job, c.M, c.N, c.sm_count) : c.tile;
-  // Fewer rows than a tile has are loaded as what they are: rows of accumulators that no row of A fills are not read.
+  // Fewer rows than a tile has are loaded as what they are: rows of accumulators that no row of A fills are not read.  (What
+  // lies behind them in shared memory, B's tile, is multiplied, too; it is inside the stage.)
   const int a_rows = pair || c.M >= FG_BM ? FG_BM : (c.M + 7) / 8 * 8;
   FusedMaps maps;
   memset(&maps, 0, sizeof(maps));

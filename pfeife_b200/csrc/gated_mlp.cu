@@ -8,8 +8,8 @@
 // add the parts up in their order.
 //
 // On a B200, bf16, forward and backward: 2048 rows of 4096 over 11008 hidden values (1.66 TFLOP) 1.18 ms in a short run,
-// 1.41 PFLOP/s; 16384 of 640 over 2560 with biases 590 us, 0.82 PFLOP/s, where gate, up, h and their gradients are 27 MB
-// a thousand rows; 13 of 4096 over 11008 192 us, of which 124 are what memory takes for the weights twice and their
+// 1.41 PFLOP/s; 16384 of 640 over 2560 with GELU and biases 575 us, 0.84 PFLOP/s, where gate, up, h and their gradients are 27 MB
+// a thousand rows; 13 of 4096 over 11008 184 us, of which 124 are what memory takes for the weights twice and their
 // gradients once.
 #include "common.cuh"
 #include "api.h"
