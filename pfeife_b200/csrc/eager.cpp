@@ -1318,7 +1318,7 @@ struct DirectHeadLoss : torch::autograd::Function<DirectHeadLoss> {
         if (nw) dw = empty(w.sizes(), xc);
         const int words = pf_head_words(N, V), parts = pf_head_parts(N, V, (int)D, e.sms);
         if (words < 0 || parts < 0) throw Failed{words < 0 ? words : parts, "pf_head_words"};
-        const Tensor dz = empty({Mp, words}, xc), acc = nx ? floats(parts * Mp * D, xc) : Tensor();
+        const Tensor dz = empty({Mp, words}, xc), acc = nx ? floats(parts * Mp * D + 1, xc) : Tensor();
         const Tensor factor = by_row ? floats(Mp + 1, xc) : Tensor();
         auto out = [](const Tensor& t) { return const_cast<void*>(at_or_null(t)); };
         ok(pf_head_bwd(g.data_ptr(), inv.data_ptr(), xc.data_ptr(), w.data_ptr(), index.data_ptr(), stats.data_ptr(),

@@ -18,6 +18,23 @@ enum Job : int {
 // What a row of the product has of the loss: reference and one over the sum; its label.
 struct RowStat { float ref, inv; };
 
+// Parts of a product whose rows are counted on the device: as many as keep `slots` workers busy and have room, none of
+// fewer than 8 k-blocks, and no fewer than were planned for all rows.
+struct PartRule {
+  int tile_rows = 0, columns = 0, slots = 0;      // rows of a tile, tiles side by side
+  int kb = 0, planned = 1, rows = 0;              // k-blocks of 64; rows of the parts' memory
+};
+__host__ __device__ inline int rows_of_part(int count) { return (count + 255) / 256 * 256; }
+__host__ __device__ inline int parts_of(const PartRule& r, int count) {
+  const int tiles = (count + r.tile_rows - 1) / r.tile_rows * r.columns;
+  if (!tiles) return r.planned;
+  int p = r.slots / tiles;
+  p = p < r.kb / 8 ? p : r.kb / 8;
+  p = p < r.rows / rows_of_part(count) ? p : r.rows / rows_of_part(count);
+  p = p < 16 ? p : 16;
+  return p > r.planned ? p : r.planned;
+}
+
 struct FusedCall {
   // product [M, N] over K.  GLU_FWD: N hidden values, each of two columns
   int M = 0, N = 0, K = 0;
@@ -45,9 +62,13 @@ struct FusedCall {
   float unit = 1.f;
   int split = 1;               // PARTS: parts of the reduction, part i in rows i * part_rows of C on
   int part_rows = 0;
+  PartRule rule;               // PARTS with `rows`: its parts, each rows_of_part(*rows) rows behind the one before;
+  int* parts_word = nullptr;   // how many they are, for whoever adds them up
+  void* direct = nullptr;      // [*, N] 16-bit: where there is one part, its rows go, scaled, to the rows of `list` instead
+  const int* list = nullptr;
   int tile = -1;               // 1: tiles of CTA pairs, 0: of one CTA; -1: as fused_pairs has it
   int accumulate = 0;          // PARTS, HEAD_DW in fp32: add to C
-  const float* scale = nullptr;    // HEAD_DW: *scale times *scale2 (where given) times scale3
+  const float* scale = nullptr;    // HEAD_DW, direct: *scale times *scale2 (where given) times scale3
   const float* scale2 = nullptr;
   float scale3 = 1.f;
   int* status = nullptr;

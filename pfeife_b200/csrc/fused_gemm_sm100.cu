@@ -88,6 +88,10 @@ struct FusedParams {
   const float* factor;
   float unit;
   int first, split, part_rows, accumulate;
+  PartRule rule;
+  int* parts_word;
+  void* direct;
+  const int* list;
   const float *scale, *scale2;
   float scale3;
 };
@@ -254,9 +258,12 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
   const int M = p.rows && JOB != HEAD_DW ? count : p.M;
   const int K = p.rows && JOB == HEAD_DW ? count : p.K;
   const int num_m = (M + BMT - 1) / BMT, num_n = (p.N + NT - 1) / NT, num_mn = num_m * num_n;
-  const int split = PARTS ? p.split : 1;
-  const int num_items = num_mn * split;
   const int num_kb = (K + FG_BK - 1) / FG_BK;
+  // a last piece of few words adds to the first parts only
+  const int split = !PARTS ? 1 : p.rows ? max(1, min(parts_of(p.rule, count), num_kb / 8)) : p.split;
+  const int part_rows = PARTS && p.rows ? rows_of_part(count) : p.part_rows;
+  if (PARTS && p.parts_word && blockIdx.x == 0 && threadIdx.x == 0) *p.parts_word = split;
+  const int num_items = num_mn * split;
   // Items are dealt in rounds, every other one in reverse; tiles in bands of group_m rows of tiles, column by column.
   auto item_of = [&](int round) { return round * n_workers + ((round & 1) ? n_workers - 1 - first_tile : first_tile); };
   auto place = [&](int item, int& mt, int& nt, int& kb0, int& kb1) {
@@ -390,7 +397,8 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
       __syncwarp();
     };
     float alpha = 1.f;
-    if (JOB == HEAD_DW) alpha = (p.scale ? *p.scale : 1.f) * (p.scale2 ? *p.scale2 : 1.f) * p.scale3;
+    const bool direct = PARTS && p.direct && split == 1;
+    if (JOB == HEAD_DW || direct) alpha = (p.scale ? *p.scale : 1.f) * (p.scale2 ? *p.scale2 : 1.f) * p.scale3;
 
     // GLU backward: gate and up of one of the warp's two chunks of 32 columns, in boxes whose places their gradients take.
     // The next is asked for as soon as a chunk has left its boxes, 16 bytes a lane and whole rows of a box behind one
@@ -453,6 +461,8 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
       const int row0 = mt * BMT + int(cta_rank) * FG_BM + quad * 32, row = row0 + lane;
       const int n0 = nt * NT;
       const bool row_ok = row < M;
+      [[maybe_unused]] int target = 0;                  // row of `direct` that the lane's row goes to
+      if (direct && row_ok) target = p.list[row];
 
       [[maybe_unused]] int label = -1;                  // as a column of this product
       [[maybe_unused]] float ref = 0.f, inv = 0.f, factor = 0.f, total = 0.f;
@@ -685,7 +695,7 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = 0.f;
               }
-            } else if (JOB == HEAD_DW) {
+            } else if (JOB == HEAD_DW || direct) {
               if (empty) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = 0.f;
@@ -695,17 +705,30 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
                   f2_unpack(mul2(f2_pack(v[i], v[i + 1]), f2_pack(alpha, alpha)), v[i], v[i + 1]);
               }
             }
-            fill_box<OutT, RB>(boxes, lane, s, v);
+            if (direct) fill_box<T, 64>(boxes, lane, 0, v);
+            else fill_box<OutT, RB>(boxes, lane, s, v);
           }
+          if (direct) {                                 // 16 bytes a lane, 64 of each row
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = 8 * i + (lane >> 2), to = __shfl_sync(0xffffffffu, target, r), at = col + (lane & 3) * 8;
+              if (row0 + r < M && at < p.N)
+                *reinterpret_cast<uint4*>(static_cast<T*>(p.direct) + (long long)to * p.N + at) =
+                    *box_at<64>(boxes, r, lane & 3);
+            }
+            __syncwarp();
+            continue;
+          }
+          const int part = PARTS ? ks * part_rows : 0;
           if (sizeof(OutT) == 4 && p.accumulate) {      // rows and columns that do not exist are clipped
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              if (row0 < M) tma_reduce_add_2d(&maps.c, boxes, col, row0);
+              if (row0 < M) tma_reduce_add_2d(&maps.c, boxes, col, row0 + part);
               tma_store_commit();
             }
           } else {
-            const int part = PARTS ? ks * p.part_rows : 0;
             store(boxes, p.C, p.ldc, col, row0 + part, JOB == HEAD_DZ ? p.c_rows : M + part);
           }
         }
@@ -749,8 +772,9 @@ static int launch_fused(const FusedMaps& maps, const FusedParams& p, int sm_coun
     if (known) configured[dev] = true;
   }
   constexpr int BMT = PAIR ? 2 * FG_BM : FG_BM, BNT = PAIR ? 2 * FG_BN : FG_BN, NT = JOB == GLU_FWD ? BNT / 2 : BNT;
-  const long long items = (long long)((p.M + BMT - 1) / BMT) * ((p.N + NT - 1) / NT) * p.split;
+  long long items = (long long)((p.M + BMT - 1) / BMT) * ((p.N + NT - 1) / NT) * p.split;
   if (items > 0x7fffffffll) return -3;
+  if (p.rule.rows && items < sm_count) items = sm_count;               // fewer rows may come in more parts
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(fg_threads(PAIR));
   cfg.dynamicSmemBytes = S::TOTAL;
@@ -869,7 +893,7 @@ int fused_gemm(Job job, const FusedCall& c) {
   } else {
     if ((r = make_tmap_2d_16bit(&maps.b, B, fmt, c.N, c.K, c.ldb, 64, FG_BK))) return r;
   }
-  if (c.accumulate && (r = make_tmap_out(&maps.c, c.C, PF_F32, c.N, c.M, c.ldc))) return r;
+  if (c.accumulate && (r = make_tmap_out(&maps.c, c.C, PF_F32, c.N, c.M > c.rule.rows ? c.M : c.rule.rows, c.ldc))) return r;
   FusedParams p;
   memset(&p, 0, sizeof(p));
   p.M = c.M; p.N = c.N; p.K = c.K; p.fmt = fmt;
@@ -886,6 +910,7 @@ int fused_gemm(Job job, const FusedCall& c) {
   p.a_rows = a_rows;
   p.C = c.C; p.ldc = c.ldc; p.two = job == GLU_FWD ? c.gu : c.dgu; p.c_rows = (c.M + 255) / 256 * 256;
   p.first = c.first; p.split = job == PARTS_K || job == PARTS_N ? c.split : 1; p.part_rows = c.part_rows; p.accumulate = c.accumulate;
+  p.rule = c.rule; p.parts_word = c.parts_word; p.direct = c.direct; p.list = c.list;
   p.scale = c.scale; p.scale2 = c.scale2; p.scale3 = c.scale3;
   return c.dtype == PF_F16 ? fused_by_job<__half>(job, maps, p, pair, c)
                            : fused_by_job<__nv_bfloat16>(job, maps, p, pair, c);

@@ -17,6 +17,7 @@
 //
 // dz is rounded to 16 bits as p - onehot, times 2^15 for fp16: from 6e-5 / 2^15 on the probabilities keep all
 // their bits, whatever the gradient of the loss is; that and the mean's factor come in 32 bits behind the products.
+#include <algorithm>
 #include "common.cuh"
 #include "api.h"
 #include "fused_gemm.h"
@@ -170,58 +171,63 @@ head_pick_kernel(const long long* __restrict__ target, const T* __restrict__ x, 
   }
 }
 
-// Joins the parts of FOLD_ROWS rows: 128 threads share the parts of a row, with lanes on neighbouring rows; then a warp
-// has a row.  References are integers: 2^(a - b) is exact.  The row's loss is formed in 64 bits; `sums` gets a CTA's sum
+// Joins the parts of ROWS rows: 1024 / ROWS threads share the parts of a row, with lanes on neighbouring rows; then a warp
+// has a row at a time.  Few parts would leave most of 128 threads with none (4 parts of 13965 rows: 40 us with 8 rows a CTA,
+// 10 with 128).  References are integers: 2^(a - b) is exact.  The row's loss is formed in 64 bits; `sums` gets a CTA's sum
 // of them, and the CTA that finishes last adds those up in their order.
-constexpr int FOLD_ROWS = 8, FOLD_LANES = 1024 / FOLD_ROWS;
+constexpr int FOLD_ROWS = 8, FOLD_MOST_ROWS = 128, FOLD_FEW_PARTS = 32;
 __device__ __forceinline__ void join(float& ref, float& sum, float ref2, float sum2) {
   const float m = fmaxf(ref, ref2), sub = m == -INFINITY ? 0.f : m;
   sum = sum * exp2f(ref - sub) + sum2 * exp2f(ref2 - sub);
   ref = m;
 }
+template <int ROWS>
 __global__ void __launch_bounds__(1024)
 head_fold_kernel(const RowStat* __restrict__ parts, long long pitch, int n_parts, const float* __restrict__ picked,
                  HeadIndex ix, RowStat* __restrict__ stats, float* __restrict__ loss_of_row, float* __restrict__ loss,
                  float* __restrict__ inv, double* __restrict__ sums, int mean) {
   after_previous();
-  __shared__ RowStat all[FOLD_ROWS][FOLD_LANES + 1];
-  __shared__ double rows[32];
+  constexpr int LANES = 1024 / ROWS;
+  __shared__ RowStat all[ROWS][LANES + 1];
+  __shared__ double rows[ROWS > 32 ? ROWS : 32];
   __shared__ int last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int count = *ix.count, row0 = blockIdx.x * FOLD_ROWS;
+  const int count = *ix.count, row0 = blockIdx.x * ROWS;
   if (row0 < count) {
-    const int r = threadIdx.x % FOLD_ROWS, l = threadIdx.x / FOLD_ROWS, row = row0 + r;
+    const int r = threadIdx.x % ROWS, l = threadIdx.x / ROWS, row = row0 + r;
     float ref = -INFINITY, sum = 0.f;
     if (row < count) {
       const RowStat* src = parts + row;
-      for (int k = l; k < n_parts; k += 8 * FOLD_LANES) {
+      for (int k = l; k < n_parts; k += 8 * LANES) {
         RowStat q[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-          if (k + FOLD_LANES * u < n_parts) q[u] = src[(k + FOLD_LANES * u) * pitch];
+          if (k + LANES * u < n_parts) q[u] = src[(k + LANES * u) * pitch];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-          if (k + FOLD_LANES * u < n_parts) join(ref, sum, q[u].ref, q[u].inv);
+          if (k + LANES * u < n_parts) join(ref, sum, q[u].ref, q[u].inv);
       }
     }
     all[r][l] = {ref, sum};
   }
   __syncthreads();
-  const int row = row0 + warp;
-  if (lane == 0) rows[warp] = 0.0;
-  if (warp < FOLD_ROWS && row < count) {
+  for (int r = warp; r < ROWS; r += 32) {
+    const int row = row0 + r;
+    if (lane == 0) rows[r] = 0.0;
+    if (row >= count) continue;
     float ref = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < FOLD_LANES / 32; ++k) join(ref, sum, all[warp][lane + 32 * k].ref, all[warp][lane + 32 * k].inv);
+    for (int k = 0; k < (LANES + 31) / 32; ++k)
+      if (LANES >= 32 || lane < LANES) join(ref, sum, all[r][lane + 32 * k].ref, all[r][lane + 32 * k].inv);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+    for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1)
       join(ref, sum, __shfl_xor_sync(0xffffffffu, ref, o), __shfl_xor_sync(0xffffffffu, sum, o));
     if (lane == 0) {
       if (ref == -INFINITY) ref = 0.f;
       stats[row] = {ref, 1.f / sum};
       constexpr double ln2 = 0.69314718055994531;
       const double l = (log2((double)sum) + (double)ref - (double)picked[row] * (double)1.4426950408889634f) * ln2;
-      rows[warp] = l;
+      rows[r] = l;
       if (loss_of_row) loss_of_row[ix.list[row]] = (float)l;
     }
   }
@@ -229,7 +235,7 @@ head_fold_kernel(const RowStat* __restrict__ parts, long long pitch, int n_parts
   __syncthreads();
   if (threadIdx.x == 0) {
     double s = 0.0;
-    for (int i = 0; i < FOLD_ROWS; ++i) s += rows[i];
+    for (int i = 0; i < ROWS; ++i) s += rows[i];
     sums[blockIdx.x] = s;
     __threadfence();
     last = atomicAdd(ix.count + 1, 1) == (int)gridDim.x - 1;
@@ -238,7 +244,7 @@ head_fold_kernel(const RowStat* __restrict__ parts, long long pitch, int n_parts
   if (!last) return;
   __threadfence();
   double s = 0.0;
-  for (int i = threadIdx.x; i < (count + FOLD_ROWS - 1) / FOLD_ROWS; i += 1024)
+  for (int i = threadIdx.x; i < (count + ROWS - 1) / ROWS; i += 1024)
     s += reinterpret_cast<volatile double*>(sums)[i];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -286,45 +292,60 @@ head_factor_kernel(const float* __restrict__ g, long long step, HeadIndex ix, fl
 constexpr int DX_COLUMNS = 512;
 template <typename T>
 __global__ void __launch_bounds__(256)
-head_dx_kernel(const float* __restrict__ acc, T* __restrict__ dx, HeadIndex ix, long long N, int D, int Dp, int parts,
-               long long part_size, const float* __restrict__ scale, const float* __restrict__ scale2, float scale3,
-               int vec) {
+head_dx_kernel(const float* __restrict__ acc, T* __restrict__ dx, HeadIndex ix, long long N, int D, int Dp,
+               const int* __restrict__ parts_word, const float* __restrict__ scale, const float* __restrict__ scale2,
+               float scale3, int vec, int direct) {
   after_previous();
+  const int parts = *parts_word;
+  const long long part_size = (long long)rows_of_part(*ix.count) * Dp;
   const float s = *scale * (scale2 ? *scale2 : 1.f) * scale3;
   const int lane = threadIdx.x & 31;
   const long long n = blockIdx.x * 8ll + (threadIdx.x >> 5);
   if (n >= N) return;
-  const int at = ix.at[n], begin = blockIdx.y * DX_COLUMNS, end = min(D, begin + DX_COLUMNS);
+  const int at = ix.at[n];
+  if (at >= 0 && direct && parts == 1) return;          // the product has written it
   const float* src = acc + (long long)at * Dp;
   T* dst = dx + n * D;
-  if (vec) {
-    for (int c = begin + lane * 8; c < end; c += 256) {
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int begin = blockIdx.y * DX_COLUMNS; begin < D; begin += gridDim.y * DX_COLUMNS) {
+    const int end = min(D, begin + DX_COLUMNS);
+    if (vec) {
+      float v[2][8] = {};
       if (at >= 0) {
-#pragma unroll 4
+#pragma unroll 2
         for (int k = 0; k < parts; ++k) {
-          const float4* q = reinterpret_cast<const float4*>(src + k * part_size + c);
-          const float4 a = q[0], b = q[1];
-          v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-          v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+          float4 q[2][2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int c = begin + lane * 8 + 256 * u;
+            const float4* from = reinterpret_cast<const float4*>(src + k * part_size + c);
+            if (c < end) { q[u][0] = from[0]; q[u][1] = from[1]; }
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float* e = reinterpret_cast<const float*>(q[u]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[u][j] += e[j];
+          }
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= s;
       }
-      uint4 q;
-      T* e = reinterpret_cast<T*>(&q);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j]);
-      *reinterpret_cast<uint4*>(dst + c) = q;
-    }
-  } else {
-    for (int c = begin + lane; c < end; c += 32) {
-      float v = 0.f;
-      if (at >= 0) {
-        for (int k = 0; k < parts; ++k) v += src[k * part_size + c];
-        v *= s;
+      for (int u = 0; u < 2; ++u) {
+        const int c = begin + lane * 8 + 256 * u;
+        uint4 q;
+        T* e = reinterpret_cast<T*>(&q);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(at >= 0 ? v[u][j] * s : 0.f);
+        if (c < end) *reinterpret_cast<uint4*>(dst + c) = q;
       }
-      dst[c] = from_f32<T>(v);
+    } else {
+      for (int c = begin + lane; c < end; c += 32) {
+        float v = 0.f;
+        if (at >= 0) {
+          for (int k = 0; k < parts; ++k) v += src[k * part_size + c];
+          v *= s;
+        }
+        dst[c] = from_f32<T>(v);
+      }
     }
   }
 }
@@ -365,13 +386,13 @@ PF_API int pf_head_words(long long N, long long V) {
   return (int)(((V + pieces - 1) / pieces + 255) / 256 * 256);
 }
 
-// Parts in which the reduction of dx over the words of the only piece is split, where few rows leave SMs idle
+// Parts in which the reduction of dx over the words of a piece is split if all rows count, where they leave SMs idle.  In
+// the memory of these go more parts of fewer rows.
 PF_API int pf_head_parts(long long N, long long V, int D, int sm_count) {
   if (!head_sizes_ok(N, V, D)) return -3;
   if (sm_count <= 0) sm_count = 148;
   const long long words = pf_head_words(N, V);
-  if (words < V) return 1;
-  return N > 0 ? plan_parts(N, (D + 7) / 8 * 8, V, sm_count, true).parts : 1;
+  return N > 0 ? plan_parts(N, (D + 7) / 8 * 8, words < V ? words : V, sm_count, true).parts : 1;
 }
 
 // x [N, D] (rows ldx apart), w [V, Dp] (Dp: D up to a multiple of 8, filled with zeros; rows ldw apart), target [N].
@@ -423,17 +444,23 @@ PF_API int pf_head_fwd(const void* x, const void* w, const void* target, void* x
     c.status = status; c.sm_count = sm_count; c.stream = st;
     if ((r = fused_gemm(HEAD_STATS, c))) return r;
   }
-  const unsigned grid = (unsigned)(N > 0 ? (N + FOLD_ROWS - 1) / FOLD_ROWS : 1);
-  after(head_fold_kernel, grid, 1024, 0, st)((const RowStat*)parts, Mp, n_parts, (const float*)picked, ix,
-                                             (RowStat*)stats, each, each ? nullptr : (float*)loss, (float*)inv, sums,
-                                             (int)(reduction == 1));
-  PF_CHECK_LAUNCH();
+  const auto fold = [&](auto* kernel, int rows) -> int {
+    const unsigned grid = (unsigned)(N > 0 ? (N + rows - 1) / rows : 1);
+    after(kernel, grid, 1024, 0, st)((const RowStat*)parts, Mp, n_parts, (const float*)picked, ix, (RowStat*)stats, each,
+                                     each ? nullptr : (float*)loss, (float*)inv, sums, (int)(reduction == 1));
+    PF_CHECK_LAUNCH();
+    return 0;
+  };
+  // 128 rows a CTA where each of its 8 threads has few parts and there are rows for all SMs
+  if (n_parts <= FOLD_FEW_PARTS && N >= (long long)sm_count * FOLD_MOST_ROWS / 4)
+    return fold(head_fold_kernel<FOLD_MOST_ROWS>, FOLD_MOST_ROWS);
+  return fold(head_fold_kernel<FOLD_ROWS>, FOLD_ROWS);
   return 0;
 }
 
 // dloss: one value, or with by_row the rows' dloss[n * dloss_step]; inv as the forward left it.
 // dx [N, D] packed, dw [V, Dp] (rows lddw apart, added to where accumulate); either may be null.
-// dz [Mp, pf_head_words], acc [pf_head_parts * Mp, Dp] (with dx), factor [Mp + 1] (with by_row) are scratch.
+// dz [Mp, pf_head_words], acc [pf_head_parts * Mp * Dp + 1] (with dx), factor [Mp + 1] (with by_row) are scratch.
 PF_API int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const void* w, void* index, const void* stats,
                        void* dx, void* dw, void* dz, void* acc, void* factor, long long N, long long V, int D, int Dp,
                        long long dloss_step, long long ldw, long long lddw, int by_row, int accumulate, int dtype,
@@ -448,8 +475,7 @@ PF_API int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const
   const long long Mp = padded_rows(N);
   const HeadIndex ix = head_index(static_cast<int*>(index), N);
   const int words = pf_head_words(N, V), parts = pf_head_parts(N, V, D, sm_count);
-  // where the vocabulary is one piece, with the tiles that go with its parts
-  const int tile = words >= V && N > 0 ? plan_parts(N, Dp, V, sm_count, true).pair : -1;
+  const int tile = N > 0 ? plan_parts(N, Dp, words < V ? words : V, sm_count, true).pair : 0;
   const float unit = dtype == PF_F16 ? 32768.f : 1.f;
   const float* scale = static_cast<const float*>(dloss);
   const float* scale2 = static_cast<const float*>(inv);
@@ -463,6 +489,15 @@ PF_API int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const
   }
   FusedCall base;
   base.dtype = dtype; base.rows = ix.count; base.status = status; base.sm_count = sm_count; base.stream = st;
+  int* parts_word = reinterpret_cast<int*>(static_cast<float*>(acc) + parts * Mp * Dp);
+  // One piece in one part is dx itself, by way of the rows' list: 13965 rows of 4096 over 256 words, both directions, 365 us
+  // with 32 bits in between and 295 without.
+  const int vec = D == Dp && on_vectors(dx), direct = vec && words >= V;
+  PartRule rule;                                        // of the first piece; no other has more words
+  rule.tile_rows = tile ? 256 : 128; rule.columns = (Dp + rule.tile_rows - 1) / rule.tile_rows;
+  rule.slots = tile ? sm_count / 2 : sm_count;
+  rule.kb = (int)(((words < V ? words : V) + 63) / 64); rule.planned = parts;
+  rule.rows = (int)std::min<long long>(parts * Mp, 0x7fffffff);
   const size_t es = dw_dtype == PF_F32 ? 4 : 2;
   if (N == 0) {                                         // nothing to add up, and no rows for a tensor map
     return dw && !accumulate ? (int)cudaMemsetAsync(dw, 0, (size_t)V * lddw * es, st) : 0;
@@ -479,7 +514,9 @@ PF_API int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const
     if (dx) {
       FusedCall c = base;
       c.M = (int)N; c.N = Dp; c.K = n; c.A = dz; c.B = wp; c.lda = words; c.ldb = ldw; c.C = acc; c.ldc = Dp;
-      c.out_dtype = PF_F32; c.split = parts; c.tile = tile; c.part_rows = (int)Mp; c.accumulate = v0 > 0;
+      c.out_dtype = PF_F32; c.split = parts; c.tile = tile; c.rule = rule; c.accumulate = v0 > 0;
+      c.parts_word = v0 ? nullptr : parts_word;
+      if (direct) { c.direct = dx; c.list = ix.list; c.scale = scale; c.scale2 = scale2; c.scale3 = 1.f / unit; }
       if ((r = fused_gemm(PARTS_N, c))) return r;
     }
     if (dw) {
@@ -491,14 +528,15 @@ PF_API int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const
     }
   }
   if (dx) {
-    const int vec = D == Dp && on_vectors(dx);
-    const dim3 grid((unsigned)((N + 7) / 8), (unsigned)((D + DX_COLUMNS - 1) / DX_COLUMNS));
+    // columns side by side as far as rows leave SMs idle
+    const long long rows = (N + 7) / 8, columns = (D + DX_COLUMNS - 1) / DX_COLUMNS, most = (8ll * sm_count + rows - 1) / rows;
+    const dim3 grid((unsigned)rows, (unsigned)std::min(columns, most));
     if (dtype == PF_F16)
-      after(head_dx_kernel<__half>, grid, 256, 0, st)((const float*)acc, (__half*)dx, ix, N, D, Dp, parts, Mp * Dp, scale,
-                                                      scale2, 1.f / unit, vec);
+      after(head_dx_kernel<__half>, grid, 256, 0, st)((const float*)acc, (__half*)dx, ix, N, D, Dp, (const int*)parts_word,
+                                                      scale, scale2, 1.f / unit, vec, direct);
     else
-      after(head_dx_kernel<__nv_bfloat16>, grid, 256, 0, st)((const float*)acc, (__nv_bfloat16*)dx, ix, N, D, Dp, parts,
-                                                             Mp * Dp, scale, scale2, 1.f / unit, vec);
+      after(head_dx_kernel<__nv_bfloat16>, grid, 256, 0, st)((const float*)acc, (__nv_bfloat16*)dx, ix, N, D, Dp,
+                                                             (const int*)parts_word, scale, scale2, 1.f / unit, vec, direct);
     PF_CHECK_LAUNCH();
   }
   return 0;

@@ -753,7 +753,7 @@ def head_bwd(dloss: torch.Tensor, xc: torch.Tensor, index: torch.Tensor, stats: 
     dx = new(N, D, dtype=xc.dtype) if need_dx else None
     words = _count(L.pf_head_words(N, V), "pf_head_words")
     dz = new(Mp, words, dtype=xc.dtype)
-    acc = new(_count(L.pf_head_parts(N, V, D, sms), "pf_head_parts") * Mp, Dp) if need_dx else None
+    acc = new(_count(L.pf_head_parts(N, V, D, sms), "pf_head_parts") * Mp * Dp + 1) if need_dx else None
     factor = new(Mp + 1) if by_row else None
     check(L.pf_head_bwd(dloss, inv, xc, w, index, stats, dx, dw, dz, acc, factor, N, V, D, Dp,
                         dloss.stride(0) if by_row else 0, w.stride(0), Dp, int(by_row), int(add), dt(xc.dtype),

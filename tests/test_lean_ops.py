@@ -365,6 +365,30 @@ def test_many_rows_of_which_some_count(N):
     assert not loss[out].any() and not dx[out].any()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("N,D,V,part", [(5000, 24, 40000, 0.03), (5000, 24, 40000, 0.5), (5200, 264, 40000, 0.002),
+                                        (6000, 72, 2000, 0.9), (6000, 72, 2000, 0.02), (9000, 20, 300, 0.3),
+                                        (9000, 20, 300, 0.0), (4800, 1032, 130, 1.0), (300, 520, 9001, 0.1)], ids=str)
+def test_parts_by_the_rows_there_are(N, D, V, part, dtype):
+    """The parts of dx follow the rows that count: one or more of them, in one piece of the vocabulary or several."""
+    x = normal(N, D, device="cuda", dtype=dtype, seed=1).requires_grad_()
+    w = normal(V, D, device="cuda", dtype=dtype, seed=2, std=2.0 * D ** -0.5).requires_grad_()
+    target = torch.randint(0, V, (N,), generator=gen(3))
+    target[torch.rand(N, generator=gen(4)) >= part] = -100
+    target = target.cuda()
+    g = torch.tensor(0.37, device="cuda")
+    loss = ops.linear_cross_entropy(x, w, target)
+    dx, dw = torch.autograd.grad(loss, [x, w], g, retain_graph=True)
+    want = head64(x, w, target, g, "mean", U[dtype], 2.0 ** 15 if dtype == torch.float16 else 2.0 ** 100)
+    within(loss.detach(), *want[0])
+    within(dx, *want[1])
+    within(dw, *want[2])
+    assert not dx[target < 0].any()
+    again = torch.autograd.grad(loss, [x, w], g)
+    assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_rows_that_do_not_count_reach_nothing(device):
     """Whatever they hold: infinities and NaN, in rows between others and behind the last."""
