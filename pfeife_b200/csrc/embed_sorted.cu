@@ -573,10 +573,12 @@ PF_API int pf_scaled_embed_bwd(const void* dout, const void* ids, void* dtable, 
   if (dtype == ID && table_dtype == TD) {                                                                              \
     if (vec) {                                                                                                         \
       after(table_grad_kernel<T_, TT_, 8>, grid, 128, 0, st)((const T_*)dout, (TT_*)dtable, p);                        \
-      if (joins > 0) after(table_join_kernel<TT_, 8>, (unsigned)joins, 128 * JOIN_GROUPS, 0, st)((TT_*)dtable, pj);                \
+      if (joins > 0)                                                                                                   \
+        after(table_join_kernel<TT_, 8>, (unsigned)joins, 128 * JOIN_GROUPS, 0, st)((TT_*)dtable, pj);                 \
     } else {                                                                                                           \
       after(table_grad_kernel<T_, TT_, 1>, grid, 128, 0, st)((const T_*)dout, (TT_*)dtable, p);                        \
-      if (joins > 0) after(table_join_kernel<TT_, 1>, (unsigned)joins, 128 * JOIN_GROUPS, 0, st)((TT_*)dtable, pj);                \
+      if (joins > 0)                                                                                                   \
+        after(table_join_kernel<TT_, 1>, (unsigned)joins, 128 * JOIN_GROUPS, 0, st)((TT_*)dtable, pj);                 \
     }                                                                                                                  \
   } else
   PF_BWD(PF_F32, float, PF_F32, float)

@@ -55,8 +55,8 @@ struct FusedSmem {
   static constexpr int STAGES = STAGING <= 32768 ? 6 : 5;
   static constexpr int BAR_OFFSET = STAGES * FG_STAGE_BYTES;
   static constexpr int STAGING_OFFSET = BAR_OFFSET + 1024;
-  // With A boxes of fewer rows there are as many stages as have room.  (13 rows over 11008 x 4096 weights, 11 for 6: products
-  // with N innermost 40 us for 44, K innermost 34 for 35, GLU_BWD 26 for 30.)
+  // With A boxes of fewer rows there are as many stages as have room.  (13 rows over 11008 x 4096 weights, 11 for 6:
+  // products with N innermost 40 us for 44, K innermost 34 for 35, GLU_BWD 26 for 30.)
   static constexpr int MOST = PAIR ? STAGES : 12;
   static constexpr int stages(int a_rows) {
     const int n = BAR_OFFSET / ((a_rows + FG_BN) * FG_BK * 2);
@@ -177,7 +177,8 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
       : "memory");
 }
 
-// Where 16 bytes lie in a box, as TMA has it for outputs that are added to: chunk c of row r, rows of 128 bytes swizzled over 128 or of 64 over 64.
+// Where 16 bytes lie in a box, as TMA has it for outputs that are added to: chunk c of row r, rows of 128 bytes swizzled
+// over 128 or of 64 over 64.
 // The 16-byte accesses of eight lanes, of one row or one chunk, meet no bank twice.
 template <int ROW_BYTES>
 __device__ __forceinline__ uint4* box_at(uint8_t* box, int r, int c) {
@@ -909,7 +910,8 @@ int fused_gemm(Job job, const FusedCall& c) {
   p.factor = c.factor; p.unit = c.unit;
   p.a_rows = a_rows;
   p.C = c.C; p.ldc = c.ldc; p.two = job == GLU_FWD ? c.gu : c.dgu; p.c_rows = (c.M + 255) / 256 * 256;
-  p.first = c.first; p.split = job == PARTS_K || job == PARTS_N ? c.split : 1; p.part_rows = c.part_rows; p.accumulate = c.accumulate;
+  p.first = c.first; p.split = job == PARTS_K || job == PARTS_N ? c.split : 1; p.part_rows = c.part_rows;
+  p.accumulate = c.accumulate;
   p.rule = c.rule; p.parts_word = c.parts_word; p.direct = c.direct; p.list = c.list;
   p.scale = c.scale; p.scale2 = c.scale2; p.scale3 = c.scale3;
   return c.dtype == PF_F16 ? fused_by_job<__half>(job, maps, p, pair, c)

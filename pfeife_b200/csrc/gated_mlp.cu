@@ -8,8 +8,8 @@
 // add the parts up in their order.
 //
 // On a B200, bf16, forward and backward: 2048 rows of 4096 over 11008 hidden values (1.66 TFLOP) 1.18 ms in a short run,
-// 1.41 PFLOP/s; 16384 of 640 over 2560 with GELU and biases 575 us, 0.84 PFLOP/s, where gate, up, h and their gradients are 27 MB
-// a thousand rows; 13 of 4096 over 11008 184 us, of which 124 are what memory takes for the weights twice and their
+// 1.41 PFLOP/s; 16384 of 640 over 2560 with GELU and biases 575 us, 0.84 PFLOP/s, where gate, up, their gradients and h are
+// 26 MB a thousand rows; 13 of 4096 over 11008 190 us, of which 124 are what memory takes for the weights twice and their
 // gradients once.
 #include "common.cuh"
 #include "api.h"
@@ -344,7 +344,8 @@ static int mlp_backward(const Block& b, const void* dy, const void* x, const voi
     }
   }
   if (g.dw1 && (r = b.weight_grad(dgu, ldgu, x, ldx, g.dw1, 2 * b.H, b.D, g.dw1_dtype, g.add & 1))) return r;
-  return b.bias_grads<T>({dgu, ldgu, 2 * b.H, g.db1_dtype, g.add & 4, g.db1}, {dy, lddy, b.N, g.db2_dtype, g.add & 8, g.db2});
+  return b.bias_grads<T>({dgu, ldgu, 2 * b.H, g.db1_dtype, g.add & 4, g.db1},
+                         {dy, lddy, b.N, g.db2_dtype, g.add & 8, g.db2});
 }
 
 static int mlp_block(Block& b, int M, int D, int H, int N, int act, int dtype, void* ws, int ws_kib, int* status,

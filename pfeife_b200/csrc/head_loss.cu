@@ -11,9 +11,9 @@
 // from forward to backward is the rows and 8 bytes of each, and what is alive at one time PIECE values.
 //
 // On a B200, bf16, forward and backward, 4096 values a row and 32000 words: 2048 rows 1.42 ms in a short run (four
-// products 1384 us at 1.45 to 1.63 PFLOP/s, picking the rows 12, the fold 13, dx 13); 13 rows 0.23 ms, bound by what
-// memory takes for W three times and dW once.  The fold reads 8 bytes of each row and 64 words, 1/16 of what the logits
-// in 16 bits would be.
+// products 1384 us at 1.45 to 1.63 PFLOP/s, picking the rows 12, the fold 13, zeros for rows that do not count 6);
+// 13 rows 0.23 ms, bound by what memory takes for W three times and dW once.  The fold reads 8 bytes of each row and 64
+// words, 1/16 of what the logits in 16 bits would be.
 //
 // dz is rounded to 16 bits as p - onehot, times 2^15 for fp16: from 6e-5 / 2^15 on the probabilities keep all
 // their bits, whatever the gradient of the loss is; that and the mean's factor come in 32 bits behind the products.
@@ -529,7 +529,8 @@ PF_API int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const
   }
   if (dx) {
     // columns side by side as far as rows leave SMs idle
-    const long long rows = (N + 7) / 8, columns = (D + DX_COLUMNS - 1) / DX_COLUMNS, most = (8ll * sm_count + rows - 1) / rows;
+    const long long rows = (N + 7) / 8, columns = (D + DX_COLUMNS - 1) / DX_COLUMNS;
+    const long long most = (8ll * sm_count + rows - 1) / rows;
     const dim3 grid((unsigned)rows, (unsigned)std::min(columns, most));
     if (dtype == PF_F16)
       after(head_dx_kernel<__half>, grid, 256, 0, st)((const float*)acc, (__half*)dx, ix, N, D, Dp, (const int*)parts_word,

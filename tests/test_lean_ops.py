@@ -510,6 +510,33 @@ def test_refusals(device):
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """A table, and gate and up, of more than 2^31 values: what lies at their end, against small calls."""
+    V, D, N = 270000, 8192, 300
+    table = torch.zeros(V, D, device="cuda", dtype=torch.bfloat16)
+    table[-9:] = normal(9, D, device="cuda", dtype=torch.bfloat16, seed=1)
+    table.requires_grad_()
+    ids = torch.randint(V - 9, V, (N,), generator=gen(2)).cuda()
+    small = table.detach()[-9:].clone().requires_grad_()
+    y, want = ops.scaled_embedding(ids, table, 2.0), ops.scaled_embedding(ids - (V - 9), small, 2.0)
+    assert torch.equal(y, want)
+    (g,), (gw,) = torch.autograd.grad(y, table, y.detach()), torch.autograd.grad(want, small, y.detach())
+    assert torch.equal(g[-9:], gw) and not g[:-9].any()
+    del table, g
+    M, D, H, N = 106000, 64, 10240, 64
+    x, dy = (normal(M, D, device="cuda", dtype=torch.bfloat16, seed=s).requires_grad_() for s in (3, 4))
+    w1, w2 = (normal(*s, device="cuda", dtype=torch.bfloat16, seed=5, std=0.05) for s in ((2 * H, D), (N, H)))
+    y = ops.gated_mlp(x, w1, None, w2, None)
+    (g,) = torch.autograd.grad(y, x, dy.detach())
+    part = x.detach()[-2048:].clone().requires_grad_()
+    want = ops.gated_mlp(part, w1, None, w2, None)
+    (gw,) = torch.autograd.grad(want, part, dy.detach()[-2048:])
+    # the same sums, in another order where a reduction is split
+    for a, b in ((y[-2048:], want), (g[-2048:], gw)):
+        assert float((a - b).detach().float().norm()) <= 4 * 2.0 ** -8 * float(b.detach().float().norm())
+
+
+@pytest.mark.gpu
 def test_operands_of_two_devices_are_refused():
     new = lambda *s, d="cuda": torch.zeros(*s, device=d, dtype=torch.bfloat16)
     for bad in (lambda: ops.gated_mlp(new(4, 8), new(16, 8, d="cpu"), None, new(8, 8), None),
