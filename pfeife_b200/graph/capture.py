@@ -18,6 +18,8 @@ from typing import Any, List, Optional, Sequence
 import torch
 import torch.fx as fx
 
+from ..ops.functional import stages_precision
+
 _SRC_ATOM = re.compile(r"\._(modules|parameters|buffers)\['([^']+)'\]|\.([A-Za-z_][A-Za-z_0-9]*)")
 
 
@@ -53,6 +55,7 @@ class GraphInput:
 class CapturedGraph:
     gm: fx.GraphModule
     inputs: List[GraphInput]
+    precision: Optional[torch.dtype] = None      # what the stages compute in, if not in their tensors' types
 
     @property
     def params(self) -> List[GraphInput]:
@@ -76,15 +79,18 @@ class CapturedGraph:
         those ops read the 16-bit shadow of the weight, never its fp32 master, so a
         data-parallel rank that does not own such a parameter needs no current master copy of
         it.  Anything else (biases, norm weights, position embeddings, a weight that an ATen op
-        touches) is read in fp32."""
+        touches, a table whose embedded tokens have another type than the stages compute in, a weight
+        of a product in a local autocast region) is read in fp32."""
         out = set()
         by_name = {n.name: n for n in self.gm.graph.nodes}
+        local = _in_autocast_regions(self.gm.graph)
         for gi in self.inputs:
             if not gi.is_state:
                 continue
             node = by_name.get(gi.node_name)
             users = list(node.users) if node is not None else []
-            if users and all(_reads_shadow(u, node) for u in users):
+            if users and not local.intersection(users) and \
+                    all(_reads_shadow(u, node, self.precision or gi.tensor.dtype) for u in users):
                 out.add(gi.index)
         return out
 
@@ -96,9 +102,25 @@ class CapturedGraph:
 # op name -> positions of the weight operands that the op reads through the 16-bit shadow
 _SHADOW_OPERANDS = {"linear_fwd": (1,), "mlp_fwd": (1, 3), "conv2d_fwd": (1,), "embed_fwd": (1,),
                     "gated_mlp_fwd": (1, 3), "head_loss_fwd": (1,), "scaled_embed_fwd": (1,)}
+# Products compute in the stages' precision.  These ops have the type of their result as an argument, and read the
+# shadow only where it is the shadow's.
+_RESULT_TYPES = {"embed_fwd": 2, "scaled_embed_fwd": 3}
 
 
-def _reads_shadow(user: fx.Node, value: fx.Node) -> bool:
+def _in_autocast_regions(graph: fx.Graph) -> set:
+    """The nodes between entering an autocast region of the model's own and leaving it."""
+    out, depth = set(), 0
+    for n in graph.nodes:
+        if n.target is torch.amp.autocast_mode._enter_autocast:
+            depth += 1
+        elif n.target is torch.amp.autocast_mode._exit_autocast:
+            depth -= 1
+        elif depth:
+            out.add(n)
+    return out
+
+
+def _reads_shadow(user: fx.Node, value: fx.Node, precision: torch.dtype) -> bool:
     if user.op != "call_function":
         return False
     name = str(user.target)
@@ -106,6 +128,9 @@ def _reads_shadow(user: fx.Node, value: fx.Node) -> bool:
         return False
     for op, positions in _SHADOW_OPERANDS.items():
         if f"pfeife.{op}" in name or f"pfeife::{op}" in name:
+            at = _RESULT_TYPES.get(op)
+            if at is not None and (len(user.args) <= at or user.args[at] != precision):
+                return False
             uses = [i for i, a in enumerate(user.args) if a is value]
             return bool(uses) and all(i in positions for i in uses) and \
                 value not in user.kwargs.values()
@@ -147,4 +172,4 @@ def classify_inputs(gm: fx.GraphModule, example_inputs: Sequence[Any]) -> Captur
         raise RuntimeError(
             "the captured GraphModule owns parameters (call_module graph); this framework "
             "expects parameters as graph inputs (torch >= 2.4 with inline_inbuilt_nn_modules)")
-    return CapturedGraph(gm, inputs)
+    return CapturedGraph(gm, inputs, stages_precision())

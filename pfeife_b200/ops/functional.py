@@ -138,6 +138,16 @@ def stage_precision(dtype: Optional[torch.dtype]):
         _trace_tls.dtype = prev
 
 
+def stages_precision() -> Optional[torch.dtype]:
+    """The type that ``stage_precision`` declares, or that of autocast where it declares none."""
+    declared = getattr(_trace_tls, "dtype", None)
+    if declared is None:
+        for dev in ("cuda", "cpu"):
+            if torch.is_autocast_enabled(dev):
+                return torch.get_autocast_dtype(dev)
+    return declared
+
+
 def compute_dtype(x: Tensor) -> torch.dtype:
     """dtype GEMM-like ops run in: the autocast dtype when autocast is on (or, while a graph is
     traced, the one declared by ``stage_precision``), else x's dtype."""

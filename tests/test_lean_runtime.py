@@ -189,3 +189,55 @@ def test_weights_that_are_read_in_16_bits_only():
     assert {i.qualname for i in cap.inputs if i.is_state and i.index in only} == {
         "embed.weight", "layers.0.qkv.weight", "layers.0.o_proj.weight", "layers.0.gate_up.weight",
         "layers.0.down.weight", "lm_head.weight"}
+
+
+@pytest.mark.parametrize("kind", ["embedding", "scaled_embedding"])
+@pytest.mark.parametrize("precision", [torch.bfloat16, torch.float16, None], ids=str)
+def test_tables_that_are_read_in_their_own_type(kind, precision):
+    """The embeddings read a table's 16-bit shadow where the result has its type, else the fp32 master, which a replica
+    then has to have; one such reader of several is enough."""
+    from pfeife_b200.ops import functional
+    from test_graph import capture
+    types = [torch.bfloat16, torch.float16, torch.float32]
+
+    class Tables(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.tables = torch.nn.ParameterList(torch.nn.Parameter(torch.randn(6, 8)) for _ in range(5))
+
+        def forward(self, ids):
+            read = getattr(ops, kind)
+            out = [read(ids, t, out_dtype=d) for t, d in zip(self.tables, types)]
+            out += [read(ids, self.tables[3]), read(ids, self.tables[4]), read(ids, self.tables[4], out_dtype=torch.float32)]
+            return sum(y.float() for y in out)
+
+    with functional.stage_precision(precision), torch.autocast("cpu", precision, enabled=precision is not None):
+        cap, _, _ = capture(Tables(), torch.arange(4))
+    only = cap.shadow_only_inputs()
+    want = {types.index(precision), 3} if precision is not None else {2, 3, 4}
+    assert {int(i.qualname.split(".")[-1]) for i in cap.params if i.index in only} == want
+
+
+def test_weights_of_a_region_without_autocast():
+    """Products that the model takes out of the stages' precision read the fp32 weights."""
+    from pfeife_b200.ops import functional
+    from test_graph import capture
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            for name, shape in (("before", (8, 8)), ("inside", (8, 8)), ("after", (8, 8)), ("both", (8, 8)),
+                                ("gate_up", (16, 8)), ("down", (8, 8)), ("head", (6, 8))):
+                setattr(self, name, torch.nn.Parameter(torch.randn(shape)))
+
+        def forward(self, x, labels):
+            x = ops.linear(ops.linear(x, self.before), self.both)
+            with torch.autocast("cpu", enabled=False):
+                x = ops.linear(ops.linear(x.float(), self.inside), self.both)
+                x = ops.gated_mlp(x, self.gate_up, None, self.down, None)
+            return ops.linear_cross_entropy(ops.linear(x, self.after), self.head, labels)
+
+    with functional.stage_precision(torch.bfloat16), torch.autocast("cpu", torch.bfloat16):
+        cap, _, _ = capture(Net(), torch.randn(3, 8), torch.arange(3))
+    only = cap.shadow_only_inputs()
+    assert {i.qualname for i in cap.params if i.index in only} == {"before", "after", "head"}
