@@ -161,14 +161,15 @@ def compute_dtype(x: Tensor) -> torch.dtype:
 
 
 def _weight_as(w: Tensor, dtype: torch.dtype) -> Tensor:
-    """`w` in `dtype`: itself, its registered 16-bit shadow, or a cast copy."""
-    if w.dtype == dtype:
-        return w
+    """`w` in `dtype`: itself (which is the shadow where the model holds its weights in 16 bits), its registered 16-bit
+    shadow, or a cast copy."""
     s = _slot(w)
     if s is not None and s.lp is not None and s.lp.dtype == dtype:
         if _stale(s):
             _gather_now(s)
-        return s.lp
+        return w if w.dtype == dtype else s.lp
+    if w.dtype == dtype:
+        return w
     return kx.cast(w, dtype) if w.is_cuda else w.to(dtype)
 
 

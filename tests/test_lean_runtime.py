@@ -241,3 +241,59 @@ def test_weights_of_a_region_without_autocast():
         cap, _, _ = capture(Net(), torch.randn(3, 8), torch.arange(3))
     only = cap.shadow_only_inputs()
     assert {i.qualname for i in cap.params if i.index in only} == {"before", "after", "head"}
+
+
+@pytest.mark.parametrize("own_type", [False, True], ids=["fp32 weights", "16-bit weights"])
+def test_rows_of_other_replicas_come_before_a_weight_is_read(own_type, monkeypatch):
+    """Row-sharded weights are completed by their first reader after an optimizer step, whether the model holds them in
+    fp32 beside a 16-bit shadow or in 16 bits itself."""
+    from pfeife_b200.ops import functional as Fn
+    from pfeife_b200.ops import kernels as kx
+    master = torch.randn(8, 4)
+    lp = torch.zeros(8, 4, dtype=torch.bfloat16)
+    pulled = []
+    monkeypatch.setattr(kx, "gather_rows", lambda rows, *a: pulled.append(rows.copy_(master)))
+    w = lp.detach() if own_type else master
+    try:
+        ops.register_param(master, lp, None)
+        Fn.set_gather(master, Fn.GatherInfo(None, (4, 8), 2, 0, None))
+        for turn in range(1, 3):
+            lp.zero_()
+            Fn._weight_as(w, torch.bfloat16)             # outside of a session weights are complete
+            assert len(pulled) == turn - 1
+            Fn.gather_session(True)
+            for _ in range(2):
+                assert torch.equal(Fn._weight_as(w, torch.bfloat16), master.to(torch.bfloat16)) and len(pulled) == turn
+            Fn.gather_session(False)
+    finally:
+        Fn.gather_session(False)
+        ops.unregister_params()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("own_type", [False, True], ids=["fp32 weights", "16-bit weights"])
+def test_lean_operators_complete_the_weights_that_they_read(own_type, monkeypatch):
+    from pfeife_b200.ops import functional as Fn
+    from pfeife_b200.ops import kernels as kx
+    full = [torch.randn(*s, device="cuda") * 0.2 for s in ((64, 32), (96, 32), (32, 48), (64, 32))]
+    low = [t.to(torch.bfloat16) for t in full]
+    held = [t.clone() for t in low]
+    of = {t.data_ptr(): i for i, t in enumerate(low)}
+    monkeypatch.setattr(kx, "gather_rows", lambda rows, *a: rows.copy_(held[of[rows.data_ptr()]]))
+    ids, labels = (torch.randint(0, 64, (40,), device="cuda") for _ in range(2))
+
+    def run(table, w1, w2, head):
+        with torch.autocast("cuda", torch.bfloat16):
+            h = ops.scaled_embedding(ids, table, 2.0, out_dtype=torch.bfloat16)
+            return ops.linear_cross_entropy(ops.gated_mlp(h, w1, None, w2, None), head, labels)
+    want = run(*held)
+    try:
+        for master, lp in zip(full, low):
+            ops.register_param(master, lp, None)
+            Fn.set_gather(master, Fn.GatherInfo(None, (len(lp) // 2, len(lp)), 2, 0, None))
+            lp[: len(lp) // 2] = 0
+        Fn.gather_session(True)
+        assert torch.equal(run(*([t.detach() for t in low] if own_type else full)), want)
+    finally:
+        Fn.gather_session(False)
+        ops.unregister_params()
