@@ -184,8 +184,8 @@ __device__ __forceinline__ void join(float& ref, float& sum, float ref2, float s
 template <int ROWS>
 __global__ void __launch_bounds__(1024)
 head_fold_kernel(const RowStat* __restrict__ parts, long long pitch, int n_parts, const float* __restrict__ picked,
-                 HeadIndex ix, RowStat* __restrict__ stats, float* __restrict__ loss_of_row, float* __restrict__ loss,
-                 float* __restrict__ inv, double* __restrict__ sums, int mean) {
+                 HeadIndex ix, RowStat* __restrict__ stats, float* __restrict__ loss, float* __restrict__ inv,
+                 double* __restrict__ sums, int reduction) {
   after_previous();
   constexpr int LANES = 1024 / ROWS;
   __shared__ RowStat all[ROWS][LANES + 1];
@@ -228,10 +228,10 @@ head_fold_kernel(const RowStat* __restrict__ parts, long long pitch, int n_parts
       constexpr double ln2 = 0.69314718055994531;
       const double l = (log2((double)sum) + (double)ref - (double)picked[row] * (double)1.4426950408889634f) * ln2;
       rows[r] = l;
-      if (loss_of_row) loss_of_row[ix.list[row]] = (float)l;
+      if (reduction == 0) loss[ix.list[row]] = (float)l;
     }
   }
-  if (loss_of_row) return;
+  if (reduction == 0) return;                           // of no rows the losses have no address
   __syncthreads();
   if (threadIdx.x == 0) {
     double s = 0.0;
@@ -253,7 +253,7 @@ head_fold_kernel(const RowStat* __restrict__ parts, long long pitch, int n_parts
   if (threadIdx.x == 0) {
     s = 0.0;
     for (int i = 0; i < 32; ++i) s += rows[i];
-    const double n = mean ? (double)max(count, 1) : 1.0;
+    const double n = reduction == 1 ? (double)max(count, 1) : 1.0;
     *loss = (float)(s / n);
     *inv = (float)(1.0 / n);
   }
@@ -446,8 +446,8 @@ PF_API int pf_head_fwd(const void* x, const void* w, const void* target, void* x
   }
   const auto fold = [&](auto* kernel, int rows) -> int {
     const unsigned grid = (unsigned)(N > 0 ? (N + rows - 1) / rows : 1);
-    after(kernel, grid, 1024, 0, st)((const RowStat*)parts, Mp, n_parts, (const float*)picked, ix, (RowStat*)stats, each,
-                                     each ? nullptr : (float*)loss, (float*)inv, sums, (int)(reduction == 1));
+    after(kernel, grid, 1024, 0, st)((const RowStat*)parts, Mp, n_parts, (const float*)picked, ix, (RowStat*)stats,
+                                     (float*)loss, (float*)inv, sums, reduction);
     PF_CHECK_LAUNCH();
     return 0;
   };

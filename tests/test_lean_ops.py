@@ -882,3 +882,19 @@ def test_checkpoints_and_second_backwards():
     through = torch.autograd.grad(checkpoint(run, ids, labels, use_reentrant=False), leaves)
     for a, b, c in zip(want, again, through):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_no_rows(reduction, dtype, device):
+    """The losses of no rows are none, and have no address; a sum over them is 0."""
+    x = torch.zeros(3, 0, 24, device=device, dtype=dtype, requires_grad=True)
+    w = normal(40, 24, device=device, dtype=dtype, seed=1).requires_grad_()
+    target = torch.zeros(3, 0, device=device, dtype=torch.int64)
+    with torch.no_grad():
+        loss = ops.linear_cross_entropy(x, w, target, reduction=reduction)
+    assert loss.shape == ((3, 0) if reduction == "none" else ()) and not loss.any()
+    loss = ops.linear_cross_entropy(x, w, target, reduction=reduction)
+    dx, dw = torch.autograd.grad(loss, [x, w], torch.ones_like(loss))
+    assert dx.shape == x.shape and not dw.any()
