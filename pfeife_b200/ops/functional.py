@@ -677,24 +677,35 @@ def _(x, w1, b1, w2, b2, residual, act, keep):
     return x.new_empty(x.shape[:-1] + (w2.shape[0],), dtype=cd), gu
 
 
+def _gated_mlp_types(cd, w1, b1, w2, b2) -> Tuple[torch.dtype, ...]:
+    """Types of (dx, dw1, db1, dw2, db2), needed or not"""
+    of = lambda b: torch.float32 if b is None else b.dtype
+    return cd, w1.dtype, of(b1), w2.dtype, of(b2)
+
+
 @_custom_op("pfeife::gated_mlp_bwd")
 def gated_mlp_bwd(dy: Tensor, x: Tensor, w1: Tensor, w2: Tensor, gu: Tensor, act: int, need_dx: bool, need_dw1: bool,
                   need_db1: bool, need_dw2: bool, need_db2: bool, b1: Optional[Tensor] = None,
                   b2: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """-> (dx, dw1, db1, dw2, db2); what is not needed, or went into a registered gradient bucket, comes back empty.
+    """-> (dx, dw1, db1, dw2, db2), the parameters' in the parameters' types (biases that are not given: fp32); what is
+    not needed, or went into a registered gradient bucket, comes back empty.
     The gradient of h is formed in the epilogue of its product, where the kept gate and up turn it into their
     gradients and into h itself, which the forward did not keep."""
+    grads = _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1, b2)
+    return tuple(g.to(d) for g, d in zip(grads, _gated_mlp_types(dy.dtype, w1, b1, w2, b2)))
+
+
+def _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1, b2):
     cd = dy.dtype
     H = w2.shape[1]
     empty = dy.new_empty(0)
     if not dy.numel():                   # no rows: the products would leave the weights' gradients as they are
-        zeros = lambda n, t, need, **kw: dy.new_zeros(n if need and _grad_bucket(t) is None else 0, **kw)
-        f32 = dict(dtype=torch.float32)
-        return (dy.new_zeros(x.shape), zeros(w1.shape, w1, need_dw1, dtype=w1.dtype), zeros(2 * H, b1, need_db1, **f32),
-                zeros(w2.shape, w2, need_dw2, dtype=w2.dtype), zeros(w2.shape[0], b2, need_db2, **f32))
+        zeros = lambda n, t, need: dy.new_zeros(n if need and _grad_bucket(t) is None else 0, dtype=torch.float32)
+        return (dy.new_zeros(x.shape if need_dx else 0), zeros(w1.shape, w1, need_dw1), zeros(2 * H, b1, need_db1),
+                zeros(w2.shape, w2, need_dw2), zeros(w2.shape[0], b2, need_db2))
     native = dy.is_cuda and cd in (torch.float16, torch.bfloat16)
     if _glu_native(dy, cd, w1, w2):
-        return _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1, b2)
+        return _gated_mlp_native_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1, b2)
     dh = linear_bwd.plain(dy, gu[..., :H], w2, empty, ACT_NONE, True, False, False)[0] if native else dy @ w2.to(cd)
     gate, up, dh = _wide(gu[..., :H]), _wide(gu[..., H:]), _wide(dh)
     a, slope = _act_slope(gate, act)
@@ -711,7 +722,7 @@ def gated_mlp_bwd(dy: Tensor, x: Tensor, w1: Tensor, w2: Tensor, gu: Tensor, act
         (need_db1, lambda: d1.sum(0)), (need_dw2, lambda: (d2.t() @ h2).to(w2.dtype)), (need_db2, lambda: d2.sum(0))))
 
 
-def _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1, b2):
+def _gated_mlp_native_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1, b2):
     """``gated_mlp_bwd`` by its kernels"""
     cd, dev = dy.dtype, dy.device
     x2 = _rows(x if x.dtype == cd else kx.cast(x, cd))
@@ -746,16 +757,15 @@ def _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_d
         buckets.append(name)
     dx, dw1, db1, dw2, db2 = (out[k] if k in out and k not in buckets else dy.new_empty(0)
                               for k in ("dx", "dw1", "db1", "dw2", "db2"))
-    return dx.view(x.shape) if need_dx else dx, dw1.to(w1.dtype), db1, dw2.to(w2.dtype), db2
+    return dx.view(x.shape) if need_dx else dx, dw1, db1, dw2, db2
 
 
 @gated_mlp_bwd.register_fake
 def _(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1=None, b2=None):
-    e, f32 = dy.new_empty(0), torch.float32
-    return (dy.new_empty(x.shape) if need_dx else e, torch.empty_like(w1) if need_dw1 else e,
-            dy.new_empty(w1.shape[0] if need_db1 else 0, dtype=b1.dtype if b1 is not None else f32),
-            torch.empty_like(w2) if need_dw2 else e,
-            dy.new_empty(w2.shape[0] if need_db2 else 0, dtype=b2.dtype if b2 is not None else f32))
+    sizes = ((x.shape, need_dx), (w1.shape, need_dw1), (w1.shape[0], need_db1), (w2.shape, need_dw2),
+             (w2.shape[0], need_db2))
+    return tuple(dy.new_empty(n if need else 0, dtype=d)
+                 for (n, need), d in zip(sizes, _gated_mlp_types(dy.dtype, w1, b1, w2, b2)))
 
 
 def _gated_mlp_setup(ctx, inputs, output):
@@ -1504,7 +1514,7 @@ def head_loss_bwd(dloss: Tensor, xc: Tensor, index: Tensor, stats: Tensor, inv: 
 def _(dloss, xc, index, stats, inv, w, N, by_row, need_dx, need_dw):
     e = xc.new_empty(0)
     return (xc.new_empty((N, w.shape[1])) if need_dx else e,
-            torch.empty_like(w) if need_dw else xc.new_empty(0, dtype=w.dtype))
+            w.new_empty(w.shape if need_dw else 0))
 
 
 def _head_loss_setup(ctx, inputs, output):

@@ -898,3 +898,33 @@ def test_no_rows(reduction, dtype, device):
     loss = ops.linear_cross_entropy(x, w, target, reduction=reduction)
     dx, dw = torch.autograd.grad(loss, [x, w], torch.ones_like(loss))
     assert dx.shape == x.shape and not dw.any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32, torch.float64], ids=str)
+@pytest.mark.parametrize("M,D,H,N", [(4, 8, 16, 8), (4, 6, 5, 7), (0, 8, 16, 8)], ids=str)
+def test_what_a_tracer_is_told(M, D, H, N, dtype, device):
+    """Shapes and types of the registered ops' outputs without data are those with it: whole widths and odd ones, no rows,
+    operands of two types, transposed weights, any gradients."""
+    from torch.library import opcheck
+    from pfeife_b200.ops import functional as Fn
+    tests = ("test_schema", "test_autograd_registration", "test_faketensor")
+    new = lambda *s, d=dtype: normal(*s, device=device, dtype=d, seed=len(s))
+    other = torch.float32 if dtype != torch.float32 else torch.bfloat16
+    for wide in (dtype, other):
+        x, w1, b1, w2, b2 = new(M, D), new(2 * H, D, d=wide), new(2 * H, d=wide), new(H, N, d=wide).t(), new(N, d=wide)
+        dy, gu = new(M, N), new(M, 2 * H)
+        for keep in (True, False):
+            opcheck(Fn.gated_mlp_fwd, (x, w1, b1, w2, b2, dy, 3, keep), test_utils=tests)
+        for need in ((True,) * 5, (False, True, True, False, False), (True, False, False, True, True)):
+            for p, q in ((b1, b2), (b1, None), (None, None)):
+                want = need[:2] + (need[2] and p is not None, need[3], need[4] and q is not None)
+                opcheck(Fn.gated_mlp_bwd, (dy, x, w1, w2, gu, 3, *want, p, q), test_utils=tests)
+        w, target = new(D, H, d=wide).t(), torch.arange(M, device=device) % (H + 1)
+        for reduction in range(3):
+            opcheck(Fn.head_loss_fwd, (x, w, target, -100, reduction), test_utils=tests)
+            loss, *kept = Fn.head_loss_fwd(x, w, target, -100, reduction)
+            for need in ((True, True), (False, True), (True, False)):
+                opcheck(Fn.head_loss_bwd, (torch.ones_like(loss), *kept, w, M, reduction == 0, *need), test_utils=tests)
+        opcheck(Fn.scaled_embed_fwd, (target, w, 2.0, dtype), test_utils=tests)
+        opcheck(Fn.scaled_embed_bwd, (x, target, w, 2.0), test_utils=tests)
