@@ -1456,7 +1456,7 @@ def head_loss_fwd(x: Tensor, w: Tensor, target: Tensor, ignore_index: int, reduc
     z = _wide(F.linear(_wide(xc[:N, :D]), _wide(w.to(cd))))
     each = (torch.logsumexp(z, -1) - z.gather(1, labels.unsqueeze(1)).squeeze(1)).masked_fill(~live, 0)
     count = index[0].clamp(min=1) if reduction == 1 else torch.ones_like(index[0])
-    inv = 1.0 / count.float()
+    inv = 1.0 / count.to(_loss_dtype(x))
     if reduction == 0:
         loss = z.new_zeros(N).index_copy(0, rows, each)
     else:
@@ -1474,7 +1474,8 @@ def _(x, w, target, ignore_index, reduction):
     Mp, Dp, size = _head_kept(N, D)
     f32 = lambda *shape: x.new_empty(shape, dtype=torch.float32)
     return (x.new_empty((N,) if reduction == 0 else (), dtype=_loss_dtype(x)),
-            x.new_empty((Mp, Dp), dtype=compute_dtype(x)), x.new_empty(size, dtype=torch.int32), f32(Mp, 2), f32())
+            x.new_empty((Mp, Dp), dtype=compute_dtype(x)), x.new_empty(size, dtype=torch.int32), f32(Mp, 2),
+            x.new_empty((), dtype=_loss_dtype(x)))
 
 
 @_custom_op("pfeife::head_loss_bwd")

@@ -928,3 +928,19 @@ def test_what_a_tracer_is_told(M, D, H, N, dtype, device):
                 opcheck(Fn.head_loss_bwd, (torch.ones_like(loss), *kept, w, M, reduction == 0, *need), test_utils=tests)
         opcheck(Fn.scaled_embed_fwd, (target, w, 2.0, dtype), test_utils=tests)
         opcheck(Fn.scaled_embed_bwd, (x, target, w, 2.0), test_utils=tests)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_head_in_64_bits(reduction, device):
+    """Gradients as exact as their type, the mean's factor among them."""
+    x, w = (torch.randn(s, 6, dtype=torch.float64, generator=gen(s)).to(device).requires_grad_() for s in (7, 9))
+    target = torch.tensor([0, 3, -100, 8, 3, 9, 1], device=device)
+    g = torch.randn(7 if reduction == "none" else (), dtype=torch.float64, generator=gen(3)).to(device)
+    got = torch.autograd.grad(ops.linear_cross_entropy(x, w, target, reduction=reduction), [x, w], g)
+    coef = torch.where((target >= 0) & (target < 9), g / 5 if reduction == "mean" else g, 0.0)
+    d = torch.softmax(x.detach() @ w.detach().t(), -1)
+    d -= torch.nn.functional.one_hot(target.clamp(0, 8), 9)
+    d *= coef[:, None]
+    for a, b in zip(got, (d @ w.detach(), d.t() @ x.detach())):
+        assert float((a - b).norm()) <= 1e-13 * float(b.norm())      # some hundred roundings of 2^-53
