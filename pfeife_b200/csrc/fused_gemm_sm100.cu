@@ -16,7 +16,8 @@
 // 74 pairs, 86 % of two rounds.  GLU_BWD moves 10 bytes for each of its values (420 MB for the short reduction, 63 us) and
 // has the longest epilogue, which a reduction of 640 does not cover.  Products of few rows are bound by memory.
 //
-// GLU_FWD: a tile has as many gate columns as up columns.  B comes from two tensor maps, the gate and the up rows of
+// GLU_FWD: a tile has as many gate columns as up columns.  What is kept of both is saturated: h of a gate of 7e4 and an up
+// value of 0.5 is finite in fp16, and a kept infinity would turn its gradients into NaN at any loss scale.  B comes from two tensor maps, the gate and the up rows of
 // one weight; of a pair, the even CTA loads the gate rows and the odd one the up rows, so that the accumulator
 // of every row has the gate in its left half and up in its right half, and one thread has both values.
 // HEAD_STATS: a thread keeps the maximum and the sum of exponentials of its columns; references are integers in
@@ -548,11 +549,16 @@ fused_gemm_kernel(const __grid_constant__ FusedMaps maps, const FusedParams p) {
               for (int j = 0; j < 8; ++j) e[j] = from_f32<OutT>(v[8 * k + j]);
               return q;
             };
-            if (p.save) {
+            if (p.save) {                                // within the type: h may be where a gate is not
+              auto kept = [&](const float (&v)[16], int k) {
+                const float* e = v + 8 * k;
+                return make_uint4(saturated2<OutT>(e[0], e[1]), saturated2<OutT>(e[2], e[3]),
+                                  saturated2<OutT>(e[4], e[5]), saturated2<OutT>(e[6], e[7]));
+              };
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                *box_at<RB>(boxes, lane, s / 8 + k) = packed(g, k);
-                *box_at<RB>(boxes + S::BOX, lane, s / 8 + k) = packed(u, k);
+                *box_at<RB>(boxes, lane, s / 8 + k) = kept(g, k);
+                *box_at<RB>(boxes + S::BOX, lane, s / 8 + k) = kept(u, k);
               }
             }
             auto all = [&](auto kind) {

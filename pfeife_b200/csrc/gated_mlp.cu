@@ -46,6 +46,10 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float (
   for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j]);
   *reinterpret_cast<uint4*>(p) = q;
 }
+template <typename T> __device__ __forceinline__ void store8_saturated(T* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(saturated2<T>(v[0], v[1]), saturated2<T>(v[2], v[3]),
+                                            saturated2<T>(v[4], v[5]), saturated2<T>(v[6], v[7]));
+}
 __device__ __forceinline__ void add_bias8(const void* b, int dtype, int i, float (&v)[8]) {
   if (!b) return;
 #pragma unroll
@@ -83,9 +87,9 @@ glu_join_kernel(const Parts p, const void* __restrict__ bias, int bias_dtype, T*
   sum_parts(p, (long long)m * 2 * H + H + c, u);
   add_bias8(bias, bias_dtype, c, g);
   add_bias8(bias, bias_dtype, H + c, u);
-  if (gu) {
-    store8(gu + (long long)m * 2 * H + c, g);
-    store8(gu + (long long)m * 2 * H + H + c, u);
+  if (gu) {                                             // within the type, see fused_gemm_sm100.cu
+    store8_saturated(gu + (long long)m * 2 * H + c, g);
+    store8_saturated(gu + (long long)m * 2 * H + H + c, u);
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {

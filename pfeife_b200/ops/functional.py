@@ -667,7 +667,14 @@ def gated_mlp_fwd(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: O
     h = (_act_slope(wide[..., :H], act)[0] * wide[..., H:]).to(cd)
     w = _aligned(_pad_k(w2)) if w2.is_cuda and w2.dtype == cd else w2
     y, _ = linear_fwd.plain(h if w.shape[1] == H else _pad_k(h), w, b2, residual, ACT_NONE)
-    return y, (wide.to(cd) if keep else x.new_empty(0))
+    return y, (_saturated(wide, cd) if keep else x.new_empty(0))
+
+
+def _saturated(t: Tensor, dtype: torch.dtype) -> Tensor:
+    """`t` in `dtype`, values beyond 16 bits as the largest there are; NaN stays NaN"""
+    if dtype in (torch.float16, torch.bfloat16):
+        t = t.clamp(-torch.finfo(dtype).max, torch.finfo(dtype).max)
+    return t.to(dtype)
 
 
 @gated_mlp_fwd.register_fake
@@ -808,7 +815,8 @@ def gated_mlp(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: Optio
     with Wg its first and Wu its last H rows (as ``swiglu`` and ``geglu`` have them), b1 [2H], w2 [N, H], b2 [N] and
     residual [..., N].  Activations: silu, gelu, gelu_tanh.  One product computes both projections, the activation and
     their product; gate and up are kept for the backward, which computes the values that W2 reads from them again.
-    Gate and up are rounded to x's type where they are kept, not on their way into the activation."""
+    Gate and up are rounded to x's type where they are kept, not on their way into the activation; those that 16 bits
+    do not have are kept as the largest values there are, and gradients are those of that."""
     if activation not in ("silu", "gelu", "gelu_tanh", "gelu_pytorch_tanh"):
         raise ValueError(f"gated_mlp: unknown activation {activation!r}")
     act = _ACT_NAMES[activation]

@@ -944,3 +944,32 @@ def test_head_in_64_bits(reduction, device):
     d *= coef[:, None]
     for a, b in zip(got, (d @ w.detach(), d.t() @ x.detach())):
         assert float((a - b).norm()) <= 1e-13 * float(b.norm())      # some hundred roundings of 2^-53
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [8, 9, 2048], ids=["whole", "odd", "parts"])
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh"])
+def test_gates_beyond_fp16(kind, D, device):
+    """Gates and up values that fp16 does not have, of hidden values that it has: they are kept as its largest, and
+    gradients are those of that."""
+    H, top = 8, 65504.0
+    gates = torch.tensor([7e4, 1.3e5, -7e4, -1.3e5, 3e4, 0.25, 7e4, 1e5])
+    ups = torch.tensor([0.5, 0.25, 0.5, -0.25, 2.0, 1.3e5, -0.5, 7e4 / 2 ** 17])
+    x = torch.zeros(1, D, device=device, dtype=torch.float16)
+    x[0, :2] = 2.0
+    w1 = torch.zeros(2 * H, D, device=device, dtype=torch.float16)
+    w1[:H, 0], w1[H:, 1] = (gates / 2).to(w1), (ups / 2).to(w1)
+    x, w1, w2 = x.requires_grad_(), w1.requires_grad_(), torch.eye(H, device=device, dtype=torch.float16).requires_grad_()
+    gate, up = (2 * w1.detach()[i * H:i * H + H, i].double() for i in range(2))
+    dy = torch.full((1, H), 2.0 ** -6, device=device, dtype=torch.float16)
+    y = ops.gated_mlp(x, w1, None, w2, None, kind)
+    within(y.detach()[0], act64(gate.clamp(-1e4, 1e4), kind)[0].where(gate < 1e4, gate) * up, 1e-6 * (1 + gate.abs()) * up.abs())
+    dx, dw1, dw2 = torch.autograd.grad(y, [x, w1, w2], dy)
+    gate, up = gate.clamp(-top, top), up.clamp(-top, top)
+    a, slope = act64(gate.clamp(-1e4, 1e4), kind)
+    a = a.where(gate < 1e4, gate)
+    u = U[torch.float16]
+    within(dw1[:H, 0], 2.0 ** -5 * up * slope, 2.0 ** -5 * up.abs() * (1e-6 + u) + 2.0 ** -24)
+    within(dw1[H:, 1], 2.0 ** -5 * a, 2.0 ** -5 * a.abs() * u + 1e-6)
+    within(dw2[0], 2.0 ** -6 * a * up, 2.0 ** -6 * (a * up).abs() * u + 1e-3)
+    assert torch.isfinite(dx).all()
