@@ -795,16 +795,16 @@ static int launch_fused(const FusedMaps& maps, const FusedParams& p, int sm_coun
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     cfg.gridDim = dim3(2 * (sm_count / 2));
+    // what the device takes is the same for every call, what a call is given is not
     int most = known ? resident_pairs[dev] : 0;
     if (most == 0) {
-      int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+      if (cudaOccupancyMaxActiveClusters(&most, kern, &cfg) != cudaSuccess || most <= 0) {
         (void)cudaGetLastError();
-        n = sm_count / 2;
+        most = 0;
       }
-      most = n < sm_count / 2 ? n : sm_count / 2;
       if (known) resident_pairs[dev] = most;
     }
+    if (most == 0 || most > sm_count / 2) most = sm_count / 2;
     cfg.gridDim = dim3(2 * (unsigned)(items < most ? items : most));
   } else {
     cfg.gridDim = dim3((unsigned)(items < sm_count ? items : sm_count));

@@ -836,18 +836,18 @@ static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    // pairs that can be resident at once (the two CTAs of a pair sit on neighbouring SMs)
+    // pairs that can be resident at once (the two CTAs of a pair sit on neighbouring SMs): the device's
+    // number is kept, the call's number of SMs may differ from the next one's
     static int resident_pairs[64] = {};
     int max_pairs = (dev >= 0 && dev < 64) ? resident_pairs[dev] : 0;
     if (max_pairs == 0) {
-      int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+      if (cudaOccupancyMaxActiveClusters(&max_pairs, kern, &cfg) != cudaSuccess || max_pairs <= 0) {
         (void)cudaGetLastError();
-        n = sm_count / 2;
+        max_pairs = 0;
       }
-      max_pairs = n < sm_count / 2 ? n : sm_count / 2;
       if (dev >= 0 && dev < 64) resident_pairs[dev] = max_pairs;
     }
+    if (max_pairs == 0 || max_pairs > sm_count / 2) max_pairs = sm_count / 2;
     const int pairs = num_tiles < max_pairs ? num_tiles : max_pairs;
     cfg.gridDim = dim3(2 * pairs);
     cudaError_t e = LaunchAfter<CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, GemmParams>{

@@ -973,3 +973,27 @@ def test_gates_beyond_fp16(kind, D, device):
     within(dw1[H:, 1], 2.0 ** -5 * a, 2.0 ** -5 * a.abs() * u + 1e-6)
     within(dw2[0], 2.0 ** -6 * a * up, 2.0 ** -6 * (a * up).abs() * u + 1e-3)
     assert torch.isfinite(dx).all()
+
+
+@pytest.mark.gpu
+def test_products_take_the_sms_that_a_call_is_given(monkeypatch, tmp_path):
+    """Whatever calls before it were given: CTAs of pairs of a gated block and of a plain product."""
+    import json
+    from torch.profiler import ProfilerActivity, profile
+    from pfeife_b200.ops import kernels as kx
+    new = lambda *s: normal(*s, device="cuda", dtype=torch.bfloat16, seed=1, std=0.1)
+    x, w1, w2 = new(2048, 256), new(4096, 256), new(256, 2048)
+    grids, out = {}, []
+    for sms in (148, 16, 132, 24):
+        monkeypatch.setattr(kx, "sm_count", lambda device: sms)
+        with profile(activities=[ProfilerActivity.CUDA]) as p:
+            out.append((kx.gated_mlp_fwd(x, w1, None, w2, None, None, 3, False)[0], kx.gemm(x, w1)))
+            torch.cuda.synchronize()
+        p.export_chrome_trace(str(tmp_path / "trace.json"))
+        events = json.loads((tmp_path / "trace.json").read_text())["traceEvents"]
+        grids[sms] = [e["args"]["grid"][0] for e in events if "gemm" in e.get("name", "") and "grid" in e.get("args", {})]
+    assert all(len(g) >= 3 and max(g) <= sms for sms, g in grids.items()), grids
+    # 128 tiles of a pair each: as many pairs as there may be, where the device takes that many
+    assert grids[16][0] == 16 and grids[24][0] == 24 and grids[148][0] > 100 and grids[132][0] > 100, grids
+    for y, z in out[1:]:
+        assert torch.equal(z, out[0][1]) and float((y - out[0][0]).float().norm()) <= 2.0 ** -8 * float(y.float().norm())
