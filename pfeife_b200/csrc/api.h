@@ -42,6 +42,7 @@ PF_DECL int pf_head_index(long long N);
 PF_DECL int pf_head_scratch(long long N, long long V);
 PF_DECL int pf_head_words(long long N, long long V);
 PF_DECL int pf_head_parts(long long N, long long V, int D, int sm_count);
+PF_DECL int pf_head_tile(long long N, long long V, int D, int sm_count);
 PF_DECL int pf_head_fwd(const void* x, const void* w, const void* target, void* xc, void* index, void* stats, void* loss,
                         void* inv, void* scratch, long long N, long long V, int D, int Dp, long long ldx, long long ldw,
                         long long ignore_index, int reduction, int dtype, int* status, int sm_count, void* stream);

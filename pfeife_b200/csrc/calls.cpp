@@ -110,7 +110,7 @@ PyMethodDef methods[] = {
     PF_CALL(pf_groupnorm_fwd), PF_CALL(pf_groupnorm_bwd), PF_CALL(pf_upsample2x),
     PF_CALL(pf_conv_gemm), PF_CALL(pf_conv_wgrad), PF_CALL(pf_conv_pack), PF_CALL(pf_conv_unpack),
     PF_CALL(pf_gated_mlp_scratch), PF_CALL(pf_gated_mlp_fwd), PF_CALL(pf_gated_mlp_bwd), PF_CALL(pf_head_index), PF_CALL(pf_head_scratch),
-    PF_CALL(pf_head_words), PF_CALL(pf_head_parts), PF_CALL(pf_head_fwd), PF_CALL(pf_head_bwd),
+    PF_CALL(pf_head_words), PF_CALL(pf_head_parts), PF_CALL(pf_head_tile), PF_CALL(pf_head_fwd), PF_CALL(pf_head_bwd),
     PF_CALL(pf_scaled_embed_fwd), PF_CALL(pf_scaled_embed_scratch), PF_CALL(pf_scaled_embed_bwd),
     {nullptr, nullptr, 0, nullptr}};
 

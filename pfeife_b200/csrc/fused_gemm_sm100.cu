@@ -834,7 +834,7 @@ PartPlan plan_parts(long long M, long long N, long long K, int sm_count, bool jo
     const long long bt = pair ? 2 * FG_BM : FG_BM, slots = pair ? sm_count / 2 : sm_count;
     const long long rows = (M + bt - 1) / bt, tiles = rows * ((N + bt - 1) / bt);
     const double each = pair ? 0.37 : 0.25, fed = (double)(bt * FG_BK * 2) / rows * slots / 5.5e6;
-    for (int p = 1; p <= 16 && (p == 1 || kb >= 8ll * p) && p * M * N <= (64ll << 20); ++p) {
+    for (int p = 1; p <= 16 && (p == 1 || (kb >= 8ll * p && p * M * N <= (64ll << 20))); ++p) {
       const long long items = tiles * p, full = items / slots, rest = items % slots;
       const double blocks = (double)((kb + p - 1) / p) + 1.5;
       double t = full * blocks * (each > fed ? each : fed);

@@ -386,13 +386,20 @@ PF_API int pf_head_words(long long N, long long V) {
   return (int)(((V + pieces - 1) / pieces + 255) / 256 * 256);
 }
 
+static PartPlan head_plan(long long N, long long V, int D, int sm_count) {
+  const long long words = pf_head_words(N, V);
+  return N > 0 ? plan_parts(N, (D + 7) / 8 * 8, words < V ? words : V, sm_count > 0 ? sm_count : 148, true) : PartPlan();
+}
+
 // Parts in which the reduction of dx over the words of a piece is split if all rows count, where they leave SMs idle.  In
 // the memory of these go more parts of fewer rows.
 PF_API int pf_head_parts(long long N, long long V, int D, int sm_count) {
-  if (!head_sizes_ok(N, V, D)) return -3;
-  if (sm_count <= 0) sm_count = 148;
-  const long long words = pf_head_words(N, V);
-  return N > 0 ? plan_parts(N, (D + 7) / 8 * 8, words < V ? words : V, sm_count, true).parts : 1;
+  return head_sizes_ok(N, V, D) ? head_plan(N, V, D, sm_count).parts : -3;
+}
+
+// Rows of the tiles of that product: 256 of a pair of CTAs, or 128
+PF_API int pf_head_tile(long long N, long long V, int D, int sm_count) {
+  return !head_sizes_ok(N, V, D) ? -3 : head_plan(N, V, D, sm_count).pair ? 256 : 128;
 }
 
 // x [N, D] (rows ldx apart), w [V, Dp] (Dp: D up to a multiple of 8, filled with zeros; rows ldw apart), target [N].
@@ -455,7 +462,6 @@ PF_API int pf_head_fwd(const void* x, const void* w, const void* target, void* x
   if (n_parts <= FOLD_FEW_PARTS && N >= (long long)sm_count * FOLD_MOST_ROWS / 4)
     return fold(head_fold_kernel<FOLD_MOST_ROWS>, FOLD_MOST_ROWS);
   return fold(head_fold_kernel<FOLD_ROWS>, FOLD_ROWS);
-  return 0;
 }
 
 // dloss: one value, or with by_row the rows' dloss[n * dloss_step]; inv as the forward left it.
@@ -474,8 +480,8 @@ PF_API int pf_head_bwd(const void* dloss, const void* inv, const void* xc, const
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const long long Mp = padded_rows(N);
   const HeadIndex ix = head_index(static_cast<int*>(index), N);
-  const int words = pf_head_words(N, V), parts = pf_head_parts(N, V, D, sm_count);
-  const int tile = N > 0 ? plan_parts(N, Dp, words < V ? words : V, sm_count, true).pair : 0;
+  const PartPlan plan = head_plan(N, V, D, sm_count);
+  const int words = pf_head_words(N, V), parts = plan.parts, tile = plan.pair;
   const float unit = dtype == PF_F16 ? 32768.f : 1.f;
   const float* scale = static_cast<const float*>(dloss);
   const float* scale2 = static_cast<const float*>(inv);

@@ -997,3 +997,35 @@ def test_products_take_the_sms_that_a_call_is_given(monkeypatch, tmp_path):
     assert grids[16][0] == 16 and grids[24][0] == 24 and grids[148][0] > 100 and grids[132][0] > 100, grids
     for y, z in out[1:]:
         assert torch.equal(z, out[0][1]) and float((y - out[0][0]).float().norm()) <= 2.0 ** -8 * float(y.float().norm())
+
+
+@pytest.mark.parametrize("N,D,V,rows", [(128, 4096, 300, 128), (2048, 4096, 32000, 256), (9000, 8192, 32000, 256),
+                                        (16384, 4096, 32000, 256), (16385, 4096, 32000, 256), (32768, 4096, 32000, 256),
+                                        (1 << 18, 8192, 128011, 256)], ids=str)
+def test_tiles_of_many_rows(calls, N, D, V, rows):
+    """Tiles of pairs however many outputs there are; what bounds memory are the parts, and there only their number."""
+    parts = calls.pf_head_parts(N, V, D, 148)
+    assert calls.pf_head_tile(N, V, D, 148) == rows and (parts == 1 or parts * N * D <= 2 ** 26)
+    assert calls.pf_head_tile(-1, V, D, 148) == calls.pf_head_tile(N, 0, D, 148) == -3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,D,V", [(17000, 4096, 300), (33000, 2056, 4500)])
+def test_more_outputs_than_parts_may_have(N, D, V):
+    """Gradients of so many rows that they come in one part, in one piece of the vocabulary and in two."""
+    x = normal(N, D, device="cuda", dtype=torch.bfloat16, seed=1).requires_grad_()
+    w = normal(V, D, device="cuda", dtype=torch.bfloat16, seed=2, std=2.0 * D ** -0.5).requires_grad_()
+    target = torch.randint(0, V, (N,), generator=gen(3)).cuda()
+    target[::9] = -100
+    g = torch.tensor(2.0 ** 10, device="cuda")
+    loss = ops.linear_cross_entropy(x, w, target)
+    dx, dw = torch.autograd.grad(loss, [x, w], g)
+    assert not dx[::9].any()
+    rows = torch.cat([torch.arange(0, 300), torch.arange(N - 300, N)]).cuda()      # each row's own, the mean over all
+    n = int((target >= 0).sum())
+    want = head64(x[rows], w, target[rows], g / n, "sum", U[torch.bfloat16], 2.0 ** 100)
+    within(dx[rows], *want[1])
+    part = ops.linear_cross_entropy(x.detach()[:N // 2].requires_grad_(), w, target[:N // 2], reduction="sum")
+    rest = ops.linear_cross_entropy(x.detach()[N // 2:].requires_grad_(), w, target[N // 2:], reduction="sum")
+    total = sum(torch.autograd.grad(s, w)[0].double() for s in (part, rest)) * (2.0 ** 10 / n)
+    assert float((dw.double() - total).norm()) <= 4 * 2.0 ** -8 * float(total.norm())
