@@ -1547,12 +1547,15 @@ _autograd(head_loss_fwd, 1, _head_loss_backward, setup=_head_loss_setup)
 
 def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int = -100,
                          reduction: str = "mean") -> Tensor:
-    """``cross_entropy(linear(x, weight), target)`` of x [..., D], weight [V, D] and target [...], without the logits:
-    neither they nor their gradient are ever whole in memory, and no more than x's rows and two numbers of each are kept
-    for the backward.  Logits are fp32 sums that are not rounded.  Rows whose target is ``ignore_index`` or outside
-    the vocabulary do not count: they are not read, cost no products, have a loss of 0 and a gradient of zeros,
-    whatever x holds there.  ``reduction``: mean over the rows that count (0 if there are none), sum, or none
-    (fp32 [...])."""
+    """``cross_entropy(linear(x, weight), target)`` of x [..., D], weight [V, D] and target [...], without keeping logits:
+    what is kept for the backward are the rows that count and two numbers of each.  In 16 bits on CUDA no logits reach
+    memory.  The forward has 8 bytes of scratch for each row and 64 words; the backward has the gradient of the logits in
+    16 bits, of a piece of the vocabulary at a time: 2^27 values (all of it, where there are no more) or 4096 words of every
+    row, whichever is more, and x's gradient in 32 bits.  In the other types PyTorch's products have all logits in memory
+    while a direction runs.  The products are four for the three of separate operators: where the logits fit, those are
+    faster.  Logits are fp32 sums that are not rounded.  Rows whose target is ``ignore_index`` or outside the vocabulary do
+    not count: they are not read, cost no products, have a loss of 0 and a gradient of zeros, whatever x holds there.
+    ``reduction``: mean over the rows that count (0 if there are none), sum, or none (fp32 [...])."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
     loss = _native_layer("linear_cross_entropy", x, weight, target, ignore_index, _REDUCTIONS[reduction])

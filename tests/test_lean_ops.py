@@ -1029,3 +1029,74 @@ def test_more_outputs_than_parts_may_have(N, D, V):
     rest = ops.linear_cross_entropy(x.detach()[N // 2:].requires_grad_(), w, target[N // 2:], reduction="sum")
     total = sum(torch.autograd.grad(s, w)[0].double() for s in (part, rest)) * (2.0 ** 10 / n)
     assert float((dw.double() - total).norm()) <= 4 * 2.0 ** -8 * float(total.norm())
+
+
+def _bytes(call, leaves, grad):
+    """Bytes asked for beside what was there before: (kept from forward to backward, the most at one time in the forward, in
+    the backward, those of the gradients)"""
+    of = lambda what: torch.cuda.memory_stats()[f"requested_bytes.all.{what}"]
+    torch.cuda.synchronize()
+    before = of("current")
+    torch.cuda.reset_peak_memory_stats()
+    y = call()
+    kept, top = of("current") - before, of("peak") - before
+    torch.cuda.reset_peak_memory_stats()
+    grads = torch.autograd.grad(y, leaves, grad)
+    return kept, top, of("peak") - before, sum(t.numel() * t.element_size() for t in grads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,D,V,reduction", [(8192, 256, 32000, "mean"), (40000, 64, 32000, "none"), (2048, 512, 4000, "mean")],
+                         ids=str)
+def test_memory_of_a_head(N, D, V, reduction):
+    """Kept: the rows, their index and 8 bytes of each.  Alive beside that: forward 8 bytes of each row and 64 words;
+    backward dz of a piece, of 2^27 values or 4096 words, and the parts of dx in fp32."""
+    x = normal(N, D, device="cuda", dtype=torch.bfloat16, seed=1).requires_grad_()
+    w = normal(V, D, device="cuda", dtype=torch.bfloat16, seed=2, std=0.1).requires_grad_()
+    target = torch.randint(0, V, (N,), generator=gen(3)).cuda()
+    g = torch.ones(N if reduction == "none" else (), device="cuda")
+    call = lambda: ops.linear_cross_entropy(x, w, target, reduction=reduction)
+    torch.autograd.grad(call(), [x, w], g)               # what is made once for the device
+    kept, forward, backward, size = _bytes(call, [x, w], g)
+    rows = (N + 255) // 256 * 256
+    slack = 16 * 1024                                    # words that stand by themselves, KiB rounded up
+    least = rows * D * 2 + rows * 12 + N * 4
+    assert kept <= least + N * 4 + rows * 8 + slack
+    assert forward <= kept + rows * ((V + 63) // 64 * 8 + 4 + 1) + slack
+    piece = max(min(rows * (V + 255), 2 ** 27), rows * 4096)
+    assert backward <= kept + size + piece * 2 + max(rows * D, 2 ** 26) * 4 + rows * 4 + slack
+    if N > 2048:                                         # 2 bytes a logit, and as many for the gradient
+        assert backward < N * V * 2
+
+
+@pytest.mark.gpu
+def test_memory_of_a_gated_block():
+    """Kept: gate and up.  Alive beside them: h in either direction, gate's and up's gradients in the backward, and the
+    parts of products that are split, which the workspace's size says."""
+    M, D, H = 4096, 256, 2048
+    x, w1, w2 = (normal(*s, device="cuda", dtype=torch.bfloat16, seed=1, std=0.1).requires_grad_()
+                 for s in ((M, D), (2 * H, D), (D, H)))
+    call = lambda: ops.gated_mlp(x, w1, None, w2, None)
+    dy = torch.ones(M, D, device="cuda", dtype=torch.bfloat16)
+    torch.autograd.grad(call(), [x, w1, w2], dy)
+    kept, forward, backward, size = _bytes(call, [x, w1, w2], dy)
+    slack = 16 * 1024
+    assert kept <= (M * 2 * H + M * D) * 2 + slack       # with the result
+    parts = _lib.calls().pf_gated_mlp_scratch(M, D, H, D, 0) * 1024
+    assert forward <= kept + M * H * 2 + parts + slack and backward <= kept + size + M * 3 * H * 2 + parts + slack
+    assert parts <= 2 ** 28                              # 2^26 sums
+
+
+@pytest.mark.gpu
+def test_memory_of_embedded_tokens():
+    """Nothing is kept; beside the gradient there are 12 bytes a token, 8 a word and the windows' parts."""
+    N, V, D = 8192, 30000, 512
+    table = torch.zeros(V, D, device="cuda", requires_grad=True)
+    ids = tokens("any", N, V).cuda()
+    call = lambda: ops.scaled_embedding(ids, table, 2.0, out_dtype=torch.bfloat16)
+    dy = torch.ones(N, D, device="cuda", dtype=torch.bfloat16)
+    torch.autograd.grad(call(), table, dy)
+    kept, forward, backward, size = _bytes(call, [table], dy)
+    slack = 16 * 1024
+    assert kept <= N * D * 2 + slack and forward <= kept + slack
+    assert backward <= kept + size + 12 * N + 8 * V + N // 8 * 2 * D * 4 + slack
