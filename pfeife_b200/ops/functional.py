@@ -1695,7 +1695,9 @@ _autograd(scaled_embed_fwd, 1, _scaled_embed_backward, setup=_scaled_embed_setup
 
 def scaled_embedding(ids: Tensor, table: Tensor, scale: float = 1.0, out_dtype: Optional[torch.dtype] = None) -> Tensor:
     """scale * table[ids] for integers ids [...] and a table [V, D], rounded once to ``out_dtype`` (default: as
-    ``embedding``).  Ids outside the table, such as -1 for padding, have zeros and no gradient.  The table's gradient
+    ``embedding``).  A registered table has a 16-bit shadow: its rows are read, in place of the table's, where ``out_dtype``
+    is its type, as by ``embedding``; they are rounded before the scale, too.
+    Ids outside the table, such as -1 for padding, have zeros and no gradient.  The table's gradient
     adds up each row's tokens in their order, in 32 bits, rounded once: the same call gives the same bits, unlike
     ``embedding``'s, whose sums are atomic."""
     if out_dtype is None:
