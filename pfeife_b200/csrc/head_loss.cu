@@ -263,8 +263,8 @@ head_fold_kernel(const RowStat* __restrict__ parts, long long pitch, int n_parts
   }
 }
 
-// Gradients that arrive row by row, of the rows that count: divided by a power of two near their largest, which goes into
-// `scale`, so that 16 bits hold the products.
+// Gradients that arrive row by row, of the rows that count: divided by a power of two near the largest number among
+// them, which goes into `scale`, so that 16 bits hold the products.
 __global__ void __launch_bounds__(1024)
 head_factor_kernel(const float* __restrict__ g, long long step, HeadIndex ix, float* __restrict__ factor,
                    float* __restrict__ scale) {
@@ -275,14 +275,14 @@ head_factor_kernel(const float* __restrict__ g, long long step, HeadIndex ix, fl
   for (int i = threadIdx.x; i < count; i += 1024) {
     const float v = g[ix.list[i] * step];
     factor[i] = v;
-    top = fmaxf(top, fabsf(v));
+    if (fabsf(v) < INFINITY) top = fmaxf(top, fabsf(v));
   }
   top = warp_max(top);
   if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
   __syncthreads();
   top = warp_max(tops[threadIdx.x & 31]);
   int e = 0;
-  if (top > 0.f && top < INFINITY) {
+  if (top > 0.f) {
     frexpf(top, &e);
     e = max(-120, min(120, e));
   }

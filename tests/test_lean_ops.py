@@ -1100,3 +1100,20 @@ def test_memory_of_embedded_tokens():
     slack = 16 * 1024
     assert kept <= N * D * 2 + slack and forward <= kept + slack
     assert backward <= kept + size + 12 * N + 8 * V + N // 8 * 2 * D * 4 + slack
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan], ids=str)
+def test_a_gradient_that_is_no_number_stays_with_its_row(bad, device):
+    """Rows' gradients are divided by a power of two near the largest: of those that are numbers."""
+    N, D, V = 40, 16, 50
+    x = normal(N, D, device=device, dtype=torch.float16, seed=1).requires_grad_()
+    w = normal(V, D, device=device, dtype=torch.float16, seed=2, std=0.3)
+    target = torch.randint(0, V, (N,), generator=gen(3)).to(device)
+    g = torch.linspace(500.0, 1000.0, N, device=device)
+    want = head64(x, w, target, g, "none", U[torch.float16], 2.0 ** 13)[1]
+    g[7] = bad
+    (dx,) = torch.autograd.grad(ops.linear_cross_entropy(x, w, target, reduction="none"), x, g)
+    rest = torch.arange(N, device=device) != 7
+    assert not torch.isfinite(dx[7]).any()
+    within(dx[rest], want[0][rest], want[1][rest])
