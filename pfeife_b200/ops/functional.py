@@ -628,7 +628,8 @@ def _act_slope(z: Tensor, act: int) -> Tuple[Tensor, Tensor]:
     if act == ACT_GELU_TANH:
         c = math.sqrt(2 / math.pi)
         t = torch.tanh(c * (z + 0.044715 * z ** 3))
-        return 0.5 * z * (1.0 + t), 0.5 * (1.0 + t) + 0.5 * z * (1.0 - t * t) * c * (1.0 + 3 * 0.044715 * z * z)
+        z2 = (z * z).clamp(max=1e6)      # t is 1 or -1 beyond, where fp32 may not have the square
+        return 0.5 * z * (1.0 + t), 0.5 * (1.0 + t) + 0.5 * z * (1.0 - t * t) * c * (1.0 + 3 * 0.044715 * z2)
     sg = torch.sigmoid(z)
     return z * sg, sg * (1.0 + z * (1.0 - sg))
 

@@ -1117,3 +1117,19 @@ def test_a_gradient_that_is_no_number_stays_with_its_row(bad, device):
     rest = torch.arange(N, device=device) != 7
     assert not torch.isfinite(dx[7]).any()
     within(dx[rest], want[0][rest], want[1][rest])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [8, 9], ids=["whole", "odd"])
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh"])
+def test_gates_whose_square_fp32_does_not_have(kind, D, device):
+    gates = torch.tensor([1e30, -1e30, 2e19, -2e19, 1e13, -1e13, 1e38, -1e38])
+    x = torch.ones(1, D, device=device, dtype=torch.bfloat16)
+    w1 = torch.zeros(16, D, device=device, dtype=torch.bfloat16)
+    w1[:8, 0], w1[8:, 1] = gates.to(w1), 2.0 ** -10
+    w1.requires_grad_()
+    y = ops.gated_mlp(x, w1, None, torch.eye(8, device=device, dtype=torch.bfloat16), None, kind)
+    gate = w1.detach()[:8, 0]
+    assert torch.equal(y.detach()[0], gate.clamp(min=0) * 2.0 ** -10)
+    (dw1,) = torch.autograd.grad(y, w1, torch.ones_like(y))
+    assert torch.equal(dw1[:8, 0], (gate > 0).to(gate) * 2.0 ** -10) and torch.equal(dw1[8:, 1], gate.clamp(min=0))
