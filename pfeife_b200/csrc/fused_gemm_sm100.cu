@@ -6,8 +6,8 @@
 // under the next tile's products.  Tiles are 256 x 256 of a CTA pair (cta_group::2) or 128 x 128 of one CTA.
 //
 // In short runs on a B200, rows x columns x reduction, bf16:
-//   GLU_FWD     2048 x (2 x 11008) x 4096   245 us  1.51 PFLOP/s    16384 x (2 x 2560) x 640   90 us  1.19 PFLOP/s
-//   GLU_BWD     2048 x 11008 x 4096         150 us  1.23            16384 x 2560 x 640        110 us  0.49
+//   GLU_FWD     2048 x (2 x 11008) x 4096   254 us  1.45 PFLOP/s    16384 x (2 x 2560) x 640   94 us  1.14 PFLOP/s
+//   GLU_BWD     2048 x 11008 x 4096         154 us  1.20            16384 x 2560 x 640        117 us  0.46
 //   HEAD_STATS  2048 x 32000 x 4096         330 us  1.63            13 x 32000 x 4096          58 us  4.5 TB/s of W
 //   HEAD_DZ     the same                    339 us  1.58                                       48 us  5.5 TB/s
 //   PARTS_N     2048 x 4096 x 32000         370 us  1.45            13 x 4096 x 32000          42 us  6.2 TB/s

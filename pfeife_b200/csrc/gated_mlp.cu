@@ -3,12 +3,14 @@
 //
 // Forward 6 M D H operations in two products (the first with both projections, the activation and their product in its
 // epilogue), backward 12 M D H in five: dh with everything that follows from it in the epilogue, dx and the weights'
-// gradients.  For few rows the weights are what moves, and products have few tiles: one is then split over its reduction
+// gradients.  Gate, up, their gradients and h are operands of 16-bit products, or kept for them, and rounded to that (gate and
+// up within the type's range); activations and their derivatives are of fp32 sums forward, and of what was kept backward.
+// For few rows the weights are what moves, and products have few tiles: one is then split over its reduction
 // into as many parts as keep all SMs reading (plan_parts), and what its epilogue does is done by the kernels here, which
 // add the parts up in their order.
 //
-// On a B200, bf16, forward and backward: 2048 rows of 4096 over 11008 hidden values (1.66 TFLOP) 1.18 ms in a short run,
-// 1.41 PFLOP/s; 16384 of 640 over 2560 with GELU and biases 575 us, 0.84 PFLOP/s, where gate, up, their gradients and h are
+// On a B200, bf16, forward and backward: 2048 rows of 4096 over 11008 hidden values (1.66 TFLOP) 1.17 ms in a short run,
+// 1.42 PFLOP/s; 16384 of 640 over 2560 with GELU and biases 568 us, 0.85 PFLOP/s, where gate, up, their gradients and h are
 // 26 MB a thousand rows; 13 of 4096 over 11008 190 us, of which 124 are what memory takes for the weights twice and their
 // gradients once.
 #include "common.cuh"
