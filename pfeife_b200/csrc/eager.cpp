@@ -182,7 +182,11 @@ constexpr int EPI_OF_ACT[4] = {NONE, GELU, GELU_TANH, SILU};
 // x as rows the TMA can read
 Tensor rows(const Tensor& x) {
   Tensor r = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
-  if (r.stride(1) != 1 || r.stride(0) % 8 || !aligned(r)) r = r.contiguous();
+  if (r.stride(1) != 1 || r.stride(0) % 8 || !aligned(r)) {
+    r = r.contiguous();
+    // which leaves a view that starts off 16 bytes, or one row of a wider matrix, as it was
+    if (!aligned(r) || r.stride(0) != r.size(1)) r = r.clone(at::MemoryFormat::Contiguous);
+  }
   return r;
 }
 bool readable(const Tensor& m) {

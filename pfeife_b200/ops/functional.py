@@ -215,6 +215,9 @@ def _rows(x: Tensor) -> Tensor:
     x2 = x.reshape(-1, x.shape[-1])
     if x2.stride(-1) != 1 or (x2.stride(0) * x2.element_size()) % 16 or x2.data_ptr() % 16:
         x2 = x2.contiguous()
+        # which leaves a view that starts off 16 bytes, or one row of a wider matrix, as it was
+        if x2.data_ptr() % 16 or x2.stride(0) != x2.shape[1]:
+            x2 = x2.clone(memory_format=torch.contiguous_format)
     return x2
 
 

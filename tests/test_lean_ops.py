@@ -1133,3 +1133,29 @@ def test_gates_whose_square_fp32_does_not_have(kind, D, device):
     assert torch.equal(y.detach()[0], gate.clamp(min=0) * 2.0 ** -10)
     (dw1,) = torch.autograd.grad(y, w1, torch.ones_like(y))
     assert torch.equal(dw1[:8, 0], (gate > 0).to(gate) * 2.0 ** -10) and torch.equal(dw1[8:, 1], gate.clamp(min=0))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("through", ["C++", "Python"])
+@pytest.mark.parametrize("M", [1, 3])
+def test_rows_that_start_anywhere(M, through, device, monkeypatch):
+    """Rows, residual and gradient of a block and rows of a head that are contiguous but off their vectors, or one row of a
+    matrix whose rows are."""
+    if through == "Python":
+        monkeypatch.setattr(_lib, "_eager", None)
+        monkeypatch.setattr(_lib, "eager", lambda: None)
+    new = lambda *s, seed: normal(*s, device=device, dtype=torch.bfloat16, seed=seed, std=0.5)
+    w1, w2, w3 = new(48, 16, seed=1), new(32, 24, seed=2), new(20, 16, seed=3)
+    places = [lambda t: t,
+              lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape),
+              lambda t: torch.cat([t.new_zeros(M, 3), t], 1)[:, 3:]]
+    x, res, dy, target = new(M, 16, seed=4), new(M, 32, seed=5), new(M, 32, seed=6), torch.arange(M, device=device)
+    want = None
+    for place in places:
+        a, r = (place(t).detach().requires_grad_() for t in (x, res))
+        y = ops.gated_mlp(a, w1, None, w2, None, "silu", r)
+        got = [y.detach(), *torch.autograd.grad(y, [a, r], place(dy))]
+        loss = ops.linear_cross_entropy(a, w3, target)
+        got += [loss.detach(), *torch.autograd.grad(loss, a)]
+        want = want or got
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
