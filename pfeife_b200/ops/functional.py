@@ -717,8 +717,13 @@ def _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_d
     native = dy.is_cuda and cd in (torch.float16, torch.bfloat16)
     if _glu_native(dy, cd, w1, w2):
         return _gated_mlp_native_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1, b2)
-    dh = linear_bwd.plain(dy, gu[..., :H], w2, empty, ACT_NONE, True, False, False)[0] if native else dy @ w2.to(cd)
-    gate, up, dh = _wide(gu[..., :H]), _wide(gu[..., H:]), _wide(dh)
+    if native:                           # fp32 sums, as the kernels' epilogue has them; zeros fill rows and columns up
+        N, w = w2.shape[0], _weight_as(w2, cd)
+        w = _aligned(F.pad(w, (0, -H % 8, 0, -N % 8)) if H % 8 or N % 8 else w)
+        dh = kx.gemm(_rows(_pad_k(_rows(dy))), w, b_mn=True, out_dtype=torch.float32)[:, :H].view(gu.shape[:-1] + (H,))
+    else:
+        dh = _wide(dy) @ _wide(w2.to(cd))
+    gate, up = _wide(gu[..., :H]), _wide(gu[..., H:])
     a, slope = _act_slope(gate, act)
     dgu, h = torch.cat([dh * up * slope, dh * a], -1).to(cd), (a * up).to(cd)
     if native:

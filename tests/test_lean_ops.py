@@ -1159,3 +1159,29 @@ def test_rows_that_start_anywhere(M, through, device, monkeypatch):
         got += [loss.detach(), *torch.autograd.grad(loss, a)]
         want = want or got
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("M,K,H,N", [(2, 65, 109, 430), (1413, 4, 4, 35), (70, 24, 27, 16), (9, 5, 16, 13), (40, 12, 33, 2050)],
+                         ids=str)
+def test_gradients_of_odd_widths(M, K, H, N, device):
+    """The gradient of h is not rounded on its way to gate's and up's, whatever the widths."""
+    new = lambda *s, seed, std=1.0: normal(*s, device=device, dtype=torch.bfloat16, seed=seed, std=std).requires_grad_()
+    x, w1, w2 = new(M, K, seed=1), new(2 * H, K, seed=2, std=1.5 * K ** -0.5), new(N, H, seed=3, std=H ** -0.5)
+    dy = new(M, N, seed=4).detach()
+    u = U[torch.bfloat16]
+    want = mlp64(x, w1, None, w2, None, None, dy, "silu", u)
+    y = ops.gated_mlp(x, w1, None, w2, None)
+    for got, w in zip(torch.autograd.grad(y, [x, w1, w2], dy), want[1:]):
+        within(got, *w)
+    # of one row that has one value, 1: gate and up are columns of w1, exactly, and gradients of biases those of gate and up
+    one = torch.zeros(1, K, device=device, dtype=torch.bfloat16)
+    one[0, K // 2] = 1.0
+    b1 = torch.zeros(2 * H, device=device, dtype=torch.bfloat16, requires_grad=True)
+    (db,) = torch.autograd.grad(ops.gated_mlp(one, w1, b1, w2, None), b1, dy[:1])
+    dh, dhm = ((f(dy[:1].double()) @ f(w2.detach().double()))[0] for f in (lambda t: t, torch.abs))
+    gate, up = w1.detach()[:, K // 2].double().view(2, H)
+    a, slope = act64(gate, "silu")
+    edh = sums(N) * dhm
+    within(db, torch.cat([dh * up * slope, dh * a]), torch.cat([
+        up.abs() * (edh * 1.2 + dh.abs() * 1e-6 * (1 + gate.abs())), edh * a.abs() + dh.abs() * 1e-6 * (1 + gate.abs())]))
