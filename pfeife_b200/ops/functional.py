@@ -221,6 +221,12 @@ def _rows(x: Tensor) -> Tensor:
     return x2
 
 
+def _aligned(w: Tensor) -> Tensor:
+    """`w` with rows on 16 bytes, as the products read them"""
+    return w if w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.data_ptr() % 16 == 0 else \
+        w.clone(memory_format=torch.contiguous_format)
+
+
 # --------------------------------------------------------------------------- calling the ops
 # A call through the dispatcher costs some 40 us of host time per op and direction (schema
 # checks, several Python kernels), more than most of the launches it makes.  Graph capture needs it;
@@ -389,6 +395,7 @@ def linear_fwd(x: Tensor, w: Tensor, bias: Optional[Tensor], residual: Optional[
         w2 = slot.lp if fused_gather else _weight_as(w, cd)
         if x2.shape[1] % 8:
             x2, w2 = _pad_k(x2), _pad_k(w2)
+        w2 = _aligned(w2)
         r2 = None
         if residual is not None:
             r2 = _rows(residual if residual.dtype == cd else kx.cast(residual, cd))
@@ -440,9 +447,9 @@ def linear_bwd(dy: Tensor, x: Tensor, w: Tensor, aux: Tensor, act: int, need_dx:
         if need_dx:
             w2 = _weight_as(w, cd)
             if N % 8 == 0 and K % 8 == 0:
-                dx = kx.gemm(dy2, w2, b_mn=True).view(x.shape[:-1] + (K,))
+                dx = kx.gemm(dy2, _aligned(w2), b_mn=True).view(x.shape[:-1] + (K,))
             elif N % 8 == 0:
-                dx = kx.gemm(dy2, _pad_k(w2), b_mn=True)[:, :K].reshape(x.shape[:-1] + (K,))
+                dx = kx.gemm(dy2, _aligned(_pad_k(w2)), b_mn=True)[:, :K].reshape(x.shape[:-1] + (K,))
             else:
                 dx = (dy2 @ w2).view(x.shape[:-1] + (K,))
         if need_dw:
@@ -641,12 +648,6 @@ def _glu_native(x: Tensor, cd: torch.dtype, w1: Tensor, w2: Tensor) -> bool:
     """The kernels that have the activation in the products' epilogue: whole vectors of every width."""
     return x.is_cuda and cd in (torch.float16, torch.bfloat16) and w1.shape[1] % 8 == 0 and w2.shape[0] % 8 == 0 \
         and w2.shape[1] % 8 == 0
-
-
-def _aligned(w: Tensor) -> Tensor:
-    """`w` with rows on 16 bytes, as the products read them"""
-    return w if w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.data_ptr() % 16 == 0 else \
-        w.clone(memory_format=torch.contiguous_format)
 
 
 @_custom_op("pfeife::gated_mlp_fwd")

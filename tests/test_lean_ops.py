@@ -1185,3 +1185,25 @@ def test_gradients_of_odd_widths(M, K, H, N, device):
     edh = sums(N) * dhm
     within(db, torch.cat([dh * up * slope, dh * a]), torch.cat([
         up.abs() * (edh * 1.2 + dh.abs() * 1e-6 * (1 + gate.abs())), edh * a.abs() + dh.abs() * 1e-6 * (1 + gate.abs())]))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("K,H,N", [(16, 24, 32), (88, 33, 896), (13, 16, 24), (24, 9, 5)], ids=str)
+def test_weights_that_lie_anywhere(K, H, N, device):
+    """Transposed ones, every other row of a matrix, and ones that start off 16 bytes, in blocks and in linear layers."""
+    new = lambda *s, seed: normal(*s, device=device, dtype=torch.bfloat16, seed=seed, std=0.2)
+    x, w1, w2, dy = new(5, K, seed=1), new(2 * H, K, seed=2), new(N, H, seed=3), new(5, N, seed=4)
+    x.requires_grad_()
+    places = [lambda t: t, lambda t: t.t().contiguous().t(),
+              lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape),
+              lambda t: torch.stack([t, t], 1).view(-1, t.shape[1])[::2],
+              lambda t: torch.cat([t, t], 1)[:, :t.shape[1]]]
+    want = None
+    for place in places:
+        a, b = (place(t).detach().requires_grad_() for t in (w1, w2))
+        y = ops.gated_mlp(x, a, None, b, None)
+        z = ops.linear(x, a, activation="gelu")
+        got = [y.detach(), z.detach(), *torch.autograd.grad(y, [x, a, b], dy),
+               *torch.autograd.grad(z, [x, a], torch.ones_like(z))]
+        want = want or got
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
