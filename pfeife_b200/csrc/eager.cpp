@@ -182,11 +182,7 @@ constexpr int EPI_OF_ACT[4] = {NONE, GELU, GELU_TANH, SILU};
 // x as rows the TMA can read
 Tensor rows(const Tensor& x) {
   Tensor r = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
-  if (r.stride(1) != 1 || r.stride(0) % 8 || !aligned(r)) {
-    r = r.contiguous();
-    // which leaves a view that starts off 16 bytes, or one row of a wider matrix, as it was
-    if (!aligned(r) || r.stride(0) != r.size(1)) r = r.clone(at::MemoryFormat::Contiguous);
-  }
+  if (r.stride(1) != 1 || r.stride(0) % 8 || !aligned(r)) r = r.contiguous();
   return r;
 }
 bool readable(const Tensor& m) {
@@ -1166,10 +1162,15 @@ Tensor gated_workspace(const GatedSizes& g, const Env& e, const Tensor& like, in
   kib = pf_gated_mlp_scratch(g.M, g.D, g.H, g.N, e.sms);
   return kib ? floats(kib * 256ll, like) : Tensor();
 }
+// contiguous() leaves one row of a wider matrix and values that start anywhere as they are
+Tensor whole_rows(const Tensor& x) {
+  const Tensor r = rows(x);
+  return readable(r) ? r : r.clone(at::MemoryFormat::Contiguous);
+}
 std::pair<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& w1, const Tensor& b1, const Tensor& w2,
                                         const Tensor& b2, const Tensor& res, int act, bool keep) {
   const Env e(x);
-  const Tensor x2 = rows(x), r2 = res.defined() ? rows(res) : Tensor();
+  const Tensor x2 = whole_rows(x), r2 = res.defined() ? whole_rows(res) : Tensor();
   const GatedSizes g(x2, w2);
   const Tensor h = empty({g.M, g.H}, x), gu = keep ? empty({g.M, 2 * g.H}, x) : Tensor(), y = empty({g.M, g.N}, x);
   int kib;
@@ -1221,7 +1222,7 @@ struct DirectGatedMlp : torch::autograd::Function<DirectGatedMlp> {
                (!b1.defined() || number(b1)) && (!b2.defined() || number(b2))) {
       below([&] {
         const Env e(dy);
-        const Tensor x2 = rows(x), dy2 = rows(dy);
+        const Tensor x2 = whole_rows(x), dy2 = whole_rows(dy);
         Tensor kept = gu.contiguous();
         if (!aligned(kept)) kept = kept.clone();
         const GatedSizes g(x2, w2);

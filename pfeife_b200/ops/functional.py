@@ -215,16 +215,7 @@ def _rows(x: Tensor) -> Tensor:
     x2 = x.reshape(-1, x.shape[-1])
     if x2.stride(-1) != 1 or (x2.stride(0) * x2.element_size()) % 16 or x2.data_ptr() % 16:
         x2 = x2.contiguous()
-        # which leaves a view that starts off 16 bytes, or one row of a wider matrix, as it was
-        if x2.data_ptr() % 16 or x2.stride(0) != x2.shape[1]:
-            x2 = x2.clone(memory_format=torch.contiguous_format)
     return x2
-
-
-def _aligned(w: Tensor) -> Tensor:
-    """`w` with rows on 16 bytes, as the products read them"""
-    return w if w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.data_ptr() % 16 == 0 else \
-        w.clone(memory_format=torch.contiguous_format)
 
 
 # --------------------------------------------------------------------------- calling the ops
@@ -395,7 +386,6 @@ def linear_fwd(x: Tensor, w: Tensor, bias: Optional[Tensor], residual: Optional[
         w2 = slot.lp if fused_gather else _weight_as(w, cd)
         if x2.shape[1] % 8:
             x2, w2 = _pad_k(x2), _pad_k(w2)
-        w2 = _aligned(w2)
         r2 = None
         if residual is not None:
             r2 = _rows(residual if residual.dtype == cd else kx.cast(residual, cd))
@@ -447,9 +437,9 @@ def linear_bwd(dy: Tensor, x: Tensor, w: Tensor, aux: Tensor, act: int, need_dx:
         if need_dx:
             w2 = _weight_as(w, cd)
             if N % 8 == 0 and K % 8 == 0:
-                dx = kx.gemm(dy2, _aligned(w2), b_mn=True).view(x.shape[:-1] + (K,))
+                dx = kx.gemm(dy2, w2, b_mn=True).view(x.shape[:-1] + (K,))
             elif N % 8 == 0:
-                dx = kx.gemm(dy2, _aligned(_pad_k(w2)), b_mn=True)[:, :K].reshape(x.shape[:-1] + (K,))
+                dx = kx.gemm(dy2, _pad_k(w2), b_mn=True)[:, :K].reshape(x.shape[:-1] + (K,))
             else:
                 dx = (dy2 @ w2).view(x.shape[:-1] + (K,))
         if need_dw:
@@ -650,6 +640,19 @@ def _glu_native(x: Tensor, cd: torch.dtype, w1: Tensor, w2: Tensor) -> bool:
         and w2.shape[1] % 8 == 0
 
 
+def _aligned(w: Tensor) -> Tensor:
+    """`w` with rows on 16 bytes, as the products read them"""
+    return w if w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.data_ptr() % 16 == 0 else \
+        w.clone(memory_format=torch.contiguous_format)
+
+
+def _whole_rows(x: Tensor) -> Tensor:
+    """``_rows`` that lie on 16 bytes whatever x is a view of, if they are of whole vectors (others are filled up or take
+    other ways): contiguous() leaves one row of a wider matrix and values that start anywhere as they are"""
+    x2 = _rows(x)
+    return x2 if x2.shape[1] % 8 else _aligned(x2)
+
+
 @_custom_op("pfeife::gated_mlp_fwd")
 def gated_mlp_fwd(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: Optional[Tensor],
                   residual: Optional[Tensor], act: int, keep: bool) -> Tuple[Tensor, Tensor]:
@@ -657,12 +660,14 @@ def gated_mlp_fwd(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: O
     cd = compute_dtype(x)
     shape, H = x.shape[:-1], w2.shape[1]
     if _glu_native(x, cd, w1, w2):
-        cast = lambda t: _rows(t if t.dtype == cd else kx.cast(t, cd))
+        cast = lambda t: _whole_rows(t if t.dtype == cd else kx.cast(t, cd))
         y, gu = kx.gated_mlp_fwd(cast(x), _aligned(_weight_as(w1, cd)), b1, _aligned(_weight_as(w2, cd)), b2,
                                  None if residual is None else cast(residual), act, keep)
         return y.view(shape + (w2.shape[0],)), (gu.view(shape + (2 * H,)) if keep else x.new_empty(0))
     if x.is_cuda and cd in (torch.float16, torch.bfloat16):      # odd widths, product by product
-        x2, w = _rows(x if x.dtype == cd else kx.cast(x, cd)), _weight_as(w1, cd)
+        x2, w = _whole_rows(x if x.dtype == cd else kx.cast(x, cd)), _weight_as(w1, cd)
+        if residual is not None and residual.dtype == cd:
+            residual = _whole_rows(residual).view(residual.shape)
         wide = kx.gemm(_aligned(_pad_k(x2)), _aligned(_pad_k(w)), out_dtype=torch.float32, bias=b1).view(
             shape + (2 * H,))
     else:
@@ -721,6 +726,7 @@ def _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_d
     if native:                           # fp32 sums, as the kernels' epilogue has them; zeros fill rows and columns up
         N, w = w2.shape[0], _weight_as(w2, cd)
         w = _aligned(F.pad(w, (0, -H % 8, 0, -N % 8)) if H % 8 or N % 8 else w)
+        dy = _whole_rows(dy).view(dy.shape)
         dh = kx.gemm(_rows(_pad_k(_rows(dy))), w, b_mn=True, out_dtype=torch.float32)[:, :H].view(gu.shape[:-1] + (H,))
     else:
         dh = _wide(dy) @ _wide(w2.to(cd))
@@ -729,6 +735,10 @@ def _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_d
     dgu, h = torch.cat([dh * up * slope, dh * a], -1).to(cd), (a * up).to(cd)
     if native:
         _, dw2, db2 = linear_bwd.plain(dy, h, w2, empty, ACT_NONE, False, need_dw2, need_db2, b2)
+        if x.dtype == cd:
+            x = _whole_rows(x).view(x.shape)
+        if w1.dtype == cd and w1.shape[1] % 8 == 0:
+            w1 = _aligned(w1)            # itself, where it is registered
         dx, dw1, db1 = linear_bwd.plain(dgu, x, w1, empty, ACT_NONE, need_dx, need_dw1, need_db1, b1)
         return dx, dw1, db1, dw2, db2
     K, N = w1.shape[1], w2.shape[0]
@@ -742,7 +752,7 @@ def _gated_mlp_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_d
 def _gated_mlp_native_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1, need_dw2, need_db2, b1, b2):
     """``gated_mlp_bwd`` by its kernels"""
     cd, dev = dy.dtype, dy.device
-    x2 = _rows(x if x.dtype == cd else kx.cast(x, cd))
+    x2 = _whole_rows(x if x.dtype == cd else kx.cast(x, cd))
     out, buckets, late = {}, [], []
     if need_dx:
         out["dx"] = torch.empty(x2.shape, dtype=cd, device=dev)
@@ -767,7 +777,7 @@ def _gated_mlp_native_grads(dy, x, w1, w2, gu, act, need_dx, need_dw1, need_db1,
             else:
                 dtype = b.dtype if b is not None and b.dtype in (torch.float16, torch.bfloat16) else torch.float32
                 out[name] = torch.empty(n, dtype=dtype, device=dev)
-    kx.gated_mlp_bwd(_rows(dy), x2, _aligned(_weight_as(w1, cd)), _aligned(_weight_as(w2, cd)), _rows(gu), act,
+    kx.gated_mlp_bwd(_whole_rows(dy), x2, _aligned(_weight_as(w1, cd)), _aligned(_weight_as(w2, cd)), _rows(gu), act,
                      add=tuple(buckets), **out)
     for name, bucket in late:
         bucket.add_(out[name])

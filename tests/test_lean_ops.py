@@ -1137,15 +1137,15 @@ def test_gates_whose_square_fp32_does_not_have(kind, D, device):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("through", ["C++", "Python"])
-@pytest.mark.parametrize("M", [1, 3])
-def test_rows_that_start_anywhere(M, through, device, monkeypatch):
+@pytest.mark.parametrize("M,H", [(1, 24), (3, 24), (1, 11), (3, 20)])
+def test_rows_that_start_anywhere(M, H, through, device, monkeypatch):
     """Rows, residual and gradient of a block and rows of a head that are contiguous but off their vectors, or one row of a
     matrix whose rows are."""
     if through == "Python":
         monkeypatch.setattr(_lib, "_eager", None)
         monkeypatch.setattr(_lib, "eager", lambda: None)
     new = lambda *s, seed: normal(*s, device=device, dtype=torch.bfloat16, seed=seed, std=0.5)
-    w1, w2, w3 = new(48, 16, seed=1), new(32, 24, seed=2), new(20, 16, seed=3)
+    w1, w2, w3 = new(2 * H, 16, seed=1), new(32, H, seed=2), new(20, 16, seed=3)
     places = [lambda t: t,
               lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape),
               lambda t: torch.cat([t.new_zeros(M, 3), t], 1)[:, 3:]]
@@ -1190,7 +1190,7 @@ def test_gradients_of_odd_widths(M, K, H, N, device):
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("K,H,N", [(16, 24, 32), (88, 33, 896), (13, 16, 24), (24, 9, 5)], ids=str)
 def test_weights_that_lie_anywhere(K, H, N, device):
-    """Transposed ones, every other row of a matrix, and ones that start off 16 bytes, in blocks and in linear layers."""
+    """Transposed ones, every other row of a matrix, and ones that start off 16 bytes."""
     new = lambda *s, seed: normal(*s, device=device, dtype=torch.bfloat16, seed=seed, std=0.2)
     x, w1, w2, dy = new(5, K, seed=1), new(2 * H, K, seed=2), new(N, H, seed=3), new(5, N, seed=4)
     x.requires_grad_()
@@ -1202,8 +1202,6 @@ def test_weights_that_lie_anywhere(K, H, N, device):
     for place in places:
         a, b = (place(t).detach().requires_grad_() for t in (w1, w2))
         y = ops.gated_mlp(x, a, None, b, None)
-        z = ops.linear(x, a, activation="gelu")
-        got = [y.detach(), z.detach(), *torch.autograd.grad(y, [x, a, b], dy),
-               *torch.autograd.grad(z, [x, a], torch.ones_like(z))]
+        got = [y.detach(), *torch.autograd.grad(y, [x, a, b], dy)]
         want = want or got
         assert all(torch.equal(p, q) for p, q in zip(got, want))
