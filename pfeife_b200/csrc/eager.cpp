@@ -1148,9 +1148,11 @@ struct DirectConv2d : torch::autograd::Function<DirectConv2d> {
 };
 
 // ------------------------------------------------------------------------------ gated feed-forward block
+// rows that TMA reads and that are apart: tensor maps are not made for a row that stands for several
+bool whole(const Tensor& m) { return readable(m) && m.stride(0) >= m.size(1); }
 // 3 activations of gated_mlp.cu; weights [2H, D] and [N, H] of whole vectors
 bool gated_fits(const Tensor& x, const Tensor& w1, const Tensor& w2) {
-  return layer_fits(x, w1, {}) && w2.scalar_type() == x.scalar_type() && readable(w2) && w1.size(0) == 2 * w2.size(1) &&
+  return layer_fits(x, w1, {}) && w2.scalar_type() == x.scalar_type() && whole(w1) && whole(w2) && w1.size(0) == 2 * w2.size(1) &&
          w2.size(1) > 0 && w2.size(1) % 8 == 0 && w2.size(0) > 0 && w2.size(0) % 8 == 0 && w2.size(0) < (1ll << 31);
 }
 struct GatedSizes {
@@ -1165,7 +1167,7 @@ Tensor gated_workspace(const GatedSizes& g, const Env& e, const Tensor& like, in
 // contiguous() leaves one row of a wider matrix and values that start anywhere as they are
 Tensor whole_rows(const Tensor& x) {
   const Tensor r = rows(x);
-  return readable(r) ? r : r.clone(at::MemoryFormat::Contiguous);
+  return whole(r) ? r : r.clone(at::MemoryFormat::Contiguous);
 }
 std::pair<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& w1, const Tensor& b1, const Tensor& w2,
                                         const Tensor& b2, const Tensor& res, int act, bool keep) {
@@ -1255,7 +1257,7 @@ struct DirectGatedMlp : torch::autograd::Function<DirectGatedMlp> {
 
 // ------------------------------------------------------------------------------ output head with its cross entropy
 bool head_fits(const Tensor& x, const Tensor& w, const Tensor& target) {
-  return x.dim() >= 2 && half(x) && x.numel() > 0 && w.scalar_type() == x.scalar_type() && readable(w) &&
+  return x.dim() >= 2 && half(x) && x.numel() > 0 && w.scalar_type() == x.scalar_type() && whole(w) &&
          w.size(1) == x.size(-1) && w.size(1) % 8 == 0 && w.size(0) > 0 && w.size(0) <= (1ll << 28) &&
          target.scalar_type() == at::kLong && target.sizes() == x.sizes().slice(0, x.dim() - 1) &&
          target.numel() <= (1ll << 28) && w.size(1) <= (1ll << 20);
@@ -1311,7 +1313,7 @@ struct DirectHeadLoss : torch::autograd::Function<DirectHeadLoss> {
     const Tensor g = by_row ? grads[0].reshape({-1}) : grads[0];
     const int64_t D = shape.back(), Mp = padded_rows(N);
     Tensor dx, dw;
-    if (direct(g, w, xc, index, stats, inv) && half(xc) && w.scalar_type() == xc.scalar_type() && readable(w) &&
+    if (direct(g, w, xc, index, stats, inv) && half(xc) && w.scalar_type() == xc.scalar_type() && whole(w) &&
         w.size(1) == D && xc.dim() == 2 && xc.size(0) == Mp && xc.size(1) == D && xc.is_contiguous() && aligned(xc) &&
         packed_floats(stats, 2 * Mp) && packed_floats(inv, 1) && index.scalar_type() == at::kInt &&
         index.is_contiguous() && index.numel() == pf_head_index(N) && g.scalar_type() == at::kFloat &&

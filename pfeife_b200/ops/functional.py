@@ -641,9 +641,9 @@ def _glu_native(x: Tensor, cd: torch.dtype, w1: Tensor, w2: Tensor) -> bool:
 
 
 def _aligned(w: Tensor) -> Tensor:
-    """`w` with rows on 16 bytes, as the products read them"""
-    return w if w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.data_ptr() % 16 == 0 else \
-        w.clone(memory_format=torch.contiguous_format)
+    """`w` with rows on 16 bytes, as the products read them, and apart: tensor maps are not made for a row that stands for
+    several"""
+    return w if kx.whole_rows(w) else w.clone(memory_format=torch.contiguous_format)
 
 
 def _whole_rows(x: Tensor) -> Tensor:

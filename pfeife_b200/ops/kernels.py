@@ -104,6 +104,11 @@ def _vectors(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def whole_rows(t: torch.Tensor) -> bool:
+    """Whether the rows of 16-bit values lie on 16 bytes and apart."""
+    return t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0
+
+
 def _split_workspace(L, M: int, N: int, K: int, accumulate: bool, conv: int, tile_n: int, device
                      ) -> Tuple[Optional[torch.Tensor], int]:
     """(workspace, KiB) in which the parts of a split reduction wait to be added in their order."""
@@ -703,8 +708,7 @@ def _head_weight(w: torch.Tensor) -> torch.Tensor:
     """[V, D] -> rows on 16 bytes, D filled up with zeros to a multiple of 8"""
     if w.shape[1] % 8:
         return torch.nn.functional.pad(w, (0, -w.shape[1] % 8))
-    return w if w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.data_ptr() % 16 == 0 else \
-        w.clone(memory_format=torch.contiguous_format)
+    return w if whole_rows(w) else w.clone(memory_format=torch.contiguous_format)
 
 
 def head_fwd(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, ignore_index: int, reduction: int

@@ -1207,3 +1207,26 @@ def test_weights_that_lie_anywhere(K, H, N, device):
         got = [y.detach(), *torch.autograd.grad(y, [x, a, b], dy)]
         want = want or got
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("through", ["C++", "Python"])
+def test_rows_that_stand_for_several(through, device, monkeypatch):
+    """Operands that are one row, expanded, or rows that overlap: as the rows written out."""
+    if through == "Python":
+        monkeypatch.setattr(_lib, "_eager", None)
+        monkeypatch.setattr(_lib, "eager", lambda: None)
+    new = lambda *s, seed: normal(*s, device=device, dtype=torch.bfloat16, seed=seed, std=0.3)
+    wide = lambda n, d, seed: new(8 * n + d, seed=seed).as_strided((n, d), (8, 1))
+    one = lambda n, d, seed: new(1, d, seed=seed).expand(n, d)
+    target = torch.arange(6, device=device)
+    for make in (wide, one):
+        ops_in = [make(*s, seed=i) for i, s in enumerate(((6, 32), (48, 32), (16, 24), (6, 16), (40, 32)))]
+        got = []
+        for x, w1, w2, res, head in (ops_in, [t.contiguous() for t in ops_in]):
+            x, w1, w2, res, head = (t.detach().requires_grad_() for t in (x, w1, w2, res, head))
+            y = ops.gated_mlp(x, w1, None, w2, None, "silu", res)
+            loss = ops.linear_cross_entropy(x, head, target)
+            got.append([y.detach(), loss.detach(), *torch.autograd.grad(y, [x, w1, w2, res], one(6, 16, 9)),
+                        *torch.autograd.grad(loss, [x, head])])
+        assert all(torch.equal(a, b) for a, b in zip(*got))
